@@ -84,6 +84,13 @@ bool tysor_cuda_buffer_write(void* buffer, const float* data, size_t count);
 /* A view of `count` elements starting at element `offset` of `base`
  * (plan-once arenas).  No reference counterpart. */
 void* tysor_cuda_buffer_view(void* base, size_t offset, size_t count);
+/* A buffer over `count` floats of device memory that the caller owns (another
+ * library's tensor): on the context's device, kept alive by the caller until
+ * the buffer is freed, which leaves the memory as it is.  Dispatches run on
+ * the context's stream: a caller that writes or reads the memory on another
+ * stream orders the two (tysor_cuda_context_stream).  No reference
+ * counterpart. */
+void* tysor_cuda_buffer_wrap(void* context, float* data, size_t count);
 /* Element count of a buffer or view. */
 size_t tysor_cuda_buffer_count(void* buffer);
 
@@ -212,6 +219,87 @@ bool tysor_cuda_dispatch_cross_entropy_labels_backward(void* context, void* logi
 /* Exchange axes a and b of a row-major tensor of rank <= 8. */
 bool tysor_cuda_dispatch_transpose(void* context, void* input, void* out, const int64_t* dims,
                                    int rank, int a, int b);
+
+/* Language-model operators (extensions, no reference counterpart).  Their
+ * gradients are the formulas' own, unlike the reference's shortened rules
+ * for rms_norm and softmax.  No output may overlap an input or another
+ * output; `accumulate` adds into every gradient instead of storing it;
+ * operands marked "may be NULL" may be left out.  `stats` buffers hold pairs
+ * of floats and start on an 8-byte boundary. */
+
+/* Layer normalisation: y = (x - mean) * rstd * gain + bias per row of
+ * `width` values, rstd = 1 / sqrt(variance + eps) (population variance).
+ * gain, bias [width] may be NULL (1 and 0).  stats may be NULL or receives
+ * [rows][2] = (mean, rstd), which the backward reads. */
+bool tysor_cuda_dispatch_layer_norm(void* context, void* input, void* gain, void* bias, void* out,
+                                    void* stats, uint32_t rows, uint32_t width, float eps);
+/* With n = (x - mean) * rstd and g = dy * gain:
+ * dx (+)= rstd * (g - mean(g) - n * mean(g * n)), dgain (+)= sum over rows of
+ * dy * n, dbias (+)= sum over rows of dy.  gain, dgain and dbias may be NULL. */
+bool tysor_cuda_dispatch_layer_norm_backward(void* context, void* input, void* gain, void* stats, void* dy,
+                                             void* dx, void* dgain, void* dbias, uint32_t rows,
+                                             uint32_t width, bool accumulate);
+/* Rotary positions over several axes (time, height, width, ...): x is
+ * [batch][heads][seq_len][2 * half] or, with seq_major,
+ * [batch][seq_len][heads][2 * half], half = the sum of sections[0..axes)
+ * (1 to 8 axes, each of at least one pair).  Pair i (elements i and half + i,
+ * as in rope) turns by positions[b][axis][s] * theta^(-i / half), `axis` the
+ * one whose section holds i; positions is [batch][axes][seq_len].  With equal
+ * positions 0, 1, 2, ... on every axis this is rope.  Angles are formed in
+ * 64 bits. */
+bool tysor_cuda_dispatch_rope_axes(void* context, void* input, void* positions, void* out, uint32_t batch,
+                                   uint32_t heads, uint32_t seq_len, const int64_t* sections, int axes,
+                                   double theta, bool seq_major);
+/* dx (+)= grad turned back. */
+bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* positions, void* dx,
+                                            uint32_t batch, uint32_t heads, uint32_t seq_len,
+                                            const int64_t* sections, int axes, double theta, bool seq_major,
+                                            bool accumulate);
+/* Causal attention over a sliding window, the first `sinks` keys staying
+ * visible.  Query row r of sequence b stands at p = starts[b] + r; with
+ * n = lengths[b] it sees key j if 0 <= p < n, j <= p and (window == 0 or
+ * p - j < window or j < sinks).  out = softmax(scale * q.k) . v over those
+ * keys; a row that sees none gets 0.  Keys that no row sees are not read into
+ * any result, whatever they hold.  q, out: [batch][heads][q_len][head_dim];
+ * k, v: [batch][kv_heads][k_len][head_dim], kv_heads dividing heads (query
+ * heads h * heads / kv_heads ... share key head h); with seq_major
+ * [batch][length][heads][head_dim].  head_dim 1 to 128, scale at least 2^-126.  starts [batch] may
+ * be NULL (k_len - q_len: the queries end where the keys end), lengths
+ * [batch] may be NULL (k_len); both hold whole numbers as floats, checked on
+ * the device ("Attention start or length out of range").  stats may be NULL
+ * or receives [batch][heads][q_len][2] = (greatest visible score, sum of
+ * exp(score - greatest)), (-inf, 0) for a row that sees nothing; the backward
+ * reads it.  Serving calls it with q_len 1 and starts = lengths - 1. */
+bool tysor_cuda_dispatch_window_attention(void* context, void* q, void* k, void* v, void* starts,
+                                          void* lengths, void* out, void* stats, uint32_t batch,
+                                          uint32_t heads, uint32_t kv_heads, uint32_t q_len, uint32_t k_len,
+                                          uint32_t head_dim, uint32_t window, uint32_t sinks, float scale,
+                                          bool seq_major);
+/* dq, dk, dv (+)= the exact gradients of `out` for dout; dk and dv are summed
+ * over the query heads that share a key head, in a fixed order. */
+bool tysor_cuda_dispatch_window_attention_backward(void* context, void* q, void* k, void* v, void* starts,
+                                                   void* lengths, void* out, void* stats, void* dout,
+                                                   void* dq, void* dk, void* dv, uint32_t batch,
+                                                   uint32_t heads, uint32_t kv_heads, uint32_t q_len,
+                                                   uint32_t k_len, uint32_t head_dim, uint32_t window,
+                                                   uint32_t sinks, float scale, bool seq_major,
+                                                   bool accumulate);
+/* Distillation from a teacher's best `top` (1 to 1024) logits per row: p is
+ * the softmax of teacher[r][.] / T, q that of logits[r][.] / T over the whole
+ * width; out[r] = T^2 * sum_e p_e * (ln p_e - ln q[ids[r][e]]).  ids are f32;
+ * an id below 0 is an absent entry, and a row without any has loss 0.  An id
+ * of width or more is an error ("Embedding index out of range").  An id
+ * given twice counts twice.  stats may be NULL or receives [rows][2] =
+ * (greatest logit, sum of exp((logit - greatest) / T)). */
+bool tysor_cuda_dispatch_distill_loss(void* context, void* logits, void* ids, void* teacher, void* out,
+                                      void* stats, uint32_t rows, uint32_t width, uint32_t top,
+                                      float temperature);
+/* grad (+)= dloss[r] * T * (q - p scattered to the ids); 0 for a row without
+ * entries.  dloss may be NULL (1). */
+bool tysor_cuda_dispatch_distill_loss_backward(void* context, void* logits, void* ids, void* teacher,
+                                               void* stats, void* dloss, void* grad, uint32_t rows,
+                                               uint32_t width, uint32_t top, float temperature,
+                                               bool accumulate);
 
 /* ---- device-resident graph executor -------------------------------------
  * Replaces the host interpreters (runtime/graph_executor.rs:249-356,

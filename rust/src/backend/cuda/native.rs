@@ -40,6 +40,7 @@ pub mod ffi {
         pub fn tysor_cuda_buffer_read(buffer: *mut c_void, out_data: *mut f32, count: usize) -> bool;
         pub fn tysor_cuda_buffer_write(buffer: *mut c_void, data: *const f32, count: usize) -> bool;
         pub fn tysor_cuda_buffer_view(base: *mut c_void, offset: usize, count: usize) -> *mut c_void;
+        pub fn tysor_cuda_buffer_wrap(context: *mut c_void, data: *mut f32, count: usize) -> *mut c_void;
         pub fn tysor_cuda_buffer_count(buffer: *mut c_void) -> usize;
         pub fn tysor_cuda_dispatch_matmul(context: *mut c_void, lhs: *mut c_void, rhs: *mut c_void, out: *mut c_void, m: u32, n: u32, k: u32) -> bool;
         pub fn tysor_cuda_dispatch_unary(context: *mut c_void, op: c_int, input: *mut c_void, out: *mut c_void, count: u32, param: f32) -> bool;
@@ -72,6 +73,14 @@ pub mod ffi {
         pub fn tysor_cuda_dispatch_cross_entropy_labels(context: *mut c_void, logits: *mut c_void, labels: *mut c_void, out: *mut c_void, rows: u32, width: u32) -> bool;
         pub fn tysor_cuda_dispatch_cross_entropy_labels_backward(context: *mut c_void, logits: *mut c_void, labels: *mut c_void, grad: *mut c_void, rows: u32, width: u32, accumulate: bool) -> bool;
         pub fn tysor_cuda_dispatch_transpose(context: *mut c_void, input: *mut c_void, out: *mut c_void, dims: *const i64, rank: c_int, a: c_int, b: c_int) -> bool;
+        pub fn tysor_cuda_dispatch_layer_norm(context: *mut c_void, input: *mut c_void, gain: *mut c_void, bias: *mut c_void, out: *mut c_void, stats: *mut c_void, rows: u32, width: u32, eps: f32) -> bool;
+        pub fn tysor_cuda_dispatch_layer_norm_backward(context: *mut c_void, input: *mut c_void, gain: *mut c_void, stats: *mut c_void, dy: *mut c_void, dx: *mut c_void, dgain: *mut c_void, dbias: *mut c_void, rows: u32, width: u32, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_rope_axes(context: *mut c_void, input: *mut c_void, positions: *mut c_void, out: *mut c_void, batch: u32, heads: u32, seq_len: u32, sections: *const i64, axes: c_int, theta: f64, seq_major: bool) -> bool;
+        pub fn tysor_cuda_dispatch_rope_axes_backward(context: *mut c_void, grad: *mut c_void, positions: *mut c_void, dx: *mut c_void, batch: u32, heads: u32, seq_len: u32, sections: *const i64, axes: c_int, theta: f64, seq_major: bool, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_window_attention(context: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, starts: *mut c_void, lengths: *mut c_void, out: *mut c_void, stats: *mut c_void, batch: u32, heads: u32, kv_heads: u32, q_len: u32, k_len: u32, head_dim: u32, window: u32, sinks: u32, scale: f32, seq_major: bool) -> bool;
+        pub fn tysor_cuda_dispatch_window_attention_backward(context: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, starts: *mut c_void, lengths: *mut c_void, out: *mut c_void, stats: *mut c_void, dout: *mut c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, batch: u32, heads: u32, kv_heads: u32, q_len: u32, k_len: u32, head_dim: u32, window: u32, sinks: u32, scale: f32, seq_major: bool, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_distill_loss(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, teacher: *mut c_void, out: *mut c_void, stats: *mut c_void, rows: u32, width: u32, top: u32, temperature: f32) -> bool;
+        pub fn tysor_cuda_dispatch_distill_loss_backward(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, teacher: *mut c_void, stats: *mut c_void, dloss: *mut c_void, grad: *mut c_void, rows: u32, width: u32, top: u32, temperature: f32, accumulate: bool) -> bool;
         pub fn tysor_cuda_graph_new(context: *mut c_void, graph_text: *const c_char) -> *mut c_void;
         pub fn tysor_cuda_graph_free(graph: *mut c_void);
         pub fn tysor_cuda_graph_set_shape(graph: *mut c_void, name: *const c_char, dims: *const i64, rank: c_int) -> bool;

@@ -6,11 +6,13 @@
 #include <string.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <vector>
 
 #include "../../include/tysor_cuda.h"
 #include "context.cuh"
+#include "lm_ops.cuh"
 #include "ops.cuh"
 
 namespace tysor {
@@ -27,6 +29,7 @@ const char* device_error_message(int code) {
     case kErrIndexRange: return "Embedding index out of range";
     case kErrBarrierTimeout: return "a tensor-core pipeline wait timed out";
     case kErrTmemAlloc: return "tensor memory allocation failed";
+    case kErrSequence: return "Attention start or length out of range";
     default: return "unknown device error";
   }
 }
@@ -63,6 +66,21 @@ const float2* Context::rope_table(int64_t seq, int64_t half, double theta) {
   TYSOR_CUDA(cudaMalloc(&d, sizeof(float2) * tab.size()));
   TYSOR_CUDA(cudaMemcpy(d, tab.data(), sizeof(float2) * tab.size(), cudaMemcpyHostToDevice));
   rope_tables[key] = d;
+  return d;
+}
+
+const double* Context::rope_rate_table(int64_t half, double theta) {
+  uint64_t bits;
+  std::memcpy(&bits, &theta, sizeof bits);
+  auto key = std::make_tuple(half, bits);
+  auto it = rope_rates.find(key);
+  if (it != rope_rates.end()) return it->second;
+  std::vector<double> rate((size_t)half);
+  for (int64_t i = 0; i < half; ++i) rate[i] = pow(theta, -(double)i / (double)half) / (2.0 * 3.14159265358979323846);
+  double* d = nullptr;
+  TYSOR_CUDA(cudaMalloc(&d, sizeof(double) * rate.size()));
+  TYSOR_CUDA(cudaMemcpy(d, rate.data(), sizeof(double) * rate.size(), cudaMemcpyHostToDevice));
+  rope_rates[key] = d;
   return d;
 }
 
@@ -146,6 +164,121 @@ float* scratch_floats(Context* c, int64_t n) {
   return (float*)c->ensure_scratch(sizeof(float) * (size_t)(n > 0 ? n : 1));
 }
 
+// A dispatch's operands: each holds what the call needs and lies on the
+// context's device, pairs of values (statistics) are 8-byte aligned, and no
+// output overlaps an input or another output.
+struct Operands {
+  Context* ctx;
+  struct Range {
+    uintptr_t begin, end;
+    const char* what;
+    bool written;
+  };
+  std::vector<Range> ranges;
+
+  explicit Operands(Context* c) : ctx(c) {}
+
+  float* take(void* p, size_t need, const char* what, bool written) {
+    float* f = ptr_of(p, need, what);
+    if (buf_of(p)->ctx->device != ctx->device)
+      throw CudaError(std::string(what) + " buffer is on another device");
+    if (std::strcmp(what, "stats") == 0 && ((uintptr_t)f & 7) != 0)
+      throw CudaError("stats buffer must start on an 8-byte boundary");
+    ranges.push_back({(uintptr_t)f, (uintptr_t)(f + need), what, written});
+    return f;
+  }
+  const float* in(void* p, size_t need, const char* what) { return take(p, need, what, false); }
+  const float* in_or_null(void* p, size_t need, const char* what) { return p ? in(p, need, what) : nullptr; }
+  float* out(void* p, size_t need, const char* what) { return take(p, need, what, true); }
+  float* out_or_null(void* p, size_t need, const char* what) { return p ? out(p, need, what) : nullptr; }
+
+  void check_overlap() const {
+    for (const Range& a : ranges)
+      for (const Range& b : ranges)
+        if (&a != &b && a.written && a.begin < a.end && b.begin < b.end && a.begin < b.end && b.begin < a.end)
+          throw CudaError(std::string(a.what) + " overlaps " + b.what);
+  }
+};
+
+// The product of sizes, refused where no buffer could hold it.
+size_t elems(std::initializer_list<uint64_t> sizes) {
+  uint64_t n = 1;
+  for (uint64_t d : sizes)
+    if (d == 0) return 0;
+  for (uint64_t d : sizes) {
+    if (n > ((uint64_t)1 << 60) / d) throw CudaError("sizes overflow");
+    n *= d;
+  }
+  return (size_t)n;
+}
+
+void check_norm(uint32_t width, float eps) {
+  if (width == 0) throw CudaError("layer_norm requires a width of at least 1");
+  if (!(eps >= 0.0f) || isinf(eps)) throw CudaError("layer_norm requires a finite eps >= 0");
+}
+
+void check_distill(uint32_t width, uint32_t top, float temperature) {
+  if (width == 0 || width > 0x7fffffffu) throw CudaError("distill_loss requires a width of 1 to 2^31 - 1");
+  if (top == 0 || top > (uint32_t)kMaxDistillTop)
+    throw CudaError("distill_loss takes 1 to " + std::to_string(kMaxDistillTop) + " entries per row");
+  if (!(temperature > 0.0f) || isinf(temperature)) throw CudaError("distill_loss requires a finite temperature > 0");
+}
+
+AttentionShape attention_shape(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t q_len, uint32_t k_len,
+                               uint32_t head_dim, uint32_t window, uint32_t sinks, float scale, bool seq_major) {
+  if (heads == 0 || kv_heads == 0 || heads % kv_heads != 0)
+    throw CudaError("window_attention: the key heads must divide the query heads");
+  if (head_dim == 0 || head_dim > (uint32_t)kMaxHeadDim)
+    throw CudaError("window_attention takes heads of 1 to " + std::to_string(kMaxHeadDim) + " values");
+  const uint32_t most = 1u << 30;
+  if (q_len > most || k_len > most || batch > most || heads > most)
+    throw CudaError("window_attention takes lengths, batches and heads up to 2^30");
+  // A subnormal scale would hold fewer bits than the scores it multiplies.
+  if (!(scale >= 1.17549435e-38f) || isinf(scale))
+    throw CudaError("window_attention requires a finite scale of at least 2^-126");
+  AttentionShape s{};
+  s.batch = (int)batch;
+  s.heads = (int)heads;
+  s.kv_heads = (int)kv_heads;
+  s.q_len = (int)q_len;
+  s.k_len = (int)k_len;
+  s.head_dim = (int)head_dim;
+  s.window = (int)(window < most ? window : most);  // no position lies further back
+  s.sinks = (int)(sinks < most ? sinks : most);
+  s.scale = scale;
+  s.seq_major = seq_major;
+  return s;
+}
+
+void rope_axes(void* context, void* x, void* positions, void* out, uint32_t batch, uint32_t heads, uint32_t seq_len,
+               const int64_t* sections, int axes, double theta, bool seq_major, bool back, bool accumulate) {
+  Operands o(ctx_of(context));
+  if (sections == nullptr || axes < 1 || axes > kMaxRopeAxes)
+    throw CudaError("rope_axes takes 1 to " + std::to_string(kMaxRopeAxes) + " axes");
+  if (!(theta > 0.0) || isinf(theta)) throw CudaError("rope_axes requires a finite theta > 0");
+  const uint32_t most = 1u << 30;
+  if (batch > most || heads > most || seq_len > most) throw CudaError("rope_axes takes sizes up to 2^30");
+  RopeAxes s{};
+  s.batch = (int)batch;
+  s.heads = (int)heads;
+  s.seq = (int)seq_len;
+  s.axes = axes;
+  s.seq_major = seq_major;
+  int64_t half = 0;
+  for (int a = 0; a < axes; ++a) {
+    if (sections[a] < 1 || sections[a] > 65536) throw CudaError("rope_axes sections hold 1 to 65536 pairs");
+    half += sections[a];
+    s.ends[a] = (int)half;
+  }
+  s.half = (int)half;
+  const size_t n = elems({batch, heads, seq_len, 2 * (uint64_t)half});
+  const float* in = o.in(x, n, back ? "grad" : "input");
+  const float* pos = o.in(positions, elems({batch, (uint64_t)axes, seq_len}), "positions");
+  float* y = o.out(out, n, back ? "dx" : "out");
+  o.check_overlap();
+  launch_rope_axes(in, pos, o.ctx->rope_rate_table(half, theta), y, s, back, accumulate, o.ctx->stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -182,6 +315,7 @@ void tysor_cuda_context_free(void* context) {
     cudaSetDevice(c->device);
     cudaStreamSynchronize(c->stream);
     for (auto& kv : c->rope_tables) cudaFree(kv.second);
+    for (auto& kv : c->rope_rates) cudaFree(kv.second);
     if (c->scratch) cudaFree(c->scratch);
     if (c->d_err) cudaFree(c->d_err);
     if (c->comm) tysor_cuda_comm_free(c);
@@ -289,6 +423,25 @@ void* tysor_cuda_buffer_view(void* base, size_t offset, size_t count) {
     v->count = count;
     v->owned = false;
     out = v;
+  });
+  return out;
+}
+
+void* tysor_cuda_buffer_wrap(void* context, float* data, size_t count) {
+  Buffer* out = nullptr;
+  guarded([&] {
+    Context* c = ctx_of(context);
+    if (data == nullptr) throw CudaError("wrap: null device pointer");
+    if (((uintptr_t)data & 3) != 0) throw CudaError("wrap: the memory is not aligned to its fp32 values");
+    cudaPointerAttributes attr;
+    TYSOR_CUDA(cudaPointerGetAttributes(&attr, data));
+    if (attr.type != cudaMemoryTypeDevice || attr.device != c->device)
+      throw CudaError("wrap: the memory is not on the context's device");
+    auto* b = new Buffer();
+    b->ctx = c;
+    b->ptr = data;
+    b->count = count;
+    out = b;
   });
   return out;
 }
@@ -608,6 +761,148 @@ bool tysor_cuda_dispatch_cross_entropy_labels_backward(void* context, void* logi
     launch_cross_entropy_labels_backward(ptr_of(logits, n, "logits"), ptr_of(labels, rows, "labels"),
                                          ptr_of(grad, n, "grad"), rows, width, accumulate, c->d_err,
                                          c->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_layer_norm(void* context, void* input, void* gain, void* bias, void* out,
+                                    void* stats, uint32_t rows, uint32_t width, float eps) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    check_norm(width, eps);
+    const size_t n = (size_t)rows * width;
+    const float* x = o.in(input, n, "input");
+    const float* g = o.in_or_null(gain, width, "gain");
+    const float* b = o.in_or_null(bias, width, "bias");
+    float* y = o.out(out, n, "out");
+    float* s = o.out_or_null(stats, (size_t)rows * 2, "stats");
+    o.check_overlap();
+    launch_layer_norm(x, g, b, y, s, rows, width, eps, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_layer_norm_backward(void* context, void* input, void* gain, void* stats, void* dy,
+                                             void* dx, void* dgain, void* dbias, uint32_t rows,
+                                             uint32_t width, bool accumulate) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    check_norm(width, 0.0f);
+    const size_t n = (size_t)rows * width;
+    const float* x = o.in(input, n, "input");
+    const float* g = o.in_or_null(gain, width, "gain");
+    const float* s = o.in(stats, (size_t)rows * 2, "stats");
+    const float* gy = o.in(dy, n, "dy");
+    float* gx = o.out(dx, n, "dx");
+    float* gg = o.out_or_null(dgain, width, "dgain");
+    float* gb = o.out_or_null(dbias, width, "dbias");
+    o.check_overlap();
+    float* partial = scratch_floats(o.ctx, layer_norm_partial_elems(rows, width));
+    launch_layer_norm_backward(x, g, s, gy, gx, gg, gb, partial, rows, width, accumulate, accumulate,
+                               o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_rope_axes(void* context, void* input, void* positions, void* out, uint32_t batch,
+                                   uint32_t heads, uint32_t seq_len, const int64_t* sections, int axes,
+                                   double theta, bool seq_major) {
+  return guarded([&] {
+    rope_axes(context, input, positions, out, batch, heads, seq_len, sections, axes, theta, seq_major, false,
+              false);
+  });
+}
+
+bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* positions, void* dx,
+                                            uint32_t batch, uint32_t heads, uint32_t seq_len,
+                                            const int64_t* sections, int axes, double theta, bool seq_major,
+                                            bool accumulate) {
+  return guarded([&] {
+    rope_axes(context, grad, positions, dx, batch, heads, seq_len, sections, axes, theta, seq_major, true,
+              accumulate);
+  });
+}
+
+bool tysor_cuda_dispatch_window_attention(void* context, void* q, void* k, void* v, void* starts,
+                                          void* lengths, void* out, void* stats, uint32_t batch,
+                                          uint32_t heads, uint32_t kv_heads, uint32_t q_len, uint32_t k_len,
+                                          uint32_t head_dim, uint32_t window, uint32_t sinks, float scale,
+                                          bool seq_major) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    AttentionShape s = attention_shape(batch, heads, kv_heads, q_len, k_len, head_dim, window, sinks, scale, seq_major);
+    const size_t nq = elems({batch, heads, q_len, head_dim}), nk = elems({batch, kv_heads, k_len, head_dim});
+    const float* qp = o.in(q, nq, "q");
+    const float* kp = o.in(k, nk, "k");
+    const float* vp = o.in(v, nk, "v");
+    s.starts = o.in_or_null(starts, batch, "starts");
+    s.lengths = o.in_or_null(lengths, batch, "lengths");
+    float* op = o.out(out, nq, "out");
+    float* sp = o.out_or_null(stats, elems({batch, heads, q_len, 2}), "stats");
+    o.check_overlap();
+    float* work = scratch_floats(o.ctx, window_attention_work_elems(s));
+    launch_window_attention(s, qp, kp, vp, op, sp, work, o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_window_attention_backward(void* context, void* q, void* k, void* v, void* starts,
+                                                   void* lengths, void* out, void* stats, void* dout,
+                                                   void* dq, void* dk, void* dv, uint32_t batch,
+                                                   uint32_t heads, uint32_t kv_heads, uint32_t q_len,
+                                                   uint32_t k_len, uint32_t head_dim, uint32_t window,
+                                                   uint32_t sinks, float scale, bool seq_major,
+                                                   bool accumulate) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    AttentionShape s = attention_shape(batch, heads, kv_heads, q_len, k_len, head_dim, window, sinks, scale, seq_major);
+    const size_t nq = elems({batch, heads, q_len, head_dim}), nk = elems({batch, kv_heads, k_len, head_dim});
+    const float* qp = o.in(q, nq, "q");
+    const float* kp = o.in(k, nk, "k");
+    const float* vp = o.in(v, nk, "v");
+    s.starts = o.in_or_null(starts, batch, "starts");
+    s.lengths = o.in_or_null(lengths, batch, "lengths");
+    const float* op = o.in(out, nq, "out");
+    const float* sp = o.in(stats, elems({batch, heads, q_len, 2}), "stats");
+    const float* gp = o.in(dout, nq, "dout");
+    float* gq = o.out(dq, nq, "dq");
+    float* gk = o.out(dk, nk, "dk");
+    float* gv = o.out(dv, nk, "dv");
+    o.check_overlap();
+    float* work = scratch_floats(o.ctx, window_attention_backward_work_elems(s));
+    launch_window_attention_backward(s, qp, kp, vp, op, sp, gp, gq, gk, gv, work, accumulate, accumulate, accumulate,
+                                     o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_distill_loss(void* context, void* logits, void* ids, void* teacher, void* out,
+                                      void* stats, uint32_t rows, uint32_t width, uint32_t top,
+                                      float temperature) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    check_distill(width, top, temperature);
+    const float* z = o.in(logits, (size_t)rows * width, "logits");
+    const float* id = o.in(ids, (size_t)rows * top, "ids");
+    const float* t = o.in(teacher, (size_t)rows * top, "teacher");
+    float* l = o.out(out, rows, "out");
+    float* s = o.out_or_null(stats, (size_t)rows * 2, "stats");
+    o.check_overlap();
+    launch_distill_loss(z, id, t, l, s, rows, width, (int)top, temperature, o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_distill_loss_backward(void* context, void* logits, void* ids, void* teacher,
+                                               void* stats, void* dloss, void* grad, uint32_t rows,
+                                               uint32_t width, uint32_t top, float temperature,
+                                               bool accumulate) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    check_distill(width, top, temperature);
+    const float* z = o.in(logits, (size_t)rows * width, "logits");
+    const float* id = o.in(ids, (size_t)rows * top, "ids");
+    const float* t = o.in(teacher, (size_t)rows * top, "teacher");
+    const float* s = o.in(stats, (size_t)rows * 2, "stats");
+    const float* d = o.in_or_null(dloss, rows, "dloss");
+    float* g = o.out(grad, (size_t)rows * width, "grad");
+    o.check_overlap();
+    launch_distill_loss_backward(z, id, t, s, d, g, rows, width, (int)top, temperature, accumulate, o.ctx->d_err,
+                                 o.ctx->stream);
   });
 }
 

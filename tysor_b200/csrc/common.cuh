@@ -34,6 +34,7 @@ enum DeviceError : int {
   kErrIndexRange = 1,      // embedding / label index outside [0, n)
   kErrBarrierTimeout = 2,  // an mbarrier wait ran past its time limit
   kErrTmemAlloc = 3,
+  kErrSequence = 4,        // an attention start or length that fits no sequence
 };
 
 struct CudaError : std::runtime_error {

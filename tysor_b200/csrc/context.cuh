@@ -30,6 +30,8 @@ struct Context {
   size_t scratch_bytes = 0;
   // cos/sin tables for RoPE, keyed by (seq, half, theta bits).
   std::map<std::tuple<int64_t, int64_t, uint64_t>, float2*> rope_tables;
+  // rope_axes' rates in revolutions per position, keyed by (half, theta bits).
+  std::map<std::tuple<int64_t, uint64_t>, double*> rope_rates;
   // NCCL communicator (opaque ncclComm_t) when data parallel.
   void* comm = nullptr;
   int nranks = 1;
@@ -39,6 +41,8 @@ struct Context {
   void* ensure_scratch(size_t bytes);
   // Device (cos, sin) table for rope over `seq` positions and `half` freqs.
   const float2* rope_table(int64_t seq, int64_t half, double theta);
+  // Device theta^(-i / half) / 2 pi for rope_axes' `half` pairs.
+  const double* rope_rate_table(int64_t half, double theta);
   // Waits for the stream and turns a recorded device error into a message.
   void sync_and_check();
 };

@@ -14,6 +14,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <cmath>
 #include <deque>
 #include <functional>
 #include <map>
@@ -21,10 +22,12 @@
 #include <set>
 #include <sstream>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "../../include/tysor_cuda.h"
 #include "context.cuh"
+#include "lm_ops.cuh"
 #include "ops.cuh"
 
 namespace tysor {
@@ -61,7 +64,7 @@ struct Slot {
 };
 
 struct HVal {
-  enum T { None, Int, Float, Bool, Tensor, Linear, Embedding, Act, RmsNorm } t = None;
+  enum T { None, Int, Float, Bool, Tensor, Linear, Embedding, Act, RmsNorm, LayerNorm } t = None;
   int64_t i = 0;
   double f = 0;
   bool b = false;
@@ -93,7 +96,7 @@ struct Param {
   // Backward items that must run before the gradient is final (the index
   // just past the last item that writes it).
   size_t grad_ready = 0;
-  // initialiser: 0 linear weight, 1 linear bias, 2 embedding weight, 3 ones
+  // initialiser: 0 linear weight, 1 linear bias, 2 embedding weight, 3 ones, 6 zeros
   int init = 0;
 };
 
@@ -299,6 +302,7 @@ struct Executor {
     causal_leak.clear();
     folded_transpose.clear();
     grad_alias.clear();
+    op_stats.clear();
     loss = grad_block = scratch = param_block = nullptr;
     param_block_n = 0;
     scratch_floats = 0;
@@ -464,6 +468,7 @@ struct Executor {
       case 2: launch_pattern(p, n, 17, 1.0f, 8.0f, st); break;    // layers.rs:65-75
       case 3: launch_fill(p, n, 1.0f, st); break;                 // RMSNorm gain
       case 4: launch_pattern(p, n, 11, -5.0f, 16.0f, st); break;  // backward.rs:225-235
+      case 6: launch_fill(p, n, 0.0f, st); break;                 // LayerNorm bias
       default: launch_pattern(p, n, 17, 1.0f, 8.0f, st); break;   // tensor.rs:24-34
     }
   }
@@ -1215,7 +1220,150 @@ struct Executor {
       });
       return o;
     }
+    if (op == "rope_axes") {
+      const RopeCall r = rope_call(node);
+      HVal o = new_tensor(val(node.inputs[0]).shape);
+      Slot *a = val(node.inputs[0]).slot, *pos = val(node.inputs[1]).slot, *c = o.slot;
+      forward.push_back([=](cudaStream_t st) { launch_rope_axes(a->p, pos->p, r.rates, c->p, r.axes, 0, 0, st); });
+      return o;
+    }
+    if (op == "window_attention") {
+      const AttentionCall ac = attention_call(node);
+      HVal o = new_tensor(val(node.inputs[0]).shape);
+      Slot *q = val(node.inputs[0]).slot, *k = val(node.inputs[1]).slot, *v = val(node.inputs[2]).slot, *c = o.slot;
+      Slot* stats = mode == kModeRun ? nullptr : alloc((size_t)ac.s.batch * ac.s.heads * ac.s.q_len * 2);
+      op_stats[node.output] = stats;
+      need_scratch((size_t)window_attention_work_elems(ac.s));
+      Slot** scr = &scratch;
+      Context* cx = ctx;
+      forward.push_back([=](cudaStream_t st) {
+        launch_window_attention(ac.shape(), q->p, k->p, v->p, c->p, stats ? stats->p : nullptr, (*scr)->p, cx->d_err,
+                                st);
+      });
+      return o;
+    }
+    if (op == "distill_loss") {
+      const HVal& z = tensor(node.inputs.at(0), "distill_loss");
+      const HVal& id = tensor(node.inputs.at(1), "distill_loss ids");
+      const HVal& t = tensor(node.inputs.at(2), "distill_loss teacher");
+      const float temperature = (float)number(val(node.inputs.at(3)));
+      if (node.inputs.size() != 4 || z.shape.empty() || z.shape.back() < 1)
+        fail("distill_loss expects (logits, ids, teacher, temperature)");
+      const int64_t w = z.shape.back(), rows = numel(z.shape) / w;
+      const int64_t top = id.shape.empty() ? 0 : id.shape.back();
+      if (id.shape != t.shape || top < 1 || numel(id.shape) != rows * top)
+        fail("distill_loss expects ids and teacher of [rows, top] for logits " + shape_str(z.shape) + ", got " +
+             shape_str(id.shape) + " and " + shape_str(t.shape));
+      if (top > kMaxDistillTop || w > INT32_MAX) fail("distill_loss takes 1 to " + std::to_string(kMaxDistillTop) + " entries per row");
+      if (!(temperature > 0.0f) || std::isinf(temperature)) fail("distill_loss requires a finite temperature > 0");
+      HVal o = new_tensor({rows, 1});
+      Slot *a = z.slot, *ix = id.slot, *ts = t.slot, *c = o.slot;
+      Slot* stats = mode == kModeRun ? nullptr : alloc((size_t)rows * 2);
+      op_stats[node.output] = stats;
+      Context* cx = ctx;
+      forward.push_back([=](cudaStream_t st) {
+        launch_distill_loss(a->p, ix->p, ts->p, c->p, stats ? stats->p : nullptr, rows, w, (int)top, temperature,
+                            cx->d_err, st);
+      });
+      return o;
+    }
     fail("Unsupported library graph call '" + op + "'");
+  }
+
+  // Row statistics that a layer_norm, window_attention or distill_loss node's
+  // forward leaves for its backward (null in --run).
+  std::map<int, Slot*> op_stats;
+
+  // rope_axes(x, positions, theta, section, ... [, seq_major]).
+  struct RopeCall {
+    RopeAxes axes;
+    const double* rates;
+  };
+  // A trailing truth value among a call's constant arguments from `first` on:
+  // whether sequences come before heads ([B, S, H, hd]).
+  bool trailing_seq_major(const GNode& node, size_t first, size_t* end) const {
+    *end = node.inputs.size();
+    if (*end <= first || val(node.inputs[*end - 1]).t != HVal::Bool) return false;
+    --*end;
+    return val(node.inputs[*end]).b;
+  }
+
+  RopeCall rope_call(const GNode& node) {
+    const HVal& x = tensor(node.inputs.at(0), "rope_axes");
+    const HVal& pos = tensor(node.inputs.at(1), "rope_axes positions");
+    const double theta = number(val(node.inputs.at(2)));
+    size_t end;
+    RopeCall r{};
+    r.axes.seq_major = trailing_seq_major(node, 3, &end);
+    r.axes.axes = (int)(end - 3);
+    if (end < 4 || r.axes.axes > kMaxRopeAxes)
+      fail("rope_axes takes 1 to " + std::to_string(kMaxRopeAxes) + " sections");
+    if (!(theta > 0.0) || std::isinf(theta)) fail("rope_axes requires a finite theta > 0");
+    int64_t half = 0;
+    for (size_t i = 3; i < end; ++i) {
+      const int64_t n = integer(val(node.inputs[i]));
+      if (n < 1 || n > 65536) fail("rope_axes sections hold 1 to 65536 pairs");
+      half += n;
+      r.axes.ends[i - 3] = (int)half;
+    }
+    if (x.shape.size() != 4 || x.shape[3] != 2 * half)
+      fail("rope_axes expects a rank-4 input of heads of " + std::to_string(2 * half) + ", got " + shape_str(x.shape));
+    r.axes.batch = (int)x.shape[0];
+    r.axes.heads = (int)x.shape[r.axes.seq_major ? 2 : 1];
+    r.axes.seq = (int)x.shape[r.axes.seq_major ? 1 : 2];
+    r.axes.half = (int)half;
+    if (pos.shape != std::vector<int64_t>{x.shape[0], (int64_t)r.axes.axes, (int64_t)r.axes.seq})
+      fail("rope_axes expects positions [batch, axes, sequence], got " + shape_str(pos.shape));
+    r.rates = ctx->rope_rate_table(half, theta);
+    return r;
+  }
+
+  // window_attention(q, k, v, window, sinks [, lengths [, starts]] [, seq_major]),
+  // scores scaled by 1 / sqrt(head width).
+  struct AttentionCall {
+    AttentionShape s;
+    Slot* starts = nullptr;
+    Slot* lengths = nullptr;
+    AttentionShape shape() const {
+      AttentionShape r = s;
+      r.starts = starts ? starts->p : nullptr;
+      r.lengths = lengths ? lengths->p : nullptr;
+      return r;
+    }
+  };
+
+  AttentionCall attention_call(const GNode& node) {
+    const HVal& q = tensor(node.inputs.at(0), "window_attention");
+    const HVal& k = tensor(node.inputs.at(1), "window_attention keys");
+    const HVal& v = tensor(node.inputs.at(2), "window_attention values");
+    const int64_t window = integer(val(node.inputs.at(3))), sinks = integer(val(node.inputs.at(4)));
+    AttentionCall c;
+    size_t end;
+    c.s.seq_major = trailing_seq_major(node, 5, &end);
+    const int sl = c.s.seq_major ? 1 : 2, hl = c.s.seq_major ? 2 : 1;
+    if (q.shape.size() != 4 || k.shape.size() != 4 || k.shape != v.shape || k.shape[0] != q.shape[0] ||
+        k.shape[3] != q.shape[3] || q.shape[hl] % k.shape[hl] != 0)
+      fail("window_attention expects q, k, v of rank 4 with k and v alike and heads that share theirs, got " +
+           shape_str(q.shape) + ", " + shape_str(k.shape) + " and " + shape_str(v.shape));
+    if (q.shape[3] > kMaxHeadDim)
+      fail("window_attention takes heads of 1 to " + std::to_string(kMaxHeadDim) + " values");
+    if (window < 0 || sinks < 0) fail("window_attention requires window >= 0 and sinks >= 0");
+    for (size_t i = 5; i < end; ++i) {
+      const HVal& t = tensor(node.inputs[i], "window_attention lengths");
+      if (i > 6 || numel(t.shape) != q.shape[0]) fail("window_attention expects one length and one start per sequence");
+      (i == 5 ? c.lengths : c.starts) = t.slot;
+    }
+    const int64_t most = 1 << 30;
+    c.s.batch = (int)q.shape[0];
+    c.s.heads = (int)q.shape[hl];
+    c.s.kv_heads = (int)k.shape[hl];
+    c.s.q_len = (int)q.shape[sl];
+    c.s.k_len = (int)k.shape[sl];
+    c.s.head_dim = (int)q.shape[3];
+    c.s.window = (int)(window < most ? window : most);
+    c.s.sinks = (int)(sinks < most ? sinks : most);
+    c.s.scale = (float)(1.0 / std::sqrt((double)q.shape[3]));
+    return c;
   }
 
   HVal plan_ctor(const GNode& node) {
@@ -1259,6 +1407,17 @@ struct Executor {
       h.eps = in.size() > 1 ? number(val(in[1])) : 1e-5;
       return h;
     }
+    if (node.op == "LayerNorm") {
+      // LayerNorm(width [, eps [, bias]]): a learned gain and, unless `bias`
+      // is false, a learned bias.
+      h.t = HVal::LayerNorm;
+      h.hidden = integer(val(in.at(0)));
+      h.eps = in.size() > 1 ? number(val(in[1])) : 1e-5;
+      if (in.size() > 2) h.with_bias = boolean(val(in[2]));
+      if (h.hidden < 1 || h.hidden > INT32_MAX || !(h.eps >= 0.0) || std::isinf(h.eps))
+        fail("LayerNorm requires a width of at least 1 and a finite eps >= 0");
+      return h;
+    }
     fail("Unsupported library constructor '" + node.op + "'");
   }
 
@@ -1266,6 +1425,8 @@ struct Executor {
   std::string linear_bias_name(int id) { return "linear_" + std::to_string(id) + "_bias"; }
   std::string embedding_weight_name(int id) { return "embedding_" + std::to_string(id) + "_weight"; }
   std::string gain_name(int id) { return "rmsnorm_" + std::to_string(id) + "_gain"; }
+
+  std::string layer_norm_name(int id, const char* what) { return "layernorm_" + std::to_string(id) + "_" + what; }
 
   // Table of an Embedding constructor: named parameter (train, created on
   // first use) or the constant pattern.
@@ -1348,6 +1509,27 @@ struct Executor {
         const int64_t h = cl.hidden, rows = numel(x.shape) / h;
         const float eps = (float)cl.eps;
         forward.push_back([=](cudaStream_t st) { launch_rms_norm_gain(a->p, g->p, c->p, rows, h, eps, st); });
+        return o;
+      }
+      case HVal::LayerNorm: {
+        if (x.shape.empty() || x.shape.back() != cl.hidden)
+          fail("layer_norm hidden size mismatch: expected " + std::to_string(cl.hidden) + ", got " + shape_str(x.shape));
+        const bool train = mode == kModeTrain;
+        Slot* g = train ? ensure_param(layer_norm_name(cl.ctor_id, "gain"), {cl.hidden}, 3).value
+                        : const_pattern({cl.hidden}, 3);
+        Slot* b = nullptr;
+        if (cl.with_bias)
+          b = train ? ensure_param(layer_norm_name(cl.ctor_id, "bias"), {cl.hidden}, 6).value
+                    : const_pattern({cl.hidden}, 6);
+        HVal o = new_tensor(x.shape);
+        Slot *a = x.slot, *c = o.slot;
+        const int64_t h = cl.hidden, rows = numel(x.shape) / h;
+        const float eps = (float)cl.eps;
+        Slot* stats = mode == kModeRun ? nullptr : alloc((size_t)rows * 2);
+        op_stats[node.output] = stats;
+        forward.push_back([=](cudaStream_t st) {
+          launch_layer_norm(a->p, g->p, b ? b->p : nullptr, c->p, stats ? stats->p : nullptr, rows, h, eps, st);
+        });
         return o;
       }
       case HVal::Act: {
@@ -1739,6 +1921,65 @@ struct Executor {
       });
       return;
     }
+    if (op == "rope_axes") {
+      const RopeCall r = rope_call(node);
+      Slot* pos = val(node.inputs[1]).slot;
+      auto [d, acc] = contrib(xi);
+      backward.push_back([=](cudaStream_t st) { launch_rope_axes(g->p, pos->p, r.rates, d->p, r.axes, 1, acc, st); });
+      return;
+    }
+    if (op == "window_attention") {
+      const AttentionCall ac = attention_call(node);
+      Slot* in[3];
+      Slot* grad[3];
+      bool acc[3];
+      std::vector<std::pair<Slot*, Slot*>> sums;  // (value's gradient, its further contribution)
+      for (int i = 0; i < 3; ++i) {
+        const int id = node.inputs[i];
+        in[i] = val(id).slot;
+        auto [d, a] = contrib(id);
+        grad[i] = d;
+        acc[i] = a;
+        // One value read as two of q, k and v: the kernels write its
+        // gradients at the same time, so the later one gets memory of its own.
+        for (int j = 0; j < i; ++j)
+          if (node.inputs[j] == id) {
+            grad[i] = alloc((size_t)numel(val(id).shape));
+            acc[i] = false;
+            sums.push_back({d, grad[i]});
+            break;
+          }
+      }
+      Slot *q = in[0], *k = in[1], *v = in[2], *dq = grad[0], *dk = grad[1], *dv = grad[2];
+      const bool aq = acc[0], ak = acc[1], av = acc[2];
+      Slot *o = out.slot, *stats = op_stats.at(node.output);
+      need_scratch((size_t)window_attention_backward_work_elems(ac.s));
+      Slot** scr = &scratch;
+      Context* cx = ctx;
+      backward.push_back([=](cudaStream_t st) {
+        launch_window_attention_backward(ac.shape(), q->p, k->p, v->p, o->p, stats->p, g->p, dq->p, dk->p, dv->p,
+                                         (*scr)->p, aq, ak, av, cx->d_err, st);
+      });
+      for (auto [total, part] : sums)
+        backward.push_back([total = total, part = part](cudaStream_t st) {
+          launch_add_inplace(total->p, part->p, (int64_t)total->n, st);
+        });
+      return;
+    }
+    if (op == "distill_loss") {
+      const int64_t w = x.shape.back(), rows = numel(x.shape) / w;
+      const int64_t top = val(node.inputs[1]).shape.back();
+      const float temperature = (float)number(val(node.inputs[3]));
+      Slot *z = x.slot, *ix = val(node.inputs[1]).slot, *ts = val(node.inputs[2]).slot;
+      Slot* stats = op_stats.at(node.output);
+      auto [d, acc] = contrib(xi);
+      Context* cx = ctx;
+      backward.push_back([=](cudaStream_t st) {
+        launch_distill_loss_backward(z->p, ix->p, ts->p, stats->p, g->p, d->p, rows, w, (int)top, temperature, acc,
+                                     cx->d_err, st);
+      });
+      return;
+    }
     if (!train) fail("Unsupported library op '" + op + "' in graph backward");
     if (op == "tied_logits") {
       // dh (+)= g . E  and  dE (+)= g^T . h  (g: [m, num], E: [num, dim])
@@ -1855,6 +2096,25 @@ struct Executor {
         Slot* xs = x.slot;
         backward.push_back([=](cudaStream_t st) {
           launch_rms_norm_gain_backward(xs->p, gain->p, g->p, d->p, dg->p, (*scr)->p, rows, h, eps, acc, accg, st);
+        });
+        return;
+      }
+      case HVal::LayerNorm: {
+        const int64_t h = cl.hidden, rows = numel(x.shape) / h;
+        Slot* gain = train ? params.at(layer_norm_name(cl.ctor_id, "gain")).value : const_pattern({h}, 3);
+        Slot *dg = nullptr, *db = nullptr;
+        bool accg = false;
+        if (train) {
+          std::tie(dg, accg) = param_contrib(layer_norm_name(cl.ctor_id, "gain"));
+          if (cl.with_bias) db = param_contrib(layer_norm_name(cl.ctor_id, "bias")).first;
+        }
+        auto [d, acc] = contrib(xi);
+        need_scratch((size_t)layer_norm_partial_elems(rows, h));
+        Slot** scr = &scratch;
+        Slot *xs = x.slot, *stats = op_stats.at(node.output);
+        backward.push_back([=](cudaStream_t st) {
+          launch_layer_norm_backward(xs->p, gain->p, stats->p, g->p, d->p, dg ? dg->p : nullptr, db ? db->p : nullptr,
+                                     (*scr)->p, rows, h, acc, accg, st);
         });
         return;
       }

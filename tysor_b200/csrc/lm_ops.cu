@@ -1,0 +1,818 @@
+// Layer norm, rotary positions over several axes and distillation from a
+// teacher's top logits (lm_ops.cuh), forward and backward.  All of them move
+// memory far more than they compute: every kernel reads and writes each value
+// once, and what limits it is HBM (or, for a few rows, one launch's latency).
+#include <limits.h>
+#include <math.h>
+
+#include "lm_ops.cuh"
+
+namespace tysor {
+namespace {
+
+void check_launch() {
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  TYSOR_CUDA(cudaGetLastError());
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sums of (a, b) over the threads of a group of TPR threads (TPR a multiple
+// of the warp).  `red` is the group's own shared array of 2 * TPR / 32 floats;
+// groups of one block wait on barriers of their own.  `phase` alternates
+// between calls so that one barrier per call is enough.
+template <int TPR>
+__device__ __forceinline__ void group_sum2(float& a, float& b, float2* red, int group, int phase) {
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int t = threadIdx.x % TPR;
+    float2* r = red + phase * W;
+    if ((t & 31) == 0) r[t >> 5] = make_float2(a, b);
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+    a = 0.0f;
+    b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      a += r[i].x;
+      b += r[i].y;
+    }
+  }
+}
+
+// A thread's share of a row: NV float4 at columns 4 (t + i TPR), or, where a
+// row may start off a 16-byte boundary, 4 NV floats at columns t + i TPR.
+template <int TPR, int NV, bool VEC>
+struct RowPart {
+  static constexpr int E = 4 * NV;
+  __device__ static __forceinline__ int col(int t, int e) {
+    return VEC ? 4 * (t + (e / 4) * TPR) + e % 4 : t + e * TPR;
+  }
+  __device__ static __forceinline__ void load(const float* __restrict__ p, int width, int t, float (&v)[E],
+                                              float fill) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 4 * (t + i * TPR);
+        const float4 f = c < width ? *(const float4*)(p + c) : make_float4(fill, fill, fill, fill);
+        v[4 * i] = f.x;
+        v[4 * i + 1] = f.y;
+        v[4 * i + 2] = f.z;
+        v[4 * i + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = t + i * TPR;
+        v[i] = c < width ? p[c] : fill;
+      }
+    }
+  }
+  __device__ static __forceinline__ void store(float* __restrict__ p, int width, int t, const float (&v)[E]) {
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = 4 * (t + i * TPR);
+        if (c < width) *(float4*)(p + c) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int c = t + i * TPR;
+        if (c < width) p[c] = v[i];
+      }
+    }
+  }
+};
+
+// ---- layer norm -------------------------------------------------------------
+
+// One group of TPR threads per row, the row in registers: the mean first,
+// then the squared distances from it (no difference of large sums).
+template <int TPR, int NV, bool VEC, int kThreads>
+__global__ void __launch_bounds__(kThreads) layer_norm_kernel(const float* __restrict__ x,
+                                                              const float* __restrict__ gain,
+                                                              const float* __restrict__ bias, float* __restrict__ y,
+                                                              float* __restrict__ stats, int64_t rows, int width,
+                                                              float eps) {
+  using Part = RowPart<TPR, NV, VEC>;
+  constexpr int G = kThreads / TPR;
+  __shared__ float2 red[G][2 * (TPR > 32 ? TPR / 32 : 1)];
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  for (int64_t r = (int64_t)blockIdx.x * G + group; r < rows; r += (int64_t)gridDim.x * G) {
+    float v[Part::E];
+    Part::load(x + r * width, width, t, v, 0.0f);
+    float s = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int e = 0; e < Part::E; ++e) s += v[e];
+    group_sum2<TPR>(s, none, red[group], group, 0);
+    const float mean = s / (float)width;
+    float q = 0.0f;
+#pragma unroll
+    for (int e = 0; e < Part::E; ++e) {
+      const float d = v[e] - mean;
+      q += Part::col(t, e) < width ? d * d : 0.0f;
+    }
+    group_sum2<TPR>(q, none, red[group], group, 1);
+    const float rstd = 1.0f / sqrtf(q / (float)width + eps);
+    float w[Part::E];
+    if (gain != nullptr) {
+      Part::load(gain, width, t, w, 0.0f);
+#pragma unroll
+      for (int e = 0; e < Part::E; ++e) v[e] = (v[e] - mean) * rstd * w[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < Part::E; ++e) v[e] = (v[e] - mean) * rstd;
+    }
+    if (bias != nullptr) {
+      Part::load(bias, width, t, w, 0.0f);
+#pragma unroll
+      for (int e = 0; e < Part::E; ++e) v[e] += w[e];
+    }
+    Part::store(y + r * width, width, t, v);
+    if (stats != nullptr && t == 0) *(float2*)(stats + 2 * r) = make_float2(mean, rstd);
+  }
+}
+
+// Rows wider than a block's registers hold: three passes over the row, the
+// later ones from L2.
+__global__ void __launch_bounds__(1024) layer_norm_wide_kernel(const float* __restrict__ x,
+                                                               const float* __restrict__ gain,
+                                                               const float* __restrict__ bias, float* __restrict__ y,
+                                                               float* __restrict__ stats, int64_t rows,
+                                                               int64_t width, float eps) {
+  __shared__ float2 red[64];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float* xr = x + r * width;
+    float s = 0.0f, none = 0.0f;
+    for (int64_t c = threadIdx.x; c < width; c += 1024) s += xr[c];
+    group_sum2<1024>(s, none, red, 0, 0);
+    const float mean = s / (float)width;
+    float q = 0.0f;
+    for (int64_t c = threadIdx.x; c < width; c += 1024) {
+      const float d = xr[c] - mean;
+      q += d * d;
+    }
+    group_sum2<1024>(q, none, red, 0, 1);
+    const float rstd = 1.0f / sqrtf(q / (float)width + eps);
+    for (int64_t c = threadIdx.x; c < width; c += 1024) {
+      const float n = (xr[c] - mean) * rstd * (gain ? gain[c] : 1.0f);
+      y[r * width + c] = bias ? n + bias[c] : n;
+    }
+    if (stats != nullptr && threadIdx.x == 0) *(float2*)(stats + 2 * r) = make_float2(mean, rstd);
+  }
+}
+
+// dx of one row per group and step; each thread owns its columns' share of
+// dgain and dbias in registers over all rows of the block.  The block's groups
+// add theirs in order in shared memory, and `partial` gets one line per block
+// (summed in a fixed order by column_sum_kernel).
+template <int TPR, int NV, bool VEC>
+__global__ void __launch_bounds__(512) layer_norm_backward_kernel(
+    const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ stats,
+    const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width,
+    int accumulate) {
+  using Part = RowPart<TPR, NV, VEC>;
+  constexpr int G = 512 / TPR;
+  __shared__ float2 red[G][2 * (TPR > 32 ? TPR / 32 : 1)];
+  extern __shared__ float sums[];  // [2][width]
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  float w[Part::E], dg[Part::E], db[Part::E];
+  if (gain != nullptr) Part::load(gain, width, t, w, 0.0f);
+#pragma unroll
+  for (int e = 0; e < Part::E; ++e) {
+    if (gain == nullptr) w[e] = 1.0f;
+    dg[e] = 0.0f;
+    db[e] = 0.0f;
+  }
+  const float inv = 1.0f / (float)width;
+  int phase = 0;
+  for (int64_t r = (int64_t)blockIdx.x * G + group; r < rows; r += (int64_t)gridDim.x * G) {
+    float n[Part::E], g[Part::E];
+    Part::load(x + r * width, width, t, n, 0.0f);
+    Part::load(dy + r * width, width, t, g, 0.0f);
+    const float2 st = *(const float2*)(stats + 2 * r);
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int e = 0; e < Part::E; ++e) {
+      n[e] = (n[e] - st.x) * st.y;
+      // Columns past the row hold g = 0 and add nothing anywhere.
+      dg[e] += g[e] * n[e];
+      db[e] += g[e];
+      g[e] *= w[e];
+      a += g[e];
+      b += g[e] * n[e];
+    }
+    group_sum2<TPR>(a, b, red[group], group, phase);
+    phase ^= 1;
+    a *= inv;
+    b *= inv;
+#pragma unroll
+    for (int e = 0; e < Part::E; ++e) g[e] = (g[e] - a - n[e] * b) * st.y;
+    if (accumulate) {
+      Part::load(dx + r * width, width, t, n, 0.0f);
+#pragma unroll
+      for (int e = 0; e < Part::E; ++e) g[e] = n[e] + g[e];
+    }
+    Part::store(dx + r * width, width, t, g);
+  }
+  if (partial == nullptr) return;
+  for (int k = 0; k < G; ++k) {
+    if (k == group)
+#pragma unroll
+      for (int e = 0; e < Part::E; ++e) {
+        const int c = Part::col(t, e);
+        if (c < width) {
+          sums[c] = k == 0 ? dg[e] : sums[c] + dg[e];
+          sums[width + c] = k == 0 ? db[e] : sums[width + c] + db[e];
+        }
+      }
+    __syncthreads();
+  }
+  for (int c = threadIdx.x; c < 2 * width; c += 512) partial[(int64_t)blockIdx.x * 2 * width + c] = sums[c];
+}
+
+// Wide rows: dx alone, two passes over the row.
+__global__ void __launch_bounds__(1024) layer_norm_backward_wide_kernel(
+    const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ stats,
+    const float* __restrict__ dy, float* __restrict__ dx, int64_t rows, int64_t width, int accumulate) {
+  __shared__ float2 red[64];
+  int phase = 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float* xr = x + r * width;
+    const float* yr = dy + r * width;
+    const float2 st = *(const float2*)(stats + 2 * r);
+    float a = 0.0f, b = 0.0f;
+    for (int64_t c = threadIdx.x; c < width; c += 1024) {
+      const float g = yr[c] * (gain ? gain[c] : 1.0f);
+      a += g;
+      b += g * ((xr[c] - st.x) * st.y);
+    }
+    group_sum2<1024>(a, b, red, 0, phase);
+    phase ^= 1;
+    a /= (float)width;
+    b /= (float)width;
+    for (int64_t c = threadIdx.x; c < width; c += 1024) {
+      const float g = yr[c] * (gain ? gain[c] : 1.0f);
+      const float d = (g - a - (xr[c] - st.x) * st.y * b) * st.y;
+      float* o = dx + r * width + c;
+      *o = accumulate ? *o + d : d;
+    }
+  }
+}
+
+// Wide rows: the partial column sums of dy * n and dy over one block's rows.
+__global__ void __launch_bounds__(256) layer_norm_columns_kernel(const float* __restrict__ x,
+                                                                 const float* __restrict__ stats,
+                                                                 const float* __restrict__ dy,
+                                                                 float* __restrict__ partial, int64_t rows,
+                                                                 int64_t width) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= width) return;
+  float dg = 0.0f, db = 0.0f;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float g = dy[r * width + c];
+    dg += g * ((x[r * width + c] - stats[2 * r]) * stats[2 * r + 1]);
+    db += g;
+  }
+  partial[(int64_t)blockIdx.y * 2 * width + c] = dg;
+  partial[(int64_t)blockIdx.y * 2 * width + width + c] = db;
+}
+
+// dgain / dbias (+)= the sum of `lines` partial lines of 2 * width floats: 32
+// columns per block, 16 threads a column, their parts added in order.
+__global__ void __launch_bounds__(512) column_sum_kernel(const float* __restrict__ partial, float* __restrict__ dgain,
+                                                         float* __restrict__ dbias, int lines, int64_t width,
+                                                         int accumulate) {
+  __shared__ float part[16][33];
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < 2 * width)
+#pragma unroll 4
+    for (int l = slice; l < lines; l += 16) s += partial[(int64_t)l * 2 * width + c];
+  part[slice][lane] = s;
+  __syncthreads();
+  if (slice != 0 || c >= 2 * width) return;
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += part[i][lane];
+  float* out = c < width ? dgain : dbias;
+  if (out == nullptr) return;
+  out += c < width ? c : c - width;
+  *out = accumulate ? *out + s : s;
+}
+
+// ---- rotary positions ---------------------------------------------------------
+
+struct RopeArgs {
+  RopeAxes s;
+  int head_chunk;  // heads a thread turns
+  int back, accumulate;
+};
+
+// Each thread turns V neighbouring pairs of one token in `head_chunk` heads
+// with one evaluation of their angles: positions times rates in 64 bits,
+// reduced to a fraction of a revolution, so that far positions lose nothing.
+template <int V>
+__global__ void __launch_bounds__(256) rope_axes_kernel(const float* __restrict__ x,
+                                                        const float* __restrict__ positions,
+                                                        const double* __restrict__ rates, float* __restrict__ out,
+                                                        RopeArgs a) {
+  const RopeAxes& s = a.s;
+  const int per = s.half / V;
+  const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t tokens = (int64_t)s.batch * s.seq;
+  if (item >= tokens * per) return;
+  const int64_t token = item / per;
+  const int i0 = (int)(item - token * per) * V;
+  const int64_t b = token / s.seq, at = token - b * s.seq;
+  float cs[V], sn[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    int axis = 0;
+#pragma unroll
+    for (int e = 0; e < kMaxRopeAxes - 1; ++e) axis += i0 + v >= s.ends[e];
+    const double turns = (double)positions[(b * s.axes + axis) * s.seq + at] * rates[i0 + v];
+    sincospif(2.0f * (float)(turns - rint(turns)), &sn[v], &cs[v]);
+    if (a.back) sn[v] = -sn[v];
+  }
+  const int64_t step = s.seq_major ? 2 * (int64_t)s.half : 2 * (int64_t)s.half * s.seq;
+  const int64_t base =
+      (s.seq_major ? (b * s.seq + at) * s.heads : b * s.heads * s.seq + at) * 2 * (int64_t)s.half + i0;
+  const int h0 = blockIdx.y * a.head_chunk;
+  const int h1 = min(s.heads, h0 + a.head_chunk);
+#pragma unroll 4
+  for (int h = h0; h < h1; ++h) {
+    const int64_t o = base + h * step;
+    float lo[V], hi[V];
+    if (V == 4) {
+      const float4 l = *(const float4*)(x + o), u = *(const float4*)(x + o + s.half);
+      lo[0] = l.x, lo[1 % V] = l.y, lo[2 % V] = l.z, lo[3 % V] = l.w;
+      hi[0] = u.x, hi[1 % V] = u.y, hi[2 % V] = u.z, hi[3 % V] = u.w;
+    } else {
+      lo[0] = x[o];
+      hi[0] = x[o + s.half];
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float p = lo[v] * cs[v] - hi[v] * sn[v];
+      hi[v] = lo[v] * sn[v] + hi[v] * cs[v];
+      lo[v] = p;
+    }
+    if (a.accumulate) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        lo[v] = out[o + v] + lo[v];
+        hi[v] = out[o + s.half + v] + hi[v];
+      }
+    }
+    if (V == 4) {
+      *(float4*)(out + o) = make_float4(lo[0], lo[1 % V], lo[2 % V], lo[3 % V]);
+      *(float4*)(out + o + s.half) = make_float4(hi[0], hi[1 % V], hi[2 % V], hi[3 % V]);
+    } else {
+      out[o] = lo[0];
+      out[o + s.half] = hi[0];
+    }
+  }
+}
+
+// ---- distillation -------------------------------------------------------------
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// The index an id stands for: -1 for an absent entry.
+__device__ __forceinline__ int entry_id(float id, int64_t width, int* err) {
+  if (id < 0.0f) return -1;
+  if (!(id < (float)width) || (int64_t)id >= width) {  // NaN too
+    atomicCAS(err, 0, (int)kErrIndexRange);
+    return -1;
+  }
+  return (int)id;
+}
+
+// The teacher's probabilities of one row into p[0..top), its ids into ids[],
+// by one warp; returns whether the row has an entry of any weight.  Entries
+// that are absent get p = 0.  `log_mass` is ln(sum of exp((t - best) / T)).
+__device__ __forceinline__ bool teacher_row(const float* __restrict__ idr, const float* __restrict__ tr, int top,
+                                            int64_t width, float inv_t, int* ids, float* p, float* best_out,
+                                            double* log_mass, int* err) {
+  const int lane = threadIdx.x & 31;
+  float best = -INFINITY;
+  bool bad = false;
+  for (int e = lane; e < top; e += 32) {
+    const int id = entry_id(idr[e], width, err);
+    ids[e] = id;
+    const float w = id < 0 ? -INFINITY : tr[e];
+    p[e] = w;
+    bad |= w != w;
+    best = fmaxf(best, w);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (__any_sync(0xffffffffu, bad)) best = NAN;
+  float mass = 0.0f;
+  for (int e = lane; e < top; e += 32) {
+    const float w = best == -INFINITY || p[e] == -INFINITY ? 0.0f : exp2f((p[e] - best) * inv_t * kLog2e);
+    p[e] = w;
+    mass += w;
+  }
+  mass = warp_sum(mass);
+  const float scale = mass > 0.0f ? 1.0f / mass : 0.0f;
+  for (int e = lane; e < top; e += 32) p[e] = mass == mass ? p[e] * scale : NAN;
+  __syncwarp();
+  *best_out = best;
+  *log_mass = log((double)mass);
+  return best != -INFINITY;
+}
+
+struct Online {
+  float m, s;  // greatest value, sum of exp2((v - m) * c)
+};
+
+__device__ __forceinline__ Online join(Online a, Online b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  if (m == -INFINITY) return {m, a.s + b.s};
+  return {m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
+}
+
+__device__ __forceinline__ void take(Online& o, float v, float c) {
+  if (v > o.m) {
+    o.s = o.s * exp2f((o.m - v) * c) + 1.0f;
+    o.m = v;
+  } else {
+    o.s += v == o.m && v == -INFINITY ? 0.0f : exp2f((v - o.m) * c);
+  }
+}
+
+// Greatest logit and sum of one row in one pass, the row split over a cluster
+// of gridDim.y blocks (one for many rows) whose parts the first block joins in
+// order through distributed shared memory; then the loss of the row's entries.
+constexpr int kDistillThreads = 512;
+__global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
+    const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
+    float* __restrict__ loss, float* __restrict__ stats, int64_t rows, int64_t width, int top, float temperature,
+    int* err) {
+  __shared__ Online warp_part[kDistillThreads / 32];
+  __shared__ Online part[8];  // block 0's: one entry per block of the cluster
+  extern __shared__ float entry[];  // [2][top]: ids, probabilities
+  const int64_t r = blockIdx.x;
+  const int parts = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
+  // Arrives for "this block runs": the first block's shared memory is written
+  // only once every block of the cluster has got here.
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const float inv_t = 1.0f / temperature, c = inv_t * kLog2e;
+  const float* row = logits + r * width;
+  // Chunks of whole float4 from the row's first 16-byte boundary; the values
+  // before it and after the last whole float4 go to the first block.
+  const int64_t head = min(width, (int64_t)((4 - (((uintptr_t)row >> 2) & 3)) & 3));
+  const int64_t quads = (width - head) / 4;
+  const int64_t per = (quads + parts - 1) / parts;
+  const int64_t q0 = min(quads, rank * per), q1 = min(quads, q0 + per);
+  const float4* body = (const float4*)(row + head);
+  Online o{-INFINITY, 0.0f};
+  bool bad = false;
+  int64_t i = q0 + tid;
+  for (; i + 3 * kDistillThreads < q1; i += 4 * kDistillThreads) {
+    float4 f[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f[u] = body[i + u * kDistillThreads];
+    float m = o.m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) m = fmaxf(m, fmaxf(fmaxf(f[u].x, f[u].y), fmaxf(f[u].z, f[u].w)));
+    if (m == -INFINITY) {  // nothing but -inf so far, or NaN, which fmaxf drops
+#pragma unroll
+      for (int u = 0; u < 4; ++u) bad |= f[u].x != f[u].x || f[u].y != f[u].y || f[u].z != f[u].z || f[u].w != f[u].w;
+      continue;
+    }
+    float s = o.s * exp2f((o.m - m) * c);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      s += (exp2f((f[u].x - m) * c) + exp2f((f[u].y - m) * c)) + (exp2f((f[u].z - m) * c) + exp2f((f[u].w - m) * c));
+    o.m = m;
+    o.s = s;
+  }
+  for (; i < q1; i += kDistillThreads) {
+    const float4 f = body[i];
+    take(o, f.x, c), take(o, f.y, c), take(o, f.z, c), take(o, f.w, c);
+    bad |= f.x != f.x || f.y != f.y || f.z != f.z || f.w != f.w;
+  }
+  if (rank == 0) {
+    const int64_t tail = head + 4 * quads;
+    if (tid < head) take(o, row[tid], c), bad |= row[tid] != row[tid];
+    if (tid < width - tail) take(o, row[tail + tid], c), bad |= row[tail + tid] != row[tail + tid];
+  }
+  if (bad) o.s = NAN;
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    const Online p{__shfl_xor_sync(0xffffffffu, o.m, k), __shfl_xor_sync(0xffffffffu, o.s, k)};
+    o = join(o, p, c);
+  }
+  if ((tid & 31) == 0) warp_part[tid >> 5] = o;
+  __syncthreads();
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid == 0) {
+    for (int w = 1; w < kDistillThreads / 32; ++w) o = join(o, warp_part[w], c);
+    uint32_t dst;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&part[rank]);
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"(mine));
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(dst), "f"(o.m), "f"(o.s) : "memory");
+  }
+  if (parts > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  if (tid >= 32) return;
+  Online all = part[0];
+  for (int w = 1; w < parts; ++w) all = join(all, part[w], c);
+  if (stats != nullptr && tid == 0) *(float2*)(stats + 2 * r) = make_float2(all.m, all.s);
+  int* eid = (int*)entry;
+  float* p = entry + top;
+  float best;
+  double log_mass;
+  const bool any =
+      teacher_row(ids + r * top, teacher + r * top, top, width, inv_t, eid, p, &best, &log_mass, err);
+  // ln p - ln q per entry in 64 bits: the two logarithms nearly cancel where
+  // the student follows the teacher.
+  const double log_sum = log((double)all.s);
+  float sum = 0.0f;
+  if (any)
+    for (int e = tid; e < top; e += 32) {
+      if (p[e] == 0.0f) continue;
+      const double t = ((double)teacher[r * top + e] - (double)best) / temperature - log_mass;
+      const double z = ((double)row[eid[e]] - (double)all.m) / temperature - log_sum;
+      sum += (float)((double)p[e] * (t - z));
+    }
+  sum = warp_sum(sum);
+  if (tid == 0) loss[r] = temperature * temperature * sum;
+}
+
+// One block per row and chunk of columns: T * dloss * q in one pass from the
+// row's statistics, then the few entries' own terms.
+template <bool VEC>
+__global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
+    const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
+    const float* __restrict__ stats, const float* __restrict__ dloss, float* __restrict__ grad, int64_t rows,
+    int64_t width, int64_t chunk, int top, float temperature, int accumulate, int* err) {
+  extern __shared__ float entry[];  // [2][top]
+  __shared__ int any_entry;
+  const int64_t r = blockIdx.x;
+  const int64_t c0 = blockIdx.y * chunk, c1 = min(width, c0 + chunk);
+  const int tid = threadIdx.x;
+  int* eid = (int*)entry;
+  float* p = entry + top;
+  if (tid < 32) {
+    float best;
+    double log_mass;
+    const bool any = teacher_row(ids + r * top, teacher + r * top, top, width, 1.0f / temperature, eid, p, &best,
+                                 &log_mass, err);
+    if (tid == 0) any_entry = any;
+  }
+  __syncthreads();
+  const float* row = logits + r * width;
+  float* out = grad + r * width;
+  const float2 st = *(const float2*)(stats + 2 * r);
+  const float c = kLog2e / temperature;
+  const float up = temperature * (dloss ? dloss[r] : 1.0f);
+  const float coef = up / st.y;
+  const bool any = any_entry;
+  if (!any) {  // whatever the row holds
+    if (!accumulate)
+      for (int64_t i = c0 + tid; i < c1; i += kDistillThreads) out[i] = 0.0f;
+    return;
+  }
+  const int64_t head = VEC ? min(c1 - c0, (int64_t)((4 - (((uintptr_t)(row + c0) >> 2) & 3)) & 3)) : 0;
+  const int64_t quads = VEC ? (c1 - c0 - head) / 4 : 0;
+  const float4* src = (const float4*)(row + c0 + head);
+  float4* dst = (float4*)(out + c0 + head);
+  int64_t i = tid;
+  for (; i + 3 * kDistillThreads < quads; i += 4 * kDistillThreads) {
+    float4 f[4], old[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f[u] = src[i + u * kDistillThreads];
+    if (accumulate)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) old[u] = dst[i + u * kDistillThreads];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float4 g = make_float4(coef * exp2f((f[u].x - st.x) * c), coef * exp2f((f[u].y - st.x) * c),
+                             coef * exp2f((f[u].z - st.x) * c), coef * exp2f((f[u].w - st.x) * c));
+      if (accumulate) g.x += old[u].x, g.y += old[u].y, g.z += old[u].z, g.w += old[u].w;
+      dst[i + u * kDistillThreads] = g;
+    }
+  }
+  auto one = [&](int64_t at) {
+    const float g = coef * exp2f((row[at] - st.x) * c);
+    out[at] = accumulate ? out[at] + g : g;
+  };
+  for (; i < quads; i += kDistillThreads) {
+    const int64_t at = c0 + head + 4 * i;
+    one(at), one(at + 1), one(at + 2), one(at + 3);
+  }
+  if (VEC && tid < head) one(c0 + tid);
+  for (int64_t at = c0 + head + 4 * quads + tid; at < c1; at += kDistillThreads) one(at);
+  __syncthreads();
+  for (int e = tid; e < top; e += kDistillThreads) {
+    const int id = eid[e];
+    if (id < c0 || id >= c1) continue;
+    // An id given twice: its first entry takes all of its probability, in order.
+    float mass = 0.0f;
+    bool first = true;
+    for (int f = 0; f < top; ++f) {
+      if (eid[f] != id) continue;
+      if (f < e) {
+        first = false;
+        break;
+      }
+      mass += p[f];
+    }
+    if (first) out[id] -= up * mass;
+  }
+}
+
+}  // namespace
+
+// ---- launchers ------------------------------------------------------------------
+
+namespace {
+
+template <int TPR, int NV, bool VEC>
+void layer_norm_run(const float* x, const float* gain, const float* bias, float* y, float* stats, int64_t rows,
+                    int width, float eps, cudaStream_t st) {
+  constexpr int kThreads = TPR > 256 ? TPR : 256;
+  const int64_t want = ceil_div(rows, kThreads / TPR);
+  const int blocks = (int)(want < 148 * 64 ? want : 148 * 64);
+  layer_norm_kernel<TPR, NV, VEC, kThreads><<<blocks, kThreads, 0, st>>>(x, gain, bias, y, stats, rows, width, eps);
+  check_launch();
+}
+
+// A row takes the fewest threads that hold it 16 values each: below that a
+// block has too few loads in flight, above it the sums' barriers cost more.
+template <bool VEC>
+void layer_norm_pick(const float* x, const float* gain, const float* bias, float* y, float* stats, int64_t rows,
+                     int64_t width, float eps, cudaStream_t st) {
+  const int w = (int)width;
+  if (width <= 128) layer_norm_run<32, 1, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else if (width <= 512) layer_norm_run<32, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else if (width <= 1024) layer_norm_run<64, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else if (width <= 2048) layer_norm_run<128, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else if (width <= 4096) layer_norm_run<256, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else if (width <= 8192) layer_norm_run<512, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+  else layer_norm_run<1024, 4, VEC>(x, gain, bias, y, stats, rows, w, eps, st);
+}
+
+constexpr int64_t kLayerNormMost = 16384;         // widest row in registers, forward
+constexpr int64_t kLayerNormBackwardMost = 8192;  // backward
+
+int layer_norm_lines(int64_t rows, int64_t width) {
+  if (width > kLayerNormBackwardMost) return (int)(rows < 64 ? rows : 64);
+  int tpr = 32;
+  while (tpr * 16 < width) tpr *= 2;
+  const int64_t want = ceil_div(rows, 512 / tpr);
+  return (int)(want < 148 * 2 ? want : 148 * 2);
+}
+
+template <int TPR, bool VEC>
+void layer_norm_backward_run(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
+                             float* partial, int64_t rows, int width, int accumulate, cudaStream_t st) {
+  const size_t smem = partial ? sizeof(float) * 2 * (size_t)width : 0;
+  if (smem > 48 * 1024)
+    TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_backward_kernel<TPR, 4, VEC>,
+                                    cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+  layer_norm_backward_kernel<TPR, 4, VEC><<<layer_norm_lines(rows, width), 512, smem, st>>>(
+      x, gain, stats, dy, dx, partial, rows, width, accumulate);
+  check_launch();
+}
+
+template <bool VEC>
+void layer_norm_backward_pick(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
+                              float* partial, int64_t rows, int64_t width, int accumulate, cudaStream_t st) {
+  const int w = (int)width;
+  if (width <= 512) layer_norm_backward_run<32, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 1024) layer_norm_backward_run<64, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 2048) layer_norm_backward_run<128, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 4096) layer_norm_backward_run<256, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else layer_norm_backward_run<512, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+}
+
+}  // namespace
+
+void launch_layer_norm(const float* x, const float* gain, const float* bias, float* y, float* stats, int64_t rows,
+                       int64_t width, float eps, cudaStream_t st) {
+  if (rows <= 0 || width <= 0) return;
+  if (width > kLayerNormMost) {
+    layer_norm_wide_kernel<<<(int)(rows < 148 * 2 ? rows : 148 * 2), 1024, 0, st>>>(x, gain, bias, y, stats, rows,
+                                                                                    width, eps);
+    check_launch();
+    return;
+  }
+  const bool vec = width % 4 == 0 && aligned16(x) && aligned16(y) && aligned16(gain) && aligned16(bias);
+  if (vec) layer_norm_pick<true>(x, gain, bias, y, stats, rows, width, eps, st);
+  else layer_norm_pick<false>(x, gain, bias, y, stats, rows, width, eps, st);
+}
+
+int64_t layer_norm_partial_elems(int64_t rows, int64_t width) {
+  if (rows <= 0 || width <= 0) return 1;
+  return (int64_t)layer_norm_lines(rows, width) * 2 * width;
+}
+
+void launch_layer_norm_backward(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
+                                float* dgain, float* dbias, float* partial, int64_t rows, int64_t width,
+                                int accumulate_dx, int accumulate_params, cudaStream_t st) {
+  if (width <= 0) return;
+  const bool columns = dgain != nullptr || dbias != nullptr;
+  int lines = 0;
+  if (rows > 0) {
+    lines = layer_norm_lines(rows, width);
+    float* part = columns ? partial : nullptr;
+    if (width > kLayerNormBackwardMost) {
+      layer_norm_backward_wide_kernel<<<(int)(rows < 148 * 2 ? rows : 148 * 2), 1024, 0, st>>>(
+          x, gain, stats, dy, dx, rows, width, accumulate_dx);
+      check_launch();
+      if (columns) {
+        const dim3 grid((unsigned)ceil_div(width, 256), (unsigned)lines);
+        layer_norm_columns_kernel<<<grid, 256, 0, st>>>(x, stats, dy, part, rows, width);
+        check_launch();
+      }
+    } else {
+      const bool vec = width % 4 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gain);
+      if (vec) layer_norm_backward_pick<true>(x, gain, stats, dy, dx, part, rows, width, accumulate_dx, st);
+      else layer_norm_backward_pick<false>(x, gain, stats, dy, dx, part, rows, width, accumulate_dx, st);
+    }
+  }
+  if (!columns) return;
+  column_sum_kernel<<<(unsigned)ceil_div(2 * width, 32), 512, 0, st>>>(partial, dgain, dbias, lines, width,
+                                                                       accumulate_params);
+  check_launch();
+}
+
+void launch_rope_axes(const float* x, const float* positions, const double* rates, float* out, const RopeAxes& shape,
+                      int back, int accumulate, cudaStream_t st) {
+  const int64_t tokens = (int64_t)shape.batch * shape.seq;
+  if (tokens <= 0 || shape.heads <= 0 || shape.half <= 0) return;
+  const bool vec = shape.half % 4 == 0 && aligned16(x) && aligned16(out);
+  const int64_t items = tokens * (shape.half / (vec ? 4 : 1));
+  // All heads of a token in one thread share its angles; where that leaves
+  // fewer than two blocks per SM, the heads are spread over more threads.
+  int64_t chunk = shape.heads * items / (148 * 2 * 256);
+  chunk = chunk < 1 ? 1 : chunk > shape.heads ? shape.heads : chunk;
+  RopeArgs a{shape, (int)chunk, back, accumulate};
+  for (int e = shape.axes - 1; e < kMaxRopeAxes; ++e) a.s.ends[e] = INT_MAX;  // the last axis takes the rest
+  const dim3 grid((unsigned)ceil_div(items, 256), (unsigned)ceil_div(shape.heads, chunk));
+  if (vec) rope_axes_kernel<4><<<grid, 256, 0, st>>>(x, positions, rates, out, a);
+  else rope_axes_kernel<1><<<grid, 256, 0, st>>>(x, positions, rates, out, a);
+  check_launch();
+}
+
+void launch_distill_loss(const float* logits, const float* ids, const float* teacher, float* loss, float* stats,
+                         int64_t rows, int64_t width, int top, float temperature, int* err, cudaStream_t st) {
+  if (rows <= 0) return;
+  // A row is split over up to eight blocks where whole rows leave SMs idle
+  // and a part still gives each thread a few loads.
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 148 * 4 && width / (parts * 2) >= 4 * kDistillThreads) parts *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows, (unsigned)parts);
+  cfg.blockDim = dim3(kDistillThreads);
+  cfg.dynamicSmemBytes = sizeof(float) * 2 * (size_t)top;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {1, (unsigned)parts, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TYSOR_CUDA(cudaLaunchKernelEx(&cfg, distill_loss_kernel, logits, ids, teacher, loss, stats, rows, width, top,
+                                temperature, err));
+  check_launch();
+}
+
+void launch_distill_loss_backward(const float* logits, const float* ids, const float* teacher, const float* stats,
+                                  const float* dloss, float* grad, int64_t rows, int64_t width, int top,
+                                  float temperature, int accumulate, int* err, cudaStream_t st) {
+  if (rows <= 0) return;
+  int64_t parts = 1;
+  while (rows * parts < 148 * 4 && width / (parts * 2) >= 4 * kDistillThreads && parts < 1024) parts *= 2;
+  const int64_t chunk = ceil_div(ceil_div(width, parts), 4) * 4;
+  const dim3 grid((unsigned)rows, (unsigned)ceil_div(width, chunk));
+  const size_t smem = sizeof(float) * 2 * (size_t)top;
+  // Rows of both tensors then start at the same offset from a 16-byte boundary.
+  const bool vec = (((uintptr_t)logits ^ (uintptr_t)grad) & 15) == 0;
+  if (vec)
+    distill_backward_kernel<true><<<grid, kDistillThreads, smem, st>>>(logits, ids, teacher, stats, dloss, grad, rows,
+                                                                       width, chunk, top, temperature, accumulate, err);
+  else
+    distill_backward_kernel<false><<<grid, kDistillThreads, smem, st>>>(
+        logits, ids, teacher, stats, dloss, grad, rows, width, chunk, top, temperature, accumulate, err);
+  check_launch();
+}
+
+}  // namespace tysor

@@ -25,11 +25,11 @@ Accepted (src/compiler/parser.rs, frontend_ir.rs, ir/builder.rs):
 Lowering follows the reference builder (ir/builder.rs:97-174): parameters
 first, then each statement's expression in post-order; a literal argument
 becomes a Constant node where it is met; a call of a builtin constructor
-(`linear`, `SiLU`, `Softmax`, `Embedding`, `Dropout`, `RMSNorm`) is a
-LibraryCtor, of a primitive (`matmul`, `relu`, `scale`) a PrimitiveCall, of a
+(`linear`, `SiLU`, `Softmax`, `Embedding`, `Dropout`, `RMSNorm`,
+`LayerNorm`) is a LibraryCtor, of a primitive (`matmul`, `relu`, `scale`) a PrimitiveCall, of a
 library function (`rms_norm`, `cross_entropy`, `reshape`, `repeat_kv`,
-`flatten_heads`, `causal_mask`, `rope`, `transpose`, `tied_logits`) a
-LibraryCall, of a local variable an Apply.  A pipeline `a -> f(x) -> g()`
+`flatten_heads`, `causal_mask`, `rope`, `transpose`, `rope_axes`,
+`window_attention`, `distill_loss`, `tied_logits`) a LibraryCall, of a local variable an Apply.  A pipeline `a -> f(x) -> g()`
 is the nested call `g()(f(x)(a))` for constructor stages (the constructor
 is created, then its input lowered, then applied) and `f(a, x)` for
 function stages.

@@ -24,12 +24,19 @@ from typing import Any, Dict, List, Optional, Sequence, Union
 # Primitive tensor ops (src/ops/library.rs:49-93: matmul, relu, scale).
 PRIMITIVE_OPS = ("matmul", "relu", "scale")
 # Library calls the reference runtime executes (graph_executor.rs:114-161),
-# plus `transpose`, an extension with no reference counterpart.
+# plus extensions with no reference counterpart: `transpose`, and the
+# language-model operators
+#   rope_axes(x, positions, theta, section, ... [, seq_major])
+#   window_attention(q, k, v, window, sinks [, lengths [, starts]] [, seq_major])
+#   distill_loss(logits, ids, teacher, temperature)
+# x, q, k and v are [batch, heads, length, head_dim], or with a trailing
+# `True` [batch, length, heads, head_dim].
 LIBRARY_CALLS = ("rms_norm", "cross_entropy", "reshape", "repeat_kv", "flatten_heads",
-                 "causal_mask", "rope", "transpose")
-# Layer constructors (graph_executor.rs:163-223), plus `RMSNorm`, an
-# extension: rms_norm with a learned gain and a configurable eps.
-LIBRARY_CTORS = ("linear", "SiLU", "Softmax", "Embedding", "Dropout", "RMSNorm")
+                 "causal_mask", "rope", "transpose", "rope_axes", "window_attention", "distill_loss")
+# Layer constructors (graph_executor.rs:163-223), plus two extensions:
+# `RMSNorm`, rms_norm with a learned gain and a configurable eps, and
+# `LayerNorm(width [, eps [, bias]])` with a learned gain and bias.
+LIBRARY_CTORS = ("linear", "SiLU", "Softmax", "Embedding", "Dropout", "RMSNorm", "LayerNorm")
 
 NODE_KINDS = ("const", "binary", "primitive", "call", "ctor", "apply")
 VALUE_KINDS = ("tensor", "int", "float", "bool", "callable")

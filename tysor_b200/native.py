@@ -39,6 +39,7 @@ SIGNATURES = {
     "tysor_cuda_buffer_read": (c_bool, [V, FP, c_size_t]),
     "tysor_cuda_buffer_write": (c_bool, [V, FP, c_size_t]),
     "tysor_cuda_buffer_view": (V, [V, c_size_t, c_size_t]),
+    "tysor_cuda_buffer_wrap": (V, [V, V, c_size_t]),
     "tysor_cuda_buffer_count": (c_size_t, [V]),
     "tysor_cuda_dispatch_matmul": (c_bool, [V, V, V, V, U32, U32, U32]),
     "tysor_cuda_dispatch_unary": (c_bool, [V, c_int, V, V, U32, c_float]),
@@ -72,6 +73,15 @@ SIGNATURES = {
     "tysor_cuda_dispatch_cross_entropy_labels": (c_bool, [V, V, V, V, U32, U32]),
     "tysor_cuda_dispatch_cross_entropy_labels_backward": (c_bool, [V, V, V, V, U32, U32, c_bool]),
     "tysor_cuda_dispatch_transpose": (c_bool, [V, V, V, I64P, c_int, c_int, c_int]),
+    "tysor_cuda_dispatch_layer_norm": (c_bool, [V, V, V, V, V, V, U32, U32, c_float]),
+    "tysor_cuda_dispatch_layer_norm_backward": (c_bool, [V, V, V, V, V, V, V, V, U32, U32, c_bool]),
+    "tysor_cuda_dispatch_rope_axes": (c_bool, [V, V, V, V, U32, U32, U32, I64P, c_int, c_double, c_bool]),
+    "tysor_cuda_dispatch_rope_axes_backward": (c_bool, [V, V, V, V, U32, U32, U32, I64P, c_int, c_double, c_bool,
+                                                        c_bool]),
+    "tysor_cuda_dispatch_window_attention": (c_bool, [V] * 8 + [U32] * 8 + [c_float, c_bool]),
+    "tysor_cuda_dispatch_window_attention_backward": (c_bool, [V] * 12 + [U32] * 8 + [c_float, c_bool, c_bool]),
+    "tysor_cuda_dispatch_distill_loss": (c_bool, [V, V, V, V, V, V, U32, U32, U32, c_float]),
+    "tysor_cuda_dispatch_distill_loss_backward": (c_bool, [V, V, V, V, V, V, V, U32, U32, U32, c_float, c_bool]),
     "tysor_cuda_graph_new": (V, [V, c_char_p]),
     "tysor_cuda_graph_free": (None, [V]),
     "tysor_cuda_graph_set_shape": (c_bool, [V, c_char_p, I64P, c_int]),

@@ -431,11 +431,69 @@ def llama_block_flops(batch: int, seq: int, d_model: int, n_heads: int, n_kv_hea
     return 3.0 * (proj + attn)
 
 
+def student_lm(layers: int = 2, batch: int = 2, seq: int = 256, d_model: int = 256, n_heads: int = 4,
+               n_kv_heads: int = 2, hidden: int = 512, vocab: int = 1000, window: int = 64, sinks: int = 4,
+               sections=(8, 12, 12), theta: float = 10000.0, eps: float = 1e-5, temperature: float = 2.0,
+               lr: float = 1e-3, iterations: int = 1) -> Graph:
+    """Language model with attention over a sliding window, trained from a
+    teacher's best logits:
+
+        x      = Embedding(vocab, d_model)(ids)            ids: [batch*seq]
+        h      = x + o_proj(window_attention(q, k, v))     of LayerNorm(x)
+        x      = h + down(SiLU(gate(.)) * up(.))           of LayerNorm(h)
+        logits = tied_logits(LayerNorm(x), embedding)
+        loss   = distill_loss(logits, teacher_ids, teacher_logits)
+
+    q and k are turned by rope_axes with `positions` [batch, axes, seq];
+    `lengths` [batch] holds each sequence's tokens (the rest is padding) and
+    teacher_ids / teacher_logits [batch*seq, top] the teacher's entries, an id
+    below 0 being absent (so a padded position has loss and gradient 0)."""
+    b = GraphBuilder("student")
+    ids, positions, lengths = b.param("ids"), b.param("positions"), b.param("lengths")
+    teacher_ids, teacher = b.param("teacher_ids"), b.param("teacher")
+    hd = d_model // n_heads
+    if 2 * sum(sections) != hd:
+        raise ValueError(f"sections {sections} must hold the {hd // 2} pairs of a head")
+    emb = b.let("embed", b.ctor("Embedding", vocab, d_model))
+    x = b.let("x0", b.apply(emb, ids))
+    for i in range(layers):
+        P = f"l{i}_"
+        n1 = b.let(P + "attn_norm", b.ctor("LayerNorm", d_model, eps))
+        qp = b.let(P + "q_proj", b.ctor("linear", d_model, n_heads * hd, False))
+        kp = b.let(P + "k_proj", b.ctor("linear", d_model, n_kv_heads * hd, False))
+        vp = b.let(P + "v_proj", b.ctor("linear", d_model, n_kv_heads * hd, False))
+        op = b.let(P + "o_proj", b.ctor("linear", n_heads * hd, d_model, False))
+        n2 = b.let(P + "ffn_norm", b.ctor("LayerNorm", d_model, eps))
+        gp = b.let(P + "gate_proj", b.ctor("linear", d_model, hidden, False))
+        up = b.let(P + "up_proj", b.ctor("linear", d_model, hidden, False))
+        dp = b.let(P + "down_proj", b.ctor("linear", hidden, d_model, False))
+        act = b.let(P + "act", b.ctor("SiLU"))
+        hn = b.let(P + "hn", b.apply(n1, x))
+
+        def turned(proj, heads):
+            t = b.call("reshape", b.apply(proj, hn), batch, seq, heads, hd)
+            return b.call("rope_axes", t, positions, theta, *[int(s) for s in sections], True)
+
+        q, k = b.let(P + "q", turned(qp, n_heads)), b.let(P + "k", turned(kp, n_kv_heads))
+        v = b.let(P + "v", b.call("reshape", b.apply(vp, hn), batch, seq, n_kv_heads, hd))
+        ctx = b.call("window_attention", q, k, v, window, sinks, lengths, True)
+        h = b.let(P + "h", b.binary("+", x, b.apply(op, b.call("reshape", ctx, batch * seq, n_heads * hd))))
+        hn2 = b.let(P + "hn2", b.apply(n2, h))
+        ff = b.binary("*", b.apply(act, b.apply(gp, hn2)), b.apply(up, hn2))
+        x = b.let(f"x{i + 1}", b.binary("+", h, b.apply(dp, ff)))
+    norm = b.let("final_norm", b.ctor("LayerNorm", d_model, eps))
+    logits = b.let("logits", b.call("tied_logits", b.apply(norm, x), emb))
+    b.ret(b.let("loss", b.call("distill_loss", logits, teacher_ids, teacher, temperature)))
+    b.train(objective="loss", lr=lr, iterations=iterations)
+    return b.build()
+
+
 def random_parameters(graph: Graph, seed: int = 1234, std: float = 0.02) -> Dict[str, np.ndarray]:
     """Seeded initial values for every trainable parameter a graph's
     constructors create under the train executor's names
     (training/executor.rs:152-221): linear weights [in, out] and embedding
-    tables [num, dim] N(0, std), linear biases 0, RMSNorm gains N(1, std).
+    tables [num, dim] N(0, std), linear biases 0, RMSNorm and LayerNorm gains
+    N(1, std), LayerNorm biases N(0, std).
     Constructors are visited in graph order, so a seed fixes every value."""
     rng = np.random.default_rng(seed)
     consts = {n.output: n.const for n in graph.nodes if n.kind == "const"}
@@ -457,4 +515,9 @@ def random_parameters(graph: Graph, seed: int = 1234, std: float = 0.02) -> Dict
         elif n.op == "RMSNorm":
             h = int(consts[n.inputs[0]])
             params[f"rmsnorm_{n.output}_gain"] = (1.0 + std * rng.standard_normal(h)).astype(np.float32)
+        elif n.op == "LayerNorm":
+            h = int(consts[n.inputs[0]])
+            params[f"layernorm_{n.output}_gain"] = (1.0 + std * rng.standard_normal(h)).astype(np.float32)
+            if len(n.inputs) < 3 or bool(consts[n.inputs[2]]):
+                params[f"layernorm_{n.output}_bias"] = (std * rng.standard_normal(h)).astype(np.float32)
     return params

@@ -101,6 +101,34 @@ class DeviceBuffer:
         check(h, "buffer_new_zeroed")
         return cls(ctx, h, int(count))
 
+    @classmethod
+    def wrap(cls, ctx: CudaContext, array) -> "DeviceBuffer":
+        """A buffer over the memory of a contiguous float32 array on the
+        context's device (anything with __cuda_array_interface__, such as a
+        torch tensor), which the buffer keeps alive.  Dispatches run on the
+        context's stream; work on the array on another stream has to be
+        ordered with it by the caller."""
+        face = array.__cuda_array_interface__
+        if face["typestr"] != "<f4":
+            raise ValueError(f"wrap: expected float32 values, got {face['typestr']}")
+        shape = [int(d) for d in face["shape"]]
+        count = int(np.prod(shape, dtype=np.int64))
+        step, packed = 4, face.get("strides") is None or count == 0
+        if not packed:
+            packed = True
+            for d, stride in zip(reversed(shape), reversed(face["strides"])):
+                packed = packed and (d == 1 or stride == step)
+                step *= d
+        if not packed:
+            raise ValueError("wrap: the array is not contiguous")
+        if count == 0:
+            return cls.zeros(ctx, 0)
+        h = native.lib().tysor_cuda_buffer_wrap(ctx.handle, int(face["data"][0]), count)
+        check(h, "buffer_wrap")
+        out = cls(ctx, h, count)
+        out._array = array
+        return out
+
     def read(self, count: Optional[int] = None) -> np.ndarray:
         n = self.count if count is None else count
         out = np.empty(n, dtype=np.float32)
