@@ -455,8 +455,8 @@ def test_window_attention_refusals(lib):
     bad("finite scale", 1, 2, 1, 16, 16, 32, 4, 1, float("inf"), False)
     bad("q buffer holds 4096", 1, 2, 1, 65, 16, 32, 4, 1, 0.1, False)
     bad("k buffer holds 4096", 1, 2, 1, 16, 129, 32, 4, 1, 0.1, False)
-    bad("sizes overflow", 1 << 30, 1 << 20, 1, 1 << 30, 1, 32, 4, 1, 0.1, False)
-    bad("up to 2^30", (1 << 30) + 1, 2, 1, 16, 16, 32, 4, 1, 0.1, False)
+    bad("sizes overflow", 1 << 29, 1 << 20, 1, 1 << 29, 1, 32, 4, 1, 0.1, False)
+    bad("up to 2^29", (1 << 29) + 1, 2, 1, 16, 16, 32, 4, 1, 0.1, False)
     lib.refused("out overlaps q", "window_attention", q, k, v, None, None, q, None, *ok)
     lib.refused("lengths buffer holds 0", "window_attention", q, k, v, None, lib.zeros(0), out, None, *ok)
     lib.refused("null buffer", "window_attention_backward", q, k, v, None, None, out, None, q, k, v, out, *ok, False)

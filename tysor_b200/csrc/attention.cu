@@ -1,9 +1,11 @@
 // Causal attention over a sliding window and the first keys (lm_ops.cuh),
 // forward and backward.
+#include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
 
 #include "lm_ops.cuh"
+#include "tcgen05.cuh"
 
 namespace tysor {
 namespace {
@@ -42,7 +44,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionShape& s, int b, 
   }
   if (s.starts != nullptr) {
     const float v = s.starts[b];
-    if (v > -1073741824.0f && v < 1073741824.0f) {
+    if (v > -536870912.0f && v < 536870912.0f) {  // positions stay below 2^30
       q.start = (int)v;
     } else {
       q.n = 0;
@@ -58,11 +60,11 @@ struct Seen {
   int first, low, high;
 };
 
-__device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence& q, int64_t p) {
+__device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence& q, int p) {
   if (p < 0 || p >= q.n) return {0, 0, 0};
-  Seen v{0, 0, (int)p + 1};
+  Seen v{0, 0, p + 1};
   if (s.window > 0 && p + 1 > s.window) {
-    v.low = (int)(p + 1 - s.window);
+    v.low = p + 1 - s.window;
     v.first = min(s.sinks, v.low);
   }
   return v;
@@ -100,7 +102,7 @@ __device__ __forceinline__ float lane_dot(const float (&a)[kLaneDims], const flo
 __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
                                    const float* v, float* out, float* stats, int b, int h, int r) {
   const int g = h / (s.heads / s.kv_heads);
-  const Seen seen = seen_by(s, sq, (int64_t)sq.start + r);
+  const Seen seen = seen_by(s, sq, sq.start + r);
   float qv[kLaneDims], acc[kLaneDims] = {};
   lane_load(q + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, qv);
   float m = -INFINITY, l = 0.0f;
@@ -138,7 +140,7 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
                               const float* v, const float* out, const float* stats, const float* dout, float* dq,
                               int accumulate, int b, int h, int r) {
   const int g = h / (s.heads / s.kv_heads);
-  const Seen seen = seen_by(s, sq, (int64_t)sq.start + r);
+  const Seen seen = seen_by(s, sq, sq.start + r);
   const int64_t at = row_at(s, b, h, r, s.heads, s.q_len);
   float qv[kLaneDims], gv[kLaneDims], kv[kLaneDims], vv[kLaneDims], acc[kLaneDims] = {};
   lane_load(out + at, s.head_dim, kv);
@@ -172,11 +174,10 @@ __global__ void __launch_bounds__(256) simple_dq_kernel(AttentionShape s, const 
 
 // The query rows that see key j: those at positions [j, end).
 __device__ __forceinline__ void rows_seeing(const AttentionShape& s, const Sequence& sq, int j, int* r0, int* r1) {
-  int64_t end = sq.n;
-  if (s.window > 0 && j >= s.sinks && end > (int64_t)j + s.window) end = (int64_t)j + s.window;
-  const int64_t a = (int64_t)j - sq.start, z = end - sq.start;
-  *r0 = (int)(a < 0 ? 0 : a > s.q_len ? s.q_len : a);
-  *r1 = j >= sq.n ? *r0 : (int)(z < 0 ? 0 : z > s.q_len ? s.q_len : z);
+  int end = sq.n;
+  if (s.window > 0 && j >= s.sinks && end - j > s.window) end = j + s.window;
+  *r0 = min(max(j - sq.start, 0), s.q_len);
+  *r1 = j >= sq.n ? *r0 : min(max(end - sq.start, 0), s.q_len);
 }
 
 __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
@@ -224,15 +225,807 @@ __global__ void __launch_bounds__(256) simple_dkv_kernel(AttentionShape s, const
   simple_dkv_row(s, sequence_of(s, b, err), q, k, v, out, stats, dout, dk, dv, accumulate_k, accumulate_v, b, g, j);
 }
 
+// ---- operands of the tensor-core kernels ---------------------------------------------
+
+// fp32 accuracy out of fp16 matrix instructions: an operand is multiplied by a
+// power of two that brings its tile's largest magnitude into [2^14, 2^15) and
+// split into hi = fp16(x) and lo = fp16(x - hi), 22 bits together; a product
+// is lo.hi + hi.lo + hi.hi, its factors' powers of two undone afterwards.  The
+// lowest bit of lo stands for 2^-39 of the tile's largest value, so a row much
+// smaller than its neighbours loses bits only where they hardly count.
+//
+// A packed tile holds 128 rows (queries or keys) of one head, `DP` columns
+// (head_dim rounded up to 64 or 128, zeros behind it): [hi | lo][DP / 64] boxes
+// of 128 rows x 64 columns, each row 128 bytes, its 16-byte pieces exchanged
+// as the matrix unit's 128-byte swizzle wants them.  A copy of whole boxes, or
+// of 64 of their rows, is then one untiled bulk copy, and the same box serves
+// as an operand summed over its columns (scores) or over its rows (values).
+constexpr int kTile = 128;
+constexpr int kBox = kTile * 128;  // bytes
+constexpr uint32_t kLayoutSW128 = 2;
+
+template <int DP>
+constexpr int kTileBytes = 2 * (DP / 64) * kBox;
+
+__host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
+
+// One operand to pack: `heads` heads of `len` rows; rows are keys (valid below
+// the sequence's n) or queries (valid where they stand in the sequence).
+struct PackJob {
+  const float* x;
+  uint8_t* tiles;   // [batch][heads][tiles_of(len)] packed tiles
+  float* factors;   // the power of two that undoes each tile's scale; NaN: a value is not finite
+  int heads, len, queries;
+  // Queries' gradient only: delta[row] = sum of x * out over the row.
+  const float* out;
+  float* delta;
+};
+struct PackJobs {
+  AttentionShape s;
+  PackJob job[4];
+  int first[5];  // first block of each job
+};
+
+template <int DP>
+__global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
+  constexpr int kChunks = DP / 8;                  // 8-column pieces of a row
+  constexpr int kPer = kTile * kChunks / 256;      // pieces a thread holds
+  __shared__ uint32_t warp_max[8];
+  int which = 0;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) which += (int)blockIdx.x >= p.first[i];
+  const PackJob& j = p.job[which];
+  const AttentionShape& s = p.s;
+  const int tiles = tiles_of(j.len);
+  const int index = (int)blockIdx.x - p.first[which];
+  const int t = index % tiles, h = index / tiles % j.heads, b = index / tiles / j.heads;
+  const Sequence sq = sequence_of(s, b, err);
+  // Valid rows of the whole operand: [v0, v1).
+  int v0 = 0, v1 = sq.n;
+  if (j.queries) v0 = -sq.start, v1 = sq.n - sq.start;
+  const int r0 = max(t * kTile, v0), r1 = min(min(j.len, (t + 1) * kTile), v1);
+  if (r0 >= r1) {  // nothing reads this tile's values
+    if (threadIdx.x == 0) j.factors[index] = 1.0f;
+    if (j.delta != nullptr)
+      for (int r = threadIdx.x; r < kTile && t * kTile + r < j.len; r += 256)
+        j.delta[((int64_t)b * j.heads + h) * j.len + t * kTile + r] = 0.0f;
+    return;
+  }
+  const bool vec = s.head_dim % 4 == 0 && ((uintptr_t)j.x & 15) == 0 && ((uintptr_t)j.out & 15) == 0;
+  float v[kPer][8];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int item = threadIdx.x + 256 * i;
+    const int r = t * kTile + item / kChunks, c = item % kChunks * 8;
+    const float* src = j.x + row_at(s, b, h, r, j.heads, j.len) + c;
+    const bool live = r >= r0 && r < r1;
+    if (vec) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 f = live && c + e < s.head_dim ? *(const float4*)(src + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[i][e] = f.x, v[i][e + 1] = f.y, v[i][e + 2] = f.z, v[i][e + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = live && c + e < s.head_dim ? src[e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+  }
+  if (j.delta != nullptr) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int item = threadIdx.x + 256 * i;
+      const int r = t * kTile + item / kChunks, c = item % kChunks * 8;
+      const float* src = j.out + row_at(s, b, h, r, j.heads, j.len) + c;
+      float d = 0.0f;
+      if (r >= r0 && r < r1)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < s.head_dim) d += v[i][e] * src[e];
+#pragma unroll
+      for (int o = kChunks / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      if (item % kChunks == 0 && r < j.len) j.delta[((int64_t)b * j.heads + h) * j.len + r] = d;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = max(top, warp_max[w]);
+  const int exponent = (int)(top >> 23) - 127;  // of the largest magnitude; 128: not finite
+  const int up = top == 0 ? 0 : min(14 - exponent, 126);
+  const float scale = __uint_as_float((uint32_t)(up + 127) << 23);
+  if (threadIdx.x == 0)
+    j.factors[index] = exponent == 128 ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
+  uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int item = threadIdx.x + 256 * i;
+    const int r = item / kChunks, chunk = item % kChunks;
+    uint4 hi, lo;
+    uint32_t* hw = &hi.x;
+    uint32_t* lw = &lo.x;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float a = v[i][e] * scale, c = v[i][e + 1] * scale;
+      const __half2 h2 = __floats2half2_rn(a, c);
+      const float2 back = __half22float2(h2);
+      const __half2 l2 = __floats2half2_rn(a - back.x, c - back.y);
+      hw[e / 2] = *(const uint32_t*)&h2;
+      lw[e / 2] = *(const uint32_t*)&l2;
+    }
+    uint8_t* at = dst + (chunk / 8) * kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+    *(uint4*)at = hi;
+    *(uint4*)(at + (DP / 64) * kBox) = lo;
+  }
+}
+
+// ---- pieces of the tensor-core kernels ---------------------------------------------------
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const uint8_t* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+// A bounded wait whose outcome a whole warp shares.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+}
+
+// D (+)= A . B over 16 terms, fp16 operands, fp32 accumulator in tensor
+// memory; A from shared memory, or (a row per lane, two terms per column) from
+// tensor memory.
+// Descriptors of shared-memory operands come as their low words (see
+// column_word and row_word): the high one is the same for all, and the words
+// of an operand's steps lie constants apart.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (kLayoutSW128 << 29);  // 1024 bytes between 8-row groups
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(add));
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(add));
+}
+// fp16 x fp16 -> fp32, M = 128; `b_rows`: B is summed over its rows.
+constexpr uint32_t umma_idesc(int n, bool b_rows) {
+  return (1u << 4) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// A box as an operand summed over its columns: 16 columns are 32 bytes.
+constexpr uint32_t kColumnStep = 32 >> 4;
+__device__ __forceinline__ uint32_t column_word(uint32_t box) { return box >> 4 | 1u << 16; }
+// Boxes `stride` bytes apart as an operand summed over their rows: 16 rows are 2048 bytes.
+constexpr uint32_t kRowStep = 2048 >> 4;
+__device__ __forceinline__ uint32_t row_word(uint32_t box, uint32_t stride) { return box >> 4 | stride >> 4 << 16; }
+
+// A load and the wait for it in one statement: nothing reads the registers in between.
+__device__ __forceinline__ void tmem_ld16(uint32_t at, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(at), "r"(at + 32)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
+}
+
+// 2^x to about 2^-22, subnormal results as 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// hi and lo of 32 neighbouring values as an A operand's 32 columns: 16 with hi
+// (two values each), 16 with lo.
+__device__ __forceinline__ void split32(const float* v, uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    const float2 back = __half22float2(h);
+    const __half2 l = __floats2half2_rn(v[2 * i] - back.x, v[2 * i + 1] - back.y);
+    r[i] = *(const uint32_t*)&h;
+    r[16 + i] = *(const uint32_t*)&l;
+  }
+}
+// Column of the t-th 16 terms' hi part in such an operand (lo: 16 further).
+__device__ __forceinline__ uint32_t split_col(int t) { return (uint32_t)((t >> 1) * 32 + (t & 1) * 8); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Bits e with lo <= first + e < hi.
+__device__ __forceinline__ uint32_t bits_between(int lo, int hi, int first) {
+  const int a = min(max(lo - first, 0), 32), z = min(max(hi - first, 0), 32);
+  if (a >= z) return 0;
+  return (0xffffffffu >> (32 - (z - a))) << a;
+}
+
+// The key tiles that a tile of query rows needs: [0, sinks) and then `low` on.
+struct TileRange {
+  int sinks, low, count;
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : low + i - sinks; }
+};
+struct RowRange {
+  int p0, p1;  // positions of the first and last row that exist
+  bool all;    // 128 rows, each standing in the sequence
+};
+
+__device__ __forceinline__ RowRange rows_of(const AttentionShape& s, const Sequence& q, int r0) {
+  RowRange r;
+  r.p0 = q.start + r0;
+  r.p1 = q.start + min(r0 + kTile, s.q_len) - 1;
+  r.all = r.p0 >= 0 && r.p1 < q.n && r0 + kTile <= s.q_len;
+  return r;
+}
+
+__device__ __forceinline__ TileRange keys_for(const AttentionShape& s, const Sequence& q, const RowRange& r) {
+  const int a = max(r.p0, 0), z = min(r.p1, q.n - 1);
+  if (a > z) return {0, 0, 0};
+  const int low = s.window > 0 ? max(a + 1 - s.window, 0) : 0;
+  TileRange t;
+  t.low = low / kTile;
+  t.sinks = min(tiles_of(min(s.sinks, low)), t.low);
+  t.count = t.sinks + z / kTile - t.low + 1;
+  return t;
+}
+
+// Whether every row of the tile sees every key of tile t.
+__device__ __forceinline__ bool sees_all(const AttentionShape& s, const RowRange& r, int t) {
+  const int j0 = t * kTile, j1 = j0 + kTile - 1;
+  return r.all && j1 <= r.p0 && (s.window == 0 || r.p1 - j0 < s.window || j1 < s.sinks);
+}
+
+// ---- forward ----------------------------------------------------------------------------
+
+// One block per SM walks work items (128 query rows of a head) and, for each,
+// the key tiles of 128 that its rows see; the tiles of all items form one
+// stream, so that an item's start and end overlap its neighbours' arithmetic.
+//   warps 0-7    probabilities: two threads share a row, 64 columns each.  A
+//                tile's probabilities are taken relative to the row's greatest
+//                score in that tile alone, so that no state goes from tile to
+//                tile here: p = 2^(s - m + 14), split into fp16 halves over
+//                the scores in tensor memory.
+//   warps 8-15   output: each tile's P.V is added to fp32 registers, both
+//                brought to the greater of the two reference scores.  (An
+//                accumulator that stayed in tensor memory would lose up to a
+//                step per matrix instruction, always toward zero.)
+//   warp 16      copies packed tiles into a ring of 32 KB slots,
+//   warp 17      issues the matrix instructions: the scores of a tile before
+//                the values of the one before it, so that the two overlap.
+constexpr int kThreads = 20 * 32;  // warps 18 and 19 only hold registers for the others
+constexpr int kSlotBytes = 2 * kBox;
+
+// Registers per thread: launched with 96 (640 threads), 480 for the five warps
+// of each quarter of an SM; after the split 2 x 120 + 2 x 88 + 64 = 480.
+constexpr int kScoreRegs = 120, kOutputRegs = 88, kFewRegs = 64;
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int DP>
+struct ForwardPlan {
+  static constexpr int kHalves = DP / 64;
+  static constexpr int kSlots = DP == 64 ? 5 : 4;
+  static constexpr int kSmem = 1024 + kTileBytes<DP> + kSlots * kSlotBytes + 6144;
+};
+
+struct ForwardArgs {
+  AttentionShape s;
+  const float *q, *k, *v;
+  const uint8_t *pq, *pk, *pv;
+  const float *fq, *fk, *fv;
+  float *out, *stats;
+};
+
+// Work item `index`: 128 rows of a head, those that see the most keys first.
+struct QueryItem {
+  int b, h, g, r0, n;  // n: key tiles to walk; 0: none, or values that are not finite
+  Sequence sq;
+  RowRange rows;
+  TileRange range;
+  int q_index, k_index;  // of the item's query tile and its head's first key tile
+};
+
+// Called by whole warps.  `others`: per-tile factors that have to be finite
+// besides fq, fk and fv (the gradient's), or null.
+__device__ __forceinline__ QueryItem query_item(const AttentionShape& s, int index, const float* fq, const float* fk,
+                                                const float* fv, const float* others, int* err) {
+  QueryItem t;
+  const int tiles_q = tiles_of(s.q_len);
+  const int tq = tiles_q - 1 - index / (s.heads * s.batch);
+  t.h = index % s.heads;
+  t.b = index / s.heads % s.batch;
+  t.g = t.h / (s.heads / s.kv_heads);
+  t.r0 = tq * kTile;
+  t.sq = sequence_of(s, t.b, err);
+  t.rows = rows_of(s, t.sq, t.r0);
+  t.range = keys_for(s, t.sq, t.rows);
+  t.q_index = (t.b * s.heads + t.h) * tiles_q + tq;
+  t.k_index = (t.b * s.kv_heads + t.g) * tiles_of(s.k_len);
+  float sum = fq[t.q_index] + (others != nullptr ? others[t.q_index] : 0.0f);
+  for (int i = threadIdx.x & 31; i < t.range.count; i += 32)
+    sum += fk[t.k_index + t.range.at(i)] + fv[t.k_index + t.range.at(i)];
+  // A product with a hidden value that is not finite would not be 0: such
+  // rows go key by key instead.
+  t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  return t;
+}
+
+// The block's item of a round (-1: none in this one); false after the last
+// round.  Items come heaviest first, and every other round runs backwards over
+// the blocks, so that the rounds' differences even out.
+__device__ __forceinline__ bool item_of(int round, int items, int* w) {
+  const int blocks = gridDim.x, x = blockIdx.x;
+  const int at = round * blocks + (round & 1 ? blocks - 1 - x : x);
+  *w = at < items ? at : -1;
+  return round * blocks < items;
+}
+
+// What a row of an item sees, for the masks of tiles that not all rows see whole.
+struct RowMask {
+  int low, high, sinks;  // [low, high) and [0, sinks)
+};
+__device__ __forceinline__ RowMask mask_of(const AttentionShape& s, const QueryItem& t, int row) {
+  const int p = t.rows.p0 + row;
+  RowMask m;
+  m.high = t.r0 + row < s.q_len && p >= 0 && p < t.sq.n ? p + 1 : 0;
+  m.low = s.window > 0 ? max(p + 1 - s.window, 0) : 0;
+  m.sinks = min(m.high, s.sinks);
+  return m;
+}
+__device__ __forceinline__ uint32_t seen_bits(const RowMask& m, int first) {
+  return bits_between(m.low, m.high, first) | bits_between(0, m.sinks, first);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int items, int* err) {
+  using Plan = ForwardPlan<DP>;
+  constexpr int kHalves = Plan::kHalves;
+  const AttentionShape& s = a.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t q_smem = smem_u32(smem);
+  const uint32_t slots = q_smem + kTileBytes<DP>;
+  uint8_t* misc = smem + kTileBytes<DP> + Plan::kSlots * kSlotBytes;
+  float* ref = (float*)misc;            // [2][128] reference exponents of a tile's rows
+  float* sum = ref + 2 * kTile;         // [2][2][128] sums of each half of the tile's columns
+  float* most = sum + 4 * kTile;        // [2][2][128] greatest scores of each half
+  uint64_t* bars = (uint64_t*)(most + 4 * kTile);
+  const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8, slot_full = q_empty + 8;
+  const uint32_t slot_empty = slot_full + 8 * Plan::kSlots, s_full = slot_empty + 8 * Plan::kSlots;
+  const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16, pair_full = o_empty + 16, drained = pair_full + 32;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 15);
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < Plan::kSlots; ++i) mbar_init(slot_full + 8 * i, 1), mbar_init(slot_empty + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 8);
+      mbar_init(o_full + 8 * i, 1);
+      mbar_init(o_empty + 8 * i, 8);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(pair_full + 8 * i, 2);
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Tensor memory: two buffers of scores (128 columns), two of values (DP).
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 18) {
+    fewer_registers<kFewRegs>();
+  } else if (warp == 16) {
+    fewer_registers<kFewRegs>();
+    const uint8_t* values = nullptr;  // the tile before's values
+    uint32_t it = 0, loaded = 0;      // slots filled, query tiles loaded
+    bool ok = true;
+    auto fill = [&](const uint8_t* src, bool is_values) {
+      for (int d = 0; d < kHalves && ok; ++d, ++it) {
+        const uint32_t slot = it % Plan::kSlots, use = it / Plan::kSlots;
+        if (use > 0) ok = mbar_wait(slot_empty + 8 * slot, (use - 1) & 1, err);
+        if (!ok) break;
+        const uint32_t full = slot_full + 8 * slot, dst = slots + slot * kSlotBytes;
+        mbar_expect_tx(full, kSlotBytes);
+        if (!is_values || kHalves == 1) {
+          // 128 rows of one box, hi and lo.
+          bulk_load(dst, src + d * kBox, kBox, full);
+          bulk_load(dst + kBox, src + (kHalves + d) * kBox, kBox, full);
+        } else {
+          // 64 rows (keys) of every box: hi boxes, then lo boxes.
+#pragma unroll
+          for (int x = 0; x < 2 * kHalves; ++x)
+            bulk_load(dst + x * (kBox / 2), src + x * kBox + d * (kBox / 2), kBox / 2, full);
+        }
+      }
+    };
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      if (lane == 0 && t.n > 0) {
+        if (loaded > 0) ok = mbar_wait(q_empty, (loaded - 1) & 1, err);
+        if (ok) {
+          mbar_expect_tx(q_full, kTileBytes<DP>);
+          bulk_load(q_smem, a.pq + (int64_t)t.q_index * kTileBytes<DP>, kTileBytes<DP>, q_full);
+          ++loaded;
+        }
+        for (int i = 0; i < t.n && ok; ++i) {
+          const int64_t tile = (int64_t)(t.k_index + t.range.at(i)) * kTileBytes<DP>;
+          fill(a.pk + tile, false);
+          if (ok && values != nullptr) fill(values, true);
+          values = a.pv + tile;
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+    if (lane == 0) {
+      if (ok && values != nullptr) fill(values, true);
+      if (!ok) {  // copies in flight end before the block does
+        if (loaded > 0) mbar_wait(q_full, (loaded - 1) & 1, err);
+        for (uint32_t f = it > Plan::kSlots ? it - Plan::kSlots : 0; f < it; ++f)
+          mbar_wait(slot_full + 8 * (f % Plan::kSlots), (f / Plan::kSlots) & 1, err);
+      }
+    }
+  } else if (warp == 17) {
+    fewer_registers<kFewRegs>();
+    constexpr uint32_t kScore = umma_idesc(kTile, false), kValue = umma_idesc(DP, true);
+    uint32_t it = 0, gi = 0, item = 0;  // slots, tiles and items issued so far
+    bool ok = true;
+    auto values = [&](uint32_t t) {  // of tile t of the stream
+      const int buf = t & 1;
+      const uint32_t p = tmem + buf * kTile, d = tmem + 2 * kTile + buf * DP;
+      ok = mbar_wait(p_full + 8 * buf, (t >> 1) & 1, err);
+      if (ok && t >= 2) ok = mbar_wait(o_empty + 8 * buf, ((t >> 1) - 1) & 1, err);
+      for (int x = 0; x < kHalves && ok; ++x, ++it) {
+        const uint32_t slot = it % Plan::kSlots;
+        ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        constexpr int kSteps = kTile / 16 / kHalves;
+        constexpr uint32_t kStride = kBox / kHalves;  // between the slot's boxes
+        const uint32_t v = row_word(slots + slot * kSlotBytes, kStride);
+        const uint32_t px = p + split_col(x * kSteps);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const uint32_t ph = px + split_col(k), vh = v + k * kRowStep, vl = vh + (kBox >> 4);
+          umma_ts(d, ph + 16, vh, kValue, x != 0 || k != 0);
+          umma_ts(d, ph, vl, kValue, 1u);
+          umma_ts(d, ph, vh, kValue, 1u);
+        }
+        umma_commit(slot_empty + 8 * slot);
+      }
+      if (ok) umma_commit(o_full + 8 * buf);
+    };
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      if (lane == 0 && t.n > 0) {
+        ok = mbar_wait(q_full, item & 1, err);
+        ++item;
+        for (int i = 0; i < t.n && ok; ++i, ++gi) {
+          const uint32_t d = tmem + (gi & 1) * kTile;
+          for (int x = 0; x < kHalves && ok; ++x, ++it) {
+            const uint32_t slot = it % Plan::kSlots;
+            ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t q = column_word(q_smem + x * kBox), key = column_word(slots + slot * kSlotBytes);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t qh = q + k * kColumnStep, ql = qh + (kHalves * kBox >> 4);
+              const uint32_t kh = key + k * kColumnStep, kl = kh + (kBox >> 4);
+              umma_ss(d, ql, kh, kScore, x != 0 || k != 0);
+              umma_ss(d, qh, kl, kScore, 1u);
+              umma_ss(d, qh, kh, kScore, 1u);
+            }
+            umma_commit(slot_empty + 8 * slot);
+          }
+          if (!ok) break;
+          umma_commit(s_full + 8 * (gi & 1));
+          if (i == t.n - 1) umma_commit(q_empty);
+          if (gi > 0) values(gi - 1);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+    if (lane == 0) {
+      if (ok && gi > 0) values(gi - 1);
+      if (!ok) {  // instructions in flight end before the block does
+        umma_commit(drained);
+        mbar_wait(drained, 0, err);
+      }
+    }
+  } else if (warp < 8) {
+    more_registers<kScoreRegs>();
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+    uint32_t gi = 0;
+    bool ok = true;
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      if (t.n == 0) {
+        for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
+          simple_forward_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, t.b, t.h, r);
+        continue;
+      }
+      const RowMask mask = mask_of(s, t, row);
+      const double to_log2 = (double)a.fq[t.q_index] * (double)s.scale * 1.4426950408889634;
+      for (int i = 0; i < t.n; ++i, ++gi) {
+        const int buf = gi & 1, tile = t.range.at(i);
+        const float f = (float)(to_log2 * (double)a.fk[t.k_index + tile]);
+        const bool whole = sees_all(s, t.rows, tile);
+        ok = warp_wait(s_full + 8 * buf, (gi >> 1) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        float v[64];
+        tmem_ld64(at + buf * kTile, v);
+        if (!whole) {
+          const int j0 = tile * kTile + half * 64;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t seen = seen_bits(mask, j0 + 32 * c);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1u)) v[32 * c + e] = -INFINITY;
+          }
+        }
+        float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
+#pragma unroll
+        for (int e = 4; e < 64; e += 4) {
+          m0 = fmaxf(m0, v[e]);
+          m1 = fmaxf(m1, v[e + 1]);
+          m2 = fmaxf(m2, v[e + 2]);
+          m3 = fmaxf(m3, v[e + 3]);
+        }
+        m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        // The row's other half is in the warp four further; `most` and `sum` of
+        // the tile before last have been read once its output buffer is free.
+        if (gi >= 2) ok = warp_wait(o_empty + 8 * buf, ((gi >> 1) - 1) & 1, err);
+        if (!ok) break;
+        most[(buf * 2 + half) * kTile + row] = m0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pair_full + 8 * (warp & 3));
+        ok = warp_wait(pair_full + 8 * (warp & 3), gi & 1, err);
+        if (!ok) break;
+        m0 = fmaxf(m0, most[(buf * 2 + 1 - half) * kTile + row]);
+        const float c0 = m0 == -INFINITY ? 0.0f : fmaf(m0, f, -14.0f);
+        float l[4] = {};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            v[32 * c + e] = exp2_fast(fmaf(v[32 * c + e], f, -c0));
+            l[e & 3] += v[32 * c + e];
+          }
+          uint32_t r[32];
+          split32(v + 32 * c, r);
+          tmem_st32(at + buf * kTile + 32 * c, r);
+        }
+        sum[(buf * 2 + half) * kTile + row] = (l[0] + l[1]) + (l[2] + l[3]);
+        if (half == 0) ref[buf * kTile + row] = m0 == -INFINITY ? -INFINITY : c0;
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8 * buf);
+      }
+    }
+  } else {
+    fewer_registers<kOutputRegs>();
+    constexpr int kCols = DP / 2;  // output columns of a thread
+    const int quad = warp & 3, half = (warp - 8) >> 2, row = quad * 32 + lane;
+    const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + 2 * kTile + half * kCols;
+    uint32_t gi = 0;
+    bool ok = true;
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      if (t.n == 0) continue;
+      float acc[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+      float top = -INFINITY, l = 0.0f;
+      for (int i = 0; i < t.n; ++i, ++gi) {
+        const int buf = gi & 1;
+        const float fv = a.fv[t.k_index + t.range.at(i)];
+        ok = warp_wait(p_full + 8 * buf, (gi >> 1) & 1, err) && warp_wait(o_full + 8 * buf, (gi >> 1) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        const float c0 = ref[buf * kTile + row];
+        const float next = fmaxf(top, c0);
+        const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - next);
+        const float take = c0 == -INFINITY ? 0.0f : exp2_fast(c0 - next);
+        l = l * keep + (sum[2 * buf * kTile + row] + sum[(2 * buf + 1) * kTile + row]) * take;
+        top = next;
+        const float tv = take * fv;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          float v[16];
+          tmem_ld16(at + buf * DP + c, v);
+          if (c == kCols - 16) {  // the last values are out: the buffer is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty + 8 * buf);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(acc[c + e], keep, v[e] * tv);
+        }
+      }
+      const int r = t.r0 + row;
+      if (ok && r < s.q_len) {
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      float* dst = a.out + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols;
+      const int cols = s.head_dim - half * kCols;
+      if (s.head_dim % 4 == 0 && ((uintptr_t)a.out & 15) == 0) {
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4)
+          if (c < cols)
+            *(float4*)(dst + c) =
+                make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+      } else {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+          if (c < cols) dst[c] = acc[c] * inv;
+      }
+      if (a.stats != nullptr && half == 0) {
+        // Natural units; the sum takes up what rounding the greatest score
+        // loses, so that the backward's 2^(s - max) / sum is consistent.
+        const float m = top == -INFINITY ? -INFINITY : (top + 14.0f) * kLn2;
+        const float z = top == -INFINITY ? 0.0f : l * exp2f(top - m * kLog2e);
+        *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = make_float2(m, z);
+      }
+      }
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 17) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
 }  // namespace
 
-int64_t window_attention_work_elems(const AttentionShape&) { return 1; }
+namespace {
+
+// Sections of the workspace, in floats, each on a 256-byte boundary.
+struct Carver {
+  float* base;
+  int64_t used = 0;
+  float* take(int64_t floats) {
+    float* p = base ? base + used : nullptr;
+    used += (floats + 63) / 64 * 64;
+    return p;
+  }
+};
+
+constexpr int64_t kSms = 148;
+
+int padded_dim(const AttentionShape& s) { return s.head_dim <= 64 ? 64 : 128; }
+
+struct ForwardWork {
+  uint8_t *pq, *pk, *pv;
+  float *fq, *fk, *fv;
+  int64_t floats;
+};
+ForwardWork forward_work(const AttentionShape& s, float* base) {
+  Carver c{base};
+  const int64_t tile = padded_dim(s) == 64 ? kTileBytes<64> / 4 : kTileBytes<128> / 4;
+  const int64_t nq = (int64_t)s.batch * s.heads * tiles_of(s.q_len), nk = (int64_t)s.batch * s.kv_heads * tiles_of(s.k_len);
+  ForwardWork w;
+  w.pq = (uint8_t*)c.take(nq * tile);
+  w.pk = (uint8_t*)c.take(nk * tile);
+  w.pv = (uint8_t*)c.take(nk * tile);
+  w.fq = c.take(nq);
+  w.fk = c.take(nk);
+  w.fv = c.take(nk);
+  w.floats = c.used;
+  return w;
+}
+
+bool uses_tiles(const AttentionShape& s) { return s.q_len >= 16; }
+
+void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, cudaStream_t st) {
+  PackJobs p{};
+  p.s = s;
+  int64_t at = 0;
+  for (int i = 0; i < 4; ++i) {
+    p.first[i] = i < count ? (int)at : INT_MAX;
+    if (i >= count) continue;
+    p.job[i] = jobs[i];
+    at += (int64_t)s.batch * jobs[i].heads * tiles_of(jobs[i].len);
+  }
+  if (at > INT_MAX) throw CudaError("window_attention: too many rows");
+  if (padded_dim(s) == 64) pack_kernel<64><<<(unsigned)at, 256, 0, st>>>(p, err);
+  else pack_kernel<128><<<(unsigned)at, 256, 0, st>>>(p, err);
+  check_launch();
+}
+
+template <int DP>
+void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
+  TYSOR_CUDA(cudaFuncSetAttribute(forward_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  ForwardPlan<DP>::kSmem));
+  const int64_t items = (int64_t)tiles_of(a.s.q_len) * a.s.heads * a.s.batch;  // at most what run_pack took
+  forward_kernel<DP><<<(unsigned)(items < kSms ? items : kSms), kThreads, ForwardPlan<DP>::kSmem, st>>>(
+      a, (int)items, err);
+  check_launch();
+}
+
+}  // namespace
+
+int64_t window_attention_work_elems(const AttentionShape& s) {
+  return uses_tiles(s) ? forward_work(s, nullptr).floats : 1;
+}
 int64_t window_attention_backward_work_elems(const AttentionShape&) { return 1; }
 
 void launch_window_attention(const AttentionShape& s, const float* q, const float* k, const float* v, float* out,
-                             float* stats, float*, int* err, cudaStream_t st) {
+                             float* stats, float* work, int* err, cudaStream_t st) {
   const int64_t rows = (int64_t)s.batch * s.heads * s.q_len;
   if (rows <= 0) return;
+  if (uses_tiles(s)) {
+    const ForwardWork w = forward_work(s, work);
+    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1, nullptr, nullptr},
+                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, nullptr, nullptr},
+                       {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, nullptr, nullptr}};
+    run_pack(s, jobs, 3, err, st);
+    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats};
+    if (padded_dim(s) == 64) run_forward<64>(a, err, st);
+    else run_forward<128>(a, err, st);
+    return;
+  }
   simple_forward_kernel<<<(unsigned)ceil_div(rows, 8), 256, 0, st>>>(s, q, k, v, out, stats, err);
   check_launch();
 }

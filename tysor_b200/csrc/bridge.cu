@@ -230,9 +230,9 @@ AttentionShape attention_shape(uint32_t batch, uint32_t heads, uint32_t kv_heads
     throw CudaError("window_attention: the key heads must divide the query heads");
   if (head_dim == 0 || head_dim > (uint32_t)kMaxHeadDim)
     throw CudaError("window_attention takes heads of 1 to " + std::to_string(kMaxHeadDim) + " values");
-  const uint32_t most = 1u << 30;
+  const uint32_t most = 1u << 29;  // positions stay below 2^30
   if (q_len > most || k_len > most || batch > most || heads > most)
-    throw CudaError("window_attention takes lengths, batches and heads up to 2^30");
+    throw CudaError("window_attention takes lengths, batches and heads up to 2^29");
   // A subnormal scale would hold fewer bits than the scores it multiplies.
   if (!(scale >= 1.17549435e-38f) || isinf(scale))
     throw CudaError("window_attention requires a finite scale of at least 2^-126");

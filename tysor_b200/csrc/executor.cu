@@ -1353,7 +1353,9 @@ struct Executor {
       if (i > 6 || numel(t.shape) != q.shape[0]) fail("window_attention expects one length and one start per sequence");
       (i == 5 ? c.lengths : c.starts) = t.slot;
     }
-    const int64_t most = 1 << 30;
+    const int64_t most = 1 << 29;
+    if (q.shape[0] > most || q.shape[hl] > most || q.shape[sl] > most || k.shape[sl] > most)
+      fail("window_attention takes lengths, batches and heads up to 2^29");
     c.s.batch = (int)q.shape[0];
     c.s.heads = (int)q.shape[hl];
     c.s.kv_heads = (int)k.shape[hl];

@@ -35,6 +35,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace tysor {
 namespace {
@@ -42,50 +43,6 @@ namespace {
 constexpr int BM = 128;
 constexpr int BK = 16;  // fp32 elements of K per stage (64 bytes)
 constexpr int kGroupM = 16;  // tile rows per raster group of the 1-SM kernel
-constexpr long long kWaitCycles = 4000000000LL;  // about 2 s at 1.9 GHz
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Waits for the given phase parity; gives up after `limit` cycles,
-// recording kErrBarrierTimeout, so a lost arrival can never hang the GPU.
-__device__ bool mbar_wait_limit(uint32_t bar, uint32_t parity, int* err, long long limit) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity)) {
-    if (clock64() - t0 > limit) {
-      atomicCAS(err, 0, (int)kErrBarrierTimeout);
-      return false;
-    }
-  }
-  return true;
-}
-
-__device__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err) {
-  return mbar_wait_limit(bar, parity, err, kWaitCycles);
-}
 
 // One thread initialises a barrier that expects one arrival, never arrives,
 // and waits on it with the pipelines' own wait: the wait must give up after
@@ -116,19 +73,6 @@ __device__ __forceinline__ void umma_tf32(uint32_t d_tmem, uint64_t adesc, uint6
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   uint32_t r[16];
   asm volatile(
@@ -141,18 +85,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float* v) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Shared-memory matrix descriptor (tcgen05 "version 1" format).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo,
-                                              uint32_t layout) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)layout << 61;
-  return d;
 }
 
 // Layout types of the descriptor (bits 61-63).
@@ -199,10 +131,6 @@ constexpr int kChunkKb = 8;
 __device__ __forceinline__ int chunk_kb(const GemmEpilogue& ep) { return ep.chunk_kb > 0 ? ep.chunk_kb : kChunkKb; }
 constexpr int kAccWarps = 8;
 constexpr int kThreadsTC = 64 + 32 * kAccWarps;
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 
 // Causal attention GEMMs (GemmEpilogue::tri): for a tile of rows
 // [r0, r0 + rows) and columns from c0, narrows the k-block range to the
