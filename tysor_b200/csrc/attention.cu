@@ -4,6 +4,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "lm_ops.cuh"
 #include "tcgen05.cuh"
 
@@ -124,16 +126,6 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
   lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, acc, inv, 0);
   if (stats != nullptr && (threadIdx.x & 31) == 0)
     *(float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r)) = make_float2(m, l);
-}
-
-__global__ void __launch_bounds__(256) simple_forward_kernel(AttentionShape s, const float* __restrict__ q,
-                                                             const float* __restrict__ k,
-                                                             const float* __restrict__ v, float* __restrict__ out,
-                                                             float* __restrict__ stats, int* err) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= (int64_t)s.batch * s.heads * s.q_len) return;
-  const int r = (int)(i % s.q_len), h = (int)(i / s.q_len % s.heads), b = (int)(i / s.q_len / s.heads);
-  simple_forward_row(s, sequence_of(s, b, err), q, k, v, out, stats, b, h, r);
 }
 
 __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
@@ -937,6 +929,206 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   }
 }
 
+// ---- a few query rows over a long cache ----------------------------------------------------
+
+// The rows that share a key head (at most R of them per block) go over its
+// keys once, straight from the fp32 cache: with so few rows the reads bound
+// it, not the products.  The keys are split over `splits` blocks; each warp
+// takes 8 keys at a time, eight lanes per key with 4 NI columns each, and each
+// group of eight lanes keeps a running maximum, sum and output of its own, so
+// that only the dot products cross lanes.  Groups, warps and splits are joined
+// at the end in a fixed order.
+constexpr int kDecodeThreads = 128;
+constexpr int kDecodeRows = 8;
+
+template <int NI, int R, bool VEC>
+__global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s, const float* __restrict__ q,
+                                                                const float* __restrict__ k,
+                                                                const float* __restrict__ v, float* __restrict__ out,
+                                                                float* __restrict__ stats, float* __restrict__ part,
+                                                                int splits, int row_blocks, int* err) {
+  constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
+  __shared__ float qs[R][kDims];
+  __shared__ float joined[kWarps][R][kDims + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
+  int64_t index = blockIdx.x;
+  const int split = (int)(index % splits);
+  index /= splits;
+  const int rb = (int)(index % row_blocks);
+  index /= row_blocks;
+  const int g = (int)(index % s.kv_heads), b = (int)(index / s.kv_heads);
+  const int group = s.heads / s.kv_heads, total = group * s.q_len;
+  const Sequence sq = sequence_of(s, b, err);
+  // Keys that some row sees: [0, first) and [low, high), counted through.
+  const int a = max(sq.start, 0), z = min(sq.start + s.q_len, sq.n);  // live positions [a, z)
+  const int low = a < z && s.window > 0 ? max(a + 1 - s.window, 0) : 0;
+  const int first = a < z ? min(s.window > 0 ? s.sinks : 0, low) : 0;
+  const int keys = a < z ? first + z - low : 0;
+  const int per = ((keys + splits - 1) / splits + 31) / 32 * 32;
+  const int u0 = min(keys, split * per), u1 = min(keys, u0 + per);
+  for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
+    const int r = rb * R + i / kDims, c = i % kDims;
+    qs[i / kDims][c] = r < total && c < s.head_dim
+                           ? q[row_at(s, b, g * group + r / s.q_len, r % s.q_len, s.heads, s.q_len) + c]
+                           : 0.0f;
+  }
+  int at[R];  // position of each row; below 0: not a row, or not in the sequence
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int p = sq.start + (rb * R + r) % s.q_len;
+    at[r] = rb * R + r < total && p < sq.n ? p : -1;
+  }
+  __syncthreads();
+  float m[R], l[R], acc[R][4 * NI];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 4 * NI; ++c) acc[r][c] = 0.0f;
+  }
+  const int64_t step = s.seq_major ? (int64_t)s.kv_heads * s.head_dim : s.head_dim;
+  const int64_t base = row_at(s, b, g, 0, s.kv_heads, s.k_len);
+  auto load = [&](const float* __restrict__ x, int j, float (&d)[4 * NI]) {
+    const float* src = x + base + j * step;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int c = 4 * l8 + 32 * i;
+      if (VEC) {
+        const float4 f = c < s.head_dim ? __ldg((const float4*)(src + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        d[4 * i] = f.x, d[4 * i + 1] = f.y, d[4 * i + 2] = f.z, d[4 * i + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[4 * i + e] = c + e < s.head_dim ? __ldg(src + c + e) : 0.0f;
+      }
+    }
+  };
+  for (int u = u0 + key_of; u < u1; u += 8 * kWarps) {
+    const bool two = u + 4 * kWarps < u1;
+    const int u2 = two ? u + 4 * kWarps : u;
+    const int j[2] = {u < first ? u : low + u - first, u2 < first ? u2 : low + u2 - first};
+    float kd[2][4 * NI], vd[2][4 * NI];
+    load(k, j[0], kd[0]);
+    load(k, j[1], kd[1]);
+    load(v, j[0], vd[0]);
+    load(v, j[1], vd[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float d[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const float4 f = *(const float4*)&qs[r][4 * l8 + 32 * i];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          d[w] = fmaf(f.x, kd[w][4 * i], d[w]);
+          d[w] = fmaf(f.y, kd[w][4 * i + 1], d[w]);
+          d[w] = fmaf(f.z, kd[w][4 * i + 2], d[w]);
+          d[w] = fmaf(f.w, kd[w][4 * i + 3], d[w]);
+        }
+      }
+      // All eight lanes of a key are here together (they share u).
+      const uint32_t lanes = 0xffu << (lane & 24);
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        d[0] += __shfl_xor_sync(lanes, d[0], o);
+        d[1] += __shfl_xor_sync(lanes, d[1], o);
+      }
+      bool sees[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        d[w] *= s.scale;
+        sees[w] = (w == 0 || two) && j[w] <= at[r] && (s.window == 0 || at[r] - j[w] < s.window || j[w] < s.sinks);
+        if (!sees[w]) d[w] = -INFINITY;
+      }
+      const float top = fmaxf(m[r], fmaxf(d[0], d[1]));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float keep = exp2f((m[r] - ref) * kLog2e);
+      m[r] = top;
+      l[r] *= keep;
+#pragma unroll
+      for (int c = 0; c < 4 * NI; ++c) acc[r][c] *= keep;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (sees[w]) {  // a hidden value takes no part, not even times 0
+          const float p = exp2f((d[w] - ref) * kLog2e);
+          l[r] += p;
+#pragma unroll
+          for (int c = 0; c < 4 * NI; ++c) acc[r][c] = fmaf(p, vd[w][c], acc[r][c]);
+        }
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float top = m[r];
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float w = m[r] == -INFINITY ? (l[r] == 0.0f ? 0.0f : 1.0f) : exp2f((m[r] - top) * kLog2e);
+    float sum = l[r] * w;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+#pragma unroll
+    for (int c = 0; c < 4 * NI; ++c) {
+      float x = acc[r][c] * w;
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (lane < 8) joined[warp][r][4 * l8 + 32 * (c / 4) + c % 4] = x;
+    }
+    if (lane == 0) joined[warp][r][kDims] = top, joined[warp][r][kDims + 1] = sum;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
+    const int r = i / kDims, c = i % kDims, row = rb * R + r;
+    if (row >= total || c >= s.head_dim) continue;
+    const int h = g * group + row / s.q_len, qr = row % s.q_len;
+    float top = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, joined[w][r][kDims]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float one = joined[w][r][kDims] == top ? 1.0f : exp2f((joined[w][r][kDims] - top) * kLog2e);
+      sum += joined[w][r][kDims + 1] * one;
+      x += joined[w][r][c] * one;
+    }
+    const int64_t line = ((int64_t)b * s.heads + h) * s.q_len + qr;
+    if (splits == 1) {
+      out[row_at(s, b, h, qr, s.heads, s.q_len) + c] = sum == 0.0f ? 0.0f : x / sum;
+      if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = make_float2(top, sum);
+    } else {
+      float* dst = part + (line * splits + split) * (s.head_dim + 2);
+      dst[2 + c] = x;
+      if (c == 0) dst[0] = top, dst[1] = sum;
+    }
+  }
+}
+
+// One warp per row joins its splits in order.
+__global__ void __launch_bounds__(128) decode_join_kernel(AttentionShape s, const float* __restrict__ part,
+                                                          float* __restrict__ out, float* __restrict__ stats,
+                                                          int splits) {
+  const int64_t line = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (line >= (int64_t)s.batch * s.heads * s.q_len) return;
+  const int lane = threadIdx.x & 31;
+  const int r = (int)(line % s.q_len), h = (int)(line / s.q_len % s.heads), b = (int)(line / s.q_len / s.heads);
+  const float* src = part + line * splits * (s.head_dim + 2);
+  float top = -INFINITY;
+  for (int i = lane; i < splits; i += 32) top = fmaxf(top, src[(int64_t)i * (s.head_dim + 2)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.0f, x[kLaneDims] = {};
+#pragma unroll 4
+  for (int i = 0; i < splits; ++i) {
+    const float* p = src + (int64_t)i * (s.head_dim + 2);
+    const float one = p[0] == top ? 1.0f : exp2f((p[0] - top) * kLog2e);
+    sum += p[1] * one;
+#pragma unroll
+    for (int d = 0; d < kLaneDims; ++d)
+      if (lane + 32 * d < s.head_dim) x[d] += p[2 + lane + 32 * d] * one;
+  }
+  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, x, sum == 0.0f ? 0.0f : 1.0f / sum, 0);
+  if (stats != nullptr && lane == 0) *(float2*)(stats + 2 * line) = make_float2(top, sum);
+}
+
 }  // namespace
 
 namespace {
@@ -976,7 +1168,53 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   return w;
 }
 
-bool uses_tiles(const AttentionShape& s) { return s.q_len >= 16; }
+// Up to this many rows per key head go through decode_kernel.
+constexpr int64_t kFewRows = 16;
+bool uses_tiles(const AttentionShape& s) { return (int64_t)s.q_len * (s.heads / s.kv_heads) > kFewRows; }
+
+struct DecodePlan {
+  int rows, row_blocks, splits;
+};
+DecodePlan decode_plan(const AttentionShape& s) {
+  DecodePlan p;
+  const int total = s.q_len * (s.heads / s.kv_heads);
+  p.rows = total == 1 ? 1 : total <= 4 ? 4 : kDecodeRows;
+  p.row_blocks = (int)ceil_div(total, p.rows);
+  // About eight blocks of four warps per SM, none with fewer than 128 keys.
+  int64_t most = s.k_len;
+  if (s.window > 0) most = std::min<int64_t>(most, (int64_t)s.window + s.sinks + s.q_len - 1);
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks;
+  int64_t splits = std::min(ceil_div(kSms * 8, blocks > 0 ? blocks : 1), most / 128);
+  p.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
+  return p;
+}
+int64_t decode_work_elems(const AttentionShape& s) {
+  const DecodePlan p = decode_plan(s);
+  if (p.splits == 1) return 1;
+  return (int64_t)s.batch * s.heads * s.q_len * p.splits * (s.head_dim + 2);
+}
+
+template <int NI, int R>
+void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v, float* out,
+                float* stats, float* part, int* err, cudaStream_t st) {
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks * p.splits;
+  if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
+  const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+  if (vec)
+    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits,
+                                                                            p.row_blocks, err);
+  else
+    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits,
+                                                                             p.row_blocks, err);
+  check_launch();
+}
+template <int NI>
+void run_decode_rows(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v,
+                     float* out, float* stats, float* part, int* err, cudaStream_t st) {
+  if (p.rows == 1) run_decode<NI, 1>(s, p, q, k, v, out, stats, part, err, st);
+  else if (p.rows == 4) run_decode<NI, 4>(s, p, q, k, v, out, stats, part, err, st);
+  else run_decode<NI, kDecodeRows>(s, p, q, k, v, out, stats, part, err, st);
+}
 
 void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, cudaStream_t st) {
   PackJobs p{};
@@ -1007,7 +1245,7 @@ void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
 }  // namespace
 
 int64_t window_attention_work_elems(const AttentionShape& s) {
-  return uses_tiles(s) ? forward_work(s, nullptr).floats : 1;
+  return uses_tiles(s) ? forward_work(s, nullptr).floats : decode_work_elems(s);
 }
 int64_t window_attention_backward_work_elems(const AttentionShape&) { return 1; }
 
@@ -1026,8 +1264,17 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
     else run_forward<128>(a, err, st);
     return;
   }
-  simple_forward_kernel<<<(unsigned)ceil_div(rows, 8), 256, 0, st>>>(s, q, k, v, out, stats, err);
-  check_launch();
+  const DecodePlan p = decode_plan(s);
+  switch ((s.head_dim + 31) / 32) {
+    case 1: run_decode_rows<1>(s, p, q, k, v, out, stats, work, err, st); break;
+    case 2: run_decode_rows<2>(s, p, q, k, v, out, stats, work, err, st); break;
+    case 3: run_decode_rows<3>(s, p, q, k, v, out, stats, work, err, st); break;
+    default: run_decode_rows<4>(s, p, q, k, v, out, stats, work, err, st); break;
+  }
+  if (p.splits > 1) {
+    decode_join_kernel<<<(unsigned)ceil_div(rows, 4), 128, 0, st>>>(s, work, out, stats, p.splits);
+    check_launch();
+  }
 }
 
 void launch_window_attention_backward(const AttentionShape& s, const float* q, const float* k, const float* v,
