@@ -469,6 +469,15 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi, int first) {
   return (0xffffffffu >> (32 - (z - a))) << a;
 }
 
+// A row's statistics in natural units from its reference exponent (in powers
+// of two) and sum.  The sum takes up what rounding the exponent loses, so that
+// exp(score - greatest) / sum stays consistent.
+__device__ __forceinline__ float2 natural_stats(float top, float sum) {
+  if (top == -INFINITY) return make_float2(-INFINITY, sum);
+  const float m = top * kLn2;
+  return make_float2(m, sum * exp2f(top - m * kLog2e));
+}
+
 // The key tiles that a tile of query rows needs: [0, sinks) and then `low` on.
 struct TileRange {
   int sinks, low, count;
@@ -910,11 +919,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           if (c < cols) dst[c] = acc[c] * inv;
       }
       if (a.stats != nullptr && half == 0) {
-        // Natural units; the sum takes up what rounding the greatest score
-        // loses, so that the backward's 2^(s - max) / sum is consistent.
-        const float m = top == -INFINITY ? -INFINITY : (top + 14.0f) * kLn2;
-        const float z = top == -INFINITY ? 0.0f : l * exp2f(top - m * kLog2e);
-        *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = make_float2(m, z);
+        // p was 2^(s - top) with top 14 below the greatest score.
+        const float2 st = natural_stats(top == -INFINITY ? top : top + 14.0f, l * 0x1p-14f);
+        *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = st;
       }
       }
       __syncwarp();
@@ -940,13 +947,27 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 // at the end in a fixed order.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
+constexpr int kMostSplits = 512;
+
+// The keys that some row of a sequence sees: [0, first) and `count` - first
+// more from `low` on.
+struct SeenKeys {
+  int first, low, count;
+};
+__device__ __forceinline__ SeenKeys keys_of(const AttentionShape& s, const Sequence& q) {
+  const int a = max(q.start, 0), z = min(q.start + s.q_len, q.n);  // live positions [a, z)
+  if (a >= z) return {0, 0, 0};
+  const int low = s.window > 0 ? max(a + 1 - s.window, 0) : 0;
+  const int first = s.window > 0 ? min(s.sinks, low) : 0;
+  return {first, low, first + z - low};
+}
 
 template <int NI, int R, bool VEC>
 __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s, const float* __restrict__ q,
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
                                                                 float* __restrict__ stats, float* __restrict__ part,
-                                                                int splits, int row_blocks, int* err) {
+                                                                int splits, int per, int row_blocks, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ float qs[R][kDims];
   __shared__ float joined[kWarps][R][kDims + 2];
@@ -959,13 +980,11 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   const int g = (int)(index % s.kv_heads), b = (int)(index / s.kv_heads);
   const int group = s.heads / s.kv_heads, total = group * s.q_len;
   const Sequence sq = sequence_of(s, b, err);
-  // Keys that some row sees: [0, first) and [low, high), counted through.
-  const int a = max(sq.start, 0), z = min(sq.start + s.q_len, sq.n);  // live positions [a, z)
-  const int low = a < z && s.window > 0 ? max(a + 1 - s.window, 0) : 0;
-  const int first = a < z ? min(s.window > 0 ? s.sinks : 0, low) : 0;
-  const int keys = a < z ? first + z - low : 0;
-  const int per = ((keys + splits - 1) / splits + 31) / 32 * 32;
+  const SeenKeys seen = keys_of(s, sq);
+  const int first = seen.first, low = seen.low, keys = seen.count;
   const int u0 = min(keys, split * per), u1 = min(keys, u0 + per);
+  if (splits > 1 && u0 == u1 && split > 0) return;  // the join knows how many splits hold keys
+  const float to_log2 = s.scale * kLog2e;
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
     const int r = rb * R + i / kDims, c = i % kDims;
     qs[i / kDims][c] = r < total && c < s.head_dim
@@ -1033,24 +1052,26 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
         d[0] += __shfl_xor_sync(lanes, d[0], o);
         d[1] += __shfl_xor_sync(lanes, d[1], o);
       }
-      bool sees[2];
+      bool sees[2] = {true, two};
+      if (s.q_len > 1)
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        d[w] *= s.scale;
-        sees[w] = (w == 0 || two) && j[w] <= at[r] && (s.window == 0 || at[r] - j[w] < s.window || j[w] < s.sinks);
-        if (!sees[w]) d[w] = -INFINITY;
+        for (int w = 0; w < 2; ++w)
+          sees[w] = sees[w] && j[w] <= at[r] && (s.window == 0 || at[r] - j[w] < s.window || j[w] < s.sinks);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) d[w] = sees[w] ? d[w] * to_log2 : -INFINITY;
+      const float top = fmaxf(d[0], d[1]);
+      if (top > m[r]) {  // seldom after a row's first keys
+        const float keep = exp2_fast(m[r] - top);
+        m[r] = top;
+        l[r] *= keep;
+#pragma unroll
+        for (int c = 0; c < 4 * NI; ++c) acc[r][c] *= keep;
       }
-      const float top = fmaxf(m[r], fmaxf(d[0], d[1]));
-      const float ref = top == -INFINITY ? 0.0f : top;
-      const float keep = exp2f((m[r] - ref) * kLog2e);
-      m[r] = top;
-      l[r] *= keep;
-#pragma unroll
-      for (int c = 0; c < 4 * NI; ++c) acc[r][c] *= keep;
+      const float ref = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
       for (int w = 0; w < 2; ++w)
         if (sees[w]) {  // a hidden value takes no part, not even times 0
-          const float p = exp2f((d[w] - ref) * kLog2e);
+          const float p = exp2_fast(d[w] - ref);
           l[r] += p;
 #pragma unroll
           for (int c = 0; c < 4 * NI; ++c) acc[r][c] = fmaf(p, vd[w][c], acc[r][c]);
@@ -1063,7 +1084,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     float top = m[r];
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-    const float w = m[r] == -INFINITY ? (l[r] == 0.0f ? 0.0f : 1.0f) : exp2f((m[r] - top) * kLog2e);
+    const float w = m[r] == -INFINITY ? (l[r] == 0.0f ? 0.0f : 1.0f) : exp2_fast(m[r] - top);
     float sum = l[r] * w;
     sum += __shfl_xor_sync(0xffffffffu, sum, 8);
     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
@@ -1086,14 +1107,14 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, joined[w][r][kDims]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float one = joined[w][r][kDims] == top ? 1.0f : exp2f((joined[w][r][kDims] - top) * kLog2e);
+      const float one = joined[w][r][kDims] == top ? 1.0f : exp2_fast(joined[w][r][kDims] - top);
       sum += joined[w][r][kDims + 1] * one;
       x += joined[w][r][c] * one;
     }
     const int64_t line = ((int64_t)b * s.heads + h) * s.q_len + qr;
     if (splits == 1) {
       out[row_at(s, b, h, qr, s.heads, s.q_len) + c] = sum == 0.0f ? 0.0f : x / sum;
-      if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = make_float2(top, sum);
+      if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = natural_stats(top, sum);
     } else {
       float* dst = part + (line * splits + split) * (s.head_dim + 2);
       dst[2 + c] = x;
@@ -1102,31 +1123,45 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   }
 }
 
-// One warp per row joins its splits in order.
+// One block per row joins its splits: each warp takes every fourth, the warps'
+// parts are added in order.
 __global__ void __launch_bounds__(128) decode_join_kernel(AttentionShape s, const float* __restrict__ part,
                                                           float* __restrict__ out, float* __restrict__ stats,
-                                                          int splits) {
-  const int64_t line = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (line >= (int64_t)s.batch * s.heads * s.q_len) return;
-  const int lane = threadIdx.x & 31;
+                                                          int splits, int per, int* err) {
+  __shared__ float weight[kMostSplits], joined[4][kMaxHeadDim], tops[4], sums[4];
+  const int64_t line = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = (int)(line % s.q_len), h = (int)(line / s.q_len % s.heads), b = (int)(line / s.q_len / s.heads);
+  const int used = max(1, (keys_of(s, sequence_of(s, b, err)).count + per - 1) / per);
   const float* src = part + line * splits * (s.head_dim + 2);
   float top = -INFINITY;
-  for (int i = lane; i < splits; i += 32) top = fmaxf(top, src[(int64_t)i * (s.head_dim + 2)]);
+  for (int i = threadIdx.x; i < used; i += 128) top = fmaxf(top, weight[i] = src[(int64_t)i * (s.head_dim + 2)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   float sum = 0.0f, x[kLaneDims] = {};
 #pragma unroll 4
-  for (int i = 0; i < splits; ++i) {
+  for (int i = warp; i < used; i += 4) {
     const float* p = src + (int64_t)i * (s.head_dim + 2);
-    const float one = p[0] == top ? 1.0f : exp2f((p[0] - top) * kLog2e);
+    const float one = weight[i] == top ? 1.0f : exp2_fast(weight[i] - top);
     sum += p[1] * one;
 #pragma unroll
     for (int d = 0; d < kLaneDims; ++d)
       if (lane + 32 * d < s.head_dim) x[d] += p[2 + lane + 32 * d] * one;
   }
-  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, x, sum == 0.0f ? 0.0f : 1.0f / sum, 0);
-  if (stats != nullptr && lane == 0) *(float2*)(stats + 2 * line) = make_float2(top, sum);
+#pragma unroll
+  for (int d = 0; d < kLaneDims; ++d) joined[warp][lane + 32 * d] = x[d];
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  const int c = threadIdx.x;
+  if (c < s.head_dim) {
+    const float o = (joined[0][c] + joined[1][c]) + (joined[2][c] + joined[3][c]);
+    out[row_at(s, b, h, r, s.heads, s.q_len) + c] = sum == 0.0f ? 0.0f : o / sum;
+  }
+  if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = natural_stats(top, sum);
 }
 
 }  // namespace
@@ -1173,19 +1208,21 @@ constexpr int64_t kFewRows = 16;
 bool uses_tiles(const AttentionShape& s) { return (int64_t)s.q_len * (s.heads / s.kv_heads) > kFewRows; }
 
 struct DecodePlan {
-  int rows, row_blocks, splits;
+  int rows, row_blocks, splits, per;
 };
 DecodePlan decode_plan(const AttentionShape& s) {
   DecodePlan p;
   const int total = s.q_len * (s.heads / s.kv_heads);
   p.rows = total == 1 ? 1 : total <= 4 ? 4 : kDecodeRows;
   p.row_blocks = (int)ceil_div(total, p.rows);
-  // About eight blocks of four warps per SM, none with fewer than 128 keys.
+  // Each split takes the same number of keys, whatever its sequence's length:
+  // about six blocks per SM at full length, at least 256 keys each.
   int64_t most = s.k_len;
   if (s.window > 0) most = std::min<int64_t>(most, (int64_t)s.window + s.sinks + s.q_len - 1);
   const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks;
-  int64_t splits = std::min(ceil_div(kSms * 8, blocks > 0 ? blocks : 1), most / 128);
-  p.splits = (int)(splits < 1 ? 1 : splits > 512 ? 512 : splits);
+  const int64_t want = std::max<int64_t>(1, std::min(ceil_div(kSms * 6, blocks > 0 ? blocks : 1), most / 256));
+  p.per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(most, std::min<int64_t>(want, kMostSplits))), 32) * 32);
+  p.splits = (int)std::max<int64_t>(1, ceil_div(most, p.per));
   return p;
 }
 int64_t decode_work_elems(const AttentionShape& s) {
@@ -1201,10 +1238,10 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   if (vec)
-    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits,
+    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
                                                                             p.row_blocks, err);
   else
-    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits,
+    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
                                                                              p.row_blocks, err);
   check_launch();
 }
@@ -1272,7 +1309,8 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
     default: run_decode_rows<4>(s, p, q, k, v, out, stats, work, err, st); break;
   }
   if (p.splits > 1) {
-    decode_join_kernel<<<(unsigned)ceil_div(rows, 4), 128, 0, st>>>(s, work, out, stats, p.splits);
+    if (rows > INT_MAX) throw CudaError("window_attention: too many rows");
+    decode_join_kernel<<<(unsigned)rows, 128, 0, st>>>(s, work, out, stats, p.splits, p.per, err);
     check_launch();
   }
 }

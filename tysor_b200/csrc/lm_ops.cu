@@ -47,6 +47,23 @@ __device__ __forceinline__ void group_sum2(float& a, float& b, float2* red, int 
   }
 }
 
+// The sum of one value, likewise.
+template <int TPR>
+__device__ __forceinline__ float group_sum(float a, float* red, int group, int phase) {
+  a = warp_sum(a);
+  if (TPR > 32) {
+    constexpr int W = TPR / 32;
+    const int t = threadIdx.x % TPR;
+    float* r = red + phase * W;
+    if ((t & 31) == 0) r[t >> 5] = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+    a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) a += r[i];
+  }
+  return a;
+}
+
 // A thread's share of a row: NV float4 at columns 4 (t + i TPR), or, where a
 // row may start off a 16-byte boundary, 4 NV floats at columns t + i TPR.
 template <int TPR, int NV, bool VEC>
@@ -104,24 +121,23 @@ __global__ void __launch_bounds__(kThreads) layer_norm_kernel(const float* __res
                                                               float eps) {
   using Part = RowPart<TPR, NV, VEC>;
   constexpr int G = kThreads / TPR;
-  __shared__ float2 red[G][2 * (TPR > 32 ? TPR / 32 : 1)];
+  __shared__ float red[G][2 * (TPR > 32 ? TPR / 32 : 1)];
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const float inv = 1.0f / (float)width;
   for (int64_t r = (int64_t)blockIdx.x * G + group; r < rows; r += (int64_t)gridDim.x * G) {
     float v[Part::E];
     Part::load(x + r * width, width, t, v, 0.0f);
-    float s = 0.0f, none = 0.0f;
+    float s = 0.0f;
 #pragma unroll
     for (int e = 0; e < Part::E; ++e) s += v[e];
-    group_sum2<TPR>(s, none, red[group], group, 0);
-    const float mean = s / (float)width;
+    const float mean = group_sum<TPR>(s, red[group], group, 0) * inv;
     float q = 0.0f;
 #pragma unroll
     for (int e = 0; e < Part::E; ++e) {
       const float d = v[e] - mean;
       q += Part::col(t, e) < width ? d * d : 0.0f;
     }
-    group_sum2<TPR>(q, none, red[group], group, 1);
-    const float rstd = 1.0f / sqrtf(q / (float)width + eps);
+    const float rstd = rsqrtf(group_sum<TPR>(q, red[group], group, 1) * inv + eps);
     float w[Part::E];
     if (gain != nullptr) {
       Part::load(gain, width, t, w, 0.0f);
@@ -148,20 +164,18 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_kernel(const float* __re
                                                                const float* __restrict__ bias, float* __restrict__ y,
                                                                float* __restrict__ stats, int64_t rows,
                                                                int64_t width, float eps) {
-  __shared__ float2 red[64];
+  __shared__ float red[64];
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float* xr = x + r * width;
-    float s = 0.0f, none = 0.0f;
+    float s = 0.0f;
     for (int64_t c = threadIdx.x; c < width; c += 1024) s += xr[c];
-    group_sum2<1024>(s, none, red, 0, 0);
-    const float mean = s / (float)width;
+    const float mean = group_sum<1024>(s, red, 0, 0) / (float)width;
     float q = 0.0f;
     for (int64_t c = threadIdx.x; c < width; c += 1024) {
       const float d = xr[c] - mean;
       q += d * d;
     }
-    group_sum2<1024>(q, none, red, 0, 1);
-    const float rstd = 1.0f / sqrtf(q / (float)width + eps);
+    const float rstd = rsqrtf(group_sum<1024>(q, red, 0, 1) / (float)width + eps);
     for (int64_t c = threadIdx.x; c < width; c += 1024) {
       const float n = (xr[c] - mean) * rstd * (gain ? gain[c] : 1.0f);
       y[r * width + c] = bias ? n + bias[c] : n;
@@ -388,6 +402,13 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const float* __restrict_
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 2^x to about 2^-22, subnormal results as 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The index an id stands for: -1 for an absent entry.
 __device__ __forceinline__ int entry_id(float id, int64_t width, int* err) {
   if (id < 0.0f) return -1;
@@ -440,15 +461,15 @@ struct Online {
 __device__ __forceinline__ Online join(Online a, Online b, float c) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return {m, a.s + b.s};
-  return {m, a.s * exp2f((a.m - m) * c) + b.s * exp2f((b.m - m) * c)};
+  return {m, a.s * exp2_fast((a.m - m) * c) + b.s * exp2_fast((b.m - m) * c)};
 }
 
 __device__ __forceinline__ void take(Online& o, float v, float c) {
   if (v > o.m) {
-    o.s = o.s * exp2f((o.m - v) * c) + 1.0f;
+    o.s = o.s * exp2_fast((o.m - v) * c) + 1.0f;
     o.m = v;
   } else {
-    o.s += v == o.m && v == -INFINITY ? 0.0f : exp2f((v - o.m) * c);
+    o.s += v == o.m && v == -INFINITY ? 0.0f : exp2_fast((v - o.m) * c);
   }
 }
 
@@ -492,10 +513,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
       for (int u = 0; u < 4; ++u) bad |= f[u].x != f[u].x || f[u].y != f[u].y || f[u].z != f[u].z || f[u].w != f[u].w;
       continue;
     }
-    float s = o.s * exp2f((o.m - m) * c);
+    float s = o.s * exp2_fast((o.m - m) * c);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      s += (exp2f((f[u].x - m) * c) + exp2f((f[u].y - m) * c)) + (exp2f((f[u].z - m) * c) + exp2f((f[u].w - m) * c));
+      s += (exp2_fast((f[u].x - m) * c) + exp2_fast((f[u].y - m) * c)) + (exp2_fast((f[u].z - m) * c) + exp2_fast((f[u].w - m) * c));
     o.m = m;
     o.s = s;
   }
@@ -604,14 +625,14 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
       for (int u = 0; u < 4; ++u) old[u] = dst[i + u * kDistillThreads];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      float4 g = make_float4(coef * exp2f((f[u].x - st.x) * c), coef * exp2f((f[u].y - st.x) * c),
-                             coef * exp2f((f[u].z - st.x) * c), coef * exp2f((f[u].w - st.x) * c));
+      float4 g = make_float4(coef * exp2_fast((f[u].x - st.x) * c), coef * exp2_fast((f[u].y - st.x) * c),
+                             coef * exp2_fast((f[u].z - st.x) * c), coef * exp2_fast((f[u].w - st.x) * c));
       if (accumulate) g.x += old[u].x, g.y += old[u].y, g.z += old[u].z, g.w += old[u].w;
       dst[i + u * kDistillThreads] = g;
     }
   }
   auto one = [&](int64_t at) {
-    const float g = coef * exp2f((row[at] - st.x) * c);
+    const float g = coef * exp2_fast((row[at] - st.x) * c);
     out[at] = accumulate ? out[at] + g : g;
   };
   for (; i < quads; i += kDistillThreads) {
