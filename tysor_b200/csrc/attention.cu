@@ -232,6 +232,8 @@ __global__ void __launch_bounds__(256) simple_dkv_kernel(AttentionShape s, const
 // as the matrix unit's 128-byte swizzle wants them.  A copy of whole boxes, or
 // of 64 of their rows, is then one untiled bulk copy, and the same box serves
 // as an operand summed over its columns (scores) or over its rows (values).
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;
 constexpr int kBox = kTile * 128;  // bytes
 constexpr uint32_t kLayoutSW128 = 2;
@@ -248,9 +250,15 @@ struct PackJob {
   uint8_t* tiles;   // [batch][heads][tiles_of(len)] packed tiles
   float* factors;   // the power of two that undoes each tile's scale; NaN: a value is not finite
   int heads, len, queries;
-  // Queries' gradient only: delta[row] = sum of x * out over the row.
-  const float* out;
-  float* delta;
+  // For the gradients (all null otherwise), rows counted in whole tiles: the
+  // rows' 2-norms and each tile's greatest; and with the output and statistics
+  // (x is the output's gradient) each row's (greatest score in powers of two,
+  // 1 / sum, delta = sum of x * out, norm), zeros for rows that see nothing,
+  // and each tile's greatest |delta| (NaN if a row's values are not finite).
+  float *norm, *tile_norm;
+  const float *out, *stats;
+  float4* info;
+  float* tile_delta;
 };
 struct PackJobs {
   AttentionShape s;
@@ -277,13 +285,17 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   if (j.queries) v0 = -sq.start, v1 = sq.n - sq.start;
   const int r0 = max(t * kTile, v0), r1 = min(min(j.len, (t + 1) * kTile), v1);
   if (r0 >= r1) {  // nothing reads this tile's values
-    if (threadIdx.x == 0) j.factors[index] = 1.0f;
-    if (j.delta != nullptr)
-      for (int r = threadIdx.x; r < kTile && t * kTile + r < j.len; r += 256)
-        j.delta[((int64_t)b * j.heads + h) * j.len + t * kTile + r] = 0.0f;
+    if (threadIdx.x == 0) {
+      j.factors[index] = 1.0f;
+      if (j.tile_norm != nullptr) j.tile_norm[index] = 0.0f;
+      if (j.tile_delta != nullptr) j.tile_delta[index] = 0.0f;
+    }
+    if (j.info != nullptr && threadIdx.x < kTile)
+      j.info[(int64_t)index * kTile + threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (j.norm != nullptr && threadIdx.x < kTile) j.norm[(int64_t)index * kTile + threadIdx.x] = 0.0f;
     return;
   }
-  const bool vec = s.head_dim % 4 == 0 && ((uintptr_t)j.x & 15) == 0 && ((uintptr_t)j.out & 15) == 0;
+  const bool vec = s.head_dim % 4 == 0 && ((uintptr_t)j.x & 15) == 0;
   float v[kPer][8];
   uint32_t top = 0;
 #pragma unroll
@@ -305,22 +317,6 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
   }
-  if (j.delta != nullptr) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int item = threadIdx.x + 256 * i;
-      const int r = t * kTile + item / kChunks, c = item % kChunks * 8;
-      const float* src = j.out + row_at(s, b, h, r, j.heads, j.len) + c;
-      float d = 0.0f;
-      if (r >= r0 && r < r1)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < s.head_dim) d += v[i][e] * src[e];
-#pragma unroll
-      for (int o = kChunks / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (item % kChunks == 0 && r < j.len) j.delta[((int64_t)b * j.heads + h) * j.len + r] = d;
-    }
-  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = top;
@@ -333,10 +329,42 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   if (threadIdx.x == 0)
     j.factors[index] = exponent == 128 ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
+  float most_norm = 0.0f;
+  uint32_t most_delta = 0;  // as bits: NaN is the greatest
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int item = threadIdx.x + 256 * i;
     const int r = item / kChunks, chunk = item % kChunks;
+    if (j.norm != nullptr) {
+      const float back = __uint_as_float((uint32_t)(127 - up) << 23);
+      const int row = t * kTile + r;
+      const float* o = j.out != nullptr ? j.out + row_at(s, b, h, row, j.heads, j.len) + chunk * 8 : nullptr;
+      float q = 0.0f, d = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        q += v[i][e] * scale * (v[i][e] * scale);
+        if (o != nullptr && row >= r0 && row < r1 && chunk * 8 + e < s.head_dim) d += v[i][e] * o[e];
+      }
+#pragma unroll
+      for (int w = kChunks / 2; w > 0; w >>= 1) {
+        q += __shfl_xor_sync(0xffffffffu, q, w);
+        d += __shfl_xor_sync(0xffffffffu, d, w);
+      }
+      q = sqrtf(q) * back;
+      most_norm = fmaxf(most_norm, q);
+      if (chunk == 0) {
+        j.norm[(int64_t)index * kTile + r] = q;
+        if (j.info != nullptr) {
+          float2 st = make_float2(0.0f, 0.0f);
+          if (row >= r0 && row < r1) st = *(const float2*)(j.stats + 2 * (((int64_t)b * j.heads + h) * j.len + row));
+          const float4 f =
+              st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(st.x * kLog2e, 1.0f / st.y, d, q);
+          j.info[(int64_t)index * kTile + r] = f;
+          const float all = f.x * 0.0f + f.y * 0.0f + f.z * 0.0f;  // 0, or NaN if one is not finite
+          most_delta = max(most_delta, __float_as_uint(fabsf(f.z) + all) & 0x7fffffffu);
+        }
+      }
+    }
     uint4 hi, lo;
     uint32_t* hw = &hi.x;
     uint32_t* lw = &lo.x;
@@ -352,6 +380,20 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     uint8_t* at = dst + (chunk / 8) * kBox + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
     *(uint4*)at = hi;
     *(uint4*)(at + (DP / 64) * kBox) = lo;
+  }
+  if (j.norm == nullptr) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
+    most_delta = max(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+  }
+  __shared__ uint32_t tops[2][8];  // both as bits of numbers that are not negative
+  if ((threadIdx.x & 31) == 0) tops[0][threadIdx.x >> 5] = __float_as_uint(most_norm), tops[1][threadIdx.x >> 5] = most_delta;
+  __syncthreads();
+  if (threadIdx.x < 2 && (threadIdx.x == 0 || j.tile_delta != nullptr)) {
+    uint32_t m = 0;
+    for (int w = 0; w < 8; ++w) m = max(m, tops[threadIdx.x][w]);
+    (threadIdx.x == 0 ? j.tile_norm : j.tile_delta)[index] = __uint_as_float(m);
   }
 }
 
@@ -414,6 +456,17 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_ld32(uint32_t at, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
   uint32_t r[64];
   asm volatile(
@@ -458,9 +511,6 @@ __device__ __forceinline__ void split32(const float* v, uint32_t (&r)[32]) {
 }
 // Column of the t-th 16 terms' hi part in such an operand (lo: 16 further).
 __device__ __forceinline__ uint32_t split_col(int t) { return (uint32_t)((t >> 1) * 32 + (t & 1) * 8); }
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // Bits e with lo <= first + e < hi.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi, int first) {
@@ -936,6 +986,520 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   }
 }
 
+// ---- gradients ------------------------------------------------------------------------------
+
+// Three passes of one pipeline, each summing its own gradient in a fixed order
+// (one pass for all three would have to add into dq from many blocks):
+//
+//   pass      rows (resident)   columns (streamed)   second product   summed
+//   kGradQ    queries: Q, dO    keys: K, V           dP = dO.V^T      dq += dS.K
+//   kGradK    keys: K, V        queries: Q, dO       dP^T = V.dO^T    dk += dS^T.Q
+//   kGradV    keys: K           queries: Q, dO       none             dv += P^T.dO
+//
+// A work item is 128 rows; its columns come in steps of 64.  Each step forms
+// the scores (and dP), then P = 2^(score - max) / sum and dS = P (dP - delta)
+// replace the scores as fp16 halves, an operand for the step's third product,
+// which is added to fp32 registers.  dS is brought near 2^15 by a power of two
+// from |dS| <= |dO_i| |V_j| + |delta_i|, with the norms of single rows on the
+// resident side and a tile's greatest on the streamed one.
+// Roles as in forward_kernel.  Shared memory holds the resident tiles and a
+// ring of two steps of the operand that is used twice; its lo half is used,
+// and freed, first, so that the next step's copies have started before the
+// last product ends.
+enum GradPass { kGradQ, kGradK, kGradV };
+constexpr int kStep = 64;
+constexpr int kStepBox = kStep * 128;  // bytes of 64 rows of a box
+
+struct GradArgs {
+  AttentionShape s;
+  const float *q, *k, *v, *out, *stats, *dout;
+  const uint8_t *pq, *pk, *pv, *po;
+  const float *fq, *fk, *fv, *fo;      // factors
+  const float *nv, *tnv, *tno, *tdo;   // norms of V's rows; greatest norm of V's and dO's tiles, greatest |delta|
+  const float4* info;                  // of query rows
+  float *dq, *dk, *dv;
+  int add_q, add_k, add_v;
+};
+
+template <int DP, int PASS>
+struct GradPlan {
+  static constexpr int kHalves = DP / 64;
+  static constexpr bool kTwo = PASS != kGradV;           // dP is needed
+  static constexpr int kPart = kHalves * kStepBox;       // a step's hi or lo half
+  static constexpr int kFirstSteps = 2;                  // ring of the operand of the scores
+  static constexpr int kSecondSteps = PASS == kGradV ? 2 : 1;
+  static constexpr int kResident = (kTwo ? 2 : 1) * kTileBytes<DP>;
+  static constexpr int kInfo = PASS == kGradQ ? 0 : 2 * kStep * 16;
+  static constexpr int kRing = 2 * (kFirstSteps + kSecondSteps);  // half steps
+  static constexpr int kSmem = kResident + kRing * kPart + kInfo + 512;
+  static_assert(kSmem <= 227 * 1024, "shared memory of one block");
+};
+
+// 128 rows of one head and the steps of 64 columns they need.
+struct GradItem {
+  int b, h, g, r0, n;  // h: kGradQ's head; n: steps (per head: kGradK, kGradV); 0: none, or values not finite
+  Sequence sq;
+  RowRange rows;       // kGradQ
+  TileRange range;     // in steps of 64
+  int row_tile;        // index of the resident tile
+};
+
+template <int PASS>
+__device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int* err) {
+  const AttentionShape& s = a.s;
+  GradItem t;
+  const int group = s.heads / s.kv_heads, lane = threadIdx.x & 31;
+  const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
+  float sum;
+  if (PASS == kGradQ) {
+    const int tq = tiles_q - 1 - index / (s.heads * s.batch);
+    t.h = index % s.heads;
+    t.b = index / s.heads % s.batch;
+    t.g = t.h / group;
+    t.r0 = tq * kTile;
+    t.sq = sequence_of(s, t.b, err);
+    t.rows = rows_of(s, t.sq, t.r0);
+    t.row_tile = (t.b * s.heads + t.h) * tiles_q + tq;
+    const int x = max(t.rows.p0, 0), z = min(t.rows.p1, t.sq.n - 1);
+    const int low = s.window > 0 ? max(x + 1 - s.window, 0) : 0;
+    t.range.low = low / kStep;
+    t.range.sinks = min((min(s.sinks, low) + kStep - 1) / kStep, t.range.low);
+    t.range.count = x > z ? 0 : t.range.sinks + z / kStep - t.range.low + 1;
+    sum = a.fq[t.row_tile] + a.fo[t.row_tile];
+    const int first = (t.b * s.kv_heads + t.g) * tiles_k;
+    for (int i = lane; i < t.range.count; i += 32) {
+      const int k = first + t.range.at(i) / 2;
+      sum += a.fk[k] + a.fv[k];
+    }
+  } else {
+    // The first keys are seen by the most queries.
+    const int tk = index / (s.kv_heads * s.batch);
+    t.g = index % s.kv_heads;
+    t.b = index / s.kv_heads % s.batch;
+    t.h = t.g * group;
+    t.r0 = tk * kTile;
+    t.sq = sequence_of(s, t.b, err);
+    t.rows = {0, 0, false};
+    t.row_tile = (t.b * s.kv_heads + t.g) * tiles_k + tk;
+    // Rows that see some key of the tile: positions from the first key on, up
+    // to where the last key leaves the window (none leaves it among the sinks).
+    const int last = min(t.r0 + kTile, t.sq.n) - 1;
+    int end = t.sq.n;
+    if (s.window > 0 && t.r0 >= s.sinks && end - last > s.window) end = last + s.window;
+    const int x = max(t.r0 - t.sq.start, 0), z = min(end - t.sq.start, s.q_len) - 1;
+    t.range.sinks = 0;
+    t.range.low = x / kStep;
+    t.range.count = t.r0 >= t.sq.n || x > z ? 0 : z / kStep - t.range.low + 1;
+    sum = a.fk[t.row_tile] + a.fv[t.row_tile];
+    for (int i = lane; i < t.range.count * group; i += 32) {
+      const int q = (t.b * s.heads + t.h + i / t.range.count) * tiles_q + t.range.at(i % t.range.count) / 2;
+      sum += a.fq[q] + a.fo[q] + a.tdo[q] * 0.0f;
+    }
+  }
+  t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  return t;
+}
+
+// The power of two (its exponent) that brings values up to `bound` below 2^15.
+__device__ __forceinline__ int scale_exponent(float bound) {
+  const int e = (int)(__float_as_uint(bound) >> 23 & 255u) - 127;
+  return bound == 0.0f ? 0 : min(max(14 - e, -126), 126);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+template <int DP, int PASS>
+__global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
+  using Plan = GradPlan<DP, PASS>;
+  constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart;
+  constexpr bool kTwo = Plan::kTwo;
+  const AttentionShape& s = a.s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = s.heads / s.kv_heads, heads = PASS == kGradQ ? 1 : group;  // heads an item walks
+  const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_u32(smem);
+  if ((base & 1023u) != 0) {  // the swizzle needs it; with no static shared memory it always holds
+    if (threadIdx.x == 0) atomicCAS(err, 0, (int)kErrTmemAlloc);
+    return;
+  }
+  const uint32_t ring1 = base + Plan::kResident, ring2 = ring1 + 2 * Plan::kFirstSteps * kPart;
+  uint8_t* info_smem = smem + Plan::kResident + Plan::kRing * kPart;
+  uint64_t* bars = (uint64_t*)(info_smem + Plan::kInfo);
+  constexpr int kHalves1 = 2 * Plan::kFirstSteps, kHalves2 = 2 * Plan::kSecondSteps;  // ring entries (half steps)
+  const uint32_t a_full = smem_u32(bars), a_empty = a_full + 8;
+  const uint32_t full1 = a_empty + 8, empty1 = full1 + 8 * kHalves1, full2 = empty1 + 8 * kHalves1;
+  const uint32_t empty2 = full2 + 8 * kHalves2, s_full = empty2 + 8 * kHalves2, p_full = s_full + 16;
+  const uint32_t o_full = p_full + 16, o_empty = o_full + 16, drained = o_empty + 16;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 + 2 * kHalves1 + 2 * kHalves2 + 9);
+  if (threadIdx.x == 0) {
+    mbar_init(a_full, 1);
+    mbar_init(a_empty, 1);
+    for (int i = 0; i < kHalves1; ++i) mbar_init(full1 + 8 * i, 1), mbar_init(empty1 + 8 * i, 1);
+    for (int i = 0; i < kHalves2; ++i) mbar_init(full2 + 8 * i, 1), mbar_init(empty2 + 8 * i, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 8);
+      mbar_init(o_full + 8 * i, 1);
+      mbar_init(o_empty + 8 * i, 8);
+    }
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 17) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // Tensor memory: two buffers of (scores, dP) of 64 columns each, two of DP for the step's sums.
+  const uint32_t tmem = *tmem_slot;
+
+  // Index of the streamed tile of step i of head x of an item.
+  auto column_tile = [&](const GradItem& t, int x, int i) {
+    return PASS == kGradQ ? (t.b * s.kv_heads + t.g) * tiles_k + t.range.at(i) / 2
+                          : (t.b * s.heads + t.h + x) * tiles_q + t.range.at(i) / 2;
+  };
+
+  if (warp >= 18) {
+    fewer_registers<kFewRegs>();
+  } else if (warp == 16) {
+    fewer_registers<kFewRegs>();
+    uint32_t it1 = 0, it2 = 0, loaded = 0;  // half steps, resident tiles
+    bool ok = true;
+    // Half `part` (0: lo, 1: hi) of 64 rows of a packed tile.
+    auto half = [&](uint32_t dst, uint32_t full, const uint8_t* tile, int step, int part) {
+#pragma unroll
+      for (int x = 0; x < kHalves; ++x)
+        bulk_load(dst + x * kStepBox, tile + ((1 - part) * kHalves + x) * kBox + (step & 1) * kStepBox, kStepBox, full);
+    };
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const GradItem t = grad_item<PASS>(a, w, err);
+      if (lane == 0 && t.n > 0) {
+        if (loaded > 0) ok = mbar_wait(a_empty, (loaded - 1) & 1, err);
+        if (ok) {
+          mbar_expect_tx(a_full, Plan::kResident);
+          const int64_t at = (int64_t)t.row_tile * kTileBytes<DP>;
+          bulk_load(base, (PASS == kGradQ ? a.pq : a.pk) + at, kTileBytes<DP>, a_full);
+          if (kTwo) bulk_load(base + kTileBytes<DP>, (PASS == kGradQ ? a.po : a.pv) + at, kTileBytes<DP>, a_full);
+          ++loaded;
+        }
+        for (int x = 0; x < heads && ok; ++x)
+          for (int i = 0; i < t.n && ok; ++i) {
+            const int tile = column_tile(t, x, i), step = t.range.at(i);
+            const uint8_t* one = (PASS == kGradQ ? a.pk : a.pq) + (int64_t)tile * kTileBytes<DP>;
+            const uint8_t* two = (PASS == kGradQ ? a.pv : a.po) + (int64_t)tile * kTileBytes<DP>;
+            for (int part = 0; part < 2 && ok; ++part, ++it1) {
+              const uint32_t slot = it1 % kHalves1, use = it1 / kHalves1;
+              if (use > 0) ok = mbar_wait(empty1 + 8 * slot, (use - 1) & 1, err);
+              if (!ok) break;
+              // kGradK: the rows' statistics come with the operand that stays until they have been used.
+              const bool with_info = PASS == kGradK && part == 1;
+              mbar_expect_tx(full1 + 8 * slot, kPart + (with_info ? kStep * 16 : 0));
+              half(ring1 + slot * kPart, full1 + 8 * slot, one, step, part);
+              if (with_info)
+                bulk_load(smem_u32(info_smem) + (it1 / 2 & 1) * (kStep * 16),
+                          (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16,
+                          full1 + 8 * slot);
+            }
+            for (int part = 0; part < 2 && ok; ++part, ++it2) {
+              const uint32_t slot = it2 % kHalves2, use = it2 / kHalves2;
+              if (use > 0) ok = mbar_wait(empty2 + 8 * slot, (use - 1) & 1, err);
+              if (!ok) break;
+              const bool with_info = PASS == kGradV && part == 1;
+              mbar_expect_tx(full2 + 8 * slot, kPart + (with_info ? kStep * 16 : 0));
+              half(ring2 + slot * kPart, full2 + 8 * slot, two, step, part);
+              if (with_info)
+                bulk_load(smem_u32(info_smem) + (it2 / 2 & 1) * (kStep * 16),
+                          (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16,
+                          full2 + 8 * slot);
+            }
+          }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+    if (lane == 0 && !ok) {  // copies in flight end before the block does
+      if (loaded > 0) mbar_wait(a_full, (loaded - 1) & 1, err);
+      for (uint32_t f = it1 > kHalves1 ? it1 - kHalves1 : 0; f < it1; ++f)
+        mbar_wait(full1 + 8 * (f % kHalves1), (f / kHalves1) & 1, err);
+      for (uint32_t f = it2 > kHalves2 ? it2 - kHalves2 : 0; f < it2; ++f)
+        mbar_wait(full2 + 8 * (f % kHalves2), (f / kHalves2) & 1, err);
+    }
+  } else if (warp == 17) {
+    fewer_registers<kFewRegs>();
+    constexpr uint32_t kScore = umma_idesc(kStep, false), kSum = umma_idesc(DP, true);
+    uint32_t gi = 0, item = 0;  // steps and items issued so far
+    bool ok = true;
+    // D = resident tile . (64 columns of a half-step ring)^T; `release`: the ring's entries are free after it.
+    auto scores = [&](uint32_t d, uint32_t rows, uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries,
+                      bool release) {
+      for (uint32_t part = 0; part < 2 && ok; ++part) {
+        const uint32_t entry = 2 * gi + part, slot = entry % entries;
+        ok = mbar_wait(full + 8 * slot, (entry / entries) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < kHalves; ++x) {
+          const uint32_t r = column_word(rows + x * kBox), c = column_word(ring + slot * kPart + x * kStepBox);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t rh = r + k * kColumnStep, rl = rh + (kHalves * kBox >> 4), ch = c + k * kColumnStep;
+            if (part == 0) {
+              umma_ss(d, rh, ch, kScore, x != 0 || k != 0);
+            } else {
+              umma_ss(d, rl, ch, kScore, 1u);
+              umma_ss(d, rh, ch, kScore, 1u);
+            }
+          }
+        }
+        if (release) umma_commit(empty + 8 * slot);
+      }
+    };
+    // The sums of step t: P or dS (in tensor memory) times the 64 rows of a ring step.
+    auto sums = [&](uint32_t t) {
+      const int buf = t & 1;
+      const uint32_t p = tmem + buf * 2 * kStep, d = tmem + 4 * kStep + buf * DP;
+      const uint32_t ring = PASS == kGradV ? ring2 : ring1, full = PASS == kGradV ? full2 : full1;
+      const uint32_t empty = PASS == kGradV ? empty2 : empty1, entries = PASS == kGradV ? kHalves2 : kHalves1;
+      ok = mbar_wait(p_full + 8 * buf, (t >> 1) & 1, err);
+      if (ok && t >= 2) ok = mbar_wait(o_empty + 8 * buf, ((t >> 1) - 1) & 1, err);
+      for (uint32_t part = 0; part < 2 && ok; ++part) {
+        const uint32_t entry = 2 * t + part, slot = entry % entries;
+        ok = mbar_wait(full + 8 * slot, (entry / entries) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t c = row_word(ring + slot * kPart, kStepBox);
+#pragma unroll
+        for (int k = 0; k < kStep / 16; ++k) {
+          const uint32_t ph = p + split_col(k), ch = c + k * kRowStep;
+          if (part == 0) {
+            umma_ts(d, ph, ch, kSum, k != 0);
+          } else {
+            umma_ts(d, ph + 16, ch, kSum, 1u);
+            umma_ts(d, ph, ch, kSum, 1u);
+          }
+        }
+        umma_commit(empty + 8 * slot);
+      }
+      if (ok) umma_commit(o_full + 8 * buf);
+    };
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const GradItem t = grad_item<PASS>(a, w, err);
+      if (lane == 0 && t.n > 0) {
+        ok = mbar_wait(a_full, item & 1, err);
+        ++item;
+        const int steps = heads * t.n;
+        for (int i = 0; i < steps && ok; ++i, ++gi) {
+          const uint32_t d = tmem + (gi & 1) * 2 * kStep;
+          scores(d, base, ring1, full1, empty1, kHalves1, PASS == kGradV);
+          if (kTwo && ok) scores(d + kStep, base + kTileBytes<DP>, ring2, full2, empty2, kHalves2, true);
+          if (!ok) break;
+          umma_commit(s_full + 8 * (gi & 1));
+          if (i == steps - 1) umma_commit(a_empty);
+          if (gi > 0) sums(gi - 1);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+    }
+    if (lane == 0) {
+      if (ok && gi > 0) sums(gi - 1);
+      if (!ok) {  // instructions in flight end before the block does
+        umma_commit(drained);
+        mbar_wait(drained, 0, err);
+      }
+    }
+  } else if (warp < 8) {
+    more_registers<kScoreRegs>();
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 32;
+    uint32_t gi = 0;
+    bool ok = true;
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const GradItem t = grad_item<PASS>(a, w, err);
+      if (t.n == 0) {
+        if (PASS == kGradQ)
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
+            simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
+        if (PASS == kGradK)  // and dv, which kGradV leaves out
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 8)
+            simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
+        continue;
+      }
+      // kGradQ: what the row sees and its statistics; else the key's rows [s0, s1) and its norm.
+      RowMask mask = {0, 0, 0};
+      float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      int s0 = 0, s1 = 0;
+      float norm = 0.0f;
+      if (PASS == kGradQ) {
+        QueryItem q;
+        q.rows = t.rows, q.sq = t.sq, q.r0 = t.r0;
+        mask = mask_of(s, q, row);
+        st = a.info[(int64_t)t.row_tile * kTile + row];
+        norm = st.w;
+      } else {
+        if (t.r0 + row < t.sq.n) rows_seeing(s, t.sq, t.r0 + row, &s0, &s1);
+        if (kTwo) norm = a.nv[(int64_t)t.row_tile * kTile + row];
+      }
+      const float* f_row1 = PASS == kGradQ ? a.fq : a.fk;
+      const double to_log2 = (double)f_row1[t.row_tile] * (double)s.scale * 1.4426950408889634;
+      const float f_row2 = PASS == kGradQ ? a.fo[t.row_tile] : kTwo ? a.fv[t.row_tile] : 0.0f;
+      for (int x = 0; x < heads && ok; ++x)
+        for (int i = 0; i < t.n; ++i, ++gi) {
+          const int buf = gi & 1, step = t.range.at(i), tile = column_tile(t, x, i), c0 = step * kStep;
+          const float f = (float)(to_log2 * (double)(PASS == kGradQ ? a.fk : a.fq)[tile]);
+          bool whole;
+          uint32_t seen = 0xffffffffu;
+          if (PASS == kGradQ) {
+            whole = t.rows.all && c0 + kStep - 1 <= t.rows.p0 &&
+                    (s.window == 0 || t.rows.p1 - c0 < s.window || c0 + kStep <= s.sinks);
+            if (!whole) seen = seen_bits(mask, c0 + 32 * half);
+          } else {
+            const int first = t.sq.start + c0, last = first + kStep - 1, k1 = t.r0 + kTile - 1;
+            whole = k1 <= first && last < t.sq.n && c0 + kStep <= s.q_len &&
+                    (s.window == 0 || last - t.r0 < s.window || k1 < s.sinks);
+            if (!whole) seen = bits_between(s0, s1, c0 + 32 * half);
+          }
+          float up = 16384.0f;  // P <= 1
+          float f2 = 0.0f;
+          if (kTwo) {
+            const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] +
+                                (PASS == kGradQ ? fabsf(st.z) : a.tdo[tile]);
+            up = power_of_two(scale_exponent(bound));
+            f2 = f_row2 * (PASS == kGradQ ? a.fv : a.fo)[tile];
+          }
+          ok = warp_wait(s_full + 8 * buf, (gi >> 1) & 1, err);
+          if (PASS != kGradQ && ok) {  // the statistics' copy, with the second half of its step
+            const uint32_t entries = PASS == kGradV ? kHalves2 : kHalves1, entry = 2 * gi + 1;
+            ok = warp_wait((PASS == kGradV ? full2 : full1) + 8 * (entry % entries), (entry / entries) & 1, err);
+          }
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t here = at + buf * 2 * kStep;
+          float v[32];
+          tmem_ld32(here, v);
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1u)) v[e] = -INFINITY;
+          }
+          const float4* col = (const float4*)(info_smem + buf * (kStep * 16)) + 32 * half;
+          if (kTwo) {
+            float d[32];
+            tmem_ld32(here + kStep, d);
+            const float scaled = st.y * up;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              if (PASS == kGradQ) {
+                v[e] = exp2_fast(fmaf(v[e], f, -st.x)) * scaled * fmaf(d[e], f2, -st.z);
+              } else {
+                const float4 c = col[e];
+                v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up) * fmaf(d[e], f2, -c.z);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float2 c = *(const float2*)&col[e];
+              v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up);
+            }
+          }
+          uint32_t r[32];
+          split32(v, r);
+          tmem_st32(here, r);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full + 8 * buf);
+        }
+    }
+  } else {
+    fewer_registers<kOutputRegs>();
+    constexpr int kCols = DP / 2;  // columns of a thread
+    const int quad = warp & 3, half = (warp - 8) >> 2, row = quad * 32 + lane;
+    const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + 4 * kStep + half * kCols;
+    uint32_t gi = 0;
+    bool ok = true;
+    for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const GradItem t = grad_item<PASS>(a, w, err);
+      if (t.n == 0) continue;
+      float norm = 0.0f, delta = 0.0f;
+      if (PASS == kGradQ) {
+        const float4 st = a.info[(int64_t)t.row_tile * kTile + row];
+        norm = st.w;
+        delta = fabsf(st.z);
+      } else if (kTwo) {
+        norm = a.nv[(int64_t)t.row_tile * kTile + row];
+      }
+      float acc[kCols];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+      for (int x = 0; x < heads && ok; ++x)
+        for (int i = 0; i < t.n; ++i, ++gi) {
+          const int buf = gi & 1, tile = column_tile(t, x, i);
+          float down = 0x1p-14f * (PASS == kGradV ? a.fo[tile] : 1.0f);
+          if (kTwo) {
+            const float bound =
+                norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] + (PASS == kGradQ ? delta : a.tdo[tile]);
+            down = power_of_two(-scale_exponent(bound)) * (PASS == kGradQ ? a.fk : a.fq)[tile];
+          }
+          ok = warp_wait(o_full + 8 * buf, (gi >> 1) & 1, err);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < kCols; c += 16) {
+            float v[16];
+            tmem_ld16(at + buf * DP + c, v);
+            if (c == kCols - 16) {  // the last values are out: the buffer is free
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(o_empty + 8 * buf);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], down, acc[c + e]);
+          }
+        }
+      const int r = t.r0 + row;
+      if (ok && r < (PASS == kGradQ ? s.q_len : s.k_len)) {
+        const float by = PASS == kGradV ? 1.0f : s.scale;
+        float* out = PASS == kGradQ ? a.dq : PASS == kGradK ? a.dk : a.dv;
+        const int add = PASS == kGradQ ? a.add_q : PASS == kGradK ? a.add_k : a.add_v;
+        float* dst = out + half * kCols +
+                     (PASS == kGradQ ? row_at(s, t.b, t.h, r, s.heads, s.q_len) : row_at(s, t.b, t.g, r, s.kv_heads, s.k_len));
+        const int cols = s.head_dim - half * kCols;
+        if (s.head_dim % 4 == 0 && ((uintptr_t)out & 15) == 0) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 4)
+            if (c < cols) {
+              float4 o = make_float4(acc[c] * by, acc[c + 1] * by, acc[c + 2] * by, acc[c + 3] * by);
+              if (add) {
+                const float4 p = *(const float4*)(dst + c);
+                o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+              }
+              *(float4*)(dst + c) = o;
+            }
+        } else {
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+            if (c < cols) dst[c] = add ? dst[c] + acc[c] * by : acc[c] * by;
+        }
+      }
+      __syncwarp();
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 17) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
 // ---- a few query rows over a long cache ----------------------------------------------------
 
 // The rows that share a key head (at most R of them per block) go over its
@@ -1269,6 +1833,51 @@ void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, 
   check_launch();
 }
 
+struct GradWork {
+  uint8_t *pq, *pk, *pv, *po;
+  float *fq, *fk, *fv, *fo, *nv, *no, *tnv, *tno, *tdo;
+  float4* info;
+  int64_t floats;
+};
+GradWork grad_work(const AttentionShape& s, float* base) {
+  Carver c{base};
+  const int64_t tile = padded_dim(s) == 64 ? kTileBytes<64> / 4 : kTileBytes<128> / 4;
+  const int64_t nq = (int64_t)s.batch * s.heads * tiles_of(s.q_len), nk = (int64_t)s.batch * s.kv_heads * tiles_of(s.k_len);
+  GradWork w;
+  w.pq = (uint8_t*)c.take(nq * tile);
+  w.po = (uint8_t*)c.take(nq * tile);
+  w.pk = (uint8_t*)c.take(nk * tile);
+  w.pv = (uint8_t*)c.take(nk * tile);
+  w.fq = c.take(nq);
+  w.fo = c.take(nq);
+  w.fk = c.take(nk);
+  w.fv = c.take(nk);
+  w.nv = c.take(nk * kTile);
+  w.no = c.take(nq * kTile);
+  w.tnv = c.take(nk);
+  w.tno = c.take(nq);
+  w.tdo = c.take(nq);
+  w.info = (float4*)c.take(nq * kTile * 4);
+  w.floats = c.used;
+  return w;
+}
+
+// Below a tile's half in rows or keys the packing and the padded products cost
+// more than a warp per row.
+bool grads_use_tiles(const AttentionShape& s) { return s.q_len >= 16; }
+
+template <int DP, int PASS>
+void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
+  constexpr int kSmem = GradPlan<DP, PASS>::kSmem;
+  TYSOR_CUDA(cudaFuncSetAttribute(grad_kernel<DP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  const AttentionShape& s = a.s;
+  const int64_t items = PASS == kGradQ ? (int64_t)tiles_of(s.q_len) * s.heads * s.batch
+                                       : (int64_t)tiles_of(s.k_len) * s.kv_heads * s.batch;
+  if (items == 0) return;
+  grad_kernel<DP, PASS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
+  check_launch();
+}
+
 template <int DP>
 void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
   TYSOR_CUDA(cudaFuncSetAttribute(forward_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1284,7 +1893,9 @@ void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
 int64_t window_attention_work_elems(const AttentionShape& s) {
   return uses_tiles(s) ? forward_work(s, nullptr).floats : decode_work_elems(s);
 }
-int64_t window_attention_backward_work_elems(const AttentionShape&) { return 1; }
+int64_t window_attention_backward_work_elems(const AttentionShape& s) {
+  return grads_use_tiles(s) ? grad_work(s, nullptr).floats : 1;
+}
 
 void launch_window_attention(const AttentionShape& s, const float* q, const float* k, const float* v, float* out,
                              float* stats, float* work, int* err, cudaStream_t st) {
@@ -1292,9 +1903,9 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
   if (rows <= 0) return;
   if (uses_tiles(s)) {
     const ForwardWork w = forward_work(s, work);
-    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1, nullptr, nullptr},
-                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, nullptr, nullptr},
-                       {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, nullptr, nullptr}};
+    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
+                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
+                       {v, w.pv, w.fv, s.kv_heads, s.k_len, 0}};
     run_pack(s, jobs, 3, err, st);
     const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats};
     if (padded_dim(s) == 64) run_forward<64>(a, err, st);
@@ -1317,9 +1928,29 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
 
 void launch_window_attention_backward(const AttentionShape& s, const float* q, const float* k, const float* v,
                                       const float* out, const float* stats, const float* dout, float* dq, float* dk,
-                                      float* dv, float*, int accumulate_q, int accumulate_k, int accumulate_v,
+                                      float* dv, float* work, int accumulate_q, int accumulate_k, int accumulate_v,
                                       int* err, cudaStream_t st) {
   const int64_t rows = (int64_t)s.batch * s.heads * s.q_len, keys = (int64_t)s.batch * s.kv_heads * s.k_len;
+  if (rows > 0 && grads_use_tiles(s)) {
+    const GradWork w = grad_work(s, work);
+    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
+                       {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.tdo},
+                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
+                       {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
+    run_pack(s, jobs, 4, err, st);
+    const GradArgs a{s,    q,    k,    v,    out,  stats, dout,  w.pq,  w.pk,   w.pv, w.po, w.fq,         w.fk,
+                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v};
+    if (padded_dim(s) == 64) {
+      run_grad<64, kGradQ>(a, err, st);
+      run_grad<64, kGradK>(a, err, st);
+      run_grad<64, kGradV>(a, err, st);
+    } else {
+      run_grad<128, kGradQ>(a, err, st);
+      run_grad<128, kGradK>(a, err, st);
+      run_grad<128, kGradV>(a, err, st);
+    }
+    return;
+  }
   if (rows > 0) {
     simple_dq_kernel<<<(unsigned)ceil_div(rows, 8), 256, 0, st>>>(s, q, k, v, out, stats, dout, dq, accumulate_q, err);
     check_launch();
