@@ -410,21 +410,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* er
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
 
-// D (+)= A . B over 16 terms, fp16 operands, fp32 accumulator in tensor
-// memory; A from shared memory, or (a row per lane, two terms per column) from
-// tensor memory.
-// Descriptors of shared-memory operands come as their low words (see
-// column_word and row_word): the high one is the same for all, and the words
-// of an operand's steps lie constants apart.
+// D (+)= A . B over 16 terms, fp16 operands, fp32 accumulator; A (a row per
+// lane, two terms per column) and D in tensor memory, B in shared memory.  B's
+// descriptor comes as its low word (see column_word and row_word): the high one
+// is the same for all, and the words of an operand's steps lie constants apart.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (kLayoutSW128 << 29);  // 1024 bytes between 8-row groups
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 x, {%1, %3};\n\tmov.b64 y, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p;\n\t}\n" ::"r"(d),
-      "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(add));
-}
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
@@ -512,6 +502,28 @@ __device__ __forceinline__ void split32(const float* v, uint32_t (&r)[32]) {
 // Column of the t-th 16 terms' hi part in such an operand (lo: 16 further).
 __device__ __forceinline__ uint32_t split_col(int t) { return (uint32_t)((t >> 1) * 32 + (t & 1) * 8); }
 
+// A resident packed tile from shared memory into tensor memory, where it is the
+// A operand of every score product: one read instead of one per instruction
+// (an instruction reads A and B from shared memory at about 64 bytes a cycle,
+// so that with both there the reads, not the products, take the time: 90
+// cycles measured for 128 x 64 x 16 instead of 32).  Row r is lane r; its hi
+// columns are DP / 2 columns of tensor memory, its lo columns the DP / 2 after
+// them.  Called by the eight score warps; `half` is the warp's.
+template <int DP>
+__device__ __forceinline__ void rows_to_tmem(uint32_t tmem_rows, uint32_t tile, int row, int half) {
+#pragma unroll
+  for (int u = 0; u < DP / 64; ++u) {
+    const int unit = 2 * u + half;  // box of the tile: [hi | lo][DP / 64]
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r[4 * c]), "=r"(r[4 * c + 1]), "=r"(r[4 * c + 2]), "=r"(r[4 * c + 3])
+                   : "r"(tile + unit * kBox + row * 128 + ((c ^ (row & 7)) << 4)));
+    tmem_st32(tmem_rows + unit * 32, r);
+  }
+}
+
 // Bits e with lo <= first + e < hi.
 __device__ __forceinline__ uint32_t bits_between(int lo, int hi, int first) {
   const int a = min(max(lo - first, 0), 32), z = min(max(hi - first, 0), 32);
@@ -577,9 +589,11 @@ __device__ __forceinline__ bool sees_all(const AttentionShape& s, const RowRange
 //                brought to the greater of the two reference scores.  (An
 //                accumulator that stayed in tensor memory would lose up to a
 //                step per matrix instruction, always toward zero.)
-//   warp 16      copies packed tiles into a ring of 32 KB slots,
+//   warp 16      copies packed tiles: the next item's queries, and the keys and
+//                values into a ring of 32 KB slots,
 //   warp 17      issues the matrix instructions: the scores of a tile before
 //                the values of the one before it, so that the two overlap.
+// The query tile is kept in tensor memory (rows_to_tmem).
 constexpr int kThreads = 20 * 32;  // warps 18 and 19 only hold registers for the others
 constexpr int kSlotBytes = 2 * kBox;
 
@@ -619,10 +633,9 @@ struct QueryItem {
   int q_index, k_index;  // of the item's query tile and its head's first key tile
 };
 
-// Called by whole warps.  `others`: per-tile factors that have to be finite
-// besides fq, fk and fv (the gradient's), or null.
+// Called by whole warps.
 __device__ __forceinline__ QueryItem query_item(const AttentionShape& s, int index, const float* fq, const float* fk,
-                                                const float* fv, const float* others, int* err) {
+                                                const float* fv, int* err) {
   QueryItem t;
   const int tiles_q = tiles_of(s.q_len);
   const int tq = tiles_q - 1 - index / (s.heads * s.batch);
@@ -635,7 +648,7 @@ __device__ __forceinline__ QueryItem query_item(const AttentionShape& s, int ind
   t.range = keys_for(s, t.sq, t.rows);
   t.q_index = (t.b * s.heads + t.h) * tiles_q + tq;
   t.k_index = (t.b * s.kv_heads + t.g) * tiles_of(s.k_len);
-  float sum = fq[t.q_index] + (others != nullptr ? others[t.q_index] : 0.0f);
+  float sum = fq[t.q_index];
   for (int i = threadIdx.x & 31; i < t.range.count; i += 32)
     sum += fk[t.k_index + t.range.at(i)] + fv[t.k_index + t.range.at(i)];
   // A product with a hidden value that is not finite would not be 0: such
@@ -687,17 +700,20 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   uint64_t* bars = (uint64_t*)(most + 4 * kTile);
   const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8, slot_full = q_empty + 8;
   const uint32_t slot_empty = slot_full + 8 * Plan::kSlots, s_full = slot_empty + 8 * Plan::kSlots;
-  const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16, pair_full = o_empty + 16, drained = pair_full + 32;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 15);
+  const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16, st_empty = o_empty + 16;
+  const uint32_t pair_full = st_empty + 16, q_ready = pair_full + 32, drained = q_ready + 8;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 18);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 8);
+    mbar_init(q_ready, 8);
     for (int i = 0; i < Plan::kSlots; ++i) mbar_init(slot_full + 8 * i, 1), mbar_init(slot_empty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 8);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, 8);
+      mbar_init(st_empty + 8 * i, 8);
     }
     for (int i = 0; i < 4; ++i) mbar_init(pair_full + 8 * i, 2);
     mbar_init(drained, 1);
@@ -711,14 +727,14 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // Tensor memory: two buffers of scores (128 columns), two of values (DP).
-  const uint32_t tmem = *tmem_slot;
+  // Tensor memory: the query tile (DP columns), two buffers of scores (128 each) and of values (DP; one if DP is 128).
+  constexpr int kOut = DP == 64 ? 2 : 1;
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem + DP, tmem_o = tmem_s + 2 * kTile;
 
   if (warp >= 18) {
     fewer_registers<kFewRegs>();
   } else if (warp == 16) {
     fewer_registers<kFewRegs>();
-    const uint8_t* values = nullptr;  // the tile before's values
     uint32_t it = 0, loaded = 0;      // slots filled, query tiles loaded
     bool ok = true;
     auto fill = [&](const uint8_t* src, bool is_values) {
@@ -742,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
       if (lane == 0 && t.n > 0) {
         if (loaded > 0) ok = mbar_wait(q_empty, (loaded - 1) & 1, err);
         if (ok) {
@@ -750,22 +766,17 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           bulk_load(q_smem, a.pq + (int64_t)t.q_index * kTileBytes<DP>, kTileBytes<DP>, q_full);
           ++loaded;
         }
-        for (int i = 0; i < t.n && ok; ++i) {
-          const int64_t tile = (int64_t)(t.k_index + t.range.at(i)) * kTileBytes<DP>;
-          fill(a.pk + tile, false);
-          if (ok && values != nullptr) fill(values, true);
-          values = a.pv + tile;
+        for (int i = 0; i <= t.n && ok; ++i) {  // a tile's keys, then the values of the one before
+          if (i < t.n) fill(a.pk + (int64_t)(t.k_index + t.range.at(i)) * kTileBytes<DP>, false);
+          if (ok && i > 0) fill(a.pv + (int64_t)(t.k_index + t.range.at(i - 1)) * kTileBytes<DP>, true);
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0) {
-      if (ok && values != nullptr) fill(values, true);
-      if (!ok) {  // copies in flight end before the block does
-        if (loaded > 0) mbar_wait(q_full, (loaded - 1) & 1, err);
-        for (uint32_t f = it > Plan::kSlots ? it - Plan::kSlots : 0; f < it; ++f)
-          mbar_wait(slot_full + 8 * (f % Plan::kSlots), (f / Plan::kSlots) & 1, err);
-      }
+    if (lane == 0 && !ok) {  // copies in flight end before the block does
+      if (loaded > 0) mbar_wait(q_full, (loaded - 1) & 1, err);
+      for (uint32_t f = it > Plan::kSlots ? it - Plan::kSlots : 0; f < it; ++f)
+        mbar_wait(slot_full + 8 * (f % Plan::kSlots), (f / Plan::kSlots) & 1, err);
     }
   } else if (warp == 17) {
     fewer_registers<kFewRegs>();
@@ -773,10 +784,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     uint32_t it = 0, gi = 0, item = 0;  // slots, tiles and items issued so far
     bool ok = true;
     auto values = [&](uint32_t t) {  // of tile t of the stream
-      const int buf = t & 1;
-      const uint32_t p = tmem + buf * kTile, d = tmem + 2 * kTile + buf * DP;
-      ok = mbar_wait(p_full + 8 * buf, (t >> 1) & 1, err);
-      if (ok && t >= 2) ok = mbar_wait(o_empty + 8 * buf, ((t >> 1) - 1) & 1, err);
+      const uint32_t p = tmem_s + (t & 1) * kTile, out = t % kOut, d = tmem_o + out * DP;
+      ok = mbar_wait(p_full + 8 * (t & 1), (t >> 1) & 1, err);
+      if (ok && t >= kOut) ok = mbar_wait(o_empty + 8 * out, (t / kOut - 1) & 1, err);
       for (int x = 0; x < kHalves && ok; ++x, ++it) {
         const uint32_t slot = it % Plan::kSlots;
         ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
@@ -795,61 +805,69 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         }
         umma_commit(slot_empty + 8 * slot);
       }
-      if (ok) umma_commit(o_full + 8 * buf);
+      if (ok) umma_commit(o_full + 8 * out);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
       if (lane == 0 && t.n > 0) {
-        ok = mbar_wait(q_full, item & 1, err);
+        ok = mbar_wait(q_ready, item & 1, err);
         ++item;
-        for (int i = 0; i < t.n && ok; ++i, ++gi) {
-          const uint32_t d = tmem + (gi & 1) * kTile;
-          for (int x = 0; x < kHalves && ok; ++x, ++it) {
-            const uint32_t slot = it % Plan::kSlots;
-            ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t q = column_word(q_smem + x * kBox), key = column_word(slots + slot * kSlotBytes);
+        for (int i = 0; i <= t.n && ok; ++i) {
+          if (i < t.n) {
+            const uint32_t d = tmem_s + (gi & 1) * kTile;
+            for (int x = 0; x < kHalves && ok; ++x, ++it) {
+              const uint32_t slot = it % Plan::kSlots;
+              ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t q = tmem + 32 * x, key = column_word(slots + slot * kSlotBytes);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t qh = q + k * kColumnStep, ql = qh + (kHalves * kBox >> 4);
-              const uint32_t kh = key + k * kColumnStep, kl = kh + (kBox >> 4);
-              umma_ss(d, ql, kh, kScore, x != 0 || k != 0);
-              umma_ss(d, qh, kl, kScore, 1u);
-              umma_ss(d, qh, kh, kScore, 1u);
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t qh = q + 8 * k, ql = qh + DP / 2, kh = key + k * kColumnStep, kl = kh + (kBox >> 4);
+                umma_ts(d, ql, kh, kScore, x != 0 || k != 0);
+                umma_ts(d, qh, kl, kScore, 1u);
+                umma_ts(d, qh, kh, kScore, 1u);
+              }
+              umma_commit(slot_empty + 8 * slot);
             }
-            umma_commit(slot_empty + 8 * slot);
+            if (!ok) break;
+            umma_commit(s_full + 8 * (gi & 1));
+            ++gi;
           }
-          if (!ok) break;
-          umma_commit(s_full + 8 * (gi & 1));
-          if (i == t.n - 1) umma_commit(q_empty);
-          if (gi > 0) values(gi - 1);
+          // The values of the tile before (gi now counts the scores issued).
+          if (i > 0) values(gi - (i < t.n ? 2 : 1));
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0) {
-      if (ok && gi > 0) values(gi - 1);
-      if (!ok) {  // instructions in flight end before the block does
-        umma_commit(drained);
-        mbar_wait(drained, 0, err);
-      }
+    if (lane == 0 && !ok) {  // instructions in flight end before the block does
+      umma_commit(drained);
+      mbar_wait(drained, 0, err);
     }
   } else if (warp < 8) {
     more_registers<kScoreRegs>();
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
-    uint32_t gi = 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, at = tmem_s + lanes + half * 64;
+    uint32_t gi = 0, item = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
       if (t.n == 0) {
         for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
           simple_forward_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, t.b, t.h, r);
         continue;
       }
+      // The products with the query tile before are done: their scores have been read.
+      ok = warp_wait(q_full, item & 1, err);
+      if (!ok) break;
+      rows_to_tmem<DP>(tmem + lanes, q_smem, row, half);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready), mbar_arrive(q_empty);
+      ++item;
       const RowMask mask = mask_of(s, t, row);
       const double to_log2 = (double)a.fq[t.q_index] * (double)s.scale * 1.4426950408889634;
       for (int i = 0; i < t.n; ++i, ++gi) {
@@ -880,9 +898,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           m3 = fmaxf(m3, v[e + 3]);
         }
         m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-        // The row's other half is in the warp four further; `most` and `sum` of
-        // the tile before last have been read once its output buffer is free.
-        if (gi >= 2) ok = warp_wait(o_empty + 8 * buf, ((gi >> 1) - 1) & 1, err);
+        // The row's other half is in the warp four further.
+        if (gi >= 2) ok = warp_wait(st_empty + 8 * buf, ((gi >> 1) - 1) & 1, err);
         if (!ok) break;
         most[(buf * 2 + half) * kTile + row] = m0;
         __syncwarp();
@@ -915,12 +932,12 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     fewer_registers<kOutputRegs>();
     constexpr int kCols = DP / 2;  // output columns of a thread
     const int quad = warp & 3, half = (warp - 8) >> 2, row = quad * 32 + lane;
-    const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + 2 * kTile + half * kCols;
+    const uint32_t at = tmem_o + ((uint32_t)(quad * 32) << 16) + half * kCols;
     uint32_t gi = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, nullptr, err);
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
       if (t.n == 0) continue;
       float acc[kCols];
 #pragma unroll
@@ -929,24 +946,30 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       for (int i = 0; i < t.n; ++i, ++gi) {
         const int buf = gi & 1;
         const float fv = a.fv[t.k_index + t.range.at(i)];
-        ok = warp_wait(p_full + 8 * buf, (gi >> 1) & 1, err) && warp_wait(o_full + 8 * buf, (gi >> 1) & 1, err);
+        const uint32_t ob = gi % kOut;
+        ok = warp_wait(p_full + 8 * buf, (gi >> 1) & 1, err);
+        if (!ok) break;
+        const float c0 = ref[buf * kTile + row];
+        const float parts = sum[2 * buf * kTile + row] + sum[(2 * buf + 1) * kTile + row];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(st_empty + 8 * buf);
+        ok = warp_wait(o_full + 8 * ob, (gi / kOut) & 1, err);
         if (!ok) break;
         tc_fence_after();
-        const float c0 = ref[buf * kTile + row];
         const float next = fmaxf(top, c0);
         const float keep = top == -INFINITY ? 0.0f : exp2_fast(top - next);
         const float take = c0 == -INFINITY ? 0.0f : exp2_fast(c0 - next);
-        l = l * keep + (sum[2 * buf * kTile + row] + sum[(2 * buf + 1) * kTile + row]) * take;
+        l = l * keep + parts * take;
         top = next;
         const float tv = take * fv;
 #pragma unroll
         for (int c = 0; c < kCols; c += 16) {
           float v[16];
-          tmem_ld16(at + buf * DP + c, v);
+          tmem_ld16(at + ob * DP + c, v);
           if (c == kCols - 16) {  // the last values are out: the buffer is free
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(o_empty + 8 * buf);
+            if (lane == 0) mbar_arrive(o_empty + 8 * ob);
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(acc[c + e], keep, v[e] * tv);
@@ -1002,13 +1025,23 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 // which is added to fp32 registers.  dS is brought near 2^15 by a power of two
 // from |dS| <= |dO_i| |V_j| + |delta_i|, with the norms of single rows on the
 // resident side and a tile's greatest on the streamed one.
-// Roles as in forward_kernel.  Shared memory holds the resident tiles and a
-// ring of two steps of the operand that is used twice; its lo half is used,
-// and freed, first, so that the next step's copies have started before the
-// last product ends.
+// Roles as in forward_kernel, the resident tiles in tensor memory
+// (rows_to_tmem).  With two of them, 128 wide, there is room for one buffer of
+// scores and dP: a step's sums then come before the next one's scores, and P is
+// formed while dP is still being summed.  Elsewhere two steps overlap.
+// A key tile's queries may be many (a sink's are all that follow): its steps
+// are cut into segments that go to different blocks, each leaving its part in
+// the workspace, joined in order by grad_join_kernel.
 enum GradPass { kGradQ, kGradK, kGradV };
 constexpr int kStep = 64;
 constexpr int kStepBox = kStep * 128;  // bytes of 64 rows of a box
+
+// How the key tiles' steps are cut: the first `long_tiles` of each head into
+// long_segs segments, the others into short_segs.  A unit is a segment of a
+// tile of a head, counted tile by tile.
+struct Segments {
+  int long_tiles, long_segs, short_segs;
+};
 
 struct GradArgs {
   AttentionShape s;
@@ -1019,6 +1052,8 @@ struct GradArgs {
   const float4* info;                  // of query rows
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
+  Segments seg;                        // of the key tiles' steps
+  float* part;                         // [unit][128][DP]
 };
 
 template <int DP, int PASS>
@@ -1031,6 +1066,11 @@ struct GradPlan {
   static constexpr int kResident = (kTwo ? 2 : 1) * kTileBytes<DP>;
   static constexpr int kInfo = PASS == kGradQ ? 0 : 2 * kStep * 16;
   static constexpr int kRing = 2 * (kFirstSteps + kSecondSteps);  // half steps
+  static constexpr int kRows = (kTwo ? 2 : 1) * DP;      // tensor memory: resident tiles,
+  static constexpr int kScoreBufs = kTwo && DP == 128 ? 1 : 2;
+  static constexpr int kScoreCols = (kTwo ? 2 : 1) * kStep;  // buffers of scores (and dP),
+  static constexpr int kOutBufs = kTwo && DP == 128 ? 1 : 2;  // and of DP columns of sums
+  static_assert(kRows + kScoreBufs * kScoreCols + kOutBufs * DP <= 512, "tensor memory");
   static constexpr int kSmem = kResident + kRing * kPart + kInfo + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory of one block");
 };
@@ -1042,6 +1082,9 @@ struct GradItem {
   RowRange rows;       // kGradQ
   TileRange range;     // in steps of 64
   int row_tile;        // index of the resident tile
+  int f0, f1;          // the unit's part of the heads' steps, counted head by head
+  int segs;            // segments of the tile's steps
+  bool first;          // the first of them
 };
 
 template <int PASS>
@@ -1051,6 +1094,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
   const int group = s.heads / s.kv_heads, lane = threadIdx.x & 31;
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
   float sum;
+  int seg = 0;
   if (PASS == kGradQ) {
     const int tq = tiles_q - 1 - index / (s.heads * s.batch);
     t.h = index % s.heads;
@@ -1065,6 +1109,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     t.range.low = low / kStep;
     t.range.sinks = min((min(s.sinks, low) + kStep - 1) / kStep, t.range.low);
     t.range.count = x > z ? 0 : t.range.sinks + z / kStep - t.range.low + 1;
+    t.segs = 1;
     sum = a.fq[t.row_tile] + a.fo[t.row_tile];
     const int first = (t.b * s.kv_heads + t.g) * tiles_k;
     for (int i = lane; i < t.range.count; i += 32) {
@@ -1073,7 +1118,12 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     }
   } else {
     // The first keys are seen by the most queries.
-    const int tk = index / (s.kv_heads * s.batch);
+    const int of_long = a.seg.long_tiles * a.seg.long_segs * s.kv_heads * s.batch;
+    const bool is_long = index < of_long;
+    t.segs = is_long ? a.seg.long_segs : a.seg.short_segs;
+    if (!is_long) index -= of_long;
+    const int tk = index / (t.segs * s.kv_heads * s.batch) + (is_long ? 0 : a.seg.long_tiles);
+    seg = index / (s.kv_heads * s.batch) % t.segs;
     t.g = index % s.kv_heads;
     t.b = index / s.kv_heads % s.batch;
     t.h = t.g * group;
@@ -1097,6 +1147,10 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     }
   }
   t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  const int total = (PASS == kGradQ ? 1 : group) * t.n, each = (total + t.segs - 1) / t.segs;
+  t.f0 = min(total, seg * each);
+  t.f1 = min(total, t.f0 + each);
+  t.first = seg == 0;
   return t;
 }
 
@@ -1110,34 +1164,35 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 template <int DP, int PASS>
 __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
   using Plan = GradPlan<DP, PASS>;
-  constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart;
+  constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart, kScoreBufs = Plan::kScoreBufs, kOutBufs = Plan::kOutBufs;
   constexpr bool kTwo = Plan::kTwo;
   const AttentionShape& s = a.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = s.heads / s.kv_heads, heads = PASS == kGradQ ? 1 : group;  // heads an item walks
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];  // at the start of shared memory, as there is no other
   const uint32_t base = smem_u32(smem);
-  if ((base & 1023u) != 0) {  // the swizzle needs it; with no static shared memory it always holds
-    if (threadIdx.x == 0) atomicCAS(err, 0, (int)kErrTmemAlloc);
-    return;
-  }
   const uint32_t ring1 = base + Plan::kResident, ring2 = ring1 + 2 * Plan::kFirstSteps * kPart;
   uint8_t* info_smem = smem + Plan::kResident + Plan::kRing * kPart;
   uint64_t* bars = (uint64_t*)(info_smem + Plan::kInfo);
   constexpr int kHalves1 = 2 * Plan::kFirstSteps, kHalves2 = 2 * Plan::kSecondSteps;  // ring entries (half steps)
-  const uint32_t a_full = smem_u32(bars), a_empty = a_full + 8;
-  const uint32_t full1 = a_empty + 8, empty1 = full1 + 8 * kHalves1, full2 = empty1 + 8 * kHalves1;
-  const uint32_t empty2 = full2 + 8 * kHalves2, s_full = empty2 + 8 * kHalves2, p_full = s_full + 16;
-  const uint32_t o_full = p_full + 16, o_empty = o_full + 16, drained = o_empty + 16;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 + 2 * kHalves1 + 2 * kHalves2 + 9);
+  const uint32_t a_full = smem_u32(bars), a_empty = a_full + 8, a_ready = a_empty + 8;
+  const uint32_t full1 = a_ready + 8, empty1 = full1 + 8 * kHalves1, full2 = empty1 + 8 * kHalves1;
+  const uint32_t empty2 = full2 + 8 * kHalves2, s_full = empty2 + 8 * kHalves2, d_full = s_full + 16;
+  const uint32_t p_full = d_full + 16, o_full = p_full + 16, o_empty = o_full + 16, drained = o_empty + 16;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 2 * kHalves1 + 2 * kHalves2 + 11);
+  if ((base & 1023u) != 0) {  // the swizzle needs it
+    if (threadIdx.x == 0) atomicCAS(err, 0, (int)kErrTmemAlloc);
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(a_full, 1);
-    mbar_init(a_empty, 1);
+    mbar_init(a_empty, 8);
+    mbar_init(a_ready, 8);
     for (int i = 0; i < kHalves1; ++i) mbar_init(full1 + 8 * i, 1), mbar_init(empty1 + 8 * i, 1);
     for (int i = 0; i < kHalves2; ++i) mbar_init(full2 + 8 * i, 1), mbar_init(empty2 + 8 * i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + 8 * i, 1);
+      mbar_init(d_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 8);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, 8);
@@ -1153,8 +1208,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // Tensor memory: two buffers of (scores, dP) of 64 columns each, two of DP for the step's sums.
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem + Plan::kRows, tmem_o = tmem_s + kScoreBufs * Plan::kScoreCols;
 
   // Index of the streamed tile of step i of head x of an item.
   auto column_tile = [&](const GradItem& t, int x, int i) {
@@ -1166,18 +1220,28 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
     fewer_registers<kFewRegs>();
   } else if (warp == 16) {
     fewer_registers<kFewRegs>();
-    uint32_t it1 = 0, it2 = 0, loaded = 0;  // half steps, resident tiles
+    uint32_t it = 0, loaded = 0;  // half steps of each ring, items
     bool ok = true;
-    // Half `part` (0: lo, 1: hi) of 64 rows of a packed tile.
-    auto half = [&](uint32_t dst, uint32_t full, const uint8_t* tile, int step, int part) {
+    // Half a step of one ring: `part` 0 the lo boxes, 1 the hi ones, and with
+    // the latter the rows' statistics where `with_info`.
+    auto fill = [&](uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries, const uint8_t* packed, int tile,
+                    int step, int part, bool with_info) {
+      const uint32_t slot = it % entries, use = it / entries, bar = full + 8 * slot;
+      if (use > 0) ok = mbar_wait(empty + 8 * slot, (use - 1) & 1, err);
+      if (!ok) return;
+      mbar_expect_tx(bar, kPart + (with_info ? kStep * 16 : 0));
+      const uint8_t* src = packed + (int64_t)tile * kTileBytes<DP> + (1 - part) * kHalves * kBox + (step & 1) * kStepBox;
 #pragma unroll
       for (int x = 0; x < kHalves; ++x)
-        bulk_load(dst + x * kStepBox, tile + ((1 - part) * kHalves + x) * kBox + (step & 1) * kStepBox, kStepBox, full);
+        bulk_load(ring + slot * kPart + x * kStepBox, src + x * kBox, kStepBox, bar);
+      if (with_info)
+        bulk_load(smem_u32(info_smem) + (it / 2 & 1) * (kStep * 16),
+                  (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16, bar);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<PASS>(a, w, err);
-      if (lane == 0 && t.n > 0) {
+      if (lane == 0 && t.f0 < t.f1) {
         if (loaded > 0) ok = mbar_wait(a_empty, (loaded - 1) & 1, err);
         if (ok) {
           mbar_expect_tx(a_full, Plan::kResident);
@@ -1186,53 +1250,36 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
           if (kTwo) bulk_load(base + kTileBytes<DP>, (PASS == kGradQ ? a.po : a.pv) + at, kTileBytes<DP>, a_full);
           ++loaded;
         }
-        for (int x = 0; x < heads && ok; ++x)
-          for (int i = 0; i < t.n && ok; ++i) {
-            const int tile = column_tile(t, x, i), step = t.range.at(i);
-            const uint8_t* one = (PASS == kGradQ ? a.pk : a.pq) + (int64_t)tile * kTileBytes<DP>;
-            const uint8_t* two = (PASS == kGradQ ? a.pv : a.po) + (int64_t)tile * kTileBytes<DP>;
-            for (int part = 0; part < 2 && ok; ++part, ++it1) {
-              const uint32_t slot = it1 % kHalves1, use = it1 / kHalves1;
-              if (use > 0) ok = mbar_wait(empty1 + 8 * slot, (use - 1) & 1, err);
-              if (!ok) break;
-              // kGradK: the rows' statistics come with the operand that stays until they have been used.
-              const bool with_info = PASS == kGradK && part == 1;
-              mbar_expect_tx(full1 + 8 * slot, kPart + (with_info ? kStep * 16 : 0));
-              half(ring1 + slot * kPart, full1 + 8 * slot, one, step, part);
-              if (with_info)
-                bulk_load(smem_u32(info_smem) + (it1 / 2 & 1) * (kStep * 16),
-                          (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16,
-                          full1 + 8 * slot);
-            }
-            for (int part = 0; part < 2 && ok; ++part, ++it2) {
-              const uint32_t slot = it2 % kHalves2, use = it2 / kHalves2;
-              if (use > 0) ok = mbar_wait(empty2 + 8 * slot, (use - 1) & 1, err);
-              if (!ok) break;
-              const bool with_info = PASS == kGradV && part == 1;
-              mbar_expect_tx(full2 + 8 * slot, kPart + (with_info ? kStep * 16 : 0));
-              half(ring2 + slot * kPart, full2 + 8 * slot, two, step, part);
-              if (with_info)
-                bulk_load(smem_u32(info_smem) + (it2 / 2 & 1) * (kStep * 16),
-                          (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16,
-                          full2 + 8 * slot);
-            }
-          }
+        for (int f = t.f0; f < t.f1 && ok; ++f, it += 2) {
+          const int x = f / t.n, i = f - x * t.n, tile = column_tile(t, x, i), step = t.range.at(i);
+          // The statistics come with the operand that stays until they have been used.
+          for (int part = 0; part < 2 && ok; ++part, ++it)
+            fill(ring1, full1, empty1, kHalves1, PASS == kGradQ ? a.pk : a.pq, tile, step, part,
+                 PASS == kGradK && part == 1);
+          it -= 2;
+          for (int part = 0; part < 2 && ok; ++part, ++it)
+            fill(ring2, full2, empty2, kHalves2, PASS == kGradQ ? a.pv : a.po, tile, step, part,
+                 PASS == kGradV && part == 1);
+          it -= 2;
+        }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0 && !ok) {  // copies in flight end before the block does
-      if (loaded > 0) mbar_wait(a_full, (loaded - 1) & 1, err);
-      for (uint32_t f = it1 > kHalves1 ? it1 - kHalves1 : 0; f < it1; ++f)
-        mbar_wait(full1 + 8 * (f % kHalves1), (f / kHalves1) & 1, err);
-      for (uint32_t f = it2 > kHalves2 ? it2 - kHalves2 : 0; f < it2; ++f)
-        mbar_wait(full2 + 8 * (f % kHalves2), (f / kHalves2) & 1, err);
+    if (lane == 0 && !ok) {
+      // Copies in flight end before the block does.  The last step may have
+      // been begun only in part: a wait for a fill that never came runs out.
+      if (loaded > 0) mbar_wait_limit(a_full, (loaded - 1) & 1, err, kWaitCycles / 8);
+      for (uint32_t f = it > kHalves1 ? it - kHalves1 : 0; f < it + 2; ++f) {
+        mbar_wait_limit(full1 + 8 * (f % kHalves1), (f / kHalves1) & 1, err, kWaitCycles / 8);
+        mbar_wait_limit(full2 + 8 * (f % kHalves2), (f / kHalves2) & 1, err, kWaitCycles / 8);
+      }
     }
   } else if (warp == 17) {
     fewer_registers<kFewRegs>();
     constexpr uint32_t kScore = umma_idesc(kStep, false), kSum = umma_idesc(DP, true);
     uint32_t gi = 0, item = 0;  // steps and items issued so far
     bool ok = true;
-    // D = resident tile . (64 columns of a half-step ring)^T; `release`: the ring's entries are free after it.
+    // D = resident rows (tensor memory) times 64 streamed ones; `release`: the ring's entries are free after it.
     auto scores = [&](uint32_t d, uint32_t rows, uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries,
                       bool release) {
       for (uint32_t part = 0; part < 2 && ok; ++part) {
@@ -1242,15 +1289,15 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
         tc_fence_after();
 #pragma unroll
         for (int x = 0; x < kHalves; ++x) {
-          const uint32_t r = column_word(rows + x * kBox), c = column_word(ring + slot * kPart + x * kStepBox);
+          const uint32_t r = rows + 32 * x, c = column_word(ring + slot * kPart + x * kStepBox);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t rh = r + k * kColumnStep, rl = rh + (kHalves * kBox >> 4), ch = c + k * kColumnStep;
+            const uint32_t rh = r + 8 * k, rl = rh + DP / 2, ch = c + k * kColumnStep;
             if (part == 0) {
-              umma_ss(d, rh, ch, kScore, x != 0 || k != 0);
+              umma_ts(d, rh, ch, kScore, x != 0 || k != 0);
             } else {
-              umma_ss(d, rl, ch, kScore, 1u);
-              umma_ss(d, rh, ch, kScore, 1u);
+              umma_ts(d, rl, ch, kScore, 1u);
+              umma_ts(d, rh, ch, kScore, 1u);
             }
           }
         }
@@ -1259,12 +1306,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
     };
     // The sums of step t: P or dS (in tensor memory) times the 64 rows of a ring step.
     auto sums = [&](uint32_t t) {
-      const int buf = t & 1;
-      const uint32_t p = tmem + buf * 2 * kStep, d = tmem + 4 * kStep + buf * DP;
+      const uint32_t buf = t % kScoreBufs, out = t % kOutBufs;
+      const uint32_t p = tmem_s + buf * Plan::kScoreCols, d = tmem_o + out * DP;
       const uint32_t ring = PASS == kGradV ? ring2 : ring1, full = PASS == kGradV ? full2 : full1;
       const uint32_t empty = PASS == kGradV ? empty2 : empty1, entries = PASS == kGradV ? kHalves2 : kHalves1;
-      ok = mbar_wait(p_full + 8 * buf, (t >> 1) & 1, err);
-      if (ok && t >= 2) ok = mbar_wait(o_empty + 8 * buf, ((t >> 1) - 1) & 1, err);
+      ok = mbar_wait(p_full + 8 * buf, (t / kScoreBufs) & 1, err);
+      if (ok && t >= kOutBufs) ok = mbar_wait(o_empty + 8 * out, (t / kOutBufs - 1) & 1, err);
       for (uint32_t part = 0; part < 2 && ok; ++part) {
         const uint32_t entry = 2 * t + part, slot = entry % entries;
         ok = mbar_wait(full + 8 * slot, (entry / entries) & 1, err);
@@ -1283,52 +1330,65 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
         }
         umma_commit(empty + 8 * slot);
       }
-      if (ok) umma_commit(o_full + 8 * buf);
+      if (ok) umma_commit(o_full + 8 * out);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<PASS>(a, w, err);
-      if (lane == 0 && t.n > 0) {
-        ok = mbar_wait(a_full, item & 1, err);
+      if (lane == 0 && t.f0 < t.f1) {
+        ok = mbar_wait(a_ready, item & 1, err);
         ++item;
-        const int steps = heads * t.n;
-        for (int i = 0; i < steps && ok; ++i, ++gi) {
-          const uint32_t d = tmem + (gi & 1) * 2 * kStep;
-          scores(d, base, ring1, full1, empty1, kHalves1, PASS == kGradV);
-          if (kTwo && ok) scores(d + kStep, base + kTileBytes<DP>, ring2, full2, empty2, kHalves2, true);
+        const int steps = t.f1 - t.f0;
+        for (int i = 0; i < steps && ok; ++i) {
+          const uint32_t buf = gi % kScoreBufs, d = tmem_s + buf * Plan::kScoreCols;
+          scores(d, tmem, ring1, full1, empty1, kHalves1, PASS == kGradV);
+          if (ok) umma_commit(s_full + 8 * buf);
+          if (kTwo && ok) {
+            scores(d + kStep, tmem + DP, ring2, full2, empty2, kHalves2, true);
+            if (ok) umma_commit(d_full + 8 * buf);
+          }
           if (!ok) break;
-          umma_commit(s_full + 8 * (gi & 1));
-          if (i == steps - 1) umma_commit(a_empty);
-          if (gi > 0) sums(gi - 1);
+          ++gi;
+          // With one buffer this step's sums, with two the ones of the step before.
+          if (kScoreBufs == 1) sums(gi - 1);
+          else if (i > 0) sums(gi - 2);
         }
+        if (kScoreBufs == 2 && ok) sums(gi - 1);
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0) {
-      if (ok && gi > 0) sums(gi - 1);
-      if (!ok) {  // instructions in flight end before the block does
-        umma_commit(drained);
-        mbar_wait(drained, 0, err);
-      }
+    if (lane == 0 && !ok) {  // instructions in flight end before the block does
+      umma_commit(drained);
+      mbar_wait(drained, 0, err);
     }
   } else if (warp < 8) {
     more_registers<kScoreRegs>();
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 32;
-    uint32_t gi = 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, at = tmem_s + lanes + half * 32;
+    uint32_t gi = 0, item = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<PASS>(a, w, err);
-      if (t.n == 0) {
+      if (t.n == 0 && t.first) {
         if (PASS == kGradQ)
           for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
             simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
         if (PASS == kGradK)  // and dv, which kGradV leaves out
           for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 8)
             simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
-        continue;
       }
+      if (t.f0 >= t.f1) continue;
+      // The products with the resident tiles before are done: their scores have been read.
+      ok = warp_wait(a_full, item & 1, err);
+      if (!ok) break;
+      rows_to_tmem<DP>(tmem + lanes, base, row, half);
+      if (kTwo) rows_to_tmem<DP>(tmem + DP + lanes, base + kTileBytes<DP>, row, half);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_ready), mbar_arrive(a_empty);
+      ++item;
       // kGradQ: what the row sees and its statistics; else the key's rows [s0, s1) and its norm.
       RowMask mask = {0, 0, 0};
       float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1347,86 +1407,86 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       const float* f_row1 = PASS == kGradQ ? a.fq : a.fk;
       const double to_log2 = (double)f_row1[t.row_tile] * (double)s.scale * 1.4426950408889634;
       const float f_row2 = PASS == kGradQ ? a.fo[t.row_tile] : kTwo ? a.fv[t.row_tile] : 0.0f;
-      for (int x = 0; x < heads && ok; ++x)
-        for (int i = 0; i < t.n; ++i, ++gi) {
-          const int buf = gi & 1, step = t.range.at(i), tile = column_tile(t, x, i), c0 = step * kStep;
-          const float f = (float)(to_log2 * (double)(PASS == kGradQ ? a.fk : a.fq)[tile]);
-          bool whole;
-          uint32_t seen = 0xffffffffu;
+      for (int n = t.f0; n < t.f1; ++n, ++gi) {
+        const uint32_t buf = gi % kScoreBufs, phase = (gi / kScoreBufs) & 1;
+        const int x = n / t.n, i = n - x * t.n;
+        const int step = t.range.at(i), tile = column_tile(t, x, i), c0 = step * kStep;
+        const float f = (float)(to_log2 * (double)(PASS == kGradQ ? a.fk : a.fq)[tile]);
+        bool whole;
+        uint32_t seen = 0xffffffffu;
+        if (PASS == kGradQ) {
+          whole = t.rows.all && c0 + kStep - 1 <= t.rows.p0 &&
+                  (s.window == 0 || t.rows.p1 - c0 < s.window || c0 + kStep <= s.sinks);
+          if (!whole) seen = seen_bits(mask, c0 + 32 * half);
+        } else {
+          const int first = t.sq.start + c0, last = first + kStep - 1, k1 = t.r0 + kTile - 1;
+          whole = k1 <= first && last < t.sq.n && c0 + kStep <= s.q_len &&
+                  (s.window == 0 || last - t.r0 < s.window || k1 < s.sinks);
+          if (!whole) seen = bits_between(s0, s1, c0 + 32 * half);
+        }
+        float up = 16384.0f;  // P <= 1
+        float f2 = 0.0f;
+        if (kTwo) {
+          const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] +
+                              (PASS == kGradQ ? fabsf(st.z) : a.tdo[tile]);
+          up = power_of_two(scale_exponent(bound));
+          f2 = f_row2 * (PASS == kGradQ ? a.fv : a.fo)[tile];
+        }
+        ok = warp_wait(s_full + 8 * buf, phase, err);
+        if (PASS != kGradQ && ok) {  // the statistics' copy, with the second half of its step
+          const uint32_t entries = PASS == kGradV ? kHalves2 : kHalves1, entry = 2 * gi + 1;
+          ok = warp_wait((PASS == kGradV ? full2 : full1) + 8 * (entry % entries), (entry / entries) & 1, err);
+        }
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t here = at + buf * Plan::kScoreCols;
+        const float4* col = (const float4*)(info_smem + (gi & 1) * (kStep * 16)) + 32 * half;
+        float v[32];
+        tmem_ld32(here, v);
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1u)) v[e] = -INFINITY;
+        }
+        const float scaled = st.y * up;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
           if (PASS == kGradQ) {
-            whole = t.rows.all && c0 + kStep - 1 <= t.rows.p0 &&
-                    (s.window == 0 || t.rows.p1 - c0 < s.window || c0 + kStep <= s.sinks);
-            if (!whole) seen = seen_bits(mask, c0 + 32 * half);
+            v[e] = exp2_fast(fmaf(v[e], f, -st.x)) * scaled;
           } else {
-            const int first = t.sq.start + c0, last = first + kStep - 1, k1 = t.r0 + kTile - 1;
-            whole = k1 <= first && last < t.sq.n && c0 + kStep <= s.q_len &&
-                    (s.window == 0 || last - t.r0 < s.window || k1 < s.sinks);
-            if (!whole) seen = bits_between(s0, s1, c0 + 32 * half);
+            const float2 c = *(const float2*)&col[e];
+            v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up);
           }
-          float up = 16384.0f;  // P <= 1
-          float f2 = 0.0f;
-          if (kTwo) {
-            const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] +
-                                (PASS == kGradQ ? fabsf(st.z) : a.tdo[tile]);
-            up = power_of_two(scale_exponent(bound));
-            f2 = f_row2 * (PASS == kGradQ ? a.fv : a.fo)[tile];
-          }
-          ok = warp_wait(s_full + 8 * buf, (gi >> 1) & 1, err);
-          if (PASS != kGradQ && ok) {  // the statistics' copy, with the second half of its step
-            const uint32_t entries = PASS == kGradV ? kHalves2 : kHalves1, entry = 2 * gi + 1;
-            ok = warp_wait((PASS == kGradV ? full2 : full1) + 8 * (entry % entries), (entry / entries) & 1, err);
-          }
+        }
+        if (kTwo) {
+          ok = warp_wait(d_full + 8 * buf, phase, err);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t here = at + buf * 2 * kStep;
-          float v[32];
-          tmem_ld32(here, v);
-          if (!whole) {
+          float d[32];
+          tmem_ld32(here + kStep, d);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen >> e & 1u)) v[e] = -INFINITY;
-          }
-          const float4* col = (const float4*)(info_smem + buf * (kStep * 16)) + 32 * half;
-          if (kTwo) {
-            float d[32];
-            tmem_ld32(here + kStep, d);
-            const float scaled = st.y * up;
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (PASS == kGradQ) {
-                v[e] = exp2_fast(fmaf(v[e], f, -st.x)) * scaled * fmaf(d[e], f2, -st.z);
-              } else {
-                const float4 c = col[e];
-                v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up) * fmaf(d[e], f2, -c.z);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float2 c = *(const float2*)&col[e];
-              v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up);
-            }
-          }
-          uint32_t r[32];
-          split32(v, r);
-          tmem_st32(here, r);
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_full + 8 * buf);
+          for (int e = 0; e < 32; ++e) v[e] *= fmaf(d[e], f2, PASS == kGradQ ? -st.z : -col[e].z);
         }
+        uint32_t r[32];
+        split32(v, r);
+        tmem_st32(here, r);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8 * buf);
+      }
     }
   } else {
     fewer_registers<kOutputRegs>();
     constexpr int kCols = DP / 2;  // columns of a thread
     const int quad = warp & 3, half = (warp - 8) >> 2, row = quad * 32 + lane;
-    const uint32_t at = tmem + ((uint32_t)(quad * 32) << 16) + 4 * kStep + half * kCols;
+    const uint32_t at = tmem_o + ((uint32_t)(quad * 32) << 16) + half * kCols;
     uint32_t gi = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<PASS>(a, w, err);
-      if (t.n == 0) continue;
+      if (t.f0 >= t.f1) continue;
       float norm = 0.0f, delta = 0.0f;
       if (PASS == kGradQ) {
         const float4 st = a.info[(int64_t)t.row_tile * kTile + row];
@@ -1438,40 +1498,44 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       float acc[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
-      for (int x = 0; x < heads && ok; ++x)
-        for (int i = 0; i < t.n; ++i, ++gi) {
-          const int buf = gi & 1, tile = column_tile(t, x, i);
-          float down = 0x1p-14f * (PASS == kGradV ? a.fo[tile] : 1.0f);
-          if (kTwo) {
-            const float bound =
-                norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] + (PASS == kGradQ ? delta : a.tdo[tile]);
-            down = power_of_two(-scale_exponent(bound)) * (PASS == kGradQ ? a.fk : a.fq)[tile];
-          }
-          ok = warp_wait(o_full + 8 * buf, (gi >> 1) & 1, err);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < kCols; c += 16) {
-            float v[16];
-            tmem_ld16(at + buf * DP + c, v);
-            if (c == kCols - 16) {  // the last values are out: the buffer is free
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(o_empty + 8 * buf);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], down, acc[c + e]);
-          }
+      for (int n = t.f0; n < t.f1; ++n, ++gi) {
+        const uint32_t out = gi % kOutBufs;
+        const int x = n / t.n, tile = column_tile(t, x, n - x * t.n);
+        float down = 0x1p-14f * (PASS == kGradV ? a.fo[tile] : 1.0f);
+        if (kTwo) {
+          const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] + (PASS == kGradQ ? delta : a.tdo[tile]);
+          down = power_of_two(-scale_exponent(bound)) * (PASS == kGradQ ? a.fk : a.fq)[tile];
         }
+        ok = warp_wait(o_full + 8 * out, (gi / kOutBufs) & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kCols; c += 16) {
+          float v[16];
+          tmem_ld16(at + out * DP + c, v);
+          if (c == kCols - 16) {  // the last values are out: the buffer is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty + 8 * out);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], down, acc[c + e]);
+        }
+      }
       const int r = t.r0 + row;
-      if (ok && r < (PASS == kGradQ ? s.q_len : s.k_len)) {
+      if (ok && t.segs > 1) {
+        float* dst = a.part + ((int64_t)w * kTile + row) * DP + half * kCols;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4)
+          *(float4*)(dst + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+      } else if (ok && r < (PASS == kGradQ ? s.q_len : s.k_len)) {
         const float by = PASS == kGradV ? 1.0f : s.scale;
-        float* out = PASS == kGradQ ? a.dq : PASS == kGradK ? a.dk : a.dv;
+        float* grad = PASS == kGradQ ? a.dq : PASS == kGradK ? a.dk : a.dv;
         const int add = PASS == kGradQ ? a.add_q : PASS == kGradK ? a.add_k : a.add_v;
-        float* dst = out + half * kCols +
+        float* dst = grad + half * kCols +
                      (PASS == kGradQ ? row_at(s, t.b, t.h, r, s.heads, s.q_len) : row_at(s, t.b, t.g, r, s.kv_heads, s.k_len));
         const int cols = s.head_dim - half * kCols;
-        if (s.head_dim % 4 == 0 && ((uintptr_t)out & 15) == 0) {
+        if (s.head_dim % 4 == 0 && ((uintptr_t)grad & 15) == 0) {
 #pragma unroll
           for (int c = 0; c < kCols; c += 4)
             if (c < cols) {
@@ -1497,6 +1561,30 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   if (warp == 17) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// Adds the segments of one key tile in order: one block per 32 rows of a tile.
+template <int DP, int PASS>
+__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int* err) {
+  const AttentionShape& s = a.s;
+  const int tile = blockIdx.x / 4, rows = blockIdx.x % 4 * 32;
+  // The tile's first segment; the next ones follow `stride` units apart.
+  const int unit = first + tile / stride * segs * stride + tile % stride;
+  const GradItem t = grad_item<PASS>(a, unit, err);
+  if (t.n == 0) return;  // written key by key
+  const int total = s.heads / s.kv_heads * t.n, each = (total + segs - 1) / segs, used = (total + each - 1) / each;
+  float* grad = PASS == kGradK ? a.dk : a.dv;
+  const int add = PASS == kGradK ? a.add_k : a.add_v;
+  const float by = PASS == kGradK ? s.scale : 1.0f;
+  for (int i = threadIdx.x; i < 32 * DP; i += 256) {
+    const int r = rows + i / DP, c = i % DP;
+    if (t.r0 + r >= s.k_len || c >= s.head_dim) continue;
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < used; ++k) sum += a.part[((int64_t)(unit + k * stride) * kTile + r) * DP + c];
+    float* dst = grad + row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len) + c;
+    *dst = add ? *dst + sum * by : sum * by;
   }
 }
 
@@ -1837,8 +1925,31 @@ struct GradWork {
   uint8_t *pq, *pk, *pv, *po;
   float *fq, *fk, *fv, *fo, *nv, *no, *tnv, *tno, *tdo;
   float4* info;
+  float* part;
   int64_t floats;
 };
+
+// Segments of a key tile's steps, about sixteen steps each where that makes
+// eight units per SM (below that a unit's start and end cost more than the
+// uneven blocks do).
+Segments segments_of(const AttentionShape& s) {
+  const int64_t group = s.heads / s.kv_heads, all = ceil_div(s.q_len, kStep);
+  const int64_t some = s.window > 0 ? std::min<int64_t>(all, ((int64_t)s.window + kTile + 2 * kStep - 3) / kStep) : all;
+  Segments g;
+  const int tiles = tiles_of(s.k_len);
+  g.long_tiles = s.window > 0 ? std::min(tiles, tiles_of(std::min(s.sinks, s.k_len))) : tiles;
+  // Without a window a tile's steps are half of all on average.
+  const int64_t steps = (s.window > 0 ? g.long_tiles * all : tiles * all / 2) + (tiles - g.long_tiles) * some;
+  const int64_t each = std::max<int64_t>(16, steps * group * s.batch * s.kv_heads / (kSms * 8));
+  g.long_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * all / each));
+  g.short_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * some / each));
+  return g;
+}
+int64_t grad_units(const AttentionShape& s, const Segments& g) {
+  const int64_t tiles = tiles_of(s.k_len);
+  return (g.long_tiles * (int64_t)g.long_segs + (tiles - g.long_tiles) * g.short_segs) * s.kv_heads * s.batch;
+}
+
 GradWork grad_work(const AttentionShape& s, float* base) {
   Carver c{base};
   const int64_t tile = padded_dim(s) == 64 ? kTileBytes<64> / 4 : kTileBytes<128> / 4;
@@ -1858,6 +1969,8 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.tno = c.take(nq);
   w.tdo = c.take(nq);
   w.info = (float4*)c.take(nq * kTile * 4);
+  const Segments g = segments_of(s);
+  w.part = c.take(g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * kTile * padded_dim(s) : 0);
   w.floats = c.used;
   return w;
 }
@@ -1871,11 +1984,23 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   constexpr int kSmem = GradPlan<DP, PASS>::kSmem;
   TYSOR_CUDA(cudaFuncSetAttribute(grad_kernel<DP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const AttentionShape& s = a.s;
-  const int64_t items = PASS == kGradQ ? (int64_t)tiles_of(s.q_len) * s.heads * s.batch
-                                       : (int64_t)tiles_of(s.k_len) * s.kv_heads * s.batch;
+  const int64_t items = PASS == kGradQ ? (int64_t)tiles_of(s.q_len) * s.heads * s.batch : grad_units(s, a.seg);
   if (items == 0) return;
+  if (items > INT_MAX / 4) throw CudaError("window_attention: too many keys");
   grad_kernel<DP, PASS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
+  if (PASS == kGradQ) return;
+  const int stride = s.kv_heads * s.batch, of_long = a.seg.long_tiles * a.seg.long_segs * stride;
+  if (a.seg.long_segs > 1 && a.seg.long_tiles > 0) {
+    grad_join_kernel<DP, PASS><<<(unsigned)(a.seg.long_tiles * stride * 4), 256, 0, st>>>(
+        a, 0, a.seg.long_segs, stride, err);
+    check_launch();
+  }
+  if (a.seg.short_segs > 1 && tiles_of(s.k_len) > a.seg.long_tiles) {
+    grad_join_kernel<DP, PASS><<<(unsigned)((tiles_of(s.k_len) - a.seg.long_tiles) * stride * 4), 256, 0, st>>>(
+        a, of_long, a.seg.short_segs, stride, err);
+    check_launch();
+  }
 }
 
 template <int DP>
@@ -1939,7 +2064,8 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
     run_pack(s, jobs, 4, err, st);
     const GradArgs a{s,    q,    k,    v,    out,  stats, dout,  w.pq,  w.pk,   w.pv, w.po, w.fq,         w.fk,
-                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v};
+                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v,
+                     segments_of(s), w.part};
     if (padded_dim(s) == 64) {
       run_grad<64, kGradQ>(a, err, st);
       run_grad<64, kGradK>(a, err, st);
