@@ -410,6 +410,19 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* er
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
 }
 
+// One lane of a converged warp.  The issuing warps run their loops with all
+// lanes and issue from this one: addresses and descriptors then stay in the
+// warp's uniform registers, which the matrix instructions take them from.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 // D (+)= A . B over 16 terms, fp16 operands, fp32 accumulator; A (a row per
 // lane, two terms per column) and D in tensor memory, B in shared memory.  B's
 // descriptor comes as its low word (see column_word and row_word): the high one
@@ -613,7 +626,7 @@ template <int DP>
 struct ForwardPlan {
   static constexpr int kHalves = DP / 64;
   static constexpr int kSlots = DP == 64 ? 5 : 4;
-  static constexpr int kSmem = 1024 + kTileBytes<DP> + kSlots * kSlotBytes + 6144;
+  static constexpr int kSmem = 1024 + kTileBytes<DP> + kSlots * kSlotBytes + 9216;
 };
 
 struct ForwardArgs {
@@ -694,15 +707,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   const uint32_t q_smem = smem_u32(smem);
   const uint32_t slots = q_smem + kTileBytes<DP>;
   uint8_t* misc = smem + kTileBytes<DP> + Plan::kSlots * kSlotBytes;
-  float* ref = (float*)misc;            // [2][128] reference exponents of a tile's rows
-  float* sum = ref + 2 * kTile;         // [2][2][128] sums of each half of the tile's columns
-  float* most = sum + 4 * kTile;        // [2][2][128] greatest scores of each half
+  float* ref = (float*)misc;            // [4][128] reference exponents of a tile's rows
+  float* sum = ref + 4 * kTile;         // [4][2][128] sums of each half of the tile's columns
+  float* most = sum + 8 * kTile;        // [2][2][128] greatest scores of each half
   uint64_t* bars = (uint64_t*)(most + 4 * kTile);
   const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8, slot_full = q_empty + 8;
   const uint32_t slot_empty = slot_full + 8 * Plan::kSlots, s_full = slot_empty + 8 * Plan::kSlots;
-  const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16, st_empty = o_empty + 16;
-  const uint32_t pair_full = st_empty + 16, q_ready = pair_full + 32, drained = q_ready + 8;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 18);
+  const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16;
+  const uint32_t pair_full = o_empty + 16, q_ready = pair_full + 32, drained = q_ready + 8;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 16);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 8);
@@ -713,7 +726,6 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       mbar_init(p_full + 8 * i, 8);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, 8);
-      mbar_init(st_empty + 8 * i, 8);
     }
     for (int i = 0; i < 4; ++i) mbar_init(pair_full + 8 * i, 2);
     mbar_init(drained, 1);
@@ -729,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   tc_fence_after();
   // Tensor memory: the query tile (DP columns), two buffers of scores (128 each) and of values (DP; one if DP is 128).
   constexpr int kOut = DP == 64 ? 2 : 1;
-  const uint32_t tmem = *tmem_slot, tmem_s = tmem + DP, tmem_o = tmem_s + 2 * kTile;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_s = tmem + DP, tmem_o = tmem_s + 2 * kTile;
 
   if (warp >= 18) {
     fewer_registers<kFewRegs>();
@@ -781,47 +793,52 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   } else if (warp == 17) {
     fewer_registers<kFewRegs>();
     constexpr uint32_t kScore = umma_idesc(kTile, false), kValue = umma_idesc(DP, true);
+    const bool leader = elect_one();
     uint32_t it = 0, gi = 0, item = 0;  // slots, tiles and items issued so far
     bool ok = true;
     auto values = [&](uint32_t t) {  // of tile t of the stream
       const uint32_t p = tmem_s + (t & 1) * kTile, out = t % kOut, d = tmem_o + out * DP;
-      ok = mbar_wait(p_full + 8 * (t & 1), (t >> 1) & 1, err);
-      if (ok && t >= kOut) ok = mbar_wait(o_empty + 8 * out, (t / kOut - 1) & 1, err);
+      ok = warp_wait(p_full + 8 * (t & 1), (t >> 1) & 1, err);
+      if (ok && t >= kOut) ok = warp_wait(o_empty + 8 * out, (t / kOut - 1) & 1, err);
       for (int x = 0; x < kHalves && ok; ++x, ++it) {
         const uint32_t slot = it % Plan::kSlots;
-        ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
+        ok = warp_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
         if (!ok) break;
         tc_fence_after();
         constexpr int kSteps = kTile / 16 / kHalves;
         constexpr uint32_t kStride = kBox / kHalves;  // between the slot's boxes
         const uint32_t v = row_word(slots + slot * kSlotBytes, kStride);
         const uint32_t px = p + split_col(x * kSteps);
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const uint32_t ph = px + split_col(k), vh = v + k * kRowStep, vl = vh + (kBox >> 4);
-          umma_ts(d, ph + 16, vh, kValue, x != 0 || k != 0);
-          umma_ts(d, ph, vl, kValue, 1u);
-          umma_ts(d, ph, vh, kValue, 1u);
+          for (int k = 0; k < kSteps; ++k) {
+            const uint32_t ph = px + split_col(k), vh = v + k * kRowStep, vl = vh + (kBox >> 4);
+            umma_ts(d, ph + 16, vh, kValue, x != 0 || k != 0);
+            umma_ts(d, ph, vl, kValue, 1u);
+            umma_ts(d, ph, vh, kValue, 1u);
+          }
+          umma_commit(slot_empty + 8 * slot);
+          if (x == kHalves - 1) umma_commit(o_full + 8 * out);
         }
-        umma_commit(slot_empty + 8 * slot);
+        __syncwarp();
       }
-      if (ok) umma_commit(o_full + 8 * out);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (lane == 0 && t.n > 0) {
-        ok = mbar_wait(q_ready, item & 1, err);
-        ++item;
-        for (int i = 0; i <= t.n && ok; ++i) {
-          if (i < t.n) {
-            const uint32_t d = tmem_s + (gi & 1) * kTile;
-            for (int x = 0; x < kHalves && ok; ++x, ++it) {
-              const uint32_t slot = it % Plan::kSlots;
-              ok = mbar_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t q = tmem + 32 * x, key = column_word(slots + slot * kSlotBytes);
+      const int n = __shfl_sync(0xffffffffu, query_item(s, w, a.fq, a.fk, a.fv, err).n, 0);
+      if (n == 0) continue;
+      ok = warp_wait(q_ready, item & 1, err);
+      ++item;
+      for (int i = 0; i <= n && ok; ++i) {
+        if (i < n) {
+          const uint32_t d = tmem_s + (gi & 1) * kTile;
+          for (int x = 0; x < kHalves && ok; ++x, ++it) {
+            const uint32_t slot = it % Plan::kSlots;
+            ok = warp_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t q = tmem + 32 * x, key = column_word(slots + slot * kSlotBytes);
+            if (leader) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t qh = q + 8 * k, ql = qh + DP / 2, kh = key + k * kColumnStep, kl = kh + (kBox >> 4);
@@ -830,18 +847,18 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
                 umma_ts(d, qh, kh, kScore, 1u);
               }
               umma_commit(slot_empty + 8 * slot);
+              if (x == kHalves - 1) umma_commit(s_full + 8 * (gi & 1));
             }
-            if (!ok) break;
-            umma_commit(s_full + 8 * (gi & 1));
-            ++gi;
+            __syncwarp();
           }
-          // The values of the tile before (gi now counts the scores issued).
-          if (i > 0) values(gi - (i < t.n ? 2 : 1));
+          if (!ok) break;
+          ++gi;
         }
+        // The values of the tile before (gi now counts the scores issued).
+        if (i > 0) values(gi - (i < n ? 2 : 1));
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0 && !ok) {  // instructions in flight end before the block does
+    if (!ok && leader) {  // instructions in flight end before the block does
       umma_commit(drained);
       mbar_wait(drained, 0, err);
     }
@@ -899,8 +916,6 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         }
         m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
         // The row's other half is in the warp four further.
-        if (gi >= 2) ok = warp_wait(st_empty + 8 * buf, ((gi >> 1) - 1) & 1, err);
-        if (!ok) break;
         most[(buf * 2 + half) * kTile + row] = m0;
         __syncwarp();
         if (lane == 0) mbar_arrive(pair_full + 8 * (warp & 3));
@@ -920,8 +935,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           split32(v + 32 * c, r);
           tmem_st32(at + buf * kTile + 32 * c, r);
         }
-        sum[(buf * 2 + half) * kTile + row] = (l[0] + l[1]) + (l[2] + l[3]);
-        if (half == 0) ref[buf * kTile + row] = m0 == -INFINITY ? -INFINITY : c0;
+        // Four buffers: these scores come after the values of two tiles before
+        // were issued, which waited until the output warps had taken the tile
+        // before that, and its statistics.
+        sum[((gi & 3) * 2 + half) * kTile + row] = (l[0] + l[1]) + (l[2] + l[3]);
+        if (half == 0) ref[(gi & 3) * kTile + row] = m0 == -INFINITY ? -INFINITY : c0;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
@@ -949,10 +967,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         const uint32_t ob = gi % kOut;
         ok = warp_wait(p_full + 8 * buf, (gi >> 1) & 1, err);
         if (!ok) break;
-        const float c0 = ref[buf * kTile + row];
-        const float parts = sum[2 * buf * kTile + row] + sum[(2 * buf + 1) * kTile + row];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(st_empty + 8 * buf);
+        const float c0 = ref[(gi & 3) * kTile + row];
+        const float parts = sum[(gi & 3) * 2 * kTile + row] + sum[((gi & 3) * 2 + 1) * kTile + row];
         ok = warp_wait(o_full + 8 * ob, (gi / kOut) & 1, err);
         if (!ok) break;
         tc_fence_after();
@@ -1208,7 +1224,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot, tmem_s = tmem + Plan::kRows, tmem_o = tmem_s + kScoreBufs * Plan::kScoreCols;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_s = tmem + Plan::kRows, tmem_o = tmem_s + kScoreBufs * Plan::kScoreCols;
 
   // Index of the streamed tile of step i of head x of an item.
   auto column_tile = [&](const GradItem& t, int x, int i) {
@@ -1277,31 +1293,37 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   } else if (warp == 17) {
     fewer_registers<kFewRegs>();
     constexpr uint32_t kScore = umma_idesc(kStep, false), kSum = umma_idesc(DP, true);
+    const bool leader = elect_one();
     uint32_t gi = 0, item = 0;  // steps and items issued so far
     bool ok = true;
-    // D = resident rows (tensor memory) times 64 streamed ones; `release`: the ring's entries are free after it.
+    // D = resident rows (tensor memory) times 64 streamed ones, then `done`;
+    // `release`: the ring's entries are free after it.
     auto scores = [&](uint32_t d, uint32_t rows, uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries,
-                      bool release) {
+                      bool release, uint32_t done) {
       for (uint32_t part = 0; part < 2 && ok; ++part) {
         const uint32_t entry = 2 * gi + part, slot = entry % entries;
-        ok = mbar_wait(full + 8 * slot, (entry / entries) & 1, err);
+        ok = warp_wait(full + 8 * slot, (entry / entries) & 1, err);
         if (!ok) break;
         tc_fence_after();
+        const uint32_t c0 = column_word(ring + slot * kPart);
+        if (leader) {
 #pragma unroll
-        for (int x = 0; x < kHalves; ++x) {
-          const uint32_t r = rows + 32 * x, c = column_word(ring + slot * kPart + x * kStepBox);
+          for (int x = 0; x < kHalves; ++x) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t rh = r + 8 * k, rl = rh + DP / 2, ch = c + k * kColumnStep;
-            if (part == 0) {
-              umma_ts(d, rh, ch, kScore, x != 0 || k != 0);
-            } else {
-              umma_ts(d, rl, ch, kScore, 1u);
-              umma_ts(d, rh, ch, kScore, 1u);
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t rh = rows + 32 * x + 8 * k, rl = rh + DP / 2, ch = c0 + x * (kStepBox >> 4) + k * kColumnStep;
+              if (part == 0) {
+                umma_ts(d, rh, ch, kScore, x != 0 || k != 0);
+              } else {
+                umma_ts(d, rl, ch, kScore, 1u);
+                umma_ts(d, rh, ch, kScore, 1u);
+              }
             }
           }
+          if (release) umma_commit(empty + 8 * slot);
+          if (part == 1) umma_commit(done);
         }
-        if (release) umma_commit(empty + 8 * slot);
+        __syncwarp();
       }
     };
     // The sums of step t: P or dS (in tensor memory) times the 64 rows of a ring step.
@@ -1310,54 +1332,51 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       const uint32_t p = tmem_s + buf * Plan::kScoreCols, d = tmem_o + out * DP;
       const uint32_t ring = PASS == kGradV ? ring2 : ring1, full = PASS == kGradV ? full2 : full1;
       const uint32_t empty = PASS == kGradV ? empty2 : empty1, entries = PASS == kGradV ? kHalves2 : kHalves1;
-      ok = mbar_wait(p_full + 8 * buf, (t / kScoreBufs) & 1, err);
-      if (ok && t >= kOutBufs) ok = mbar_wait(o_empty + 8 * out, (t / kOutBufs - 1) & 1, err);
+      ok = warp_wait(p_full + 8 * buf, (t / kScoreBufs) & 1, err);
+      if (ok && t >= kOutBufs) ok = warp_wait(o_empty + 8 * out, (t / kOutBufs - 1) & 1, err);
       for (uint32_t part = 0; part < 2 && ok; ++part) {
         const uint32_t entry = 2 * t + part, slot = entry % entries;
-        ok = mbar_wait(full + 8 * slot, (entry / entries) & 1, err);
+        ok = warp_wait(full + 8 * slot, (entry / entries) & 1, err);
         if (!ok) break;
         tc_fence_after();
         const uint32_t c = row_word(ring + slot * kPart, kStepBox);
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < kStep / 16; ++k) {
-          const uint32_t ph = p + split_col(k), ch = c + k * kRowStep;
-          if (part == 0) {
-            umma_ts(d, ph, ch, kSum, k != 0);
-          } else {
-            umma_ts(d, ph + 16, ch, kSum, 1u);
-            umma_ts(d, ph, ch, kSum, 1u);
+          for (int k = 0; k < kStep / 16; ++k) {
+            const uint32_t ph = p + split_col(k), ch = c + k * kRowStep;
+            if (part == 0) {
+              umma_ts(d, ph, ch, kSum, k != 0);
+            } else {
+              umma_ts(d, ph + 16, ch, kSum, 1u);
+              umma_ts(d, ph, ch, kSum, 1u);
+            }
           }
+          umma_commit(empty + 8 * slot);
+          if (part == 1) umma_commit(o_full + 8 * out);
         }
-        umma_commit(empty + 8 * slot);
+        __syncwarp();
       }
-      if (ok) umma_commit(o_full + 8 * out);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<PASS>(a, w, err);
-      if (lane == 0 && t.f0 < t.f1) {
-        ok = mbar_wait(a_ready, item & 1, err);
-        ++item;
-        const int steps = t.f1 - t.f0;
-        for (int i = 0; i < steps && ok; ++i) {
-          const uint32_t buf = gi % kScoreBufs, d = tmem_s + buf * Plan::kScoreCols;
-          scores(d, tmem, ring1, full1, empty1, kHalves1, PASS == kGradV);
-          if (ok) umma_commit(s_full + 8 * buf);
-          if (kTwo && ok) {
-            scores(d + kStep, tmem + DP, ring2, full2, empty2, kHalves2, true);
-            if (ok) umma_commit(d_full + 8 * buf);
-          }
-          if (!ok) break;
-          ++gi;
-          // With one buffer this step's sums, with two the ones of the step before.
-          if (kScoreBufs == 1) sums(gi - 1);
-          else if (i > 0) sums(gi - 2);
-        }
-        if (kScoreBufs == 2 && ok) sums(gi - 1);
+      const int steps = __shfl_sync(0xffffffffu, t.f1 - t.f0, 0);
+      if (steps <= 0) continue;
+      ok = warp_wait(a_ready, item & 1, err);
+      ++item;
+      for (int i = 0; i < steps && ok; ++i) {
+        const uint32_t buf = gi % kScoreBufs, d = tmem_s + buf * Plan::kScoreCols;
+        scores(d, tmem, ring1, full1, empty1, kHalves1, PASS == kGradV, s_full + 8 * buf);
+        if (kTwo && ok) scores(d + kStep, tmem + DP, ring2, full2, empty2, kHalves2, true, d_full + 8 * buf);
+        if (!ok) break;
+        ++gi;
+        // With one buffer this step's sums, with two the ones of the step before.
+        if (kScoreBufs == 1) sums(gi - 1);
+        else if (i > 0) sums(gi - 2);
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (kScoreBufs == 2 && ok) sums(gi - 1);
     }
-    if (lane == 0 && !ok) {  // instructions in flight end before the block does
+    if (!ok && leader) {  // instructions in flight end before the block does
       umma_commit(drained);
       mbar_wait(drained, 0, err);
     }
@@ -1564,11 +1583,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   }
 }
 
-// Adds the segments of one key tile in order: one block per 32 rows of a tile.
+// Adds the segments of one key tile in order, `rows` rows per block: few for a
+// sink tile, whose many segments few blocks would read one after the other.
 template <int DP, int PASS>
-__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int* err) {
+__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int rows, int* err) {
   const AttentionShape& s = a.s;
-  const int tile = blockIdx.x / 4, rows = blockIdx.x % 4 * 32;
+  const int tile = blockIdx.x / (kTile / rows), row0 = blockIdx.x % (kTile / rows) * rows;
   // The tile's first segment; the next ones follow `stride` units apart.
   const int unit = first + tile / stride * segs * stride + tile % stride;
   const GradItem t = grad_item<PASS>(a, unit, err);
@@ -1577,11 +1597,11 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
   float* grad = PASS == kGradK ? a.dk : a.dv;
   const int add = PASS == kGradK ? a.add_k : a.add_v;
   const float by = PASS == kGradK ? s.scale : 1.0f;
-  for (int i = threadIdx.x; i < 32 * DP; i += 256) {
-    const int r = rows + i / DP, c = i % DP;
+  for (int i = threadIdx.x; i < rows * DP; i += 256) {
+    const int r = row0 + i / DP, c = i % DP;
     if (t.r0 + r >= s.k_len || c >= s.head_dim) continue;
     float sum = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < used; ++k) sum += a.part[((int64_t)(unit + k * stride) * kTile + r) * DP + c];
     float* dst = grad + row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len) + c;
     *dst = add ? *dst + sum * by : sum * by;
@@ -1986,19 +2006,20 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   const AttentionShape& s = a.s;
   const int64_t items = PASS == kGradQ ? (int64_t)tiles_of(s.q_len) * s.heads * s.batch : grad_units(s, a.seg);
   if (items == 0) return;
-  if (items > INT_MAX / 4) throw CudaError("window_attention: too many keys");
+  if (items > INT_MAX / 64) throw CudaError("window_attention: too many keys");
   grad_kernel<DP, PASS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
   if (PASS == kGradQ) return;
   const int stride = s.kv_heads * s.batch, of_long = a.seg.long_tiles * a.seg.long_segs * stride;
   if (a.seg.long_segs > 1 && a.seg.long_tiles > 0) {
-    grad_join_kernel<DP, PASS><<<(unsigned)(a.seg.long_tiles * stride * 4), 256, 0, st>>>(
-        a, 0, a.seg.long_segs, stride, err);
+    const int rows = s.window > 0 ? 2 : 32;
+    grad_join_kernel<DP, PASS><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
+        a, 0, a.seg.long_segs, stride, rows, err);
     check_launch();
   }
   if (a.seg.short_segs > 1 && tiles_of(s.k_len) > a.seg.long_tiles) {
     grad_join_kernel<DP, PASS><<<(unsigned)((tiles_of(s.k_len) - a.seg.long_tiles) * stride * 4), 256, 0, st>>>(
-        a, of_long, a.seg.short_segs, stride, err);
+        a, of_long, a.seg.short_segs, stride, 32, err);
     check_launch();
   }
 }
