@@ -1027,28 +1027,36 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 
 // ---- gradients ------------------------------------------------------------------------------
 
-// Three passes of one pipeline, each summing its own gradient in a fixed order
+// Two passes of one pipeline, each summing its own gradients in a fixed order
 // (one pass for all three would have to add into dq from many blocks):
 //
-//   pass      rows (resident)   columns (streamed)   second product   summed
-//   kGradQ    queries: Q, dO    keys: K, V           dP = dO.V^T      dq += dS.K
-//   kGradK    keys: K, V        queries: Q, dO       dP^T = V.dO^T    dk += dS^T.Q
-//   kGradV    keys: K           queries: Q, dO       none             dv += P^T.dO
+//   pass      rows (resident)    columns (streamed)   summed
+//   queries   queries: Q, dO     keys: K, V           dq += dS.K
+//   keys      keys: K, V         queries: Q, dO       dv += P^T.dO, dk += dS^T.Q
 //
-// A work item is 128 rows; its columns come in steps of 64.  Each step forms
-// the scores (and dP), then P = 2^(score - max) / sum and dS = P (dP - delta)
-// replace the scores as fp16 halves, an operand for the step's third product,
-// which is added to fp32 registers.  dS is brought near 2^15 by a power of two
-// from |dS| <= |dO_i| |V_j| + |delta_i|, with the norms of single rows on the
-// resident side and a tile's greatest on the streamed one.
-// Roles as in forward_kernel, the resident tiles in tensor memory
-// (rows_to_tmem).  With two of them, 128 wide, there is room for one buffer of
-// scores and dP: a step's sums then come before the next one's scores, and P is
-// formed while dP is still being summed.  Elsewhere two steps overlap.
+// A work item is 128 rows; its columns come in steps of 64.  A step forms the
+// scores Q.K^T and dP = dO.V^T (or their transposes); P = 2^(score - max) / sum
+// and dS = P (dP - delta) become fp16 halves in tensor memory, operands of the
+// step's sums, which are added to fp32 registers.  P is at most 1; dS is
+// brought near 2^15 by a power of two from |dS| <= |dO_i| |V_j| + |delta_i|, with
+// the norms of single rows on the resident side and a tile's greatest on the
+// streamed one.
+//   warps 0-3    P and dS: a thread owns a row,
+//   warps 4-11   sums into registers, half of the columns each,
+//   warp 12      copies: resident tiles of the next item, rings of half steps (a
+//                step's lo boxes, then its hi ones),
+//   warp 13      matrix instructions.  Of a step g: dv of g, the scores of g + 1,
+//                dq or dk of g, dP of g + 1.  P of a step is formed while the
+//                last step's dS is summed, and its dS while the next scores are.
+// Resident tiles are in tensor memory (rows_to_tmem), with one buffer each of
+// scores (keys: then P) and of dP (then dS), and two of 64 columns of sums.
 // A key tile's queries may be many (a sink's are all that follow): its steps
 // are cut into segments that go to different blocks, each leaving its part in
 // the workspace, joined in order by grad_join_kernel.
-enum GradPass { kGradQ, kGradK, kGradV };
+constexpr int kGradThreads = 16 * 32;  // warps 14 and 15 only hold registers for the others
+// Launched with 128 registers a thread, 512 for the four warps of each quarter
+// of an SM; after the split 144 + 2 x 160 + 48 = 512.
+constexpr int kProbRegs = 144, kSumRegs = 160, kGradFewRegs = 48;
 constexpr int kStep = 64;
 constexpr int kStepBox = kStep * 128;  // bytes of 64 rows of a box
 
@@ -1068,34 +1076,28 @@ struct GradArgs {
   const float4* info;                  // of query rows
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
-  Segments seg;                        // of the key tiles' steps
-  float* part;                         // [unit][128][DP]
+  Segments seg;
+  float* part;                         // [unit][dk, dv][128][DP]
 };
 
-template <int DP, int PASS>
+template <int DP, bool KEYS>
 struct GradPlan {
   static constexpr int kHalves = DP / 64;
-  static constexpr bool kTwo = PASS != kGradV;           // dP is needed
-  static constexpr int kPart = kHalves * kStepBox;       // a step's hi or lo half
-  static constexpr int kFirstSteps = 2;                  // ring of the operand of the scores
-  static constexpr int kSecondSteps = PASS == kGradV ? 2 : 1;
-  static constexpr int kResident = (kTwo ? 2 : 1) * kTileBytes<DP>;
-  static constexpr int kInfo = PASS == kGradQ ? 0 : 2 * kStep * 16;
-  static constexpr int kRing = 2 * (kFirstSteps + kSecondSteps);  // half steps
-  static constexpr int kRows = (kTwo ? 2 : 1) * DP;      // tensor memory: resident tiles,
-  static constexpr int kScoreBufs = kTwo && DP == 128 ? 1 : 2;
-  static constexpr int kScoreCols = (kTwo ? 2 : 1) * kStep;  // buffers of scores (and dP),
-  static constexpr int kOutBufs = kTwo && DP == 128 ? 1 : 2;  // and of DP columns of sums
-  static_assert(kRows + kScoreBufs * kScoreCols + kOutBufs * DP <= 512, "tensor memory");
-  static constexpr int kSmem = kResident + kRing * kPart + kInfo + 512;
+  static constexpr int kPart = kHalves * kStepBox;  // a step's hi or lo half
+  static constexpr int kEntries1 = 4;               // ring of the scores' operand, used twice: two steps
+  static constexpr int kEntries2 = 2;               // ring of dP's operand: one step
+  static constexpr int kResident = 2 * kTileBytes<DP>;
+  static constexpr int kInfo = KEYS ? 2 * kStep * 16 : 0;
+  static constexpr int kSmem = kResident + (kEntries1 + kEntries2) * kPart + kInfo + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory of one block");
+  static_assert(2 * DP + 4 * kStep <= 512, "tensor memory");
 };
 
 // 128 rows of one head and the steps of 64 columns they need.
 struct GradItem {
-  int b, h, g, r0, n;  // h: kGradQ's head; n: steps (per head: kGradK, kGradV); 0: none, or values not finite
+  int b, h, g, r0, n;  // h: the queries' head, or the first of the keys'; n: steps (keys: per head); 0: none, or values not finite
   Sequence sq;
-  RowRange rows;       // kGradQ
+  RowRange rows;       // queries
   TileRange range;     // in steps of 64
   int row_tile;        // index of the resident tile
   int f0, f1;          // the unit's part of the heads' steps, counted head by head
@@ -1103,7 +1105,7 @@ struct GradItem {
   bool first;          // the first of them
 };
 
-template <int PASS>
+template <bool KEYS>
 __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int* err) {
   const AttentionShape& s = a.s;
   GradItem t;
@@ -1111,7 +1113,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
   float sum;
   int seg = 0;
-  if (PASS == kGradQ) {
+  if (!KEYS) {
     const int tq = tiles_q - 1 - index / (s.heads * s.batch);
     t.h = index % s.heads;
     t.b = index / s.heads % s.batch;
@@ -1163,7 +1165,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     }
   }
   t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
-  const int total = (PASS == kGradQ ? 1 : group) * t.n, each = (total + t.segs - 1) / t.segs;
+  const int total = (KEYS ? group : 1) * t.n, each = (total + t.segs - 1) / t.segs;
   t.f0 = min(total, seg * each);
   t.f1 = min(total, t.f0 + each);
   t.first = seg == 0;
@@ -1177,46 +1179,69 @@ __device__ __forceinline__ int scale_exponent(float bound) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-template <int DP, int PASS>
-__global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
-  using Plan = GradPlan<DP, PASS>;
-  constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart, kScoreBufs = Plan::kScoreBufs, kOutBufs = Plan::kOutBufs;
-  constexpr bool kTwo = Plan::kTwo;
+// A thread's columns of a gradient row, stored or added.
+template <int N>
+__device__ __forceinline__ void store_row(float* __restrict__ dst, const float (&v)[N], float by, int cols, bool vec,
+                                          int add) {
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4)
+      if (c < cols) {
+        float4 o = make_float4(v[c] * by, v[c + 1] * by, v[c + 2] * by, v[c + 3] * by);
+        if (add) {
+          const float4 p = *(const float4*)(dst + c);
+          o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+        }
+        *(float4*)(dst + c) = o;
+      }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < cols) dst[c] = add ? dst[c] + v[c] * by : v[c] * by;
+  }
+}
+
+template <int DP, bool KEYS>
+__global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
+  using Plan = GradPlan<DP, KEYS>;
+  constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart;
+  constexpr uint32_t kEntries1 = Plan::kEntries1, kEntries2 = Plan::kEntries2;
   const AttentionShape& s = a.s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
   extern __shared__ __align__(1024) uint8_t smem[];  // at the start of shared memory, as there is no other
   const uint32_t base = smem_u32(smem);
-  const uint32_t ring1 = base + Plan::kResident, ring2 = ring1 + 2 * Plan::kFirstSteps * kPart;
-  uint8_t* info_smem = smem + Plan::kResident + Plan::kRing * kPart;
+  const uint32_t ring1 = base + Plan::kResident, ring2 = ring1 + kEntries1 * kPart;
+  uint8_t* info_smem = smem + Plan::kResident + (kEntries1 + kEntries2) * kPart;
   uint64_t* bars = (uint64_t*)(info_smem + Plan::kInfo);
-  constexpr int kHalves1 = 2 * Plan::kFirstSteps, kHalves2 = 2 * Plan::kSecondSteps;  // ring entries (half steps)
   const uint32_t a_full = smem_u32(bars), a_empty = a_full + 8, a_ready = a_empty + 8;
-  const uint32_t full1 = a_ready + 8, empty1 = full1 + 8 * kHalves1, full2 = empty1 + 8 * kHalves1;
-  const uint32_t empty2 = full2 + 8 * kHalves2, s_full = empty2 + 8 * kHalves2, d_full = s_full + 16;
-  const uint32_t p_full = d_full + 16, o_full = p_full + 16, o_empty = o_full + 16, drained = o_empty + 16;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 2 * kHalves1 + 2 * kHalves2 + 11);
+  const uint32_t full1 = a_ready + 8, empty1 = full1 + 8 * kEntries1, full2 = empty1 + 8 * kEntries1;
+  const uint32_t empty2 = full2 + 8 * kEntries2, s_full = empty2 + 8 * kEntries2, d_full = s_full + 8;
+  const uint32_t s_done = d_full + 8, ds_full = s_done + 8, o_full = ds_full + 8, o_empty = o_full + 16;
+  const uint32_t drained = o_empty + 16;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 3 + 2 * kEntries1 + 2 * kEntries2 + 9);
   if ((base & 1023u) != 0) {  // the swizzle needs it
     if (threadIdx.x == 0) atomicCAS(err, 0, (int)kErrTmemAlloc);
     return;
   }
   if (threadIdx.x == 0) {
     mbar_init(a_full, 1);
-    mbar_init(a_empty, 8);
-    mbar_init(a_ready, 8);
-    for (int i = 0; i < kHalves1; ++i) mbar_init(full1 + 8 * i, 1), mbar_init(empty1 + 8 * i, 1);
-    for (int i = 0; i < kHalves2; ++i) mbar_init(full2 + 8 * i, 1), mbar_init(empty2 + 8 * i, 1);
+    mbar_init(a_empty, 4);
+    mbar_init(a_ready, 4);
+    for (int i = 0; i < (int)kEntries1; ++i) mbar_init(full1 + 8 * i, 1), mbar_init(empty1 + 8 * i, 1);
+    for (int i = 0; i < (int)kEntries2; ++i) mbar_init(full2 + 8 * i, 1), mbar_init(empty2 + 8 * i, 1);
+    mbar_init(s_full, 1);
+    mbar_init(d_full, 1);
+    mbar_init(s_done, 4);
+    mbar_init(ds_full, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(d_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 8);
       mbar_init(o_full + 8 * i, 1);
-      mbar_init(o_empty + 8 * i, 8);
+      mbar_init(o_empty + 8 * i, kHalves == 2 ? 4 : 8);
     }
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 17) {
+  if (warp == 13) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -1224,25 +1249,28 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0), tmem_s = tmem + Plan::kRows, tmem_o = tmem_s + kScoreBufs * Plan::kScoreCols;
+  // Tensor memory: resident tiles, scores, dP, two buffers of sums.
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const uint32_t tmem_s = tmem + 2 * DP, tmem_d = tmem_s + kStep, tmem_o = tmem_d + kStep;
 
-  // Index of the streamed tile of step i of head x of an item.
-  auto column_tile = [&](const GradItem& t, int x, int i) {
-    return PASS == kGradQ ? (t.b * s.kv_heads + t.g) * tiles_k + t.range.at(i) / 2
-                          : (t.b * s.heads + t.h + x) * tiles_q + t.range.at(i) / 2;
+  // Index of the streamed tile of step n of an item's heads' steps.
+  auto column_tile = [&](const GradItem& t, int n, int* step) {
+    const int x = KEYS ? n / t.n : 0;
+    *step = t.range.at(n - x * t.n);
+    return KEYS ? (t.b * s.heads + t.h + x) * tiles_q + *step / 2 : (t.b * s.kv_heads + t.g) * tiles_k + *step / 2;
   };
 
-  if (warp >= 18) {
-    fewer_registers<kFewRegs>();
-  } else if (warp == 16) {
-    fewer_registers<kFewRegs>();
-    uint32_t it = 0, loaded = 0;  // half steps of each ring, items
+  if (warp >= 14) {
+    fewer_registers<kGradFewRegs>();
+  } else if (warp == 12) {
+    fewer_registers<kGradFewRegs>();
+    uint32_t gi = 0, loaded = 0;  // steps, items
     bool ok = true;
-    // Half a step of one ring: `part` 0 the lo boxes, 1 the hi ones, and with
-    // the latter the rows' statistics where `with_info`.
+    // Half a step of a ring: `part` 0 the lo boxes, 1 the hi ones; with the
+    // latter the rows' statistics where `with_info`.
     auto fill = [&](uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries, const uint8_t* packed, int tile,
-                    int step, int part, bool with_info) {
-      const uint32_t slot = it % entries, use = it / entries, bar = full + 8 * slot;
+                    int step, uint32_t part, bool with_info) {
+      const uint32_t entry = 2 * gi + part, slot = entry % entries, use = entry / entries, bar = full + 8 * slot;
       if (use > 0) ok = mbar_wait(empty + 8 * slot, (use - 1) & 1, err);
       if (!ok) return;
       mbar_expect_tx(bar, kPart + (with_info ? kStep * 16 : 0));
@@ -1251,32 +1279,29 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       for (int x = 0; x < kHalves; ++x)
         bulk_load(ring + slot * kPart + x * kStepBox, src + x * kBox, kStepBox, bar);
       if (with_info)
-        bulk_load(smem_u32(info_smem) + (it / 2 & 1) * (kStep * 16),
+        bulk_load(smem_u32(info_smem) + (gi & 1) * (kStep * 16),
                   (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16, bar);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const GradItem t = grad_item<PASS>(a, w, err);
+      const GradItem t = grad_item<KEYS>(a, w, err);
       if (lane == 0 && t.f0 < t.f1) {
         if (loaded > 0) ok = mbar_wait(a_empty, (loaded - 1) & 1, err);
         if (ok) {
           mbar_expect_tx(a_full, Plan::kResident);
           const int64_t at = (int64_t)t.row_tile * kTileBytes<DP>;
-          bulk_load(base, (PASS == kGradQ ? a.pq : a.pk) + at, kTileBytes<DP>, a_full);
-          if (kTwo) bulk_load(base + kTileBytes<DP>, (PASS == kGradQ ? a.po : a.pv) + at, kTileBytes<DP>, a_full);
+          bulk_load(base, (KEYS ? a.pk : a.pq) + at, kTileBytes<DP>, a_full);
+          bulk_load(base + kTileBytes<DP>, (KEYS ? a.pv : a.po) + at, kTileBytes<DP>, a_full);
           ++loaded;
         }
-        for (int f = t.f0; f < t.f1 && ok; ++f, it += 2) {
-          const int x = f / t.n, i = f - x * t.n, tile = column_tile(t, x, i), step = t.range.at(i);
+        for (int n = t.f0; n < t.f1 && ok; ++n, ++gi) {
+          int step;
+          const int tile = column_tile(t, n, &step);
           // The statistics come with the operand that stays until they have been used.
-          for (int part = 0; part < 2 && ok; ++part, ++it)
-            fill(ring1, full1, empty1, kHalves1, PASS == kGradQ ? a.pk : a.pq, tile, step, part,
-                 PASS == kGradK && part == 1);
-          it -= 2;
-          for (int part = 0; part < 2 && ok; ++part, ++it)
-            fill(ring2, full2, empty2, kHalves2, PASS == kGradQ ? a.pv : a.po, tile, step, part,
-                 PASS == kGradV && part == 1);
-          it -= 2;
+          fill(ring1, full1, empty1, kEntries1, KEYS ? a.pq : a.pk, tile, step, 0, false);
+          if (ok) fill(ring1, full1, empty1, kEntries1, KEYS ? a.pq : a.pk, tile, step, 1, KEYS);
+          if (ok) fill(ring2, full2, empty2, kEntries2, KEYS ? a.po : a.pv, tile, step, 0, false);
+          if (ok) fill(ring2, full2, empty2, kEntries2, KEYS ? a.po : a.pv, tile, step, 1, false);
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -1285,23 +1310,23 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       // Copies in flight end before the block does.  The last step may have
       // been begun only in part: a wait for a fill that never came runs out.
       if (loaded > 0) mbar_wait_limit(a_full, (loaded - 1) & 1, err, kWaitCycles / 8);
-      for (uint32_t f = it > kHalves1 ? it - kHalves1 : 0; f < it + 2; ++f) {
-        mbar_wait_limit(full1 + 8 * (f % kHalves1), (f / kHalves1) & 1, err, kWaitCycles / 8);
-        mbar_wait_limit(full2 + 8 * (f % kHalves2), (f / kHalves2) & 1, err, kWaitCycles / 8);
+      for (uint32_t f = gi > 1 ? 2 * gi - 2 : 0; f < 2 * gi + 2; ++f) {
+        mbar_wait_limit(full1 + 8 * (f % kEntries1), (f / kEntries1) & 1, err, kWaitCycles / 8);
+        mbar_wait_limit(full2 + 8 * (f % kEntries2), (f / kEntries2) & 1, err, kWaitCycles / 8);
       }
     }
-  } else if (warp == 17) {
-    fewer_registers<kFewRegs>();
-    constexpr uint32_t kScore = umma_idesc(kStep, false), kSum = umma_idesc(DP, true);
+  } else if (warp == 13) {
+    fewer_registers<kGradFewRegs>();
+    constexpr uint32_t kProduct = umma_idesc(kStep, false), kSum = umma_idesc(64, true);
     const bool leader = elect_one();
-    uint32_t gi = 0, item = 0;  // steps and items issued so far
+    uint32_t gi = 0, item = 0;           // steps whose scores, items that were issued
+    uint32_t sums0 = 0, sums1 = 0;       // sums issued into each buffer
     bool ok = true;
-    // D = resident rows (tensor memory) times 64 streamed ones, then `done`;
-    // `release`: the ring's entries are free after it.
-    auto scores = [&](uint32_t d, uint32_t rows, uint32_t ring, uint32_t full, uint32_t empty, uint32_t entries,
-                      bool release, uint32_t done) {
+    // D = resident rows (tensor memory) times the 64 streamed ones of step g, then `done`.
+    auto product = [&](uint32_t g, uint32_t d, uint32_t rows, uint32_t ring, uint32_t full, uint32_t entries,
+                       uint32_t done) {
       for (uint32_t part = 0; part < 2 && ok; ++part) {
-        const uint32_t entry = 2 * gi + part, slot = entry % entries;
+        const uint32_t entry = 2 * g + part, slot = entry % entries;
         ok = warp_wait(full + 8 * slot, (entry / entries) & 1, err);
         if (!ok) break;
         tc_fence_after();
@@ -1313,107 +1338,124 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
             for (int k = 0; k < 4; ++k) {
               const uint32_t rh = rows + 32 * x + 8 * k, rl = rh + DP / 2, ch = c0 + x * (kStepBox >> 4) + k * kColumnStep;
               if (part == 0) {
-                umma_ts(d, rh, ch, kScore, x != 0 || k != 0);
+                umma_ts(d, rh, ch, kProduct, x != 0 || k != 0);
               } else {
-                umma_ts(d, rl, ch, kScore, 1u);
-                umma_ts(d, rh, ch, kScore, 1u);
+                umma_ts(d, rl, ch, kProduct, 1u);
+                umma_ts(d, rh, ch, kProduct, 1u);
               }
             }
           }
-          if (release) umma_commit(empty + 8 * slot);
           if (part == 1) umma_commit(done);
         }
         __syncwarp();
       }
     };
-    // The sums of step t: P or dS (in tensor memory) times the 64 rows of a ring step.
-    auto sums = [&](uint32_t t) {
-      const uint32_t buf = t % kScoreBufs, out = t % kOutBufs;
-      const uint32_t p = tmem_s + buf * Plan::kScoreCols, d = tmem_o + out * DP;
-      const uint32_t ring = PASS == kGradV ? ring2 : ring1, full = PASS == kGradV ? full2 : full1;
-      const uint32_t empty = PASS == kGradV ? empty2 : empty1, entries = PASS == kGradV ? kHalves2 : kHalves1;
-      ok = warp_wait(p_full + 8 * buf, (t / kScoreBufs) & 1, err);
-      if (ok && t >= kOutBufs) ok = warp_wait(o_empty + 8 * out, (t / kOutBufs - 1) & 1, err);
-      for (uint32_t part = 0; part < 2 && ok; ++part) {
-        const uint32_t entry = 2 * t + part, slot = entry % entries;
-        ok = warp_wait(full + 8 * slot, (entry / entries) & 1, err);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t c = row_word(ring + slot * kPart, kStepBox);
-        if (leader) {
+    // A buffer of sums = P or dS (tensor memory) times 64 columns (x) of step g's 64 rows.
+    auto sum_half = [&](uint32_t g, uint32_t p, uint32_t ring, uint32_t entries, int x, uint32_t buf, uint32_t& count) {
+      if (count > 0) ok = warp_wait(o_empty + 8 * buf, (count - 1) & 1, err);
+      ++count;
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t lo = (2 * g) % entries, hi = (2 * g + 1) % entries, d = tmem_o + 64 * buf;
+      const uint32_t cl = row_word(ring + lo * kPart + x * kStepBox, kStepBox);
+      const uint32_t chi = row_word(ring + hi * kPart + x * kStepBox, kStepBox);
+      if (leader) {
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k) {
-            const uint32_t ph = p + split_col(k), ch = c + k * kRowStep;
-            if (part == 0) {
-              umma_ts(d, ph, ch, kSum, k != 0);
-            } else {
-              umma_ts(d, ph + 16, ch, kSum, 1u);
-              umma_ts(d, ph, ch, kSum, 1u);
-            }
-          }
-          umma_commit(empty + 8 * slot);
-          if (part == 1) umma_commit(o_full + 8 * out);
+        for (int k = 0; k < kStep / 16; ++k) {
+          umma_ts(d, p + split_col(k), cl + k * kRowStep, kSum, k != 0);
+          umma_ts(d, p + split_col(k) + 16, chi + k * kRowStep, kSum, 1u);
+          umma_ts(d, p + split_col(k), chi + k * kRowStep, kSum, 1u);
         }
-        __syncwarp();
+        umma_commit(o_full + 8 * buf);
       }
+      __syncwarp();
+    };
+    auto free_step = [&](uint32_t g, uint32_t empty, uint32_t entries) {
+      if (leader) {
+        umma_commit(empty + 8 * ((2 * g) % entries));
+        umma_commit(empty + 8 * ((2 * g + 1) % entries));
+      }
+      __syncwarp();
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const GradItem t = grad_item<PASS>(a, w, err);
+      const GradItem t = grad_item<KEYS>(a, w, err);
       const int steps = __shfl_sync(0xffffffffu, t.f1 - t.f0, 0);
       if (steps <= 0) continue;
       ok = warp_wait(a_ready, item & 1, err);
       ++item;
-      for (int i = 0; i < steps && ok; ++i) {
-        const uint32_t buf = gi % kScoreBufs, d = tmem_s + buf * Plan::kScoreCols;
-        scores(d, tmem, ring1, full1, empty1, kHalves1, PASS == kGradV, s_full + 8 * buf);
-        if (kTwo && ok) scores(d + kStep, tmem + DP, ring2, full2, empty2, kHalves2, true, d_full + 8 * buf);
+      if (ok) product(gi, tmem_s, tmem, ring1, full1, kEntries1, s_full);
+      if (ok) product(gi, tmem_d, tmem + DP, ring2, full2, kEntries2, d_full);
+      if (ok && !KEYS) free_step(gi, empty2, kEntries2);
+      for (int i = 0; i < steps && ok; ++i, ++gi) {
+        const bool more = i + 1 < steps;
+        ok = warp_wait(s_done, gi & 1, err);  // the scores have been read; keys: P is there
         if (!ok) break;
-        ++gi;
-        // With one buffer this step's sums, with two the ones of the step before.
-        if (kScoreBufs == 1) sums(gi - 1);
-        else if (i > 0) sums(gi - 2);
+        tc_fence_after();
+        if (KEYS) {
+          sum_half(gi, tmem_s, ring2, kEntries2, 0, 0, sums0);
+          if (kHalves == 2 && ok) sum_half(gi, tmem_s, ring2, kEntries2, 1, 1, sums1);
+          if (ok) free_step(gi, empty2, kEntries2);
+        }
+        if (ok && more) product(gi + 1, tmem_s, tmem, ring1, full1, kEntries1, s_full);
+        if (ok) ok = warp_wait(ds_full, gi & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        if (kHalves == 2) {
+          sum_half(gi, tmem_d, ring1, kEntries1, 0, 0, sums0);
+          if (ok) sum_half(gi, tmem_d, ring1, kEntries1, 1, 1, sums1);
+        } else {
+          sum_half(gi, tmem_d, ring1, kEntries1, 0, 1, sums1);
+        }
+        if (ok) free_step(gi, empty1, kEntries1);
+        if (ok && more) {
+          product(gi + 1, tmem_d, tmem + DP, ring2, full2, kEntries2, d_full);
+          if (ok && !KEYS) free_step(gi + 1, empty2, kEntries2);
+        }
       }
-      if (kScoreBufs == 2 && ok) sums(gi - 1);
     }
     if (!ok && leader) {  // instructions in flight end before the block does
       umma_commit(drained);
       mbar_wait(drained, 0, err);
     }
-  } else if (warp < 8) {
-    more_registers<kScoreRegs>();
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, at = tmem_s + lanes + half * 32;
+  } else if (warp < 4) {
+    more_registers<kProbRegs>();
+    const int row = warp * 32 + lane;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     uint32_t gi = 0, item = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const GradItem t = grad_item<PASS>(a, w, err);
+      const GradItem t = grad_item<KEYS>(a, w, err);
       if (t.n == 0 && t.first) {
-        if (PASS == kGradQ)
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
+        if (!KEYS)
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 4)
             simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
-        if (PASS == kGradK)  // and dv, which kGradV leaves out
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 8)
+        else
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 4)
             simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
       }
       if (t.f0 >= t.f1) continue;
-      // The products with the resident tiles before are done: their scores have been read.
+      // The products with the resident tiles before are done: they have been read.
       ok = warp_wait(a_full, item & 1, err);
       if (!ok) break;
-      rows_to_tmem<DP>(tmem + lanes, base, row, half);
-      if (kTwo) rows_to_tmem<DP>(tmem + DP + lanes, base + kTileBytes<DP>, row, half);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        rows_to_tmem<DP>(tmem + lanes, base, row, half);
+        rows_to_tmem<DP>(tmem + DP + lanes, base + kTileBytes<DP>, row, half);
+      }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(a_ready), mbar_arrive(a_empty);
       ++item;
-      // kGradQ: what the row sees and its statistics; else the key's rows [s0, s1) and its norm.
+      // Queries: what the row sees and its statistics; keys: the rows [s0, s1)
+      // that see the key, and its norm.
       RowMask mask = {0, 0, 0};
       float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       int s0 = 0, s1 = 0;
-      float norm = 0.0f;
-      if (PASS == kGradQ) {
+      float norm;
+      if (!KEYS) {
         QueryItem q;
         q.rows = t.rows, q.sq = t.sq, q.r0 = t.r0;
         mask = mask_of(s, q, row);
@@ -1421,155 +1463,157 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
         norm = st.w;
       } else {
         if (t.r0 + row < t.sq.n) rows_seeing(s, t.sq, t.r0 + row, &s0, &s1);
-        if (kTwo) norm = a.nv[(int64_t)t.row_tile * kTile + row];
+        norm = a.nv[(int64_t)t.row_tile * kTile + row];
       }
-      const float* f_row1 = PASS == kGradQ ? a.fq : a.fk;
-      const double to_log2 = (double)f_row1[t.row_tile] * (double)s.scale * 1.4426950408889634;
-      const float f_row2 = PASS == kGradQ ? a.fo[t.row_tile] : kTwo ? a.fv[t.row_tile] : 0.0f;
+      const double to_log2 = (double)(KEYS ? a.fk : a.fq)[t.row_tile] * (double)s.scale * 1.4426950408889634;
+      const float f_row = (KEYS ? a.fv : a.fo)[t.row_tile];
       for (int n = t.f0; n < t.f1; ++n, ++gi) {
-        const uint32_t buf = gi % kScoreBufs, phase = (gi / kScoreBufs) & 1;
-        const int x = n / t.n, i = n - x * t.n;
-        const int step = t.range.at(i), tile = column_tile(t, x, i), c0 = step * kStep;
-        const float f = (float)(to_log2 * (double)(PASS == kGradQ ? a.fk : a.fq)[tile]);
+        int step;
+        const int tile = column_tile(t, n, &step), c0 = step * kStep;
+        const float f = (float)(to_log2 * (double)(KEYS ? a.fq : a.fk)[tile]);
+        const float f2 = f_row * (KEYS ? a.fo : a.fv)[tile];
+        const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
+        const float up = power_of_two(scale_exponent(bound));
         bool whole;
-        uint32_t seen = 0xffffffffu;
-        if (PASS == kGradQ) {
+        uint32_t seen[2];
+        if (!KEYS) {
           whole = t.rows.all && c0 + kStep - 1 <= t.rows.p0 &&
                   (s.window == 0 || t.rows.p1 - c0 < s.window || c0 + kStep <= s.sinks);
-          if (!whole) seen = seen_bits(mask, c0 + 32 * half);
+          seen[0] = seen_bits(mask, c0);
+          seen[1] = seen_bits(mask, c0 + 32);
         } else {
           const int first = t.sq.start + c0, last = first + kStep - 1, k1 = t.r0 + kTile - 1;
           whole = k1 <= first && last < t.sq.n && c0 + kStep <= s.q_len &&
                   (s.window == 0 || last - t.r0 < s.window || k1 < s.sinks);
-          if (!whole) seen = bits_between(s0, s1, c0 + 32 * half);
+          seen[0] = bits_between(s0, s1, c0);
+          seen[1] = bits_between(s0, s1, c0 + 32);
         }
-        float up = 16384.0f;  // P <= 1
-        float f2 = 0.0f;
-        if (kTwo) {
-          const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] +
-                              (PASS == kGradQ ? fabsf(st.z) : a.tdo[tile]);
-          up = power_of_two(scale_exponent(bound));
-          f2 = f_row2 * (PASS == kGradQ ? a.fv : a.fo)[tile];
-        }
-        ok = warp_wait(s_full + 8 * buf, phase, err);
-        if (PASS != kGradQ && ok) {  // the statistics' copy, with the second half of its step
-          const uint32_t entries = PASS == kGradV ? kHalves2 : kHalves1, entry = 2 * gi + 1;
-          ok = warp_wait((PASS == kGradV ? full2 : full1) + 8 * (entry % entries), (entry / entries) & 1, err);
+        ok = warp_wait(s_full, gi & 1, err);
+        if (KEYS && ok) {  // the statistics' copy, with the second half of its step
+          const uint32_t entry = 2 * gi + 1;
+          ok = warp_wait(full1 + 8 * (entry % kEntries1), (entry / kEntries1) & 1, err);
         }
         if (!ok) break;
         tc_fence_after();
-        const uint32_t here = at + buf * Plan::kScoreCols;
-        const float4* col = (const float4*)(info_smem + (gi & 1) * (kStep * 16)) + 32 * half;
-        float v[32];
-        tmem_ld32(here, v);
+        const float4* col = (const float4*)(info_smem + (gi & 1) * (kStep * 16));
+        float v[64];
+        tmem_ld64(tmem_s + lanes, v);
+        if (!KEYS) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_done);
+        }
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!(seen >> e & 1u)) v[e] = -INFINITY;
+          for (int e = 0; e < 64; ++e)
+            if (!(seen[e / 32] >> (e & 31) & 1u)) v[e] = -INFINITY;
         }
         const float scaled = st.y * up;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          if (PASS == kGradQ) {
+        for (int e = 0; e < 64; ++e) {
+          if (!KEYS) {
             v[e] = exp2_fast(fmaf(v[e], f, -st.x)) * scaled;
           } else {
             const float2 c = *(const float2*)&col[e];
-            v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * up);
+            v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * 16384.0f);
           }
         }
-        if (kTwo) {
-          ok = warp_wait(d_full + 8 * buf, phase, err);
-          if (!ok) break;
-          tc_fence_after();
-          float d[32];
-          tmem_ld32(here + kStep, d);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] *= fmaf(d[e], f2, PASS == kGradQ ? -st.z : -col[e].z);
-        }
         uint32_t r[32];
-        split32(v, r);
-        tmem_st32(here, r);
+        if (KEYS) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            split32(v + 32 * c, r);
+            tmem_st32(tmem_s + lanes + 32 * c, r);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_done);
+        }
+        ok = warp_wait(d_full, gi & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        const float rescale = up * 0x1p-14f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float d[32];
+          tmem_ld32(tmem_d + lanes + 32 * c, d);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (!KEYS) d[e] = v[32 * c + e] * fmaf(d[e], f2, -st.z);
+            else d[e] = v[32 * c + e] * (fmaf(d[e], f2, -col[32 * c + e].z) * rescale);
+          }
+          split32(d, r);
+          tmem_st32(tmem_d + lanes + 32 * c, r);
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 8 * buf);
+        if (lane == 0) mbar_arrive(ds_full);
       }
     }
   } else {
-    fewer_registers<kOutputRegs>();
+    more_registers<kSumRegs>();
     constexpr int kCols = DP / 2;  // columns of a thread
-    const int quad = warp & 3, half = (warp - 8) >> 2, row = quad * 32 + lane;
-    const uint32_t at = tmem_o + ((uint32_t)(quad * 32) << 16) + half * kCols;
-    uint32_t gi = 0;
+    const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t taken0 = 0, taken1 = 0;  // sums taken from each buffer
     bool ok = true;
+    // acc += by * the next sums of buffer `buf`.
+    auto take = [&](float (&acc)[kCols], float by, uint32_t buf, uint32_t& taken) {
+      ok = warp_wait(o_full + 8 * buf, taken & 1, err);
+      ++taken;
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t at = tmem_o + lanes + 64 * buf + (kHalves == 2 ? 0 : half * kCols);
+#pragma unroll
+      for (int c = 0; c < kCols; c += 16) {
+        float v[16];
+        tmem_ld16(at + c, v);
+        if (c == kCols - 16) {  // the last values are out: the buffer is free
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_empty + 8 * buf);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], by, acc[c + e]);
+      }
+    };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const GradItem t = grad_item<PASS>(a, w, err);
+      const GradItem t = grad_item<KEYS>(a, w, err);
       if (t.f0 >= t.f1) continue;
-      float norm = 0.0f, delta = 0.0f;
-      if (PASS == kGradQ) {
-        const float4 st = a.info[(int64_t)t.row_tile * kTile + row];
-        norm = st.w;
-        delta = fabsf(st.z);
-      } else if (kTwo) {
-        norm = a.nv[(int64_t)t.row_tile * kTile + row];
-      }
-      float acc[kCols];
+      const float4 st = KEYS ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a.info[(int64_t)t.row_tile * kTile + row];
+      const float norm = KEYS ? a.nv[(int64_t)t.row_tile * kTile + row] : st.w;
+      float acc[kCols], acc_v[kCols];  // acc_v: keys only
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
-      for (int n = t.f0; n < t.f1; ++n, ++gi) {
-        const uint32_t out = gi % kOutBufs;
-        const int x = n / t.n, tile = column_tile(t, x, n - x * t.n);
-        float down = 0x1p-14f * (PASS == kGradV ? a.fo[tile] : 1.0f);
-        if (kTwo) {
-          const float bound = norm * (PASS == kGradQ ? a.tnv : a.tno)[tile] + (PASS == kGradQ ? delta : a.tdo[tile]);
-          down = power_of_two(-scale_exponent(bound)) * (PASS == kGradQ ? a.fk : a.fq)[tile];
+      for (int c = 0; c < kCols; ++c) acc[c] = acc_v[c] = 0.0f;
+      for (int n = t.f0; n < t.f1 && ok; ++n) {
+        int step;
+        const int tile = column_tile(t, n, &step);
+        const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
+        const float down = power_of_two(-scale_exponent(bound)) * (KEYS ? a.fq : a.fk)[tile];
+        if (KEYS) {
+          const float down_v = 0x1p-14f * a.fo[tile];
+          if (kHalves == 1 || half == 0) take(acc_v, down_v, 0, taken0);
+          else take(acc_v, down_v, 1, taken1);
+          if (!ok) break;
         }
-        ok = warp_wait(o_full + 8 * out, (gi / kOutBufs) & 1, err);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < kCols; c += 16) {
-          float v[16];
-          tmem_ld16(at + out * DP + c, v);
-          if (c == kCols - 16) {  // the last values are out: the buffer is free
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(o_empty + 8 * out);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], down, acc[c + e]);
-        }
+        if (kHalves == 2 && half == 0) take(acc, down, 0, taken0);
+        else take(acc, down, 1, taken1);
       }
-      const int r = t.r0 + row;
+      const int r = t.r0 + row, cols = s.head_dim - half * kCols;
       if (ok && t.segs > 1) {
-        float* dst = a.part + ((int64_t)w * kTile + row) * DP + half * kCols;
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4)
-          *(float4*)(dst + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-      } else if (ok && r < (PASS == kGradQ ? s.q_len : s.k_len)) {
-        const float by = PASS == kGradV ? 1.0f : s.scale;
-        float* grad = PASS == kGradQ ? a.dq : PASS == kGradK ? a.dk : a.dv;
-        const int add = PASS == kGradQ ? a.add_q : PASS == kGradK ? a.add_k : a.add_v;
-        float* dst = grad + half * kCols +
-                     (PASS == kGradQ ? row_at(s, t.b, t.h, r, s.heads, s.q_len) : row_at(s, t.b, t.g, r, s.kv_heads, s.k_len));
-        const int cols = s.head_dim - half * kCols;
-        if (s.head_dim % 4 == 0 && ((uintptr_t)grad & 15) == 0) {
-#pragma unroll
-          for (int c = 0; c < kCols; c += 4)
-            if (c < cols) {
-              float4 o = make_float4(acc[c] * by, acc[c + 1] * by, acc[c + 2] * by, acc[c + 3] * by);
-              if (add) {
-                const float4 p = *(const float4*)(dst + c);
-                o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
-              }
-              *(float4*)(dst + c) = o;
-            }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-            if (c < cols) dst[c] = add ? dst[c] + acc[c] * by : acc[c] * by;
-        }
+        float* dst = a.part + ((int64_t)w * 2 * kTile + row) * DP + half * kCols;
+        store_row(dst, acc, s.scale, kCols, true, 0);
+        store_row(dst + kTile * DP, acc_v, 1.0f, kCols, true, 0);
+      } else if (ok && KEYS && r < s.k_len) {
+        const int64_t at = row_at(s, t.b, t.g, r, s.kv_heads, s.k_len) + half * kCols;
+        store_row(a.dk + at, acc, s.scale, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dk & 15) == 0, a.add_k);
+        store_row(a.dv + at, acc_v, 1.0f, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dv & 15) == 0, a.add_v);
+      } else if (ok && !KEYS && r < s.q_len) {
+        store_row(a.dq + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols, acc, s.scale, cols,
+                  s.head_dim % 4 == 0 && ((uintptr_t)a.dq & 15) == 0, a.add_q);
       }
       __syncwarp();
     }
@@ -1577,7 +1621,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 17) {
+  if (warp == 13) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
@@ -1585,26 +1629,27 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
 
 // Adds the segments of one key tile in order, `rows` rows per block: few for a
 // sink tile, whose many segments few blocks would read one after the other.
-template <int DP, int PASS>
+template <int DP>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int rows, int* err) {
   const AttentionShape& s = a.s;
   const int tile = blockIdx.x / (kTile / rows), row0 = blockIdx.x % (kTile / rows) * rows;
   // The tile's first segment; the next ones follow `stride` units apart.
   const int unit = first + tile / stride * segs * stride + tile % stride;
-  const GradItem t = grad_item<PASS>(a, unit, err);
+  const GradItem t = grad_item<true>(a, unit, err);
   if (t.n == 0) return;  // written key by key
   const int total = s.heads / s.kv_heads * t.n, each = (total + segs - 1) / segs, used = (total + each - 1) / each;
-  float* grad = PASS == kGradK ? a.dk : a.dv;
-  const int add = PASS == kGradK ? a.add_k : a.add_v;
-  const float by = PASS == kGradK ? s.scale : 1.0f;
-  for (int i = threadIdx.x; i < rows * DP; i += 256) {
-    const int r = row0 + i / DP, c = i % DP;
+  for (int i = threadIdx.x; i < 2 * rows * DP / 4; i += 256) {
+    const int which = i / (rows * DP / 4), r = row0 + i / (DP / 4) % rows, c = i % (DP / 4) * 4;
     if (t.r0 + r >= s.k_len || c >= s.head_dim) continue;
-    float sum = 0.0f;
+    float v[4] = {};
 #pragma unroll 8
-    for (int k = 0; k < used; ++k) sum += a.part[((int64_t)(unit + k * stride) * kTile + r) * DP + c];
-    float* dst = grad + row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len) + c;
-    *dst = add ? *dst + sum * by : sum * by;
+    for (int k = 0; k < used; ++k) {
+      const float4 p = *(const float4*)(a.part + (((int64_t)(unit + k * stride) * 2 + which) * kTile + r) * DP + c);
+      v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+    }
+    float* grad = which ? a.dv : a.dk;
+    store_row(grad + row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len) + c, v, 1.0f, s.head_dim - c,
+              s.head_dim % 4 == 0 && ((uintptr_t)grad & 15) == 0, which ? a.add_v : a.add_k);
   }
 }
 
@@ -1990,7 +2035,7 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.tdo = c.take(nq);
   w.info = (float4*)c.take(nq * kTile * 4);
   const Segments g = segments_of(s);
-  w.part = c.take(g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * kTile * padded_dim(s) : 0);
+  w.part = c.take(g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 * kTile * padded_dim(s) : 0);
   w.floats = c.used;
   return w;
 }
@@ -1999,27 +2044,27 @@ GradWork grad_work(const AttentionShape& s, float* base) {
 // more than a warp per row.
 bool grads_use_tiles(const AttentionShape& s) { return s.q_len >= 16; }
 
-template <int DP, int PASS>
+template <int DP, bool KEYS>
 void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
-  constexpr int kSmem = GradPlan<DP, PASS>::kSmem;
-  TYSOR_CUDA(cudaFuncSetAttribute(grad_kernel<DP, PASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  constexpr int kSmem = GradPlan<DP, KEYS>::kSmem;
+  TYSOR_CUDA(cudaFuncSetAttribute(grad_kernel<DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const AttentionShape& s = a.s;
-  const int64_t items = PASS == kGradQ ? (int64_t)tiles_of(s.q_len) * s.heads * s.batch : grad_units(s, a.seg);
+  const int64_t items = KEYS ? grad_units(s, a.seg) : (int64_t)tiles_of(s.q_len) * s.heads * s.batch;
   if (items == 0) return;
-  if (items > INT_MAX / 64) throw CudaError("window_attention: too many keys");
-  grad_kernel<DP, PASS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
+  if (items > INT_MAX / 64) throw CudaError("window_attention: too many rows");
+  grad_kernel<DP, KEYS><<<(unsigned)(items < kSms ? items : kSms), kGradThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
-  if (PASS == kGradQ) return;
-  const int stride = s.kv_heads * s.batch, of_long = a.seg.long_tiles * a.seg.long_segs * stride;
+  if (!KEYS) return;
+  const int tiles = tiles_of(s.k_len), stride = s.kv_heads * s.batch;
   if (a.seg.long_segs > 1 && a.seg.long_tiles > 0) {
-    const int rows = s.window > 0 ? 2 : 32;
-    grad_join_kernel<DP, PASS><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
+    const int rows = s.window > 0 ? 2 : 8;
+    grad_join_kernel<DP><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
         a, 0, a.seg.long_segs, stride, rows, err);
     check_launch();
   }
-  if (a.seg.short_segs > 1 && tiles_of(s.k_len) > a.seg.long_tiles) {
-    grad_join_kernel<DP, PASS><<<(unsigned)((tiles_of(s.k_len) - a.seg.long_tiles) * stride * 4), 256, 0, st>>>(
-        a, of_long, a.seg.short_segs, stride, 32, err);
+  if (a.seg.short_segs > 1 && tiles > a.seg.long_tiles) {
+    grad_join_kernel<DP><<<(unsigned)((tiles - a.seg.long_tiles) * stride * (kTile / 8)), 256, 0, st>>>(
+        a, a.seg.long_tiles * a.seg.long_segs * stride, a.seg.short_segs, stride, 8, err);
     check_launch();
   }
 }
@@ -2088,13 +2133,11 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                      w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v,
                      segments_of(s), w.part};
     if (padded_dim(s) == 64) {
-      run_grad<64, kGradQ>(a, err, st);
-      run_grad<64, kGradK>(a, err, st);
-      run_grad<64, kGradV>(a, err, st);
+      run_grad<64, false>(a, err, st);
+      run_grad<64, true>(a, err, st);
     } else {
-      run_grad<128, kGradQ>(a, err, st);
-      run_grad<128, kGradK>(a, err, st);
-      run_grad<128, kGradV>(a, err, st);
+      run_grad<128, false>(a, err, st);
+      run_grad<128, true>(a, err, st);
     }
     return;
   }
