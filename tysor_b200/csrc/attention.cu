@@ -258,6 +258,7 @@ struct PackJob {
   float *norm, *tile_norm;
   const float *out, *stats;
   float4* info;
+  float2* col;  // (greatest score + log2 of the sum - 14, delta); a row that sees nothing: a score no exponent reaches
   float* tile_delta;
 };
 struct PackJobs {
@@ -290,8 +291,10 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
       if (j.tile_norm != nullptr) j.tile_norm[index] = 0.0f;
       if (j.tile_delta != nullptr) j.tile_delta[index] = 0.0f;
     }
-    if (j.info != nullptr && threadIdx.x < kTile)
+    if (j.info != nullptr && threadIdx.x < kTile) {
       j.info[(int64_t)index * kTile + threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      j.col[(int64_t)index * kTile + threadIdx.x] = make_float2(1e30f, 0.0f);
+    }
     if (j.norm != nullptr && threadIdx.x < kTile) j.norm[(int64_t)index * kTile + threadIdx.x] = 0.0f;
     return;
   }
@@ -360,6 +363,8 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
           const float4 f =
               st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(st.x * kLog2e, 1.0f / st.y, d, q);
           j.info[(int64_t)index * kTile + r] = f;
+          j.col[(int64_t)index * kTile + r] =
+              st.y == 0.0f ? make_float2(1e30f, 0.0f) : make_float2(f.x + (log2f(st.y) - 14.0f), d);
           const float all = f.x * 0.0f + f.y * 0.0f + f.z * 0.0f;  // 0, or NaN if one is not finite
           most_delta = max(most_delta, __float_as_uint(fabsf(f.z) + all) & 0x7fffffffu);
         }
@@ -482,6 +487,9 @@ __device__ __forceinline__ void tmem_ld64(uint32_t at, float (&v)[64]) {
 #pragma unroll
   for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -500,17 +508,31 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// hi and lo of 32 neighbouring values as an A operand's 32 columns: 16 with hi
-// (two values each), 16 with lo.
-__device__ __forceinline__ void split32(const float* v, uint32_t (&r)[32]) {
+// Stores hi and lo of 32 neighbouring values as an A operand's 32 columns: 16
+// with hi (two values each), 16 with lo.
+__device__ __forceinline__ void store_split32(uint32_t at, const float* v) {
+  // Step by step over all of them, here and in the kernels: value by value, the
+  // chain of dependent instructions takes 40 cycles each.
+  uint32_t h[16], l[16];
+  float rest[32];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    const float2 back = __half22float2(h);
-    const __half2 l = __floats2half2_rn(v[2 * i] - back.x, v[2 * i + 1] - back.y);
-    r[i] = *(const uint32_t*)&h;
-    r[16 + i] = *(const uint32_t*)&l;
+    const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    h[i] = *(const uint32_t*)&x;
   }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 back = __half22float2(*(const __half2*)&h[i]);
+    rest[2 * i] = v[2 * i] - back.x;
+    rest[2 * i + 1] = v[2 * i + 1] - back.y;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const __half2 y = __floats2half2_rn(rest[2 * i], rest[2 * i + 1]);
+    l[i] = *(const uint32_t*)&y;
+  }
+  tmem_st16(at, h);
+  tmem_st16(at + 16, l);
 }
 // Column of the t-th 16 terms' hi part in such an operand (lo: 16 further).
 __device__ __forceinline__ uint32_t split_col(int t) { return (uint32_t)((t >> 1) * 32 + (t & 1) * 8); }
@@ -927,13 +949,12 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            v[32 * c + e] = exp2_fast(fmaf(v[32 * c + e], f, -c0));
-            l[e & 3] += v[32 * c + e];
-          }
-          uint32_t r[32];
-          split32(v + 32 * c, r);
-          tmem_st32(at + buf * kTile + 32 * c, r);
+          for (int e = 0; e < 32; ++e) v[32 * c + e] = fmaf(v[32 * c + e], f, -c0);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[32 * c + e] = exp2_fast(v[32 * c + e]);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) l[e & 3] += v[32 * c + e];
+          store_split32(at + buf * kTile + 32 * c, v + 32 * c);
         }
         // Four buffers: these scores come after the values of two tiles before
         // were issued, which waited until the output warps had taken the tile
@@ -1074,6 +1095,7 @@ struct GradArgs {
   const float *fq, *fk, *fv, *fo;      // factors
   const float *nv, *tnv, *tno, *tdo;   // norms of V's rows; greatest norm of V's and dO's tiles, greatest |delta|
   const float4* info;                  // of query rows
+  const float2* col;                   // the same for rows that are streamed
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
   Segments seg;
@@ -1087,7 +1109,7 @@ struct GradPlan {
   static constexpr int kEntries1 = 4;               // ring of the scores' operand, used twice: two steps
   static constexpr int kEntries2 = 2;               // ring of dP's operand: one step
   static constexpr int kResident = 2 * kTileBytes<DP>;
-  static constexpr int kInfo = KEYS ? 2 * kStep * 16 : 0;
+  static constexpr int kInfo = KEYS ? 2 * kStep * 8 : 0;
   static constexpr int kSmem = kResident + (kEntries1 + kEntries2) * kPart + kInfo + 512;
   static_assert(kSmem <= 227 * 1024, "shared memory of one block");
   static_assert(2 * DP + 4 * kStep <= 512, "tensor memory");
@@ -1273,14 +1295,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       const uint32_t entry = 2 * gi + part, slot = entry % entries, use = entry / entries, bar = full + 8 * slot;
       if (use > 0) ok = mbar_wait(empty + 8 * slot, (use - 1) & 1, err);
       if (!ok) return;
-      mbar_expect_tx(bar, kPart + (with_info ? kStep * 16 : 0));
+      mbar_expect_tx(bar, kPart + (with_info ? kStep * 8 : 0));
       const uint8_t* src = packed + (int64_t)tile * kTileBytes<DP> + (1 - part) * kHalves * kBox + (step & 1) * kStepBox;
 #pragma unroll
       for (int x = 0; x < kHalves; ++x)
         bulk_load(ring + slot * kPart + x * kStepBox, src + x * kBox, kStepBox, bar);
       if (with_info)
-        bulk_load(smem_u32(info_smem) + (gi & 1) * (kStep * 16),
-                  (const uint8_t*)(a.info + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 16, bar);
+        bulk_load(smem_u32(info_smem) + (gi & 1) * (kStep * 8),
+                  (const uint8_t*)(a.col + (int64_t)tile * kTile + (step & 1) * kStep), kStep * 8, bar);
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
@@ -1495,7 +1517,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         }
         if (!ok) break;
         tc_fence_after();
-        const float4* col = (const float4*)(info_smem + (gi & 1) * (kStep * 16));
+        const float2* col = (const float2*)(info_smem + (gi & 1) * (kStep * 8));
         float v[64];
         tmem_ld64(tmem_s + lanes, v);
         if (!KEYS) {
@@ -1508,23 +1530,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
           for (int e = 0; e < 64; ++e)
             if (!(seen[e / 32] >> (e & 31) & 1u)) v[e] = -INFINITY;
         }
-        const float scaled = st.y * up;
+        // Keys: 2^14 P, the 2^14 / sum and the greatest score in one exponent.
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          if (!KEYS) {
-            v[e] = exp2_fast(fmaf(v[e], f, -st.x)) * scaled;
-          } else {
-            const float2 c = *(const float2*)&col[e];
-            v[e] = exp2_fast(fmaf(v[e], f, -c.x)) * (c.y * 16384.0f);
-          }
-        }
-        uint32_t r[32];
+        for (int e = 0; e < 64; ++e) v[e] = fmaf(v[e], f, KEYS ? -col[e].x : -st.x);
+#pragma unroll
+        for (int e = 0; e < 64; ++e) v[e] = exp2_fast(v[e]);
         if (KEYS) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            split32(v + 32 * c, r);
-            tmem_st32(tmem_s + lanes + 32 * c, r);
-          }
+          for (int c = 0; c < 2; ++c) store_split32(tmem_s + lanes + 32 * c, v + 32 * c);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           tc_fence_before();
           __syncwarp();
@@ -1533,18 +1546,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         ok = warp_wait(d_full, gi & 1, err);
         if (!ok) break;
         tc_fence_after();
-        const float rescale = up * 0x1p-14f;
+        const float rescale = KEYS ? up * 0x1p-14f : up * st.y;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float d[32];
           tmem_ld32(tmem_d + lanes + 32 * c, d);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (!KEYS) d[e] = v[32 * c + e] * fmaf(d[e], f2, -st.z);
-            else d[e] = v[32 * c + e] * (fmaf(d[e], f2, -col[32 * c + e].z) * rescale);
-          }
-          split32(d, r);
-          tmem_st32(tmem_d + lanes + 32 * c, r);
+          for (int e = 0; e < 32; ++e) d[e] = fmaf(d[e], f2, KEYS ? -col[32 * c + e].y : -st.z);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[32 * c + e] *= rescale;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) d[e] *= v[32 * c + e];
+          store_split32(tmem_d + lanes + 32 * c, d);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -1990,6 +2003,7 @@ struct GradWork {
   uint8_t *pq, *pk, *pv, *po;
   float *fq, *fk, *fv, *fo, *nv, *no, *tnv, *tno, *tdo;
   float4* info;
+  float2* col;
   float* part;
   int64_t floats;
 };
@@ -2034,6 +2048,7 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.tno = c.take(nq);
   w.tdo = c.take(nq);
   w.info = (float4*)c.take(nq * kTile * 4);
+  w.col = (float2*)c.take(nq * kTile * 2);
   const Segments g = segments_of(s);
   w.part = c.take(g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 * kTile * padded_dim(s) : 0);
   w.floats = c.used;
@@ -2125,12 +2140,12 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
   if (rows > 0 && grads_use_tiles(s)) {
     const GradWork w = grad_work(s, work);
     PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
-                       {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.tdo},
+                       {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.col, w.tdo},
                        {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
     run_pack(s, jobs, 4, err, st);
     const GradArgs a{s,    q,    k,    v,    out,  stats, dout,  w.pq,  w.pk,   w.pv, w.po, w.fq,         w.fk,
-                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v,
+                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, w.col, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v,
                      segments_of(s), w.part};
     if (padded_dim(s) == 64) {
       run_grad<64, false>(a, err, st);
