@@ -1677,6 +1677,20 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
 // at the end in a fixed order.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
+
+// Two fp32 values in one 64-bit register: one instruction multiplies and adds both.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float first_of(uint64_t p) { return __uint_as_float((uint32_t)p); }
+__device__ __forceinline__ float second_of(uint64_t p) { return __uint_as_float((uint32_t)(p >> 32)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
 constexpr int kMostSplits = 512;
 
 // The keys that some row of a sequence sees: [0, first) and `count` - first
@@ -1699,7 +1713,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
                                                                 float* __restrict__ stats, float* __restrict__ part,
                                                                 int splits, int per, int row_blocks, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
-  __shared__ float qs[R][kDims];
+  __shared__ __align__(16) float qs[R][kDims];
   __shared__ float joined[kWarps][R][kDims + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
   int64_t index = blockIdx.x;
@@ -1728,27 +1742,30 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     at[r] = rb * R + r < total && p < sq.n ? p : -1;
   }
   __syncthreads();
-  float m[R], l[R], acc[R][4 * NI];
+  float m[R], l[R];
+  uint64_t acc[R][2 * NI];  // pairs of values
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4 * NI; ++c) acc[r][c] = 0.0f;
+    for (int c = 0; c < 2 * NI; ++c) acc[r][c] = 0;
   }
   const int64_t step = s.seq_major ? (int64_t)s.kv_heads * s.head_dim : s.head_dim;
   const int64_t base = row_at(s, b, g, 0, s.kv_heads, s.k_len);
-  auto load = [&](const float* __restrict__ x, int j, float (&d)[4 * NI]) {
+  auto load = [&](const float* __restrict__ x, int j, uint64_t (&d)[2 * NI]) {
     const float* src = x + base + j * step;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = 4 * l8 + 32 * i;
       if (VEC) {
-        const float4 f = c < s.head_dim ? __ldg((const float4*)(src + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        d[4 * i] = f.x, d[4 * i + 1] = f.y, d[4 * i + 2] = f.z, d[4 * i + 3] = f.w;
+        const ulonglong2 f = c < s.head_dim ? __ldg((const ulonglong2*)(src + c)) : make_ulonglong2(0, 0);
+        d[2 * i] = f.x, d[2 * i + 1] = f.y;
       } else {
+        float e[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) d[4 * i + e] = c + e < s.head_dim ? __ldg(src + c + e) : 0.0f;
+        for (int k = 0; k < 4; ++k) e[k] = c + k < s.head_dim ? __ldg(src + c + k) : 0.0f;
+        d[2 * i] = pair_of(e[0], e[1]), d[2 * i + 1] = pair_of(e[2], e[3]);
       }
     }
   };
@@ -1756,55 +1773,64 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     const bool two = u + 4 * kWarps < u1;
     const int u2 = two ? u + 4 * kWarps : u;
     const int j[2] = {u < first ? u : low + u - first, u2 < first ? u2 : low + u2 - first};
-    float kd[2][4 * NI], vd[2][4 * NI];
+    uint64_t kd[2][2 * NI], vd[2][2 * NI];
     load(k, j[0], kd[0]);
     load(k, j[1], kd[1]);
     load(v, j[0], vd[0]);
     load(v, j[1], vd[1]);
+    // All eight lanes of a key are here together (they share u).
+    const uint32_t lanes = 0xffu << (lane & 24);
+    float d[R][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float d[2] = {0.0f, 0.0f};
+      uint64_t x[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const float4 f = *(const float4*)&qs[r][4 * l8 + 32 * i];
+        const ulonglong2 f = *(const ulonglong2*)&qs[r][4 * l8 + 32 * i];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          d[w] = fmaf(f.x, kd[w][4 * i], d[w]);
-          d[w] = fmaf(f.y, kd[w][4 * i + 1], d[w]);
-          d[w] = fmaf(f.z, kd[w][4 * i + 2], d[w]);
-          d[w] = fmaf(f.w, kd[w][4 * i + 3], d[w]);
+          x[w] = fma_pair(f.x, kd[w][2 * i], x[w]);
+          x[w] = fma_pair(f.y, kd[w][2 * i + 1], x[w]);
         }
       }
-      // All eight lanes of a key are here together (they share u).
-      const uint32_t lanes = 0xffu << (lane & 24);
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        d[0] += __shfl_xor_sync(lanes, d[0], o);
-        d[1] += __shfl_xor_sync(lanes, d[1], o);
+      for (int w = 0; w < 2; ++w) d[r][w] = first_of(x[w]) + second_of(x[w]);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        d[r][0] += __shfl_xor_sync(lanes, d[r][0], o);
+        d[r][1] += __shfl_xor_sync(lanes, d[r][1], o);
       }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       bool sees[2] = {true, two};
       if (s.q_len > 1)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
           sees[w] = sees[w] && j[w] <= at[r] && (s.window == 0 || at[r] - j[w] < s.window || j[w] < s.sinks);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) d[w] = sees[w] ? d[w] * to_log2 : -INFINITY;
-      const float top = fmaxf(d[0], d[1]);
+      for (int w = 0; w < 2; ++w) d[r][w] = sees[w] ? d[r][w] * to_log2 : -INFINITY;
+      const float top = fmaxf(d[r][0], d[r][1]);
       if (top > m[r]) {  // seldom after a row's first keys
         const float keep = exp2_fast(m[r] - top);
         m[r] = top;
         l[r] *= keep;
+        const uint64_t both = pair_of(keep, keep);
 #pragma unroll
-        for (int c = 0; c < 4 * NI; ++c) acc[r][c] *= keep;
+        for (int c = 0; c < 2 * NI; ++c) acc[r][c] = fma_pair(acc[r][c], both, 0);
       }
       const float ref = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
       for (int w = 0; w < 2; ++w)
         if (sees[w]) {  // a hidden value takes no part, not even times 0
-          const float p = exp2_fast(d[w] - ref);
+          const float p = exp2_fast(d[r][w] - ref);
           l[r] += p;
+          const uint64_t both = pair_of(p, p);
 #pragma unroll
-          for (int c = 0; c < 4 * NI; ++c) acc[r][c] = fmaf(p, vd[w][c], acc[r][c]);
+          for (int c = 0; c < 2 * NI; ++c) acc[r][c] = fma_pair(both, vd[w][c], acc[r][c]);
         }
     }
   }
@@ -1820,7 +1846,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
 #pragma unroll
     for (int c = 0; c < 4 * NI; ++c) {
-      float x = acc[r][c] * w;
+      float x = (c & 1 ? second_of(acc[r][c / 2]) : first_of(acc[r][c / 2])) * w;
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
       if (lane < 8) joined[warp][r][4 * l8 + 32 * (c / 4) + c % 4] = x;

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_kernel(const float* __re
 // add theirs in order in shared memory, and `partial` gets one line per block
 // (summed in a fixed order by column_sum_kernel).
 template <int TPR, int NV, bool VEC>
-__global__ void __launch_bounds__(512) layer_norm_backward_kernel(
+__global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) layer_norm_backward_kernel(
     const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ stats,
     const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width,
     int accumulate) {
@@ -483,6 +483,11 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     int* err) {
   __shared__ Online warp_part[kDistillThreads / 32];
   __shared__ Online part[8];  // block 0's: one entry per block of the cluster
+  __shared__ struct {
+    float best;
+    double log_mass;
+    bool any;
+  } teach;
   extern __shared__ float entry[];  // [2][top]: ids, probabilities
   const int64_t r = blockIdx.x;
   const int parts = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
@@ -498,13 +503,23 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
   const int64_t per = (quads + parts - 1) / parts;
   const int64_t q0 = min(quads, rank * per), q1 = min(quads, q0 + per);
   const float4* body = (const float4*)(row + head);
+  // The last warp of the first block prepares the teacher's entries meanwhile.
+  int* eid = (int*)entry;
+  float* p = entry + top;
+  if (rank == 0 && tid >= kDistillThreads - 32) {
+    float best;
+    double log_mass;
+    const bool any = teacher_row(ids + r * top, teacher + r * top, top, width, inv_t, eid, p, &best, &log_mass, err);
+    if ((tid & 31) == 0) teach = {best, log_mass, any};
+  }
   Online o{-INFINITY, 0.0f};
   bool bad = false;
-  int64_t i = q0 + tid;
-  for (; i + 3 * kDistillThreads < q1; i += 4 * kDistillThreads) {
+  for (int64_t i = q0 + tid; i < q1; i += 4 * kDistillThreads) {
     float4 f[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) f[u] = body[i + u * kDistillThreads];
+    for (int u = 0; u < 4; ++u)
+      f[u] = i + u * kDistillThreads < q1 ? body[i + u * kDistillThreads]
+                                          : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     float m = o.m;
 #pragma unroll
     for (int u = 0; u < 4; ++u) m = fmaxf(m, fmaxf(fmaxf(f[u].x, f[u].y), fmaxf(f[u].z, f[u].w)));
@@ -516,14 +531,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     float s = o.s * exp2_fast((o.m - m) * c);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      s += (exp2_fast((f[u].x - m) * c) + exp2_fast((f[u].y - m) * c)) + (exp2_fast((f[u].z - m) * c) + exp2_fast((f[u].w - m) * c));
+      s += (exp2_fast((f[u].x - m) * c) + exp2_fast((f[u].y - m) * c)) +
+           (exp2_fast((f[u].z - m) * c) + exp2_fast((f[u].w - m) * c));
     o.m = m;
     o.s = s;
-  }
-  for (; i < q1; i += kDistillThreads) {
-    const float4 f = body[i];
-    take(o, f.x, c), take(o, f.y, c), take(o, f.z, c), take(o, f.w, c);
-    bad |= f.x != f.x || f.y != f.y || f.z != f.z || f.w != f.w;
   }
   if (rank == 0) {
     const int64_t tail = head + 4 * quads;
@@ -556,20 +567,14 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
   Online all = part[0];
   for (int w = 1; w < parts; ++w) all = join(all, part[w], c);
   if (stats != nullptr && tid == 0) *(float2*)(stats + 2 * r) = make_float2(all.m, all.s);
-  int* eid = (int*)entry;
-  float* p = entry + top;
-  float best;
-  double log_mass;
-  const bool any =
-      teacher_row(ids + r * top, teacher + r * top, top, width, inv_t, eid, p, &best, &log_mass, err);
   // ln p - ln q per entry in 64 bits: the two logarithms nearly cancel where
   // the student follows the teacher.
   const double log_sum = log((double)all.s);
   float sum = 0.0f;
-  if (any)
+  if (teach.any)
     for (int e = tid; e < top; e += 32) {
       if (p[e] == 0.0f) continue;
-      const double t = ((double)teacher[r * top + e] - (double)best) / temperature - log_mass;
+      const double t = ((double)teacher[r * top + e] - (double)teach.best) / temperature - teach.log_mass;
       const double z = ((double)row[eid[e]] - (double)all.m) / temperature - log_sum;
       sum += (float)((double)p[e] * (t - z));
     }
@@ -591,25 +596,22 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
   const int tid = threadIdx.x;
   int* eid = (int*)entry;
   float* p = entry + top;
-  if (tid < 32) {
+  if (tid >= kDistillThreads - 32) {
     float best;
     double log_mass;
     const bool any = teacher_row(ids + r * top, teacher + r * top, top, width, 1.0f / temperature, eid, p, &best,
                                  &log_mass, err);
-    if (tid == 0) any_entry = any;
+    if ((tid & 31) == 0) any_entry = any;
   }
-  __syncthreads();
   const float* row = logits + r * width;
   float* out = grad + r * width;
   const float2 st = *(const float2*)(stats + 2 * r);
   const float c = kLog2e / temperature;
   const float up = temperature * (dloss ? dloss[r] : 1.0f);
   const float coef = up / st.y;
-  const bool any = any_entry;
-  if (!any) {  // whatever the row holds
-    if (!accumulate)
-      for (int64_t i = c0 + tid; i < c1; i += kDistillThreads) out[i] = 0.0f;
-    return;
+  if (accumulate) {  // a row without entries stays as it is
+    __syncthreads();
+    if (!any_entry) return;
   }
   const int64_t head = VEC ? min(c1 - c0, (int64_t)((4 - (((uintptr_t)(row + c0) >> 2) & 3)) & 3)) : 0;
   const int64_t quads = VEC ? (c1 - c0 - head) / 4 : 0;
@@ -642,6 +644,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
   if (VEC && tid < head) one(c0 + tid);
   for (int64_t at = c0 + head + 4 * quads + tid; at < c1; at += kDistillThreads) one(at);
   __syncthreads();
+  if (!any_entry) {  // 0, whatever the row holds
+    for (int64_t at = c0 + tid; at < c1; at += kDistillThreads) out[at] = 0.0f;
+    return;
+  }
   for (int e = tid; e < top; e += kDistillThreads) {
     const int id = eid[e];
     if (id < c0 || id >= c1) continue;
@@ -697,32 +703,35 @@ constexpr int64_t kLayerNormBackwardMost = 8192;  // backward
 int layer_norm_lines(int64_t rows, int64_t width) {
   if (width > kLayerNormBackwardMost) return (int)(rows < 64 ? rows : 64);
   int tpr = 32;
-  while (tpr * 16 < width) tpr *= 2;
+  while (tpr * 8 < width && tpr < 512) tpr *= 2;
   const int64_t want = ceil_div(rows, 512 / tpr);
   return (int)(want < 148 * 2 ? want : 148 * 2);
 }
 
-template <int TPR, bool VEC>
+template <int TPR, int NV, bool VEC>
 void layer_norm_backward_run(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
                              float* partial, int64_t rows, int width, int accumulate, cudaStream_t st) {
   const size_t smem = partial ? sizeof(float) * 2 * (size_t)width : 0;
   if (smem > 48 * 1024)
-    TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_backward_kernel<TPR, 4, VEC>,
+    TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_backward_kernel<TPR, NV, VEC>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
-  layer_norm_backward_kernel<TPR, 4, VEC><<<layer_norm_lines(rows, width), 512, smem, st>>>(
+  layer_norm_backward_kernel<TPR, NV, VEC><<<layer_norm_lines(rows, width), 512, smem, st>>>(
       x, gain, stats, dy, dx, partial, rows, width, accumulate);
   check_launch();
 }
 
+// Eight values of a row per thread up to 4096: two blocks of 512 threads then
+// fit an SM.
 template <bool VEC>
 void layer_norm_backward_pick(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
                               float* partial, int64_t rows, int64_t width, int accumulate, cudaStream_t st) {
   const int w = (int)width;
-  if (width <= 512) layer_norm_backward_run<32, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
-  else if (width <= 1024) layer_norm_backward_run<64, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
-  else if (width <= 2048) layer_norm_backward_run<128, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
-  else if (width <= 4096) layer_norm_backward_run<256, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
-  else layer_norm_backward_run<512, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  if (width <= 256) layer_norm_backward_run<32, 2, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 512) layer_norm_backward_run<64, 2, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 1024) layer_norm_backward_run<128, 2, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 2048) layer_norm_backward_run<256, 2, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else if (width <= 4096) layer_norm_backward_run<512, 2, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
+  else layer_norm_backward_run<512, 4, VEC>(x, gain, stats, dy, dx, partial, rows, w, accumulate, st);
 }
 
 }  // namespace
