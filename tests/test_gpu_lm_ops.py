@@ -531,6 +531,21 @@ def test_distill_loss_of_absent_and_repeated_entries(lib):
     compare_distill(got, want, 2.0)
 
 
+def test_distill_loss_of_entries_that_are_no_numbers(lib):
+    """A teacher's NaN makes its own row's loss NaN, absent entries beside it
+    notwithstanding, and no other row's."""
+    z, ids, teacher, dloss = distill_inputs(5, 300, 6)
+    clean = run_distill(lib, z, ids, teacher, dloss, 2.0)
+    ids[1, 3:] = -1
+    teacher[1, 0], teacher[3, 2] = np.nan, np.inf
+    got = run_distill(lib, z, ids, teacher, dloss, 2.0)
+    assert np.isnan(got["loss"][[1, 3]]).all()
+    keep = [0, 2, 4]
+    for n in ("loss", "grad", "stats"):
+        assert np.array_equal(got[n][keep], clean[n][keep]), n
+    lib.ctx.synchronize()
+
+
 def test_distill_gradient_against_differences(lib):
     z, ids, teacher, dloss = distill_inputs(4, 30, 5)
     got = run_distill(lib, z, ids, teacher, dloss, 1.5)["grad"]

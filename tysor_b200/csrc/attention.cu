@@ -1677,6 +1677,11 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
 // at the end in a fixed order.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
+constexpr int kDecodeStages = 3;
+
+__device__ __forceinline__ void copy16(float* to, const float* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
 
 // Two fp32 values in one 64-bit register: one instruction multiplies and adds both.
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -1753,33 +1758,59 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   }
   const int64_t step = s.seq_major ? (int64_t)s.kv_heads * s.head_dim : s.head_dim;
   const int64_t base = row_at(s, b, g, 0, s.kv_heads, s.k_len);
-  auto load = [&](const float* __restrict__ x, int j, uint64_t (&d)[2 * NI]) {
-    const float* src = x + base + j * step;
+  // A lane's 4 NI values of two keys and values per step of the loop, VEC: from
+  // a ring that the lane fills for itself two steps ahead, so that loads stay in
+  // flight while it computes; otherwise straight from memory.
+  extern __shared__ __align__(16) float ring[];  // [warps][kDecodeStages][K, V][2][4][kDims]
+  float* mine = ring + ((size_t)warp * kDecodeStages * 16 + (lane >> 3)) * kDims + 4 * l8;
+  auto key_at = [&](int u) { return u < first ? u : low + u - first; };
+  auto copy = [&](int it) {
+    if (VEC) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int u = u0 + key_of + it * 8 * kWarps + w * 4 * kWarps;
+        if (u >= u1) continue;
+        const int64_t from = base + key_at(u) * step + 4 * l8;
+        float* to = mine + (it % kDecodeStages * 16 + w * 4) * kDims;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (4 * l8 + 32 * i < s.head_dim) {
+            copy16(to + 32 * i, k + from + 32 * i);
+            copy16(to + 8 * kDims + 32 * i, v + from + 32 * i);
+          }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  auto load = [&](const float* __restrict__ x, int it, int which, int w, uint64_t (&d)[2 * NI]) {
+    const int u = u0 + key_of + it * 8 * kWarps + w * 4 * kWarps;
+    const float* src = VEC ? mine + (it % kDecodeStages * 16 + which * 8 + w * 4) * kDims
+                           : x + base + key_at(min(u, u1 - 1)) * step + 4 * l8;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int c = 4 * l8 + 32 * i;
       if (VEC) {
-        const ulonglong2 f = c < s.head_dim ? __ldg((const ulonglong2*)(src + c)) : make_ulonglong2(0, 0);
+        const ulonglong2 f = c < s.head_dim ? *(const ulonglong2*)(src + 32 * i) : make_ulonglong2(0, 0);
         d[2 * i] = f.x, d[2 * i + 1] = f.y;
       } else {
         float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = c + k < s.head_dim ? __ldg(src + c + k) : 0.0f;
+        for (int k = 0; k < 4; ++k) e[k] = c + k < s.head_dim ? __ldg(src + 32 * i + k) : 0.0f;
         d[2 * i] = pair_of(e[0], e[1]), d[2 * i + 1] = pair_of(e[2], e[3]);
       }
     }
   };
-  for (int u = u0 + key_of; u < u1; u += 8 * kWarps) {
-    const bool two = u + 4 * kWarps < u1;
-    const int u2 = two ? u + 4 * kWarps : u;
-    const int j[2] = {u < first ? u : low + u - first, u2 < first ? u2 : low + u2 - first};
+  const int steps = u1 > u0 ? (u1 - u0 + 8 * kWarps - 1) / (8 * kWarps) : 0;
+  for (int it = 0; it < kDecodeStages - 1; ++it) copy(it);
+  for (int it = 0; it < steps; ++it) {
+    copy(it + kDecodeStages - 1);
+    if (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(kDecodeStages - 1) : "memory");
+    const int u = u0 + key_of + it * 8 * kWarps;
+    const bool one = u < u1, two = u + 4 * kWarps < u1;
+    const int j[2] = {key_at(u), key_at(u + 4 * kWarps)};
     uint64_t kd[2][2 * NI], vd[2][2 * NI];
-    load(k, j[0], kd[0]);
-    load(k, j[1], kd[1]);
-    load(v, j[0], vd[0]);
-    load(v, j[1], vd[1]);
-    // All eight lanes of a key are here together (they share u).
-    const uint32_t lanes = 0xffu << (lane & 24);
+    load(k, it, 0, 0, kd[0]);
+    load(k, it, 0, 1, kd[1]);
     float d[R][2];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -1800,13 +1831,15 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     for (int o = 4; o > 0; o >>= 1) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        d[r][0] += __shfl_xor_sync(lanes, d[r][0], o);
-        d[r][1] += __shfl_xor_sync(lanes, d[r][1], o);
+        d[r][0] += __shfl_xor_sync(0xffffffffu, d[r][0], o);
+        d[r][1] += __shfl_xor_sync(0xffffffffu, d[r][1], o);
       }
     }
+    load(v, it, 1, 0, vd[0]);
+    load(v, it, 1, 1, vd[1]);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      bool sees[2] = {true, two};
+      bool sees[2] = {one, two};
       if (s.q_len > 1)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
@@ -1993,8 +2026,11 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks * p.splits;
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
+  constexpr int kRing = kDecodeThreads / 32 * kDecodeStages * 16 * 32 * NI * (int)sizeof(float);
   if (vec)
-    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
+    TYSOR_CUDA(cudaFuncSetAttribute(decode_kernel<NI, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+  if (vec)
+    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
                                                                             p.row_blocks, err);
   else
     decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,

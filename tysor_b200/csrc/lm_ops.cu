@@ -447,7 +447,8 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ idr, const
   }
   mass = warp_sum(mass);
   const float scale = mass > 0.0f ? 1.0f / mass : 0.0f;
-  for (int e = lane; e < top; e += 32) p[e] = mass == mass ? p[e] * scale : NAN;
+  // Where a weight is NaN so are all; an absent entry stays 0 (nothing reads its id).
+  for (int e = lane; e < top; e += 32) p[e] = ids[e] < 0 ? 0.0f : mass == mass ? p[e] * scale : NAN;
   __syncwarp();
   *best_out = best;
   *log_mass = log((double)mass);
@@ -476,7 +477,9 @@ __device__ __forceinline__ void take(Online& o, float v, float c) {
 // Greatest logit and sum of one row in one pass, the row split over a cluster
 // of gridDim.y blocks (one for many rows) whose parts the first block joins in
 // order through distributed shared memory; then the loss of the row's entries.
-constexpr int kDistillThreads = 512;
+// Eight small blocks per SM rather than four: while one ends its row (its few
+// entries, the logarithms), the others keep loads in flight.
+constexpr int kDistillThreads = 256;
 __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
     float* __restrict__ loss, float* __restrict__ stats, int64_t rows, int64_t width, int top, float temperature,
@@ -488,7 +491,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     double log_mass;
     bool any;
   } teach;
-  extern __shared__ float entry[];  // [2][top]: ids, probabilities
+  extern __shared__ __align__(8) uint8_t entries[];  // [top] each: gaps (double), ids, probabilities
   const int64_t r = blockIdx.x;
   const int parts = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
   // Arrives for "this block runs": the first block's shared memory is written
@@ -504,13 +507,20 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
   const int64_t q0 = min(quads, rank * per), q1 = min(quads, q0 + per);
   const float4* body = (const float4*)(row + head);
   // The last warp of the first block prepares the teacher's entries meanwhile.
-  int* eid = (int*)entry;
-  float* p = entry + top;
+  double* gap = (double*)entries;
+  int* eid = (int*)(gap + top);
+  float* p = (float*)(eid + top);
   if (rank == 0 && tid >= kDistillThreads - 32) {
     float best;
     double log_mass;
     const bool any = teacher_row(ids + r * top, teacher + r * top, top, width, inv_t, eid, p, &best, &log_mass, err);
     if ((tid & 31) == 0) teach = {best, log_mass, any};
+    // What the end needs of each entry: the teacher's logarithm less the
+    // student's logit, in 64 bits (the two logarithms nearly cancel where the
+    // student follows the teacher).
+    for (int e = tid & 31; e < top; e += 32)
+      if (p[e] != 0.0f)
+        gap[e] = ((double)teacher[r * top + e] - (double)best - (double)row[eid[e]]) / temperature - log_mass;
   }
   Online o{-INFINITY, 0.0f};
   bool bad = false;
@@ -542,11 +552,12 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     if (tid < width - tail) take(o, row[tail + tid], c), bad |= row[tail + tid] != row[tail + tid];
   }
   if (bad) o.s = NAN;
+  float top_of_warp = o.m;
 #pragma unroll
-  for (int k = 16; k > 0; k >>= 1) {
-    const Online p{__shfl_xor_sync(0xffffffffu, o.m, k), __shfl_xor_sync(0xffffffffu, o.s, k)};
-    o = join(o, p, c);
-  }
+  for (int k = 16; k > 0; k >>= 1) top_of_warp = fmaxf(top_of_warp, __shfl_xor_sync(0xffffffffu, top_of_warp, k));
+  // A lane without a finite value holds a sum of 0, or NaN.
+  o.s = warp_sum(o.m == -INFINITY ? o.s : o.s * exp2_fast((o.m - top_of_warp) * c));
+  o.m = top_of_warp;
   if ((tid & 31) == 0) warp_part[tid >> 5] = o;
   __syncthreads();
   if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -567,17 +578,12 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
   Online all = part[0];
   for (int w = 1; w < parts; ++w) all = join(all, part[w], c);
   if (stats != nullptr && tid == 0) *(float2*)(stats + 2 * r) = make_float2(all.m, all.s);
-  // ln p - ln q per entry in 64 bits: the two logarithms nearly cancel where
-  // the student follows the teacher.
-  const double log_sum = log((double)all.s);
+  // Sum of p (ln p - ln q), ln q = (z - max) / T - ln sum.
+  const double log_sum = log((double)all.s) + (double)all.m / temperature;
   float sum = 0.0f;
   if (teach.any)
-    for (int e = tid; e < top; e += 32) {
-      if (p[e] == 0.0f) continue;
-      const double t = ((double)teacher[r * top + e] - (double)teach.best) / temperature - teach.log_mass;
-      const double z = ((double)row[eid[e]] - (double)all.m) / temperature - log_sum;
-      sum += (float)((double)p[e] * (t - z));
-    }
+    for (int e = tid; e < top; e += 32)
+      if (p[e] != 0.0f) sum += (float)((double)p[e] * (gap[e] + log_sum));
   sum = warp_sum(sum);
   if (tid == 0) loss[r] = temperature * temperature * sum;
 }
@@ -617,16 +623,18 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
   const int64_t quads = VEC ? (c1 - c0 - head) / 4 : 0;
   const float4* src = (const float4*)(row + c0 + head);
   float4* dst = (float4*)(out + c0 + head);
-  int64_t i = tid;
-  for (; i + 3 * kDistillThreads < quads; i += 4 * kDistillThreads) {
+  for (int64_t i = tid; i < quads; i += 4 * kDistillThreads) {
     float4 f[4], old[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) f[u] = src[i + u * kDistillThreads];
+    for (int u = 0; u < 4; ++u)
+      if (i + u * kDistillThreads < quads) f[u] = src[i + u * kDistillThreads];
     if (accumulate)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) old[u] = dst[i + u * kDistillThreads];
+      for (int u = 0; u < 4; ++u)
+        if (i + u * kDistillThreads < quads) old[u] = dst[i + u * kDistillThreads];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      if (i + u * kDistillThreads >= quads) break;
       float4 g = make_float4(coef * exp2_fast((f[u].x - st.x) * c), coef * exp2_fast((f[u].y - st.x) * c),
                              coef * exp2_fast((f[u].z - st.x) * c), coef * exp2_fast((f[u].w - st.x) * c));
       if (accumulate) g.x += old[u].x, g.y += old[u].y, g.z += old[u].z, g.w += old[u].w;
@@ -637,10 +645,6 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
     const float g = coef * exp2_fast((row[at] - st.x) * c);
     out[at] = accumulate ? out[at] + g : g;
   };
-  for (; i < quads; i += kDistillThreads) {
-    const int64_t at = c0 + head + 4 * i;
-    one(at), one(at + 1), one(at + 2), one(at + 3);
-  }
   if (VEC && tid < head) one(c0 + tid);
   for (int64_t at = c0 + head + 4 * quads + tid; at < c1; at += kDistillThreads) one(at);
   __syncthreads();
@@ -813,7 +817,7 @@ void launch_distill_loss(const float* logits, const float* ids, const float* tea
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows, (unsigned)parts);
   cfg.blockDim = dim3(kDistillThreads);
-  cfg.dynamicSmemBytes = sizeof(float) * 2 * (size_t)top;
+  cfg.dynamicSmemBytes = (sizeof(double) + sizeof(int) + sizeof(float)) * (size_t)top;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
