@@ -442,7 +442,7 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint
       "r"(a), "r"(b), "n"(kDescHigh), "r"(idesc), "r"(add));
 }
 // fp16 x fp16 -> fp32, M = 128; `b_rows`: B is summed over its rows.
-constexpr uint32_t umma_idesc(int n, bool b_rows) {
+__host__ __device__ constexpr uint32_t umma_idesc(int n, bool b_rows) {
   return (1u << 4) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 // A box as an operand summed over its columns: 16 columns are 32 bytes.
@@ -578,6 +578,7 @@ __device__ __forceinline__ float2 natural_stats(float top, float sum) {
 // The key tiles that a tile of query rows needs: [0, sinks) and then `low` on.
 struct TileRange {
   int sinks, low, count;
+  int width;  // of the last of the first `sinks` tiles: the columns that hold sinks, in whole 16s
   __device__ __forceinline__ int at(int i) const { return i < sinks ? i : low + i - sinks; }
 };
 struct RowRange {
@@ -595,12 +596,13 @@ __device__ __forceinline__ RowRange rows_of(const AttentionShape& s, const Seque
 
 __device__ __forceinline__ TileRange keys_for(const AttentionShape& s, const Sequence& q, const RowRange& r) {
   const int a = max(r.p0, 0), z = min(r.p1, q.n - 1);
-  if (a > z) return {0, 0, 0};
+  if (a > z) return {0, 0, 0, kTile};
   const int low = s.window > 0 ? max(a + 1 - s.window, 0) : 0;
   TileRange t;
   t.low = low / kTile;
   t.sinks = min(tiles_of(min(s.sinks, low)), t.low);
   t.count = t.sinks + z / kTile - t.low + 1;
+  t.width = min(kTile, (min(s.sinks, low) - (t.sinks - 1) * kTile + 15) / 16 * 16);
   return t;
 }
 
@@ -814,11 +816,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     }
   } else if (warp == 17) {
     fewer_registers<kFewRegs>();
-    constexpr uint32_t kScore = umma_idesc(kTile, false), kValue = umma_idesc(DP, true);
+    constexpr uint32_t kValue = umma_idesc(DP, true);
     const bool leader = elect_one();
     uint32_t it = 0, gi = 0, item = 0;  // slots, tiles and items issued so far
     bool ok = true;
-    auto values = [&](uint32_t t) {  // of tile t of the stream
+    auto values = [&](uint32_t t, int width) {  // of tile t of the stream, its first `width` keys
       const uint32_t p = tmem_s + (t & 1) * kTile, out = t % kOut, d = tmem_o + out * DP;
       ok = warp_wait(p_full + 8 * (t & 1), (t >> 1) & 1, err);
       if (ok && t >= kOut) ok = warp_wait(o_empty + 8 * out, (t / kOut - 1) & 1, err);
@@ -834,6 +836,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         if (leader) {
 #pragma unroll
           for (int k = 0; k < kSteps; ++k) {
+            if ((x * kSteps + k) * 16 >= width) break;
             const uint32_t ph = px + split_col(k), vh = v + k * kRowStep, vl = vh + (kBox >> 4);
             umma_ts(d, ph + 16, vh, kValue, x != 0 || k != 0);
             umma_ts(d, ph, vl, kValue, 1u);
@@ -847,13 +850,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const int n = __shfl_sync(0xffffffffu, query_item(s, w, a.fq, a.fk, a.fv, err).n, 0);
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
+      const int n = __shfl_sync(0xffffffffu, t.n, 0), sinks = __shfl_sync(0xffffffffu, t.range.sinks, 0);
+      const int sink_width = __shfl_sync(0xffffffffu, t.range.width, 0);
       if (n == 0) continue;
       ok = warp_wait(q_ready, item & 1, err);
       ++item;
       for (int i = 0; i <= n && ok; ++i) {
         if (i < n) {
           const uint32_t d = tmem_s + (gi & 1) * kTile;
+          const uint32_t score = umma_idesc(i == sinks - 1 ? sink_width : kTile, false);
           for (int x = 0; x < kHalves && ok; ++x, ++it) {
             const uint32_t slot = it % Plan::kSlots;
             ok = warp_wait(slot_full + 8 * slot, (it / Plan::kSlots) & 1, err);
@@ -864,9 +870,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t qh = q + 8 * k, ql = qh + DP / 2, kh = key + k * kColumnStep, kl = kh + (kBox >> 4);
-                umma_ts(d, ql, kh, kScore, x != 0 || k != 0);
-                umma_ts(d, qh, kl, kScore, 1u);
-                umma_ts(d, qh, kh, kScore, 1u);
+                umma_ts(d, ql, kh, score, x != 0 || k != 0);
+                umma_ts(d, qh, kl, score, 1u);
+                umma_ts(d, qh, kh, score, 1u);
               }
               umma_commit(slot_empty + 8 * slot);
               if (x == kHalves - 1) umma_commit(s_full + 8 * (gi & 1));
@@ -877,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           ++gi;
         }
         // The values of the tile before (gi now counts the scores issued).
-        if (i > 0) values(gi - (i < n ? 2 : 1));
+        if (i > 0) values(gi - (i < n ? 2 : 1), i == sinks ? sink_width : kTile);
       }
     }
     if (!ok && leader) {  // instructions in flight end before the block does
@@ -916,27 +922,33 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         ok = warp_wait(s_full + 8 * buf, (gi >> 1) & 1, err);
         if (!ok) break;
         tc_fence_after();
+        // Columns past a narrow tile's width hold what was there before.
+        const int width = (i == t.range.sinks - 1 ? t.range.width : kTile) - half * 64;
         float v[64];
-        tmem_ld64(at + buf * kTile, v);
-        if (!whole) {
-          const int j0 = tile * kTile + half * 64;
+        float m0 = -INFINITY;
+        if (width > 0) {
+          tmem_ld64(at + buf * kTile, v);
+          if (!whole) {
+            const int j0 = tile * kTile + half * 64;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t seen = seen_bits(mask, j0 + 32 * c);
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t seen = 32 * c < width ? seen_bits(mask, j0 + 32 * c) & bits_between(0, width, 32 * c) : 0u;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen >> e & 1u)) v[32 * c + e] = -INFINITY;
+              for (int e = 0; e < 32; ++e)
+                if (!(seen >> e & 1u)) v[32 * c + e] = -INFINITY;
+            }
           }
-        }
-        float m0 = v[0], m1 = v[1], m2 = v[2], m3 = v[3];
+          float m1 = v[1], m2 = v[2], m3 = v[3];
+          m0 = v[0];
 #pragma unroll
-        for (int e = 4; e < 64; e += 4) {
-          m0 = fmaxf(m0, v[e]);
-          m1 = fmaxf(m1, v[e + 1]);
-          m2 = fmaxf(m2, v[e + 2]);
-          m3 = fmaxf(m3, v[e + 3]);
+          for (int e = 4; e < 64; e += 4) {
+            m0 = fmaxf(m0, v[e]);
+            m1 = fmaxf(m1, v[e + 1]);
+            m2 = fmaxf(m2, v[e + 2]);
+            m3 = fmaxf(m3, v[e + 3]);
+          }
+          m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
         }
-        m0 = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
         // The row's other half is in the warp four further.
         most[(buf * 2 + half) * kTile + row] = m0;
         __syncwarp();
@@ -948,6 +960,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         float l[4] = {};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (32 * c >= width) break;
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[32 * c + e] = fmaf(v[32 * c + e], f, -c0);
 #pragma unroll
@@ -2005,11 +2018,14 @@ DecodePlan decode_plan(const AttentionShape& s) {
   p.rows = total == 1 ? 1 : total <= 4 ? 4 : kDecodeRows;
   p.row_blocks = (int)ceil_div(total, p.rows);
   // Each split takes the same number of keys, whatever its sequence's length:
-  // about six blocks per SM at full length, at least 256 keys each.
+  // about four blocks per SM at full length, at least 384 keys each.  Measured
+  // for one token, 16 heads over 4, 128 wide: four sequences of up to 32768 keys
+  // 83 us (two blocks per SM 89, six 88, twelve 93), 32 sequences with a window
+  // of 1024 41 us (at least 512 keys 41, 256 keys 47 to 49).
   int64_t most = s.k_len;
   if (s.window > 0) most = std::min<int64_t>(most, (int64_t)s.window + s.sinks + s.q_len - 1);
   const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks;
-  const int64_t want = std::max<int64_t>(1, std::min(ceil_div(kSms * 6, blocks > 0 ? blocks : 1), most / 256));
+  const int64_t want = std::max<int64_t>(1, std::min(ceil_div(kSms * 4, blocks > 0 ? blocks : 1), most / 384));
   p.per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(most, std::min<int64_t>(want, kMostSplits))), 32) * 32);
   p.splits = (int)std::max<int64_t>(1, ceil_div(most, p.per));
   return p;
