@@ -453,6 +453,17 @@ constexpr uint32_t kRowStep = 2048 >> 4;
 __device__ __forceinline__ uint32_t row_word(uint32_t box, uint32_t stride) { return box >> 4 | stride >> 4 << 16; }
 
 // A load and the wait for it in one statement: nothing reads the registers in between.
+__device__ __forceinline__ void tmem_ld8(uint32_t at, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_ld16(uint32_t at, float (&v)[16]) {
   uint32_t r[16];
   asm volatile(
@@ -508,34 +519,33 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Stores hi and lo of 32 neighbouring values as an A operand's 32 columns: 16
-// with hi (two values each), 16 with lo.
-__device__ __forceinline__ void store_split32(uint32_t at, const float* v) {
-  // Step by step over all of them, here and in the kernels: value by value, the
-  // chain of dependent instructions takes 40 cycles each.
-  uint32_t h[16], l[16];
-  float rest[32];
+// Stores 16 neighbouring values as an A operand's 16 columns: 8 with hi (two
+// values each), 8 with lo.  Step by step over all of them, here and in the
+// kernels: value by value, the chain of dependent instructions takes 40 cycles
+// each.
+__device__ __forceinline__ void store_split16(uint32_t at, const float* v) {
+  uint32_t r[16];
+  float rest[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const __half2 x = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-    h[i] = *(const uint32_t*)&x;
+    r[i] = *(const uint32_t*)&x;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float2 back = __half22float2(*(const __half2*)&h[i]);
+  for (int i = 0; i < 8; ++i) {
+    const float2 back = __half22float2(*(const __half2*)&r[i]);
     rest[2 * i] = v[2 * i] - back.x;
     rest[2 * i + 1] = v[2 * i + 1] - back.y;
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const __half2 y = __floats2half2_rn(rest[2 * i], rest[2 * i + 1]);
-    l[i] = *(const uint32_t*)&y;
+    r[8 + i] = *(const uint32_t*)&y;
   }
-  tmem_st16(at, h);
-  tmem_st16(at + 16, l);
+  tmem_st16(at, r);
 }
-// Column of the t-th 16 terms' hi part in such an operand (lo: 16 further).
-__device__ __forceinline__ uint32_t split_col(int t) { return (uint32_t)((t >> 1) * 32 + (t & 1) * 8); }
+// Columns of such an operand per 16 terms, and from their hi to their lo part.
+constexpr uint32_t kSplitStep = 16, kSplitLo = 8;
 
 // A resident packed tile from shared memory into tensor memory, where it is the
 // A operand of every score product: one read instead of one per instruction
@@ -832,13 +842,13 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         constexpr int kSteps = kTile / 16 / kHalves;
         constexpr uint32_t kStride = kBox / kHalves;  // between the slot's boxes
         const uint32_t v = row_word(slots + slot * kSlotBytes, kStride);
-        const uint32_t px = p + split_col(x * kSteps);
+        const uint32_t px = p + x * kSteps * kSplitStep;
         if (leader) {
 #pragma unroll
           for (int k = 0; k < kSteps; ++k) {
             if ((x * kSteps + k) * 16 >= width) break;
-            const uint32_t ph = px + split_col(k), vh = v + k * kRowStep, vl = vh + (kBox >> 4);
-            umma_ts(d, ph + 16, vh, kValue, x != 0 || k != 0);
+            const uint32_t ph = px + k * kSplitStep, vh = v + k * kRowStep, vl = vh + (kBox >> 4);
+            umma_ts(d, ph + kSplitLo, vh, kValue, x != 0 || k != 0);
             umma_ts(d, ph, vl, kValue, 1u);
             umma_ts(d, ph, vh, kValue, 1u);
           }
@@ -967,7 +977,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           for (int e = 0; e < 32; ++e) v[32 * c + e] = exp2_fast(v[32 * c + e]);
 #pragma unroll
           for (int e = 0; e < 32; ++e) l[e & 3] += v[32 * c + e];
-          store_split32(at + buf * kTile + 32 * c, v + 32 * c);
+          store_split16(at + buf * kTile + 32 * c, v + 32 * c);
+          store_split16(at + buf * kTile + 32 * c + 16, v + 32 * c + 16);
         }
         // Four buffers: these scores come after the values of two tiles before
         // were issued, which waited until the output warps had taken the tile
@@ -1075,11 +1086,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 // brought near 2^15 by a power of two from |dS| <= |dO_i| |V_j| + |delta_i|, with
 // the norms of single rows on the resident side and a tile's greatest on the
 // streamed one.
-//   warps 0-3    P and dS: a thread owns a row,
-//   warps 4-11   sums into registers, half of the columns each,
-//   warp 12      copies: resident tiles of the next item, rings of half steps (a
+//   warps 0-7    P and dS: two threads share a row, 32 columns each,
+//   warps 8-15   sums into registers, half of the columns each,
+//   warp 16      copies: resident tiles of the next item, rings of half steps (a
 //                step's lo boxes, then its hi ones),
-//   warp 13      matrix instructions.  Of a step g: dv of g, the scores of g + 1,
+//   warp 17      matrix instructions.  Of a step g: dv of g, the scores of g + 1,
 //                dq or dk of g, dP of g + 1.  P of a step is formed while the
 //                last step's dS is summed, and its dS while the next scores are.
 // Resident tiles are in tensor memory (rows_to_tmem), with one buffer each of
@@ -1087,10 +1098,19 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 // A key tile's queries may be many (a sink's are all that follow): its steps
 // are cut into segments that go to different blocks, each leaving its part in
 // the workspace, joined in order by grad_join_kernel.
-constexpr int kGradThreads = 16 * 32;  // warps 14 and 15 only hold registers for the others
-// Launched with 128 registers a thread, 512 for the four warps of each quarter
-// of an SM; after the split 144 + 2 x 160 + 48 = 512.
-constexpr int kProbRegs = 144, kSumRegs = 160, kGradFewRegs = 48;
+// Registers after the split, as in the forward: the keys' pass keeps sums of two
+// gradients, 2 x 64 + 2 x 152 + 48 = 480; the queries' 2 x 112 + 2 x 88 + 64 = 464.
+template <bool KEYS>
+constexpr int kProbRegs = KEYS ? 64 : 112;
+template <bool KEYS>
+constexpr int kSumRegs = KEYS ? 152 : 88;
+template <bool KEYS>
+constexpr int kGradFewRegs = KEYS ? 48 : 64;
+template <int N>
+__device__ __forceinline__ void set_registers() {  // from the 96 of the launch
+  if constexpr (N < 96) fewer_registers<N>();
+  else more_registers<N>();
+}
 constexpr int kStep = 64;
 constexpr int kStepBox = kStep * 128;  // bytes of 64 rows of a box
 
@@ -1237,7 +1257,7 @@ __device__ __forceinline__ void store_row(float* __restrict__ dst, const float (
 }
 
 template <int DP, bool KEYS>
-__global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
+__global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
   using Plan = GradPlan<DP, KEYS>;
   constexpr int kHalves = Plan::kHalves, kPart = Plan::kPart;
   constexpr uint32_t kEntries1 = Plan::kEntries1, kEntries2 = Plan::kEntries2;
@@ -1261,14 +1281,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
   }
   if (threadIdx.x == 0) {
     mbar_init(a_full, 1);
-    mbar_init(a_empty, 4);
-    mbar_init(a_ready, 4);
+    mbar_init(a_empty, 8);
+    mbar_init(a_ready, 8);
     for (int i = 0; i < (int)kEntries1; ++i) mbar_init(full1 + 8 * i, 1), mbar_init(empty1 + 8 * i, 1);
     for (int i = 0; i < (int)kEntries2; ++i) mbar_init(full2 + 8 * i, 1), mbar_init(empty2 + 8 * i, 1);
     mbar_init(s_full, 1);
     mbar_init(d_full, 1);
-    mbar_init(s_done, 4);
-    mbar_init(ds_full, 4);
+    mbar_init(s_done, 8);
+    mbar_init(ds_full, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, kHalves == 2 ? 4 : 8);
@@ -1276,7 +1296,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 13) {
+  if (warp == 17) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -1295,10 +1315,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
     return KEYS ? (t.b * s.heads + t.h + x) * tiles_q + *step / 2 : (t.b * s.kv_heads + t.g) * tiles_k + *step / 2;
   };
 
-  if (warp >= 14) {
-    fewer_registers<kGradFewRegs>();
-  } else if (warp == 12) {
-    fewer_registers<kGradFewRegs>();
+  if (warp >= 18) {
+    set_registers<kGradFewRegs<KEYS>>();
+  } else if (warp == 16) {
+    set_registers<kGradFewRegs<KEYS>>();
     uint32_t gi = 0, loaded = 0;  // steps, items
     bool ok = true;
     // Half a step of a ring: `part` 0 the lo boxes, 1 the hi ones; with the
@@ -1350,8 +1370,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         mbar_wait_limit(full2 + 8 * (f % kEntries2), (f / kEntries2) & 1, err, kWaitCycles / 8);
       }
     }
-  } else if (warp == 13) {
-    fewer_registers<kGradFewRegs>();
+  } else if (warp == 17) {
+    set_registers<kGradFewRegs<KEYS>>();
     constexpr uint32_t kProduct = umma_idesc(kStep, false), kSum = umma_idesc(64, true);
     const bool leader = elect_one();
     uint32_t gi = 0, item = 0;           // steps whose scores, items that were issued
@@ -1397,9 +1417,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       if (leader) {
 #pragma unroll
         for (int k = 0; k < kStep / 16; ++k) {
-          umma_ts(d, p + split_col(k), cl + k * kRowStep, kSum, k != 0);
-          umma_ts(d, p + split_col(k) + 16, chi + k * kRowStep, kSum, 1u);
-          umma_ts(d, p + split_col(k), chi + k * kRowStep, kSum, 1u);
+          umma_ts(d, p + k * kSplitStep, cl + k * kRowStep, kSum, k != 0);
+          umma_ts(d, p + k * kSplitStep + kSplitLo, chi + k * kRowStep, kSum, 1u);
+          umma_ts(d, p + k * kSplitStep, chi + k * kRowStep, kSum, 1u);
         }
         umma_commit(o_full + 8 * buf);
       }
@@ -1453,10 +1473,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       umma_commit(drained);
       mbar_wait(drained, 0, err);
     }
-  } else if (warp < 4) {
-    more_registers<kProbRegs>();
-    const int row = warp * 32 + lane;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+  } else if (warp < 8) {
+    set_registers<kProbRegs<KEYS>>();
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, at_s = tmem_s + lanes + 32 * half, at_d = tmem_d + lanes + 32 * half;
     uint32_t gi = 0, item = 0;
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
@@ -1464,21 +1484,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       const GradItem t = grad_item<KEYS>(a, w, err);
       if (t.n == 0 && t.first) {
         if (!KEYS)
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 4)
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
             simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
         else
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 4)
+          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 8)
             simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
       }
       if (t.f0 >= t.f1) continue;
       // The products with the resident tiles before are done: they have been read.
       ok = warp_wait(a_full, item & 1, err);
       if (!ok) break;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        rows_to_tmem<DP>(tmem + lanes, base, row, half);
-        rows_to_tmem<DP>(tmem + DP + lanes, base + kTileBytes<DP>, row, half);
-      }
+      rows_to_tmem<DP>(tmem + lanes, base, row, half);
+      rows_to_tmem<DP>(tmem + DP + lanes, base + kTileBytes<DP>, row, half);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
@@ -1510,18 +1527,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
         const float up = power_of_two(scale_exponent(bound));
         bool whole;
-        uint32_t seen[2];
+        uint32_t seen;
         if (!KEYS) {
           whole = t.rows.all && c0 + kStep - 1 <= t.rows.p0 &&
                   (s.window == 0 || t.rows.p1 - c0 < s.window || c0 + kStep <= s.sinks);
-          seen[0] = seen_bits(mask, c0);
-          seen[1] = seen_bits(mask, c0 + 32);
+          seen = seen_bits(mask, c0 + 32 * half);
         } else {
           const int first = t.sq.start + c0, last = first + kStep - 1, k1 = t.r0 + kTile - 1;
           whole = k1 <= first && last < t.sq.n && c0 + kStep <= s.q_len &&
                   (s.window == 0 || last - t.r0 < s.window || k1 < s.sinks);
-          seen[0] = bits_between(s0, s1, c0);
-          seen[1] = bits_between(s0, s1, c0 + 32);
+          seen = bits_between(s0, s1, c0 + 32 * half);
         }
         ok = warp_wait(s_full, gi & 1, err);
         if (KEYS && ok) {  // the statistics' copy, with the second half of its step
@@ -1530,9 +1545,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         }
         if (!ok) break;
         tc_fence_after();
-        const float2* col = (const float2*)(info_smem + (gi & 1) * (kStep * 8));
-        float v[64];
-        tmem_ld64(tmem_s + lanes, v);
+        const float2* col = (const float2*)(info_smem + (gi & 1) * (kStep * 8)) + 32 * half;
+        float v[32];
+        tmem_ld32(at_s, v);
         if (!KEYS) {
           tc_fence_before();
           __syncwarp();
@@ -1540,37 +1555,37 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
         }
         if (!whole) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!(seen[e / 32] >> (e & 31) & 1u)) v[e] = -INFINITY;
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1u)) v[e] = -INFINITY;
         }
         // Keys: 2^14 P, the 2^14 / sum and the greatest score in one exponent.
 #pragma unroll
-        for (int e = 0; e < 64; ++e) v[e] = fmaf(v[e], f, KEYS ? -col[e].x : -st.x);
+        for (int e = 0; e < 32; ++e) v[e] = fmaf(v[e], f, KEYS ? -col[e].x : -st.x);
 #pragma unroll
-        for (int e = 0; e < 64; ++e) v[e] = exp2_fast(v[e]);
+        for (int e = 0; e < 32; ++e) v[e] = exp2_fast(v[e]);
         if (KEYS) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) store_split32(tmem_s + lanes + 32 * c, v + 32 * c);
+          store_split16(at_s, v);
+          store_split16(at_s + 16, v + 16);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(s_done);
         }
+        const float rescale = KEYS ? up * 0x1p-14f : up * st.y;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] *= rescale;
         ok = warp_wait(d_full, gi & 1, err);
         if (!ok) break;
         tc_fence_after();
-        const float rescale = KEYS ? up * 0x1p-14f : up * st.y;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float d[32];
-          tmem_ld32(tmem_d + lanes + 32 * c, d);
+        for (int c = 0; c < 32; c += 16) {
+          float d[16];
+          tmem_ld16(at_d + c, d);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) d[e] = fmaf(d[e], f2, KEYS ? -col[32 * c + e].y : -st.z);
+          for (int e = 0; e < 16; ++e) d[e] = fmaf(d[e], f2, KEYS ? -col[c + e].y : -st.z);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[32 * c + e] *= rescale;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) d[e] *= v[32 * c + e];
-          store_split32(tmem_d + lanes + 32 * c, d);
+          for (int e = 0; e < 16; ++e) d[e] *= v[c + e];
+          store_split16(at_d + c, d);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
@@ -1579,9 +1594,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       }
     }
   } else {
-    more_registers<kSumRegs>();
+    set_registers<kSumRegs<KEYS>>();
     constexpr int kCols = DP / 2;  // columns of a thread
-    const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+    const int half = (warp - 8) >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t taken0 = 0, taken1 = 0;  // sums taken from each buffer
     bool ok = true;
@@ -1593,16 +1608,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
       tc_fence_after();
       const uint32_t at = tmem_o + lanes + 64 * buf + (kHalves == 2 ? 0 : half * kCols);
 #pragma unroll
-      for (int c = 0; c < kCols; c += 16) {
-        float v[16];
-        tmem_ld16(at + c, v);
-        if (c == kCols - 16) {  // the last values are out: the buffer is free
+      for (int c = 0; c < kCols; c += 8) {
+        float v[8];
+        tmem_ld8(at + c, v);
+        if (c == kCols - 8) {  // the last values are out: the buffer is free
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(o_empty + 8 * buf);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[c + e] = fmaf(v[e], by, acc[c + e]);
+        for (int e = 0; e < 8; ++e) acc[c + e] = fmaf(v[e], by, acc[c + e]);
       }
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
@@ -1647,7 +1662,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(GradArgs a, int i
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 17) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
@@ -2145,7 +2160,7 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   const int64_t items = KEYS ? grad_units(s, a.seg) : (int64_t)tiles_of(s.q_len) * s.heads * s.batch;
   if (items == 0) return;
   if (items > INT_MAX / 64) throw CudaError("window_attention: too many rows");
-  grad_kernel<DP, KEYS><<<(unsigned)(items < kSms ? items : kSms), kGradThreads, kSmem, st>>>(a, (int)items, err);
+  grad_kernel<DP, KEYS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
   if (!KEYS) return;
   const int tiles = tiles_of(s.k_len), stride = s.kv_heads * s.batch;
