@@ -53,6 +53,7 @@ def window_attention(q, k, v, starts, lengths, window, sinks, scale, seq_major, 
     out = np.zeros(q.shape)
     stats = np.zeros((batch, heads, q_len, 2))
     dq, dk, dv = np.zeros(q.shape), np.zeros(k.shape), np.zeros(v.shape)
+    size_q, size_k = np.zeros(q.shape), np.zeros(k.shape)
     for b in range(batch):
         any_row = seen[b].any(0)
         live = seen[b].any(1)
@@ -74,9 +75,13 @@ def window_attention(q, k, v, starts, lengths, window, sinks, scale, seq_major, 
                 dq[b, h] = ds @ kk
                 dk[b, h // group] += ds.T @ qq
                 dv[b, h // group] += p.T @ g
+                # The size of the terms whose difference dS is.
+                terms = p * (np.abs(g) @ np.abs(vv).T + (np.abs(g) * np.abs(o)).sum(1, keepdims=True)) * scale
+                size_q[b, h] = terms @ np.abs(kk)
+                size_k[b, h // group] += terms.T @ np.abs(qq)
     r = {"out": out, "stats": stats}
     if dout is not None:
-        r.update(dq=dq, dk=dk, dv=dv)
+        r.update(dq=dq, dk=dk, dv=dv, size_dq=size_q, size_dk=size_k)
     if seq_major:
         r = {n: t if n == "stats" else np.swapaxes(t, 1, 2) for n, t in r.items()}
     return r

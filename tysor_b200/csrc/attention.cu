@@ -72,7 +72,11 @@ __device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence&
   return v;
 }
 
-// ---- every shape and every value: one warp per row --------------------------------
+// ---- every value: one warp per row -------------------------------------------------
+
+// What is not finite would spoil the hidden places of a matrix product (0 times
+// it is not 0), so rows and keys that meet such values go one by one, taking in
+// only what they see; so do those that see nothing.
 
 // A row's values over a warp's lanes: lane l holds columns l, l + 32, ...
 constexpr int kLaneDims = kMaxHeadDim / 32;
@@ -105,8 +109,8 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
                                    const float* v, float* out, float* stats, int b, int h, int r) {
   const int g = h / (s.heads / s.kv_heads);
   const Seen seen = seen_by(s, sq, sq.start + r);
-  float qv[kLaneDims], acc[kLaneDims] = {};
-  lane_load(q + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, qv);
+  float qv[kLaneDims] = {}, acc[kLaneDims] = {};
+  if (seen.high > 0) lane_load(q + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, qv);
   float m = -INFINITY, l = 0.0f;
   for (int j = 0; j < seen.high; ++j) {
     if (j == seen.first && j < seen.low) j = seen.low;
@@ -135,6 +139,10 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
   const Seen seen = seen_by(s, sq, sq.start + r);
   const int64_t at = row_at(s, b, h, r, s.heads, s.q_len);
   float qv[kLaneDims], gv[kLaneDims], kv[kLaneDims], vv[kLaneDims], acc[kLaneDims] = {};
+  if (seen.high == 0) {
+    if (!accumulate) lane_store(dq + at, s.head_dim, acc, 1.0f, 0);
+    return;
+  }
   lane_load(out + at, s.head_dim, kv);
   lane_load(dout + at, s.head_dim, gv);
   lane_load(q + at, s.head_dim, qv);
@@ -150,18 +158,6 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
     for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * kv[i];
   }
   lane_store(dq + at, s.head_dim, acc, s.scale, accumulate);
-}
-
-__global__ void __launch_bounds__(256) simple_dq_kernel(AttentionShape s, const float* __restrict__ q,
-                                                        const float* __restrict__ k, const float* __restrict__ v,
-                                                        const float* __restrict__ out,
-                                                        const float* __restrict__ stats,
-                                                        const float* __restrict__ dout, float* __restrict__ dq,
-                                                        int accumulate, int* err) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= (int64_t)s.batch * s.heads * s.q_len) return;
-  const int r = (int)(i % s.q_len), h = (int)(i / s.q_len % s.heads), b = (int)(i / s.q_len / s.heads);
-  simple_dq_row(s, sequence_of(s, b, err), q, k, v, out, stats, dout, dq, accumulate, b, h, r);
 }
 
 // The query rows that see key j: those at positions [j, end).
@@ -180,6 +176,7 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
   float kv[kLaneDims], vv[kLaneDims], ak[kLaneDims] = {}, av[kLaneDims] = {};
   int r0, r1;
   rows_seeing(s, sq, j, &r0, &r1);
+  if (r0 >= r1 && accumulate_k && accumulate_v) return;
   if (r0 < r1) {
     lane_load(k + at, s.head_dim, kv);
     lane_load(v + at, s.head_dim, vv);
@@ -202,19 +199,6 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
   }
   lane_store(dk + at, s.head_dim, ak, s.scale, accumulate_k);
   lane_store(dv + at, s.head_dim, av, 1.0f, accumulate_v);
-}
-
-__global__ void __launch_bounds__(256) simple_dkv_kernel(AttentionShape s, const float* __restrict__ q,
-                                                         const float* __restrict__ k, const float* __restrict__ v,
-                                                         const float* __restrict__ out,
-                                                         const float* __restrict__ stats,
-                                                         const float* __restrict__ dout, float* __restrict__ dk,
-                                                         float* __restrict__ dv, int accumulate_k, int accumulate_v,
-                                                         int* err) {
-  const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= (int64_t)s.batch * s.kv_heads * s.k_len) return;
-  const int j = (int)(i % s.k_len), g = (int)(i / s.k_len % s.kv_heads), b = (int)(i / s.k_len / s.kv_heads);
-  simple_dkv_row(s, sequence_of(s, b, err), q, k, v, out, stats, dout, dk, dv, accumulate_k, accumulate_v, b, g, j);
 }
 
 // ---- operands of the tensor-core kernels ---------------------------------------------
@@ -639,9 +623,10 @@ __device__ __forceinline__ bool sees_all(const AttentionShape& s, const RowRange
 //   warp 16      copies packed tiles: the next item's queries, and the keys and
 //                values into a ring of 32 KB slots,
 //   warp 17      issues the matrix instructions: the scores of a tile before
-//                the values of the one before it, so that the two overlap.
+//                the values of the one before it, so that the two overlap,
+//   warps 18-19  rows that take no part in that.
 // The query tile is kept in tensor memory (rows_to_tmem).
-constexpr int kThreads = 20 * 32;  // warps 18 and 19 only hold registers for the others
+constexpr int kThreads = 20 * 32;
 constexpr int kSlotBytes = 2 * kBox;
 
 // Registers per thread: launched with 96 (640 threads), 480 for the five warps
@@ -779,6 +764,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
 
   if (warp >= 18) {
     fewer_registers<kFewRegs>();
+    // Items that see nothing or meet values that are not finite, key by key.
+    // No wait of the pipeline depends on these warps, however long they take.
+    for (int round = 0, w; item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
+      if (t.n == 0)
+        for (int r = t.r0 + warp - 18; r < min(t.r0 + kTile, s.q_len); r += 2)
+          simple_forward_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, t.b, t.h, r);
+    }
   } else if (warp == 16) {
     fewer_registers<kFewRegs>();
     uint32_t it = 0, loaded = 0;      // slots filled, query tiles loaded
@@ -909,11 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (t.n == 0) {
-        for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
-          simple_forward_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, t.b, t.h, r);
-        continue;
-      }
+      if (t.n == 0) continue;
       // The products with the query tile before are done: their scores have been read.
       ok = warp_wait(q_full, item & 1, err);
       if (!ok) break;
@@ -1317,6 +1307,16 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
 
   if (warp >= 18) {
     set_registers<kGradFewRegs<KEYS>>();
+    // As in the forward: items for which the matrix unit is of no use.
+    for (int round = 0, w; item_of(round, items, &w); ++round) {
+      if (w < 0) continue;
+      const GradItem t = grad_item<KEYS>(a, w, err);
+      if (t.n != 0 || !t.first) continue;
+      for (int r = t.r0 + warp - 18; r < min(t.r0 + kTile, KEYS ? s.k_len : s.q_len); r += 2) {
+        if (!KEYS) simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
+        else simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
+      }
+    }
   } else if (warp == 16) {
     set_registers<kGradFewRegs<KEYS>>();
     uint32_t gi = 0, loaded = 0;  // steps, items
@@ -1482,14 +1482,6 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<KEYS>(a, w, err);
-      if (t.n == 0 && t.first) {
-        if (!KEYS)
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.q_len); r += 8)
-            simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
-        else
-          for (int r = t.r0 + warp; r < min(t.r0 + kTile, s.k_len); r += 8)
-            simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
-      }
       if (t.f0 >= t.f1) continue;
       // The products with the resident tiles before are done: they have been read.
       ok = warp_wait(a_full, item & 1, err);
@@ -1696,7 +1688,7 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
 
 // ---- a few query rows over a long cache ----------------------------------------------------
 
-// The rows that share a key head (at most R of them per block) go over its
+// The rows that share a key head (at most R) go over its
 // keys once, straight from the fp32 cache: with so few rows the reads bound
 // it, not the products.  The keys are split over `splits` blocks; each warp
 // takes 8 keys at a time, eight lanes per key with 4 NI columns each, and each
@@ -1744,7 +1736,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
                                                                 float* __restrict__ stats, float* __restrict__ part,
-                                                                int splits, int per, int row_blocks, int* err) {
+                                                                int splits, int per, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ __align__(16) float qs[R][kDims];
   __shared__ float joined[kWarps][R][kDims + 2];
@@ -1752,8 +1744,6 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   int64_t index = blockIdx.x;
   const int split = (int)(index % splits);
   index /= splits;
-  const int rb = (int)(index % row_blocks);
-  index /= row_blocks;
   const int g = (int)(index % s.kv_heads), b = (int)(index / s.kv_heads);
   const int group = s.heads / s.kv_heads, total = group * s.q_len;
   const Sequence sq = sequence_of(s, b, err);
@@ -1763,7 +1753,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   if (splits > 1 && u0 == u1 && split > 0) return;  // the join knows how many splits hold keys
   const float to_log2 = s.scale * kLog2e;
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
-    const int r = rb * R + i / kDims, c = i % kDims;
+    const int r = i / kDims, c = i % kDims;
     qs[i / kDims][c] = r < total && c < s.head_dim
                            ? q[row_at(s, b, g * group + r / s.q_len, r % s.q_len, s.heads, s.q_len) + c]
                            : 0.0f;
@@ -1771,8 +1761,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   int at[R];  // position of each row; below 0: not a row, or not in the sequence
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int p = sq.start + (rb * R + r) % s.q_len;
-    at[r] = rb * R + r < total && p < sq.n ? p : -1;
+    const int p = sq.start + r % s.q_len;
+    at[r] = r < total && p < sq.n ? p : -1;
   }
   __syncthreads();
   float m[R], l[R];
@@ -1916,9 +1906,9 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
-    const int r = i / kDims, c = i % kDims, row = rb * R + r;
-    if (row >= total || c >= s.head_dim) continue;
-    const int h = g * group + row / s.q_len, qr = row % s.q_len;
+    const int r = i / kDims, c = i % kDims;
+    if (r >= total || c >= s.head_dim) continue;
+    const int h = g * group + r / s.q_len, qr = r % s.q_len;
     float top = -INFINITY, sum = 0.0f, x = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, joined[w][r][kDims]);
@@ -2020,18 +2010,19 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   return w;
 }
 
-// Up to this many rows per key head go through decode_kernel.
-constexpr int64_t kFewRows = 16;
-bool uses_tiles(const AttentionShape& s) { return (int64_t)s.q_len * (s.heads / s.kv_heads) > kFewRows; }
+// Up to kDecodeRows rows per key head go through decode_kernel, more through the
+// tiles.  Measured without a window, 128 wide: 8 rows over 4096 keys of 8
+// sequences and 4 key heads 103 us against 122, over 8192 keys of 4 sequences
+// and 16 key heads 284 against 300; 16 rows, two blocks of them, 169 and 515.
+bool uses_tiles(const AttentionShape& s) { return (int64_t)s.q_len * (s.heads / s.kv_heads) > kDecodeRows; }
 
 struct DecodePlan {
-  int rows, row_blocks, splits, per;
+  int rows, splits, per;
 };
 DecodePlan decode_plan(const AttentionShape& s) {
   DecodePlan p;
   const int total = s.q_len * (s.heads / s.kv_heads);
   p.rows = total == 1 ? 1 : total <= 4 ? 4 : kDecodeRows;
-  p.row_blocks = (int)ceil_div(total, p.rows);
   // Each split takes the same number of keys, whatever its sequence's length:
   // about four blocks per SM at full length, at least 384 keys each.  Measured
   // for one token, 16 heads over 4, 128 wide: four sequences of up to 32768 keys
@@ -2039,7 +2030,7 @@ DecodePlan decode_plan(const AttentionShape& s) {
   // of 1024 41 us (at least 512 keys 41, 256 keys 47 to 49).
   int64_t most = s.k_len;
   if (s.window > 0) most = std::min<int64_t>(most, (int64_t)s.window + s.sinks + s.q_len - 1);
-  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks;
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads;
   const int64_t want = std::max<int64_t>(1, std::min(ceil_div(kSms * 4, blocks > 0 ? blocks : 1), most / 384));
   p.per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(most, std::min<int64_t>(want, kMostSplits))), 32) * 32);
   p.splits = (int)std::max<int64_t>(1, ceil_div(most, p.per));
@@ -2054,18 +2045,16 @@ int64_t decode_work_elems(const AttentionShape& s) {
 template <int NI, int R>
 void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v, float* out,
                 float* stats, float* part, int* err, cudaStream_t st) {
-  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.row_blocks * p.splits;
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.splits;
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   constexpr int kRing = kDecodeThreads / 32 * kDecodeStages * 16 * 32 * NI * (int)sizeof(float);
   if (vec)
     TYSOR_CUDA(cudaFuncSetAttribute(decode_kernel<NI, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
   if (vec)
-    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
-                                                                            p.row_blocks, err);
+    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
   else
-    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per,
-                                                                             p.row_blocks, err);
+    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
   check_launch();
 }
 template <int NI>
@@ -2148,10 +2137,6 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   return w;
 }
 
-// Below a tile's half in rows or keys the packing and the padded products cost
-// more than a warp per row.
-bool grads_use_tiles(const AttentionShape& s) { return s.q_len >= 16; }
-
 template <int DP, bool KEYS>
 void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   constexpr int kSmem = GradPlan<DP, KEYS>::kSmem;
@@ -2193,7 +2178,7 @@ int64_t window_attention_work_elems(const AttentionShape& s) {
   return uses_tiles(s) ? forward_work(s, nullptr).floats : decode_work_elems(s);
 }
 int64_t window_attention_backward_work_elems(const AttentionShape& s) {
-  return grads_use_tiles(s) ? grad_work(s, nullptr).floats : 1;
+  return grad_work(s, nullptr).floats;
 }
 
 void launch_window_attention(const AttentionShape& s, const float* q, const float* k, const float* v, float* out,
@@ -2229,34 +2214,22 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                                       const float* out, const float* stats, const float* dout, float* dq, float* dk,
                                       float* dv, float* work, int accumulate_q, int accumulate_k, int accumulate_v,
                                       int* err, cudaStream_t st) {
-  const int64_t rows = (int64_t)s.batch * s.heads * s.q_len, keys = (int64_t)s.batch * s.kv_heads * s.k_len;
-  if (rows > 0 && grads_use_tiles(s)) {
-    const GradWork w = grad_work(s, work);
-    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
-                       {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.col, w.tdo},
-                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
-                       {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
-    run_pack(s, jobs, 4, err, st);
-    const GradArgs a{s,    q,    k,    v,    out,  stats, dout,  w.pq,  w.pk,   w.pv, w.po, w.fq,         w.fk,
-                     w.fv, w.fo, w.nv, w.tnv, w.tno, w.tdo, w.info, w.col, dq,   dk,   dv,   accumulate_q, accumulate_k, accumulate_v,
-                     segments_of(s), w.part};
-    if (padded_dim(s) == 64) {
-      run_grad<64, false>(a, err, st);
-      run_grad<64, true>(a, err, st);
-    } else {
-      run_grad<128, false>(a, err, st);
-      run_grad<128, true>(a, err, st);
-    }
-    return;
-  }
-  if (rows > 0) {
-    simple_dq_kernel<<<(unsigned)ceil_div(rows, 8), 256, 0, st>>>(s, q, k, v, out, stats, dout, dq, accumulate_q, err);
-    check_launch();
-  }
-  if (keys > 0) {
-    simple_dkv_kernel<<<(unsigned)ceil_div(keys, 8), 256, 0, st>>>(s, q, k, v, out, stats, dout, dk, dv, accumulate_k,
-                                                                    accumulate_v, err);
-    check_launch();
+  if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return;
+  const GradWork w = grad_work(s, work);
+  PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
+                     {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.col, w.tdo},
+                     {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
+                     {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
+  run_pack(s, jobs, 4, err, st);
+  const GradArgs a{s,     q,     k,     v,      out,   stats, dout, w.pq, w.pk, w.pv,         w.po,         w.fq,         w.fk,
+                   w.fv,  w.fo,  w.nv,  w.tnv,  w.tno, w.tdo, w.info, w.col, dq, dk,          dv,           accumulate_q, accumulate_k,
+                   accumulate_v, segments_of(s), w.part};
+  if (padded_dim(s) == 64) {
+    run_grad<64, false>(a, err, st);
+    run_grad<64, true>(a, err, st);
+  } else {
+    run_grad<128, false>(a, err, st);
+    run_grad<128, true>(a, err, st);
   }
 }
 

@@ -798,7 +798,8 @@ void launch_rope_axes(const float* x, const float* positions, const double* rate
   // All heads of a token in one thread share its angles; where that leaves
   // fewer than two blocks per SM, the heads are spread over more threads.
   int64_t chunk = shape.heads * items / (148 * 2 * 256);
-  chunk = chunk < 1 ? 1 : chunk > shape.heads ? shape.heads : chunk;
+  const int64_t least = ceil_div(shape.heads, 65535);  // blocks of the grid's second axis
+  chunk = chunk < least ? least : chunk > shape.heads ? shape.heads : chunk;
   RopeArgs a{shape, (int)chunk, back, accumulate};
   for (int e = shape.axes - 1; e < kMaxRopeAxes; ++e) a.s.ends[e] = INT_MAX;  // the last axis takes the rest
   const dim3 grid((unsigned)ceil_div(items, 256), (unsigned)ceil_div(shape.heads, chunk));
@@ -810,6 +811,7 @@ void launch_rope_axes(const float* x, const float* positions, const double* rate
 void launch_distill_loss(const float* logits, const float* ids, const float* teacher, float* loss, float* stats,
                          int64_t rows, int64_t width, int top, float temperature, int* err, cudaStream_t st) {
   if (rows <= 0) return;
+  if (rows > INT_MAX) throw CudaError("distill_loss takes up to 2^31 - 1 rows");
   // A row is split over up to eight blocks where whole rows leave SMs idle
   // and a part still gives each thread a few loads.
   int parts = 1;
@@ -833,6 +835,7 @@ void launch_distill_loss_backward(const float* logits, const float* ids, const f
                                   const float* dloss, float* grad, int64_t rows, int64_t width, int top,
                                   float temperature, int accumulate, int* err, cudaStream_t st) {
   if (rows <= 0) return;
+  if (rows > INT_MAX) throw CudaError("distill_loss takes up to 2^31 - 1 rows");
   int64_t parts = 1;
   while (rows * parts < 148 * 4 && width / (parts * 2) >= 4 * kDistillThreads && parts < 1024) parts *= 2;
   const int64_t chunk = ceil_div(ceil_div(width, parts), 4) * 4;
