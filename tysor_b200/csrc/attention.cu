@@ -5,6 +5,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "lm_ops.cuh"
 #include "tcgen05.cuh"
@@ -1988,6 +1989,17 @@ struct Carver {
 
 constexpr int64_t kSms = 148;
 
+// Lets a kernel take `bytes` of dynamic shared memory, once per device.
+template <typename K>
+void allow_shared(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  TYSOR_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return;
+  TYSOR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+}
+
 int padded_dim(const AttentionShape& s) { return s.head_dim <= 64 ? 64 : 128; }
 
 struct ForwardWork {
@@ -2049,8 +2061,8 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   constexpr int kRing = kDecodeThreads / 32 * kDecodeStages * 16 * 32 * NI * (int)sizeof(float);
-  if (vec)
-    TYSOR_CUDA(cudaFuncSetAttribute(decode_kernel<NI, R, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+  static std::atomic<uint64_t> done{0};
+  if (vec) allow_shared(decode_kernel<NI, R, true>, kRing, done);
   if (vec)
     decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
   else
@@ -2140,7 +2152,8 @@ GradWork grad_work(const AttentionShape& s, float* base) {
 template <int DP, bool KEYS>
 void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   constexpr int kSmem = GradPlan<DP, KEYS>::kSmem;
-  TYSOR_CUDA(cudaFuncSetAttribute(grad_kernel<DP, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+  static std::atomic<uint64_t> done{0};
+  allow_shared(grad_kernel<DP, KEYS>, kSmem, done);
   const AttentionShape& s = a.s;
   const int64_t items = KEYS ? grad_units(s, a.seg) : (int64_t)tiles_of(s.q_len) * s.heads * s.batch;
   if (items == 0) return;
@@ -2164,8 +2177,8 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
 
 template <int DP>
 void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
-  TYSOR_CUDA(cudaFuncSetAttribute(forward_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  ForwardPlan<DP>::kSmem));
+  static std::atomic<uint64_t> done{0};
+  allow_shared(forward_kernel<DP>, ForwardPlan<DP>::kSmem, done);
   const int64_t items = (int64_t)tiles_of(a.s.q_len) * a.s.heads * a.s.batch;  // at most what run_pack took
   forward_kernel<DP><<<(unsigned)(items < kSms ? items : kSms), kThreads, ForwardPlan<DP>::kSmem, st>>>(
       a, (int)items, err);
