@@ -221,7 +221,8 @@ void check_distill(uint32_t width, uint32_t top, float temperature) {
   if (width == 0 || width > 0x7fffffffu) throw CudaError("distill_loss requires a width of 1 to 2^31 - 1");
   if (top == 0 || top > (uint32_t)kMaxDistillTop)
     throw CudaError("distill_loss takes 1 to " + std::to_string(kMaxDistillTop) + " entries per row");
-  if (!(temperature > 0.0f) || isinf(temperature)) throw CudaError("distill_loss requires a finite temperature > 0");
+  if (!distill_temperature(temperature))
+    throw CudaError("distill_loss requires a finite temperature > 0, from 2^-60 to 2^60");
 }
 
 AttentionShape attention_shape(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t q_len, uint32_t k_len,

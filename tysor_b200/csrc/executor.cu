@@ -1255,7 +1255,8 @@ struct Executor {
         fail("distill_loss expects ids and teacher of [rows, top] for logits " + shape_str(z.shape) + ", got " +
              shape_str(id.shape) + " and " + shape_str(t.shape));
       if (top > kMaxDistillTop || w > INT32_MAX) fail("distill_loss takes 1 to " + std::to_string(kMaxDistillTop) + " entries per row");
-      if (!(temperature > 0.0f) || std::isinf(temperature)) fail("distill_loss requires a finite temperature > 0");
+      if (!distill_temperature(temperature))
+        fail("distill_loss requires a finite temperature > 0, from 2^-60 to 2^60");
       HVal o = new_tensor({rows, 1});
       Slot *a = z.slot, *ix = id.slot, *ts = t.slot, *c = o.slot;
       Slot* stats = mode == kModeRun ? nullptr : alloc((size_t)rows * 2);

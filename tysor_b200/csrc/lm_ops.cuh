@@ -49,6 +49,8 @@ void launch_rope_axes(const float* x, const float* positions, const double* rate
 // stats receives [rows][2] = (max logit, sum of exp((logit - max) / T)); the
 // gradient reads it.  dloss null: 1 for every row.
 constexpr int kMaxDistillTop = 1024;
+// Temperatures for which 1 / T and T^2 are far from the ends of fp32.
+inline bool distill_temperature(float t) { return t >= 0x1p-60f && t <= 0x1p60f; }
 void launch_distill_loss(const float* logits, const float* ids, const float* teacher, float* loss, float* stats,
                          int64_t rows, int64_t width, int top, float temperature, int* err, cudaStream_t st);
 void launch_distill_loss_backward(const float* logits, const float* ids, const float* teacher, const float* stats,
