@@ -263,8 +263,14 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * any result, whatever they hold.  q, out: [batch][heads][q_len][head_dim];
  * k, v: [batch][kv_heads][k_len][head_dim], kv_heads dividing heads (query
  * heads h * heads / kv_heads ... share key head h); with seq_major
- * [batch][length][heads][head_dim].  head_dim 1 to 128, scale at least 2^-126.  starts [batch] may
- * be NULL (k_len - q_len: the queries end where the keys end), lengths
+ * [batch][length][heads][head_dim].  head_dim 1 to 128, lengths up to 2^29,
+ * scale at least 2^-126.  Products carry fp32's accuracy relative to the
+ * greatest value among 128 rows of a head; rows that meet values of 2^100 and
+ * more, infinities or NaN are computed key by key, many times slower.  The
+ * call's workspace belongs to the context and grows with the sizes, which frees
+ * the old one: a caller that captures the context's stream into a graph calls
+ * the largest sizes once before, and lets one such graph run at a time.
+ * starts [batch] may be NULL (k_len - q_len: the queries end where the keys end), lengths
  * [batch] may be NULL (k_len); both hold whole numbers as floats, checked on
  * the device ("Attention start or length out of range").  stats may be NULL
  * or receives [batch][heads][q_len][2] = (greatest visible score, sum of
@@ -289,7 +295,7 @@ bool tysor_cuda_dispatch_window_attention_backward(void* context, void* q, void*
  * width; out[r] = T^2 * sum_e p_e * (ln p_e - ln q[ids[r][e]]).  ids are f32;
  * an id below 0 is an absent entry, and a row without any has loss 0.  An id
  * of width or more is an error ("Embedding index out of range").  An id
- * given twice counts twice.  stats may be NULL or receives [rows][2] =
+ * given twice counts twice.  The temperature is from 2^-60 to 2^60.  stats may be NULL or receives [rows][2] =
  * (greatest logit, sum of exp((logit - greatest) / T)). */
 bool tysor_cuda_dispatch_distill_loss(void* context, void* logits, void* ids, void* teacher, void* out,
                                       void* stats, uint32_t rows, uint32_t width, uint32_t top,

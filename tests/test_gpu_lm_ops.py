@@ -371,6 +371,46 @@ def test_window_attention_of_any_size(lib, size):
         near_norm(got[n], want[n], tol, n)
 
 
+@pytest.mark.parametrize("which,size", [("qk", 2.0 ** -70), ("v", 2.0 ** 126), ("q0", 2.0 ** 90)])
+def test_window_attention_at_the_ends_of_the_range(lib, which, size):
+    """Queries and keys so small that a score is below fp32's least value (every
+    visible key then counts the same), values near fp32's greatest, and a query
+    of zeros beside ones so large that no score of theirs fits fp32."""
+    dims = (1, 2, 1, 270, 270, 64)
+    q, k, v, dout = attention_inputs(13, *dims, False)
+    if which == "qk":
+        q, k = q * np.float32(size), k * np.float32(size)
+    elif which == "v":
+        v = np.clip(v, -1, 1) * np.float32(size)
+        dout *= np.float32(2.0 ** -100)
+    else:
+        q, k = q * np.float32(size), k * np.float32(size)
+        q[:, :, 77] = 0
+    want = R.window_attention(q, k, v, None, None, 100, 3, 0.125, False, dout)
+    got = run_attention(lib, q, k, v, dout, None, None, dims, 100, 3, 0.125, False)
+    if which == "q0":  # only the row of zeros has a value to compare
+        near_norm(got["out"][:, :, 77], want["out"][:, :, 77], 510 * U, "out")
+        return
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    # The terms of dS cancel where all probabilities are alike: their own size counts.
+    for n in ("dq", "dk", "dv"):
+        near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_window_attention_of_many_short_items(lib, dim):
+    """More work items than blocks, of one to three key tiles each: a block's
+    items follow one another through the pipeline."""
+    dims = (3, 40, 8, 384, 384, dim)
+    q, k, v, dout = attention_inputs(17, *dims, True)
+    lengths = np.array([384, 100, 257], np.float32)
+    starts = np.zeros(3, np.float32)
+    want = R.window_attention(q, k, v, starts, lengths, 60, 2, dim ** -0.5, True, dout)
+    for _ in range(3):
+        got = run_attention(lib, q, k, v, dout, starts, lengths, dims, 60, 2, dim ** -0.5, True)
+        compare_attention(got, want)
+
+
 def test_window_attention_gradients_against_differences(lib):
     """A few coordinates of each gradient against central differences of the
     64-bit forward: a step h leaves h^2 / 6 of the third derivative (about 1),
@@ -583,6 +623,8 @@ def test_distill_refusals(lib):
     lib.refused("width of 1", "distill_loss", z, e, e, out, s, 10, 0, 4, 1.0)
     for t in (0.0, -1.0, float("nan"), float("inf")):
         lib.refused("finite temperature", "distill_loss", z, e, e, out, s, 10, 40, 4, t)
+    for t in (2.0 ** -61, 2.0 ** 61):
+        lib.refused("from 2^-60 to 2^60", "distill_loss", z, e, e, out, s, 10, 40, 4, t)
     lib.refused("teacher buffer holds 10", "distill_loss", z, e, out, out, s, 10, 40, 4, 1.0)
     lib.refused("grad overlaps logits", "distill_loss_backward", z, e, e, s, None, z, 10, 40, 4, 1.0, False)
     lib.ok("distill_loss", z, e, e, out, None, 0, 40, 4, 1.0)

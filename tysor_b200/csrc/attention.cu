@@ -122,13 +122,14 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
     const float keep = m == top ? 1.0f : expf(m - top);
     const float p = x == top && x == -INFINITY ? 0.0f : expf(x - top);
     lane_load(v + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, kv);
-#pragma unroll
-    for (int i = 0; i < kLaneDims; ++i) acc[i] = acc[i] * keep + p * kv[i];
+    // acc stays a mean, so that values near fp32's greatest do not overflow.
     l = l * keep + p;
+    const float take = l == 0.0f ? p : p / l;
+#pragma unroll
+    for (int i = 0; i < kLaneDims; ++i) acc[i] = acc[i] * (1.0f - take) + take * kv[i];
     m = top;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, acc, inv, 0);
+  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, acc, 1.0f, 0);
   if (stats != nullptr && (threadIdx.x & 31) == 0)
     *(float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r)) = make_float2(m, l);
 }
@@ -233,19 +234,22 @@ __host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / 
 struct PackJob {
   const float* x;
   uint8_t* tiles;   // [batch][heads][tiles_of(len)] packed tiles
-  float* factors;   // the power of two that undoes each tile's scale; NaN: a value is not finite
+  float* factors;   // the power of two that undoes each tile's scale; NaN: not for the matrix unit (kFarExponent)
   int heads, len, queries;
   // For the gradients (all null otherwise), rows counted in whole tiles: the
-  // rows' 2-norms and each tile's greatest; and with the output and statistics
-  // (x is the output's gradient) each row's (greatest score in powers of two,
-  // 1 / sum, delta = sum of x * out, norm), zeros for rows that see nothing,
-  // and each tile's greatest |delta| (NaN if a row's values are not finite).
-  float *norm, *tile_norm;
+  // tile's greatest 2-norm of a row, and the rows' norms; or, with the output and
+  // statistics (x is the output's gradient), each row's (greatest score in powers
+  // of two, 1 / sum, delta = sum of x * out, norm), zeros for rows that see
+  // nothing, and each tile's greatest |delta| (NaN if a row's values are not finite).
+  float *tile_norm, *norm;
   const float *out, *stats;
   float4* info;
   float2* col;  // (greatest score + log2 of the sum - 14, delta); a row that sees nothing: a score no exponent reaches
   float* tile_delta;
 };
+// Tiles with values of 2^100 or more, or that are not finite, go key by key: sums
+// of such values times probabilities of up to 2^14 would leave fp32.
+constexpr int kFarExponent = 100;
 struct PackJobs {
   AttentionShape s;
   PackJob job[4];
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   const int up = top == 0 ? 0 : min(14 - exponent, 126);
   const float scale = __uint_as_float((uint32_t)(up + 127) << 23);
   if (threadIdx.x == 0)
-    j.factors[index] = exponent == 128 ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
+    j.factors[index] = exponent >= kFarExponent ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
   float most_norm = 0.0f;
   uint32_t most_delta = 0;  // as bits: NaN is the greatest
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   for (int i = 0; i < kPer; ++i) {
     const int item = threadIdx.x + 256 * i;
     const int r = item / kChunks, chunk = item % kChunks;
-    if (j.norm != nullptr) {
+    if (j.tile_norm != nullptr) {
       const float back = __uint_as_float((uint32_t)(127 - up) << 23);
       const int row = t * kTile + r;
       const float* o = j.out != nullptr ? j.out + row_at(s, b, h, row, j.heads, j.len) + chunk * 8 : nullptr;
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
       q = sqrtf(q) * back;
       most_norm = fmaxf(most_norm, q);
       if (chunk == 0) {
-        j.norm[(int64_t)index * kTile + r] = q;
+        if (j.norm != nullptr) j.norm[(int64_t)index * kTile + r] = q;
         if (j.info != nullptr) {
           float2 st = make_float2(0.0f, 0.0f);
           if (row >= r0 && row < r1) st = *(const float2*)(j.stats + 2 * (((int64_t)b * j.heads + h) * j.len + row));
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     *(uint4*)at = hi;
     *(uint4*)(at + (DP / 64) * kBox) = lo;
   }
-  if (j.norm == nullptr) return;
+  if (j.tile_norm == nullptr) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
@@ -570,6 +574,13 @@ __device__ __forceinline__ float2 natural_stats(float top, float sum) {
   return make_float2(m, sum * exp2f(top - m * kLog2e));
 }
 
+// What a score in a tile's units is multiplied by.  Kept normal: a hidden
+// score's -inf times 0, or a score of 0 times infinity, would be NaN, and past
+// either end no score differs from 0, or none but 0 from infinity, any more.
+__device__ __forceinline__ float unit_of(double f) {
+  return fminf(fmaxf((float)f, 1.17549435e-38f), 3.40282347e38f);
+}
+
 // The key tiles that a tile of query rows needs: [0, sinks) and then `low` on.
 struct TileRange {
   int sinks, low, count;
@@ -734,8 +745,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8, slot_full = q_empty + 8;
   const uint32_t slot_empty = slot_full + 8 * Plan::kSlots, s_full = slot_empty + 8 * Plan::kSlots;
   const uint32_t p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 16;
-  const uint32_t pair_full = o_empty + 16, q_ready = pair_full + 32, drained = q_ready + 8;
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 16);
+  const uint32_t pair_full = o_empty + 16, stats_full = pair_full + 32, q_ready = stats_full + 32, drained = q_ready + 8;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * Plan::kSlots + 20);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 8);
@@ -747,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, 8);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(pair_full + 8 * i, 2);
+    for (int i = 0; i < 4; ++i) mbar_init(pair_full + 8 * i, 2), mbar_init(stats_full + 8 * i, 8);
     mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -918,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       const double to_log2 = (double)a.fq[t.q_index] * (double)s.scale * 1.4426950408889634;
       for (int i = 0; i < t.n; ++i, ++gi) {
         const int buf = gi & 1, tile = t.range.at(i);
-        const float f = (float)(to_log2 * (double)a.fk[t.k_index + tile]);
+        const float f = unit_of(to_log2 * (double)a.fk[t.k_index + tile]);
         const bool whole = sees_all(s, t.rows, tile);
         ok = warp_wait(s_full + 8 * buf, (gi >> 1) & 1, err);
         if (!ok) break;
@@ -971,15 +982,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
           store_split16(at + buf * kTile + 32 * c, v + 32 * c);
           store_split16(at + buf * kTile + 32 * c + 16, v + 32 * c + 16);
         }
-        // Four buffers: these scores come after the values of two tiles before
-        // were issued, which waited until the output warps had taken the tile
-        // before that, and its statistics.
+        // Four buffers, each with its own barrier (stats_full): the scores of
+        // tile gi come after the values of gi - 2 were issued, which waited until
+        // the output warps had taken gi - 4, its statistics and phase with it.
         sum[((gi & 3) * 2 + half) * kTile + row] = (l[0] + l[1]) + (l[2] + l[3]);
         if (half == 0) ref[(gi & 3) * kTile + row] = m0 == -INFINITY ? -INFINITY : c0;
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 8 * buf);
+        if (lane == 0) mbar_arrive(p_full + 8 * buf), mbar_arrive(stats_full + 8 * (gi & 3));
       }
     }
   } else {
@@ -998,10 +1009,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
       float top = -INFINITY, l = 0.0f;
       for (int i = 0; i < t.n; ++i, ++gi) {
-        const int buf = gi & 1;
         const float fv = a.fv[t.k_index + t.range.at(i)];
         const uint32_t ob = gi % kOut;
-        ok = warp_wait(p_full + 8 * buf, (gi >> 1) & 1, err);
+        ok = warp_wait(stats_full + 8 * (gi & 3), (gi >> 2) & 1, err);
         if (!ok) break;
         const float c0 = ref[(gi & 3) * kTile + row];
         const float parts = sum[(gi & 3) * 2 * kTile + row] + sum[((gi & 3) * 2 + 1) * kTile + row];
@@ -1515,8 +1525,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       for (int n = t.f0; n < t.f1; ++n, ++gi) {
         int step;
         const int tile = column_tile(t, n, &step), c0 = step * kStep;
-        const float f = (float)(to_log2 * (double)(KEYS ? a.fq : a.fk)[tile]);
-        const float f2 = f_row * (KEYS ? a.fo : a.fv)[tile];
+        const float f = unit_of(to_log2 * (double)(KEYS ? a.fq : a.fk)[tile]);
+        const float f2 = unit_of((double)f_row * (double)(KEYS ? a.fo : a.fv)[tile]);
         const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
         const float up = power_of_two(scale_exponent(bound));
         bool whole;
@@ -2095,7 +2105,7 @@ void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, 
 
 struct GradWork {
   uint8_t *pq, *pk, *pv, *po;
-  float *fq, *fk, *fv, *fo, *nv, *no, *tnv, *tno, *tdo;
+  float *fq, *fk, *fv, *fo, *nv, *tnv, *tno, *tdo;
   float4* info;
   float2* col;
   float* part;
@@ -2137,7 +2147,6 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.fk = c.take(nk);
   w.fv = c.take(nk);
   w.nv = c.take(nk * kTile);
-  w.no = c.take(nq * kTile);
   w.tnv = c.take(nk);
   w.tno = c.take(nq);
   w.tdo = c.take(nq);
@@ -2230,9 +2239,9 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
   if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return;
   const GradWork w = grad_work(s, work);
   PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
-                     {dout, w.po, w.fo, s.heads, s.q_len, 1, w.no, w.tno, out, stats, w.info, w.col, w.tdo},
+                     {dout, w.po, w.fo, s.heads, s.q_len, 1, w.tno, nullptr, out, stats, w.info, w.col, w.tdo},
                      {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
-                     {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.nv, w.tnv}};
+                     {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.tnv, w.nv}};
   run_pack(s, jobs, 4, err, st);
   const GradArgs a{s,     q,     k,     v,      out,   stats, dout, w.pq, w.pk, w.pv,         w.po,         w.fq,         w.fk,
                    w.fv,  w.fo,  w.nv,  w.tnv,  w.tno, w.tdo, w.info, w.col, dq, dk,          dv,           accumulate_q, accumulate_k,
