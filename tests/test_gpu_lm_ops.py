@@ -282,6 +282,9 @@ CASES = [  # batch, heads, kv_heads, q_len, k_len, dim, window, sinks
     (2, 4, 2, 1, 50, 128, 0, 0), (3, 8, 2, 1, 700, 128, 64, 4), (1, 4, 4, 1, 1500, 64, 0, 0), (2, 6, 2, 5, 333, 72, 50, 2),
     (1, 16, 1, 2, 2100, 128, 0, 0), (1, 2, 1, 40, 900, 128, 300, 4), (1, 2, 1, 200, 130, 32, 0, 0),
     (1, 1, 1, 150, 1000, 65, 0, 0), (2, 20, 4, 3, 260, 33, 30, 1),
+    # Few query tiles over many keys: their key tiles are cut into segments.
+    (1, 5, 1, 5, 3000, 128, 0, 0), (2, 3, 1, 30, 4001, 64, 0, 0), (1, 2, 1, 1300, 1300, 40, 0, 0),
+    (1, 2, 2, 130, 2500, 72, 1500, 140), (1, 1, 1, 1100, 600, 128, 0, 0),
 ]
 
 
@@ -448,6 +451,26 @@ def test_window_attention_accumulates_and_repeats(lib):
         assert np.array_equal(a[n], b[n]), n  # the same bits every time
     for n in ("dq", "dk", "dv"):
         np.testing.assert_allclose(c[n], a[n] + 1.5, rtol=4 * U, atol=4 * U * 1.5)
+
+
+@pytest.mark.parametrize("dims,window,sinks", [((3, 2, 1, 150, 2200, 64), 0, 0), ((2, 4, 1, 5, 3000, 128), 1100, 20)])
+def test_window_attention_of_segments_that_are_empty_or_not_finite(lib, dims, window, sinks):
+    """Sequences too short to fill their segments, and rows that meet a NaN."""
+    batch, heads, kv_heads, q_len, k_len, dim = dims
+    q, k, v, dout = attention_inputs(23, *dims, False)
+    lengths = np.array([k_len, 700, 0], np.float32)[:batch]
+    starts = np.array([k_len - q_len, 690, -3], np.float32)[:batch]
+    want = R.window_attention(q, k, v, starts, lengths, window, sinks, 0.1, False, dout)
+    got = run_attention(lib, q, k, v, dout, starts, lengths, dims, window, sinks, 0.1, False)
+    compare_attention(got, want)
+    k[0, :, k_len - 3] = np.nan  # seen by the last queries of the first sequence
+    got = run_attention(lib, q, k, v, dout, starts, lengths, dims, window, sinks, 0.1, False)
+    seen = R.visible(starts, lengths, batch, q_len, k_len, window, sinks)[:, :, k_len - 3]
+    assert seen[0].sum() == 3
+    for n in ("out", "dq"):
+        assert np.isnan(got[n][0, :, seen[0]]).all()
+        near_norm(got[n][0, :, ~seen[0]], want[n][0, :, ~seen[0]], 3 * 510 * U, n)
+        near_norm(got[n][1:], want[n][1:], 3 * 510 * U, n)
 
 
 def test_window_attention_far_offsets(lib):

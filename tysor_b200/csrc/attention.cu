@@ -666,21 +666,27 @@ struct ForwardArgs {
   const uint8_t *pq, *pk, *pv;
   const float *fq, *fk, *fv;
   float *out, *stats;
+  int segs;         // segments of each item's key tiles
+  float* part;      // segs > 1: [item][segment][128][DP] sums of P.V, relative to 2^exponent
+  float2* part_ml;  // and [item][segment][128] (exponent, sum of P)
 };
 
 // Work item `index`: 128 rows of a head, those that see the most keys first.
 struct QueryItem {
   int b, h, g, r0, n;  // n: key tiles to walk; 0: none, or values that are not finite
+  int f0, f1;          // the unit's segment of them
+  bool first;          // the first segment
   Sequence sq;
   RowRange rows;
   TileRange range;
   int q_index, k_index;  // of the item's query tile and its head's first key tile
 };
 
-// Called by whole warps.
-__device__ __forceinline__ QueryItem query_item(const AttentionShape& s, int index, const float* fq, const float* fk,
-                                                const float* fv, int* err) {
+// Unit `unit`: segment unit % segs of item unit / segs.  Called by whole warps.
+__device__ __forceinline__ QueryItem query_item(const ForwardArgs& a, int unit, int* err) {
+  const AttentionShape& s = a.s;
   QueryItem t;
+  const int index = unit / a.segs, seg = unit - index * a.segs;
   const int tiles_q = tiles_of(s.q_len);
   const int tq = tiles_q - 1 - index / (s.heads * s.batch);
   t.h = index % s.heads;
@@ -692,12 +698,16 @@ __device__ __forceinline__ QueryItem query_item(const AttentionShape& s, int ind
   t.range = keys_for(s, t.sq, t.rows);
   t.q_index = (t.b * s.heads + t.h) * tiles_q + tq;
   t.k_index = (t.b * s.kv_heads + t.g) * tiles_of(s.k_len);
-  float sum = fq[t.q_index];
+  float sum = a.fq[t.q_index];
   for (int i = threadIdx.x & 31; i < t.range.count; i += 32)
-    sum += fk[t.k_index + t.range.at(i)] + fv[t.k_index + t.range.at(i)];
+    sum += a.fk[t.k_index + t.range.at(i)] + a.fv[t.k_index + t.range.at(i)];
   // A product with a hidden value that is not finite would not be 0: such
   // rows go key by key instead.
   t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  const int each = (t.n + a.segs - 1) / a.segs;
+  t.f0 = min(t.n, seg * each);
+  t.f1 = min(t.n, t.f0 + each);
+  t.first = seg == 0;
   return t;
 }
 
@@ -725,6 +735,33 @@ __device__ __forceinline__ RowMask mask_of(const AttentionShape& s, const QueryI
 }
 __device__ __forceinline__ uint32_t seen_bits(const RowMask& m, int first) {
   return bits_between(m.low, m.high, first) | bits_between(0, m.sinks, first);
+}
+
+// A thread's columns of a row, stored or added.
+template <int N>
+__device__ __forceinline__ void store_row(float* __restrict__ dst, const float (&v)[N], float by, int cols, bool vec,
+                                          int add) {
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4)
+      if (c < cols) {
+        float4 o = make_float4(v[c] * by, v[c + 1] * by, v[c + 2] * by, v[c + 3] * by);
+        if (add) {
+          const float4 p = *(const float4*)(dst + c);
+          o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+        }
+        *(float4*)(dst + c) = o;
+      }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+      if (c < cols) dst[c] = add ? dst[c] + v[c] * by : v[c] * by;
+  }
+}
+
+// A row's statistics where p was 2^(s - top), top 14 below the greatest score.
+__device__ __forceinline__ float2 tile_stats(float top, float l) {
+  return natural_stats(top == -INFINITY ? top : top + 14.0f, l * 0x1p-14f);
 }
 
 template <int DP>
@@ -780,8 +817,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     // No wait of the pipeline depends on these warps, however long they take.
     for (int round = 0, w; item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (t.n == 0)
+      const QueryItem t = query_item(a, w, err);
+      if (t.n == 0 && t.first)
         for (int r = t.r0 + warp - 18; r < min(t.r0 + kTile, s.q_len); r += 2)
           simple_forward_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, t.b, t.h, r);
     }
@@ -810,17 +847,17 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (lane == 0 && t.n > 0) {
+      const QueryItem t = query_item(a, w, err);
+      if (lane == 0 && t.f0 < t.f1) {
         if (loaded > 0) ok = mbar_wait(q_empty, (loaded - 1) & 1, err);
         if (ok) {
           mbar_expect_tx(q_full, kTileBytes<DP>);
           bulk_load(q_smem, a.pq + (int64_t)t.q_index * kTileBytes<DP>, kTileBytes<DP>, q_full);
           ++loaded;
         }
-        for (int i = 0; i <= t.n && ok; ++i) {  // a tile's keys, then the values of the one before
-          if (i < t.n) fill(a.pk + (int64_t)(t.k_index + t.range.at(i)) * kTileBytes<DP>, false);
-          if (ok && i > 0) fill(a.pv + (int64_t)(t.k_index + t.range.at(i - 1)) * kTileBytes<DP>, true);
+        for (int i = t.f0; i <= t.f1 && ok; ++i) {  // a tile's keys, then the values of the one before
+          if (i < t.f1) fill(a.pk + (int64_t)(t.k_index + t.range.at(i)) * kTileBytes<DP>, false);
+          if (ok && i > t.f0) fill(a.pv + (int64_t)(t.k_index + t.range.at(i - 1)) * kTileBytes<DP>, true);
         }
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -866,10 +903,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     };
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      const int n = __shfl_sync(0xffffffffu, t.n, 0), sinks = __shfl_sync(0xffffffffu, t.range.sinks, 0);
+      const QueryItem t = query_item(a, w, err);
+      const int n = __shfl_sync(0xffffffffu, t.f1 - t.f0, 0);
+      const int sinks = __shfl_sync(0xffffffffu, t.range.sinks - t.f0, 0);
       const int sink_width = __shfl_sync(0xffffffffu, t.range.width, 0);
-      if (n == 0) continue;
+      if (n <= 0) continue;
       ok = warp_wait(q_ready, item & 1, err);
       ++item;
       for (int i = 0; i <= n && ok; ++i) {
@@ -914,8 +952,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (t.n == 0) continue;
+      const QueryItem t = query_item(a, w, err);
+      if (t.f0 >= t.f1) continue;
       // The products with the query tile before are done: their scores have been read.
       ok = warp_wait(q_full, item & 1, err);
       if (!ok) break;
@@ -927,7 +965,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
       ++item;
       const RowMask mask = mask_of(s, t, row);
       const double to_log2 = (double)a.fq[t.q_index] * (double)s.scale * 1.4426950408889634;
-      for (int i = 0; i < t.n; ++i, ++gi) {
+      for (int i = t.f0; i < t.f1; ++i, ++gi) {
         const int buf = gi & 1, tile = t.range.at(i);
         const float f = unit_of(to_log2 * (double)a.fk[t.k_index + tile]);
         const bool whole = sees_all(s, t.rows, tile);
@@ -1002,13 +1040,13 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     bool ok = true;
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
-      const QueryItem t = query_item(s, w, a.fq, a.fk, a.fv, err);
-      if (t.n == 0) continue;
+      const QueryItem t = query_item(a, w, err);
+      if (t.f0 >= t.f1) continue;
       float acc[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
       float top = -INFINITY, l = 0.0f;
-      for (int i = 0; i < t.n; ++i, ++gi) {
+      for (int i = t.f0; i < t.f1; ++i, ++gi) {
         const float fv = a.fv[t.k_index + t.range.at(i)];
         const uint32_t ob = gi % kOut;
         ok = warp_wait(stats_full + 8 * (gi & 3), (gi >> 2) & 1, err);
@@ -1038,26 +1076,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
         }
       }
       const int r = t.r0 + row;
-      if (ok && r < s.q_len) {
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      float* dst = a.out + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols;
-      const int cols = s.head_dim - half * kCols;
-      if (s.head_dim % 4 == 0 && ((uintptr_t)a.out & 15) == 0) {
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4)
-          if (c < cols)
-            *(float4*)(dst + c) =
-                make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
-      } else {
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-          if (c < cols) dst[c] = acc[c] * inv;
-      }
-      if (a.stats != nullptr && half == 0) {
-        // p was 2^(s - top) with top 14 below the greatest score.
-        const float2 st = natural_stats(top == -INFINITY ? top : top + 14.0f, l * 0x1p-14f);
-        *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = st;
-      }
+      if (ok && a.segs > 1) {
+        const int64_t at_part = (int64_t)w * kTile + row;
+        store_row(a.part + at_part * DP + half * kCols, acc, 1.0f, kCols, true, 0);
+        if (half == 0) a.part_ml[at_part] = make_float2(top, l);
+      } else if (ok && r < s.q_len) {
+        store_row(a.out + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols, acc, l > 0.0f ? 1.0f / l : 0.0f,
+                  s.head_dim - half * kCols, s.head_dim % 4 == 0 && ((uintptr_t)a.out & 15) == 0, 0);
+        if (a.stats != nullptr && half == 0)
+          *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = tile_stats(top, l);
       }
       __syncwarp();
     }
@@ -1068,6 +1095,41 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   if (warp == 17) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// Joins an item's segments in order, a few rows per block.
+constexpr int kJoinRows = 8;
+template <int DP>
+__global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a, int* err) {
+  const AttentionShape& s = a.s;
+  const int item = blockIdx.x / (kTile / kJoinRows), row0 = blockIdx.x % (kTile / kJoinRows) * kJoinRows;
+  const QueryItem t = query_item(a, item * a.segs, err);
+  if (t.n == 0) return;  // written key by key
+  const int used = (t.n + t.f1 - 1) / t.f1;  // of f1 tiles each
+  for (int i = threadIdx.x; i < kJoinRows * DP / 4; i += 256) {
+    const int row = row0 + i / (DP / 4), c = i % (DP / 4) * 4, r = t.r0 + row;
+    if (r >= s.q_len || c >= s.head_dim) continue;
+    const int64_t first = (int64_t)item * a.segs * kTile + row;
+    float top = -INFINITY, l = 0.0f, v[4] = {};
+#pragma unroll 4
+    for (int k = 0; k < used; ++k) {
+      const float2 ml = a.part_ml[first + (int64_t)k * kTile];
+      const float4 p = *(const float4*)(a.part + (first + (int64_t)k * kTile) * DP + c);
+      const float next = fmaxf(top, ml.x);
+      const float keep = top == next ? 1.0f : exp2_fast(top - next);
+      const float take = ml.x == next ? 1.0f : exp2_fast(ml.x - next);
+      l = l * keep + ml.y * take;
+      v[0] = v[0] * keep + p.x * take;
+      v[1] = v[1] * keep + p.y * take;
+      v[2] = v[2] * keep + p.z * take;
+      v[3] = v[3] * keep + p.w * take;
+      top = next;
+    }
+    store_row(a.out + row_at(s, t.b, t.h, r, s.heads, s.q_len) + c, v, l > 0.0f ? 1.0f / l : 0.0f, s.head_dim - c,
+              s.head_dim % 4 == 0 && ((uintptr_t)a.out & 15) == 0, 0);
+    if (a.stats != nullptr && c == 0)
+      *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = tile_stats(top, l);
   }
 }
 
@@ -1234,28 +1296,6 @@ __device__ __forceinline__ int scale_exponent(float bound) {
   return bound == 0.0f ? 0 : min(max(14 - e, -126), 126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
-// A thread's columns of a gradient row, stored or added.
-template <int N>
-__device__ __forceinline__ void store_row(float* __restrict__ dst, const float (&v)[N], float by, int cols, bool vec,
-                                          int add) {
-  if (vec) {
-#pragma unroll
-    for (int c = 0; c < N; c += 4)
-      if (c < cols) {
-        float4 o = make_float4(v[c] * by, v[c + 1] * by, v[c + 2] * by, v[c + 3] * by);
-        if (add) {
-          const float4 p = *(const float4*)(dst + c);
-          o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
-        }
-        *(float4*)(dst + c) = o;
-      }
-  } else {
-#pragma unroll
-    for (int c = 0; c < N; ++c)
-      if (c < cols) dst[c] = add ? dst[c] + v[c] * by : v[c] * by;
-  }
-}
 
 template <int DP, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items, int* err) {
@@ -2014,9 +2054,26 @@ int padded_dim(const AttentionShape& s) { return s.head_dim <= 64 ? 64 : 128; }
 
 struct ForwardWork {
   uint8_t *pq, *pk, *pv;
-  float *fq, *fk, *fv;
+  float *fq, *fk, *fv, *part;
+  float2* part_ml;
+  int segs;
   int64_t floats;
 };
+// Segments of a query tile's key tiles, of at least four tiles each: one unit
+// per SM where the items are about alike (a window, or few queries over a long
+// cache), two where the first queries see few keys and the last ones all.
+// Measured, 128 wide, whole / one per SM / two: 5 queries of 5 heads over 65536
+// keys of one 1074 / 98 / 116 us, 128 queries of 8 heads over as many 1179 / 279
+// / 299; 8192 over themselves, one head, 148 / 96 / 73, 4096 of four 88 / 88 / 74.
+int segments_of_queries(const AttentionShape& s) {
+  const int64_t items = (int64_t)s.batch * s.heads * tiles_of(s.q_len);
+  int64_t most = tiles_of(s.k_len);
+  if (s.window > 0)
+    most = std::min<int64_t>(most, ((int64_t)s.window + kTile - 2) / kTile + 1 + tiles_of(std::min(s.sinks, s.k_len)));
+  if (items == 0) return 1;
+  const int per_sm = s.window > 0 || s.q_len <= s.k_len / 2 ? 1 : 2;
+  return (int)std::max<int64_t>(1, std::min(most / 4, kSms * per_sm / items));
+}
 ForwardWork forward_work(const AttentionShape& s, float* base) {
   Carver c{base};
   const int64_t tile = padded_dim(s) == 64 ? kTileBytes<64> / 4 : kTileBytes<128> / 4;
@@ -2028,6 +2085,9 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   w.fq = c.take(nq);
   w.fk = c.take(nk);
   w.fv = c.take(nk);
+  w.segs = segments_of_queries(s);
+  w.part = c.take(w.segs > 1 ? nq * w.segs * kTile * padded_dim(s) : 0);
+  w.part_ml = (float2*)c.take(w.segs > 1 ? nq * w.segs * kTile * 2 : 0);
   w.floats = c.used;
   return w;
 }
@@ -2189,8 +2249,12 @@ void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   allow_shared(forward_kernel<DP>, ForwardPlan<DP>::kSmem, done);
   const int64_t items = (int64_t)tiles_of(a.s.q_len) * a.s.heads * a.s.batch;  // at most what run_pack took
-  forward_kernel<DP><<<(unsigned)(items < kSms ? items : kSms), kThreads, ForwardPlan<DP>::kSmem, st>>>(
-      a, (int)items, err);
+  const int64_t units = items * a.segs;  // segs > 1: at most two per SM
+  forward_kernel<DP><<<(unsigned)(units < kSms ? units : kSms), kThreads, ForwardPlan<DP>::kSmem, st>>>(
+      a, (int)units, err);
+  check_launch();
+  if (a.segs == 1) return;
+  forward_join_kernel<DP><<<(unsigned)(items * (kTile / kJoinRows)), 256, 0, st>>>(a, err);
   check_launch();
 }
 
@@ -2213,7 +2277,7 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
                        {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0}};
     run_pack(s, jobs, 3, err, st);
-    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats};
+    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats, w.segs, w.part, w.part_ml};
     if (padded_dim(s) == 64) run_forward<64>(a, err, st);
     else run_forward<128>(a, err, st);
     return;
