@@ -284,7 +284,7 @@ CASES = [  # batch, heads, kv_heads, q_len, k_len, dim, window, sinks
     (1, 1, 1, 150, 1000, 65, 0, 0), (2, 20, 4, 3, 260, 33, 30, 1),
     # Few query tiles over many keys: their key tiles are cut into segments.
     (1, 5, 1, 5, 3000, 128, 0, 0), (2, 3, 1, 30, 4001, 64, 0, 0), (1, 2, 1, 1300, 1300, 40, 0, 0),
-    (1, 2, 2, 130, 2500, 72, 1500, 140), (1, 1, 1, 1100, 600, 128, 0, 0),
+    (1, 2, 2, 130, 2500, 72, 1500, 140), (1, 1, 1, 1100, 600, 128, 0, 0), (1, 8, 2, 600, 600, 33, 70, 5),
 ]
 
 

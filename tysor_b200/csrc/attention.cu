@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   if (threadIdx.x == 0)
     j.factors[index] = exponent >= kFarExponent ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
+  const bool out_vec = s.head_dim % 4 == 0 && ((uintptr_t)j.out & 15) == 0;
   float most_norm = 0.0f;
   uint32_t most_delta = 0;  // as bits: NaN is the greatest
 #pragma unroll
@@ -330,12 +331,23 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     if (j.tile_norm != nullptr) {
       const float back = __uint_as_float((uint32_t)(127 - up) << 23);
       const int row = t * kTile + r;
-      const float* o = j.out != nullptr ? j.out + row_at(s, b, h, row, j.heads, j.len) + chunk * 8 : nullptr;
       float q = 0.0f, d = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        q += v[i][e] * scale * (v[i][e] * scale);
-        if (o != nullptr && row >= r0 && row < r1 && chunk * 8 + e < s.head_dim) d += v[i][e] * o[e];
+      for (int e = 0; e < 8; ++e) q += v[i][e] * scale * (v[i][e] * scale);
+      if (j.out != nullptr && row >= r0 && row < r1) {
+        const float* o = j.out + row_at(s, b, h, row, j.heads, j.len) + chunk * 8;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          if (chunk * 8 + e >= s.head_dim) continue;
+          if (out_vec) {
+            const float4 f = __ldg((const float4*)(o + e));
+            d += v[i][e] * f.x, d += v[i][e + 1] * f.y, d += v[i][e + 2] * f.z, d += v[i][e + 3] * f.w;
+          } else {
+#pragma unroll
+            for (int k = e; k < e + 4; ++k)
+              if (chunk * 8 + k < s.head_dim) d += v[i][k] * __ldg(o + k);
+          }
+        }
       }
 #pragma unroll
       for (int w = kChunks / 2; w > 0; w >>= 1) {
@@ -1179,9 +1191,10 @@ constexpr int kStepBox = kStep * 128;  // bytes of 64 rows of a box
 
 // How the key tiles' steps are cut: the first `long_tiles` of each head into
 // long_segs segments, the others into short_segs.  A unit is a segment of a
-// tile of a head, counted tile by tile.
+// tile of a head, counted tile by tile.  The query tiles' steps are cut into
+// query_segs, a tile's segments counted one after the other.
 struct Segments {
-  int long_tiles, long_segs, short_segs;
+  int long_tiles, long_segs, short_segs, query_segs;
 };
 
 struct GradArgs {
@@ -1195,7 +1208,7 @@ struct GradArgs {
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
   Segments seg;
-  float* part;                         // [unit][dk, dv][128][DP]
+  float* part;                         // queries: [unit][128][DP]; keys: [unit][dk, dv][128][DP]
 };
 
 template <int DP, bool KEYS>
@@ -1232,6 +1245,9 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
   float sum;
   int seg = 0;
   if (!KEYS) {
+    t.segs = a.seg.query_segs;
+    seg = index % t.segs;
+    index /= t.segs;
     const int tq = tiles_q - 1 - index / (s.heads * s.batch);
     t.h = index % s.heads;
     t.b = index / s.heads % s.batch;
@@ -1245,7 +1261,6 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     t.range.low = low / kStep;
     t.range.sinks = min((min(s.sinks, low) + kStep - 1) / kStep, t.range.low);
     t.range.count = x > z ? 0 : t.range.sinks + z / kStep - t.range.low + 1;
-    t.segs = 1;
     sum = a.fq[t.row_tile] + a.fo[t.row_tile];
     const int first = (t.b * s.kv_heads + t.g) * tiles_k;
     for (int i = lane; i < t.range.count; i += 32) {
@@ -1688,9 +1703,9 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       }
       const int r = t.r0 + row, cols = s.head_dim - half * kCols;
       if (ok && t.segs > 1) {
-        float* dst = a.part + ((int64_t)w * 2 * kTile + row) * DP + half * kCols;
+        float* dst = a.part + ((int64_t)w * (KEYS ? 2 : 1) * kTile + row) * DP + half * kCols;
         store_row(dst, acc, s.scale, kCols, true, 0);
-        store_row(dst + kTile * DP, acc_v, 1.0f, kCols, true, 0);
+        if (KEYS) store_row(dst + kTile * DP, acc_v, 1.0f, kCols, true, 0);
       } else if (ok && KEYS && r < s.k_len) {
         const int64_t at = row_at(s, t.b, t.g, r, s.kv_heads, s.k_len) + half * kCols;
         store_row(a.dk + at, acc, s.scale, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dk & 15) == 0, a.add_k);
@@ -1711,29 +1726,34 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   }
 }
 
-// Adds the segments of one key tile in order, `rows` rows per block: few for a
+// Adds the segments of one tile in order, `rows` rows per block: few for a
 // sink tile, whose many segments few blocks would read one after the other.
-template <int DP>
+template <int DP, bool KEYS>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int rows, int* err) {
+  constexpr int kGrads = KEYS ? 2 : 1;
   const AttentionShape& s = a.s;
   const int tile = blockIdx.x / (kTile / rows), row0 = blockIdx.x % (kTile / rows) * rows;
   // The tile's first segment; the next ones follow `stride` units apart.
   const int unit = first + tile / stride * segs * stride + tile % stride;
-  const GradItem t = grad_item<true>(a, unit, err);
+  const GradItem t = grad_item<KEYS>(a, unit, err);
   if (t.n == 0) return;  // written key by key
-  const int total = s.heads / s.kv_heads * t.n, each = (total + segs - 1) / segs, used = (total + each - 1) / each;
-  for (int i = threadIdx.x; i < 2 * rows * DP / 4; i += 256) {
+  const int total = (KEYS ? s.heads / s.kv_heads : 1) * t.n, each = (total + segs - 1) / segs;
+  const int used = (total + each - 1) / each;
+  for (int i = threadIdx.x; i < kGrads * rows * DP / 4; i += 256) {
     const int which = i / (rows * DP / 4), r = row0 + i / (DP / 4) % rows, c = i % (DP / 4) * 4;
-    if (t.r0 + r >= s.k_len || c >= s.head_dim) continue;
+    if (t.r0 + r >= (KEYS ? s.k_len : s.q_len) || c >= s.head_dim) continue;
     float v[4] = {};
 #pragma unroll 8
     for (int k = 0; k < used; ++k) {
-      const float4 p = *(const float4*)(a.part + (((int64_t)(unit + k * stride) * 2 + which) * kTile + r) * DP + c);
+      const float4 p =
+          *(const float4*)(a.part + (((int64_t)(unit + k * stride) * kGrads + which) * kTile + r) * DP + c);
       v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
     }
-    float* grad = which ? a.dv : a.dk;
-    store_row(grad + row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len) + c, v, 1.0f, s.head_dim - c,
-              s.head_dim % 4 == 0 && ((uintptr_t)grad & 15) == 0, which ? a.add_v : a.add_k);
+    float* grad = !KEYS ? a.dq : which ? a.dv : a.dk;
+    const int64_t at = KEYS ? row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len)
+                            : row_at(s, t.b, t.h, t.r0 + r, s.heads, s.q_len);
+    store_row(grad + at + c, v, 1.0f, s.head_dim - c, s.head_dim % 4 == 0 && ((uintptr_t)grad & 15) == 0,
+              !KEYS ? a.add_q : which ? a.add_v : a.add_k);
   }
 }
 
@@ -2059,20 +2079,23 @@ struct ForwardWork {
   int segs;
   int64_t floats;
 };
-// Segments of a query tile's key tiles, of at least four tiles each: one unit
+// Segments of a query tile's key tiles, of at least `least` tiles each: one unit
 // per SM where the items are about alike (a window, or few queries over a long
 // cache), two where the first queries see few keys and the last ones all.
 // Measured, 128 wide, whole / one per SM / two: 5 queries of 5 heads over 65536
 // keys of one 1074 / 98 / 116 us, 128 queries of 8 heads over as many 1179 / 279
 // / 299; 8192 over themselves, one head, 148 / 96 / 73, 4096 of four 88 / 88 / 74.
-int segments_of_queries(const AttentionShape& s) {
+// At least four: 4000 keys, 5 queries of 20 heads, 40 us (two 51, eight 44); of
+// the gradients' pass two, as a tile is two steps: 2000 tokens, window 512, two
+// heads, forward and backward 112 us (four 116, one 128).
+int segments_of_queries(const AttentionShape& s, int least) {
   const int64_t items = (int64_t)s.batch * s.heads * tiles_of(s.q_len);
   int64_t most = tiles_of(s.k_len);
   if (s.window > 0)
     most = std::min<int64_t>(most, ((int64_t)s.window + kTile - 2) / kTile + 1 + tiles_of(std::min(s.sinks, s.k_len)));
   if (items == 0) return 1;
   const int per_sm = s.window > 0 || s.q_len <= s.k_len / 2 ? 1 : 2;
-  return (int)std::max<int64_t>(1, std::min(most / 4, kSms * per_sm / items));
+  return (int)std::max<int64_t>(1, std::min(most / least, kSms * per_sm / items));
 }
 ForwardWork forward_work(const AttentionShape& s, float* base) {
   Carver c{base};
@@ -2085,7 +2108,7 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   w.fq = c.take(nq);
   w.fk = c.take(nk);
   w.fv = c.take(nk);
-  w.segs = segments_of_queries(s);
+  w.segs = segments_of_queries(s, 4);
   w.part = c.take(w.segs > 1 ? nq * w.segs * kTile * padded_dim(s) : 0);
   w.part_ml = (float2*)c.take(w.segs > 1 ? nq * w.segs * kTile * 2 : 0);
   w.floats = c.used;
@@ -2172,9 +2195,12 @@ struct GradWork {
   int64_t floats;
 };
 
-// Segments of a key tile's steps, about sixteen steps each where that makes
-// eight units per SM (below that a unit's start and end cost more than the
-// uneven blocks do).
+// Segments of a key tile's steps, about sixteen steps each where that makes at
+// most eight units per SM (below that a unit's start and end cost more than the
+// uneven blocks do); fewer, down to four, where sixteen would leave SMs idle.
+// Measured, forward and backward, 128 wide, four / always sixteen: 600 tokens of
+// 8 heads over 2 109 / 138 us, 128 queries of 2 heads over 4096 keys of one 97 /
+// 191; two units per SM instead of one: 1024 tokens of 16 heads over 4 254 / 221.
 Segments segments_of(const AttentionShape& s) {
   const int64_t group = s.heads / s.kv_heads, all = ceil_div(s.q_len, kStep);
   const int64_t some = s.window > 0 ? std::min<int64_t>(all, ((int64_t)s.window + kTile + 2 * kStep - 3) / kStep) : all;
@@ -2183,9 +2209,11 @@ Segments segments_of(const AttentionShape& s) {
   g.long_tiles = s.window > 0 ? std::min(tiles, tiles_of(std::min(s.sinks, s.k_len))) : tiles;
   // Without a window a tile's steps are half of all on average.
   const int64_t steps = (s.window > 0 ? g.long_tiles * all : tiles * all / 2) + (tiles - g.long_tiles) * some;
-  const int64_t each = std::max<int64_t>(16, steps * group * s.batch * s.kv_heads / (kSms * 8));
+  const int64_t work = steps * group * s.batch * s.kv_heads;
+  const int64_t each = std::max(std::min<int64_t>(16, std::max<int64_t>(4, work / kSms)), work / (kSms * 8));
   g.long_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * all / each));
   g.short_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * some / each));
+  g.query_segs = segments_of_queries(s, 2);
   return g;
 }
 int64_t grad_units(const AttentionShape& s, const Segments& g) {
@@ -2213,7 +2241,10 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.info = (float4*)c.take(nq * kTile * 4);
   w.col = (float2*)c.take(nq * kTile * 2);
   const Segments g = segments_of(s);
-  w.part = c.take(g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 * kTile * padded_dim(s) : 0);
+  // The queries' pass has joined its segments when the keys' begins.
+  const int64_t for_keys = g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 : 0;
+  const int64_t for_queries = g.query_segs > 1 ? nq * g.query_segs : 0;
+  w.part = c.take(std::max(for_keys, for_queries) * kTile * padded_dim(s));
   w.floats = c.used;
   return w;
 }
@@ -2224,21 +2255,27 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   allow_shared(grad_kernel<DP, KEYS>, kSmem, done);
   const AttentionShape& s = a.s;
-  const int64_t items = KEYS ? grad_units(s, a.seg) : (int64_t)tiles_of(s.q_len) * s.heads * s.batch;
+  const int64_t items = KEYS ? grad_units(s, a.seg) : (int64_t)tiles_of(s.q_len) * s.heads * s.batch * a.seg.query_segs;
   if (items == 0) return;
   if (items > INT_MAX / 64) throw CudaError("window_attention: too many rows");
   grad_kernel<DP, KEYS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
-  if (!KEYS) return;
+  if (!KEYS) {
+    if (a.seg.query_segs == 1) return;
+    const int64_t blocks = items / a.seg.query_segs * (kTile / 8);  // query_segs > 1: few items
+    grad_join_kernel<DP, false><<<(unsigned)blocks, 256, 0, st>>>(a, 0, a.seg.query_segs, 1, 8, err);
+    check_launch();
+    return;
+  }
   const int tiles = tiles_of(s.k_len), stride = s.kv_heads * s.batch;
   if (a.seg.long_segs > 1 && a.seg.long_tiles > 0) {
     const int rows = s.window > 0 ? 2 : 8;
-    grad_join_kernel<DP><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
+    grad_join_kernel<DP, true><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
         a, 0, a.seg.long_segs, stride, rows, err);
     check_launch();
   }
   if (a.seg.short_segs > 1 && tiles > a.seg.long_tiles) {
-    grad_join_kernel<DP><<<(unsigned)((tiles - a.seg.long_tiles) * stride * (kTile / 8)), 256, 0, st>>>(
+    grad_join_kernel<DP, true><<<(unsigned)((tiles - a.seg.long_tiles) * stride * (kTile / 8)), 256, 0, st>>>(
         a, a.seg.long_tiles * a.seg.long_segs * stride, a.seg.short_segs, stride, 8, err);
     check_launch();
   }
