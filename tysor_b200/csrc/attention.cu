@@ -287,14 +287,23 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     if (j.norm != nullptr && threadIdx.x < kTile) j.norm[(int64_t)index * kTile + threadIdx.x] = 0.0f;
     return;
   }
-  const bool vec = s.head_dim % 4 == 0 && ((uintptr_t)j.x & 15) == 0;
-  float v[kPer][8];
+  const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)j.x | (uintptr_t)j.out) & 15) == 0;
+  // All of a thread's loads come first, so that their latencies overlap.
+  __shared__ float2 row_stats[kTile];
+  if (j.out != nullptr && threadIdx.x < kTile) {
+    const int row = t * kTile + threadIdx.x;
+    row_stats[threadIdx.x] = row >= r0 && row < r1
+                                 ? *(const float2*)(j.stats + 2 * (((int64_t)b * j.heads + h) * j.len + row))
+                                 : make_float2(0.0f, 0.0f);
+  }
+  float v[kPer][8], dot[kPer];  // dot: of the piece with the output's
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int item = threadIdx.x + 256 * i;
     const int r = t * kTile + item / kChunks, c = item % kChunks * 8;
-    const float* src = j.x + row_at(s, b, h, r, j.heads, j.len) + c;
+    const int64_t from = row_at(s, b, h, r, j.heads, j.len) + c;
+    const float* src = j.x + from;
     const bool live = r >= r0 && r < r1;
     if (vec) {
 #pragma unroll
@@ -305,6 +314,23 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = live && c + e < s.head_dim ? src[e] : 0.0f;
+    }
+    dot[i] = 0.0f;
+    if (j.out != nullptr) {
+      const float* o = j.out + from;
+      if (vec) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          if (live && c + e < s.head_dim) {
+            const float4 f = *(const float4*)(o + e);
+            dot[i] += v[i][e] * f.x, dot[i] += v[i][e + 1] * f.y;
+            dot[i] += v[i][e + 2] * f.z, dot[i] += v[i][e + 3] * f.w;
+          }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (live && c + e < s.head_dim) dot[i] += v[i][e] * o[e];
+      }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
@@ -321,7 +347,6 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   if (threadIdx.x == 0)
     j.factors[index] = exponent >= kFarExponent ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
-  const bool out_vec = s.head_dim % 4 == 0 && ((uintptr_t)j.out & 15) == 0;
   float most_norm = 0.0f;
   uint32_t most_delta = 0;  // as bits: NaN is the greatest
 #pragma unroll
@@ -330,25 +355,9 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     const int r = item / kChunks, chunk = item % kChunks;
     if (j.tile_norm != nullptr) {
       const float back = __uint_as_float((uint32_t)(127 - up) << 23);
-      const int row = t * kTile + r;
-      float q = 0.0f, d = 0.0f;
+      float q = 0.0f, d = dot[i];
 #pragma unroll
       for (int e = 0; e < 8; ++e) q += v[i][e] * scale * (v[i][e] * scale);
-      if (j.out != nullptr && row >= r0 && row < r1) {
-        const float* o = j.out + row_at(s, b, h, row, j.heads, j.len) + chunk * 8;
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          if (chunk * 8 + e >= s.head_dim) continue;
-          if (out_vec) {
-            const float4 f = __ldg((const float4*)(o + e));
-            d += v[i][e] * f.x, d += v[i][e + 1] * f.y, d += v[i][e + 2] * f.z, d += v[i][e + 3] * f.w;
-          } else {
-#pragma unroll
-            for (int k = e; k < e + 4; ++k)
-              if (chunk * 8 + k < s.head_dim) d += v[i][k] * __ldg(o + k);
-          }
-        }
-      }
 #pragma unroll
       for (int w = kChunks / 2; w > 0; w >>= 1) {
         q += __shfl_xor_sync(0xffffffffu, q, w);
@@ -359,8 +368,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
       if (chunk == 0) {
         if (j.norm != nullptr) j.norm[(int64_t)index * kTile + r] = q;
         if (j.info != nullptr) {
-          float2 st = make_float2(0.0f, 0.0f);
-          if (row >= r0 && row < r1) st = *(const float2*)(j.stats + 2 * (((int64_t)b * j.heads + h) * j.len + row));
+          const float2 st = row_stats[r];
           const float4 f =
               st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(st.x * kLog2e, 1.0f / st.y, d, q);
           j.info[(int64_t)index * kTile + r] = f;
@@ -2195,12 +2203,14 @@ struct GradWork {
   int64_t floats;
 };
 
-// Segments of a key tile's steps, about sixteen steps each where that makes at
-// most eight units per SM (below that a unit's start and end cost more than the
-// uneven blocks do); fewer, down to four, where sixteen would leave SMs idle.
-// Measured, forward and backward, 128 wide, four / always sixteen: 600 tokens of
-// 8 heads over 2 109 / 138 us, 128 queries of 2 heads over 4096 keys of one 97 /
-// 191; two units per SM instead of one: 1024 tokens of 16 heads over 4 254 / 221.
+// Segments of a key tile's steps: sixteen steps each, more where that would make
+// over three units per SM (each unit's part is written and read once more), and
+// fewer, down to four, where it would leave SMs idle.  Measured, forward and
+// backward, 128 wide: eight units per SM instead of three, 2048 tokens of 8
+// sequences, 16 heads over 4, 2323 / 2023 us, the same of 4096 tokens and 2
+// sequences with a window of 512 852 / 803 (two 799, four 765); always sixteen
+// steps instead of four, 600 tokens of 8 heads over 2 138 / 109, 128 queries of 2
+// heads over 4096 keys of one 191 / 97.
 Segments segments_of(const AttentionShape& s) {
   const int64_t group = s.heads / s.kv_heads, all = ceil_div(s.q_len, kStep);
   const int64_t some = s.window > 0 ? std::min<int64_t>(all, ((int64_t)s.window + kTile + 2 * kStep - 3) / kStep) : all;
@@ -2210,7 +2220,7 @@ Segments segments_of(const AttentionShape& s) {
   // Without a window a tile's steps are half of all on average.
   const int64_t steps = (s.window > 0 ? g.long_tiles * all : tiles * all / 2) + (tiles - g.long_tiles) * some;
   const int64_t work = steps * group * s.batch * s.kv_heads;
-  const int64_t each = std::max(std::min<int64_t>(16, std::max<int64_t>(4, work / kSms)), work / (kSms * 8));
+  const int64_t each = std::max(std::min<int64_t>(16, std::max<int64_t>(4, work / kSms)), work / (kSms * 3));
   g.long_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * all / each));
   g.short_segs = (int)std::min<int64_t>(64, std::max<int64_t>(1, group * some / each));
   g.query_segs = segments_of_queries(s, 2);
