@@ -601,6 +601,25 @@ def test_distill_loss_of_absent_and_repeated_entries(lib):
     compare_distill(got, want, 2.0)
 
 
+@pytest.mark.parametrize("width", [1, 20, 700, 40000])
+def test_distill_loss_of_many_entries(lib, width):
+    """The most entries a row may have, ids in any order and many times."""
+    rng = np.random.default_rng(width)
+    z = (2 * rng.standard_normal((3, width))).astype(np.float32)
+    ids = rng.integers(-1, width, (3, 1024)).astype(np.float32)
+    ids[2] = rng.integers(0, min(width, 3), 1024)
+    teacher = (3 * rng.standard_normal((3, 1024))).astype(np.float32)
+    dloss = rng.standard_normal(3).astype(np.float32)
+    want = R.distill_loss(z, ids, teacher, 2.0, dloss)
+    got = run_distill(lib, z, ids, teacher, dloss, 2.0)
+    near(got["loss"], want["loss"], 240 * U * 4, "loss", 1.0)
+    # q and the entries' p cancel: both are at most 1, p sums up to 1024 terms of
+    # them (at most 1024u / 2 off, in order), times T dloss.
+    near(got["grad"], want["grad"], (240 + 512) * U, "grad", float(2 * np.abs(dloss).max()))
+    again = run_distill(lib, z, ids, teacher, dloss, 2.0)
+    assert np.array_equal(got["grad"], again["grad"])
+
+
 def test_distill_loss_of_entries_that_are_no_numbers(lib):
     """A teacher's NaN makes its own row's loss NaN, absent entries beside it
     notwithstanding, and no other row's."""
@@ -651,6 +670,73 @@ def test_distill_refusals(lib):
     lib.refused("teacher buffer holds 10", "distill_loss", z, e, out, out, s, 10, 40, 4, 1.0)
     lib.refused("grad overlaps logits", "distill_loss_backward", z, e, e, s, None, z, 10, 40, 4, 1.0, False)
     lib.ok("distill_loss", z, e, e, out, None, 0, 40, 4, 1.0)
+
+
+# ---- views -------------------------------------------------------------------------------------
+
+
+def odd(lib, a, keep):
+    """The values of `a` in a view that starts one float into its buffer."""
+    flat = np.concatenate([np.full(1, 3.0, np.float32), np.asarray(a, np.float32).reshape(-1), np.full(1, 3.0, np.float32)])
+    base = lib.put(flat)
+    keep.append(base)
+    return lib.Buffer(lib.ctx, lib.lib.tysor_cuda_buffer_view(base.handle, 1, flat.size - 2), flat.size - 2)
+
+
+def untouched(keep):
+    return all(b.read().reshape(-1)[[0, -1]].tolist() == [3.0, 3.0] for b in keep)
+
+
+@pytest.mark.parametrize("dims", [(1, 4, 2, 140, 140, 64), (2, 4, 2, 1, 900, 128)], ids=["tiles", "one"])
+def test_window_attention_on_odd_views(lib, dims):
+    q, k, v, dout = attention_inputs(29, *dims, True)
+    want = R.window_attention(q, k, v, None, None, 50, 3, 0.1, True, dout)
+    keep = []
+    bq, bk, bv, bd = (odd(lib, t, keep) for t in (q, k, v, dout))
+    out, dq, dk, dv = (odd(lib, np.full(t.shape, 9.0), keep) for t in (q, q, k, v))
+    stats = lib.zeros((dims[0], dims[1], dims[3], 2))
+    shape = (*dims, 50, 3, 0.1, True)
+    lib.ok("window_attention", bq, bk, bv, None, None, out, stats, *shape)
+    lib.ok("window_attention_backward", bq, bk, bv, None, None, out, stats, bd, dq, dk, dv, *shape, False)
+    got = {n: b.read().reshape(want[n].shape) for n, b in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv))}
+    got["stats"] = stats.read().reshape(want["stats"].shape)
+    compare_attention(got, want)
+    assert untouched(keep)
+
+
+def test_other_operators_on_odd_views(lib):
+    rng = np.random.default_rng(31)
+    keep = []
+    x, dy = (rng.standard_normal((5, 256)).astype(np.float32) for _ in range(2))
+    gain, bias = (rng.standard_normal(256).astype(np.float32) for _ in range(2))
+    want = R.layer_norm(x, gain, bias, 1e-5, dy)
+    bx, by, bg, bb = (odd(lib, t, keep) for t in (x, dy, gain, bias))
+    y, dx, dg, db = (odd(lib, np.full(t.shape, 9.0), keep) for t in (x, x, gain, bias))
+    stats = lib.zeros((5, 2))
+    lib.ok("layer_norm", bx, bg, bb, y, stats, 5, 256, 1e-5)
+    lib.ok("layer_norm_backward", bx, bg, stats, by, dx, dg, db, 5, 256, False)
+    tol = 40 * U * 4  # as in test_layer_norm, means of about 0 over a spread of about 1
+    near(y.read(), want["y"], tol, "y", 1.0)
+    near(dx.read(), want["dx"], 4 * tol, "dx", 1.0)
+    near(dg.read(), want["dgain"], 4 * tol, "dgain", 1.0)
+    near(db.read(), want["dbias"], 4 * tol, "dbias", 1.0)
+
+    section, ptr = sections_ptr((4, 8))
+    heads = rng.standard_normal((2, 3, 7, 24)).astype(np.float32)
+    pos = rng.integers(0, 5000, (2, 2, 7)).astype(np.float32)
+    out = odd(lib, np.full(heads.shape, 9.0), keep)
+    lib.ok("rope_axes", odd(lib, heads, keep), odd(lib, pos, keep), out, 2, 3, 7, ptr, 2, 10000.0, False)
+    near(out.read(), R.rope_axes(heads, pos, (4, 8), 10000.0, False), 8 * U * 2, "rope_axes", 1.0)
+
+    z, ids, teacher, dloss = distill_inputs(6, 1000, 9)
+    want = R.distill_loss(z, ids, teacher, 2.0, dloss)
+    bz, bi, bt, bd = (odd(lib, t, keep) for t in (z, ids, teacher, dloss))
+    loss, grad, stats = odd(lib, np.full(6, 9.0), keep), odd(lib, np.full(z.shape, 9.0), keep), lib.zeros((6, 2))
+    lib.ok("distill_loss", bz, bi, bt, loss, stats, 6, 1000, 9, 2.0)
+    lib.ok("distill_loss_backward", bz, bi, bt, stats, bd, grad, 6, 1000, 9, 2.0, False)
+    compare_distill({"loss": loss.read(), "stats": stats.read().reshape(6, 2), "grad": grad.read().reshape(z.shape)},
+                    want, 2.0)
+    assert untouched(keep)
 
 
 # ---- wrapped memory ----------------------------------------------------------------------------

@@ -428,6 +428,7 @@ __device__ __forceinline__ bool teacher_row(const float* __restrict__ idr, const
   const int lane = threadIdx.x & 31;
   float best = -INFINITY;
   bool bad = false;
+#pragma unroll 4
   for (int e = lane; e < top; e += 32) {
     const int id = entry_id(idr[e], width, err);
     ids[e] = id;
@@ -518,6 +519,7 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     // What the end needs of each entry: the teacher's logarithm less the
     // student's logit, in 64 bits (the two logarithms nearly cancel where the
     // student follows the teacher).
+#pragma unroll 4
     for (int e = tid & 31; e < top; e += 32)
       if (p[e] != 0.0f)
         gap[e] = ((double)teacher[r * top + e] - (double)best - (double)row[eid[e]]) / temperature - log_mass;
@@ -589,19 +591,23 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
 }
 
 // One block per row and chunk of columns: T * dloss * q in one pass from the
-// row's statistics, then the few entries' own terms.
+// row's statistics, then the few entries' own terms.  Entries of one id go
+// together: a table of `slots` (a power of two, at least twice `top`) finds each
+// id's first entry, which takes the others' in order where there are any.
 template <bool VEC>
 __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
     const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
     const float* __restrict__ stats, const float* __restrict__ dloss, float* __restrict__ grad, int64_t rows,
-    int64_t width, int64_t chunk, int top, float temperature, int accumulate, int* err) {
-  extern __shared__ float entry[];  // [2][top]
+    int64_t width, int64_t chunk, int top, int slots, float temperature, int accumulate, int* err) {
+  extern __shared__ float entry[];  // [2][top], then [slots] each: id, its first entry, its entries
   __shared__ int any_entry;
   const int64_t r = blockIdx.x;
   const int64_t c0 = blockIdx.y * chunk, c1 = min(width, c0 + chunk);
   const int tid = threadIdx.x;
   int* eid = (int*)entry;
   float* p = entry + top;
+  int *key = (int*)(p + top), *first = key + slots, *count = first + slots;
+  for (int i = tid; i < slots; i += kDistillThreads) key[i] = -1, first[i] = INT_MAX, count[i] = 0;
   if (tid >= kDistillThreads - 32) {
     float best;
     double log_mass;
@@ -652,21 +658,29 @@ __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
     for (int64_t at = c0 + tid; at < c1; at += kDistillThreads) out[at] = 0.0f;
     return;
   }
+  auto start_of = [&](int id) { return (int)((uint32_t)id * 2654435769u >> 16) & (slots - 1); };
   for (int e = tid; e < top; e += kDistillThreads) {
     const int id = eid[e];
     if (id < c0 || id >= c1) continue;
-    // An id given twice: its first entry takes all of its probability, in order.
-    float mass = 0.0f;
-    bool first = true;
-    for (int f = 0; f < top; ++f) {
-      if (eid[f] != id) continue;
-      if (f < e) {
-        first = false;
-        break;
-      }
-      mass += p[f];
+    int at = start_of(id);
+    for (;; at = (at + 1) & (slots - 1)) {  // ends: at most half of the slots are taken
+      const int held = atomicCAS(&key[at], -1, id);
+      if (held == -1 || held == id) break;
     }
-    if (first) out[id] -= up * mass;
+    atomicMin(&first[at], e);
+    atomicAdd(&count[at], 1);
+  }
+  __syncthreads();
+  for (int e = tid; e < top; e += kDistillThreads) {
+    const int id = eid[e];
+    if (id < c0 || id >= c1) continue;
+    int at = start_of(id);
+    while (key[at] != id) at = (at + 1) & (slots - 1);  // every id in [c0, c1) has its slot
+    if (first[at] != e) continue;
+    float mass = p[e];
+    for (int f = e + 1, more = count[at] - 1; more > 0 && f < top; ++f)
+      if (eid[f] == id) mass += p[f], --more;
+    out[id] -= up * mass;
   }
 }
 
@@ -840,15 +854,17 @@ void launch_distill_loss_backward(const float* logits, const float* ids, const f
   while (rows * parts < 148 * 4 && width / (parts * 2) >= 4 * kDistillThreads && parts < 1024) parts *= 2;
   const int64_t chunk = ceil_div(ceil_div(width, parts), 4) * 4;
   const dim3 grid((unsigned)rows, (unsigned)ceil_div(width, chunk));
-  const size_t smem = sizeof(float) * 2 * (size_t)top;
+  int slots = 16;
+  while (slots < 2 * top) slots *= 2;
+  const size_t smem = sizeof(float) * (2 * (size_t)top + 3 * (size_t)slots);  // 32 KB at most
   // Rows of both tensors then start at the same offset from a 16-byte boundary.
   const bool vec = (((uintptr_t)logits ^ (uintptr_t)grad) & 15) == 0;
   if (vec)
     distill_backward_kernel<true><<<grid, kDistillThreads, smem, st>>>(logits, ids, teacher, stats, dloss, grad, rows,
-                                                                       width, chunk, top, temperature, accumulate, err);
+                                                                       width, chunk, top, slots, temperature, accumulate, err);
   else
     distill_backward_kernel<false><<<grid, kDistillThreads, smem, st>>>(
-        logits, ids, teacher, stats, dloss, grad, rows, width, chunk, top, temperature, accumulate, err);
+        logits, ids, teacher, stats, dloss, grad, rows, width, chunk, top, slots, temperature, accumulate, err);
   check_launch();
 }
 
