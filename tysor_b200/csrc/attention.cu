@@ -1818,7 +1818,6 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
                                                                 int splits, int per, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ __align__(16) float qs[R][kDims];
-  __shared__ float joined[kWarps][R][kDims + 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
   int64_t index = blockIdx.x;
   const int split = (int)(index % splits);
@@ -1858,7 +1857,9 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   // A lane's 4 NI values of two keys and values per step of the loop, VEC: from
   // a ring that the lane fills for itself two steps ahead, so that loads stay in
   // flight while it computes; otherwise straight from memory.
+  // Two blocks per SM fit only because the warps' results take the ring's place.
   extern __shared__ __align__(16) float ring[];  // [warps][kDecodeStages][K, V][2][4][kDims]
+  auto joined = (float(*)[R][kDims + 2])ring;    // [warps]
   float* mine = ring + ((size_t)warp * kDecodeStages * 16 + (lane >> 3)) * kDims + 4 * l8;
   auto key_at = [&](int u) { return u < first ? u : low + u - first; };
   auto copy = [&](int it) {
@@ -1964,7 +1965,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
         }
     }
   }
-  __syncwarp();
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     float top = m[r];
@@ -2162,12 +2163,14 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   constexpr int kRing = kDecodeThreads / 32 * kDecodeStages * 16 * 32 * NI * (int)sizeof(float);
+  constexpr int kJoined = kDecodeThreads / 32 * R * (32 * NI + 2) * (int)sizeof(float);  // below 48 KB
+  static_assert(kJoined <= kRing, "the ring holds the results");
   static std::atomic<uint64_t> done{0};
   if (vec) allow_shared(decode_kernel<NI, R, true>, kRing, done);
   if (vec)
     decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
   else
-    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, 0, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
+    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, kJoined, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
   check_launch();
 }
 template <int NI>
