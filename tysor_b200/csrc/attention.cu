@@ -1888,12 +1888,12 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     for (int i = 0; i < NI; ++i) {
       const int c = 4 * l8 + 32 * i;
       if (VEC) {
-        const ulonglong2 f = c < s.head_dim ? *(const ulonglong2*)(src + 32 * i) : make_ulonglong2(0, 0);
+        const ulonglong2 f = u < u1 && c < s.head_dim ? *(const ulonglong2*)(src + 32 * i) : make_ulonglong2(0, 0);
         d[2 * i] = f.x, d[2 * i + 1] = f.y;
       } else {
         float e[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = c + k < s.head_dim ? __ldg(src + 32 * i + k) : 0.0f;
+        for (int k = 0; k < 4; ++k) e[k] = u < u1 && c + k < s.head_dim ? __ldg(src + 32 * i + k) : 0.0f;
         d[2 * i] = pair_of(e[0], e[1]), d[2 * i + 1] = pair_of(e[2], e[3]);
       }
     }
@@ -1935,6 +1935,9 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     }
     load(v, it, 1, 0, vd[0]);
     load(v, it, 1, 1, vd[1]);
+    uint32_t seen_rows = 0;  // two bits per row
+    float top[R];
+    bool up = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       bool sees[2] = {one, two};
@@ -1943,26 +1946,50 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
         for (int w = 0; w < 2; ++w)
           sees[w] = sees[w] && j[w] <= at[r] && (s.window == 0 || at[r] - j[w] < s.window || j[w] < s.sinks);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) d[r][w] = sees[w] ? d[r][w] * to_log2 : -INFINITY;
-      const float top = fmaxf(d[r][0], d[r][1]);
-      if (top > m[r]) {  // seldom after a row's first keys
-        const float keep = exp2_fast(m[r] - top);
-        m[r] = top;
+      for (int w = 0; w < 2; ++w) {
+        d[r][w] = sees[w] ? d[r][w] * to_log2 : -INFINITY;
+        seen_rows |= (uint32_t)sees[w] << (2 * r + w);
+      }
+      top[r] = fmaxf(m[r], fmaxf(d[r][0], d[r][1]));
+      up |= top[r] > m[r];
+    }
+    if (up) {  // seldom after the first keys; one branch for all rows
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float keep = top[r] == m[r] ? 1.0f : exp2_fast(m[r] - top[r]);
+        m[r] = top[r];
         l[r] *= keep;
         const uint64_t both = pair_of(keep, keep);
 #pragma unroll
         for (int c = 0; c < 2 * NI; ++c) acc[r][c] = fma_pair(acc[r][c], both, 0);
       }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       const float ref = m[r] == -INFINITY ? 0.0f : m[r];
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (sees[w]) {  // a hidden value takes no part, not even times 0
-          const float p = exp2_fast(d[r][w] - ref);
-          l[r] += p;
-          const uint64_t both = pair_of(p, p);
+      for (int w = 0; w < 2; ++w) d[r][w] = exp2_fast(d[r][w] - ref);  // 0 where hidden
+      l[r] += d[r][0] + d[r][1];
+    }
+    if (s.q_len == 1) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint64_t both = pair_of(d[r][w], d[r][w]);
 #pragma unroll
           for (int c = 0; c < 2 * NI; ++c) acc[r][c] = fma_pair(both, vd[w][c], acc[r][c]);
         }
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          if (seen_rows >> (2 * r + w) & 1u) {  // a hidden value takes no part, not even times 0
+            const uint64_t both = pair_of(d[r][w], d[r][w]);
+#pragma unroll
+            for (int c = 0; c < 2 * NI; ++c) acc[r][c] = fma_pair(both, vd[w][c], acc[r][c]);
+          }
     }
   }
   __syncthreads();
