@@ -284,6 +284,8 @@ CASES = [  # batch, heads, kv_heads, q_len, k_len, dim, window, sinks
     (1, 1, 1, 150, 1000, 65, 0, 0), (2, 20, 4, 3, 260, 33, 30, 1),
     # Few query tiles over many keys: their key tiles are cut into segments.
     (1, 5, 1, 5, 3000, 128, 0, 0), (2, 3, 1, 30, 4001, 64, 0, 0), (1, 2, 1, 1300, 1300, 40, 0, 0),
+    # More than eight rows of a key head, straight from the cache.
+    (2, 9, 1, 1, 900, 64, 0, 0), (1, 40, 2, 1, 1300, 128, 300, 5), (1, 8, 2, 5, 700, 33, 0, 0), (1, 33, 1, 2, 130, 80, 20, 3),
     (1, 2, 2, 130, 2500, 72, 1500, 140), (1, 1, 1, 1100, 600, 128, 0, 0), (1, 8, 2, 600, 600, 33, 70, 5),
 ]
 

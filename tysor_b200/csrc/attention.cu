@@ -1767,13 +1767,13 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
 
 // ---- a few query rows over a long cache ----------------------------------------------------
 
-// The rows that share a key head (at most R) go over its
-// keys once, straight from the fp32 cache: with so few rows the reads bound
-// it, not the products.  The keys are split over `splits` blocks; each warp
-// takes 8 keys at a time, eight lanes per key with 4 NI columns each, and each
-// group of eight lanes keeps a running maximum, sum and output of its own, so
-// that only the dot products cross lanes.  Groups, warps and splits are joined
-// at the end in a fixed order.
+// The rows that share a key head, R at a time, go over its keys straight from the
+// fp32 cache: with so few rows the reads bound it, not the products.  The keys
+// are split over `splits` blocks; each warp takes 8 keys at a time, eight lanes
+// per key with 4 NI columns each, and each group of eight lanes keeps a running
+// maximum, sum and output of its own, so that only the dot products cross lanes.
+// Groups, warps and splits are joined at the end in a fixed order.  `sets` blocks
+// of R rows each read the same keys one after the other, all but the first from L2.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
 constexpr int kDecodeStages = 3;
@@ -1815,11 +1815,13 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
                                                                 float* __restrict__ stats, float* __restrict__ part,
-                                                                int splits, int per, int* err) {
+                                                                int sets, int splits, int per, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ __align__(16) float qs[R][kDims];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
   int64_t index = blockIdx.x;
+  const int row0 = (int)(index % sets) * R;
+  index /= sets;
   const int split = (int)(index % splits);
   index /= splits;
   const int g = (int)(index % s.kv_heads), b = (int)(index / s.kv_heads);
@@ -1831,7 +1833,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   if (splits > 1 && u0 == u1 && split > 0) return;  // the join knows how many splits hold keys
   const float to_log2 = s.scale * kLog2e;
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
-    const int r = i / kDims, c = i % kDims;
+    const int r = row0 + i / kDims, c = i % kDims;
     qs[i / kDims][c] = r < total && c < s.head_dim
                            ? q[row_at(s, b, g * group + r / s.q_len, r % s.q_len, s.heads, s.q_len) + c]
                            : 0.0f;
@@ -1839,8 +1841,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   int at[R];  // position of each row; below 0: not a row, or not in the sequence
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int p = sq.start + r % s.q_len;
-    at[r] = r < total && p < sq.n ? p : -1;
+    const int p = sq.start + (row0 + r) % s.q_len;
+    at[r] = row0 + r < total && p < sq.n ? p : -1;
   }
   __syncthreads();
   float m[R], l[R];
@@ -2014,8 +2016,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
   __syncthreads();
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
     const int r = i / kDims, c = i % kDims;
-    if (r >= total || c >= s.head_dim) continue;
-    const int h = g * group + r / s.q_len, qr = r % s.q_len;
+    if (row0 + r >= total || c >= s.head_dim) continue;
+    const int h = g * group + (row0 + r) / s.q_len, qr = (row0 + r) % s.q_len;
     float top = -INFINITY, sum = 0.0f, x = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, joined[w][r][kDims]);
@@ -2151,19 +2153,26 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   return w;
 }
 
-// Up to kDecodeRows rows per key head go through decode_kernel, more through the
-// tiles.  Measured without a window, 128 wide: 8 rows over 4096 keys of 8
-// sequences and 4 key heads 103 us against 122, over 8192 keys of 4 sequences
-// and 16 key heads 284 against 300; 16 rows, two blocks of them, 169 and 515.
-bool uses_tiles(const AttentionShape& s) { return (int64_t)s.q_len * (s.heads / s.kv_heads) > kDecodeRows; }
+// decode_kernel or the tiles: the first reads a key head's keys once per eight of
+// its rows, the second packs them once and walks them once per 128 rows of a
+// query head.  Measured, decode / tiles, 128 wide: one query of 9 heads over one,
+// four such groups and sequences of 32768 keys, 267 / 705 us, of 16 heads 280 /
+// 1272; 5 queries of 2 heads over one, 80 wide, four such and 8000 keys, 79 / 97,
+// of 4 heads, eight such and 8192 keys, 253 / 228; 9 queries and more of one head
+// take the tiles (16 over 8000 keys of 6 heads 54).
+bool uses_tiles(const AttentionShape& s) {
+  const int64_t group = s.heads / s.kv_heads;
+  return 2 * ceil_div(group * s.q_len, kDecodeRows) > 2 + group * tiles_of(s.q_len);
+}
 
 struct DecodePlan {
-  int rows, splits, per;
+  int rows, sets, splits, per;
 };
 DecodePlan decode_plan(const AttentionShape& s) {
   DecodePlan p;
-  const int total = s.q_len * (s.heads / s.kv_heads);
+  const int64_t total = (int64_t)s.q_len * (s.heads / s.kv_heads);
   p.rows = total == 1 ? 1 : total <= 4 ? 4 : kDecodeRows;
+  p.sets = (int)ceil_div(total, p.rows);
   // Each split takes the same number of keys, whatever its sequence's length:
   // about four blocks per SM at full length, at least 384 keys each.  Measured
   // for one token, 16 heads over 4, 128 wide: four sequences of up to 32768 keys
@@ -2171,7 +2180,7 @@ DecodePlan decode_plan(const AttentionShape& s) {
   // of 1024 41 us (at least 512 keys 41, 256 keys 47 to 49).
   int64_t most = s.k_len;
   if (s.window > 0) most = std::min<int64_t>(most, (int64_t)s.window + s.sinks + s.q_len - 1);
-  const int64_t blocks = (int64_t)s.batch * s.kv_heads;
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.sets;
   const int64_t want = std::max<int64_t>(1, std::min(ceil_div(kSms * 4, blocks > 0 ? blocks : 1), most / 384));
   p.per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(most, std::min<int64_t>(want, kMostSplits))), 32) * 32);
   p.splits = (int)std::max<int64_t>(1, ceil_div(most, p.per));
@@ -2186,7 +2195,7 @@ int64_t decode_work_elems(const AttentionShape& s) {
 template <int NI, int R>
 void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v, float* out,
                 float* stats, float* part, int* err, cudaStream_t st) {
-  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.splits;
+  const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.sets * p.splits;
   if (blocks > INT_MAX) throw CudaError("window_attention: too many rows");
   const bool vec = s.head_dim % 4 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
   constexpr int kRing = kDecodeThreads / 32 * kDecodeStages * 16 * 32 * NI * (int)sizeof(float);
@@ -2195,9 +2204,9 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   static std::atomic<uint64_t> done{0};
   if (vec) allow_shared(decode_kernel<NI, R, true>, kRing, done);
   if (vec)
-    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
+    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
   else
-    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, kJoined, st>>>(s, q, k, v, out, stats, part, p.splits, p.per, err);
+    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, kJoined, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
   check_launch();
 }
 template <int NI>
