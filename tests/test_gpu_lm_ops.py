@@ -88,7 +88,8 @@ def near_norm(got, want, tol, what="", size=0.0):
 
 @pytest.mark.parametrize("rows,width", [(1, 1), (3, 2), (5, 31), (2, 128), (7, 129), (33, 512), (4, 513), (9, 1001),
                                         (6, 1024), (700, 2048), (3, 2052), (5, 4096), (3, 8190), (2, 8192), (3, 8196),
-                                        (2, 16384), (2, 16385), (3, 20000), (1300, 64)])
+                                        (2, 16384), (2, 16385), (3, 20000), (1300, 64),
+                                        (300, 8200), (151, 16384), (150, 14340), (2, 57340), (2, 57348)])
 @pytest.mark.parametrize("shift", [0.0, 100.0])
 def test_layer_norm(lib, rows, width, shift):
     rng = np.random.default_rng(rows * 100003 + width)

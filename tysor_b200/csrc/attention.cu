@@ -218,6 +218,12 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
 // as the matrix unit's 128-byte swizzle wants them.  A copy of whole boxes, or
 // of 64 of their rows, is then one untiled bulk copy, and the same box serves
 // as an operand summed over its columns (scores) or over its rows (values).
+//
+// Packing reads 4 bytes a value and writes 4, and HBM bounds it: a forward's q, k
+// and v, 201 MB both ways, 34 us = 5.9 TB/s; a gradient's operands with the output
+// and the rows' statistics, 403 MB, 88 us = 4.6 TB/s (8192 tokens, 16 heads over 4,
+// 128 wide).  Splitting inside the attention kernels instead would do it once per
+// query tile that reads a key tile.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;
@@ -558,9 +564,8 @@ constexpr uint32_t kSplitStep = 16, kSplitLo = 8;
 
 // A resident packed tile from shared memory into tensor memory, where it is the
 // A operand of every score product: one read instead of one per instruction
-// (an instruction reads A and B from shared memory at about 64 bytes a cycle,
-// so that with both there the reads, not the products, take the time: 90
-// cycles measured for 128 x 64 x 16 instead of 32).  Row r is lane r; its hi
+// (measured for 128 x 64 x 16 with both operands in shared memory 90 cycles an
+// instruction, with A here 41 to 60; 32 would be the products').  Row r is lane r; its hi
 // columns are DP / 2 columns of tensor memory, its lo columns the DP / 2 after
 // them.  Called by the eight score warps; `half` is the warp's.
 template <int DP>
@@ -658,6 +663,15 @@ __device__ __forceinline__ bool sees_all(const AttentionShape& s, const RowRange
 //                the values of the one before it, so that the two overlap,
 //   warps 18-19  rows that take no part in that.
 // The query tile is kept in tensor memory (rows_to_tmem).
+//
+// Three fp16 products bound it at 557 TFLOP/s of fp32-accurate work, all keys of a
+// tile counted.  Measured, 128 wide: 8192 causal tokens without a window 400
+// TFLOP/s; with a window of 1024 and 4 sinks 215 us = 301 TFLOP/s of the visible
+// pairs, tensor pipe 52% (the tiles at both ends of a window are half hidden, and
+// a sink tile costs a step for a few columns); 2048 tokens of 8 sequences with a
+// window of 512 260 us = 233 TFLOP/s, 44%.  An instruction of 128 x 128 x 16 takes
+// about 87 cycles of the issuing warp's chain where 64 would be the products':
+// what bounds it is the turn from scores to probabilities and back.
 constexpr int kThreads = 20 * 32;
 constexpr int kSlotBytes = 2 * kBox;
 
@@ -1177,10 +1191,17 @@ __global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a, int* e
 //                dq or dk of g, dP of g + 1.  P of a step is formed while the
 //                last step's dS is summed, and its dS while the next scores are.
 // Resident tiles are in tensor memory (rows_to_tmem), with one buffer each of
-// scores (keys: then P) and of dP (then dS), and two of 64 columns of sums.
-// A key tile's queries may be many (a sink's are all that follow): its steps
-// are cut into segments that go to different blocks, each leaving its part in
-// the workspace, joined in order by grad_join_kernel.
+// scores (keys: then P) and of dP (then dS), and two of 64 columns of sums: with
+// 256 columns for the resident tiles no wider step fits the 512.
+//
+// The products, five per visible pair and 128 columns and two of them done twice,
+// bound it.  Measured for 8192 tokens, 16 heads over 4, window 1024, 128 wide: 309
+// us for dq (tensor pipe 57%), 447 for dk and dv (54%), together 214 TFLOP/s of the
+// formulas' work.  An instruction of 128 x 64 x 16 takes 41 to 60 cycles instead of
+// 32, and the tiles at a window's ends are half hidden.
+// A key tile's queries may be many (a sink's are all that follow), and tiles may
+// be few: their steps are cut into segments that go to different blocks, each
+// leaving its part in the workspace, joined in order by grad_join_kernel.
 // Registers after the split, as in the forward: the keys' pass keeps sums of two
 // gradients, 2 x 64 + 2 x 152 + 48 = 480; the queries' 2 x 112 + 2 x 88 + 64 = 464.
 template <bool KEYS>
@@ -1735,7 +1756,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
 }
 
 // Adds the segments of one tile in order, `rows` rows per block: few for a
-// sink tile, whose many segments few blocks would read one after the other.
+// sink tile, whose many segments few blocks would read one after the other (12 us
+// for four such tiles).
 template <int DP, bool KEYS>
 __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int rows, int* err) {
   constexpr int kGrads = KEYS ? 2 : 1;
@@ -1773,7 +1795,13 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, i
 // per key with 4 NI columns each, and each group of eight lanes keeps a running
 // maximum, sum and output of its own, so that only the dot products cross lanes.
 // Groups, warps and splits are joined at the end in a fixed order.  `sets` blocks
-// of R rows each read the same keys one after the other, all but the first from L2.
+// of R rows each read the same keys side by side, all but the first from L2.
+//
+// HBM bounds it up to four rows: 4 heads over each of 4, 128 wide, four sequences of
+// up to 32768 keys, 416 MB in 77 to 88 us = 4.7 to 5.4 TB/s of 6.5 (the longest
+// sequence's blocks end last); 32 sequences with a window of 1024, 122 MB in 33 us:
+// a wave of 256 blocks, each a start, 17 steps and an end.  Eight rows take 138 us
+// where four take 103: two blocks of four warps per SM wait for their own arithmetic.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
 constexpr int kDecodeStages = 3;

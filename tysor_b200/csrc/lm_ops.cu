@@ -5,6 +5,8 @@
 #include <limits.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "lm_ops.cuh"
 
 namespace tysor {
@@ -112,7 +114,8 @@ struct RowPart {
 // ---- layer norm -------------------------------------------------------------
 
 // One group of TPR threads per row, the row in registers: the mean first,
-// then the squared distances from it (no difference of large sums).
+// then the squared distances from it (no difference of large sums).  HBM bounds
+// it: 16384 rows of 2048, 268 MB, 45 us = 5.9 TB/s; 16 rows 4.7 us a call, a launch.
 template <int TPR, int NV, bool VEC, int kThreads>
 __global__ void __launch_bounds__(kThreads) layer_norm_kernel(const float* __restrict__ x,
                                                               const float* __restrict__ gain,
@@ -184,10 +187,147 @@ __global__ void __launch_bounds__(1024) layer_norm_wide_kernel(const float* __re
   }
 }
 
+__device__ __forceinline__ void copy16(const float4* to, const float4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+
+// Rows of more than kLayerNormWide values, held in shared memory (each thread's
+// columns by the thread that reads them, so that only the sums wait): two and
+// more rows per SM are under way where registers would hold one.  8192 rows of
+// 16384, 1.07 GB, 171 us = 6.3 TB/s (in registers 262), 4096 of 20000 121 us (from
+// L2 in three passes 222).
+constexpr int kSharedRowThreads = 512;
+__global__ void __launch_bounds__(kSharedRowThreads) layer_norm_shared_kernel(
+    const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ bias, float* __restrict__ y,
+    float* __restrict__ stats, int64_t rows, int width, float eps) {
+  extern __shared__ __align__(16) float4 held[];  // [width / 4]
+  __shared__ float red[2 * kSharedRowThreads / 32];
+  const int quads = width / 4;
+  const float inv = 1.0f / (float)width;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const float4* src = (const float4*)(x + r * width);
+    for (int i = threadIdx.x; i < quads; i += kSharedRowThreads) copy16(held + i, src + i);
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    float s = 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < quads; i += kSharedRowThreads) {
+      const float4 f = held[i];
+      s += (f.x + f.y) + (f.z + f.w);
+    }
+    const float mean = group_sum<kSharedRowThreads>(s, red, 0, 0) * inv;
+    float q = 0.0f;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < quads; i += kSharedRowThreads) {
+      const float4 f = held[i];
+      const float a = f.x - mean, b = f.y - mean, c = f.z - mean, d = f.w - mean;
+      q += (a * a + b * b) + (c * c + d * d);
+    }
+    const float rstd = rsqrtf(group_sum<kSharedRowThreads>(q, red, 0, 1) * inv + eps);
+    float4* dst = (float4*)(y + r * width);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < quads; i += kSharedRowThreads) {
+      float4 f = held[i];
+      f.x = (f.x - mean) * rstd, f.y = (f.y - mean) * rstd, f.z = (f.z - mean) * rstd, f.w = (f.w - mean) * rstd;
+      if (gain != nullptr) {
+        const float4 w = ((const float4*)gain)[i];
+        f.x *= w.x, f.y *= w.y, f.z *= w.z, f.w *= w.w;
+      }
+      if (bias != nullptr) {
+        const float4 w = ((const float4*)bias)[i];
+        f.x += w.x, f.y += w.y, f.z += w.z, f.w += w.w;
+      }
+      dst[i] = f;
+    }
+    if (stats != nullptr && threadIdx.x == 0) *(float2*)(stats + 2 * r) = make_float2(mean, rstd);
+  }
+}
+
+// Their gradients: x and dy of a row in shared memory, the next row's on their
+// way where `stages` is 2; dgain and dbias as below, a thread owning its columns.
+// 8192 rows of 16384, 1.6 GB, 305 us = 5.3 TB/s, of 8196 185 us (two passes over the
+// row and a third for the columns 817 and 449).
+constexpr int kSharedQuads = 8;  // of a thread: rows up to 16384 values
+__global__ void __launch_bounds__(kSharedRowThreads) layer_norm_backward_shared_kernel(
+    const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ stats,
+    const float* __restrict__ dy, float* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width,
+    int stages, int accumulate) {
+  extern __shared__ __align__(16) float4 held[];  // [stages][x, dy][width / 4]
+  __shared__ float2 red[2 * kSharedRowThreads / 32];
+  const int quads = width / 4;
+  const float inv = 1.0f / (float)width;
+  float4 dg[kSharedQuads], db[kSharedQuads];
+#pragma unroll
+  for (int k = 0; k < kSharedQuads; ++k) dg[k] = db[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto fetch = [&](int64_t r, int stage) {
+    if (r < rows) {
+      const float4* xs = (const float4*)(x + r * width);
+      const float4* ys = (const float4*)(dy + r * width);
+      float4* to = held + (int64_t)stage * 2 * quads;
+      for (int i = threadIdx.x; i < quads; i += kSharedRowThreads) copy16(to + i, xs + i), copy16(to + quads + i, ys + i);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (stages == 2) fetch(blockIdx.x, 0);
+  int phase = 0, stage = 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    if (stages == 2) {
+      fetch(r + gridDim.x, stage ^ 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      fetch(r, 0);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    const float4 *xs = held + (int64_t)stage * 2 * quads, *ys = xs + quads;
+    const float2 st = *(const float2*)(stats + 2 * r);
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSharedQuads; ++k) {
+      const int i = threadIdx.x + k * kSharedRowThreads;
+      if (i >= quads) break;
+      const float4 f = xs[i], g = ys[i];
+      const float4 w = gain ? ((const float4*)gain)[i] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      const float4 n = make_float4((f.x - st.x) * st.y, (f.y - st.x) * st.y, (f.z - st.x) * st.y, (f.w - st.x) * st.y);
+      dg[k].x += g.x * n.x, dg[k].y += g.y * n.y, dg[k].z += g.z * n.z, dg[k].w += g.w * n.w;
+      db[k].x += g.x, db[k].y += g.y, db[k].z += g.z, db[k].w += g.w;
+      a += (g.x * w.x + g.y * w.y) + (g.z * w.z + g.w * w.w);
+      b += (g.x * w.x * n.x + g.y * w.y * n.y) + (g.z * w.z * n.z + g.w * w.w * n.w);
+    }
+    group_sum2<kSharedRowThreads>(a, b, red, 0, phase);
+    phase ^= 1;
+    a *= inv;
+    b *= inv;
+    float4* dst = (float4*)(dx + r * width);
+#pragma unroll
+    for (int k = 0; k < kSharedQuads; ++k) {
+      const int i = threadIdx.x + k * kSharedRowThreads;
+      if (i >= quads) break;
+      const float4 f = xs[i], g = ys[i];
+      const float4 w = gain ? ((const float4*)gain)[i] : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+      float4 o = make_float4((g.x * w.x - a - (f.x - st.x) * st.y * b) * st.y, (g.y * w.y - a - (f.y - st.x) * st.y * b) * st.y,
+                             (g.z * w.z - a - (f.z - st.x) * st.y * b) * st.y, (g.w * w.w - a - (f.w - st.x) * st.y * b) * st.y);
+      if (accumulate) {
+        const float4 p = dst[i];
+        o.x += p.x, o.y += p.y, o.z += p.z, o.w += p.w;
+      }
+      dst[i] = o;
+    }
+    if (stages == 2) stage ^= 1;
+  }
+  if (partial == nullptr) return;
+  float4* line = (float4*)(partial + (int64_t)blockIdx.x * 2 * width);
+#pragma unroll
+  for (int k = 0; k < kSharedQuads; ++k) {
+    const int i = threadIdx.x + k * kSharedRowThreads;
+    if (i < quads) line[i] = dg[k], line[quads + i] = db[k];
+  }
+}
+
 // dx of one row per group and step; each thread owns its columns' share of
 // dgain and dbias in registers over all rows of the block.  The block's groups
 // add theirs in order in shared memory, and `partial` gets one line per block
-// (summed in a fixed order by column_sum_kernel).
+// (summed in a fixed order by column_sum_kernel).  HBM bounds it: 16384 rows of
+// 2048, 403 MB, 68 us = 5.9 TB/s, and 8 us for the 296 lines of partial sums.
 template <int TPR, int NV, bool VEC>
 __global__ void __launch_bounds__(512, NV <= 2 ? 2 : 1) layer_norm_backward_kernel(
     const float* __restrict__ x, const float* __restrict__ gain, const float* __restrict__ stats,
@@ -334,7 +474,8 @@ struct RopeArgs {
 
 // Each thread turns V neighbouring pairs of one token in `head_chunk` heads
 // with one evaluation of their angles: positions times rates in 64 bits,
-// reduced to a fraction of a revolution, so that far positions lose nothing.
+// reduced to a fraction of a revolution, so that far positions lose nothing.  HBM
+// bounds it: 16 heads of 128 values, 16384 tokens, 268 MB in 42 us = 6.4 TB/s.
 template <int V>
 __global__ void __launch_bounds__(256) rope_axes_kernel(const float* __restrict__ x,
                                                         const float* __restrict__ positions,
@@ -479,7 +620,8 @@ __device__ __forceinline__ void take(Online& o, float v, float c) {
 // of gridDim.y blocks (one for many rows) whose parts the first block joins in
 // order through distributed shared memory; then the loss of the row's entries.
 // Eight small blocks per SM rather than four: while one ends its row (its few
-// entries, the logarithms), the others keep loads in flight.
+// entries, the logarithms), the others keep loads in flight.  HBM bounds it: 8192
+// rows of 32000, 1.05 GB in 181 us = 5.8 TB/s.
 constexpr int kDistillThreads = 256;
 __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
     const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
@@ -593,7 +735,10 @@ __global__ void __launch_bounds__(kDistillThreads) distill_loss_kernel(
 // One block per row and chunk of columns: T * dloss * q in one pass from the
 // row's statistics, then the few entries' own terms.  Entries of one id go
 // together: a table of `slots` (a power of two, at least twice `top`) finds each
-// id's first entry, which takes the others' in order where there are any.
+// id's first entry, which takes the others' in order where there are any.  HBM
+// bounds it: 8192 rows of 32000, 2.1 GB in 330 us = 6.4 TB/s.  Comparing each pair of
+// entries instead, loss and gradient took 533 us with 64 entries a row where this
+// takes 521, and 2858 where this takes 1085 with 1024.
 template <bool VEC>
 __global__ void __launch_bounds__(kDistillThreads) distill_backward_kernel(
     const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ teacher,
@@ -717,9 +862,14 @@ void layer_norm_pick(const float* x, const float* gain, const float* bias, float
 
 constexpr int64_t kLayerNormMost = 16384;         // widest row in registers, forward
 constexpr int64_t kLayerNormBackwardMost = 8192;  // backward
+// Rows above 8192 values that may be loaded 16 bytes at a time are held in shared
+// memory as far as it goes, others in registers or read again from L2.
+constexpr int64_t kLayerNormWide = 8192;
+constexpr int64_t kSharedBytes = 224 * 1024;
+constexpr int64_t kSharedBackwardMost = 4 * kSharedQuads * kSharedRowThreads;
 
 int layer_norm_lines(int64_t rows, int64_t width) {
-  if (width > kLayerNormBackwardMost) return (int)(rows < 64 ? rows : 64);
+  if (width > kLayerNormBackwardMost) return (int)(rows < 148 ? rows : 148);
   int tpr = 32;
   while (tpr * 8 < width && tpr < 512) tpr *= 2;
   const int64_t want = ceil_div(rows, 512 / tpr);
@@ -757,13 +907,21 @@ void layer_norm_backward_pick(const float* x, const float* gain, const float* st
 void launch_layer_norm(const float* x, const float* gain, const float* bias, float* y, float* stats, int64_t rows,
                        int64_t width, float eps, cudaStream_t st) {
   if (rows <= 0 || width <= 0) return;
+  const bool vec = width % 4 == 0 && aligned16(x) && aligned16(y) && aligned16(gain) && aligned16(bias);
+  if (vec && width > kLayerNormWide && width * 4 <= kSharedBytes) {
+    const int bytes = (int)width * 4, blocks = 148 * (int)std::min<int64_t>(4, kSharedBytes / (bytes + 1024));
+    TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedBytes));
+    layer_norm_shared_kernel<<<(int)std::min<int64_t>(rows, std::max(blocks, 148)), kSharedRowThreads, bytes, st>>>(
+        x, gain, bias, y, stats, rows, (int)width, eps);
+    check_launch();
+    return;
+  }
   if (width > kLayerNormMost) {
     layer_norm_wide_kernel<<<(int)(rows < 148 * 2 ? rows : 148 * 2), 1024, 0, st>>>(x, gain, bias, y, stats, rows,
                                                                                     width, eps);
     check_launch();
     return;
   }
-  const bool vec = width % 4 == 0 && aligned16(x) && aligned16(y) && aligned16(gain) && aligned16(bias);
   if (vec) layer_norm_pick<true>(x, gain, bias, y, stats, rows, width, eps, st);
   else layer_norm_pick<false>(x, gain, bias, y, stats, rows, width, eps, st);
 }
@@ -782,7 +940,15 @@ void launch_layer_norm_backward(const float* x, const float* gain, const float* 
   if (rows > 0) {
     lines = layer_norm_lines(rows, width);
     float* part = columns ? partial : nullptr;
-    if (width > kLayerNormBackwardMost) {
+    const bool vec = width % 4 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gain);
+    if (vec && width > kLayerNormBackwardMost && width <= kSharedBackwardMost && aligned16(partial)) {
+      const int stages = 16 * width <= kSharedBytes ? 2 : 1;
+      TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_backward_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)kSharedBytes));
+      layer_norm_backward_shared_kernel<<<lines, kSharedRowThreads, (size_t)(8 * width * stages), st>>>(
+          x, gain, stats, dy, dx, part, rows, (int)width, stages, accumulate_dx);
+      check_launch();
+    } else if (width > kLayerNormBackwardMost) {
       layer_norm_backward_wide_kernel<<<(int)(rows < 148 * 2 ? rows : 148 * 2), 1024, 0, st>>>(
           x, gain, stats, dy, dx, rows, width, accumulate_dx);
       check_launch();
@@ -792,7 +958,6 @@ void launch_layer_norm_backward(const float* x, const float* gain, const float* 
         check_launch();
       }
     } else {
-      const bool vec = width % 4 == 0 && aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(gain);
       if (vec) layer_norm_backward_pick<true>(x, gain, stats, dy, dx, part, rows, width, accumulate_dx, st);
       else layer_norm_backward_pick<false>(x, gain, stats, dy, dx, part, rows, width, accumulate_dx, st);
     }
