@@ -701,6 +701,7 @@ struct ForwardArgs {
   const float *fq, *fk, *fv;
   float *out, *stats;
   int segs;         // segments of each item's key tiles
+  int* steps;       // segs > 1: key tiles of each unit
   float* part;      // segs > 1: [item][segment][128][DP] sums of P.V, relative to 2^exponent
   float2* part_ml;  // and [item][segment][128] (exponent, sum of P)
 };
@@ -716,21 +717,24 @@ struct QueryItem {
   int q_index, k_index;  // of the item's query tile and its head's first key tile
 };
 
+// Where item `index` lies: heads, sequence, first row.
+__device__ __forceinline__ int query_place(const AttentionShape& s, int index, int* h, int* b) {
+  *h = index % s.heads;
+  *b = index / s.heads % s.batch;
+  return (tiles_of(s.q_len) - 1 - index / (s.heads * s.batch)) * kTile;
+}
+
 // Unit `unit`: segment unit % segs of item unit / segs.  Called by whole warps.
 __device__ __forceinline__ QueryItem query_item(const ForwardArgs& a, int unit, int* err) {
   const AttentionShape& s = a.s;
   QueryItem t;
   const int index = unit / a.segs, seg = unit - index * a.segs;
-  const int tiles_q = tiles_of(s.q_len);
-  const int tq = tiles_q - 1 - index / (s.heads * s.batch);
-  t.h = index % s.heads;
-  t.b = index / s.heads % s.batch;
+  t.r0 = query_place(s, index, &t.h, &t.b);
   t.g = t.h / (s.heads / s.kv_heads);
-  t.r0 = tq * kTile;
   t.sq = sequence_of(s, t.b, err);
   t.rows = rows_of(s, t.sq, t.r0);
   t.range = keys_for(s, t.sq, t.rows);
-  t.q_index = (t.b * s.heads + t.h) * tiles_q + tq;
+  t.q_index = (t.b * s.heads + t.h) * tiles_of(s.q_len) + t.r0 / kTile;
   t.k_index = (t.b * s.kv_heads + t.g) * tiles_of(s.k_len);
   float sum = a.fq[t.q_index];
   for (int i = threadIdx.x & 31; i < t.range.count; i += 32)
@@ -1075,6 +1079,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const QueryItem t = query_item(a, w, err);
+      if (a.segs > 1 && threadIdx.x == 8 * 32) a.steps[w] = t.f1 - t.f0;
       if (t.f0 >= t.f1) continue;
       float acc[kCols];
 #pragma unroll
@@ -1132,17 +1137,27 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(ForwardArgs a, int
   }
 }
 
+// Segments that hold a part: the first ones, as each but the last of them is full.
+__device__ __forceinline__ int segments_used(const int* steps, int segs, int stride) {
+  int used = 0;
+  for (int k = threadIdx.x & 31; k < segs; k += 32) used += steps[(int64_t)k * stride] > 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) used += __shfl_xor_sync(0xffffffffu, used, o);
+  return used;
+}
+
 // Joins an item's segments in order, a few rows per block.
 constexpr int kJoinRows = 8;
 template <int DP>
-__global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a, int* err) {
+__global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a) {
   const AttentionShape& s = a.s;
   const int item = blockIdx.x / (kTile / kJoinRows), row0 = blockIdx.x % (kTile / kJoinRows) * kJoinRows;
-  const QueryItem t = query_item(a, item * a.segs, err);
-  if (t.n == 0) return;  // written key by key
-  const int used = (t.n + t.f1 - 1) / t.f1;  // of f1 tiles each
+  int h, b;
+  const int r0 = query_place(s, item, &h, &b);
+  const int used = segments_used(a.steps + (int64_t)item * a.segs, a.segs, 1);  // 0: written key by key
+  if (used == 0) return;
   for (int i = threadIdx.x; i < kJoinRows * DP / 4; i += 256) {
-    const int row = row0 + i / (DP / 4), c = i % (DP / 4) * 4, r = t.r0 + row;
+    const int row = row0 + i / (DP / 4), c = i % (DP / 4) * 4, r = r0 + row;
     if (r >= s.q_len || c >= s.head_dim) continue;
     const int64_t first = (int64_t)item * a.segs * kTile + row;
     float top = -INFINITY, l = 0.0f, v[4] = {};
@@ -1160,10 +1175,10 @@ __global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a, int* e
       v[3] = v[3] * keep + p.w * take;
       top = next;
     }
-    store_row(a.out + row_at(s, t.b, t.h, r, s.heads, s.q_len) + c, v, l > 0.0f ? 1.0f / l : 0.0f, s.head_dim - c,
+    store_row(a.out + row_at(s, b, h, r, s.heads, s.q_len) + c, v, l > 0.0f ? 1.0f / l : 0.0f, s.head_dim - c,
               s.head_dim % 4 == 0 && ((uintptr_t)a.out & 15) == 0, 0);
     if (a.stats != nullptr && c == 0)
-      *(float2*)(a.stats + 2 * (((int64_t)t.b * s.heads + t.h) * s.q_len + r)) = tile_stats(top, l);
+      *(float2*)(a.stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r)) = tile_stats(top, l);
   }
 }
 
@@ -1237,6 +1252,7 @@ struct GradArgs {
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
   Segments seg;
+  int* steps;                          // of each unit
   float* part;                         // queries: [unit][128][DP]; keys: [unit][dk, dv][128][DP]
 };
 
@@ -1265,26 +1281,44 @@ struct GradItem {
   bool first;          // the first of them
 };
 
+// Where unit `index` lies: heads, sequence, first row, and its segment.
+template <bool KEYS>
+__device__ __forceinline__ GradItem grad_place(const GradArgs& a, int index, int* segment) {
+  const AttentionShape& s = a.s;
+  GradItem t;
+  if (!KEYS) {
+    t.segs = a.seg.query_segs;
+    *segment = index % t.segs;
+    t.r0 = query_place(s, index / t.segs, &t.h, &t.b);
+    t.g = t.h / (s.heads / s.kv_heads);
+  } else {
+    // The first keys are seen by the most queries.
+    const int of_long = a.seg.long_tiles * a.seg.long_segs * s.kv_heads * s.batch;
+    const bool is_long = index < of_long;
+    t.segs = is_long ? a.seg.long_segs : a.seg.short_segs;
+    if (!is_long) index -= of_long;
+    const int tk = index / (t.segs * s.kv_heads * s.batch) + (is_long ? 0 : a.seg.long_tiles);
+    *segment = index / (s.kv_heads * s.batch) % t.segs;
+    t.g = index % s.kv_heads;
+    t.b = index / s.kv_heads % s.batch;
+    t.h = t.g * (s.heads / s.kv_heads);
+    t.r0 = tk * kTile;
+  }
+  return t;
+}
+
 template <bool KEYS>
 __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int* err) {
   const AttentionShape& s = a.s;
-  GradItem t;
   const int group = s.heads / s.kv_heads, lane = threadIdx.x & 31;
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
+  int seg;
+  GradItem t = grad_place<KEYS>(a, index, &seg);
   float sum;
-  int seg = 0;
   if (!KEYS) {
-    t.segs = a.seg.query_segs;
-    seg = index % t.segs;
-    index /= t.segs;
-    const int tq = tiles_q - 1 - index / (s.heads * s.batch);
-    t.h = index % s.heads;
-    t.b = index / s.heads % s.batch;
-    t.g = t.h / group;
-    t.r0 = tq * kTile;
     t.sq = sequence_of(s, t.b, err);
     t.rows = rows_of(s, t.sq, t.r0);
-    t.row_tile = (t.b * s.heads + t.h) * tiles_q + tq;
+    t.row_tile = (t.b * s.heads + t.h) * tiles_q + t.r0 / kTile;
     const int x = max(t.rows.p0, 0), z = min(t.rows.p1, t.sq.n - 1);
     const int low = s.window > 0 ? max(x + 1 - s.window, 0) : 0;
     t.range.low = low / kStep;
@@ -1297,20 +1331,9 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
       sum += a.fk[k] + a.fv[k];
     }
   } else {
-    // The first keys are seen by the most queries.
-    const int of_long = a.seg.long_tiles * a.seg.long_segs * s.kv_heads * s.batch;
-    const bool is_long = index < of_long;
-    t.segs = is_long ? a.seg.long_segs : a.seg.short_segs;
-    if (!is_long) index -= of_long;
-    const int tk = index / (t.segs * s.kv_heads * s.batch) + (is_long ? 0 : a.seg.long_tiles);
-    seg = index / (s.kv_heads * s.batch) % t.segs;
-    t.g = index % s.kv_heads;
-    t.b = index / s.kv_heads % s.batch;
-    t.h = t.g * group;
-    t.r0 = tk * kTile;
     t.sq = sequence_of(s, t.b, err);
     t.rows = {0, 0, false};
-    t.row_tile = (t.b * s.kv_heads + t.g) * tiles_k + tk;
+    t.row_tile = (t.b * s.kv_heads + t.g) * tiles_k + t.r0 / kTile;
     // Rows that see some key of the tile: positions from the first key on, up
     // to where the last key leaves the window (none leaves it among the sinks).
     const int last = min(t.r0 + kTile, t.sq.n) - 1;
@@ -1710,6 +1733,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
     for (int round = 0, w; ok && item_of(round, items, &w); ++round) {
       if (w < 0) continue;
       const GradItem t = grad_item<KEYS>(a, w, err);
+      if (t.segs > 1 && threadIdx.x == 8 * 32) a.steps[w] = t.f1 - t.f0;
       if (t.f0 >= t.f1) continue;
       const float4 st = KEYS ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a.info[(int64_t)t.row_tile * kTile + row];
       const float norm = KEYS ? a.nv[(int64_t)t.row_tile * kTile + row] : st.w;
@@ -1755,30 +1779,52 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
   }
 }
 
-// Adds the segments of one tile in order, `rows` rows per block: few for a
-// sink tile, whose many segments few blocks would read one after the other (12 us
-// for four such tiles).
+// Tiles whose segments are joined: `tiles` of them, the first with unit `first`,
+// a tile's next segment `stride` units on; `rows` rows per block.
+struct JoinSet {
+  int tiles, first, segs, stride, rows;
+  __host__ __device__ int blocks() const { return segs > 1 ? tiles * (kTile / rows) : 0; }
+};
+
+// Adds the segments of one tile in a fixed order, few rows per block: very few
+// for a sink tile, whose many segments few blocks would read one after the other.
+// Threads that a block's rows leave over share the segments.
 template <int DP, bool KEYS>
-__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, int first, int segs, int stride, int rows, int* err) {
+__global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, JoinSet one, JoinSet two) {
   constexpr int kGrads = KEYS ? 2 : 1;
+  __shared__ float4 slices[256];
   const AttentionShape& s = a.s;
-  const int tile = blockIdx.x / (kTile / rows), row0 = blockIdx.x % (kTile / rows) * rows;
-  // The tile's first segment; the next ones follow `stride` units apart.
-  const int unit = first + tile / stride * segs * stride + tile % stride;
-  const GradItem t = grad_item<KEYS>(a, unit, err);
-  if (t.n == 0) return;  // written key by key
-  const int total = (KEYS ? s.heads / s.kv_heads : 1) * t.n, each = (total + segs - 1) / segs;
-  const int used = (total + each - 1) / each;
-  for (int i = threadIdx.x; i < kGrads * rows * DP / 4; i += 256) {
+  const bool is_two = (int)blockIdx.x >= one.blocks();
+  const JoinSet set = is_two ? two : one;
+  const int block = (int)blockIdx.x - (is_two ? one.blocks() : 0), rows = set.rows, segs = set.segs, stride = set.stride;
+  const int tile = block / (kTile / rows), row0 = block % (kTile / rows) * rows;
+  const int unit = set.first + tile / stride * segs * stride + tile % stride;
+  int seg;
+  const GradItem t = grad_place<KEYS>(a, unit, &seg);
+  const int used = segments_used(a.steps + unit, segs, stride);
+  if (used == 0) return;  // written key by key
+  const int items = kGrads * rows * DP / 4, count = items < 256 ? 256 / items : 1;  // slices of the segments
+  for (int i0 = 0; i0 < items; i0 += 256) {
+    // items is a power of two from 32 to 512.
+    const int i = i0 + (items < 256 ? threadIdx.x % items : threadIdx.x), slice = items < 256 ? threadIdx.x / items : 0;
     const int which = i / (rows * DP / 4), r = row0 + i / (DP / 4) % rows, c = i % (DP / 4) * 4;
-    if (t.r0 + r >= (KEYS ? s.k_len : s.q_len) || c >= s.head_dim) continue;
     float v[4] = {};
 #pragma unroll 8
-    for (int k = 0; k < used; ++k) {
+    for (int k = slice; k < used; k += count) {
       const float4 p =
           *(const float4*)(a.part + (((int64_t)(unit + k * stride) * kGrads + which) * kTile + r) * DP + c);
       v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
     }
+    if (count > 1) {
+      slices[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+      __syncthreads();
+      if (slice != 0) return;
+      for (int k = 1; k < count; ++k) {
+        const float4 p = slices[threadIdx.x + k * items];
+        v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+      }
+    }
+    if (t.r0 + r >= (KEYS ? s.k_len : s.q_len) || c >= s.head_dim) continue;
     float* grad = !KEYS ? a.dq : which ? a.dv : a.dk;
     const int64_t at = KEYS ? row_at(s, t.b, t.g, t.r0 + r, s.kv_heads, s.k_len)
                             : row_at(s, t.b, t.h, t.r0 + r, s.heads, s.q_len);
@@ -2142,7 +2188,7 @@ struct ForwardWork {
   uint8_t *pq, *pk, *pv;
   float *fq, *fk, *fv, *part;
   float2* part_ml;
-  int segs;
+  int *steps, segs;
   int64_t floats;
 };
 // Segments of a query tile's key tiles, of at least `least` tiles each: one unit
@@ -2177,6 +2223,7 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   w.segs = segments_of_queries(s, 4);
   w.part = c.take(w.segs > 1 ? nq * w.segs * kTile * padded_dim(s) : 0);
   w.part_ml = (float2*)c.take(w.segs > 1 ? nq * w.segs * kTile * 2 : 0);
+  w.steps = (int*)c.take(w.segs > 1 ? nq * w.segs : 0);
   w.floats = c.used;
   return w;
 }
@@ -2266,6 +2313,7 @@ struct GradWork {
   float *fq, *fk, *fv, *fo, *nv, *tnv, *tno, *tdo;
   float4* info;
   float2* col;
+  int* steps;
   float* part;
   int64_t floats;
 };
@@ -2321,6 +2369,7 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   // The queries' pass has joined its segments when the keys' begins.
   const int64_t for_keys = g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 : 0;
   const int64_t for_queries = g.query_segs > 1 ? nq * g.query_segs : 0;
+  w.steps = (int*)c.take(std::max<int64_t>(for_keys > 0 ? grad_units(s, g) : 0, for_queries));
   w.part = c.take(std::max(for_keys, for_queries) * kTile * padded_dim(s));
   w.floats = c.used;
   return w;
@@ -2337,25 +2386,17 @@ void run_grad(const GradArgs& a, int* err, cudaStream_t st) {
   if (items > INT_MAX / 64) throw CudaError("window_attention: too many rows");
   grad_kernel<DP, KEYS><<<(unsigned)(items < kSms ? items : kSms), kThreads, kSmem, st>>>(a, (int)items, err);
   check_launch();
+  JoinSet one{0, 0, 1, 1, 8}, two{0, 0, 1, 1, 8};
   if (!KEYS) {
-    if (a.seg.query_segs == 1) return;
-    const int64_t blocks = items / a.seg.query_segs * (kTile / 8);  // query_segs > 1: few items
-    grad_join_kernel<DP, false><<<(unsigned)blocks, 256, 0, st>>>(a, 0, a.seg.query_segs, 1, 8, err);
-    check_launch();
-    return;
+    one = {(int)(items / a.seg.query_segs), 0, a.seg.query_segs, 1, 8};
+  } else {
+    const int stride = s.kv_heads * s.batch, long_tiles = a.seg.long_tiles * stride;
+    one = {long_tiles, 0, a.seg.long_segs, stride, s.window > 0 ? 2 : 8};
+    two = {tiles_of(s.k_len) * stride - long_tiles, long_tiles * a.seg.long_segs, a.seg.short_segs, stride, 8};
   }
-  const int tiles = tiles_of(s.k_len), stride = s.kv_heads * s.batch;
-  if (a.seg.long_segs > 1 && a.seg.long_tiles > 0) {
-    const int rows = s.window > 0 ? 2 : 8;
-    grad_join_kernel<DP, true><<<(unsigned)(a.seg.long_tiles * stride * (kTile / rows)), 256, 0, st>>>(
-        a, 0, a.seg.long_segs, stride, rows, err);
-    check_launch();
-  }
-  if (a.seg.short_segs > 1 && tiles > a.seg.long_tiles) {
-    grad_join_kernel<DP, true><<<(unsigned)((tiles - a.seg.long_tiles) * stride * (kTile / 8)), 256, 0, st>>>(
-        a, a.seg.long_tiles * a.seg.long_segs * stride, a.seg.short_segs, stride, 8, err);
-    check_launch();
-  }
+  if (one.blocks() + two.blocks() == 0) return;
+  grad_join_kernel<DP, KEYS><<<one.blocks() + two.blocks(), 256, 0, st>>>(a, one, two);
+  check_launch();
 }
 
 template <int DP>
@@ -2368,7 +2409,7 @@ void run_forward(const ForwardArgs& a, int* err, cudaStream_t st) {
       a, (int)units, err);
   check_launch();
   if (a.segs == 1) return;
-  forward_join_kernel<DP><<<(unsigned)(items * (kTile / kJoinRows)), 256, 0, st>>>(a, err);
+  forward_join_kernel<DP><<<(unsigned)(items * (kTile / kJoinRows)), 256, 0, st>>>(a);
   check_launch();
 }
 
@@ -2391,7 +2432,7 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
                        {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0}};
     run_pack(s, jobs, 3, err, st);
-    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats, w.segs, w.part, w.part_ml};
+    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats, w.segs, w.steps, w.part, w.part_ml};
     if (padded_dim(s) == 64) run_forward<64>(a, err, st);
     else run_forward<128>(a, err, st);
     return;
@@ -2423,7 +2464,7 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
   run_pack(s, jobs, 4, err, st);
   const GradArgs a{s,     q,     k,     v,      out,   stats, dout, w.pq, w.pk, w.pv,         w.po,         w.fq,         w.fk,
                    w.fv,  w.fo,  w.nv,  w.tnv,  w.tno, w.tdo, w.info, w.col, dq, dk,          dv,           accumulate_q, accumulate_k,
-                   accumulate_v, segments_of(s), w.part};
+                   accumulate_v, segments_of(s), w.steps, w.part};
   if (padded_dim(s) == 64) {
     run_grad<64, false>(a, err, st);
     run_grad<64, true>(a, err, st);
