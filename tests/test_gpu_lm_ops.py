@@ -5,7 +5,9 @@ distill_loss, forward and backward.
 Tolerances (u = 2^-24, half a step of fp32), fixed from the arithmetic:
 
 * layer_norm: a row's mean and variance are sums of at most 16 values per
-  thread and 11 levels of a tree, 27u of the terms' size each; rstd has half
+  thread and 11 levels of a tree, 27u of the terms' size each (rows held in
+  shared memory: 28 additions to growing sums, 14u of the whole, and 2 + 5 + 8
+  for a quad, a warp and 16 warps: 29u); rstd has half
   the variance's error; three more roundings: 40u of the largest |n * gain|.
 * rope_axes: the angle's fraction of a turn is rounded to fp32 (at most 2^-25
   of half a turn, 2^-25 pi in the angle), the sine and cosine are within 2
