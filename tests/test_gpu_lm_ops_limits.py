@@ -1,0 +1,58 @@
+"""The language-model operators where their numbers or sizes end: inputs near
+either end of fp32's range, scores that leave nothing of a softmax but its
+greatest, sizes next to a hardware limit, and buffers whose owners let go of them.
+
+Tolerances as in test_gpu_lm_ops.py (u = 2^-24): a score is off by at most 56u of
+sum |q||k| * scale, a probability by as much relative, sums of values by 60u more;
+gradients chain two such products.  Where the scores are of size 8 on average
+over a row that is 510u for an output and three times as much for a gradient.
+"""
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+import lm_reference as R
+from test_gpu_lm_ops import U, Lib, near
+
+pytestmark = pytest.mark.gpu
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+# ---- layer norm ----------------------------------------------------------------------
+
+
+def norm_gradients(*widths):
+    """Forward and gradients of each width in turn, in a process of its own."""
+    from tysor_b200.runtime import CudaContext
+    lib = Lib(CudaContext(0))
+    for width in widths:
+        rows = 3
+        rng = np.random.default_rng(width)
+        x, dy = (rng.standard_normal((rows, width)).astype(np.float32) for _ in range(2))
+        gain = (1 + 0.1 * rng.standard_normal(width)).astype(np.float32)
+        want = R.layer_norm(x, gain, None, 1e-5, dy)
+        bx, bg, by = lib.put(x), lib.put(gain), lib.put(dy)
+        y, stats, dx, dg, db = (lib.zeros(s, 7.0) for s in (x.shape, (rows, 2), x.shape, width, width))
+        lib.ok("layer_norm", bx, bg, None, y, stats, rows, width, 1e-5)
+        lib.ok("layer_norm_backward", bx, bg, stats, by, dx, dg, db, rows, width, False)
+        # A row's mean is near 0 and its spread near 1: 40u of each value, four times that in dx.
+        near(y.read(), want["y"], 120 * U, "y", 1.0)
+        near(dx.read(), want["dx"], 480 * U, "dx", 1.0)
+        near(dg.read(), want["dgain"], 240 * U, "dgain", 1.0)
+        near(db.read(), want["dbias"], 40 * U, "dbias", 1.0)
+    lib.ctx.close()
+
+
+@pytest.mark.parametrize("widths", [(6112, 6144, 6116), (6113, 6143), (6144, 6148), (6145,)],
+                         ids=lambda w: "-".join(map(str, w)))
+def test_layer_norm_gradients_next_to_48_kb(widths):
+    """The column sums of 6113 to 6144 values pass 48 KB of shared memory only
+    together with the kernel's own; what an earlier call of the process asked for
+    must not matter."""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([os.path.dirname(HERE), HERE]))
+    r = subprocess.run([sys.executable, "-c", f"import test_gpu_lm_ops_limits as t; t.norm_gradients(*{widths})"],
+                       cwd=HERE, env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -880,7 +880,9 @@ template <int TPR, int NV, bool VEC>
 void layer_norm_backward_run(const float* x, const float* gain, const float* stats, const float* dy, float* dx,
                              float* partial, int64_t rows, int width, int accumulate, cudaStream_t st) {
   const size_t smem = partial ? sizeof(float) * 2 * (size_t)width : 0;
-  if (smem > 48 * 1024)
+  // 48 KB without the attribute, the kernel's own `red` among them.
+  constexpr size_t kRed = sizeof(float2) * 2 * (512 / TPR) * (TPR / 32);
+  if (smem + kRed > 48 * 1024)
     TYSOR_CUDA(cudaFuncSetAttribute(layer_norm_backward_kernel<TPR, NV, VEC>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
   layer_norm_backward_kernel<TPR, NV, VEC><<<layer_norm_lines(rows, width), 512, smem, st>>>(
