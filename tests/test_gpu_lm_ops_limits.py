@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 
 import lm_reference as R
-from test_gpu_lm_ops import U, Lib, near
+from test_gpu_lm_ops import U, Lib, attention_inputs, lib, near, near_norm, run_attention  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -56,3 +56,34 @@ def test_layer_norm_gradients_next_to_48_kb(widths):
     r = subprocess.run([sys.executable, "-c", f"import test_gpu_lm_ops_limits as t; t.norm_gradients(*{widths})"],
                        cwd=HERE, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# ---- attention -----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dout_size,v_size", [(1e-31, 4.0), (1e-34, 1.0), (1e-3, 1e-31), (4e-16, 4e-16), (1e-24, 1e-12)])
+@pytest.mark.parametrize("dims", [(1, 2, 1, 270, 270, 64), (1, 2, 2, 140, 140, 128)], ids=["64", "128"])
+def test_window_attention_gradients_of_small_values(lib, dims, dout_size, v_size):
+    """dP = dO.V^T far below 1: only the products of both sizes are small, and
+    dq and dk follow them in proportion."""
+    q, k, v, dout = attention_inputs(31, *dims, False)
+    v, dout = v * np.float32(v_size), dout * np.float32(dout_size)
+    scale = dims[5] ** -0.5
+    want = R.window_attention(q, k, v, None, None, 100, 3, scale, False, dout)
+    got = run_attention(lib, q, k, v, dout, None, None, dims, 100, 3, scale, False)
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    for n in ("dq", "dk", "dv"):
+        near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))
+
+
+@pytest.mark.parametrize("size", [1e-16, 1e-18])
+def test_window_attention_of_small_inputs(lib, size):
+    """All inputs small, the scale argument keeping the scores ordinary."""
+    dims = (1, 2, 1, 270, 270, 64)
+    q, k, v, dout = (t * np.float32(size) for t in attention_inputs(11, *dims, False))
+    scale = 64 ** -0.5 / size / size
+    want = R.window_attention(q, k, v, None, None, 100, 3, scale, False, dout)
+    got = run_attention(lib, q, k, v, dout, None, None, dims, 100, 3, scale, False)
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    # dP is about 1e-31 or 1e-35 here: its terms' size counts, as everywhere.
+    for n in ("dq", "dk", "dv"):
+        near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))

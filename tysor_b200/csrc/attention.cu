@@ -90,12 +90,12 @@ __device__ __forceinline__ void lane_load(const float* __restrict__ p, int dim, 
   }
 }
 
-__device__ __forceinline__ void lane_store(float* __restrict__ p, int dim, const float (&v)[kLaneDims], float scale,
+__device__ __forceinline__ void lane_store(float* __restrict__ p, int dim, const float (&v)[kLaneDims],
                                            int accumulate) {
 #pragma unroll
   for (int i = 0; i < kLaneDims; ++i) {
     const int c = (threadIdx.x & 31) + 32 * i;
-    if (c < dim) p[c] = accumulate ? p[c] + v[i] * scale : v[i] * scale;
+    if (c < dim) p[c] = accumulate ? p[c] + v[i] : v[i];
   }
 }
 
@@ -129,7 +129,7 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
     for (int i = 0; i < kLaneDims; ++i) acc[i] = acc[i] * (1.0f - take) + take * kv[i];
     m = top;
   }
-  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, acc, 1.0f, 0);
+  lane_store(out + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, acc, 0);
   if (stats != nullptr && (threadIdx.x & 31) == 0)
     *(float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r)) = make_float2(m, l);
 }
@@ -142,7 +142,7 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
   const int64_t at = row_at(s, b, h, r, s.heads, s.q_len);
   float qv[kLaneDims], gv[kLaneDims], kv[kLaneDims], vv[kLaneDims], acc[kLaneDims] = {};
   if (seen.high == 0) {
-    if (!accumulate) lane_store(dq + at, s.head_dim, acc, 1.0f, 0);
+    if (!accumulate) lane_store(dq + at, s.head_dim, acc, 0);
     return;
   }
   lane_load(out + at, s.head_dim, kv);
@@ -157,9 +157,9 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
     const float p = expf(lane_dot(qv, kv) * s.scale - st.x) / st.y;
     const float ds = p * (lane_dot(gv, vv) - delta);
 #pragma unroll
-    for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * kv[i];
+    for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * (kv[i] * s.scale);  // see `down` in grad_kernel
   }
-  lane_store(dq + at, s.head_dim, acc, s.scale, accumulate);
+  lane_store(dq + at, s.head_dim, acc, accumulate);
 }
 
 // The query rows that see key j: those at positions [j, end).
@@ -195,12 +195,12 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
 #pragma unroll
         for (int i = 0; i < kLaneDims; ++i) {
           av[i] += p * gv[i];
-          ak[i] += ds * qv[i];
+          ak[i] += ds * (qv[i] * s.scale);
         }
       }
   }
-  lane_store(dk + at, s.head_dim, ak, s.scale, accumulate_k);
-  lane_store(dv + at, s.head_dim, av, 1.0f, accumulate_v);
+  lane_store(dk + at, s.head_dim, ak, accumulate_k);
+  lane_store(dv + at, s.head_dim, av, accumulate_v);
 }
 
 // ---- operands of the tensor-core kernels ---------------------------------------------
@@ -247,6 +247,8 @@ struct PackJob {
   // statistics (x is the output's gradient), each row's (greatest score in powers
   // of two, 1 / sum, delta = sum of x * out, norm), zeros for rows that see
   // nothing, and each tile's greatest |delta| (NaN if a row's values are not finite).
+  // Norms and deltas of the output's gradient are in its tile's units, as the packed
+  // values are: however small it is, dP and delta are then of ordinary size.
   float *tile_norm, *norm;
   const float *out, *stats;
   float4* info;
@@ -360,8 +362,8 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     const int item = threadIdx.x + 256 * i;
     const int r = item / kChunks, chunk = item % kChunks;
     if (j.tile_norm != nullptr) {
-      const float back = __uint_as_float((uint32_t)(127 - up) << 23);
-      float q = 0.0f, d = dot[i];
+      const float back = j.out != nullptr ? 1.0f : __uint_as_float((uint32_t)(127 - up) << 23);
+      float q = 0.0f, d = dot[i] * scale;
 #pragma unroll
       for (int e = 0; e < 8; ++e) q += v[i][e] * scale * (v[i][e] * scale);
 #pragma unroll
@@ -1197,7 +1199,8 @@ __global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a) {
 // step's sums, which are added to fp32 registers.  P is at most 1; dS is
 // brought near 2^15 by a power of two from |dS| <= |dO_i| |V_j| + |delta_i|, with
 // the norms of single rows on the resident side and a tile's greatest on the
-// streamed one.
+// streamed one, all in the units of dO's packed tile (its factor, which may be as
+// small as a gradient, only enters where the sums leave tensor memory).
 //   warps 0-7    P and dS: two threads share a row, 32 columns each,
 //   warps 8-15   sums into registers, half of the columns each,
 //   warp 16      copies: resident tiles of the next item, rings of half steps (a
@@ -1251,6 +1254,8 @@ struct GradArgs {
   const float2* col;                   // the same for rows that are streamed
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
+  double scale_power;                  // s.scale as a power of two times a number from 1 to 2: the
+  float scale_rest;                    // power keeps `down` exact below fp32's normal numbers
   Segments seg;
   int* steps;                          // of each unit
   float* part;                         // queries: [unit][128][DP]; keys: [unit][dk, dv][128][DP]
@@ -1628,12 +1633,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
         norm = a.nv[(int64_t)t.row_tile * kTile + row];
       }
       const double to_log2 = (double)(KEYS ? a.fk : a.fq)[t.row_tile] * (double)s.scale * 1.4426950408889634;
-      const float f_row = (KEYS ? a.fv : a.fo)[t.row_tile];
+      const float f_row = KEYS ? a.fv[t.row_tile] : 0.0f;
       for (int n = t.f0; n < t.f1; ++n, ++gi) {
         int step;
         const int tile = column_tile(t, n, &step), c0 = step * kStep;
         const float f = unit_of(to_log2 * (double)(KEYS ? a.fq : a.fk)[tile]);
-        const float f2 = unit_of((double)f_row * (double)(KEYS ? a.fo : a.fv)[tile]);
+        const float f2 = KEYS ? f_row : a.fv[tile];  // of dP and delta in dO's units
         const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
         const float up = power_of_two(scale_exponent(bound));
         bool whole;
@@ -1737,6 +1742,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       if (t.f0 >= t.f1) continue;
       const float4 st = KEYS ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : a.info[(int64_t)t.row_tile * kTile + row];
       const float norm = KEYS ? a.nv[(int64_t)t.row_tile * kTile + row] : st.w;
+      const double unit = a.scale_power * (KEYS ? 1.0 : (double)a.fo[t.row_tile]);
       float acc[kCols], acc_v[kCols];  // acc_v: keys only
 #pragma unroll
       for (int c = 0; c < kCols; ++c) acc[c] = acc_v[c] = 0.0f;
@@ -1744,7 +1750,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
         int step;
         const int tile = column_tile(t, n, &step);
         const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
-        const float down = power_of_two(-scale_exponent(bound)) * (KEYS ? a.fq : a.fk)[tile];
+        // The call's scale goes here: k (or q) times the scale is of a size that fits,
+        // as the scores are, where dS times k alone may not be.
+        const float down = (float)((double)power_of_two(-scale_exponent(bound)) * unit *
+                                   ((double)(KEYS ? a.fq : a.fk)[tile] * (KEYS ? (double)a.fo[tile] : 1.0)));
         if (KEYS) {
           const float down_v = 0x1p-14f * a.fo[tile];
           if (kHalves == 1 || half == 0) take(acc_v, down_v, 0, taken0);
@@ -1757,14 +1766,14 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       const int r = t.r0 + row, cols = s.head_dim - half * kCols;
       if (ok && t.segs > 1) {
         float* dst = a.part + ((int64_t)w * (KEYS ? 2 : 1) * kTile + row) * DP + half * kCols;
-        store_row(dst, acc, s.scale, kCols, true, 0);
+        store_row(dst, acc, a.scale_rest, kCols, true, 0);
         if (KEYS) store_row(dst + kTile * DP, acc_v, 1.0f, kCols, true, 0);
       } else if (ok && KEYS && r < s.k_len) {
         const int64_t at = row_at(s, t.b, t.g, r, s.kv_heads, s.k_len) + half * kCols;
-        store_row(a.dk + at, acc, s.scale, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dk & 15) == 0, a.add_k);
+        store_row(a.dk + at, acc, a.scale_rest, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dk & 15) == 0, a.add_k);
         store_row(a.dv + at, acc_v, 1.0f, cols, s.head_dim % 4 == 0 && ((uintptr_t)a.dv & 15) == 0, a.add_v);
       } else if (ok && !KEYS && r < s.q_len) {
-        store_row(a.dq + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols, acc, s.scale, cols,
+        store_row(a.dq + row_at(s, t.b, t.h, r, s.heads, s.q_len) + half * kCols, acc, a.scale_rest, cols,
                   s.head_dim % 4 == 0 && ((uintptr_t)a.dq & 15) == 0, a.add_q);
       }
       __syncwarp();
@@ -2462,9 +2471,11 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                      {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
                      {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.tnv, w.nv}};
   run_pack(s, jobs, 4, err, st);
+  int scale_exponent;
+  const float scale_rest = 2.0f * frexpf(s.scale, &scale_exponent);
   const GradArgs a{s,     q,     k,     v,      out,   stats, dout, w.pq, w.pk, w.pv,         w.po,         w.fq,         w.fk,
                    w.fv,  w.fo,  w.nv,  w.tnv,  w.tno, w.tdo, w.info, w.col, dq, dk,          dv,           accumulate_q, accumulate_k,
-                   accumulate_v, segments_of(s), w.steps, w.part};
+                   accumulate_v, ldexp(1.0, scale_exponent - 1), scale_rest, segments_of(s), w.steps, w.part};
   if (padded_dim(s) == 64) {
     run_grad<64, false>(a, err, st);
     run_grad<64, true>(a, err, st);
