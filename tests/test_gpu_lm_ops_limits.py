@@ -87,3 +87,17 @@ def test_window_attention_of_small_inputs(lib, size):
     # dP is about 1e-31 or 1e-35 here: its terms' size counts, as everywhere.
     for n in ("dq", "dk", "dv"):
         near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))
+
+
+@pytest.mark.parametrize("dims", [(1, 2, 1, 1, 700, 64), (2, 4, 1, 1, 5000, 128), (1, 9, 1, 1, 900, 33), (1, 2, 1, 3, 600, 64)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_window_attention_of_a_few_rows_over_values_near_the_greatest(lib, dims):
+    """An output is a mean of values, which fits fp32 wherever they do."""
+    q, k, v, _ = attention_inputs(37, *dims, False)
+    k *= np.float32(0.1)  # many keys of similar weight
+    v = np.clip(v, -1, 1) * np.float32(2.0 ** 127)
+    scale = dims[5] ** -0.5
+    want = R.window_attention(q, k, v, None, None, 0, 0, scale, False)
+    got = run_attention(lib, q, k, v, None, None, None, dims, 0, 0, scale, False, backward=False)
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    near(got["stats"][..., 1] / want["stats"][..., 1], np.ones(want["stats"].shape[:-1]), 510 * U, "sums")

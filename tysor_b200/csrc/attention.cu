@@ -1893,14 +1893,24 @@ __device__ __forceinline__ SeenKeys keys_of(const AttentionShape& s, const Seque
   return {first, low, first + z - low};
 }
 
+// A row whose output came out infinite or NaN, key by key: a sum of values near
+// fp32's greatest passes it where their mean does not.
+// (Not inlined: its registers would be the loops'.)
+__device__ __noinline__ void one_row_again(const AttentionShape& s, int start, int n, const float* q, const float* k,
+                                           const float* v, float* out, float* stats, int b, int h, int r) {
+  simple_forward_row(s, {start, n}, q, k, v, out, stats, b, h, r);
+}
+
 template <int NI, int R, bool VEC>
-__global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s, const float* __restrict__ q,
+__global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
                                                                 float* __restrict__ stats, float* __restrict__ part,
                                                                 int sets, int splits, int per, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ __align__(16) float qs[R][kDims];
+  __shared__ uint32_t again;  // rows whose sums have left fp32
+  if (threadIdx.x == 0) again = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
   int64_t index = blockIdx.x;
   const int row0 = (int)(index % sets) * R;
@@ -2112,7 +2122,9 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
     }
     const int64_t line = ((int64_t)b * s.heads + h) * s.q_len + qr;
     if (splits == 1) {
-      out[row_at(s, b, h, qr, s.heads, s.q_len) + c] = sum == 0.0f ? 0.0f : x / sum;
+      const float o = sum == 0.0f ? 0.0f : x / sum;
+      if (!isfinite(o)) atomicOr(&again, 1u << r);
+      out[row_at(s, b, h, qr, s.heads, s.q_len) + c] = o;
       if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = natural_stats(top, sum);
     } else {
       float* dst = part + (line * splits + split) * (s.head_dim + 2);
@@ -2120,18 +2132,25 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(AttentionShape s
       if (c == 0) dst[0] = top, dst[1] = sum;
     }
   }
+  if (splits > 1) return;
+  __syncthreads();
+  for (int r = warp; r < R; r += kWarps)
+    if (again >> r & 1u)
+      one_row_again(s, sq.start, sq.n, q, k, v, out, stats, b, g * group + (row0 + r) / s.q_len, (row0 + r) % s.q_len);
 }
 
 // One block per row joins its splits: each warp takes every fourth, the warps'
 // parts are added in order.
-__global__ void __launch_bounds__(128) decode_join_kernel(AttentionShape s, const float* __restrict__ part,
-                                                          float* __restrict__ out, float* __restrict__ stats,
-                                                          int splits, int per, int* err) {
+__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
+                                                          const float* __restrict__ k, const float* __restrict__ v,
+                                                          const float* __restrict__ part, float* __restrict__ out,
+                                                          float* __restrict__ stats, int splits, int per, int* err) {
   __shared__ float weight[kMostSplits], joined[4][kMaxHeadDim], tops[4], sums[4];
   const int64_t line = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = (int)(line % s.q_len), h = (int)(line / s.q_len % s.heads), b = (int)(line / s.q_len / s.heads);
-  const int used = max(1, (keys_of(s, sequence_of(s, b, err)).count + per - 1) / per);
+  const Sequence sq = sequence_of(s, b, err);
+  const int used = max(1, (keys_of(s, sq).count + per - 1) / per);
   const float* src = part + line * splits * (s.head_dim + 2);
   float top = -INFINITY;
   for (int i = threadIdx.x; i < used; i += 128) top = fmaxf(top, weight[i] = src[(int64_t)i * (s.head_dim + 2)]);
@@ -2156,11 +2175,14 @@ __global__ void __launch_bounds__(128) decode_join_kernel(AttentionShape s, cons
   __syncthreads();
   sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   const int c = threadIdx.x;
+  float o = 0.0f;
   if (c < s.head_dim) {
-    const float o = (joined[0][c] + joined[1][c]) + (joined[2][c] + joined[3][c]);
-    out[row_at(s, b, h, r, s.heads, s.q_len) + c] = sum == 0.0f ? 0.0f : o / sum;
+    o = (joined[0][c] + joined[1][c]) + (joined[2][c] + joined[3][c]);
+    o = sum == 0.0f ? 0.0f : o / sum;
+    out[row_at(s, b, h, r, s.heads, s.q_len) + c] = o;
   }
   if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = natural_stats(top, sum);
+  if (__syncthreads_or(!isfinite(o)) && warp == 0) one_row_again(s, sq.start, sq.n, q, k, v, out, stats, b, h, r);
 }
 
 }  // namespace
@@ -2455,7 +2477,7 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
   }
   if (p.splits > 1) {
     if (rows > INT_MAX) throw CudaError("window_attention: too many rows");
-    decode_join_kernel<<<(unsigned)rows, 128, 0, st>>>(s, work, out, stats, p.splits, p.per, err);
+    decode_join_kernel<<<(unsigned)rows, 128, 0, st>>>(s, q, k, v, work, out, stats, p.splits, p.per, err);
     check_launch();
   }
 }
