@@ -101,3 +101,16 @@ def test_window_attention_of_a_few_rows_over_values_near_the_greatest(lib, dims)
     got = run_attention(lib, q, k, v, None, None, None, dims, 0, 0, scale, False, backward=False)
     near_norm(got["out"], want["out"], 510 * U, "out")
     near(got["stats"][..., 1] / want["stats"][..., 1], np.ones(want["stats"].shape[:-1]), 510 * U, "sums")
+
+
+def test_window_attention_of_many_keys_of_large_values(lib):
+    """Values below 2^100 whose sum over a long cache passes fp32 before the division."""
+    dims = (1, 1, 1, 9, 1 << 15, 64)
+    q, k, v, _ = attention_inputs(41, *dims, False)
+    q *= np.float32(0.01)
+    v = (np.abs(v) % 1 + 1) * np.float32(2.0 ** 99)
+    want = R.window_attention(q, k, v, None, None, 0, 0, 0.125, False)
+    got = run_attention(lib, q, k, v, None, None, None, dims, 0, 0, 0.125, False, backward=False)
+    # Scores of 0.01: what counts is the mean, taken over the keys one by one.  Each
+    # rounds it by at most 2u, with either sign: 2u sqrt(32768 / 3) = 210u together.
+    near_norm(got["out"], want["out"], 510 * U, "out")

@@ -240,7 +240,7 @@ __host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / 
 struct PackJob {
   const float* x;
   uint8_t* tiles;   // [batch][heads][tiles_of(len)] packed tiles
-  float* factors;   // the power of two that undoes each tile's scale; NaN: not for the matrix unit (kFarExponent)
+  float* factors;   // the power of two that undoes each tile's scale; NaN: not for the matrix unit (far_exponent)
   int heads, len, queries;
   // For the gradients (all null otherwise), rows counted in whole tiles: the
   // tile's greatest 2-norm of a row, and the rows' norms; or, with the output and
@@ -256,12 +256,19 @@ struct PackJob {
   float* tile_delta;
 };
 // Tiles with values of 2^100 or more, or that are not finite, go key by key: sums
-// of such values times probabilities of up to 2^14 would leave fp32.
+// of such values times probabilities of up to 2^14 would leave fp32, from 2^13 keys
+// on (which is where a sum of them reaches 2^128) those of fewer powers too.
 constexpr int kFarExponent = 100;
+inline int far_exponent(int keys) {
+  int powers = 0;
+  while (powers < 30 && 1 << powers < keys) ++powers;
+  return std::min(kFarExponent, kFarExponent + 13 - powers);
+}
 struct PackJobs {
   AttentionShape s;
   PackJob job[4];
   int first[5];  // first block of each job
+  int far;       // far_exponent of the call
 };
 
 template <int DP>
@@ -353,7 +360,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   const int up = top == 0 ? 0 : min(14 - exponent, 126);
   const float scale = __uint_as_float((uint32_t)(up + 127) << 23);
   if (threadIdx.x == 0)
-    j.factors[index] = exponent >= kFarExponent ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
+    j.factors[index] = exponent >= p.far ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
   float most_norm = 0.0f;
   uint32_t most_delta = 0;  // as bits: NaN is the greatest
@@ -2326,6 +2333,7 @@ void run_decode_rows(const AttentionShape& s, const DecodePlan& p, const float* 
 void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, cudaStream_t st) {
   PackJobs p{};
   p.s = s;
+  p.far = far_exponent(std::max(s.q_len, s.k_len));
   int64_t at = 0;
   for (int i = 0; i < 4; ++i) {
     p.first[i] = i < count ? (int)at : INT_MAX;
