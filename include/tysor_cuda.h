@@ -266,7 +266,10 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * [batch][length][heads][head_dim].  head_dim 1 to 128, lengths up to 2^29,
  * scale at least 2^-126.  Products carry fp32's accuracy relative to the
  * greatest value among 128 rows of a head; rows that meet values of 2^100 and
- * more, infinities or NaN are computed key by key, many times slower.  The
+ * more (fewer powers over more than 2^13 keys), infinities or NaN, or whose
+ * scores may pass 45000 (by the norms of 128 queries and of 128 keys), are
+ * computed key by key, many times slower; one query of a few over a cache only
+ * where its output would not be finite otherwise.  The
  * call's workspace belongs to the context and grows with the sizes, which frees
  * the old one: a caller that captures the context's stream into a graph calls
  * the largest sizes once before, and lets one such graph run at a time.

@@ -114,3 +114,49 @@ def test_window_attention_of_many_keys_of_large_values(lib):
     # Scores of 0.01: what counts is the mean, taken over the keys one by one.  Each
     # rounds it by at most 2u, with either sign: 2u sqrt(32768 / 3) = 210u together.
     near_norm(got["out"], want["out"], 510 * U, "out")
+
+
+LARGE = [(1, 2, 1, 150, 150, 64, 0, 0), (1, 2, 2, 270, 270, 128, 60, 3), (1, 4, 1, 1, 500, 64, 0, 0), (1, 1, 1, 9, 2000, 80, 0, 0)]
+
+
+@pytest.mark.parametrize("dims", LARGE, ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("size", [300.0, 3000.0, 1e5])
+def test_window_attention_of_scores_that_leave_one_key(lib, dims, size):
+    """Scores from 1e5 to 1e11: each row's greatest takes all the weight (rows whose
+    two greatest lie within 2^-18 of the terms' size are left out of the
+    comparison, what fp32 makes of their scores being either's), its output is
+    that key's value, and the gradients of the scores are 0."""
+    batch, heads, kv_heads, q_len, k_len, dim, window, sinks = dims
+    q, k, v, dout = attention_inputs(43, *dims[:6], False)
+    q, k = q * np.float32(size), k * np.float32(size)
+    scale = dim ** -0.5
+    kk, s = np.repeat(k, heads // kv_heads, 1).astype(np.float64), None
+    s = np.einsum("bhqd,bhkd->bhqk", q.astype(np.float64), kk) * scale
+    terms = np.einsum("bhqd,bhkd->bhqk", np.abs(q).astype(np.float64), np.abs(kk)) * scale
+    s = np.where(R.visible(None, None, batch, q_len, k_len, window, sinks)[:, None], s, -np.inf)
+    two = np.sort(s, -1)[..., -2:] if k_len > 1 else None
+    clear = (two[..., 1] - two[..., 0] > 2.0 ** -18 * terms.max(-1) + 30) | ~np.isfinite(two[..., 0])
+    assert clear.mean() > 0.98
+    dout[~clear] = 0  # and out of the gradients
+    want = R.window_attention(q, k, v, None, None, window, sinks, scale, False, dout)
+    got = run_attention(lib, q, k, v, dout, None, None, dims[:6], window, sinks, scale, False)
+    near_norm(got["out"][clear], want["out"][clear], 64 * U, "out")
+    near((got["stats"][..., 0] / want["stats"][..., 0])[clear], np.ones(int(clear.sum())), 2.0 ** -16, "greatest")
+    near_norm(got["dv"], want["dv"], 3 * 64 * U, "dv")
+    for n in ("dq", "dk"):
+        assert np.isfinite(got[n]).all()
+        near_norm(got[n], want[n], 3 * 64 * U, n, want["size_" + n])
+
+
+def test_window_attention_of_one_large_key(lib):
+    """A key many times larger than the others: rows that see it weigh it alone or
+    not at all, the others are as without it."""
+    dims = (1, 2, 1, 400, 400, 64)
+    q, k, v, dout = attention_inputs(47, *dims, False)
+    k[:, :, 70] *= np.float32(1e7)
+    want = R.window_attention(q, k, v, None, None, 50, 2, 0.125, False, dout)
+    got = run_attention(lib, q, k, v, dout, None, None, dims, 50, 2, 0.125, False)
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    # The terms of dS cancel where one key has all the weight: their own size counts.
+    for n in ("dq", "dk", "dv"):
+        near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))

@@ -24,6 +24,9 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+constexpr int kTile = 128;  // rows of a tile
+__host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
+
 // First value of row `r` of head `h` of sequence `b`.
 __device__ __forceinline__ int64_t row_at(const AttentionShape& s, int b, int h, int r, int heads, int len) {
   return (s.seq_major ? ((int64_t)b * len + r) * heads + h : ((int64_t)b * heads + h) * len + r) * s.head_dim;
@@ -77,7 +80,9 @@ __device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence&
 
 // What is not finite would spoil the hidden places of a matrix product (0 times
 // it is not 0), so rows and keys that meet such values go one by one, taking in
-// only what they see; so do those that see nothing.
+// only what they see; so do those that see nothing, and those whose scores may be
+// so large that a gradient has to form them as the softmax did, bit for bit, for
+// its probabilities to be any (kFarScore).
 
 // A row's values over a warp's lanes: lane l holds columns l, l + 32, ...
 constexpr int kLaneDims = kMaxHeadDim / 32;
@@ -106,6 +111,19 @@ __device__ __forceinline__ float lane_dot(const float (&a)[kLaneDims], const flo
   return warp_sum(d);
 }
 
+// A score, rounded (a multiplication and subtraction in one would not be).
+__device__ __forceinline__ float lane_score(const AttentionShape& s, const float (&q)[kLaneDims],
+                                            const float (&k)[kLaneDims]) {
+  return __fmul_rn(lane_dot(q, k), s.scale);
+}
+
+// The greatest score and the sum of exp(score - greatest) with one more score.
+__device__ __forceinline__ float2 with_score(float2 st, float x) {
+  const float top = x > st.x || x != x ? x : st.x;
+  const float keep = st.x == top ? 1.0f : expf(st.x - top);
+  return make_float2(top, st.y * keep + (x == top && x == -INFINITY ? 0.0f : expf(x - top)));
+}
+
 __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
                                    const float* v, float* out, float* stats, int b, int h, int r) {
   const int g = h / (s.heads / s.kv_heads);
@@ -113,11 +131,12 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
   float qv[kLaneDims] = {}, acc[kLaneDims] = {};
   if (seen.high > 0) lane_load(q + row_at(s, b, h, r, s.heads, s.q_len), s.head_dim, qv);
   float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
   for (int j = 0; j < seen.high; ++j) {
     if (j == seen.first && j < seen.low) j = seen.low;
     float kv[kLaneDims];
     lane_load(k + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, kv);
-    const float x = lane_dot(qv, kv) * s.scale;
+    const float x = lane_score(s, qv, kv);
     const float top = x > m || x != x ? x : m;
     const float keep = m == top ? 1.0f : expf(m - top);
     const float p = x == top && x == -INFINITY ? 0.0f : expf(x - top);
@@ -134,8 +153,10 @@ __device__ void simple_forward_row(const AttentionShape& s, const Sequence& sq, 
     *(float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r)) = make_float2(m, l);
 }
 
+// Leaves the row's greatest score and sum at `own`: those of the scores as formed
+// here and in simple_dkv_row, which the forward's may have formed in another order.
 __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
-                              const float* v, const float* out, const float* stats, const float* dout, float* dq,
+                              const float* v, const float* out, const float* dout, float* dq, float2* own,
                               int accumulate, int b, int h, int r) {
   const int g = h / (s.heads / s.kv_heads);
   const Seen seen = seen_by(s, sq, sq.start + r);
@@ -149,12 +170,20 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
   lane_load(dout + at, s.head_dim, gv);
   lane_load(q + at, s.head_dim, qv);
   const float delta = lane_dot(kv, gv);
-  const float2 st = *(const float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r));
+  float2 st = make_float2(-INFINITY, 0.0f);
+#pragma unroll 1
+  for (int j = 0; j < seen.high; ++j) {
+    if (j == seen.first && j < seen.low) j = seen.low;
+    lane_load(k + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, kv);
+    st = with_score(st, lane_score(s, qv, kv));
+  }
+  if ((threadIdx.x & 31) == 0) *own = st;
+#pragma unroll 1
   for (int j = 0; j < seen.high; ++j) {
     if (j == seen.first && j < seen.low) j = seen.low;
     lane_load(k + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, kv);
     lane_load(v + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, vv);
-    const float p = expf(lane_dot(qv, kv) * s.scale - st.x) / st.y;
+    const float p = expf(lane_score(s, qv, kv) - st.x) / st.y;
     const float ds = p * (lane_dot(gv, vv) - delta);
 #pragma unroll
     for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * (kv[i] * s.scale);  // see `down` in grad_kernel
@@ -171,7 +200,7 @@ __device__ __forceinline__ void rows_seeing(const AttentionShape& s, const Seque
 }
 
 __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, const float* q, const float* k,
-                               const float* v, const float* out, const float* stats, const float* dout, float* dk,
+                               const float* v, const float* out, const float2* stats, const float* dout, float* dk,
                                float* dv, int accumulate_k, int accumulate_v, int b, int g, int j) {
   const int group = s.heads / s.kv_heads;
   const int64_t at = row_at(s, b, g, j, s.kv_heads, s.k_len);
@@ -183,14 +212,15 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
     lane_load(k + at, s.head_dim, kv);
     lane_load(v + at, s.head_dim, vv);
     for (int h = g * group; h < (g + 1) * group; ++h)
+#pragma unroll 1
       for (int r = r0; r < r1; ++r) {
         const int64_t row = row_at(s, b, h, r, s.heads, s.q_len);
         float qv[kLaneDims], gv[kLaneDims], ov[kLaneDims];
         lane_load(q + row, s.head_dim, qv);
         lane_load(dout + row, s.head_dim, gv);
         lane_load(out + row, s.head_dim, ov);
-        const float2 st = *(const float2*)(stats + 2 * (((int64_t)b * s.heads + h) * s.q_len + r));
-        const float p = expf(lane_dot(qv, kv) * s.scale - st.x) / st.y;
+        const float2 st = stats[((int64_t)b * s.heads + h) * tiles_of(s.q_len) * kTile + r];
+        const float p = expf(lane_score(s, qv, kv) - st.x) / st.y;
         const float ds = p * (lane_dot(gv, vv) - lane_dot(gv, ov));
 #pragma unroll
         for (int i = 0; i < kLaneDims; ++i) {
@@ -226,14 +256,18 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
 // query tile that reads a key tile.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kTile = 128;
 constexpr int kBox = kTile * 128;  // bytes
 constexpr uint32_t kLayoutSW128 = 2;
 
 template <int DP>
 constexpr int kTileBytes = 2 * (DP / 64) * kBox;
 
-__host__ __device__ inline int tiles_of(int rows) { return (rows + kTile - 1) / kTile; }
+// Row and key tiles whose scores may reach this many powers of two (by their norms)
+// go key by key: a tile's score is off by up to 28 steps of 2^-23 of them (measured,
+// 2^-22), and a gradient forms it again in another order, so that beside a row's
+// greatest score a probability of 1 comes out as 2^(2^-6) here, and as infinity
+// in fp16 from 2^19 on.
+constexpr float kFarScore = 65536.0f;
 
 // One operand to pack: `heads` heads of `len` rows; rows are keys (valid below
 // the sequence's n) or queries (valid where they stand in the sequence).
@@ -242,9 +276,10 @@ struct PackJob {
   uint8_t* tiles;   // [batch][heads][tiles_of(len)] packed tiles
   float* factors;   // the power of two that undoes each tile's scale; NaN: not for the matrix unit (far_exponent)
   int heads, len, queries;
-  // For the gradients (all null otherwise), rows counted in whole tiles: the
-  // tile's greatest 2-norm of a row, and the rows' norms; or, with the output and
-  // statistics (x is the output's gradient), each row's (greatest score in powers
+  // Null where not wanted: the tile's greatest 2-norm of a row (queries and keys, for
+  // what their scores may come to: at least that, and NaN where the factor is).  For
+  // the gradients, rows counted in whole tiles: the rows' norms as well; or, with
+  // the output and statistics (x is the output's gradient), each row's (greatest score in powers
   // of two, 1 / sum, delta = sum of x * out, norm), zeros for rows that see
   // nothing, and each tile's greatest |delta| (NaN if a row's values are not finite).
   // Norms and deltas of the output's gradient are in its tile's units, as the packed
@@ -252,6 +287,7 @@ struct PackJob {
   float *tile_norm, *norm;
   const float *out, *stats;
   float4* info;
+  float2* own;  // the statistics as they are
   float2* col;  // (greatest score + log2 of the sum - 14, delta); a row that sees nothing: a score no exponent reaches
   float* tile_delta;
 };
@@ -297,6 +333,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     }
     if (j.info != nullptr && threadIdx.x < kTile) {
       j.info[(int64_t)index * kTile + threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      j.own[(int64_t)index * kTile + threadIdx.x] = make_float2(0.0f, 0.0f);
       j.col[(int64_t)index * kTile + threadIdx.x] = make_float2(1e30f, 0.0f);
     }
     if (j.norm != nullptr && threadIdx.x < kTile) j.norm[(int64_t)index * kTile + threadIdx.x] = 0.0f;
@@ -359,8 +396,16 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   const int exponent = (int)(top >> 23) - 127;  // of the largest magnitude; 128: not finite
   const int up = top == 0 ? 0 : min(14 - exponent, 126);
   const float scale = __uint_as_float((uint32_t)(up + 127) << 23);
-  if (threadIdx.x == 0)
-    j.factors[index] = exponent >= p.far ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
+  const float factor = exponent >= p.far ? NAN : __uint_as_float((uint32_t)(127 - up) << 23);
+  // Of queries and keys a bound does unless it, with another tile like this one, comes
+  // near kFarScore: the norms take a sixth of the kernel's time, and few tiles need them.
+  const float bound = exponent >= p.far ? NAN : __uint_as_float((uint32_t)max(exponent + 128, 1) << 23) * sqrtf((float)s.head_dim);
+  const bool for_scores = j.norm == nullptr && j.out == nullptr;
+  const bool norms = j.tile_norm != nullptr && !(for_scores && bound * s.scale * bound * kLog2e < kFarScore / 16.0f);
+  if (threadIdx.x == 0) {
+    j.factors[index] = factor;
+    if (!norms && j.tile_norm != nullptr) j.tile_norm[index] = bound;
+  }
   uint8_t* dst = j.tiles + (int64_t)index * kTileBytes<DP>;
   float most_norm = 0.0f;
   uint32_t most_delta = 0;  // as bits: NaN is the greatest
@@ -368,7 +413,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   for (int i = 0; i < kPer; ++i) {
     const int item = threadIdx.x + 256 * i;
     const int r = item / kChunks, chunk = item % kChunks;
-    if (j.tile_norm != nullptr) {
+    if (norms) {
       const float back = j.out != nullptr ? 1.0f : __uint_as_float((uint32_t)(127 - up) << 23);
       float q = 0.0f, d = dot[i] * scale;
 #pragma unroll
@@ -384,6 +429,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
         if (j.norm != nullptr) j.norm[(int64_t)index * kTile + r] = q;
         if (j.info != nullptr) {
           const float2 st = row_stats[r];
+          j.own[(int64_t)index * kTile + r] = st;
           const float4 f =
               st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(st.x * kLog2e, 1.0f / st.y, d, q);
           j.info[(int64_t)index * kTile + r] = f;
@@ -410,7 +456,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
     *(uint4*)at = hi;
     *(uint4*)(at + (DP / 64) * kBox) = lo;
   }
-  if (j.tile_norm == nullptr) return;
+  if (!norms) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     most_norm = fmaxf(most_norm, __shfl_xor_sync(0xffffffffu, most_norm, o));
@@ -422,7 +468,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   if (threadIdx.x < 2 && (threadIdx.x == 0 || j.tile_delta != nullptr)) {
     uint32_t m = 0;
     for (int w = 0; w < 8; ++w) m = max(m, tops[threadIdx.x][w]);
-    (threadIdx.x == 0 ? j.tile_norm : j.tile_delta)[index] = __uint_as_float(m);
+    (threadIdx.x == 0 ? j.tile_norm : j.tile_delta)[index] = __uint_as_float(m) + (for_scores ? 0.0f * factor : 0.0f);
   }
 }
 
@@ -601,9 +647,9 @@ __device__ __forceinline__ uint32_t bits_between(int lo, int hi, int first) {
 
 // A row's statistics in natural units from its reference exponent (in powers
 // of two) and sum.  The sum takes up what rounding the exponent loses, so that
-// exp(score - greatest) / sum stays consistent.
+// exp(score - greatest) / sum stays consistent (past kFarScore no gradient uses it).
 __device__ __forceinline__ float2 natural_stats(float top, float sum) {
-  if (top == -INFINITY) return make_float2(-INFINITY, sum);
+  if (!(fabsf(top) < kFarScore)) return make_float2(top == -INFINITY ? top : top * kLn2, sum);
   const float m = top * kLn2;
   return make_float2(m, sum * exp2f(top - m * kLog2e));
 }
@@ -708,6 +754,7 @@ struct ForwardArgs {
   const float *q, *k, *v;
   const uint8_t *pq, *pk, *pv;
   const float *fq, *fk, *fv;
+  const float *tnq, *tnk;  // greatest norms of the query and key tiles' rows
   float *out, *stats;
   int segs;         // segments of each item's key tiles
   int* steps;       // segs > 1: key tiles of each unit
@@ -717,7 +764,7 @@ struct ForwardArgs {
 
 // Work item `index`: 128 rows of a head, those that see the most keys first.
 struct QueryItem {
-  int b, h, g, r0, n;  // n: key tiles to walk; 0: none, or values that are not finite
+  int b, h, g, r0, n;  // n: key tiles to walk; 0: none, or not for the matrix unit
   int f0, f1;          // the unit's segment of them
   bool first;          // the first segment
   Sequence sq;
@@ -745,12 +792,15 @@ __device__ __forceinline__ QueryItem query_item(const ForwardArgs& a, int unit, 
   t.range = keys_for(s, t.sq, t.rows);
   t.q_index = (t.b * s.heads + t.h) * tiles_of(s.q_len) + t.r0 / kTile;
   t.k_index = (t.b * s.kv_heads + t.g) * tiles_of(s.k_len);
-  float sum = a.fq[t.q_index];
-  for (int i = threadIdx.x & 31; i < t.range.count; i += 32)
-    sum += a.fk[t.k_index + t.range.at(i)] + a.fv[t.k_index + t.range.at(i)];
+  const float norm = a.tnq[t.q_index] * s.scale * kLog2e;
+  bool far = false;
+  for (int i = threadIdx.x & 31; i < t.range.count; i += 32) {
+    const int k = t.k_index + t.range.at(i);
+    far |= !(norm * a.tnk[k] + 0.0f * a.fv[k] < kFarScore);
+  }
   // A product with a hidden value that is not finite would not be 0: such
   // rows go key by key instead.
-  t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  t.n = __any_sync(0xffffffffu, far) ? 0 : t.range.count;
   const int each = (t.n + a.segs - 1) / a.segs;
   t.f0 = min(t.n, seg * each);
   t.f1 = min(t.n, t.f0 + each);
@@ -1253,12 +1303,14 @@ struct Segments {
 
 struct GradArgs {
   AttentionShape s;
-  const float *q, *k, *v, *out, *stats, *dout;
+  const float *q, *k, *v, *out, *dout;
   const uint8_t *pq, *pk, *pv, *po;
   const float *fq, *fk, *fv, *fo;      // factors
+  const float *tnq, *tnk;              // greatest norms of Q's and K's tiles' rows
   const float *nv, *tnv, *tno, *tdo;   // norms of V's rows; greatest norm of V's and dO's tiles, greatest |delta|
   const float4* info;                  // of query rows
   const float2* col;                   // the same for rows that are streamed
+  float2* own;                         // statistics for what goes key by key
   float *dq, *dk, *dv;
   int add_q, add_k, add_v;
   double scale_power;                  // s.scale as a power of two times a number from 1 to 2: the
@@ -1283,7 +1335,7 @@ struct GradPlan {
 
 // 128 rows of one head and the steps of 64 columns they need.
 struct GradItem {
-  int b, h, g, r0, n;  // h: the queries' head, or the first of the keys'; n: steps (keys: per head); 0: none, or values not finite
+  int b, h, g, r0, n;  // h: the queries' head, or the first of the keys'; n: steps (keys: per head); 0: none, or not for the matrix unit
   Sequence sq;
   RowRange rows;       // queries
   TileRange range;     // in steps of 64
@@ -1326,7 +1378,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
   const int tiles_q = tiles_of(s.q_len), tiles_k = tiles_of(s.k_len);
   int seg;
   GradItem t = grad_place<KEYS>(a, index, &seg);
-  float sum;
+  bool far = false;  // or not finite
   if (!KEYS) {
     t.sq = sequence_of(s, t.b, err);
     t.rows = rows_of(s, t.sq, t.r0);
@@ -1336,11 +1388,12 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     t.range.low = low / kStep;
     t.range.sinks = min((min(s.sinks, low) + kStep - 1) / kStep, t.range.low);
     t.range.count = x > z ? 0 : t.range.sinks + z / kStep - t.range.low + 1;
-    sum = a.fq[t.row_tile] + a.fo[t.row_tile];
+    const float norm = a.tnq[t.row_tile] * s.scale * kLog2e + 0.0f * a.fo[t.row_tile];
     const int first = (t.b * s.kv_heads + t.g) * tiles_k;
+#pragma unroll 1
     for (int i = lane; i < t.range.count; i += 32) {
       const int k = first + t.range.at(i) / 2;
-      sum += a.fk[k] + a.fv[k];
+      far |= !(norm * a.tnk[k] + 0.0f * a.fv[k] < kFarScore);
     }
   } else {
     t.sq = sequence_of(s, t.b, err);
@@ -1355,13 +1408,14 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
     t.range.sinks = 0;
     t.range.low = x / kStep;
     t.range.count = t.r0 >= t.sq.n || x > z ? 0 : z / kStep - t.range.low + 1;
-    sum = a.fk[t.row_tile] + a.fv[t.row_tile];
+    const float norm = a.tnk[t.row_tile] * s.scale * kLog2e + 0.0f * a.fv[t.row_tile];
+#pragma unroll 1
     for (int i = lane; i < t.range.count * group; i += 32) {
       const int q = (t.b * s.heads + t.h + i / t.range.count) * tiles_q + t.range.at(i % t.range.count) / 2;
-      sum += a.fq[q] + a.fo[q] + a.tdo[q] * 0.0f;
+      far |= !(norm * a.tnq[q] + 0.0f * (a.fo[q] + a.tdo[q]) < kFarScore);
     }
   }
-  t.n = __any_sync(0xffffffffu, sum != sum) ? 0 : t.range.count;
+  t.n = __any_sync(0xffffffffu, far) ? 0 : t.range.count;
   const int total = (KEYS ? group : 1) * t.n, each = (total + t.segs - 1) / t.segs;
   t.f0 = min(total, seg * each);
   t.f1 = min(total, t.f0 + each);
@@ -1443,8 +1497,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       const GradItem t = grad_item<KEYS>(a, w, err);
       if (t.n != 0 || !t.first) continue;
       for (int r = t.r0 + warp - 18; r < min(t.r0 + kTile, KEYS ? s.k_len : s.q_len); r += 2) {
-        if (!KEYS) simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dq, a.add_q, t.b, t.h, r);
-        else simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.stats, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
+        if (!KEYS)
+          simple_dq_row(s, t.sq, a.q, a.k, a.v, a.out, a.dout, a.dq,
+                        a.own + (int64_t)t.row_tile * kTile + (r - t.r0), a.add_q, t.b, t.h, r);
+        else simple_dkv_row(s, t.sq, a.q, a.k, a.v, a.out, a.own, a.dout, a.dk, a.dv, a.add_k, a.add_v, t.b, t.g, r);
       }
     }
   } else if (warp == 16) {
@@ -2224,7 +2280,7 @@ int padded_dim(const AttentionShape& s) { return s.head_dim <= 64 ? 64 : 128; }
 
 struct ForwardWork {
   uint8_t *pq, *pk, *pv;
-  float *fq, *fk, *fv, *part;
+  float *fq, *fk, *fv, *tnq, *tnk, *part;
   float2* part_ml;
   int *steps, segs;
   int64_t floats;
@@ -2258,6 +2314,8 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   w.fq = c.take(nq);
   w.fk = c.take(nk);
   w.fv = c.take(nk);
+  w.tnq = c.take(nq);
+  w.tnk = c.take(nk);
   w.segs = segments_of_queries(s, 4);
   w.part = c.take(w.segs > 1 ? nq * w.segs * kTile * padded_dim(s) : 0);
   w.part_ml = (float2*)c.take(w.segs > 1 ? nq * w.segs * kTile * 2 : 0);
@@ -2349,9 +2407,9 @@ void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, 
 
 struct GradWork {
   uint8_t *pq, *pk, *pv, *po;
-  float *fq, *fk, *fv, *fo, *nv, *tnv, *tno, *tdo;
+  float *fq, *fk, *fv, *fo, *tnq, *tnk, *nv, *tnv, *tno, *tdo;
   float4* info;
-  float2* col;
+  float2 *col, *own;
   int* steps;
   float* part;
   int64_t floats;
@@ -2398,12 +2456,15 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.fo = c.take(nq);
   w.fk = c.take(nk);
   w.fv = c.take(nk);
+  w.tnq = c.take(nq);
+  w.tnk = c.take(nk);
   w.nv = c.take(nk * kTile);
   w.tnv = c.take(nk);
   w.tno = c.take(nq);
   w.tdo = c.take(nq);
   w.info = (float4*)c.take(nq * kTile * 4);
   w.col = (float2*)c.take(nq * kTile * 2);
+  w.own = (float2*)c.take(nq * kTile * 2);
   const Segments g = segments_of(s);
   // The queries' pass has joined its segments when the keys' begins.
   const int64_t for_keys = g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 : 0;
@@ -2467,11 +2528,11 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
   if (rows <= 0) return;
   if (uses_tiles(s)) {
     const ForwardWork w = forward_work(s, work);
-    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
-                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
+    PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1, w.tnq},
+                       {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, w.tnk},
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0}};
     run_pack(s, jobs, 3, err, st);
-    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, out, stats, w.segs, w.steps, w.part, w.part_ml};
+    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, w.tnq, w.tnk, out, stats, w.segs, w.steps, w.part, w.part_ml};
     if (padded_dim(s) == 64) run_forward<64>(a, err, st);
     else run_forward<128>(a, err, st);
     return;
@@ -2496,16 +2557,16 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                                       int* err, cudaStream_t st) {
   if (s.batch == 0 || (s.q_len == 0 && s.k_len == 0)) return;
   const GradWork w = grad_work(s, work);
-  PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1},
-                     {dout, w.po, w.fo, s.heads, s.q_len, 1, w.tno, nullptr, out, stats, w.info, w.col, w.tdo},
-                     {k, w.pk, w.fk, s.kv_heads, s.k_len, 0},
+  PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1, w.tnq},
+                     {dout, w.po, w.fo, s.heads, s.q_len, 1, w.tno, nullptr, out, stats, w.info, w.own, w.col, w.tdo},
+                     {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, w.tnk},
                      {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.tnv, w.nv}};
   run_pack(s, jobs, 4, err, st);
   int scale_exponent;
   const float scale_rest = 2.0f * frexpf(s.scale, &scale_exponent);
-  const GradArgs a{s,     q,     k,     v,      out,   stats, dout, w.pq, w.pk, w.pv,         w.po,         w.fq,         w.fk,
-                   w.fv,  w.fo,  w.nv,  w.tnv,  w.tno, w.tdo, w.info, w.col, dq, dk,          dv,           accumulate_q, accumulate_k,
-                   accumulate_v, ldexp(1.0, scale_exponent - 1), scale_rest, segments_of(s), w.steps, w.part};
+  const GradArgs a{s,     q,     k,      v,     out,   dout,  w.pq,  w.pk,  w.pv,  w.po,   w.fq,  w.fk, w.fv, w.fo,
+                   w.tnq, w.tnk, w.nv,   w.tnv, w.tno, w.tdo, w.info, w.col, w.own, dq,     dk,    dv,   accumulate_q,
+                   accumulate_k, accumulate_v, ldexp(1.0, scale_exponent - 1), scale_rest, segments_of(s), w.steps, w.part};
   if (padded_dim(s) == 64) {
     run_grad<64, false>(a, err, st);
     run_grad<64, true>(a, err, st);
