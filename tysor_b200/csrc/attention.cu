@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "lm_ops.cuh"
 #include "tcgen05.cuh"
@@ -1964,7 +1965,10 @@ __device__ __noinline__ void one_row_again(const AttentionShape& s, int start, i
   simple_forward_row(s, {start, n}, q, k, v, out, stats, b, h, r);
 }
 
-template <int NI, int R, bool VEC>
+// WHOLE: the keys are in one part, and this kernel writes the output.  (A kernel of
+// its own: with a call of one_row_again in it the loops of the others take longer,
+// 87 us instead of 85 for four sequences of up to 32768 keys.)
+template <int NI, int R, bool VEC, bool WHOLE>
 __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
@@ -1972,8 +1976,8 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_con
                                                                 int sets, int splits, int per, int* err) {
   constexpr int kDims = 32 * NI, kWarps = kDecodeThreads / 32;
   __shared__ __align__(16) float qs[R][kDims];
-  __shared__ uint32_t again;  // rows whose sums have left fp32
-  if (threadIdx.x == 0) again = 0;
+  __shared__ uint32_t again;  // WHOLE: rows whose sums have left fp32
+  if (WHOLE && threadIdx.x == 0) again = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, key_of = warp * 4 + (lane >> 3);
   int64_t index = blockIdx.x;
   const int row0 = (int)(index % sets) * R;
@@ -1986,7 +1990,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_con
   const SeenKeys seen = keys_of(s, sq);
   const int first = seen.first, low = seen.low, keys = seen.count;
   const int u0 = min(keys, split * per), u1 = min(keys, u0 + per);
-  if (splits > 1 && u0 == u1 && split > 0) return;  // the join knows how many splits hold keys
+  if (!WHOLE && u0 == u1 && split > 0) return;  // the join knows how many splits hold keys
   const float to_log2 = s.scale * kLog2e;
   for (int i = threadIdx.x; i < R * kDims; i += kDecodeThreads) {
     const int r = row0 + i / kDims, c = i % kDims;
@@ -2184,7 +2188,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_con
       x += joined[w][r][c] * one;
     }
     const int64_t line = ((int64_t)b * s.heads + h) * s.q_len + qr;
-    if (splits == 1) {
+    if (WHOLE) {
       const float o = sum == 0.0f ? 0.0f : x / sum;
       if (!isfinite(o)) atomicOr(&again, 1u << r);
       out[row_at(s, b, h, qr, s.heads, s.q_len) + c] = o;
@@ -2195,10 +2199,10 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_con
       if (c == 0) dst[0] = top, dst[1] = sum;
     }
   }
-  if (splits > 1) return;
+  if (!WHOLE) return;
   __syncthreads();
   for (int r = warp; r < R; r += kWarps)
-    if (again >> r & 1u)
+    if (WHOLE && again >> r & 1u)
       one_row_again(s, sq.start, sq.n, q, k, v, out, stats, b, g * group + (row0 + r) / s.q_len, (row0 + r) % s.q_len);
 }
 
@@ -2363,7 +2367,7 @@ int64_t decode_work_elems(const AttentionShape& s) {
   return (int64_t)s.batch * s.heads * s.q_len * p.splits * (s.head_dim + 2);
 }
 
-template <int NI, int R>
+template <int NI, int R, bool WHOLE>
 void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v, float* out,
                 float* stats, float* part, int* err, cudaStream_t st) {
   const int64_t blocks = (int64_t)s.batch * s.kv_heads * p.sets * p.splits;
@@ -2373,19 +2377,23 @@ void run_decode(const AttentionShape& s, const DecodePlan& p, const float* q, co
   constexpr int kJoined = kDecodeThreads / 32 * R * (32 * NI + 2) * (int)sizeof(float);  // below 48 KB
   static_assert(kJoined <= kRing, "the ring holds the results");
   static std::atomic<uint64_t> done{0};
-  if (vec) allow_shared(decode_kernel<NI, R, true>, kRing, done);
+  if (vec) allow_shared(decode_kernel<NI, R, true, WHOLE>, kRing, done);
   if (vec)
-    decode_kernel<NI, R, true><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
+    decode_kernel<NI, R, true, WHOLE><<<(unsigned)blocks, kDecodeThreads, kRing, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
   else
-    decode_kernel<NI, R, false><<<(unsigned)blocks, kDecodeThreads, kJoined, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
+    decode_kernel<NI, R, false, WHOLE><<<(unsigned)blocks, kDecodeThreads, kJoined, st>>>(s, q, k, v, out, stats, part, p.sets, p.splits, p.per, err);
   check_launch();
 }
 template <int NI>
 void run_decode_rows(const AttentionShape& s, const DecodePlan& p, const float* q, const float* k, const float* v,
                      float* out, float* stats, float* part, int* err, cudaStream_t st) {
-  if (p.rows == 1) run_decode<NI, 1>(s, p, q, k, v, out, stats, part, err, st);
-  else if (p.rows == 4) run_decode<NI, 4>(s, p, q, k, v, out, stats, part, err, st);
-  else run_decode<NI, kDecodeRows>(s, p, q, k, v, out, stats, part, err, st);
+  auto run = [&](auto whole) {
+    if (p.rows == 1) run_decode<NI, 1, whole.value>(s, p, q, k, v, out, stats, part, err, st);
+    else if (p.rows == 4) run_decode<NI, 4, whole.value>(s, p, q, k, v, out, stats, part, err, st);
+    else run_decode<NI, kDecodeRows, whole.value>(s, p, q, k, v, out, stats, part, err, st);
+  };
+  if (p.splits == 1) run(std::true_type{});
+  else run(std::false_type{});
 }
 
 void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, cudaStream_t st) {
