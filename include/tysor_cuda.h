@@ -273,9 +273,11 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * call's workspace belongs to the context and grows with the sizes, which frees
  * the old one: a caller that captures the context's stream into a graph calls
  * the largest sizes once before, and lets one such graph run at a time.
- * starts [batch] may be NULL (k_len - q_len: the queries end where the keys end), lengths
- * [batch] may be NULL (k_len); both hold whole numbers as floats, checked on
- * the device ("Attention start or length out of range").  stats may be NULL
+ * starts [batch] may be NULL (k_len - q_len: the queries end where k_len ends, also
+ * in a sequence whose length is less, whose rows from there on see nothing),
+ * lengths [batch] may be NULL (k_len); both hold whole numbers as floats (beyond
+ * 2^24 only those that fp32 holds), checked on the device ("Attention start or
+ * length out of range"; the sequence then counts as empty).  stats may be NULL
  * or receives [batch][heads][q_len][2] = (greatest visible score, sum of
  * exp(score - greatest)), (-inf, 0) for a row that sees nothing; the backward
  * reads it.  Serving calls it with q_len 1 and starts = lengths - 1. */

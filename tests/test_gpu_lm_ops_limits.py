@@ -160,3 +160,21 @@ def test_window_attention_of_one_large_key(lib):
     # The terms of dS cancel where one key has all the weight: their own size counts.
     for n in ("dq", "dk", "dv"):
         near_norm(got[n], want[n], 3 * 510 * U, n, want.get("size_" + n, np.zeros(1)))
+
+
+@pytest.mark.parametrize("dims", [(2, 2, 1, 20, 20, 32), (2, 4, 1, 1, 30, 64)], ids=["tiles", "one"])
+def test_window_attention_of_lengths_that_are_not_whole(lib, dims):
+    batch, heads, kv_heads, q_len, k_len, dim = dims
+    q, k, v, dout = attention_inputs(5, *dims, False)
+    clean = run_attention(lib, q, k, v, dout, None, None, dims, 8, 0, 0.2, False, backward=False)
+    first = float(k_len - q_len)
+    for starts, lengths in (([first, first], [k_len, k_len - 0.5]), ([first, -0.5], [k_len, k_len]),
+                            ([first, 0.25], [k_len, k_len]), ([first, first], [k_len, 1e-30])):
+        bufs = [lib.put(t) for t in (q, k, v)]
+        out = lib.zeros(q.shape, 5.0)
+        lib.ok("window_attention", *bufs, lib.put(np.float32(starts)), lib.put(np.float32(lengths)), out, None, *dims,
+               8, 0, 0.2, False)
+        with pytest.raises(lib.native.NativeError, match="start or length out of range"):
+            lib.ctx.synchronize()
+        got = out.read().reshape(q.shape)
+        assert np.array_equal(got[0], clean["out"][0]) and not got[1].any()

@@ -33,7 +33,7 @@ __device__ __forceinline__ int64_t row_at(const AttentionShape& s, int b, int h,
   return (s.seq_major ? ((int64_t)b * len + r) * heads + h : ((int64_t)b * heads + h) * len + r) * s.head_dim;
 }
 
-// A sequence's keys [0, n) and its first query's position.
+// A sequence's keys [0, n) and its first query's position, both whole numbers.
 struct Sequence {
   int start, n;
 };
@@ -42,7 +42,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionShape& s, int b, 
   Sequence q{s.k_len - s.q_len, s.k_len};
   if (s.lengths != nullptr) {
     const float v = s.lengths[b];
-    if (v >= 0.0f && v <= (float)s.k_len && (int64_t)v <= s.k_len) {
+    if (v >= 0.0f && v <= (float)s.k_len && (int64_t)v <= s.k_len && v == truncf(v)) {
       q.n = (int)v;
     } else {
       q.n = 0;
@@ -51,7 +51,7 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionShape& s, int b, 
   }
   if (s.starts != nullptr) {
     const float v = s.starts[b];
-    if (v > -536870912.0f && v < 536870912.0f) {  // positions stay below 2^30
+    if (v > -536870912.0f && v < 536870912.0f && v == truncf(v)) {  // positions stay below 2^30
       q.start = (int)v;
     } else {
       q.n = 0;
