@@ -178,3 +178,20 @@ def test_window_attention_of_lengths_that_are_not_whole(lib, dims):
             lib.ctx.synchronize()
         got = out.read().reshape(q.shape)
         assert np.array_equal(got[0], clean["out"][0]) and not got[1].any()
+
+
+@pytest.mark.parametrize("dims", [(2, 4, 2, 257, 257, 64, 60, 2), (1, 2, 1, 5, 3000, 128, 0, 0), (2, 8, 2, 1, 1500, 64, 0, 0),
+                                  (1, 2, 1, 700, 700, 128, 0, 0)], ids=lambda c: "x".join(map(str, c)))
+def test_window_attention_statistics(lib, dims):
+    """The greatest score and the sum apart: the one is off by at most 56u of the
+    terms of a score, the other by as much relative twice (the greatest's and the
+    others'), and the sum's 60u."""
+    batch, heads, kv_heads, q_len, k_len, dim, window, sinks = dims
+    q, k, v, _ = attention_inputs(53, *dims[:6], False)
+    scale = dim ** -0.5
+    want = R.window_attention(q, k, v, None, None, window, sinks, scale, False)["stats"]
+    got = run_attention(lib, q, k, v, None, None, None, dims[:6], window, sinks, scale, False, backward=False)["stats"]
+    kk = np.repeat(np.abs(k), heads // kv_heads, 1).astype(np.float64)
+    terms = (np.einsum("bhqd,bhkd->bhqk", np.abs(q).astype(np.float64), kk) * scale).max(-1)
+    assert np.all(np.abs(got[..., 0] - want[..., 0]) <= 56 * U * terms + 2 * U * np.abs(want[..., 0]))
+    assert np.all(np.abs(got[..., 1] / want[..., 1] - 1) <= 2 * 56 * U * terms + 60 * U)
