@@ -86,7 +86,8 @@ bool tysor_cuda_buffer_write(void* buffer, const float* data, size_t count);
 void* tysor_cuda_buffer_view(void* base, size_t offset, size_t count);
 /* A buffer over `count` floats of device memory that the caller owns (another
  * library's tensor): on the context's device, kept alive by the caller until
- * the buffer is freed, which leaves the memory as it is.  Dispatches run on
+ * the buffer is freed, which waits for the context's stream and leaves the
+ * memory as it is.  Buffers are freed before their context.  Dispatches run on
  * the context's stream: a caller that writes or reads the memory on another
  * stream orders the two (tysor_cuda_context_stream).  No reference
  * counterpart. */

@@ -195,3 +195,26 @@ def test_window_attention_statistics(lib, dims):
     terms = (np.einsum("bhqd,bhkd->bhqk", np.abs(q).astype(np.float64), kk) * scale).max(-1)
     assert np.all(np.abs(got[..., 0] - want[..., 0]) <= 56 * U * terms + 2 * U * np.abs(want[..., 0]))
     assert np.all(np.abs(got[..., 1] / want[..., 1] - 1) <= 2 * 56 * U * terms + 60 * U)
+
+
+# ---- memory --------------------------------------------------------------------------
+
+
+def stream_of(lib):
+    import torch
+    return torch.cuda.ExternalStream(lib.lib.tysor_cuda_context_stream(lib.ctx.handle))
+
+
+def test_a_wrapped_buffer_is_freed_after_its_last_use(lib):
+    """Its owner may give the memory back as soon as the buffer is gone."""
+    import torch
+    x, y = (torch.ones(16384, 2048, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    bx, by = (lib.Buffer.wrap(lib.ctx, t) for t in (x, y))
+    for free in (bx.free, by.free):
+        again = [lib.Buffer.wrap(lib.ctx, t) for t in (x, y)]
+        for _ in range(200):  # 45 us each
+            lib.ok("layer_norm", again[0], None, None, again[1], None, 16384, 2048, 1e-5)
+        assert not stream_of(lib).query()
+        free()
+        assert stream_of(lib).query()

@@ -386,10 +386,14 @@ void* tysor_cuda_buffer_new_with_data(void* context, const float* data, size_t c
 void tysor_cuda_buffer_free(void* buffer) {
   if (!buffer) return;
   Buffer* b = static_cast<Buffer*>(buffer);
-  if (b->owned && b->ptr) {
+  if ((b->owned || b->wrapped) && b->ptr) {
     cudaSetDevice(b->ctx->device);
-    cudaStreamSynchronize(b->ctx->stream);
-    cudaFree(b->ptr);
+    // What is under way may use the memory, which goes back to its allocator here:
+    // the library's, or the caller's.  (A capture is not under way, and no wait for it.)
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    cudaStreamIsCapturing(b->ctx->stream, &capture);
+    if (b->owned || capture == cudaStreamCaptureStatusNone) cudaStreamSynchronize(b->ctx->stream);
+    if (b->owned) cudaFree(b->ptr);
   }
   delete b;
 }
@@ -442,6 +446,7 @@ void* tysor_cuda_buffer_wrap(void* context, float* data, size_t count) {
     b->ctx = c;
     b->ptr = data;
     b->count = count;
+    b->wrapped = true;
     out = b;
   });
   return out;

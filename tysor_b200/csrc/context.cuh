@@ -52,6 +52,7 @@ struct Buffer {
   float* ptr = nullptr;
   size_t count = 0;
   bool owned = false;
+  bool wrapped = false;  // the caller's memory
 };
 
 const char* device_error_message(int code);
