@@ -247,7 +247,9 @@ bool tysor_cuda_dispatch_layer_norm_backward(void* context, void* input, void* g
  * as in rope) turns by positions[b][axis][s] * theta^(-i / half), `axis` the
  * one whose section holds i; positions is [batch][axes][seq_len].  With equal
  * positions 0, 1, 2, ... on every axis this is rope.  Angles are formed in
- * 64 bits. */
+ * 64 bits.  The first call of a (half, theta) makes a table that the context
+ * keeps, which a capture of its stream into a graph refuses (rope's too): make
+ * the call once before. */
 bool tysor_cuda_dispatch_rope_axes(void* context, void* input, void* positions, void* out, uint32_t batch,
                                    uint32_t heads, uint32_t seq_len, const int64_t* sections, int axes,
                                    double theta, bool seq_major);

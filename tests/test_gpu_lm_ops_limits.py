@@ -218,3 +218,55 @@ def test_a_wrapped_buffer_is_freed_after_its_last_use(lib):
         assert not stream_of(lib).query()
         free()
         assert stream_of(lib).query()
+
+
+def rope_inputs(lib, seed, sections=(8, 8)):
+    rng = np.random.default_rng(seed)
+    half = sum(sections)
+    x = rng.standard_normal((1, 2, 40, 2 * half)).astype(np.float32)
+    pos = rng.integers(0, 900, (1, len(sections), 40)).astype(np.float32)
+    keep = np.asarray(sections, np.int64)
+    return x, pos, keep, (lib.put(x), lib.put(pos)), lib.zeros(x.shape)
+
+
+def test_rope_tables_come_in_the_order_of_their_stream(lib):
+    """The first call of a theta copies its table on the context's own stream: it
+    neither waits for the caller's nor could be overtaken by the kernel."""
+    import torch
+    x, pos, keep, ins, y = rope_inputs(lib, 61)
+    caller = torch.cuda.default_stream()
+    waits = []
+    for i in range(4):
+        theta = 777.0 + i
+        with torch.cuda.stream(caller):
+            torch.cuda._sleep(1_000_000_000)  # half a second
+        lib.ok("rope_axes", *ins, y, 1, 2, 40, keep.ctypes.data_as(lib.native.I64P), 2, theta, False)
+        lib.ok("rope", ins[0], y, 2, 40, 16, theta)
+        waits.append(caller.query())
+        caller.synchronize()
+    assert not any(waits[1:])  # the first call also loads its kernels, which waits for all streams
+    lib.ok("rope_axes", *ins, y, 1, 2, 40, keep.ctypes.data_as(lib.native.I64P), 2, 778.0, False)
+    size = float(np.sqrt(x[..., :16].astype(np.float64) ** 2 + x[..., 16:].astype(np.float64) ** 2).max())
+    near(y.read(), R.rope_axes(x, pos, (8, 8), 778.0, False), 8 * U, "y", size)
+
+
+def test_rope_tables_in_a_capture(lib):
+    """A call that would have to make its table is refused, and the capture goes on."""
+    import torch
+    x, pos, keep, ins, y = rope_inputs(lib, 67)
+    args = (*ins, y, 1, 2, 40, keep.ctypes.data_as(lib.native.I64P), 2)
+    lib.ok("rope_axes", *args, 900.0, False)
+    want = y.read()
+    lib.ctx.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream_of(lib)):
+        graph.capture_begin()
+        lib.refused("while the context's stream is captured", "rope_axes", *args, 901.0, False)
+        lib.refused("while the context's stream is captured", "rope", ins[0], y, 2, 40, 16, 901.0)
+        lib.ok("rope_axes", *args, 900.0, False)
+        graph.capture_end()
+        y.write(np.zeros(want.size, np.float32))
+        graph.replay()
+    assert np.array_equal(y.read(), want)
+    lib.ok("rope_axes", *args, 901.0, False)
+    del graph

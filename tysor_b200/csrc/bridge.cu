@@ -45,6 +45,26 @@ void* Context::ensure_scratch(size_t bytes) {
   return scratch;
 }
 
+bool Context::capturing() const {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  TYSOR_CUDA(cudaStreamIsCapturing(stream, &status));
+  return status != cudaStreamCaptureStatusNone;
+}
+
+void* Context::new_table(const void* host, size_t bytes) {
+  if (capturing())
+    throw CudaError("rope's table of these sizes cannot be made while the context's stream is captured: "
+                    "make the call once before");
+  void* d = nullptr;
+  TYSOR_CUDA(cudaMalloc(&d, bytes));
+  // On the stream whose kernels read it, which waits for no other stream's copies.
+  cudaError_t e = cudaMemcpyAsync(d, host, bytes, cudaMemcpyHostToDevice, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  if (e != cudaSuccess) cudaFree(d);
+  TYSOR_CUDA(e);
+  return d;
+}
+
 const float2* Context::rope_table(int64_t seq, int64_t half, double theta) {
   uint64_t bits;
   std::memcpy(&bits, &theta, sizeof bits);
@@ -62,9 +82,7 @@ const float2* Context::rope_table(int64_t seq, int64_t half, double theta) {
       volatile float ang = (float)p * inv[i];
       tab[p * half + i] = make_float2(cosf(ang), sinf(ang));
     }
-  float2* d = nullptr;
-  TYSOR_CUDA(cudaMalloc(&d, sizeof(float2) * tab.size()));
-  TYSOR_CUDA(cudaMemcpy(d, tab.data(), sizeof(float2) * tab.size(), cudaMemcpyHostToDevice));
+  auto* d = (const float2*)new_table(tab.data(), sizeof(float2) * tab.size());
   rope_tables[key] = d;
   return d;
 }
@@ -77,9 +95,7 @@ const double* Context::rope_rate_table(int64_t half, double theta) {
   if (it != rope_rates.end()) return it->second;
   std::vector<double> rate((size_t)half);
   for (int64_t i = 0; i < half; ++i) rate[i] = pow(theta, -(double)i / (double)half) / (2.0 * 3.14159265358979323846);
-  double* d = nullptr;
-  TYSOR_CUDA(cudaMalloc(&d, sizeof(double) * rate.size()));
-  TYSOR_CUDA(cudaMemcpy(d, rate.data(), sizeof(double) * rate.size(), cudaMemcpyHostToDevice));
+  auto* d = (const double*)new_table(rate.data(), sizeof(double) * rate.size());
   rope_rates[key] = d;
   return d;
 }
@@ -315,8 +331,8 @@ void tysor_cuda_context_free(void* context) {
     Context* c = static_cast<Context*>(context);
     cudaSetDevice(c->device);
     cudaStreamSynchronize(c->stream);
-    for (auto& kv : c->rope_tables) cudaFree(kv.second);
-    for (auto& kv : c->rope_rates) cudaFree(kv.second);
+    for (auto& kv : c->rope_tables) cudaFree((void*)kv.second);
+    for (auto& kv : c->rope_rates) cudaFree((void*)kv.second);
     if (c->scratch) cudaFree(c->scratch);
     if (c->d_err) cudaFree(c->d_err);
     if (c->comm) tysor_cuda_comm_free(c);

@@ -29,9 +29,9 @@ struct Context {
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
   // cos/sin tables for RoPE, keyed by (seq, half, theta bits).
-  std::map<std::tuple<int64_t, int64_t, uint64_t>, float2*> rope_tables;
+  std::map<std::tuple<int64_t, int64_t, uint64_t>, const float2*> rope_tables;
   // rope_axes' rates in revolutions per position, keyed by (half, theta bits).
-  std::map<std::tuple<int64_t, uint64_t>, double*> rope_rates;
+  std::map<std::tuple<int64_t, uint64_t>, const double*> rope_rates;
   // NCCL communicator (opaque ncclComm_t) when data parallel.
   void* comm = nullptr;
   int nranks = 1;
@@ -39,6 +39,10 @@ struct Context {
 
   // Grows the shared scratch (synchronising first if it must reallocate).
   void* ensure_scratch(size_t bytes);
+  // Whether the stream is being captured into a graph.
+  bool capturing() const;
+  // A table on the device, copied in the stream's order; refused in a capture.
+  void* new_table(const void* host, size_t bytes);
   // Device (cos, sin) table for rope over `seq` positions and `half` freqs.
   const float2* rope_table(int64_t seq, int64_t half, double theta);
   // Device theta^(-i / half) / 2 pi for rope_axes' `half` pairs.
