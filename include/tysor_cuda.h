@@ -273,9 +273,10 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * scores may pass 45000 (by the norms of 128 queries and of 128 keys), are
  * computed key by key, many times slower; one query of a few over a cache only
  * where its output would not be finite otherwise.  The
- * call's workspace belongs to the context and grows with the sizes, which frees
- * the old one: a caller that captures the context's stream into a graph calls
- * the largest sizes once before, and lets one such graph run at a time.
+ * call's workspace belongs to the context and grows with the sizes, which a
+ * capture of the context's stream into a graph refuses: make the call once
+ * before.  What a captured graph uses stays until the context is freed; all of
+ * them and the context's other calls share it, so they run one after the other.
  * starts [batch] may be NULL (k_len - q_len: the queries end where k_len ends, also
  * in a sequence whose length is less, whose rows from there on see nothing),
  * lengths [batch] may be NULL (k_len); both hold whole numbers as floats (beyond

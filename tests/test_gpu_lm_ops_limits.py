@@ -270,3 +270,35 @@ def test_rope_tables_in_a_capture(lib):
     assert np.array_equal(y.read(), want)
     lib.ok("rope_axes", *args, 901.0, False)
     del graph
+
+
+def test_a_workspace_that_a_graph_uses_is_kept():
+    """A captured call, larger ones after it (whose workspace takes the place of
+    the graph's), and its replay; a call that would have to grow it in a capture is
+    refused."""
+    import torch
+    from tysor_b200.runtime import CudaContext
+    lib = Lib(CudaContext(0))
+    dims = (1, 2, 1, 200, 200, 64)
+    q, k, v, _ = attention_inputs(71, *dims, False)
+    ins, out = [lib.put(t) for t in (q, k, v)], lib.zeros(q.shape)
+    args = (*ins, None, None, out, None, *dims, 50, 2, 0.125, False)
+    large = (1, 2, 1, 3000, 3000, 64)
+    more = [lib.put(t) for t in attention_inputs(73, *large, False)]
+    big = (*more[:3], None, None, more[3], None, *large, 50, 2, 0.125, False)
+    lib.ok("window_attention", *args)
+    want = out.read()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(stream_of(lib)):
+        graph.capture_begin()
+        lib.refused("workspace cannot grow", "window_attention", *big)
+        lib.ok("window_attention", *args)
+        graph.capture_end()
+        lib.ok("window_attention", *big)
+        held = torch.full((1 << 24,), float("nan"), device="cuda")  # takes freed memory, if any was
+        out.write(np.zeros(want.size, np.float32))
+        graph.replay()
+        torch.cuda.current_stream().synchronize()
+    assert np.array_equal(out.read(), want) and bool(held.isnan().all())
+    del graph
+    lib.ctx.close()

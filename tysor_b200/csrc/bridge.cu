@@ -35,10 +35,19 @@ const char* device_error_message(int code) {
 }
 
 void* Context::ensure_scratch(size_t bytes) {
-  if (bytes <= scratch_bytes) return scratch;
+  const bool in_capture = capturing();
+  if (bytes <= scratch_bytes) {
+    scratch_captured |= in_capture;
+    return scratch;
+  }
+  if (in_capture)
+    throw CudaError("the workspace cannot grow while the context's stream is captured: make the call once before");
   TYSOR_CUDA(cudaStreamSynchronize(stream));
-  if (scratch) TYSOR_CUDA(cudaFree(scratch));
+  if (scratch_captured) former_scratch.push_back(scratch);
+  else if (scratch) TYSOR_CUDA(cudaFree(scratch));
   scratch = nullptr;
+  scratch_bytes = 0;
+  scratch_captured = false;
   size_t want = bytes + bytes / 4 + 4096;
   TYSOR_CUDA(cudaMalloc(&scratch, want));
   scratch_bytes = want;
@@ -334,6 +343,7 @@ void tysor_cuda_context_free(void* context) {
     for (auto& kv : c->rope_tables) cudaFree((void*)kv.second);
     for (auto& kv : c->rope_rates) cudaFree((void*)kv.second);
     if (c->scratch) cudaFree(c->scratch);
+    for (void* p : c->former_scratch) cudaFree(p);
     if (c->d_err) cudaFree(c->d_err);
     if (c->comm) tysor_cuda_comm_free(c);
     cudaStreamDestroy(c->stream);

@@ -28,6 +28,8 @@ struct Context {
   // Scratch shared by per-op dispatches (split operands, partial sums).
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
+  bool scratch_captured = false;       // a graph captured by the caller uses it
+  std::vector<void*> former_scratch;  // outgrown ones that such graphs use, kept as long as the context
   // cos/sin tables for RoPE, keyed by (seq, half, theta bits).
   std::map<std::tuple<int64_t, int64_t, uint64_t>, const float2*> rope_tables;
   // rope_axes' rates in revolutions per position, keyed by (half, theta bits).
@@ -37,7 +39,8 @@ struct Context {
   int nranks = 1;
   int rank = 0;
 
-  // Grows the shared scratch (synchronising first if it must reallocate).
+  // Grows the shared scratch (synchronising first if it must reallocate); in a
+  // capture it is refused if it would have to.
   void* ensure_scratch(size_t bytes);
   // Whether the stream is being captured into a graph.
   bool capturing() const;
