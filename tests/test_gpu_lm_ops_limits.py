@@ -302,3 +302,30 @@ def test_a_workspace_that_a_graph_uses_is_kept():
     assert np.array_equal(out.read(), want) and bool(held.isnan().all())
     del graph
     lib.ctx.close()
+
+
+# ---- graphs --------------------------------------------------------------------------
+
+
+def test_graphs_refuse_sizes_that_no_kernel_counts(cuda_ctx):
+    """A reshape whose sizes are negative in pairs has the right product."""
+    from tysor_b200.graph import GraphBuilder
+    from tysor_b200.native import NativeError
+    from tysor_b200.runtime import CudaGraphExecutor
+
+    def plan(message, shapes, make):
+        b = GraphBuilder()
+        p = {n: b.param(n) for n in shapes}
+        b.ret(make(b, p))
+        ex = CudaGraphExecutor(cuda_ctx, b.build(), shapes)
+        with pytest.raises(NativeError, match=message):
+            ex.run()
+        ex.close()
+
+    x = [1, 2, 8, 16]
+    for sizes in ((-1, -2, 8, 16), (1, -2, -8, 16), (1, -2, 8, -16)):
+        plan("sizes from 1", {"x": x}, lambda b, p: (lambda q: b.call("window_attention", q, q, q, 0, 0))(
+            b.call("reshape", p["x"], *sizes)))
+        plan("sizes from 1|heads of 16", {"x": x, "p": [1, 1, 8]}, lambda b, p: b.call(
+            "rope_axes", b.call("reshape", p["x"], *sizes), p["p"], 1e4, 8))
+    plan("finite eps", {"x": [4, 30]}, lambda b, p: b.apply(b.ctor("LayerNorm", 30, 1e39), p["x"]))

@@ -1289,6 +1289,12 @@ struct Executor {
     return val(node.inputs[*end]).b;
   }
 
+  // What the kernels count in 32 bits (a reshape's sizes may be anything whose product fits).
+  static void check_sizes(const char* op, const std::vector<int64_t>& shape, int64_t most) {
+    for (int64_t d : shape)
+      if (d < 1 || d > most) fail(std::string(op) + " takes sizes from 1 to " + std::to_string(most) + ", got " + shape_str(shape));
+  }
+
   RopeCall rope_call(const GNode& node) {
     const HVal& x = tensor(node.inputs.at(0), "rope_axes");
     const HVal& pos = tensor(node.inputs.at(1), "rope_axes positions");
@@ -1309,6 +1315,7 @@ struct Executor {
     }
     if (x.shape.size() != 4 || x.shape[3] != 2 * half)
       fail("rope_axes expects a rank-4 input of heads of " + std::to_string(2 * half) + ", got " + shape_str(x.shape));
+    check_sizes("rope_axes", x.shape, 1 << 30);
     r.axes.batch = (int)x.shape[0];
     r.axes.heads = (int)x.shape[r.axes.seq_major ? 2 : 1];
     r.axes.seq = (int)x.shape[r.axes.seq_major ? 1 : 2];
@@ -1342,11 +1349,14 @@ struct Executor {
     size_t end;
     c.s.seq_major = trailing_seq_major(node, 5, &end);
     const int sl = c.s.seq_major ? 1 : 2, hl = c.s.seq_major ? 2 : 1;
+    const int64_t most = 1 << 29;
+    check_sizes("window_attention", q.shape, most);
+    check_sizes("window_attention", k.shape, most);
     if (q.shape.size() != 4 || k.shape.size() != 4 || k.shape != v.shape || k.shape[0] != q.shape[0] ||
         k.shape[3] != q.shape[3] || q.shape[hl] % k.shape[hl] != 0)
       fail("window_attention expects q, k, v of rank 4 with k and v alike and heads that share theirs, got " +
            shape_str(q.shape) + ", " + shape_str(k.shape) + " and " + shape_str(v.shape));
-    if (q.shape[3] > kMaxHeadDim)
+    if (q.shape[3] < 1 || q.shape[3] > kMaxHeadDim)
       fail("window_attention takes heads of 1 to " + std::to_string(kMaxHeadDim) + " values");
     if (window < 0 || sinks < 0) fail("window_attention requires window >= 0 and sinks >= 0");
     for (size_t i = 5; i < end; ++i) {
@@ -1354,9 +1364,6 @@ struct Executor {
       if (i > 6 || numel(t.shape) != q.shape[0]) fail("window_attention expects one length and one start per sequence");
       (i == 5 ? c.lengths : c.starts) = t.slot;
     }
-    const int64_t most = 1 << 29;
-    if (q.shape[0] > most || q.shape[hl] > most || q.shape[sl] > most || k.shape[sl] > most)
-      fail("window_attention takes lengths, batches and heads up to 2^29");
     c.s.batch = (int)q.shape[0];
     c.s.heads = (int)q.shape[hl];
     c.s.kv_heads = (int)k.shape[hl];
@@ -1417,7 +1424,7 @@ struct Executor {
       h.hidden = integer(val(in.at(0)));
       h.eps = in.size() > 1 ? number(val(in[1])) : 1e-5;
       if (in.size() > 2) h.with_bias = boolean(val(in[2]));
-      if (h.hidden < 1 || h.hidden > INT32_MAX || !(h.eps >= 0.0) || std::isinf(h.eps))
+      if (h.hidden < 1 || h.hidden > INT32_MAX || !(h.eps >= 0.0) || std::isinf((float)h.eps))
         fail("LayerNorm requires a width of at least 1 and a finite eps >= 0");
       return h;
     }
