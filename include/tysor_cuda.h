@@ -267,7 +267,7 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * k, v: [batch][kv_heads][k_len][head_dim], kv_heads dividing heads (query
  * heads h * heads / kv_heads ... share key head h); with seq_major
  * [batch][length][heads][head_dim].  head_dim 1 to 128, lengths up to 2^29,
- * scale at least 2^-126.  Products carry fp32's accuracy relative to the
+ * scale from 2^-126 to 2^127.  Products carry fp32's accuracy relative to the
  * greatest value among 128 rows of a head; rows that meet values of 2^100 and
  * more (fewer powers over more than 2^13 keys), infinities or NaN, or whose
  * scores may pass 45000 (by the norms of 128 queries and of 128 keys), are

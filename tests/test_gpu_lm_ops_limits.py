@@ -197,6 +197,18 @@ def test_window_attention_statistics(lib, dims):
     assert np.all(np.abs(got[..., 1] / want[..., 1] - 1) <= 2 * 56 * U * terms + 60 * U)
 
 
+@pytest.mark.parametrize("dims", [(1, 2, 1, 1, 60, 32), (1, 2, 1, 40, 40, 32)], ids=["one", "tiles"])
+def test_window_attention_of_the_greatest_scale(lib, dims):
+    """2^127 on inputs so small that their scores are ordinary, and nothing above."""
+    q, k, v, _ = attention_inputs(79, *dims, False)
+    q, k = q * np.float32(2.0 ** -64), k * np.float32(2.0 ** -66)
+    want = R.window_attention(q, k, v, None, None, 0, 0, 2.0 ** 127, False)
+    got = run_attention(lib, q, k, v, None, None, None, dims, 0, 0, 2.0 ** 127, False, backward=False)
+    near_norm(got["out"], want["out"], 510 * U, "out")
+    bufs = [lib.put(t) for t in (q, k, v)]
+    lib.refused("at most 2^127", "window_attention", *bufs, None, None, lib.zeros(q.shape), None, *dims, 0, 0, 3e38, False)
+
+
 # ---- memory --------------------------------------------------------------------------
 
 

@@ -259,9 +259,10 @@ AttentionShape attention_shape(uint32_t batch, uint32_t heads, uint32_t kv_heads
   const uint32_t most = 1u << 29;  // positions stay below 2^30
   if (q_len > most || k_len > most || batch > most || heads > most)
     throw CudaError("window_attention takes lengths, batches and heads up to 2^29");
-  // A subnormal scale would hold fewer bits than the scores it multiplies.
-  if (!(scale >= 1.17549435e-38f) || isinf(scale))
-    throw CudaError("window_attention requires a finite scale of at least 2^-126");
+  // A subnormal scale would hold fewer bits than the scores it multiplies, and one
+  // above 2^127 leaves fp32 times log2 e.
+  if (!(scale >= 0x1p-126f) || scale > 0x1p127f)
+    throw CudaError("window_attention requires a finite scale of at least 2^-126 and at most 2^127");
   AttentionShape s{};
   s.batch = (int)batch;
   s.heads = (int)heads;
