@@ -34,7 +34,7 @@ __device__ __forceinline__ int64_t row_at(const AttentionShape& s, int b, int h,
 }
 
 // A sequence's keys [0, n) and its first query's position, both whole numbers.
-struct Sequence {
+struct __align__(8) Sequence {
   int start, n;
 };
 
@@ -42,8 +42,9 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionShape& s, int b, 
   Sequence q{s.k_len - s.q_len, s.k_len};
   if (s.lengths != nullptr) {
     const float v = s.lengths[b];
-    if (v >= 0.0f && v <= (float)s.k_len && (int64_t)v <= s.k_len && v == truncf(v)) {
-      q.n = (int)v;
+    const int n = (int)fminf(v, 536870912.0f);  // NaN: that; k_len is at most that
+    if (v >= 0.0f && n <= s.k_len && (float)n == v) {
+      q.n = n;
     } else {
       q.n = 0;
       atomicCAS(err, 0, (int)kErrSequence);
@@ -51,8 +52,9 @@ __device__ __forceinline__ Sequence sequence_of(const AttentionShape& s, int b, 
   }
   if (s.starts != nullptr) {
     const float v = s.starts[b];
-    if (v > -536870912.0f && v < 536870912.0f && v == truncf(v)) {  // positions stay below 2^30
-      q.start = (int)v;
+    const int start = (int)v;  // out of range: the end of it
+    if (fabsf(v) < 536870912.0f && (float)start == v) {  // positions stay below 2^30
+      q.start = start;
     } else {
       q.n = 0;
       q.start = 0;
@@ -306,6 +308,7 @@ struct PackJobs {
   PackJob job[4];
   int first[5];  // first block of each job
   int far;       // far_exponent of the call
+  Sequence* seqs;  // [batch] of the call, for the kernels after this one
 };
 
 template <int DP>
@@ -322,6 +325,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
   const int index = (int)blockIdx.x - p.first[which];
   const int t = index % tiles, h = index / tiles % j.heads, b = index / tiles / j.heads;
   const Sequence sq = sequence_of(s, b, err);
+  if (t == 0 && h == 0 && threadIdx.x == 0) p.seqs[b] = sq;
   // Valid rows of the whole operand: [v0, v1).
   int v0 = 0, v1 = sq.n;
   if (j.queries) v0 = -sq.start, v1 = sq.n - sq.start;
@@ -756,6 +760,7 @@ struct ForwardArgs {
   const uint8_t *pq, *pk, *pv;
   const float *fq, *fk, *fv;
   const float *tnq, *tnk;  // greatest norms of the query and key tiles' rows
+  const Sequence* seqs;
   float *out, *stats;
   int segs;         // segments of each item's key tiles
   int* steps;       // segs > 1: key tiles of each unit
@@ -788,7 +793,7 @@ __device__ __forceinline__ QueryItem query_item(const ForwardArgs& a, int unit, 
   const int index = unit / a.segs, seg = unit - index * a.segs;
   t.r0 = query_place(s, index, &t.h, &t.b);
   t.g = t.h / (s.heads / s.kv_heads);
-  t.sq = sequence_of(s, t.b, err);
+  t.sq = a.seqs[t.b];
   t.rows = rows_of(s, t.sq, t.r0);
   t.range = keys_for(s, t.sq, t.rows);
   t.q_index = (t.b * s.heads + t.h) * tiles_of(s.q_len) + t.r0 / kTile;
@@ -1308,6 +1313,7 @@ struct GradArgs {
   const uint8_t *pq, *pk, *pv, *po;
   const float *fq, *fk, *fv, *fo;      // factors
   const float *tnq, *tnk;              // greatest norms of Q's and K's tiles' rows
+  const Sequence* seqs;
   const float *nv, *tnv, *tno, *tdo;   // norms of V's rows; greatest norm of V's and dO's tiles, greatest |delta|
   const float4* info;                  // of query rows
   const float2* col;                   // the same for rows that are streamed
@@ -1381,7 +1387,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
   GradItem t = grad_place<KEYS>(a, index, &seg);
   bool far = false;  // or not finite
   if (!KEYS) {
-    t.sq = sequence_of(s, t.b, err);
+    t.sq = a.seqs[t.b];
     t.rows = rows_of(s, t.sq, t.r0);
     t.row_tile = (t.b * s.heads + t.h) * tiles_q + t.r0 / kTile;
     const int x = max(t.rows.p0, 0), z = min(t.rows.p1, t.sq.n - 1);
@@ -1397,7 +1403,7 @@ __device__ __forceinline__ GradItem grad_item(const GradArgs& a, int index, int*
       far |= !(norm * a.tnk[k] + 0.0f * a.fv[k] < kFarScore);
     }
   } else {
-    t.sq = sequence_of(s, t.b, err);
+    t.sq = a.seqs[t.b];
     t.rows = {0, 0, false};
     t.row_tile = (t.b * s.kv_heads + t.g) * tiles_k + t.r0 / kTile;
     // Rows that see some key of the tile: positions from the first key on, up
@@ -1965,11 +1971,17 @@ __device__ __noinline__ void one_row_again(const AttentionShape& s, int start, i
   simple_forward_row(s, {start, n}, q, k, v, out, stats, b, h, r);
 }
 
+// Blocks per SM that the compiler keeps registers for (0: as it likes), where that was
+// faster: four rows, four sequences of 32768 keys, 128 wide 98 us (100 without), 127
+// wide 138 (160); one row, 127 wide, 101 (108).
+template <int R>
+constexpr int kDecodeBlocks = R == 1 ? 4 : R == 4 ? 2 : 0;
+
 // WHOLE: the keys are in one part, and this kernel writes the output.  (A kernel of
 // its own: with a call of one_row_again in it the loops of the others take longer,
 // 87 us instead of 85 for four sequences of up to 32768 keys.)
 template <int NI, int R, bool VEC, bool WHOLE>
-__global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
+__global__ void __launch_bounds__(kDecodeThreads, kDecodeBlocks<R>) decode_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
                                                                 const float* __restrict__ k,
                                                                 const float* __restrict__ v, float* __restrict__ out,
                                                                 float* __restrict__ stats, float* __restrict__ part,
@@ -2208,7 +2220,7 @@ __global__ void __launch_bounds__(kDecodeThreads) decode_kernel(const __grid_con
 
 // One block per row joins its splits: each warp takes every fourth, the warps'
 // parts are added in order.
-__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ AttentionShape s, const float* __restrict__ q,
+__global__ void __launch_bounds__(128) decode_join_kernel(AttentionShape s, const float* __restrict__ q,
                                                           const float* __restrict__ k, const float* __restrict__ v,
                                                           const float* __restrict__ part, float* __restrict__ out,
                                                           float* __restrict__ stats, int splits, int per, int* err) {
@@ -2249,7 +2261,7 @@ __global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant_
     out[row_at(s, b, h, r, s.heads, s.q_len) + c] = o;
   }
   if (stats != nullptr && c == 0) *(float2*)(stats + 2 * line) = natural_stats(top, sum);
-  if (__syncthreads_or(!isfinite(o)) && warp == 0) one_row_again(s, sq.start, sq.n, q, k, v, out, stats, b, h, r);
+  if (__syncthreads_or(!isfinite(o)) && warp == 0) simple_forward_row(s, sq, q, k, v, out, stats, b, h, r);
 }
 
 }  // namespace
@@ -2286,6 +2298,7 @@ struct ForwardWork {
   uint8_t *pq, *pk, *pv;
   float *fq, *fk, *fv, *tnq, *tnk, *part;
   float2* part_ml;
+  Sequence* seqs;
   int *steps, segs;
   int64_t floats;
 };
@@ -2320,6 +2333,7 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
   w.fv = c.take(nk);
   w.tnq = c.take(nq);
   w.tnk = c.take(nk);
+  w.seqs = (Sequence*)c.take(2 * (int64_t)s.batch);
   w.segs = segments_of_queries(s, 4);
   w.part = c.take(w.segs > 1 ? nq * w.segs * kTile * padded_dim(s) : 0);
   w.part_ml = (float2*)c.take(w.segs > 1 ? nq * w.segs * kTile * 2 : 0);
@@ -2396,10 +2410,11 @@ void run_decode_rows(const AttentionShape& s, const DecodePlan& p, const float* 
   else run(std::false_type{});
 }
 
-void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, int* err, cudaStream_t st) {
+void run_pack(const AttentionShape& s, PackJob (&jobs)[4], int count, Sequence* seqs, int* err, cudaStream_t st) {
   PackJobs p{};
   p.s = s;
   p.far = far_exponent(std::max(s.q_len, s.k_len));
+  p.seqs = seqs;
   int64_t at = 0;
   for (int i = 0; i < 4; ++i) {
     p.first[i] = i < count ? (int)at : INT_MAX;
@@ -2418,6 +2433,7 @@ struct GradWork {
   float *fq, *fk, *fv, *fo, *tnq, *tnk, *nv, *tnv, *tno, *tdo;
   float4* info;
   float2 *col, *own;
+  Sequence* seqs;
   int* steps;
   float* part;
   int64_t floats;
@@ -2473,6 +2489,7 @@ GradWork grad_work(const AttentionShape& s, float* base) {
   w.info = (float4*)c.take(nq * kTile * 4);
   w.col = (float2*)c.take(nq * kTile * 2);
   w.own = (float2*)c.take(nq * kTile * 2);
+  w.seqs = (Sequence*)c.take(2 * (int64_t)s.batch);
   const Segments g = segments_of(s);
   // The queries' pass has joined its segments when the keys' begins.
   const int64_t for_keys = g.long_segs > 1 || g.short_segs > 1 ? grad_units(s, g) * 2 : 0;
@@ -2539,8 +2556,8 @@ void launch_window_attention(const AttentionShape& s, const float* q, const floa
     PackJob jobs[4] = {{q, w.pq, w.fq, s.heads, s.q_len, 1, w.tnq},
                        {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, w.tnk},
                        {v, w.pv, w.fv, s.kv_heads, s.k_len, 0}};
-    run_pack(s, jobs, 3, err, st);
-    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, w.tnq, w.tnk, out, stats, w.segs, w.steps, w.part, w.part_ml};
+    run_pack(s, jobs, 3, w.seqs, err, st);
+    const ForwardArgs a{s, q, k, v, w.pq, w.pk, w.pv, w.fq, w.fk, w.fv, w.tnq, w.tnk, w.seqs, out, stats, w.segs, w.steps, w.part, w.part_ml};
     if (padded_dim(s) == 64) run_forward<64>(a, err, st);
     else run_forward<128>(a, err, st);
     return;
@@ -2569,11 +2586,11 @@ void launch_window_attention_backward(const AttentionShape& s, const float* q, c
                      {dout, w.po, w.fo, s.heads, s.q_len, 1, w.tno, nullptr, out, stats, w.info, w.own, w.col, w.tdo},
                      {k, w.pk, w.fk, s.kv_heads, s.k_len, 0, w.tnk},
                      {v, w.pv, w.fv, s.kv_heads, s.k_len, 0, w.tnv, w.nv}};
-  run_pack(s, jobs, 4, err, st);
+  run_pack(s, jobs, 4, w.seqs, err, st);
   int scale_exponent;
   const float scale_rest = 2.0f * frexpf(s.scale, &scale_exponent);
   const GradArgs a{s,     q,     k,      v,     out,   dout,  w.pq,  w.pk,  w.pv,  w.po,   w.fq,  w.fk, w.fv, w.fo,
-                   w.tnq, w.tnk, w.nv,   w.tnv, w.tno, w.tdo, w.info, w.col, w.own, dq,     dk,    dv,   accumulate_q,
+                   w.tnq, w.tnk, w.seqs, w.nv,   w.tnv, w.tno, w.tdo, w.info, w.col, w.own, dq,     dk,    dv,   accumulate_q,
                    accumulate_k, accumulate_v, ldexp(1.0, scale_exponent - 1), scale_rest, segments_of(s), w.steps, w.part};
   if (padded_dim(s) == 64) {
     run_grad<64, false>(a, err, st);
