@@ -209,6 +209,30 @@ def test_window_attention_of_the_greatest_scale(lib, dims):
     lib.refused("at most 2^127", "window_attention", *bufs, None, None, lib.zeros(q.shape), None, *dims, 0, 0, 3e38, False)
 
 
+@pytest.mark.parametrize("dims", [(3, 4, 2, 1, 1, 33, 26, 4), (1, 2, 1, 300, 300, 64, 1, 0), (2, 2, 2, 140, 140, 128, 20, 1)],
+                         ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("size", [1.0, 300.0])
+def test_window_attention_of_rows_that_see_one_key(lib, dims, size):
+    """Their output is that key's value, and their scores have no gradients at all."""
+    q, k, v, dout = attention_inputs(83, *dims[:6], False)
+    q, k = q * np.float32(size), k * np.float32(size)
+    window, sinks = dims[6:]
+    lengths = np.full(dims[0], dims[4], np.float32)
+    lengths[-1] = 1
+    starts = np.zeros(dims[0], np.float32)
+    want = R.window_attention(q, k, v, starts, lengths, window, sinks, 0.1, False, dout)
+    for accumulate in (False, True):
+        got = run_attention(lib, q, k, v, dout, starts, lengths, dims[:6], window, sinks, 0.1, False, accumulate=accumulate)
+        fill = 5.0 if accumulate else 0.0
+        near_norm(got["out"][:, :, 0], want["out"][:, :, 0], 64 * U, "out")
+        assert np.array_equal(got["dq"][:, :, 0], np.full_like(got["dq"][:, :, 0], fill))
+        assert np.array_equal(got["dk"][-1], np.full_like(got["dk"][-1], fill))
+        if (window, sinks) == (1, 0) or dims[4] == 1:
+            assert np.array_equal(got["dq"], np.full_like(got["dq"], fill))
+            assert np.array_equal(got["dk"], np.full_like(got["dk"], fill))
+            near_norm(got["dv"] - fill, want["dv"], 64 * U, "dv", 1.0 if accumulate else 0.0)
+
+
 # ---- memory --------------------------------------------------------------------------
 
 

@@ -79,6 +79,13 @@ __device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence&
   return v;
 }
 
+// Whether the row at position p sees one key, and so has scores without gradients: its
+// probability is 1 whatever they are.  (dP and delta, formed in different orders,
+// would leave the rounding of their terms.)
+__device__ __forceinline__ bool sees_one(const AttentionShape& s, int p) {
+  return p == 0 || (s.window == 1 && s.sinks == 0);
+}
+
 // ---- every value: one warp per row -------------------------------------------------
 
 // What is not finite would spoil the hidden places of a matrix product (0 times
@@ -165,9 +172,9 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
   const Seen seen = seen_by(s, sq, sq.start + r);
   const int64_t at = row_at(s, b, h, r, s.heads, s.q_len);
   float qv[kLaneDims], gv[kLaneDims], kv[kLaneDims], vv[kLaneDims], acc[kLaneDims] = {};
-  if (seen.high == 0) {
+  if (seen.high == 0 || sees_one(s, sq.start + r)) {
     if (!accumulate) lane_store(dq + at, s.head_dim, acc, 0);
-    return;
+    if (seen.high == 0) return;
   }
   lane_load(out + at, s.head_dim, kv);
   lane_load(dout + at, s.head_dim, gv);
@@ -191,7 +198,7 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
 #pragma unroll
     for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * (kv[i] * s.scale);  // see `down` in grad_kernel
   }
-  lane_store(dq + at, s.head_dim, acc, accumulate);
+  if (!sees_one(s, sq.start + r)) lane_store(dq + at, s.head_dim, acc, accumulate);
 }
 
 // The query rows that see key j: those at positions [j, end).
@@ -224,7 +231,7 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
         lane_load(out + row, s.head_dim, ov);
         const float2 st = stats[((int64_t)b * s.heads + h) * tiles_of(s.q_len) * kTile + r];
         const float p = expf(lane_score(s, qv, kv) - st.x) / st.y;
-        const float ds = p * (lane_dot(gv, vv) - lane_dot(gv, ov));
+        const float ds = sees_one(s, sq.start + r) ? 0.0f : p * (lane_dot(gv, vv) - lane_dot(gv, ov));
 #pragma unroll
         for (int i = 0; i < kLaneDims; ++i) {
           av[i] += p * gv[i];
@@ -283,8 +290,8 @@ struct PackJob {
   // what their scores may come to: at least that, and NaN where the factor is).  For
   // the gradients, rows counted in whole tiles: the rows' norms as well; or, with
   // the output and statistics (x is the output's gradient), each row's (greatest score in powers
-  // of two, 1 / sum, delta = sum of x * out, norm), zeros for rows that see
-  // nothing, and each tile's greatest |delta| (NaN if a row's values are not finite).
+  // of two, 1 / sum or 0 for a row that sees one key, delta = sum of x * out, norm),
+  // zeros for rows that see nothing, and each tile's greatest |delta| (NaN if a row's values are not finite).
   // Norms and deltas of the output's gradient are in its tile's units, as the packed
   // values are: however small it is, dP and delta are then of ordinary size.
   float *tile_norm, *norm;
@@ -436,7 +443,8 @@ __global__ void __launch_bounds__(256) pack_kernel(PackJobs p, int* err) {
           const float2 st = row_stats[r];
           j.own[(int64_t)index * kTile + r] = st;
           const float4 f =
-              st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(st.x * kLog2e, 1.0f / st.y, d, q);
+              st.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                           : make_float4(st.x * kLog2e, sees_one(s, sq.start + t * kTile + r) ? 0.0f : 1.0f / st.y, d, q);
           j.info[(int64_t)index * kTile + r] = f;
           j.col[(int64_t)index * kTile + r] =
               st.y == 0.0f ? make_float2(1e30f, 0.0f) : make_float2(f.x + (log2f(st.y) - 14.0f), d);
@@ -1704,13 +1712,14 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(GradArgs a, int items
       }
       const double to_log2 = (double)(KEYS ? a.fk : a.fq)[t.row_tile] * (double)s.scale * 1.4426950408889634;
       const float f_row = KEYS ? a.fv[t.row_tile] : 0.0f;
+      const bool one = t.sq.n == 1 || sees_one(s, 1);  // each row sees one key: no dS
       for (int n = t.f0; n < t.f1; ++n, ++gi) {
         int step;
         const int tile = column_tile(t, n, &step), c0 = step * kStep;
         const float f = unit_of(to_log2 * (double)(KEYS ? a.fq : a.fk)[tile]);
         const float f2 = KEYS ? f_row : a.fv[tile];  // of dP and delta in dO's units
         const float bound = norm * (KEYS ? a.tno : a.tnv)[tile] + (KEYS ? a.tdo[tile] : fabsf(st.z));
-        const float up = power_of_two(scale_exponent(bound));
+        const float up = KEYS && one ? 0.0f : power_of_two(scale_exponent(bound));
         bool whole;
         uint32_t seen;
         if (!KEYS) {
