@@ -229,7 +229,8 @@ bool tysor_cuda_dispatch_transpose(void* context, void* input, void* out, const 
  * of floats and start on an 8-byte boundary. */
 
 /* Layer normalisation: y = (x - mean) * rstd * gain + bias per row of
- * `width` values, rstd = 1 / sqrt(variance + eps) (population variance).
+ * `width` values, rstd = 1 / sqrt(variance + eps) (population variance, whose
+ * squares and sums are fp32's: values up to about 1e19 over the root of width).
  * gain, bias [width] may be NULL (1 and 0).  stats may be NULL or receives
  * [rows][2] = (mean, rstd), which the backward reads. */
 bool tysor_cuda_dispatch_layer_norm(void* context, void* input, void* gain, void* bias, void* out,
@@ -304,7 +305,9 @@ bool tysor_cuda_dispatch_window_attention_backward(void* context, void* q, void*
  * width; out[r] = T^2 * sum_e p_e * (ln p_e - ln q[ids[r][e]]).  ids are f32;
  * an id below 0 is an absent entry, and a row without any has loss 0.  An id
  * of width or more is an error ("Embedding index out of range").  An id
- * given twice counts twice.  The temperature is from 2^-60 to 2^60.  stats may be NULL or receives [rows][2] =
+ * given twice counts twice.  The temperature is from 2^-60 to 2^60; the loss is
+ * off by about 2^-21 T^2, what fp32 leaves of the two logarithms, however close
+ * the student follows the teacher.  stats may be NULL or receives [rows][2] =
  * (greatest logit, sum of exp((logit - greatest) / T)). */
 bool tysor_cuda_dispatch_distill_loss(void* context, void* logits, void* ids, void* teacher, void* out,
                                       void* stats, uint32_t rows, uint32_t width, uint32_t top,

@@ -262,8 +262,10 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
 // Packing reads 4 bytes a value and writes 4, and HBM bounds it: a forward's q, k
 // and v, 201 MB both ways, 34 us = 5.9 TB/s; a gradient's operands with the output
 // and the rows' statistics, 403 MB, 88 us = 4.6 TB/s (8192 tokens, 16 heads over 4,
-// 128 wide).  Splitting inside the attention kernels instead would do it once per
-// query tile that reads a key tile.
+// 128 wide).  Splitting keys and values inside the attention kernels instead would do
+// it once per query tile that reads a key tile; a query tile is read by one item (or
+// a few segments of it), and its packing is a trip through memory that the forward
+// could do without.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBox = kTile * 128;  // bytes
@@ -1284,8 +1286,8 @@ __global__ void __launch_bounds__(256) forward_join_kernel(ForwardArgs a) {
 // 256 columns for the resident tiles no wider step fits the 512.
 //
 // The products, five per visible pair and 128 columns and two of them done twice,
-// bound it.  Measured for 8192 tokens, 16 heads over 4, window 1024, 128 wide: 309
-// us for dq (tensor pipe 57%), 447 for dk and dv (54%), together 214 TFLOP/s of the
+// bound it.  Measured for 8192 tokens, 16 heads over 4, window 1024, 128 wide: 306
+// us for dq (tensor pipe 57%), 430 for dk and dv (56%), together 220 TFLOP/s of the
 // formulas' work.  An instruction of 128 x 64 x 16 takes 41 to 60 cycles instead of
 // 32, and the tiles at a window's ends are half hidden.
 // A key tile's queries may be many (a sink's are all that follow), and tiles may
@@ -1934,8 +1936,8 @@ __global__ void __launch_bounds__(256) grad_join_kernel(GradArgs a, JoinSet one,
 // HBM bounds it up to four rows: 4 heads over each of 4, 128 wide, four sequences of
 // up to 32768 keys, 416 MB in 77 to 88 us = 4.7 to 5.4 TB/s of 6.5 (the longest
 // sequence's blocks end last); 32 sequences with a window of 1024, 122 MB in 33 us:
-// a wave of 256 blocks, each a start, 17 steps and an end.  Eight rows take 138 us
-// where four take 103: two blocks of four warps per SM wait for their own arithmetic.
+// a wave of 256 blocks, each a start, 17 steps and an end.  Eight rows take 131 us
+// where four take 98: two blocks of four warps per SM wait for their own arithmetic.
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeRows = 8;
 constexpr int kDecodeStages = 3;
@@ -2356,8 +2358,10 @@ ForwardWork forward_work(const AttentionShape& s, float* base) {
 // query head.  Measured, decode / tiles, 128 wide: one query of 9 heads over one,
 // four such groups and sequences of 32768 keys, 267 / 705 us, of 16 heads 280 /
 // 1272; 5 queries of 2 heads over one, 80 wide, four such and 8000 keys, 79 / 97,
-// of 4 heads, eight such and 8192 keys, 253 / 228; 9 queries and more of one head
-// take the tiles (16 over 8000 keys of 6 heads 54).
+// of 4 heads, eight such and 8192 keys, 253 / 228 (the rule has these go through
+// decode, 11% slower; one that sent them to the tiles would send 5 of 2 heads there
+// too, 23% slower); 9 queries and more of one head take the tiles (16 over 8000 keys
+// of 6 heads 54).
 bool uses_tiles(const AttentionShape& s) {
   const int64_t group = s.heads / s.kv_heads;
   return 2 * ceil_div(group * s.q_len, kDecodeRows) > 2 + group * tiles_of(s.q_len);
