@@ -272,8 +272,8 @@ bool tysor_cuda_dispatch_rope_axes_backward(void* context, void* grad, void* pos
  * greatest value among 128 rows of a head; rows that meet values of 2^100 and
  * more (fewer powers over more than 2^13 keys), infinities or NaN, or whose
  * scores may pass 45000 (by the norms of 128 queries and of 128 keys), are
- * computed key by key, many times slower; one query of a few over a cache only
- * where its output would not be finite otherwise.  The
+ * computed key by key, many times slower (of a few queries over a cache, those
+ * whose output would not be finite otherwise).  The
  * call's workspace belongs to the context and grows with the sizes, which a
  * capture of the context's stream into a graph refuses: make the call once
  * before.  What a captured graph uses stays until the context is freed; all of

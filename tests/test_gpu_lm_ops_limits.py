@@ -233,6 +233,18 @@ def test_window_attention_of_rows_that_see_one_key(lib, dims, size):
             near_norm(got["dv"] - fill, want["dv"], 64 * U, "dv", 1.0 if accumulate else 0.0)
 
 
+@pytest.mark.parametrize("which", ["q", "k"])
+def test_window_attention_of_one_key_that_is_no_number(lib, which):
+    """... but a score that is NaN has NaN for its probability and all that follows."""
+    dims = (1, 2, 1, 30, 30, 16)
+    q, k, v, dout = attention_inputs(89, *dims, False)
+    (q if which == "q" else k)[:, :, 0] = np.nan
+    got = run_attention(lib, q, k, v, dout, None, None, dims, 5, 0, 0.25, False)
+    assert np.isnan(got["out"][:, :, 0]).all() and np.isnan(got["dq"][:, :, 0]).all()
+    assert np.isnan(got["dk"][:, :, 0]).all() and np.isnan(got["dv"][:, :, 0]).all()
+    assert np.isfinite(got["out"][:, :, 5:]).all() and np.isfinite(got["dq"][:, :, 5:]).all()
+
+
 # ---- memory --------------------------------------------------------------------------
 
 

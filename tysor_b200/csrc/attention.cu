@@ -79,8 +79,8 @@ __device__ __forceinline__ Seen seen_by(const AttentionShape& s, const Sequence&
   return v;
 }
 
-// Whether the row at position p sees one key, and so has scores without gradients: its
-// probability is 1 whatever they are.  (dP and delta, formed in different orders,
+// Whether the row at position p sees one key, and so a score without a gradient: its
+// probability is 1 (NaN if the score is).  (dP and delta, formed in different orders,
 // would leave the rounding of their terms.)
 __device__ __forceinline__ bool sees_one(const AttentionShape& s, int p) {
   return p == 0 || (s.window == 1 && s.sinks == 0);
@@ -172,9 +172,9 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
   const Seen seen = seen_by(s, sq, sq.start + r);
   const int64_t at = row_at(s, b, h, r, s.heads, s.q_len);
   float qv[kLaneDims], gv[kLaneDims], kv[kLaneDims], vv[kLaneDims], acc[kLaneDims] = {};
-  if (seen.high == 0 || sees_one(s, sq.start + r)) {
+  if (seen.high == 0) {
     if (!accumulate) lane_store(dq + at, s.head_dim, acc, 0);
-    if (seen.high == 0) return;
+    return;
   }
   lane_load(out + at, s.head_dim, kv);
   lane_load(dout + at, s.head_dim, gv);
@@ -194,11 +194,11 @@ __device__ void simple_dq_row(const AttentionShape& s, const Sequence& sq, const
     lane_load(k + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, kv);
     lane_load(v + row_at(s, b, g, j, s.kv_heads, s.k_len), s.head_dim, vv);
     const float p = expf(lane_score(s, qv, kv) - st.x) / st.y;
-    const float ds = p * (lane_dot(gv, vv) - delta);
+    const float ds = p * (sees_one(s, sq.start + r) ? 0.0f : lane_dot(gv, vv) - delta);
 #pragma unroll
     for (int i = 0; i < kLaneDims; ++i) acc[i] += ds * (kv[i] * s.scale);  // see `down` in grad_kernel
   }
-  if (!sees_one(s, sq.start + r)) lane_store(dq + at, s.head_dim, acc, accumulate);
+  lane_store(dq + at, s.head_dim, acc, accumulate);
 }
 
 // The query rows that see key j: those at positions [j, end).
@@ -231,7 +231,7 @@ __device__ void simple_dkv_row(const AttentionShape& s, const Sequence& sq, cons
         lane_load(out + row, s.head_dim, ov);
         const float2 st = stats[((int64_t)b * s.heads + h) * tiles_of(s.q_len) * kTile + r];
         const float p = expf(lane_score(s, qv, kv) - st.x) / st.y;
-        const float ds = sees_one(s, sq.start + r) ? 0.0f : p * (lane_dot(gv, vv) - lane_dot(gv, ov));
+        const float ds = p * (sees_one(s, sq.start + r) ? 0.0f : lane_dot(gv, vv) - lane_dot(gv, ov));
 #pragma unroll
         for (int i = 0; i < kLaneDims; ++i) {
           av[i] += p * gv[i];
