@@ -319,6 +319,92 @@ bool tysor_cuda_dispatch_distill_loss_backward(void* context, void* logits, void
                                                uint32_t width, uint32_t top, float temperature,
                                                bool accumulate);
 
+/* Rotary positions on the first rotary_dim (2 to 512, even) values of each head
+ * of head_dim; the others are copied.  input and out are
+ * [batch][heads][seq_len][head_dim] or, with seq_major,
+ * [batch][seq_len][heads][head_dim].  Pair i of half = rotary_dim / 2 is
+ * (i, half + i), or (2 i, 2 i + 1) if interleaved; it turns by
+ * positions[b][s] * rate_i and is multiplied by `amplitude`.  positions
+ * [batch][seq_len] may be NULL (0, 1, 2, ...).  With base_i = theta^(-i / half),
+ * rate_i = base_i * (keep_i + (1 - keep_i) / factor), where keep_i is
+ *   TYSOR_ROTARY_PLAIN      1 (factor, original_len, low, high are not read)
+ *   TYSOR_ROTARY_LINEAR     0: positions are divided by factor
+ *   TYSOR_ROTARY_TURNS      (turns_i - low) / (high - low) between 0 and 1, turns_i =
+ *                           original_len * base_i / 2 pi: how often the pair turns
+ *                           over the context that the model was trained on
+ *   TYSOR_ROTARY_LOG_TURNS  the same with logarithms of turns_i, low and high.
+ * Angles are formed in 64 bits.  theta, factor and original_len are above 0,
+ * 0 <= low < high (0 < low by logarithms). */
+enum { TYSOR_ROTARY_PLAIN = 0, TYSOR_ROTARY_LINEAR = 1, TYSOR_ROTARY_TURNS = 2, TYSOR_ROTARY_LOG_TURNS = 3 };
+bool tysor_cuda_dispatch_rotary(void* context, void* input, void* positions, void* out, uint32_t batch,
+                                uint32_t heads, uint32_t seq_len, uint32_t head_dim, uint32_t rotary_dim,
+                                bool interleaved, double theta, int scaling, double factor,
+                                double original_len, double low, double high, double amplitude,
+                                bool seq_major);
+/* dx (+)= amplitude * grad turned back (the values behind rotary_dim as they are). */
+bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positions, void* dx, uint32_t batch,
+                                         uint32_t heads, uint32_t seq_len, uint32_t head_dim,
+                                         uint32_t rotary_dim, bool interleaved, double theta, int scaling,
+                                         double factor, double original_len, double low, double high,
+                                         double amplitude, bool seq_major, bool accumulate);
+/* Linear attention with a decay for each head: with a = exp(-decay[h]) and S_0 =
+ * state (0 if NULL), for the tokens t = 1 .. n of a sequence
+ *   S_t = a * S_(t-1) + k_t v_t^T,   out_t = scale * q_t S_t,
+ * and new_state (may be NULL) = S_n.  q: [batch][heads][seq_len][key_dim]; k:
+ * [batch][kv_heads][seq_len][key_dim]; v: [..][kv_heads][seq_len][value_dim];
+ * out: [..][heads][seq_len][value_dim], kv_heads dividing heads (query heads h *
+ * heads / kv_heads ... share key head h); with seq_major [batch][seq_len][heads]
+ * [dim].  decay: [heads], 0 or more (infinity: each token sees itself alone); one
+ * below 0 or NaN is an error ("Decay below 0 or NaN", and counts as 0).  States:
+ * [batch][heads][key_dim][value_dim], starting on a 16-byte boundary; new_state may
+ * be the buffer `state` itself (no other output may overlap anything).  lengths
+ * [batch] may be NULL (n = seq_len) and holds whole numbers as floats, checked on the
+ * device ("Attention start or length out of range"; the sequence then counts as
+ * empty); rows from n on are not read, and their out is 0.  Dims 1 to 128, lengths up
+ * to 2^29, scale from 2^-60 to 2^60.  Serving calls it with seq_len 1 and the state
+ * kept.  Products carry fp32's accuracy relative to the greatest value in a token's q
+ * or k row, in 64 tokens' values of a v column and in a column of the state; where
+ * values of 2^60 and more, below 2^-100 (0 aside), infinities or NaN come, 64 tokens
+ * at a time go one by one, many times slower.  What leaves fp32's range is infinite or NaN
+ * from there on.  The workspace is the context's, as window_attention's. */
+bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* v, void* decay, void* state,
+                                         void* lengths, void* out, void* new_state, uint32_t batch,
+                                         uint32_t heads, uint32_t kv_heads, uint32_t seq_len,
+                                         uint32_t key_dim, uint32_t value_dim, float scale,
+                                         bool seq_major);
+/* The exact gradients of `out` for dout and of new_state for dnew_state (may be
+ * NULL: 0), decay apart, which is the model's constant.  With
+ *   E_n = dnew_state + scale * q_n dout_n^T,   E_t = a * E_(t+1) + scale * q_t dout_t^T:
+ * dq_t (+)= scale * dout_t S_t^T, dk_t (+)= v_t E_t^T, dv_t (+)= k_t E_t (dk and dv
+ * summed over the query heads that share a key head, in a fixed order), dstate (+)=
+ * a * E_1 (may be NULL).  Rows from n on get 0. */
+bool tysor_cuda_dispatch_decay_attention_backward(void* context, void* q, void* k, void* v, void* decay,
+                                                  void* state, void* lengths, void* dout, void* dnew_state,
+                                                  void* dq, void* dk, void* dv, void* dstate, uint32_t batch,
+                                                  uint32_t heads, uint32_t kv_heads, uint32_t seq_len,
+                                                  uint32_t key_dim, uint32_t value_dim, float scale,
+                                                  bool seq_major, bool accumulate);
+/* Log probabilities under p, the softmax of logits[r] / T over the width (1 to 2^24):
+ * out[r][e] = ln p of ids[r][e] for `given` (0 to 128) ids a row; entropy[r] = -sum p ln p;
+ * top_ids and top_logprobs [rows][top] (top 0 to 128) the most probable tokens in order,
+ * equal ones by id, and their ln p.  ids are f32; an id below 0 is absent (0); one of
+ * width or more is an error ("Embedding index out of range").  ids and out may be NULL
+ * with given 0, entropy always, top_ids and top_logprobs with top 0.  Tokens whose logit
+ * is -inf have ln p = -inf and are no best tokens: where none is left, id -1 and -inf.  A
+ * row of nothing but -inf has entropy 0, one with NaN or +inf holds NaN and no best
+ * tokens.  T is from 2^-60 to 2^60.  stats may be NULL or receives [rows][2] =
+ * (greatest logit, sum of exp((logit - greatest) / T)); the backward reads it. */
+bool tysor_cuda_dispatch_token_logprobs(void* context, void* logits, void* ids, void* out, void* entropy,
+                                        void* top_ids, void* top_logprobs, void* stats, uint32_t rows,
+                                        uint32_t width, uint32_t given, uint32_t top, float temperature);
+/* grad (+)= (1 / T) * (sum over e of dout[r][e] * (1 at ids[r][e] - p) - dentropy[r] * p *
+ * (ln p + entropy[r])), 0 in a row of nothing but -inf.  dout (with given 0 also ids) may be
+ * NULL (0), and so may dentropy, and then entropy too. */
+bool tysor_cuda_dispatch_token_logprobs_backward(void* context, void* logits, void* ids, void* stats,
+                                                 void* entropy, void* dout, void* dentropy, void* grad,
+                                                 uint32_t rows, uint32_t width, uint32_t given,
+                                                 float temperature, bool accumulate);
+
 /* ---- device-resident graph executor -------------------------------------
  * Replaces the host interpreters (runtime/graph_executor.rs:249-356,
  * training/backward.rs:145-380, training/executor.rs:252-816) for one

@@ -81,6 +81,12 @@ pub mod ffi {
         pub fn tysor_cuda_dispatch_window_attention_backward(context: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, starts: *mut c_void, lengths: *mut c_void, out: *mut c_void, stats: *mut c_void, dout: *mut c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, batch: u32, heads: u32, kv_heads: u32, q_len: u32, k_len: u32, head_dim: u32, window: u32, sinks: u32, scale: f32, seq_major: bool, accumulate: bool) -> bool;
         pub fn tysor_cuda_dispatch_distill_loss(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, teacher: *mut c_void, out: *mut c_void, stats: *mut c_void, rows: u32, width: u32, top: u32, temperature: f32) -> bool;
         pub fn tysor_cuda_dispatch_distill_loss_backward(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, teacher: *mut c_void, stats: *mut c_void, dloss: *mut c_void, grad: *mut c_void, rows: u32, width: u32, top: u32, temperature: f32, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_rotary(context: *mut c_void, input: *mut c_void, positions: *mut c_void, out: *mut c_void, batch: u32, heads: u32, seq_len: u32, head_dim: u32, rotary_dim: u32, interleaved: bool, theta: f64, scaling: c_int, factor: f64, original_len: f64, low: f64, high: f64, amplitude: f64, seq_major: bool) -> bool;
+        pub fn tysor_cuda_dispatch_rotary_backward(context: *mut c_void, grad: *mut c_void, positions: *mut c_void, dx: *mut c_void, batch: u32, heads: u32, seq_len: u32, head_dim: u32, rotary_dim: u32, interleaved: bool, theta: f64, scaling: c_int, factor: f64, original_len: f64, low: f64, high: f64, amplitude: f64, seq_major: bool, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_decay_attention(context: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, decay: *mut c_void, state: *mut c_void, lengths: *mut c_void, out: *mut c_void, new_state: *mut c_void, batch: u32, heads: u32, kv_heads: u32, seq_len: u32, key_dim: u32, value_dim: u32, scale: f32, seq_major: bool) -> bool;
+        pub fn tysor_cuda_dispatch_decay_attention_backward(context: *mut c_void, q: *mut c_void, k: *mut c_void, v: *mut c_void, decay: *mut c_void, state: *mut c_void, lengths: *mut c_void, dout: *mut c_void, dnew_state: *mut c_void, dq: *mut c_void, dk: *mut c_void, dv: *mut c_void, dstate: *mut c_void, batch: u32, heads: u32, kv_heads: u32, seq_len: u32, key_dim: u32, value_dim: u32, scale: f32, seq_major: bool, accumulate: bool) -> bool;
+        pub fn tysor_cuda_dispatch_token_logprobs(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, out: *mut c_void, entropy: *mut c_void, top_ids: *mut c_void, top_logprobs: *mut c_void, stats: *mut c_void, rows: u32, width: u32, given: u32, top: u32, temperature: f32) -> bool;
+        pub fn tysor_cuda_dispatch_token_logprobs_backward(context: *mut c_void, logits: *mut c_void, ids: *mut c_void, stats: *mut c_void, entropy: *mut c_void, dout: *mut c_void, dentropy: *mut c_void, grad: *mut c_void, rows: u32, width: u32, given: u32, temperature: f32, accumulate: bool) -> bool;
         pub fn tysor_cuda_graph_new(context: *mut c_void, graph_text: *const c_char) -> *mut c_void;
         pub fn tysor_cuda_graph_free(graph: *mut c_void);
         pub fn tysor_cuda_graph_set_shape(graph: *mut c_void, name: *const c_char, dims: *const i64, rank: c_int) -> bool;

@@ -5,6 +5,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
@@ -30,6 +31,7 @@ const char* device_error_message(int code) {
     case kErrBarrierTimeout: return "a tensor-core pipeline wait timed out";
     case kErrTmemAlloc: return "tensor memory allocation failed";
     case kErrSequence: return "Attention start or length out of range";
+    case kErrDecay: return "Decay below 0 or NaN";
     default: return "unknown device error";
   }
 }
@@ -107,6 +109,16 @@ const double* Context::rope_rate_table(int64_t half, double theta) {
   auto* d = (const double*)new_table(rate.data(), sizeof(double) * rate.size());
   rope_rates[key] = d;
   return d;
+}
+
+const std::vector<double>& Context::rotary_rates(const RotaryRates& r) {
+  for (auto& [key, rates] : rotary_rate_lists)
+    if (key == r) return rates;
+  // Few models in a process; one that changes them from call to call pays for it.
+  if (rotary_rate_lists.size() >= 16) rotary_rate_lists.clear();
+  std::vector<double> rates((size_t)r.half);
+  rotary_fill_rates(r, rates.data());
+  return rotary_rate_lists.emplace_back(r, std::move(rates)).second;
 }
 
 void Context::sync_and_check() {
@@ -217,10 +229,13 @@ struct Operands {
   float* out(void* p, size_t need, const char* what) { return take(p, need, what, true); }
   float* out_or_null(void* p, size_t need, const char* what) { return p ? out(p, need, what) : nullptr; }
 
-  void check_overlap() const {
+  // `a_may_be` and `b_may_be`: two operands that may be the very same memory.
+  void check_overlap(const char* a_may_be = "", const char* b_may_be = "") const {
     for (const Range& a : ranges)
       for (const Range& b : ranges)
-        if (&a != &b && a.written && a.begin < a.end && b.begin < b.end && a.begin < b.end && b.begin < a.end)
+        if (&a != &b && a.begin == b.begin && std::strcmp(a.what, a_may_be) == 0 && std::strcmp(b.what, b_may_be) == 0)
+          continue;
+        else if (&a != &b && a.written && a.begin < a.end && b.begin < b.end && a.begin < b.end && b.begin < a.end)
           throw CudaError(std::string(a.what) + " overlaps " + b.what);
   }
 };
@@ -304,6 +319,69 @@ void rope_axes(void* context, void* x, void* positions, void* out, uint32_t batc
   float* y = o.out(out, n, back ? "dx" : "out");
   o.check_overlap();
   launch_rope_axes(in, pos, o.ctx->rope_rate_table(half, theta), y, s, back, accumulate, o.ctx->stream);
+}
+
+void rotary(void* context, void* x, void* positions, void* out, uint32_t batch, uint32_t heads, uint32_t seq_len,
+            uint32_t head_dim, uint32_t rotary_dim, bool interleaved, const RotaryRates& rates, double amplitude,
+            bool seq_major, bool back, bool accumulate) {
+  Operands o(ctx_of(context));
+  if (rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    throw CudaError("rotary requires an even number of turned values, at most the head's");
+  if (const char* problem = rotary_rates_problem(rates, amplitude)) throw CudaError(problem);
+  const uint32_t most = 1u << 30;
+  if (batch > most || heads > most || seq_len > most || head_dim > most)
+    throw CudaError("rotary takes sizes up to 2^30");
+  RotaryShape s{};
+  s.batch = (int)batch;
+  s.heads = (int)heads;
+  s.seq = (int)seq_len;
+  s.head_dim = (int)head_dim;
+  s.half = rates.half;
+  s.interleaved = interleaved;
+  s.seq_major = seq_major;
+  s.amplitude = (float)amplitude;
+  const size_t n = elems({batch, heads, seq_len, head_dim});
+  const float* in = o.in(x, n, back ? "grad" : "input");
+  const float* pos = o.in_or_null(positions, elems({batch, seq_len}), "positions");
+  float* y = o.out(out, n, back ? "dx" : "out");
+  o.check_overlap();
+  std::copy_n(o.ctx->rotary_rates(rates).begin(), rates.half, s.rates);
+  launch_rotary(in, pos, y, s, back, accumulate, o.ctx->stream);
+}
+
+DecayShape decay_shape(uint32_t batch, uint32_t heads, uint32_t kv_heads, uint32_t seq_len, uint32_t key_dim,
+                       uint32_t value_dim, float scale, bool seq_major) {
+  if (const char* problem = decay_attention_problem(batch, heads, kv_heads, seq_len, key_dim, value_dim, scale))
+    throw CudaError(problem);
+  return {(int)batch, (int)heads, (int)kv_heads, (int)seq_len, (int)key_dim, (int)value_dim, scale, seq_major};
+}
+
+// The operands of decay_attention and its gradients; `state` is read alone.
+DecayInputs decay_inputs(Operands& o, const DecayShape& s, void* q, void* k, void* v, void* decay, void* state,
+                         void* lengths) {
+  const uint64_t batch = s.batch, heads = s.heads, kv_heads = s.kv_heads, seq = s.seq;
+  const uint64_t key_dim = s.key_dim, value_dim = s.value_dim;
+  DecayInputs in{};
+  in.q = o.in(q, elems({batch, heads, seq, key_dim}), "q");
+  in.k = o.in(k, elems({batch, kv_heads, seq, key_dim}), "k");
+  in.v = o.in(v, elems({batch, kv_heads, seq, value_dim}), "v");
+  in.decay = o.in(decay, heads, "decay");
+  in.state = o.in_or_null(state, elems({batch, heads, key_dim, value_dim}), "state");
+  in.lengths = o.in_or_null(lengths, batch, "lengths");
+  if (((uintptr_t)in.state & 15) != 0) throw CudaError("state buffer must start on a 16-byte boundary");
+  return in;
+}
+
+LogprobShape logprob_shape(uint32_t rows, uint32_t width, uint32_t given, uint32_t top, float temperature) {
+  if (width == 0 || width > (uint32_t)kMaxLogprobWidth)
+    throw CudaError("token_logprobs requires a width of 1 to 2^24");
+  if (given > (uint32_t)kMaxGivenTokens)
+    throw CudaError("token_logprobs takes up to " + std::to_string(kMaxGivenTokens) + " given ids a row");
+  if (top > (uint32_t)kMaxTopTokens)
+    throw CudaError("token_logprobs gives up to " + std::to_string(kMaxTopTokens) + " best tokens a row");
+  if (!distill_temperature(temperature))
+    throw CudaError("token_logprobs requires a finite temperature > 0, from 2^-60 to 2^60");
+  return {rows, (int)width, (int)given, (int)top, temperature};
 }
 
 }  // namespace
@@ -936,6 +1014,110 @@ bool tysor_cuda_dispatch_distill_loss_backward(void* context, void* logits, void
     o.check_overlap();
     launch_distill_loss_backward(z, id, t, s, d, g, rows, width, (int)top, temperature, accumulate, o.ctx->d_err,
                                  o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_rotary(void* context, void* input, void* positions, void* out, uint32_t batch,
+                                uint32_t heads, uint32_t seq_len, uint32_t head_dim, uint32_t rotary_dim,
+                                bool interleaved, double theta, int scaling, double factor,
+                                double original_len, double low, double high, double amplitude,
+                                bool seq_major) {
+  return guarded([&] {
+    rotary(context, input, positions, out, batch, heads, seq_len, head_dim, rotary_dim, interleaved,
+           {(int)(rotary_dim / 2), theta, scaling, factor, original_len, low, high}, amplitude, seq_major, false, false);
+  });
+}
+
+bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positions, void* dx, uint32_t batch,
+                                         uint32_t heads, uint32_t seq_len, uint32_t head_dim,
+                                         uint32_t rotary_dim, bool interleaved, double theta, int scaling,
+                                         double factor, double original_len, double low, double high,
+                                         double amplitude, bool seq_major, bool accumulate) {
+  return guarded([&] {
+    rotary(context, grad, positions, dx, batch, heads, seq_len, head_dim, rotary_dim, interleaved,
+           {(int)(rotary_dim / 2), theta, scaling, factor, original_len, low, high}, amplitude, seq_major, true,
+           accumulate);
+  });
+}
+
+bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* v, void* decay, void* state,
+                                         void* lengths, void* out, void* new_state, uint32_t batch,
+                                         uint32_t heads, uint32_t kv_heads, uint32_t seq_len,
+                                         uint32_t key_dim, uint32_t value_dim, float scale,
+                                         bool seq_major) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    const DecayShape s = decay_shape(batch, heads, kv_heads, seq_len, key_dim, value_dim, scale, seq_major);
+    const DecayInputs in = decay_inputs(o, s, q, k, v, decay, state, lengths);
+    float* op = o.out(out, elems({batch, heads, seq_len, value_dim}), "out");
+    float* np = o.out_or_null(new_state, elems({batch, heads, key_dim, value_dim}), "new_state");
+    if (((uintptr_t)np & 15) != 0) throw CudaError("new_state buffer must start on a 16-byte boundary");
+    o.check_overlap("new_state", "state");
+    float* work = scratch_floats(o.ctx, decay_attention_work_elems(s));
+    launch_decay_attention(s, in, op, np, work, o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_decay_attention_backward(void* context, void* q, void* k, void* v, void* decay,
+                                                  void* state, void* lengths, void* dout, void* dnew_state,
+                                                  void* dq, void* dk, void* dv, void* dstate, uint32_t batch,
+                                                  uint32_t heads, uint32_t kv_heads, uint32_t seq_len,
+                                                  uint32_t key_dim, uint32_t value_dim, float scale,
+                                                  bool seq_major, bool accumulate) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    const DecayShape s = decay_shape(batch, heads, kv_heads, seq_len, key_dim, value_dim, scale, seq_major);
+    const DecayInputs in = decay_inputs(o, s, q, k, v, decay, state, lengths);
+    const size_t states = elems({batch, heads, key_dim, value_dim});
+    const float* gp = o.in(dout, elems({batch, heads, seq_len, value_dim}), "dout");
+    const float* gn = o.in_or_null(dnew_state, states, "dnew_state");
+    float* gq = o.out(dq, elems({batch, heads, seq_len, key_dim}), "dq");
+    float* gk = o.out(dk, elems({batch, kv_heads, seq_len, key_dim}), "dk");
+    float* gv = o.out(dv, elems({batch, kv_heads, seq_len, value_dim}), "dv");
+    float* gs = o.out_or_null(dstate, states, "dstate");
+    if ((((uintptr_t)gn | (uintptr_t)gs) & 15) != 0)
+      throw CudaError("dnew_state and dstate buffers must start on a 16-byte boundary");
+    o.check_overlap();
+    float* work = scratch_floats(o.ctx, decay_attention_backward_work_elems(s));
+    launch_decay_attention_backward(s, in, gp, gn, gq, gk, gv, gs, work, accumulate, accumulate, accumulate, accumulate,
+                                    o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_token_logprobs(void* context, void* logits, void* ids, void* out, void* entropy,
+                                        void* top_ids, void* top_logprobs, void* stats, uint32_t rows,
+                                        uint32_t width, uint32_t given, uint32_t top, float temperature) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    const LogprobShape s = logprob_shape(rows, width, given, top, temperature);
+    const float* z = o.in(logits, elems({rows, width}), "logits");
+    const float* id = given ? o.in(ids, elems({rows, given}), "ids") : nullptr;
+    float* op = given ? o.out(out, elems({rows, given}), "out") : nullptr;
+    float* ep = o.out_or_null(entropy, rows, "entropy");
+    float* ti = top ? o.out(top_ids, elems({rows, top}), "top_ids") : nullptr;
+    float* tl = top ? o.out(top_logprobs, elems({rows, top}), "top_logprobs") : nullptr;
+    float* sp = o.out_or_null(stats, elems({rows, 2}), "stats");
+    o.check_overlap();
+    launch_token_logprobs(s, z, id, op, ep, ti, tl, sp, o.ctx->d_err, o.ctx->stream);
+  });
+}
+
+bool tysor_cuda_dispatch_token_logprobs_backward(void* context, void* logits, void* ids, void* stats,
+                                                 void* entropy, void* dout, void* dentropy, void* grad,
+                                                 uint32_t rows, uint32_t width, uint32_t given,
+                                                 float temperature, bool accumulate) {
+  return guarded([&] {
+    Operands o(ctx_of(context));
+    const LogprobShape s = logprob_shape(rows, width, given, 0, temperature);
+    const float* z = o.in(logits, elems({rows, width}), "logits");
+    const float* id = given && dout ? o.in(ids, elems({rows, given}), "ids") : nullptr;
+    const float* sp = o.in(stats, elems({rows, 2}), "stats");
+    const float* gp = given ? o.in_or_null(dout, elems({rows, given}), "dout") : nullptr;
+    const float* gh = o.in_or_null(dentropy, rows, "dentropy");
+    const float* ep = gh ? o.in(entropy, rows, "entropy") : nullptr;
+    float* g = o.out(grad, elems({rows, width}), "grad");
+    o.check_overlap();
+    launch_token_logprobs_backward(s, z, id, sp, ep, gp, gh, g, accumulate, o.ctx->d_err, o.ctx->stream);
   });
 }
 

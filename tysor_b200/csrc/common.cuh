@@ -35,6 +35,7 @@ enum DeviceError : int {
   kErrBarrierTimeout = 2,  // an mbarrier wait ran past its time limit
   kErrTmemAlloc = 3,
   kErrSequence = 4,        // an attention start or length that fits no sequence
+  kErrDecay = 5,           // a head's decay below 0 or NaN
 };
 
 struct CudaError : std::runtime_error {

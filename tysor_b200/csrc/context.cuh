@@ -6,9 +6,11 @@
 #include <map>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "common.cuh"
+#include "lm_ops.cuh"
 
 namespace tysor {
 
@@ -34,6 +36,8 @@ struct Context {
   std::map<std::tuple<int64_t, int64_t, uint64_t>, const float2*> rope_tables;
   // rope_axes' rates in revolutions per position, keyed by (half, theta bits).
   std::map<std::tuple<int64_t, uint64_t>, const double*> rope_rates;
+  // rotary's rates of the models seen last, on the host (the kernels take them as arguments).
+  std::vector<std::pair<RotaryRates, std::vector<double>>> rotary_rate_lists;
   // NCCL communicator (opaque ncclComm_t) when data parallel.
   void* comm = nullptr;
   int nranks = 1;
@@ -50,6 +54,8 @@ struct Context {
   const float2* rope_table(int64_t seq, int64_t half, double theta);
   // Device theta^(-i / half) / 2 pi for rope_axes' `half` pairs.
   const double* rope_rate_table(int64_t half, double theta);
+  // Revolutions per position of rotary's pairs.
+  const std::vector<double>& rotary_rates(const RotaryRates& r);
   // Waits for the stream and turns a recorded device error into a message.
   void sync_and_check();
 };

@@ -1268,12 +1268,161 @@ struct Executor {
       });
       return o;
     }
+    if (op == "rotary") {
+      const RotaryShape r = rotary_call(node);
+      HVal o = new_tensor(val(node.inputs[0]).shape);
+      Slot *a = val(node.inputs[0]).slot, *pos = val(node.inputs[1]).slot, *c = o.slot;
+      forward.push_back([=](cudaStream_t st) { launch_rotary(a->p, pos->p, c->p, r, 0, 0, st); });
+      return o;
+    }
+    if (op == "decay_attention") {
+      const DecayCall dc = decay_call(node);
+      std::vector<int64_t> shape = val(node.inputs[0]).shape;
+      shape[3] = dc.s.value_dim;
+      HVal o = new_tensor(shape);
+      Slot* c = o.slot;
+      need_scratch((size_t)decay_attention_work_elems(dc.s));
+      Slot** scr = &scratch;
+      Context* cx = ctx;
+      forward.push_back([=](cudaStream_t st) {
+        launch_decay_attention(dc.s, dc.inputs(), c->p, nullptr, (*scr)->p, cx->d_err, st);
+      });
+      return o;
+    }
+    if (op == "token_logprobs" || op == "token_entropy") {
+      const LogprobShape ls = logprob_call(node);
+      HVal o = new_tensor({ls.rows, ls.given ? (int64_t)ls.given : 1});
+      Slot *z = val(node.inputs[0]).slot, *c = o.slot, *id = ls.given ? val(node.inputs[1]).slot : nullptr;
+      Slot* stats = mode == kModeRun ? nullptr : alloc((size_t)ls.rows * 2);
+      op_stats[node.output] = stats;
+      Context* cx = ctx;
+      forward.push_back([=](cudaStream_t st) {
+        launch_token_logprobs(ls, z->p, id ? id->p : nullptr, id ? c->p : nullptr, id ? nullptr : c->p, nullptr,
+                              nullptr, stats ? stats->p : nullptr, cx->d_err, st);
+      });
+      return o;
+    }
     fail("Unsupported library graph call '" + op + "'");
   }
 
-  // Row statistics that a layer_norm, window_attention or distill_loss node's
-  // forward leaves for its backward (null in --run).
+  // Row statistics that a layer_norm, window_attention, distill_loss,
+  // token_logprobs or token_entropy node's forward leaves for its backward
+  // (null in --run).
   std::map<int, Slot*> op_stats;
+
+  // rotary(x, positions, theta, rotary_dim, interleaved [, scaling, factor,
+  // original_len, low, high, amplitude] [, seq_major]).
+  RotaryShape rotary_call(const GNode& node) {
+    const HVal& x = tensor(node.inputs.at(0), "rotary");
+    const HVal& pos = tensor(node.inputs.at(1), "rotary positions");
+    RotaryShape r{};
+    size_t end;
+    r.seq_major = trailing_seq_major(node, 5, &end);
+    if (end != 5 && end != 11)
+      fail("rotary expects (x, positions, theta, rotary_dim, interleaved [, scaling, factor, original_len, low, high, "
+           "amplitude] [, seq_major])");
+    const int64_t turned = integer(val(node.inputs[3]));
+    RotaryRates rates{};
+    rates.theta = number(val(node.inputs[2]));
+    r.interleaved = boolean(val(node.inputs[4]));
+    double amplitude = 1.0;
+    if (end == 11) {
+      const int64_t scaling = integer(val(node.inputs[5]));
+      rates.scaling = scaling < 0 || scaling > INT32_MAX ? -1 : (int)scaling;
+      rates.factor = number(val(node.inputs[6]));
+      rates.context = number(val(node.inputs[7]));
+      rates.low = number(val(node.inputs[8]));
+      rates.high = number(val(node.inputs[9]));
+      amplitude = number(val(node.inputs[10]));
+    }
+    if (x.shape.size() != 4 || turned < 0 || turned % 2 != 0 || turned > x.shape[3])
+      fail("rotary expects a rank-4 input and an even number of turned values, at most the head's, got " +
+           shape_str(x.shape));
+    check_sizes("rotary", x.shape, 1 << 30);
+    rates.half = (int)(turned / 2);
+    if (const char* problem = rotary_rates_problem(rates, amplitude)) fail(problem);
+    r.batch = (int)x.shape[0];
+    r.heads = (int)x.shape[r.seq_major ? 2 : 1];
+    r.seq = (int)x.shape[r.seq_major ? 1 : 2];
+    r.head_dim = (int)x.shape[3];
+    r.half = rates.half;
+    r.amplitude = (float)amplitude;
+    if (pos.shape != std::vector<int64_t>{x.shape[0], (int64_t)r.seq})
+      fail("rotary expects positions [batch, sequence], got " + shape_str(pos.shape));
+    rotary_fill_rates(rates, r.rates);
+    return r;
+  }
+
+  // decay_attention(q, k, v, decay [, lengths] [, seq_major]), outputs scaled by
+  // 1 / sqrt(key width).
+  struct DecayCall {
+    DecayShape s;
+    Slot *q, *k, *v, *decay, *lengths = nullptr;
+    DecayInputs inputs() const {
+      return {q->p, k->p, v->p, decay->p, nullptr, lengths ? lengths->p : nullptr};
+    }
+  };
+  DecayCall decay_call(const GNode& node) {
+    const HVal& q = tensor(node.inputs.at(0), "decay_attention");
+    const HVal& k = tensor(node.inputs.at(1), "decay_attention keys");
+    const HVal& v = tensor(node.inputs.at(2), "decay_attention values");
+    const HVal& decay = tensor(node.inputs.at(3), "decay_attention decay");
+    DecayCall c{};
+    size_t end;
+    c.s.seq_major = trailing_seq_major(node, 4, &end);
+    if (end > 5) fail("decay_attention expects (q, k, v, decay [, lengths] [, seq_major])");
+    const int sl = c.s.seq_major ? 1 : 2, hl = c.s.seq_major ? 2 : 1;
+    for (const HVal* t : {&q, &k, &v}) check_sizes("decay_attention", t->shape, 1 << 29);
+    if (q.shape.size() != 4 || k.shape.size() != 4 || v.shape.size() != 4 || k.shape[0] != q.shape[0] ||
+        k.shape[sl] != q.shape[sl] || k.shape[3] != q.shape[3] || v.shape[0] != k.shape[0] || v.shape[1] != k.shape[1] ||
+        v.shape[2] != k.shape[2])
+      fail("decay_attention expects q, k, v of rank 4 and one length, with keys of q's width and v's heads, got " +
+           shape_str(q.shape) + ", " + shape_str(k.shape) + " and " + shape_str(v.shape));
+    c.s.scale = (float)(1.0 / std::sqrt((double)q.shape[3]));
+    if (const char* problem = decay_attention_problem(q.shape[0], q.shape[hl], k.shape[hl], q.shape[sl], q.shape[3],
+                                                      v.shape[3], c.s.scale))
+      fail(problem);
+    if (numel(decay.shape) != q.shape[hl])
+      fail("decay_attention expects one decay per head, got " + shape_str(decay.shape));
+    if (end == 5) {
+      const HVal& n = tensor(node.inputs[4], "decay_attention lengths");
+      if (numel(n.shape) != q.shape[0]) fail("decay_attention expects one length per sequence");
+      c.lengths = n.slot;
+    }
+    c.s.batch = (int)q.shape[0];
+    c.s.heads = (int)q.shape[hl];
+    c.s.kv_heads = (int)k.shape[hl];
+    c.s.seq = (int)q.shape[sl];
+    c.s.key_dim = (int)q.shape[3];
+    c.s.value_dim = (int)v.shape[3];
+    c.q = q.slot;
+    c.k = k.slot;
+    c.v = v.slot;
+    c.decay = decay.slot;
+    return c;
+  }
+
+  // token_logprobs(logits, ids, temperature): [rows, ids a row];
+  // token_entropy(logits, temperature): [rows, 1].
+  LogprobShape logprob_call(const GNode& node) {
+    const bool with_ids = node.op == "token_logprobs";
+    const HVal& z = tensor(node.inputs.at(0), node.op.c_str());
+    if (node.inputs.size() != (with_ids ? 3 : 2) || z.shape.empty() || z.shape.back() < 1)
+      fail(with_ids ? "token_logprobs expects (logits, ids, temperature)" : "token_entropy expects (logits, temperature)");
+    const int64_t w = z.shape.back(), rows = numel(z.shape) / w;
+    if (w > kMaxLogprobWidth) fail(node.op + " requires a width of 1 to 2^24");
+    int64_t given = 0;
+    if (with_ids) {
+      const HVal& id = tensor(node.inputs[1], "token_logprobs ids");
+      given = rows > 0 ? numel(id.shape) / rows : 0;
+      if (given < 1 || given > kMaxGivenTokens || numel(id.shape) != rows * given)
+        fail("token_logprobs expects ids of [rows] or [rows, 1 to " + std::to_string(kMaxGivenTokens) + "] for logits " +
+             shape_str(z.shape) + ", got " + shape_str(id.shape));
+    }
+    const float temperature = (float)number(val(node.inputs.back()));
+    if (!distill_temperature(temperature)) fail(node.op + " requires a finite temperature > 0, from 2^-60 to 2^60");
+    return {rows, (int)w, (int)given, 0, temperature};
+  }
 
   // rope_axes(x, positions, theta, section, ... [, seq_major]).
   struct RopeCall {
@@ -1888,6 +2037,40 @@ struct Executor {
     mark_grads_ready();
   }
 
+  // Where the gradients of a node's first three inputs go.  One value read as two
+  // of them: the kernels write its gradients at the same time, so the later one
+  // gets memory of its own, which add_parts adds.
+  struct ThreeGrads {
+    Slot* in[3];
+    Slot* grad[3];
+    bool acc[3];
+    std::vector<std::pair<Slot*, Slot*>> sums;  // (value's gradient, its further contribution)
+  };
+  ThreeGrads three_grads(const GNode& node) {
+    ThreeGrads t{};
+    for (int i = 0; i < 3; ++i) {
+      const int id = node.inputs[i];
+      t.in[i] = val(id).slot;
+      auto [d, a] = contrib(id);
+      t.grad[i] = d;
+      t.acc[i] = a;
+      for (int j = 0; j < i; ++j)
+        if (node.inputs[j] == id) {
+          t.grad[i] = alloc((size_t)numel(val(id).shape));
+          t.acc[i] = false;
+          t.sums.push_back({d, t.grad[i]});
+          break;
+        }
+    }
+    return t;
+  }
+  void add_parts(const ThreeGrads& t) {
+    for (auto [total, part] : t.sums)
+      backward.push_back([total = total, part = part](cudaStream_t st) {
+        launch_add_inplace(total->p, part->p, (int64_t)total->n, st);
+      });
+  }
+
   void plan_call_backward(const GNode& node, Slot* g, const HVal& out, int64_t n, bool train) {
     const std::string& op = node.op;
     const int xi = node.inputs.at(0);
@@ -1940,26 +2123,10 @@ struct Executor {
     }
     if (op == "window_attention") {
       const AttentionCall ac = attention_call(node);
-      Slot* in[3];
-      Slot* grad[3];
-      bool acc[3];
-      std::vector<std::pair<Slot*, Slot*>> sums;  // (value's gradient, its further contribution)
-      for (int i = 0; i < 3; ++i) {
-        const int id = node.inputs[i];
-        in[i] = val(id).slot;
-        auto [d, a] = contrib(id);
-        grad[i] = d;
-        acc[i] = a;
-        // One value read as two of q, k and v: the kernels write its
-        // gradients at the same time, so the later one gets memory of its own.
-        for (int j = 0; j < i; ++j)
-          if (node.inputs[j] == id) {
-            grad[i] = alloc((size_t)numel(val(id).shape));
-            acc[i] = false;
-            sums.push_back({d, grad[i]});
-            break;
-          }
-      }
+      const ThreeGrads t = three_grads(node);
+      Slot* const* in = t.in;
+      Slot* const* grad = t.grad;
+      const bool* acc = t.acc;
       Slot *q = in[0], *k = in[1], *v = in[2], *dq = grad[0], *dk = grad[1], *dv = grad[2];
       const bool aq = acc[0], ak = acc[1], av = acc[2];
       Slot *o = out.slot, *stats = op_stats.at(node.output);
@@ -1970,10 +2137,41 @@ struct Executor {
         launch_window_attention_backward(ac.shape(), q->p, k->p, v->p, o->p, stats->p, g->p, dq->p, dk->p, dv->p,
                                          (*scr)->p, aq, ak, av, cx->d_err, st);
       });
-      for (auto [total, part] : sums)
-        backward.push_back([total = total, part = part](cudaStream_t st) {
-          launch_add_inplace(total->p, part->p, (int64_t)total->n, st);
-        });
+      add_parts(t);
+      return;
+    }
+    if (op == "rotary") {
+      const RotaryShape r = rotary_call(node);
+      Slot* pos = val(node.inputs[1]).slot;
+      auto [d, acc] = contrib(xi);
+      backward.push_back([=](cudaStream_t st) { launch_rotary(g->p, pos->p, d->p, r, 1, acc, st); });
+      return;
+    }
+    if (op == "decay_attention") {
+      const DecayCall dc = decay_call(node);
+      const ThreeGrads t = three_grads(node);
+      Slot *dq = t.grad[0], *dk = t.grad[1], *dv = t.grad[2];
+      const bool aq = t.acc[0], ak = t.acc[1], av = t.acc[2];
+      need_scratch((size_t)decay_attention_backward_work_elems(dc.s));
+      Slot** scr = &scratch;
+      Context* cx = ctx;
+      backward.push_back([=](cudaStream_t st) {
+        launch_decay_attention_backward(dc.s, dc.inputs(), g->p, nullptr, dq->p, dk->p, dv->p, nullptr, (*scr)->p, aq,
+                                        ak, av, 0, cx->d_err, st);
+      });
+      add_parts(t);
+      return;
+    }
+    if (op == "token_logprobs" || op == "token_entropy") {
+      const LogprobShape ls = logprob_call(node);
+      Slot *z = x.slot, *id = ls.given ? val(node.inputs[1]).slot : nullptr, *stats = op_stats.at(node.output);
+      Slot* entropy = id ? nullptr : out.slot;
+      auto [d, acc] = contrib(xi);
+      Context* cx = ctx;
+      backward.push_back([=](cudaStream_t st) {
+        launch_token_logprobs_backward(ls, z->p, id ? id->p : nullptr, stats->p, entropy ? entropy->p : nullptr,
+                                       id ? g->p : nullptr, id ? nullptr : g->p, d->p, acc, cx->d_err, st);
+      });
       return;
     }
     if (op == "distill_loss") {

@@ -1,0 +1,162 @@
+// Rotary positions on part of a head, in either layout, scaled for long contexts
+// (lm_ops.cuh), forward and backward.
+#include <limits.h>
+#include <math.h>
+
+#include "lm_ops.cuh"
+
+namespace tysor {
+namespace {
+
+constexpr int kRotaryThreads = 256;
+
+// A thread takes V pairs of a token (or 2 V values behind the turned part, which
+// it copies), forms their angles once, in 64 bits, and goes over a range of heads.
+// Each value is read and written once: HBM bounds it, or one launch's latency.
+template <int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __restrict__ x,
+                                                                const float* __restrict__ positions,
+                                                                float* __restrict__ out,
+                                                                const __grid_constant__ RotaryShape s, int head_chunk,
+                                                                int back, int accumulate) {
+  const int turned = s.half / V;                                            // units that turn
+  const int per = turned + (s.head_dim - 2 * s.half + 2 * V - 1) / (2 * V);  // and those that do not
+  const int64_t item = (int64_t)blockIdx.x * kRotaryThreads + threadIdx.x;
+  const int64_t tokens = (int64_t)s.batch * s.seq;
+  if (item >= tokens * per) return;
+  const int64_t token = item / per;
+  const int unit = (int)(item - token * per);
+  const int64_t b = token / s.seq, at = token - b * s.seq;
+  const int64_t step = s.seq_major ? s.head_dim : (int64_t)s.head_dim * s.seq;
+  const int64_t base = (s.seq_major ? (b * s.seq + at) * s.heads : b * s.heads * s.seq + at) * s.head_dim;
+  const int h0 = blockIdx.y * head_chunk, h1 = min(s.heads, h0 + head_chunk);
+  if (unit >= turned) {
+    const int c = 2 * s.half + (unit - turned) * 2 * V;
+#pragma unroll 4
+    for (int h = h0; h < h1; ++h) {
+      const int64_t o = base + h * step + c;
+      if (V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+          float4 f = *(const float4*)(x + o + 4 * i);
+          if (accumulate) {
+            const float4 g = *(const float4*)(out + o + 4 * i);
+            f.x += g.x, f.y += g.y, f.z += g.z, f.w += g.w;
+          }
+          *(float4*)(out + o + 4 * i) = f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * V; ++i)
+          if (c + i < s.head_dim) out[o + i] = accumulate ? out[o + i] + x[o + i] : x[o + i];
+      }
+    }
+    return;
+  }
+  const int i0 = unit * V;
+  const double place = positions != nullptr ? (double)positions[token] : (double)at;
+  float cs[V], sn[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const double turns = place * s.rates[i0 + v];
+    sincospif(2.0f * (float)(turns - rint(turns)), &sn[v], &cs[v]);
+    cs[v] *= s.amplitude;
+    sn[v] *= back ? -s.amplitude : s.amplitude;
+  }
+  // The unit's values: V and V of them `half` apart, or 2 V in a row.
+  const int first = INTERLEAVED ? 2 * i0 : i0, second = INTERLEAVED ? first + V : first + s.half;
+#pragma unroll 4
+  for (int h = h0; h < h1; ++h) {
+    const int64_t o = base + h * step;
+    float f[2][V];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float* src = x + o + (k ? second : first);
+      if (V % 4 == 0) {
+        const float4 w = *(const float4*)src;
+        f[k][0] = w.x, f[k][1 % V] = w.y, f[k][2 % V] = w.z, f[k][3 % V] = w.w;
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[k][v] = src[v];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float& lo = INTERLEAVED ? f[2 * v / V][2 * v % V] : f[0][v];
+      float& hi = INTERLEAVED ? f[(2 * v + 1) / V][(2 * v + 1) % V] : f[1][v];
+      const float t = lo * cs[v] - hi * sn[v];
+      hi = lo * sn[v] + hi * cs[v];
+      lo = t;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float* dst = out + o + (k ? second : first);
+      if (V % 4 == 0) {
+        float4 w = make_float4(f[k][0], f[k][1 % V], f[k][2 % V], f[k][3 % V]);
+        if (accumulate) {
+          const float4 g = *(const float4*)dst;
+          w.x += g.x, w.y += g.y, w.z += g.z, w.w += g.w;
+        }
+        *(float4*)dst = w;
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) dst[v] = accumulate ? dst[v] + f[k][v] : f[k][v];
+      }
+    }
+  }
+}
+
+}  // namespace
+
+const char* rotary_rates_problem(const RotaryRates& r, double amplitude) {
+  if (r.half < 1 || r.half > kMaxRotaryPairs) return "rotary turns 2 to 512 values of a head, an even number";
+  if (!(r.theta > 0.0) || std::isinf(r.theta)) return "rotary requires a finite theta > 0";
+  if (!(fabs(amplitude) <= 3.4e38)) return "rotary requires a finite amplitude";
+  if (r.scaling < kRotaryPlain || r.scaling > kRotaryLogTurns) return "rotary takes scalings 0 to 3";
+  if (r.scaling != kRotaryPlain && (!(r.factor > 0.0) || std::isinf(r.factor)))
+    return "rotary requires a finite factor > 0";
+  if (r.scaling >= kRotaryTurns) {
+    if (!(r.context > 0.0) || std::isinf(r.context)) return "rotary requires a finite original length > 0";
+    if (!(r.low >= 0.0) || !(r.high > r.low) || std::isinf(r.high) || (r.scaling == kRotaryLogTurns && r.low == 0.0))
+      return "rotary requires turns 0 <= low < high (0 < low by logarithms)";
+  }
+  return nullptr;
+}
+
+void rotary_fill_rates(const RotaryRates& r, double* rates) {
+  const double circle = 2.0 * 3.14159265358979323846;
+  for (int i = 0; i < r.half; ++i) {
+    const double rate = pow(r.theta, -(double)i / r.half) / circle;  // revolutions a position
+    double keep = r.scaling == kRotaryPlain ? 1.0 : 0.0;
+    if (r.scaling >= kRotaryTurns) {
+      const double turns = r.context * rate;
+      keep = r.scaling == kRotaryTurns ? (turns - r.low) / (r.high - r.low) : log(turns / r.low) / log(r.high / r.low);
+      keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+    }
+    rates[i] = r.scaling == kRotaryPlain ? rate : rate * (keep + (1.0 - keep) / r.factor);
+  }
+}
+
+void launch_rotary(const float* x, const float* positions, float* out, const RotaryShape& shape, int back,
+                   int accumulate, cudaStream_t st) {
+  const int64_t tokens = (int64_t)shape.batch * shape.seq;
+  if (tokens <= 0 || shape.heads <= 0) return;
+  const bool vec = shape.half % 4 == 0 && shape.head_dim % 8 == 0 && (((uintptr_t)x | (uintptr_t)out) & 15) == 0;
+  const int V = vec ? 4 : 1;
+  const int64_t items = tokens * (shape.half / V + ceil_div(shape.head_dim - 2 * shape.half, 2 * V));
+  // All heads of a token in one thread share its angles; where that leaves
+  // fewer than two blocks per SM, the heads are spread over more threads.
+  int64_t chunk = shape.heads * items / (148 * 2 * kRotaryThreads);
+  const int64_t least = ceil_div(shape.heads, 65535);  // blocks of the grid's second axis
+  chunk = chunk < least ? least : chunk > shape.heads ? shape.heads : chunk;
+  const dim3 grid((unsigned)ceil_div(items, kRotaryThreads), (unsigned)ceil_div(shape.heads, chunk));
+  auto go = [&](auto kernel) {
+    kernel<<<grid, kRotaryThreads, 0, st>>>(x, positions, out, shape, (int)chunk, back, accumulate);
+  };
+  if (vec) shape.interleaved ? go(rotary_kernel<4, true>) : go(rotary_kernel<4, false>);
+  else shape.interleaved ? go(rotary_kernel<1, true>) : go(rotary_kernel<1, false>);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  TYSOR_CUDA(cudaGetLastError());
+}
+
+}  // namespace tysor

@@ -29,7 +29,8 @@ becomes a Constant node where it is met; a call of a builtin constructor
 `LayerNorm`) is a LibraryCtor, of a primitive (`matmul`, `relu`, `scale`) a PrimitiveCall, of a
 library function (`rms_norm`, `cross_entropy`, `reshape`, `repeat_kv`,
 `flatten_heads`, `causal_mask`, `rope`, `transpose`, `rope_axes`,
-`window_attention`, `distill_loss`, `tied_logits`) a LibraryCall, of a local variable an Apply.  A pipeline `a -> f(x) -> g()`
+`window_attention`, `distill_loss`, `rotary`, `decay_attention`, `token_logprobs`,
+`token_entropy`, `tied_logits`) a LibraryCall, of a local variable an Apply.  A pipeline `a -> f(x) -> g()`
 is the nested call `g()(f(x)(a))` for constructor stages (the constructor
 is created, then its input lowered, then applied) and `f(a, x)` for
 function stages.

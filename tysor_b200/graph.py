@@ -29,10 +29,15 @@ PRIMITIVE_OPS = ("matmul", "relu", "scale")
 #   rope_axes(x, positions, theta, section, ... [, seq_major])
 #   window_attention(q, k, v, window, sinks [, lengths [, starts]] [, seq_major])
 #   distill_loss(logits, ids, teacher, temperature)
+#   rotary(x, positions, theta, rotary_dim, interleaved [, scaling, factor, original_len, low, high, amplitude]
+#          [, seq_major])
+#   decay_attention(q, k, v, decay [, lengths] [, seq_major])
+#   token_logprobs(logits, ids, temperature), token_entropy(logits, temperature)
 # x, q, k and v are [batch, heads, length, head_dim], or with a trailing
 # `True` [batch, length, heads, head_dim].
 LIBRARY_CALLS = ("rms_norm", "cross_entropy", "reshape", "repeat_kv", "flatten_heads",
-                 "causal_mask", "rope", "transpose", "rope_axes", "window_attention", "distill_loss")
+                 "causal_mask", "rope", "transpose", "rope_axes", "window_attention", "distill_loss",
+                 "rotary", "decay_attention", "token_logprobs", "token_entropy")
 # Layer constructors (graph_executor.rs:163-223), plus two extensions:
 # `RMSNorm`, rms_norm with a learned gain and a configurable eps, and
 # `LayerNorm(width [, eps [, bias]])` with a learned gain and bias.

@@ -82,6 +82,13 @@ SIGNATURES = {
     "tysor_cuda_dispatch_window_attention_backward": (c_bool, [V] * 12 + [U32] * 8 + [c_float, c_bool, c_bool]),
     "tysor_cuda_dispatch_distill_loss": (c_bool, [V, V, V, V, V, V, U32, U32, U32, c_float]),
     "tysor_cuda_dispatch_distill_loss_backward": (c_bool, [V, V, V, V, V, V, V, U32, U32, U32, c_float, c_bool]),
+    "tysor_cuda_dispatch_rotary": (c_bool, [V] * 4 + [U32] * 5 + [c_bool, c_double, c_int] + [c_double] * 5 + [c_bool]),
+    "tysor_cuda_dispatch_rotary_backward": (c_bool, [V] * 4 + [U32] * 5 + [c_bool, c_double, c_int] + [c_double] * 5
+                                            + [c_bool, c_bool]),
+    "tysor_cuda_dispatch_decay_attention": (c_bool, [V] * 9 + [U32] * 6 + [c_float, c_bool]),
+    "tysor_cuda_dispatch_decay_attention_backward": (c_bool, [V] * 13 + [U32] * 6 + [c_float, c_bool, c_bool]),
+    "tysor_cuda_dispatch_token_logprobs": (c_bool, [V] * 8 + [U32] * 4 + [c_float]),
+    "tysor_cuda_dispatch_token_logprobs_backward": (c_bool, [V] * 8 + [U32] * 3 + [c_float, c_bool]),
     "tysor_cuda_graph_new": (V, [V, c_char_p]),
     "tysor_cuda_graph_free": (None, [V]),
     "tysor_cuda_graph_set_shape": (c_bool, [V, c_char_p, I64P, c_int]),

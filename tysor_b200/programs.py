@@ -488,6 +488,65 @@ def student_lm(layers: int = 2, batch: int = 2, seq: int = 256, d_model: int = 2
     return b.build()
 
 
+def linear_lm(layers: int = 2, batch: int = 2, seq: int = 256, d_model: int = 256, n_heads: int = 4,
+              n_kv_heads: int = 2, hidden: int = 512, vocab: int = 1000, rotary_dim: int = 32,
+              scaling=(0, 1.0, 0.0, 0.0, 0.0, 1.0), theta: float = 10000.0, eps: float = 1e-5,
+              temperature: float = 1.0, entropy_weight: float = 0.01, lr: float = 1e-3, iterations: int = 1) -> Graph:
+    """Language model of linear attention with a decay for each head, trained
+    by the log probabilities of sampled tokens:
+
+        x      = Embedding(vocab, d_model)(ids)            ids: [batch*seq]
+        h      = x + o_proj(decay_attention(q, k, v))      of LayerNorm(x)
+        x      = h + down(SiLU(gate(.)) * up(.))           of LayerNorm(h)
+        logits = tied_logits(LayerNorm(x), embedding)
+        loss   = -advantage * token_logprobs(logits, sampled) - entropy_weight * token_entropy(logits)
+
+    q and k are turned by rotary (pairs side by side, `scaling` as its six last
+    arguments) with `positions` [batch, seq]; `decay` [n_heads] is the model's
+    constant, `lengths` [batch] holds each sequence's tokens (the rest is
+    padding), `sampled` and `advantage` are [batch*seq, 1], a sampled id below 0
+    being absent."""
+    b = GraphBuilder("linear")
+    ids, positions, lengths, decay = b.param("ids"), b.param("positions"), b.param("lengths"), b.param("decay")
+    sampled, advantage = b.param("sampled"), b.param("advantage")
+    hd = d_model // n_heads
+    emb = b.let("embed", b.ctor("Embedding", vocab, d_model))
+    x = b.let("x0", b.apply(emb, ids))
+    for i in range(layers):
+        P = f"l{i}_"
+        n1 = b.let(P + "attn_norm", b.ctor("LayerNorm", d_model, eps))
+        qp = b.let(P + "q_proj", b.ctor("linear", d_model, n_heads * hd, False))
+        kp = b.let(P + "k_proj", b.ctor("linear", d_model, n_kv_heads * hd, False))
+        vp = b.let(P + "v_proj", b.ctor("linear", d_model, n_kv_heads * hd, False))
+        op = b.let(P + "o_proj", b.ctor("linear", n_heads * hd, d_model, False))
+        n2 = b.let(P + "ffn_norm", b.ctor("LayerNorm", d_model, eps))
+        gp = b.let(P + "gate_proj", b.ctor("linear", d_model, hidden, False))
+        up = b.let(P + "up_proj", b.ctor("linear", d_model, hidden, False))
+        dp = b.let(P + "down_proj", b.ctor("linear", hidden, d_model, False))
+        act = b.let(P + "act", b.ctor("SiLU"))
+        hn = b.let(P + "hn", b.apply(n1, x))
+
+        def turned(proj, heads):
+            t = b.call("reshape", b.apply(proj, hn), batch, seq, heads, hd)
+            return b.call("rotary", t, positions, theta, rotary_dim, True, *scaling, True)
+
+        q, k = b.let(P + "q", turned(qp, n_heads)), b.let(P + "k", turned(kp, n_kv_heads))
+        v = b.let(P + "v", b.call("reshape", b.apply(vp, hn), batch, seq, n_kv_heads, hd))
+        ctx = b.call("decay_attention", q, k, v, decay, lengths, True)
+        h = b.let(P + "h", b.binary("+", x, b.apply(op, b.call("reshape", ctx, batch * seq, n_heads * hd))))
+        hn2 = b.let(P + "hn2", b.apply(n2, h))
+        ff = b.binary("*", b.apply(act, b.apply(gp, hn2)), b.apply(up, hn2))
+        x = b.let(f"x{i + 1}", b.binary("+", h, b.apply(dp, ff)))
+    norm = b.let("final_norm", b.ctor("LayerNorm", d_model, eps))
+    logits = b.let("logits", b.call("tied_logits", b.apply(norm, x), emb))
+    lp = b.let("logprobs", b.call("token_logprobs", logits, sampled, temperature))
+    ent = b.let("entropy", b.call("token_entropy", logits, temperature))
+    gain = b.binary("+", b.binary("*", lp, advantage), b.binary("*", ent, entropy_weight))
+    b.ret(b.let("loss", b.binary("*", gain, -1.0)))
+    b.train(objective="loss", lr=lr, iterations=iterations)
+    return b.build()
+
+
 def random_parameters(graph: Graph, seed: int = 1234, std: float = 0.02) -> Dict[str, np.ndarray]:
     """Seeded initial values for every trainable parameter a graph's
     constructors create under the train executor's names
