@@ -7,12 +7,15 @@
 // The forward pass is a scan of (q, k, v); its gradients are three more, since
 //   dq = a scan of (dout, v, k), whose state is the forward's transposed,
 //   dv = a scan back of (k, q, dout) and dk of (v, dout, q) (the same, transposed).
+#include <cuda_fp16.h>
 #include <limits.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "lm_ops.cuh"
+#include "tcgen05.cuh"
 
 namespace tysor {
 namespace {
@@ -193,6 +196,578 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
   }
 }
 
+// ---- 64 tokens at a time ----------------------------------------------------------
+
+// With X the state before 64 tokens, i and j counting them, lead = 1 and tail = 0
+// forward in time (0 and 1 back), a scan is four matrix products:
+//   out_i = scale * (a^(i + lead) q_i X + sum over j <= i of P_ij v_j),  P_ij = a^(i - j) q_i.k_j
+//   X <- a^64 X + sum over j of a^(63 - j + tail) k_j v_j^T
+// fp32 accuracy out of fp16 matrix instructions, as in the attention kernels: an
+// operand is scaled by a power of two and split into hi = fp16(x) and lo =
+// fp16(x - hi), and a product is hi.hi + lo.hi + hi.lo.  Each q and k row (token) has
+// its own power of two, each value column one per 64 tokens, each column of X one per
+// step.  The matrix unit adds with truncation, so a step's sums leave it and X is kept
+// in fp32 registers.  Products are formed transposed (values' columns in the unit's
+// 128 rows), so that X^T, v^T and w^T = (a^(63 - j + tail) v_j)^T are operands in tensor
+// memory, written there by the threads that hold them.
+//
+// A block takes one head's tokens (or a segment of them) step by step; the loads of
+// the next step's rows run meanwhile.  Values that fp16's range would spoil (2^60 and
+// more, below 2^-100, not finite) send their step through the registers token by token.
+constexpr int kStep = 64;
+constexpr int kWorkers = 512, kScanThreads = kWorkers + 32;
+constexpr int kBoxBytes = kStep * 128;  // 64 rows of 64 fp16 values
+constexpr uint32_t kMostBiased = 127 + 60, kLeastBiased = 127 - 100;
+
+// Columns of tensor memory.
+template <int DK>
+struct ScanTmem {
+  static constexpr uint32_t kState = 0, kStateLo = DK / 2, kDelta = DK, kFrom = 2 * DK, kScore = kFrom + 64,
+                            kV = kScore + 64, kVLo = kV + 32, kW = kVLo + 32, kWLo = kW + 32, kAll = kWLo + 32;
+  static constexpr uint32_t kTake = kAll > 256 ? 512 : 256;
+};
+
+template <int DK>
+struct ScanSmem {
+  static constexpr int kBoxes = DK / 64;
+  static constexpr int kQ = 0;                              // [kBoxes][hi, lo] boxes
+  static constexpr int kK = kQ + 2 * kBoxes * kBoxBytes;    // [hi, lo][kBoxes]
+  static constexpr int kP = kK + 2 * kBoxes * kBoxBytes;    // hi, lo, and what q's lo adds
+  static constexpr int kRawQ = kP + 3 * kBoxBytes;          // fp32 rows of the next step
+  static constexpr int kRawK = kRawQ + kStep * DK * 4;
+  static constexpr int kRawV = kRawK + kStep * DK * 4;
+  static constexpr int kMisc = kRawV + kStep * kMostDim * 4;
+  static constexpr int kBytes = kMisc + 8192 + 1024;
+};
+
+struct ScanParts {
+  int segments;  // blocks that share a head's tokens
+  float* states; // [unit][segments - 1][rows * cols]: each segment's own, then the next one's first
+};
+
+__device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
+
+// 2^(14 - e) for a greatest magnitude of 2^e to 2^(e+1), and its inverse; 1 for 0.
+__device__ __forceinline__ float up_factor(uint32_t biased) {
+  return __uint_as_float((biased == 0 ? 127u : 268u - max(biased, 16u)) << 23);
+}
+__device__ __forceinline__ float down_factor(uint32_t biased) {
+  return __uint_as_float((biased == 0 ? 127u : max(biased, 16u) - 14u) << 23);
+}
+__device__ __forceinline__ uint32_t biased_of(float magnitude) { return __float_as_uint(magnitude) >> 23; }
+// Whether a tile of this greatest magnitude goes token by token.
+__device__ __forceinline__ bool far_value(float most) {
+  const uint32_t b = biased_of(most);
+  return b >= kMostBiased || (b < kLeastBiased && most != 0.0f);
+}
+
+__device__ __forceinline__ uint32_t half_pair(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *(const uint32_t*)&h;
+}
+// (a, b) as pairs of halves: hi, and what is left.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = half_pair(a, b);
+  const float2 back = __half22float2(*(const __half2*)&hi);
+  lo = half_pair(a - back.x, b - back.y);
+}
+
+__device__ __forceinline__ void copy_async16(uint32_t to, const float* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t to, const float* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+// The tokens of a sequence that segment `part` takes: [first, last) of the order of the scan.
+__device__ __forceinline__ void segment_of(int n, int segments, int part, int* first, int* last) {
+  const int steps = (n + kStep - 1) / kStep, per = (steps + segments - 1) / segments;
+  *first = min(n, part * per * kStep);
+  *last = min(n, (part + 1) * per * kStep);
+}
+
+// STATE_ONLY: the segment's own state (from 0), for the segments behind it.
+template <int DK, bool STATE_ONLY, bool VEC>
+__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s, ScanParts parts,
+                                                               int* err) {
+  using Tm = ScanTmem<DK>;
+  using Sm = ScanSmem<DK>;
+  constexpr int kBoxes = DK / 64, kMine = DK / 4;  // state values of a thread
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  float* power = (float*)(smem + Sm::kMisc);  // [65] a^i, padded to 72
+  float* q_down = power + 72;                 // [64] what undoes the rows' factors
+  float* k_down = q_down + 64;                // [64]
+  float* p_coef = k_down + 64;                // [64] k's part in P
+  float* v_most = p_coef + 64;                // [4][128]
+  float* x_most = v_most + 512;               // [4][128]
+  uint64_t* bars = (uint64_t*)(x_most + 512);
+  int* far_step = (int*)(bars + 6);           // [2]
+  uint32_t* tmem_slot = (uint32_t*)(far_step + 2);
+  const uint32_t base = smem_u32(smem);
+  const uint32_t ready = smem_u32(bars), score_full = ready + 8, sums_full = ready + 16, p_ready = ready + 24,
+                 out_full = ready + 32, far_seen = ready + 40;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int runs = STATE_ONLY ? parts.segments - 1 : parts.segments;
+  const int unit = blockIdx.x / runs, part = blockIdx.x - unit * runs;
+  const int b = unit / s.heads, h = unit - b * s.heads;
+  const int n = tokens_of(s, b, err);
+  int t0, t1;
+  segment_of(n, parts.segments, part, &t0, &t1);
+  const float decay = decay_of(s, h, err);
+  const int lead = s.back ? 0 : 1, tail = 1 - lead;
+
+  if (tid == 0) {
+    mbar_init(ready, kWorkers / 32);
+    mbar_init(score_full, 1);
+    mbar_init(sums_full, 1);
+    mbar_init(p_ready, kWorkers / 32);
+    mbar_init(out_full, 1);
+    mbar_init(far_seen, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    far_step[0] = far_step[1] = 0;
+  }
+  if (tid <= kStep) power[tid] = tid == 0 ? 1.0f : expf(-decay * tid);
+  if (warp == kWorkers / 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(Tm::kTake));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // Rows and columns that no copy writes are 0 (a last step's rows are cleared again below).
+  for (int i = tid; i < (Sm::kMisc - Sm::kRawQ) / 16; i += kScanThreads)
+    ((uint4*)(smem + Sm::kRawQ))[i] = make_uint4(0, 0, 0, 0);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  if (warp == kWorkers / 32) {
+    // The issuing warp.
+    constexpr uint32_t kNarrow = umma_idesc(kStep, false), kRows = umma_idesc(DK, true);
+    const bool leader = elect_one();
+    uint32_t steps = 0;  // those of the matrix unit
+    bool ok = true;
+    for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
+      ok = warp_wait(ready, c & 1, err);
+      if (!ok) break;
+      tc_fence_after();
+      if (*(volatile int*)&far_step[c & 1]) {
+        if (leader) mbar_arrive(far_seen);
+        continue;
+      }
+      if (leader) {
+        if (!STATE_ONLY) {
+          // P: [q hi; q lo] times k hi, then k lo.
+#pragma unroll
+          for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) {
+              const uint32_t a = column_word(base + Sm::kQ + (i / 4) * 2 * kBoxBytes) + (i & 3) * kColumnStep;
+              const uint32_t k = column_word(base + Sm::kK + (pass * kBoxes + i / 4) * kBoxBytes) + (i & 3) * kColumnStep;
+              umma_ss(tmem + Tm::kScore, a, k, kNarrow, pass + i > 0);
+            }
+          umma_commit(score_full);
+          // X^T q^T: lo.hi, hi.lo, hi.hi.
+#pragma unroll
+          for (int pass = 0; pass < 3; ++pass)
+#pragma unroll
+            for (int i = 0; i < DK / 16; ++i) {
+              const uint32_t x = tmem + (pass == 0 ? Tm::kStateLo : Tm::kState) + i * 8;
+              const uint32_t q = column_word(base + Sm::kQ + ((i / 4) * 2 + (pass == 1)) * kBoxBytes) + (i & 3) * kColumnStep;
+              umma_ts(tmem + Tm::kFrom, x, q, kNarrow, pass + i > 0);
+            }
+        }
+        // w^T k.
+#pragma unroll
+        for (int pass = 0; pass < 3; ++pass)
+#pragma unroll
+          for (int i = 0; i < kStep / 16; ++i) {
+            const uint32_t w = tmem + (pass == 0 ? Tm::kWLo : Tm::kW) + i * 8;
+            const uint32_t k = row_word(base + Sm::kK + (pass == 1) * kBoxes * kBoxBytes, kBoxBytes) + i * kRowStep;
+            umma_ts(tmem + Tm::kDelta, w, k, kRows, pass + i > 0);
+          }
+        umma_commit(sums_full);
+      }
+      if (!STATE_ONLY) {
+        ok = warp_wait(p_ready, steps & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        if (leader) {
+          // v^T P^T: lo.hi, hi.lo, hi.(q's lo), hi.hi.
+#pragma unroll
+          for (int pass = 0; pass < 4; ++pass)
+#pragma unroll
+            for (int i = 0; i < kStep / 16; ++i) {
+              const uint32_t v = tmem + (pass == 0 ? Tm::kVLo : Tm::kV) + i * 8;
+              const int box = pass == 1 ? 1 : pass == 2 ? 2 : 0;
+              const uint32_t p = column_word(base + Sm::kP + box * kBoxBytes) + i * kColumnStep;
+              umma_ts(tmem + Tm::kScore, v, p, kNarrow, pass + i > 0);
+            }
+          umma_commit(out_full);
+        }
+      }
+      ++steps;
+      __syncwarp();
+    }
+  } else {
+    const int quarter = warp & 3, group = warp >> 2;  // tensor memory lanes, and which quarter of a row's columns
+    const int col = quarter * 32 + lane;              // the value column of this thread
+    const uint32_t at_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float *q = s.q.at(b, h), *k = s.k.at(b, h), *v = s.v.at(b, h);
+    float* out = const_cast<float*>(s.out.at(b, h));
+    const int64_t state = (int64_t)unit * s.rows * s.cols;
+    auto token = [&](int t) { return (int64_t)(s.back ? n - 1 - t : t); };
+    float x[kMine];  // X^T: this column, rows group * kMine + i
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) x[i] = 0.0f;
+    if (!STATE_ONLY && col < s.cols) {
+      if (part > 0) {
+        const float* from = parts.states + ((int64_t)unit * (parts.segments - 1) + part - 1) * s.rows * s.cols;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int r = group * kMine + i;
+          if (r < s.rows) x[i] = from[(int64_t)r * s.cols + col];
+        }
+      } else if (s.from.p != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int r = group * kMine + i;
+          if (r < s.rows) x[i] = s.from.p[state + r * s.from.si + col * s.from.sj] * s.from_factor;
+        }
+      }
+    }
+    // Copies rows [t, t + 64) of the scan, zeros behind the sequence's end.
+    auto fetch = [&](int t) {
+      const int m = min(kStep, t1 - t);
+      auto rows = [&](const float* p, int64_t pitch, int dim, int offset, int width) {
+        if (VEC) {
+          const int quads = width / 4;
+          for (int i = tid; i < kStep * quads; i += kWorkers) {
+            const int r = i / quads, c = 4 * (i - r * quads);
+            const uint32_t to = base + offset + (r * width + c) * 4;
+            if (r >= m) *(float4*)(smem + offset + (r * width + c) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            else if (c < dim) copy_async16(to, p + token(t + r) * pitch + c);
+          }
+        } else {
+          for (int i = tid; i < kStep * width; i += kWorkers) {
+            const int r = i / width, c = i - r * width;
+            const uint32_t to = base + offset + (r * width + c) * 4;
+            if (r >= m) *(float*)(smem + offset + (r * width + c) * 4) = 0.0f;
+            else if (c < dim) copy_async4(to, p + token(t + r) * pitch + c);
+          }
+        }
+      };
+      if (!STATE_ONLY) rows(q, s.q.token, s.rows, Sm::kRawQ, DK);
+      rows(k, s.k.token, s.rows, Sm::kRawK, DK);
+      rows(v, s.v.token, s.cols, Sm::kRawV, kMostDim);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // X^T's greatest magnitude in this column, over the four threads that hold it.
+    auto most_of_state = [&] {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) m = fmaxf(m, x[i] == x[i] ? fabsf(x[i]) : INFINITY);
+      x_most[group * 128 + col] = m;
+      worker_sync();
+      return fmaxf(fmaxf(x_most[col], x_most[128 + col]), fmaxf(x_most[256 + col], x_most[384 + col]));
+    };
+    auto put_state = [&](float up) {
+      uint32_t hi[kMine / 2], lo[kMine / 2];
+#pragma unroll
+      for (int i = 0; i < kMine / 2; ++i) split_pair(x[2 * i] * up, x[2 * i + 1] * up, hi[i], lo[i]);
+      if constexpr (DK == 128) {
+        tmem_st16(at_lane + Tm::kState + group * (kMine / 2), hi);
+        tmem_st16(at_lane + Tm::kStateLo + group * (kMine / 2), lo);
+      } else {
+        tmem_st8(at_lane + Tm::kState + group * (kMine / 2), hi);
+        tmem_st8(at_lane + Tm::kStateLo + group * (kMine / 2), lo);
+      }
+    };
+    const float2 fade = decay_over(decay, kStep);
+    bool ok = true;
+    uint32_t steps = 0, far_steps = 0;
+    float x_down = 1.0f;
+    bool far_state = false;
+    if (t0 < t1) {
+      fetch(t0);
+      if (!STATE_ONLY) {
+        const float most = most_of_state();
+        far_state = biased_of(most) >= 255;
+        x_down = down_factor(biased_of(most));
+        put_state(up_factor(biased_of(most)));
+      }
+    }
+    for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
+      const int m = min(kStep, t1 - t);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      worker_sync();
+      // q and k rows: half a warp a row.
+      bool far = far_state;
+      {
+        const int half_lane = lane & 15;
+        for (int r = STATE_ONLY ? kStep + 2 * warp + (lane >> 4) : 2 * warp + (lane >> 4); r < 2 * kStep; r += 32) {
+          const bool is_k = r >= kStep;
+          const int row = r & (kStep - 1);
+          const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + row * DK + 4 * half_lane;
+          float4 f[kBoxes];
+          float most = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kBoxes; ++i) {
+            f[i] = *(const float4*)(raw + 64 * i);
+            // NaN counts as infinity.
+            const float a = fmaxf(fabsf(f[i].x), fabsf(f[i].y)), d = fmaxf(fabsf(f[i].z), fabsf(f[i].w));
+            const float sum = (f[i].x + f[i].y) + (f[i].z + f[i].w);
+            most = fmaxf(most, sum == sum ? fmaxf(a, d) : INFINITY);
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          far |= far_value(most);
+          const uint32_t biased = biased_of(most);
+          const float up = up_factor(biased);
+          // A key of zeros has no part in the greatest factor.
+          if (half_lane == 0) (is_k ? k_down : q_down)[row] = is_k && biased == 0 ? 0.0f : down_factor(biased);
+#pragma unroll
+          for (int i = 0; i < kBoxes; ++i) {
+            uint2 hi, lo;
+            split_pair(f[i].x * up, f[i].y * up, hi.x, lo.x);
+            split_pair(f[i].z * up, f[i].w * up, hi.y, lo.y);
+            const int at = row * 128 + (((half_lane >> 1) ^ (row & 7)) << 4) + ((half_lane & 1) << 3);
+            uint8_t* box = smem + (is_k ? Sm::kK + i * kBoxBytes : Sm::kQ + 2 * i * kBoxBytes) + at;
+            *(uint2*)box = hi;
+            *(uint2*)(box + (is_k ? kBoxes : 1) * kBoxBytes) = lo;
+          }
+        }
+      }
+      // This column's values of 16 tokens.
+      float val[16];
+      {
+        const float* raw = (const float*)(smem + Sm::kRawV) + group * 16 * kMostDim + col;
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          val[i] = raw[i * kMostDim];
+          most = fmaxf(most, val[i] == val[i] ? fabsf(val[i]) : INFINITY);
+        }
+        far |= far_value(most);
+        v_most[group * 128 + col] = most;
+      }
+      if (far) far_step[c & 1] = 1;
+      worker_sync();
+      if (tid == 0) far_step[(c + 1) & 1] = 0;
+      if (*(volatile int*)&far_step[c & 1]) {
+        // Token by token.
+        if (lane == 0) mbar_arrive(ready);
+        const float2 one = decay_over(decay, 1);
+        const float* kr = (const float*)(smem + Sm::kRawK) + group * kMine;
+        const float* qr = (const float*)(smem + Sm::kRawQ) + group * kMine;
+        const float* vr = (const float*)(smem + Sm::kRawV) + col;
+        for (int i = 0; i < m; ++i) {
+          const float w = vr[i * kMostDim];
+          float sum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < kMine; ++j) {
+            if (lead) x[j] = fmaf(x[j], one.x, x[j] * one.y);
+            x[j] = fmaf(kr[i * DK + j], w, x[j]);
+            if (!STATE_ONLY) sum = fmaf(qr[i * DK + j], x[j], sum);
+            if (!lead) x[j] = fmaf(x[j], one.x, x[j] * one.y);
+          }
+          if (!STATE_ONLY) {
+            float* sums = i & 1 ? v_most : x_most;
+            sums[group * 128 + col] = sum;
+            worker_sync();
+            if (group == 0 && col < s.cols) {
+              const float all = ((sums[col] + sums[128 + col]) + (sums[256 + col] + sums[384 + col])) * s.scale;
+              float* to = out + token(t + i) * s.out.token + col;
+              *to = s.accumulate ? *to + all : all;
+            }
+          }
+        }
+        worker_sync();  // the rows are read, and the sums
+        if (t + kStep < t1) fetch(t + kStep);
+        if (!STATE_ONLY) {
+          const float most = most_of_state();
+          far_state = biased_of(most) >= 255;
+          x_down = down_factor(biased_of(most));
+          if (t + kStep < t1) put_state(up_factor(biased_of(most)));
+        }
+        // The issuing warp keeps step.
+        if (ok) ok = warp_wait(far_seen, far_steps & 1, err);
+        ++far_steps;
+        continue;
+      }
+      if (t + kStep < t1) fetch(t + kStep);
+      // The rows' factors: P takes k's over the greatest, w takes a^(63 - j + tail) and k's over that of all.
+      float p_down, w_down;
+      {
+        const float k0 = k_down[lane], k1 = k_down[lane + 32];
+        const int last = m - 1 + tail;
+        const float w0 = lane < m ? k0 * power[last - lane] : 0.0f, w1 = lane + 32 < m ? k1 * power[last - lane - 32] : 0.0f;
+        float most_k = fmaxf(k0, k1), most_w = fmaxf(w0, w1);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          most_k = fmaxf(most_k, __shfl_xor_sync(0xffffffffu, most_k, o));
+          most_w = fmaxf(most_w, __shfl_xor_sync(0xffffffffu, most_w, o));
+        }
+        p_down = most_k;
+        if (warp == 0) {
+          const float inv = __uint_as_float((254u - biased_of(most_k)) << 23);  // a power of two's inverse
+          p_coef[lane] = k0 * inv * 0x1p-22f;
+          p_coef[lane + 32] = k1 * inv * 0x1p-22f;
+        }
+        // Below fp32's normal numbers there is nothing to add.
+        const uint32_t e = biased_of(most_w) >= 1 ? min(biased_of(most_w) + 1, 253u) : 0;
+        w_down = e ? __uint_as_float(e << 23) : 0.0f;
+        const float inv_w = e ? __uint_as_float((254u - e) << 23) : 0.0f;
+        const uint32_t biased = biased_of(fmaxf(fmaxf(v_most[col], v_most[128 + col]), fmaxf(v_most[256 + col], v_most[384 + col])));
+        const float up = up_factor(biased), down = down_factor(biased);
+        uint32_t hi[8], lo[8];
+        if (!STATE_ONLY) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) split_pair(val[2 * i] * up, val[2 * i + 1] * up, hi[i], lo[i]);
+          tmem_st8(at_lane + Tm::kV + group * 8, hi);
+          tmem_st8(at_lane + Tm::kVLo + group * 8, lo);
+        }
+        float coef[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = group * 16 + i;
+          coef[i] = __shfl_sync(0xffffffffu, group < 2 ? w0 : w1, j & 31) * inv_w * up;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_pair(val[2 * i] * coef[2 * i], val[2 * i + 1] * coef[2 * i + 1], hi[i], lo[i]);
+        tmem_st8(at_lane + Tm::kW + group * 8, hi);
+        tmem_st8(at_lane + Tm::kWLo + group * 8, lo);
+        p_down *= down * 0x1p22f;
+        w_down *= down;
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ready);
+
+      if (!STATE_ONLY) {
+        if (ok) ok = warp_wait(score_full, steps & 1, err);
+        tc_fence_after();
+        // P of 16 keys: rows (tokens) 0..63 in the lanes of quarters 0 and 1, what q's lo adds in 2 and 3.
+        float p[16];
+        tmem_ld16(at_lane + Tm::kScore + group * 16, p);
+        const int i = col & (kStep - 1);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int key = group * 16 + j;
+          p[j] = key <= i ? p[j] * (p_coef[key] * power[max(i - key, 0)]) : 0.0f;
+        }
+        uint8_t* row = smem + Sm::kP + i * 128;
+        const int x0 = ((2 * group) ^ (i & 7)) << 4, x1 = ((2 * group + 1) ^ (i & 7)) << 4;
+        uint32_t hi[8], lo[8];
+        if (quarter < 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) split_pair(p[2 * j], p[2 * j + 1], hi[j], lo[j]);
+          *(uint4*)(row + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4*)(row + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+          *(uint4*)(row + kBoxBytes + x0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *(uint4*)(row + kBoxBytes + x1) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) hi[j] = half_pair(p[2 * j], p[2 * j + 1]);
+          *(uint4*)(row + 2 * kBoxBytes + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *(uint4*)(row + 2 * kBoxBytes + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
+        }
+        tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+      }
+      // X.
+      const float from_down = x_down;
+      if (ok) ok = warp_wait(sums_full, steps & 1, err);
+      tc_fence_after();
+      {
+        const float2 a = m == kStep ? fade : decay_over(decay, m);
+#pragma unroll
+        for (int half = 0; half < kMine / 16; ++half) {
+          float d[16];
+          tmem_ld16(at_lane + Tm::kDelta + group * kMine + 16 * half, d);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            x[16 * half + i] = fmaf(x[16 * half + i], a.x, fmaf(x[16 * half + i], a.y, d[i] * w_down));
+        }
+      }
+      if (!STATE_ONLY) {
+        const float most = most_of_state();
+        far_state = biased_of(most) >= 255;
+        x_down = down_factor(biased_of(most));
+        if (t + kStep < t1) put_state(up_factor(biased_of(most)));
+        if (ok) ok = warp_wait(out_full, steps & 1, err);
+        tc_fence_after();
+        float from[16], own[16];
+        tmem_ld16(at_lane + Tm::kFrom + group * 16, from);
+        tmem_ld16(at_lane + Tm::kScore + group * 16, own);
+        if (col < s.cols) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = group * 16 + i;
+            const float o = (from[i] * (from_down * power[r + lead]) + own[i] * p_down) * (q_down[r] * s.scale);
+            if (r < m) {
+              float* to = out + token(t + r) * s.out.token + col;
+              *to = s.accumulate ? *to + o : o;
+            }
+          }
+        }
+        tc_fence_before();
+      }
+      ++steps;
+    }
+    // Rows behind the sequence's end, spread over its blocks.
+    if (!STATE_ONLY && !s.accumulate)
+      for (int r = n + part * 4 + group; r < s.seq; r += 4 * parts.segments)
+        if (col < s.cols) out[(int64_t)r * s.out.token + col] = 0.0f;
+    if (STATE_ONLY) {
+      float* to = parts.states + ((int64_t)unit * (parts.segments - 1) + part) * s.rows * s.cols;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = group * kMine + i;
+        if (r < s.rows && col < s.cols) to[(int64_t)r * s.cols + col] = x[i];
+      }
+    } else if (s.to.p != nullptr && part == parts.segments - 1) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int r = group * kMine + i;
+        if (r < s.rows && col < s.cols) {
+          float* to = s.to.p + state + r * s.to.si + col * s.to.sj;
+          const float y = x[i] * s.to_factor;
+          *to = s.accumulate_state ? *to + y : y;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWorkers / 32)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Tm::kTake));
+}
+
+// From each segment's own state the state that the next one starts from, in place.
+__global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant__ Scan s, ScanParts parts, int* err) {
+  const int unit = blockIdx.y, b = unit / s.heads, h = unit - b * s.heads;
+  const int i = blockIdx.x * 256 + threadIdx.x, elems = s.rows * s.cols;
+  if (i >= elems) return;
+  const int n = tokens_of(s, b, err);
+  const float decay = decay_of(s, h, err);
+  const int r = i / s.cols, c = i - r * s.cols;
+  float x = s.from.p != nullptr ? s.from.p[(int64_t)unit * elems + r * s.from.si + c * s.from.sj] * s.from_factor : 0.0f;
+  float* at = parts.states + (int64_t)unit * (parts.segments - 1) * elems + i;
+  for (int j = 0; j + 1 < parts.segments; ++j) {
+    int t0, t1;
+    segment_of(n, parts.segments, j, &t0, &t1);
+    const float2 a = decay_over(decay, t1 - t0);
+    x = fmaf(x, a.x, fmaf(x, a.y, at[(int64_t)j * elems]));
+    at[(int64_t)j * elems] = x;
+  }
+}
+
 // dst[b][g] (+)= sum over the heads that share key head g of src[b][h], in order.
 __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ src, Rows dst, int batch,
                                                         int kv_heads, int group, int seq, int dim, int accumulate) {
@@ -207,8 +782,69 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict_
   *to = accumulate ? *to + sum : sum;
 }
 
-void run_scan(const Scan& s, int* err, cudaStream_t st) {
+// From how many tokens on 64 at a time are faster than one by one.
+constexpr int kChunkedFrom = 24;
+
+// How many blocks share a head's tokens: they take turns of 64 tokens each, and
+// where there is more than one, a first pass over the keys and values (about half
+// the time) gives their states.
+int segments_of(int64_t units, int seq) {
+  const int64_t steps = ceil_div(seq, kStep);
+  double best = 1e30;
+  int segments = 1;
+  for (int64_t n = 1; n <= (units > 1024 ? 1 : std::min<int64_t>(steps, 64)); ++n) {
+    const double per = (double)ceil_div(steps, n);
+    double cost = (double)ceil_div(units * n, 148) * (per + 2.0);
+    if (n > 1) cost += (double)ceil_div(units * (n - 1), 148) * (0.5 * per + 2.0) + 3.0;
+    if (cost < best) best = cost, segments = (int)n;
+  }
+  return segments;
+}
+
+int64_t states_elems(const DecayShape& s) {
+  if (s.seq < kChunkedFrom) return 0;
+  return (int64_t)s.batch * s.heads * (segments_of((int64_t)s.batch * s.heads, s.seq) - 1) * s.key_dim * s.value_dim;
+}
+
+template <int DK, bool STATE_ONLY, bool VEC>
+void launch_chunks(const Scan& s, const ScanParts& parts, int blocks, int* err, cudaStream_t st) {
+  auto kernel = scan_kernel<DK, STATE_ONLY, VEC>;
+  static std::atomic<uint64_t> set{0};  // devices whose limit is set
+  int device;
+  TYSOR_CUDA(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(set.load(std::memory_order_relaxed) & bit)) {
+    TYSOR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<DK>::kBytes));
+    set.fetch_or(bit, std::memory_order_relaxed);
+  }
+  kernel<<<blocks, kScanThreads, ScanSmem<DK>::kBytes, st>>>(s, parts, err);
+  check_launch();
+}
+
+template <int DK, bool VEC>
+void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st) {
+  const int units = s.batch * s.heads;
+  if (parts.segments > 1) {
+    launch_chunks<DK, true, VEC>(s, parts, units * (parts.segments - 1), err, st);
+    scan_states_kernel<<<dim3((unsigned)ceil_div(s.rows * s.cols, 256), (unsigned)units), 256, 0, st>>>(s, parts, err);
+    check_launch();
+  }
+  launch_chunks<DK, false, VEC>(s, parts, units * parts.segments, err, st);
+}
+
+// `states`: states_elems floats.
+void run_scan(const Scan& s, float* states, int* err, cudaStream_t st) {
   if (s.batch <= 0 || s.heads <= 0) return;
+  if (s.seq >= kChunkedFrom) {
+    const ScanParts parts{segments_of((int64_t)s.batch * s.heads, s.seq), states};
+    auto wide = [](const Rows& r, int dim) {
+      return ((uintptr_t)r.p & 15) == 0 && dim % 4 == 0 && r.token % 4 == 0 && r.head % 4 == 0 && r.batch % 4 == 0;
+    };
+    const bool vec = wide(s.q, s.rows) && wide(s.k, s.rows) && wide(s.v, s.cols);
+    if (s.rows > 64) vec ? run_chunks<128, true>(s, parts, err, st) : run_chunks<128, false>(s, parts, err, st);
+    else vec ? run_chunks<64, true>(s, parts, err, st) : run_chunks<64, false>(s, parts, err, st);
+    return;
+  }
   auto plain = [&](const StateAt& x) {
     return x.p == nullptr || (x.si == s.cols && x.sj == 1 && ((uintptr_t)x.p & 15) == 0);
   };
@@ -250,14 +886,14 @@ const char* decay_attention_problem(uint64_t batch, uint64_t heads, uint64_t kv_
   return nullptr;
 }
 
-int64_t decay_attention_work_elems(const DecayShape&) { return 0; }
+int64_t decay_attention_work_elems(const DecayShape& s) { return states_elems(s); }
 
 int64_t decay_attention_backward_work_elems(const DecayShape& s) {
-  if (s.heads == s.kv_heads) return 0;
-  return (int64_t)s.batch * s.heads * s.seq * std::max(s.key_dim, s.value_dim);
+  const int64_t shared = s.heads == s.kv_heads ? 0 : (int64_t)s.batch * s.heads * s.seq * std::max(s.key_dim, s.value_dim);
+  return states_elems(s) + shared;
 }
 
-void launch_decay_attention(const DecayShape& s, const DecayInputs& in, float* out, float* new_state, float*,
+void launch_decay_attention(const DecayShape& s, const DecayInputs& in, float* out, float* new_state, float* work,
                             int* err, cudaStream_t st) {
   const int share = s.heads / s.kv_heads;
   Scan c = scan_of(s, in);
@@ -269,7 +905,7 @@ void launch_decay_attention(const DecayShape& s, const DecayInputs& in, float* o
   c.out = rows_of(s, out, s.heads, s.value_dim, 1);
   c.from = {const_cast<float*>(in.state), s.value_dim, 1};
   c.to = {new_state, s.value_dim, 1};
-  run_scan(c, err, st);
+  run_scan(c, work, err, st);
 }
 
 void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in, const float* dout,
@@ -279,6 +915,7 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   const int share = s.heads / s.kv_heads;
   const Rows q = rows_of(s, in.q, s.heads, s.key_dim, 1), k = rows_of(s, in.k, s.kv_heads, s.key_dim, share);
   const Rows v = rows_of(s, in.v, s.kv_heads, s.value_dim, share), g = rows_of(s, dout, s.heads, s.value_dim, 1);
+  float *states = work, *by_head = work + states_elems(s);
   Scan c = scan_of(s, in);
   c.rows = s.value_dim;
   c.cols = s.key_dim;
@@ -288,7 +925,7 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.out = rows_of(s, dq, s.heads, s.key_dim, 1);
   c.from = {const_cast<float*>(in.state), 1, s.value_dim};
   c.accumulate = accumulate_q;
-  run_scan(c, err, st);
+  run_scan(c, states, err, st);
 
   // The states of the scans back are the gradients' over `scale`.
   c.back = 1;
@@ -299,15 +936,15 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
     if (share == 1) {
       c.out = to;
       c.accumulate = accumulate;
-      run_scan(c, err, st);
+      run_scan(c, states, err, st);
       return;
     }
-    c.out = {work, (int64_t)s.heads * s.seq * dim, (int64_t)s.seq * dim, dim, 1};
+    c.out = {by_head, (int64_t)s.heads * s.seq * dim, (int64_t)s.seq * dim, dim, 1};
     c.accumulate = 0;
-    run_scan(c, err, st);
+    run_scan(c, states, err, st);
     const int64_t n = (int64_t)s.batch * s.kv_heads * s.seq * dim;
     if (n <= 0) return;
-    sum_heads_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(work, to, s.batch, s.kv_heads, share, s.seq, dim,
+    sum_heads_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(by_head, to, s.batch, s.kv_heads, share, s.seq, dim,
                                                                  accumulate);
     check_launch();
   };
