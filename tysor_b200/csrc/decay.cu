@@ -211,21 +211,24 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
 // 128 rows), so that X^T, v^T and w^T = (a^(63 - j + tail) v_j)^T are operands in tensor
 // memory, written there by the threads that hold them.
 //
-// A block takes one head's tokens (or a segment of them) step by step; the loads of
-// the next step's rows run meanwhile.  Values that fp16's range would spoil (2^60 and
-// more, below 2^-100, not finite) send their step through the registers token by token.
+// A block takes one head's tokens (or a segment of them) step by step: a loading warp
+// brings the next step's rows into shared memory, sixteen warps split them, form P and
+// keep X, an issuing warp feeds the matrix unit.  Values that fp16's range would spoil
+// (2^60 and more, below 2^-100, not finite) send their step through the registers token
+// by token.
 constexpr int kStep = 64;
-constexpr int kWorkers = 512, kScanThreads = kWorkers + 32;
-constexpr int kBoxBytes = kStep * 128;  // 64 rows of 64 fp16 values
-constexpr uint32_t kMostBiased = 127 + 60, kLeastBiased = 127 - 100;
+constexpr int kWorkers = 512, kScanThreads = kWorkers + 128, kLoaders = 3;  // loading warps
+constexpr int kWorkerRegs = 104, kOtherRegs = 64;  // 4 x 104 + 64 = 5 x 96, what a quarter of an SM is launched with
+constexpr int kBoxBytes = kStep * 128;             // 64 rows of 64 fp16 values
+constexpr uint32_t kLeastBiased = 127 - 100, kFarRange = 160;  // exponents from 2^-100 to 2^60
 
 // Columns of tensor memory.
 template <int DK>
 struct ScanTmem {
   static constexpr uint32_t kState = 0, kStateLo = DK / 2, kDelta = DK, kFrom = 2 * DK, kScore = kFrom + 64,
-                            kV = kScore + 64, kVLo = kV + 32, kW = kVLo + 32, kWLo = kW + 32, kAll = kWLo + 32;
-  static constexpr uint32_t kTake = kAll > 256 ? 512 : 256;
+                            kV = kScore + 64, kVLo = kV + 32, kW = kVLo + 32, kWLo = kW + 32;
 };
+constexpr uint32_t kTmemColumns = 512;
 
 template <int DK>
 struct ScanSmem {
@@ -237,7 +240,7 @@ struct ScanSmem {
   static constexpr int kRawK = kRawQ + kStep * DK * 4;
   static constexpr int kRawV = kRawK + kStep * DK * 4;
   static constexpr int kMisc = kRawV + kStep * kMostDim * 4;
-  static constexpr int kBytes = kMisc + 8192 + 1024;
+  static constexpr int kBytes = kMisc + 9216 + 1024;
 };
 
 struct ScanParts {
@@ -247,36 +250,65 @@ struct ScanParts {
 
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
-// 2^(14 - e) for a greatest magnitude of 2^e to 2^(e+1), and its inverse; 1 for 0.
-__device__ __forceinline__ float up_factor(uint32_t biased) {
-  return __uint_as_float((biased == 0 ? 127u : 268u - max(biased, 16u)) << 23);
+// Two fp32 values for the paired instructions.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-__device__ __forceinline__ float down_factor(uint32_t biased) {
-  return __uint_as_float((biased == 0 ? 127u : max(biased, 16u) - 14u) << 23);
+__device__ __forceinline__ float2 floats_of(Pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
 }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// The greatest magnitude; NaN if one is.
+__device__ __forceinline__ float most_of(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float warp_most(float v) {
+  float r;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t biased_of(float magnitude) { return __float_as_uint(magnitude) >> 23; }
-// Whether a tile of this greatest magnitude goes token by token.
-__device__ __forceinline__ bool far_value(float most) {
-  const uint32_t b = biased_of(most);
-  return b >= kMostBiased || (b < kLeastBiased && most != 0.0f);
-}
+__device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
+// 2^(14 - e) for a greatest magnitude of 2^e to 2^(e+1), and its inverse; for 0, 1.
+__device__ __forceinline__ uint32_t scale_biased(float most) { return most == 0.0f ? 141u : max(biased_of(most), 16u); }
+// Whether a tile of this greatest magnitude (0 apart) goes token by token; NaN does.
+__device__ __forceinline__ bool far_biased(uint32_t biased) { return biased - kLeastBiased >= kFarRange; }
 
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *(const uint32_t*)&h;
 }
-// (a, b) as pairs of halves: hi, and what is left.
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = half_pair(a, b);
+// Pairs of values as pairs of halves: hi, and what is left.
+__device__ __forceinline__ void split_pair(Pair v, uint32_t& hi, uint32_t& lo) {
+  const float2 f = floats_of(v);
+  hi = half_pair(f.x, f.y);
   const float2 back = __half22float2(*(const __half2*)&hi);
-  lo = half_pair(a - back.x, b - back.y);
+  const float2 rest = floats_of(fma2(pair_of(back.x, back.y), pair_of(-1.0f, -1.0f), v));
+  lo = half_pair(rest.x, rest.y);
 }
 
-__device__ __forceinline__ void copy_async16(uint32_t to, const float* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
 __device__ __forceinline__ void copy_async4(uint32_t to, const float* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_async16(uint32_t to, const float* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
 // The tokens of a sequence that segment `part` takes: [first, last) of the order of the scan.
@@ -286,7 +318,8 @@ __device__ __forceinline__ void segment_of(int n, int segments, int part, int* f
   *last = min(n, (part + 1) * per * kStep);
 }
 
-// STATE_ONLY: the segment's own state (from 0), for the segments behind it.
+// STATE_ONLY: the segment's own state (from 0), for the segments behind it.  VEC: rows of
+// whole 16-byte pieces.
 template <int DK, bool STATE_ONLY, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s, ScanParts parts,
                                                                int* err) {
@@ -295,18 +328,19 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   constexpr int kBoxes = DK / 64, kMine = DK / 4;  // state values of a thread
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  float* power = (float*)(smem + Sm::kMisc);  // [65] a^i, padded to 72
-  float* q_down = power + 72;                 // [64] what undoes the rows' factors
-  float* k_down = q_down + 64;                // [64]
-  float* p_coef = k_down + 64;                // [64] k's part in P
-  float* v_most = p_coef + 64;                // [4][128]
-  float* x_most = v_most + 512;               // [4][128]
+  float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
+  float* lefts = since + 64;                  // [2][64] a^(63 - j + tail), and the same of a last, shorter step
+  float* q_downs = lefts + 128;               // [2][64] what undoes the rows' factors, steps in turn
+  float* k_downs = q_downs + 128;             // [2][64]
+  float* v_mosts = k_downs + 128;             // [2][4][128]
+  float* x_most = v_mosts + 1024;             // [4][128]
   uint64_t* bars = (uint64_t*)(x_most + 512);
-  int* far_step = (int*)(bars + 6);           // [2]
+  int* far_step = (int*)(bars + 9);  // [2]
   uint32_t* tmem_slot = (uint32_t*)(far_step + 2);
   const uint32_t base = smem_u32(smem);
-  const uint32_t ready = smem_u32(bars), score_full = ready + 8, sums_full = ready + 16, p_ready = ready + 24,
-                 out_full = ready + 32, far_seen = ready + 40;
+  const uint32_t raw_full = smem_u32(bars), raw_empty = raw_full + 8, ready = raw_full + 16, values_ready = raw_full + 24,
+                 score_full = raw_full + 32, sums_full = raw_full + 40, p_ready = raw_full + 48,
+                 out_full = raw_full + 56, far_seen = raw_full + 64;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int runs = STATE_ONLY ? parts.segments - 1 : parts.segments;
   const int unit = blockIdx.x / runs, part = blockIdx.x - unit * runs;
@@ -316,9 +350,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   segment_of(n, parts.segments, part, &t0, &t1);
   const float decay = decay_of(s, h, err);
   const int lead = s.back ? 0 : 1, tail = 1 - lead;
+  auto power = [&](int steps) { return steps == 0 ? 1.0f : expf(-decay * steps); };
 
   if (tid == 0) {
-    mbar_init(ready, kWorkers / 32);
+    mbar_init(raw_full, 32 * kLoaders);
+    mbar_init(raw_empty, 1);
+    mbar_init(ready, 1);
+    mbar_init(values_ready, kWorkers / 32);
     mbar_init(score_full, 1);
     mbar_init(sums_full, 1);
     mbar_init(p_ready, kWorkers / 32);
@@ -327,36 +365,44 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     far_step[0] = far_step[1] = 0;
   }
-  if (tid <= kStep) power[tid] = tid == 0 ? 1.0f : expf(-decay * tid);
+  if (tid < 64) since[tid] = power(tid + lead);
+  if (tid >= 64 && tid < 192) {
+    const int j = tid & 63, m = tid < 128 ? kStep : (t1 - t0) % kStep;
+    lefts[tid - 64] = j < m ? power(m - 1 - j + tail) : 0.0f;
+  }
   if (warp == kWorkers / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(Tm::kTake));
+                 "r"(kTmemColumns));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // Rows and columns that no copy writes are 0 (a last step's rows are cleared again below).
-  for (int i = tid; i < (Sm::kMisc - Sm::kRawQ) / 16; i += kScanThreads)
-    ((uint4*)(smem + Sm::kRawQ))[i] = make_uint4(0, 0, 0, 0);
+  // Columns that no copy writes are 0.
+  if (s.rows != DK || s.cols != kMostDim)
+    for (int i = tid; i < (Sm::kMisc - Sm::kRawQ) / 16; i += kScanThreads)
+      ((uint4*)(smem + Sm::kRawQ))[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  const float *q = s.q.at(b, h), *k = s.k.at(b, h), *v = s.v.at(b, h);
+  auto token = [&](int t) { return (int64_t)(s.back ? n - 1 - t : t); };
 
-  if (warp == kWorkers / 32) {
-    // The issuing warp.
-    constexpr uint32_t kNarrow = umma_idesc(kStep, false), kRows = umma_idesc(DK, true);
-    const bool leader = elect_one();
-    uint32_t steps = 0;  // those of the matrix unit
-    bool ok = true;
-    for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
-      ok = warp_wait(ready, c & 1, err);
-      if (!ok) break;
-      tc_fence_after();
-      if (*(volatile int*)&far_step[c & 1]) {
-        if (leader) mbar_arrive(far_seen);
-        continue;
-      }
-      if (leader) {
-        if (!STATE_ONLY) {
+  if (warp >= kWorkers / 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kWorkers / 32) {
+      // The issuing warp.
+      constexpr uint32_t kNarrow = umma_idesc(kStep, false), kRows = umma_idesc(DK, true);
+      const bool leader = elect_one();
+      uint32_t steps = 0;  // those of the matrix unit
+      bool ok = true;
+      for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
+        ok = warp_wait(ready, c & 1, err);
+        if (!ok) break;
+        tc_fence_after();
+        if (*(volatile int*)&far_step[c & 1]) {
+          if (leader) mbar_arrive(far_seen);
+          continue;
+        }
+        if (!STATE_ONLY && leader) {
           // P: [q hi; q lo] times k hi, then k lo.
 #pragma unroll
           for (int pass = 0; pass < 2; ++pass)
@@ -377,104 +423,125 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
               umma_ts(tmem + Tm::kFrom, x, q, kNarrow, pass + i > 0);
             }
         }
-        // w^T k.
-#pragma unroll
-        for (int pass = 0; pass < 3; ++pass)
-#pragma unroll
-          for (int i = 0; i < kStep / 16; ++i) {
-            const uint32_t w = tmem + (pass == 0 ? Tm::kWLo : Tm::kW) + i * 8;
-            const uint32_t k = row_word(base + Sm::kK + (pass == 1) * kBoxes * kBoxBytes, kBoxBytes) + i * kRowStep;
-            umma_ts(tmem + Tm::kDelta, w, k, kRows, pass + i > 0);
-          }
-        umma_commit(sums_full);
-      }
-      if (!STATE_ONLY) {
-        ok = warp_wait(p_ready, steps & 1, err);
+        __syncwarp();
+        ok = warp_wait(values_ready, steps & 1, err);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
-          // v^T P^T: lo.hi, hi.lo, hi.(q's lo), hi.hi.
+          // w^T k.
 #pragma unroll
-          for (int pass = 0; pass < 4; ++pass)
+          for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
             for (int i = 0; i < kStep / 16; ++i) {
-              const uint32_t v = tmem + (pass == 0 ? Tm::kVLo : Tm::kV) + i * 8;
-              const int box = pass == 1 ? 1 : pass == 2 ? 2 : 0;
-              const uint32_t p = column_word(base + Sm::kP + box * kBoxBytes) + i * kColumnStep;
-              umma_ts(tmem + Tm::kScore, v, p, kNarrow, pass + i > 0);
+              const uint32_t w = tmem + (pass == 0 ? Tm::kWLo : Tm::kW) + i * 8;
+              const uint32_t k = row_word(base + Sm::kK + (pass == 1) * kBoxes * kBoxBytes, kBoxBytes) + i * kRowStep;
+              umma_ts(tmem + Tm::kDelta, w, k, kRows, pass + i > 0);
             }
-          umma_commit(out_full);
+          umma_commit(sums_full);
         }
+        if (!STATE_ONLY) {
+          __syncwarp();
+          ok = warp_wait(p_ready, steps & 1, err);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            // v^T P^T: lo.hi, hi.lo, hi.(q's lo), hi.hi.
+#pragma unroll
+            for (int pass = 0; pass < 4; ++pass)
+#pragma unroll
+              for (int i = 0; i < kStep / 16; ++i) {
+                const uint32_t v = tmem + (pass == 0 ? Tm::kVLo : Tm::kV) + i * 8;
+                const int box = pass == 1 ? 1 : pass == 2 ? 2 : 0;
+                const uint32_t p = column_word(base + Sm::kP + box * kBoxBytes) + i * kColumnStep;
+                umma_ts(tmem + Tm::kScore, v, p, kNarrow, pass + i > 0);
+              }
+            umma_commit(out_full);
+          }
+        }
+        ++steps;
+        __syncwarp();
       }
-      ++steps;
-      __syncwarp();
+    } else {
+      // The loading warps, a row at a time.
+      const int loader = warp - kWorkers / 32 - 1;
+      bool ok = true;
+      for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
+        if (c > 0) ok = warp_wait(raw_empty, (c - 1) & 1, err);
+        if (!ok) break;
+        const int m = min(kStep, t1 - t);
+        auto row = [&](const float* from, int dim, uint32_t to) {
+          if (VEC) {
+            if (4 * lane < dim) copy_async16(to + 16 * lane, from + 4 * lane);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kMostDim / 32; ++i)
+              if (lane + 32 * i < dim) copy_async4(to + 4 * (lane + 32 * i), from + lane + 32 * i);
+          }
+        };
+#pragma unroll 4
+        for (int r = loader; r < m; r += kLoaders) {
+          const int64_t at = token(t + r);
+          row(k + at * s.k.token, s.rows, base + Sm::kRawK + r * DK * 4);
+          if (!STATE_ONLY) row(q + at * s.q.token, s.rows, base + Sm::kRawQ + r * DK * 4);
+          row(v + at * s.v.token, s.cols, base + Sm::kRawV + r * kMostDim * 4);
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(raw_full) : "memory");
+      }
+      // The last copies end before the block does.
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
   } else {
-    const int quarter = warp & 3, group = warp >> 2;  // tensor memory lanes, and which quarter of a row's columns
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWorkerRegs));
+    const int quarter = warp & 3, group = warp >> 2;  // tensor memory lanes, and which 16 tokens or quarter of the rows
     const int col = quarter * 32 + lane;              // the value column of this thread
     const uint32_t at_lane = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float *q = s.q.at(b, h), *k = s.k.at(b, h), *v = s.v.at(b, h);
     float* out = const_cast<float*>(s.out.at(b, h));
     const int64_t state = (int64_t)unit * s.rows * s.cols;
-    auto token = [&](int t) { return (int64_t)(s.back ? n - 1 - t : t); };
-    float x[kMine];  // X^T: this column, rows group * kMine + i
+    Pair x[kMine / 2];  // X^T: this column, rows group * kMine + i
+    {
+      float first[kMine];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) x[i] = 0.0f;
-    if (!STATE_ONLY && col < s.cols) {
-      if (part > 0) {
-        const float* from = parts.states + ((int64_t)unit * (parts.segments - 1) + part - 1) * s.rows * s.cols;
+      for (int i = 0; i < kMine; ++i) first[i] = 0.0f;
+      if (!STATE_ONLY && col < s.cols) {
+        if (part > 0) {
+          const float* from = parts.states + ((int64_t)unit * (parts.segments - 1) + part - 1) * s.rows * s.cols;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int r = group * kMine + i;
-          if (r < s.rows) x[i] = from[(int64_t)r * s.cols + col];
-        }
-      } else if (s.from.p != nullptr) {
+          for (int i = 0; i < kMine; ++i) {
+            const int r = group * kMine + i;
+            if (r < s.rows) first[i] = from[(int64_t)r * s.cols + col];
+          }
+        } else if (s.from.p != nullptr) {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int r = group * kMine + i;
-          if (r < s.rows) x[i] = s.from.p[state + r * s.from.si + col * s.from.sj] * s.from_factor;
+          for (int i = 0; i < kMine; ++i) {
+            const int r = group * kMine + i;
+            if (r < s.rows) first[i] = s.from.p[state + r * s.from.si + col * s.from.sj] * s.from_factor;
+          }
         }
       }
+#pragma unroll
+      for (int i = 0; i < kMine / 2; ++i) x[i] = pair_of(first[2 * i], first[2 * i + 1]);
     }
-    // Copies rows [t, t + 64) of the scan, zeros behind the sequence's end.
-    auto fetch = [&](int t) {
-      const int m = min(kStep, t1 - t);
-      auto rows = [&](const float* p, int64_t pitch, int dim, int offset, int width) {
-        if (VEC) {
-          const int quads = width / 4;
-          for (int i = tid; i < kStep * quads; i += kWorkers) {
-            const int r = i / quads, c = 4 * (i - r * quads);
-            const uint32_t to = base + offset + (r * width + c) * 4;
-            if (r >= m) *(float4*)(smem + offset + (r * width + c) * 4) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            else if (c < dim) copy_async16(to, p + token(t + r) * pitch + c);
-          }
-        } else {
-          for (int i = tid; i < kStep * width; i += kWorkers) {
-            const int r = i / width, c = i - r * width;
-            const uint32_t to = base + offset + (r * width + c) * 4;
-            if (r >= m) *(float*)(smem + offset + (r * width + c) * 4) = 0.0f;
-            else if (c < dim) copy_async4(to, p + token(t + r) * pitch + c);
-          }
-        }
-      };
-      if (!STATE_ONLY) rows(q, s.q.token, s.rows, Sm::kRawQ, DK);
-      rows(k, s.k.token, s.rows, Sm::kRawK, DK);
-      rows(v, s.v.token, s.cols, Sm::kRawV, kMostDim);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     // X^T's greatest magnitude in this column, over the four threads that hold it.
     auto most_of_state = [&] {
       float m = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) m = fmaxf(m, x[i] == x[i] ? fabsf(x[i]) : INFINITY);
+      for (int i = 0; i < kMine / 2; ++i) {
+        const float2 f = floats_of(x[i]);
+        m = most_of(m, f.x, f.y);
+      }
       x_most[group * 128 + col] = m;
       worker_sync();
-      return fmaxf(fmaxf(x_most[col], x_most[128 + col]), fmaxf(x_most[256 + col], x_most[384 + col]));
+      return most_of(most_of(x_most[col], x_most[128 + col], x_most[256 + col]), x_most[384 + col], 0.0f);
     };
-    auto put_state = [&](float up) {
+    float x_down = 1.0f;  // undoes the factor of the state in tensor memory
+    auto put_state = [&](float bound) {
+      const uint32_t biased = scale_biased(bound);
+      x_down = power_of(biased - 14u);
+      const float up = power_of(268u - biased);
+      const Pair up2 = pair_of(up, up);
       uint32_t hi[kMine / 2], lo[kMine / 2];
 #pragma unroll
-      for (int i = 0; i < kMine / 2; ++i) split_pair(x[2 * i] * up, x[2 * i + 1] * up, hi[i], lo[i]);
+      for (int i = 0; i < kMine / 2; ++i) split_pair(mul2(x[i], up2), hi[i], lo[i]);
       if constexpr (DK == 128) {
         tmem_st16(at_lane + Tm::kState + group * (kMine / 2), hi);
         tmem_st16(at_lane + Tm::kStateLo + group * (kMine / 2), lo);
@@ -483,97 +550,140 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         tmem_st8(at_lane + Tm::kStateLo + group * (kMine / 2), lo);
       }
     };
+    // P's decay for this thread's row (or, in quarters 2 and 3, what q's lo adds to it) and 16 keys.
+    const int row_i = col & (kStep - 1);
+    Pair near[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int key = group * 16 + 2 * j;
+      near[j] = pair_of(key <= row_i ? power(row_i - key) : 0.0f, key + 1 <= row_i ? power(row_i - key - 1) : 0.0f);
+    }
     const float2 fade = decay_over(decay, kStep);
     bool ok = true;
     uint32_t steps = 0, far_steps = 0;
-    float x_down = 1.0f;
+    float bound = 0.0f;  // at least X^T's greatest magnitude in this column
     bool far_state = false;
     if (t0 < t1) {
-      fetch(t0);
       if (!STATE_ONLY) {
-        const float most = most_of_state();
-        far_state = biased_of(most) >= 255;
-        x_down = down_factor(biased_of(most));
-        put_state(up_factor(biased_of(most)));
+        bound = most_of_state();
+        far_state = biased_of(bound) >= 254;
+        put_state(bound);
       }
     }
     for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
       const int m = min(kStep, t1 - t);
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      worker_sync();
-      // q and k rows: half a warp a row.
+      const int turn = c & 1;
+      float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn, *v_most = v_mosts + 512 * turn;
+      if (ok) ok = warp_wait(raw_full, turn, err);
+      if (m < kStep) {  // zeros behind the sequence's end
+        for (int i = tid; i < (kStep - m) * DK; i += kWorkers) {
+          ((float*)(smem + Sm::kRawQ))[m * DK + i] = 0.0f;
+          ((float*)(smem + Sm::kRawK))[m * DK + i] = 0.0f;
+        }
+        for (int i = tid; i < (kStep - m) * kMostDim; i += kWorkers) ((float*)(smem + Sm::kRawV))[m * kMostDim + i] = 0.0f;
+        worker_sync();
+      }
+      // q and k rows, a warp eight of one of them.
       bool far = far_state;
       {
-        const int half_lane = lane & 15;
-        for (int r = STATE_ONLY ? kStep + 2 * warp + (lane >> 4) : 2 * warp + (lane >> 4); r < 2 * kStep; r += 32) {
-          const bool is_k = r >= kStep;
-          const int row = r & (kStep - 1);
-          const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + row * DK + 4 * half_lane;
-          float4 f[kBoxes];
-          float most = 0.0f;
+        constexpr int kRowsPer = STATE_ONLY ? 4 : 8;
+        const bool is_k = STATE_ONLY || warp >= 8;
+        const int row0 = STATE_ONLY ? warp * 4 : (warp & 7) * 8;
+        const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + row0 * DK + lane * (DK / 32);
+        Pair f[kRowsPer][kBoxes];
+        float mine = 0.0f;  // of row `lane`
 #pragma unroll
-          for (int i = 0; i < kBoxes; ++i) {
-            f[i] = *(const float4*)(raw + 64 * i);
-            // NaN counts as infinity.
-            const float a = fmaxf(fabsf(f[i].x), fabsf(f[i].y)), d = fmaxf(fabsf(f[i].z), fabsf(f[i].w));
-            const float sum = (f[i].x + f[i].y) + (f[i].z + f[i].w);
-            most = fmaxf(most, sum == sum ? fmaxf(a, d) : INFINITY);
+        for (int r = 0; r < kRowsPer; ++r) {
+          float most;
+          if constexpr (DK == 128) {
+            const float4 w = *(const float4*)(raw + r * DK);
+            f[r][0] = pair_of(w.x, w.y), f[r][kBoxes - 1] = pair_of(w.z, w.w);
+            most = most_of(most_of(w.x, w.y, w.z), w.w, 0.0f);
+          } else {
+            const float2 w = *(const float2*)(raw + r * DK);
+            f[r][0] = pair_of(w.x, w.y);
+            most = most_of(w.x, w.y, 0.0f);
           }
+          most = warp_most(most);
+          if (lane == r) mine = most;
+        }
+        const uint32_t biased = scale_biased(mine);
+        far |= far_biased(biased);
+        // A row of zeros has no part in the greatest factor.
+        if (lane < kRowsPer) (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u);
+        const float up = power_of(268u - biased);
+        uint8_t* box = smem + (is_k ? Sm::kK : Sm::kQ);
+        const int other = (is_k ? kBoxes : 1) * kBoxBytes;  // from hi to lo
+        if (DK == 128) box += (lane >> 4) * (is_k ? 1 : 2) * kBoxBytes;
 #pragma unroll
-          for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          far |= far_value(most);
-          const uint32_t biased = biased_of(most);
-          const float up = up_factor(biased);
-          // A key of zeros has no part in the greatest factor.
-          if (half_lane == 0) (is_k ? k_down : q_down)[row] = is_k && biased == 0 ? 0.0f : down_factor(biased);
-#pragma unroll
-          for (int i = 0; i < kBoxes; ++i) {
+        for (int r = 0; r < kRowsPer; ++r) {
+          const float u = __shfl_sync(0xffffffffu, up, r);
+          const Pair u2 = pair_of(u, u);
+          const int row = row0 + r;
+          if constexpr (DK == 128) {
             uint2 hi, lo;
-            split_pair(f[i].x * up, f[i].y * up, hi.x, lo.x);
-            split_pair(f[i].z * up, f[i].w * up, hi.y, lo.y);
-            const int at = row * 128 + (((half_lane >> 1) ^ (row & 7)) << 4) + ((half_lane & 1) << 3);
-            uint8_t* box = smem + (is_k ? Sm::kK + i * kBoxBytes : Sm::kQ + 2 * i * kBoxBytes) + at;
-            *(uint2*)box = hi;
-            *(uint2*)(box + (is_k ? kBoxes : 1) * kBoxBytes) = lo;
+            split_pair(mul2(f[r][0], u2), hi.x, lo.x);
+            split_pair(mul2(f[r][kBoxes - 1], u2), hi.y, lo.y);
+            uint8_t* to = box + row * 128 + ((((lane & 15) >> 1) ^ (row & 7)) << 4) + ((lane & 1) << 3);
+            *(uint2*)to = hi;
+            *(uint2*)(to + other) = lo;
+          } else {
+            uint32_t hi, lo;
+            split_pair(mul2(f[r][0], u2), hi, lo);
+            uint8_t* to = box + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + ((lane & 3) << 2);
+            *(uint32_t*)to = hi;
+            *(uint32_t*)(to + other) = lo;
           }
         }
       }
       // This column's values of 16 tokens.
-      float val[16];
+      Pair val[8];
       {
         const float* raw = (const float*)(smem + Sm::kRawV) + group * 16 * kMostDim + col;
         float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          val[i] = raw[i * kMostDim];
-          most = fmaxf(most, val[i] == val[i] ? fabsf(val[i]) : INFINITY);
+        for (int i = 0; i < 8; ++i) {
+          const float a = raw[2 * i * kMostDim], d = raw[(2 * i + 1) * kMostDim];
+          val[i] = pair_of(a, d);
+          most = most_of(most, a, d);
         }
-        far |= far_value(most);
+        far |= far_biased(scale_biased(most));
         v_most[group * 128 + col] = most;
       }
-      if (far) far_step[c & 1] = 1;
+      if (far) far_step[turn] = 1;
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       worker_sync();
-      if (tid == 0) far_step[(c + 1) & 1] = 0;
-      if (*(volatile int*)&far_step[c & 1]) {
+      if (tid == 0) {
+        far_step[turn ^ 1] = 0;
+        mbar_arrive(ready);
+      }
+      if (*(volatile int*)&far_step[turn]) {
         // Token by token.
-        if (lane == 0) mbar_arrive(ready);
         const float2 one = decay_over(decay, 1);
-        const float* kr = (const float*)(smem + Sm::kRawK) + group * kMine;
-        const float* qr = (const float*)(smem + Sm::kRawQ) + group * kMine;
+        const Pair hi = pair_of(one.x, one.x), lo = pair_of(one.y, one.y);
+        const float2* kr = (const float2*)(smem + Sm::kRawK) + group * (kMine / 2);
+        const float2* qr = (const float2*)(smem + Sm::kRawQ) + group * (kMine / 2);
         const float* vr = (const float*)(smem + Sm::kRawV) + col;
         for (int i = 0; i < m; ++i) {
           const float w = vr[i * kMostDim];
-          float sum = 0.0f;
+          const Pair w2 = pair_of(w, w);
+          Pair sum = 0;
 #pragma unroll
-          for (int j = 0; j < kMine; ++j) {
-            if (lead) x[j] = fmaf(x[j], one.x, x[j] * one.y);
-            x[j] = fmaf(kr[i * DK + j], w, x[j]);
-            if (!STATE_ONLY) sum = fmaf(qr[i * DK + j], x[j], sum);
-            if (!lead) x[j] = fmaf(x[j], one.x, x[j] * one.y);
+          for (int j = 0; j < kMine / 2; ++j) {
+            const float2 key = kr[i * (DK / 2) + j];
+            if (lead) x[j] = fma2(x[j], hi, mul2(x[j], lo));
+            x[j] = fma2(pair_of(key.x, key.y), w2, x[j]);
+            if (!STATE_ONLY) {
+              const float2 query = qr[i * (DK / 2) + j];
+              sum = fma2(pair_of(query.x, query.y), x[j], sum);
+            }
+            if (!lead) x[j] = fma2(x[j], hi, mul2(x[j], lo));
           }
           if (!STATE_ONLY) {
             float* sums = i & 1 ? v_most : x_most;
-            sums[group * 128 + col] = sum;
+            sums[group * 128 + col] = floats_of(sum).x + floats_of(sum).y;
             worker_sync();
             if (group == 0 && col < s.cols) {
               const float all = ((sums[col] + sums[128 + col]) + (sums[256 + col] + sums[384 + col])) * s.scale;
@@ -583,58 +693,55 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           }
         }
         worker_sync();  // the rows are read, and the sums
-        if (t + kStep < t1) fetch(t + kStep);
+        if (tid == 0 && t + kStep < t1) mbar_arrive(raw_empty);
         if (!STATE_ONLY) {
-          const float most = most_of_state();
-          far_state = biased_of(most) >= 255;
-          x_down = down_factor(biased_of(most));
-          if (t + kStep < t1) put_state(up_factor(biased_of(most)));
+          bound = most_of_state();
+          far_state = biased_of(bound) >= 254;
+          if (t + kStep < t1) put_state(bound);
         }
         // The issuing warp keeps step.
         if (ok) ok = warp_wait(far_seen, far_steps & 1, err);
         ++far_steps;
         continue;
       }
-      if (t + kStep < t1) fetch(t + kStep);
-      // The rows' factors: P takes k's over the greatest, w takes a^(63 - j + tail) and k's over that of all.
-      float p_down, w_down;
+      if (tid == 0 && t + kStep < t1) mbar_arrive(raw_empty);
+      // The keys' factors over the greatest (P), and with a^(63 - j + tail) over the greatest of those (w).
+      Pair keys[8];
+      float p_down, p_inv, w_down;
       {
+        const float* left = lefts + (m < kStep ? kStep : 0);
         const float k0 = k_down[lane], k1 = k_down[lane + 32];
-        const int last = m - 1 + tail;
-        const float w0 = lane < m ? k0 * power[last - lane] : 0.0f, w1 = lane + 32 < m ? k1 * power[last - lane - 32] : 0.0f;
-        float most_k = fmaxf(k0, k1), most_w = fmaxf(w0, w1);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          most_k = fmaxf(most_k, __shfl_xor_sync(0xffffffffu, most_k, o));
-          most_w = fmaxf(most_w, __shfl_xor_sync(0xffffffffu, most_w, o));
-        }
-        p_down = most_k;
-        if (warp == 0) {
-          const float inv = __uint_as_float((254u - biased_of(most_k)) << 23);  // a power of two's inverse
-          p_coef[lane] = k0 * inv * 0x1p-22f;
-          p_coef[lane + 32] = k1 * inv * 0x1p-22f;
-        }
+        p_down = warp_most(fmaxf(k0, k1));
+        const float most_w = warp_most(fmaxf(k0 * left[lane], k1 * left[lane + 32]));
+        p_inv = power_of(254u - biased_of(p_down)) * 0x1p-22f;
         // Below fp32's normal numbers there is nothing to add.
-        const uint32_t e = biased_of(most_w) >= 1 ? min(biased_of(most_w) + 1, 253u) : 0;
-        w_down = e ? __uint_as_float(e << 23) : 0.0f;
-        const float inv_w = e ? __uint_as_float((254u - e) << 23) : 0.0f;
-        const uint32_t biased = biased_of(fmaxf(fmaxf(v_most[col], v_most[128 + col]), fmaxf(v_most[256 + col], v_most[384 + col])));
-        const float up = up_factor(biased), down = down_factor(biased);
+        const uint32_t e = most_w >= 0x1p-126f ? min(biased_of(most_w) + 1, 253u) : 0;
+        w_down = power_of(e);
+        const uint32_t biased = scale_biased(
+            most_of(most_of(v_most[col], v_most[128 + col], v_most[256 + col]), v_most[384 + col], 0.0f));
+        const float up = power_of(268u - biased), down = power_of(biased - 14u);
+        const float inv_w = e ? power_of(254u - e) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 f = *(const float4*)(k_down + group * 16 + 4 * i);
+          keys[2 * i] = pair_of(f.x, f.y), keys[2 * i + 1] = pair_of(f.z, f.w);
+        }
         uint32_t hi[8], lo[8];
+        const Pair up2 = pair_of(up, up), inv2 = pair_of(inv_w, inv_w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) val[i] = mul2(val[i], up2);
         if (!STATE_ONLY) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) split_pair(val[2 * i] * up, val[2 * i + 1] * up, hi[i], lo[i]);
+          for (int i = 0; i < 8; ++i) split_pair(val[i], hi[i], lo[i]);
           tmem_st8(at_lane + Tm::kV + group * 8, hi);
           tmem_st8(at_lane + Tm::kVLo + group * 8, lo);
         }
-        float coef[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = group * 16 + i;
-          coef[i] = __shfl_sync(0xffffffffu, group < 2 ? w0 : w1, j & 31) * inv_w * up;
+        for (int i = 0; i < 4; ++i) {
+          const float4 l = *(const float4*)(left + group * 16 + 4 * i);
+          split_pair(mul2(val[2 * i], mul2(mul2(keys[2 * i], pair_of(l.x, l.y)), inv2)), hi[2 * i], lo[2 * i]);
+          split_pair(mul2(val[2 * i + 1], mul2(mul2(keys[2 * i + 1], pair_of(l.z, l.w)), inv2)), hi[2 * i + 1], lo[2 * i + 1]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) split_pair(val[2 * i] * coef[2 * i], val[2 * i + 1] * coef[2 * i + 1], hi[i], lo[i]);
         tmem_st8(at_lane + Tm::kW + group * 8, hi);
         tmem_st8(at_lane + Tm::kWLo + group * 8, lo);
         p_down *= down * 0x1p22f;
@@ -642,35 +749,34 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(ready);
+      if (lane == 0) mbar_arrive(values_ready);
 
       if (!STATE_ONLY) {
+        const Pair inv2 = pair_of(p_inv, p_inv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) keys[j] = mul2(mul2(keys[j], inv2), near[j]);
         if (ok) ok = warp_wait(score_full, steps & 1, err);
         tc_fence_after();
         // P of 16 keys: rows (tokens) 0..63 in the lanes of quarters 0 and 1, what q's lo adds in 2 and 3.
         float p[16];
         tmem_ld16(at_lane + Tm::kScore + group * 16, p);
-        const int i = col & (kStep - 1);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int key = group * 16 + j;
-          p[j] = key <= i ? p[j] * (p_coef[key] * power[max(i - key, 0)]) : 0.0f;
-        }
-        uint8_t* row = smem + Sm::kP + i * 128;
-        const int x0 = ((2 * group) ^ (i & 7)) << 4, x1 = ((2 * group + 1) ^ (i & 7)) << 4;
+        uint8_t* row = smem + Sm::kP + row_i * 128;
+        const int x0 = ((2 * group) ^ (row_i & 7)) << 4, x1 = ((2 * group + 1) ^ (row_i & 7)) << 4;
         uint32_t hi[8], lo[8];
         if (quarter < 2) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) split_pair(p[2 * j], p[2 * j + 1], hi[j], lo[j]);
+          for (int j = 0; j < 8; ++j) split_pair(mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]), hi[j], lo[j]);
           *(uint4*)(row + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4*)(row + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
           *(uint4*)(row + kBoxBytes + x0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           *(uint4*)(row + kBoxBytes + x1) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) hi[j] = half_pair(p[2 * j], p[2 * j + 1]);
+          for (int j = 0; j < 8; ++j) {
+            const float2 f = floats_of(mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]));
+            hi[j] = half_pair(f.x, f.y);
+          }
           *(uint4*)(row + 2 * kBoxBytes + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4*)(row + 2 * kBoxBytes + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
         }
@@ -679,43 +785,62 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
       }
-      // X.
+      // X, and a bound of it: 64 products of packed values are at most 2^36.
       const float from_down = x_down;
+      const float2 a = m == kStep ? fade : decay_over(decay, m);
       if (ok) ok = warp_wait(sums_full, steps & 1, err);
       tc_fence_after();
       {
-        const float2 a = m == kStep ? fade : decay_over(decay, m);
+        const Pair a_hi = pair_of(a.x, a.x), a_lo = pair_of(a.y, a.y), w2 = pair_of(w_down, w_down);
 #pragma unroll
-        for (int half = 0; half < kMine / 16; ++half) {
+        for (int part = 0; part < kMine / 16; ++part) {
           float d[16];
-          tmem_ld16(at_lane + Tm::kDelta + group * kMine + 16 * half, d);
+          tmem_ld16(at_lane + Tm::kDelta + group * kMine + 16 * part, d);
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            x[16 * half + i] = fmaf(x[16 * half + i], a.x, fmaf(x[16 * half + i], a.y, d[i] * w_down));
+          for (int i = 0; i < 8; ++i) {
+            Pair& y = x[8 * part + i];
+            y = fma2(y, a_hi, fma2(y, a_lo, mul2(pair_of(d[2 * i], d[2 * i + 1]), w2)));
+          }
         }
       }
       if (!STATE_ONLY) {
-        const float most = most_of_state();
-        far_state = biased_of(most) >= 255;
-        x_down = down_factor(biased_of(most));
-        if (t + kStep < t1) put_state(up_factor(biased_of(most)));
+        bound = fmaf(bound, a.x, 0x1p36f * w_down) * 1.000001f;
+        far_state = biased_of(bound) >= 254;
+        if (t + kStep < t1) put_state(bound);
         if (ok) ok = warp_wait(out_full, steps & 1, err);
         tc_fence_after();
         float from[16], own[16];
         tmem_ld16(at_lane + Tm::kFrom + group * 16, from);
         tmem_ld16(at_lane + Tm::kScore + group * 16, own);
-        if (col < s.cols) {
+        const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down, from_down), s2 = pair_of(s.scale, s.scale);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = group * 16 + i;
-            const float o = (from[i] * (from_down * power[r + lead]) + own[i] * p_down) * (q_down[r] * s.scale);
-            if (r < m) {
-              float* to = out + token(t + r) * s.out.token + col;
-              *to = s.accumulate ? *to + o : o;
-            }
+        for (int i = 0; i < 4; ++i) {
+          const float4 w = *(const float4*)(since + group * 16 + 4 * i), d = *(const float4*)(q_down + group * 16 + 4 * i);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int e = 4 * i + 2 * j;
+            const Pair o = fma2(pair_of(from[e], from[e + 1]), mul2(j ? pair_of(w.z, w.w) : pair_of(w.x, w.y), f2),
+                                mul2(pair_of(own[e], own[e + 1]), p2));
+            const float2 y = floats_of(mul2(o, mul2(j ? pair_of(d.z, d.w) : pair_of(d.x, d.y), s2)));
+            own[e] = y.x, own[e + 1] = y.y;
           }
         }
-        tc_fence_before();
+        const int rows = col < s.cols ? min(m - group * 16, 16) : 0;  // of this thread's
+        const int64_t pitch = s.back ? -s.out.token : s.out.token;
+        float* to = out + token(t + group * 16) * s.out.token + col;
+        if (s.accumulate) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < rows) own[i] = to[i * pitch] + own[i];
+        }
+        if (rows == 16) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) to[i * pitch] = own[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < rows) to[i * pitch] = own[i];
+        }
       }
       ++steps;
     }
@@ -723,21 +848,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     if (!STATE_ONLY && !s.accumulate)
       for (int r = n + part * 4 + group; r < s.seq; r += 4 * parts.segments)
         if (col < s.cols) out[(int64_t)r * s.out.token + col] = 0.0f;
-    if (STATE_ONLY) {
-      float* to = parts.states + ((int64_t)unit * (parts.segments - 1) + part) * s.rows * s.cols;
+    if (STATE_ONLY || (s.to.p != nullptr && part == parts.segments - 1)) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int r = group * kMine + i;
-        if (r < s.rows && col < s.cols) to[(int64_t)r * s.cols + col] = x[i];
-      }
-    } else if (s.to.p != nullptr && part == parts.segments - 1) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int r = group * kMine + i;
-        if (r < s.rows && col < s.cols) {
+        const float y = i & 1 ? floats_of(x[i / 2]).y : floats_of(x[i / 2]).x;
+        if (r >= s.rows || col >= s.cols) continue;
+        if (STATE_ONLY) {
+          parts.states[((int64_t)unit * (parts.segments - 1) + part) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
+        } else {
           float* to = s.to.p + state + r * s.to.si + col * s.to.sj;
-          const float y = x[i] * s.to_factor;
-          *to = s.accumulate_state ? *to + y : y;
+          *to = s.accumulate_state ? *to + y * s.to_factor : y * s.to_factor;
         }
       }
     }
@@ -746,7 +867,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   if (warp == kWorkers / 32)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Tm::kTake));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
 }
 
 // From each segment's own state the state that the next one starts from, in place.
@@ -814,6 +935,11 @@ void launch_chunks(const Scan& s, const ScanParts& parts, int blocks, int* err, 
   TYSOR_CUDA(cudaGetDevice(&device));
   const uint64_t bit = 1ull << (device & 63);
   if (!(set.load(std::memory_order_relaxed) & bit)) {
+    // The warps share out what the block is launched with.
+    cudaFuncAttributes made;
+    TYSOR_CUDA(cudaFuncGetAttributes(&made, kernel));
+    if (made.numRegs * kScanThreads < kWorkers * kWorkerRegs + (kScanThreads - kWorkers) * kOtherRegs)
+      throw CudaError("decay_attention: the kernel was built with too few registers");
     TYSOR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<DK>::kBytes));
     set.fetch_or(bit, std::memory_order_relaxed);
   }
