@@ -1,7 +1,10 @@
 // Log probabilities of given tokens with entropy and best alternatives
-// (lm_ops.cuh), forward and backward.
+// (lm_ops.cuh), forward and backward.  Both read the logits once (the gradient
+// writes as much): HBM bounds them, or for a few rows a launch.
 #include <limits.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "lm_ops.cuh"
 
@@ -9,10 +12,27 @@ namespace tysor {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kLoads = 4;                       // float4 that a thread has on their way
+constexpr int kSlab = 4 * kLoads * kThreads;    // values that a block takes at a time
+constexpr int kMostParts = 8;                   // blocks of a cluster
+constexpr float kLog2e = 1.4426950408889634f;
 
 void check_launch() {
   g_launches.fetch_add(1, std::memory_order_relaxed);
   TYSOR_CUDA(cudaGetLastError());
+}
+
+// 2^x to about 2^-22, subnormal results as 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The greatest of three; NaN if one is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 __device__ __forceinline__ int token_of(float id, int width, int* err) {
@@ -24,111 +44,405 @@ __device__ __forceinline__ int token_of(float id, int width, int* err) {
   return (int)id;
 }
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float* red, F f) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = f(v, red[w]);
-  return v;
+// Of some logits: the greatest m, the sum s of 2^y and the sum t of 2^y y, with
+// y = (logit - m) log2(e) / T.  (-inf, 0, 0) of none; NaN or +inf as m: not finite.
+struct Sums {
+  float m, s, t;
+};
+// y is kept from -inf, whose 2^y = 0 must stay 0 when multiplied by it.
+__device__ __forceinline__ float exponent(float z, float m, float c) { return fmaxf((z - m) * c, -200.0f); }
+__device__ __forceinline__ bool finite_top(float m) { return m > -INFINITY && m < INFINITY; }
+// The sums over a greater greatest value.
+__device__ __forceinline__ void raise(Sums& a, float m, float c) {
+  const float d = exponent(a.m, m, c), f = exp2_fast(d);
+  a.t = f * fmaf(a.s, d, a.t);
+  a.s *= f;
+  a.m = m;
+}
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  const float m = max3(a.m, b.m, -INFINITY);
+  if (!finite_top(m)) return {m, 0.0f, 0.0f};
+  if (a.m == -INFINITY) return b;
+  if (b.m == -INFINITY) return a;
+  raise(a, m, c);
+  raise(b, m, c);
+  return {m, a.s + b.s, a.t + b.t};
 }
 
+// A token and its logit as one number: the greater logit, then the lower id, is the
+// greater number.  (-0 counts as 0.)
+__device__ __forceinline__ uint64_t key_of(float z, int id) {
+  const uint32_t u = __float_as_uint(z == 0.0f ? 0.0f : z);
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~id;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// The candidates for a row's best tokens: those above `floor` so far.  When more
+// than `limit` have come, the best `top` stay and the floor rises to the last of
+// them.  (Later slabs hold greater ids, so a logit equal to the floor is behind.)
+constexpr int kListSize = kSlab + 4 * kMaxTopTokens + 8;
+struct TopList {
+  uint64_t key[kListSize];
+  uint64_t best[kMaxTopTokens];
+  uint64_t incoming[kMostParts * kMaxTopTokens];  // the cluster's, in the first block
+  int count, found, digit, need, same;
+  uint32_t lowest;
+  int hist[256];
+  float warp_floor[kThreads / 32];
+};
+
+// Leaves the greatest `top` of the list's keys at its start, by their digits of 8
+// bits from the highest on.  All of the block's threads.
+__device__ void keep_best(TopList& l, int top) {
+  const int tid = threadIdx.x, n = l.count;
+  __syncthreads();
+  if (n <= top) return;
+  uint64_t prefix = 0, mask = 0;
+  int need = top;
+  for (int shift = 56;; shift -= 8) {
+    l.hist[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads)
+      if ((l.key[i] & mask) == prefix) atomicAdd(&l.hist[(int)(l.key[i] >> shift) & 255], 1);
+    __syncthreads();
+    if (tid < 32) {
+      // Lane l counts the digits 8 (31 - l) ... of the greatest first.
+      const int first = 8 * (31 - tid);
+      int sum = 0;
+      for (int i = 0; i < 8; ++i) sum += l.hist[first + i];
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (tid >= o) before += x;
+      }
+      before -= sum;
+      if (before < need && before + sum >= need) {
+        int d = first + 7;
+        while (before + l.hist[d] < need) before += l.hist[d--];
+        l.digit = d;
+        l.need = need - before;
+        l.same = l.hist[d];
+      }
+    }
+    __syncthreads();
+    prefix |= (uint64_t)l.digit << shift;
+    mask |= (uint64_t)255 << shift;
+    need = l.need;
+    if (l.same == need || shift == 0) break;  // keys differ: at the last digit they are alone
+  }
+  if (tid == 0) l.found = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads)
+    if ((l.key[i] & mask) >= prefix) l.best[atomicAdd(&l.found, 1)] = l.key[i];
+  __syncthreads();
+  if (tid < top) l.key[tid] = l.best[tid];
+  if (tid == 0) l.count = top;
+  __syncthreads();
+}
+
+__device__ __forceinline__ float below(float z) { return nextafterf(z, -INFINITY); }
+
+// A first floor from a slab's greatest values, one a thread: of each warp's 32 the
+// one that enough are not below, so that all warps together hold `top` of them.
+__device__ __forceinline__ float first_floor(TopList& l, float most, int top) {
+  const int lane = threadIdx.x & 31, each = (top + kThreads / 32 - 1) / (kThreads / 32);
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {  // sorted to fall from lane 0 on
+      const float other = __shfl_xor_sync(0xffffffffu, most, j);
+      const bool first = (lane & j) == 0, falling = (lane & k) == 0;
+      most = first == falling ? fmaxf(most, other) : fminf(most, other);
+    }
+  most = __shfl_sync(0xffffffffu, most, each - 1);
+  if (lane == 0) l.warp_floor[threadIdx.x >> 5] = most;
+  __syncthreads();
+  float floor = l.warp_floor[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) floor = fminf(floor, l.warp_floor[w]);
+  return floor == -INFINITY ? floor : below(floor);
+}
+
+__device__ __forceinline__ void add_candidate(TopList& l, float z, int id, bool wanted) {
+  const uint32_t mask = __ballot_sync(0xffffffffu, wanted);
+  if (mask == 0) return;
+  const int lane = threadIdx.x & 31;
+  int at = 0;
+  if (lane == 0) at = atomicAdd(&l.count, __popc(mask));
+  at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
+  if (wanted) l.key[at] = key_of(z, id);
+}
+
+// One pass over a row, which a cluster of gridDim.y blocks shares where rows are few
+// (its first block joins their sums, and their best tokens through distributed shared
+// memory).
+template <bool TOP>
 __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, const float* __restrict__ logits,
                                                             const float* __restrict__ ids, float* __restrict__ out,
                                                             float* __restrict__ entropy, float* __restrict__ top_ids,
                                                             float* __restrict__ top_logprobs,
                                                             float* __restrict__ stats, int* err) {
-  __shared__ float red[kThreads / 32];
+  __shared__ Sums warp_part[kThreads / 32];
+  __shared__ Sums part[kMostParts];
+  __shared__ int part_count[kMostParts];
+  extern __shared__ __align__(16) uint8_t dynamic[];
+  TopList& list = *(TopList*)dynamic;  // with TOP alone
   const int64_t r = blockIdx.x;
+  const int parts = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
+  // Arrives for "this block runs": the first block's shared memory is written
+  // only once every block of the cluster has got here.
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const float c = kLog2e / s.temperature;
   const float* row = logits + r * s.width;
-  auto add = [](float a, float b) { return a + b; };
-  auto most = [](float a, float b) { return a > b || a != a ? a : b; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < s.width; i += kThreads) m = most(row[i], m);
-  m = block_reduce(m, red, most);
-  const bool none = m == -INFINITY, bad = !(m < INFINITY);
-  float sum = 0.0f, dot = 0.0f;
-  if (!none && !bad)
-    for (int i = threadIdx.x; i < s.width; i += kThreads) {
-      const float y = (row[i] - m) / s.temperature, e = expf(y);
-      sum += e;
-      if (e > 0.0f) dot += e * y;
+  // Chunks of whole float4 from the row's first 16-byte boundary; the values before it
+  // and after the last whole float4 go to the first block.
+  const int head = min(s.width, (int)((4 - (((uintptr_t)row >> 2) & 3)) & 3));
+  const int quads = (s.width - head) / 4, per = (quads + parts - 1) / parts;
+  const int q0 = min(quads, rank * per), q1 = min(quads, q0 + per);
+  const int tail = head + 4 * quads;
+  const float4* body = (const float4*)(row + head);
+  const int limit = max(4 * s.top, 256);
+  Sums o{-INFINITY, 0.0f, 0.0f};
+  bool bad = false;
+  float floor = -INFINITY;
+  auto one = [&](float z) {
+    if (!finite_top(z)) {
+      bad |= !(z == -INFINITY);
+      return;
     }
-  sum = block_reduce(sum, red, add);
-  dot = block_reduce(dot, red, add);
-  if (bad) m = sum = NAN;
-  const float log_sum = logf(sum);
-  if (threadIdx.x == 0) {
-    if (stats != nullptr) *(float2*)(stats + 2 * r) = make_float2(m, sum);
-    if (entropy != nullptr) entropy[r] = none ? 0.0f : log_sum - dot / sum;
+    if (z > o.m) {
+      if (o.m > -INFINITY) raise(o, z, c);
+      o.m = z;
+    }
+    const float y = exponent(z, o.m, c), e = exp2_fast(y);
+    o.s += e;
+    o.t = fmaf(e, y, o.t);
+  };
+  if (TOP) {
+    if (tid == 0) list.count = 0;
+    __syncthreads();
   }
-  auto value = [&](int id) { return none ? -INFINITY : (row[id] - m) / s.temperature - log_sum; };
-  for (int e = threadIdx.x; e < s.given; e += kThreads) {
+  if (rank == 0) {
+    const bool here = tid < head;
+    const float z = here ? row[tid] : -INFINITY;
+    if (here) one(z);
+    if (TOP) add_candidate(list, z, tid, here && z > -INFINITY);
+  }
+  for (int base = q0; base < q1; base += kLoads * kThreads) {
+    float4 f[kLoads];
+    const int i = base + tid;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+      f[u] = i + u * kThreads < q1 ? body[i + u * kThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    float most = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) most = max3(max3(most, f[u].x, f[u].y), f[u].z, f[u].w);
+    if (finite_top(most)) {
+      if (most > o.m) {
+        if (o.m > -INFINITY) raise(o, most, c);
+        o.m = most;
+      }
+      float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const float y0 = exponent(f[u].x, o.m, c), y1 = exponent(f[u].y, o.m, c);
+        const float y2 = exponent(f[u].z, o.m, c), y3 = exponent(f[u].w, o.m, c);
+        const float e0 = exp2_fast(y0), e1 = exp2_fast(y1), e2 = exp2_fast(y2), e3 = exp2_fast(y3);
+        sum += (e0 + e1) + (e2 + e3);
+        dot = fmaf(e0, y0, fmaf(e1, y1, fmaf(e2, y2, fmaf(e3, y3, dot))));
+      }
+      o.s += sum;
+      o.t += dot;
+    } else {
+      bad |= !(most == -INFINITY);
+    }
+    if (TOP) {
+      if (base == q0) floor = first_floor(list, most == most ? most : -INFINITY, s.top);
+      if (__any_sync(0xffffffffu, most > floor)) {
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          const int id = head + 4 * (i + u * kThreads);
+          if (!__any_sync(0xffffffffu, max3(max3(f[u].x, f[u].y, f[u].z), f[u].w, -INFINITY) > floor)) continue;
+          add_candidate(list, f[u].x, id, f[u].x > floor);
+          add_candidate(list, f[u].y, id + 1, f[u].y > floor);
+          add_candidate(list, f[u].z, id + 2, f[u].z > floor);
+          add_candidate(list, f[u].w, id + 3, f[u].w > floor);
+        }
+      }
+      __syncthreads();
+      if (list.count > limit) {
+        keep_best(list, s.top);
+        // The last of those that stay: what comes later has to be above it.
+        if (tid < 32) {
+          uint32_t low = 0xffffffffu;
+          for (int k = tid; k < s.top; k += 32) low = min(low, (uint32_t)(list.key[k] >> 32));
+          low = __reduce_min_sync(0xffffffffu, low);
+          if (tid == 0) list.lowest = low;
+        }
+        __syncthreads();
+        floor = logit_of((uint64_t)list.lowest << 32);
+      }
+      // (The next slab's first addition comes after all have read the count.)
+      __syncthreads();
+    }
+  }
+  if (rank == 0) {
+    const bool here = tid < s.width - tail;
+    const float z = here ? row[tail + tid] : -INFINITY;
+    if (here) one(z);
+    if (TOP) add_candidate(list, z, tail + tid, here && z > floor);
+  }
+  if (bad) o = {NAN, 0.0f, 0.0f};
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1)
+    o = join(o, {__shfl_xor_sync(0xffffffffu, o.m, k), __shfl_xor_sync(0xffffffffu, o.s, k), __shfl_xor_sync(0xffffffffu, o.t, k)}, c);
+  if ((tid & 31) == 0) warp_part[tid >> 5] = o;
+  __syncthreads();
+  if (TOP) keep_best(list, s.top);
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (tid == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) o = join(o, warp_part[w], c);
+    uint32_t dst;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"((uint32_t)__cvta_generic_to_shared(&part[rank])));
+    asm volatile("st.shared::cluster.f32 [%0], %1;\n\tst.shared::cluster.f32 [%0 + 4], %2;\n\tst.shared::cluster.f32 [%0 + 8], %3;" ::"r"(
+                     dst), "f"(o.m), "f"(o.s), "f"(o.t)
+                 : "memory");
+    if (TOP) {
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"((uint32_t)__cvta_generic_to_shared(&part_count[rank])));
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst), "r"(list.count) : "memory");
+    }
+  }
+  if (parts > 1) {
+    if (TOP && tid < list.count) {
+      uint32_t dst;
+      const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&list.incoming[rank * kMaxTopTokens + tid]);
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"(mine));
+      asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(dst), "l"(list.key[tid]) : "memory");
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank != 0) return;
+    if (TOP) {
+      int n = 0;
+      for (int p = 0; p < parts; ++p) {
+        if (tid < part_count[p]) list.key[n + tid] = list.incoming[p * kMaxTopTokens + tid];
+        n += part_count[p];
+      }
+      if (tid == 0) list.count = n;
+      __syncthreads();
+      keep_best(list, s.top);
+    }
+  }
+  __syncthreads();
+  Sums all = part[0];
+  for (int w = 1; w < parts; ++w) all = join(all, part[w], c);
+  const bool none = all.m == -INFINITY, fine = finite_top(all.m);
+  const double log_sum = log((double)all.s);
+  if (tid == 0) {
+    if (stats != nullptr) *(float2*)(stats + 2 * r) = none || fine ? make_float2(all.m, all.s) : make_float2(NAN, NAN);
+    if (entropy != nullptr)
+      entropy[r] = none ? 0.0f : fine ? (float)(log_sum - 0.6931471805599453 * (double)all.t / (double)all.s) : NAN;
+  }
+  auto value = [&](float z) {
+    return none ? -INFINITY : fine ? (float)(((double)z - (double)all.m) / (double)s.temperature - log_sum) : NAN;
+  };
+  for (int e = tid; e < s.given; e += kThreads) {
     const int id = token_of(ids[r * s.given + e], s.width, err);
-    out[r * s.given + e] = id < 0 ? 0.0f : value(id);
+    out[r * s.given + e] = id < 0 ? 0.0f : value(row[id]);
   }
-  // The best token below the one before, one by one.
-  float last = INFINITY;
-  int last_id = -1;
-  for (int k = 0; k < s.top; ++k) {
-    float best = -INFINITY;
-    int id = INT_MAX;
-    for (int i = threadIdx.x; i < s.width; i += kThreads) {
-      const float v = row[i];
-      if ((v < last || (v == last && i > last_id)) && v > best) best = v, id = i;
-    }
-    const float all = block_reduce(best, red, most);
-    const float at = block_reduce(best == all ? (float)id : 1e30f, red, [](float a, float b) { return fminf(a, b); });
-    const bool found = all > -INFINITY && !bad;
-    last = all, last_id = found ? (int)at : 0;
-    if (threadIdx.x == 0) {
-      top_ids[r * s.top + k] = found ? at : -1.0f;
-      top_logprobs[r * s.top + k] = bad ? NAN : found ? value(last_id) : -INFINITY;
+  if (TOP && tid < s.top) {
+    const int n = fine ? list.count : 0;
+    if (tid < n) {
+      const uint64_t key = list.key[tid];
+      int place = 0;
+      for (int k = 0; k < n; ++k) place += list.key[k] > key;
+      top_ids[r * s.top + place] = (float)id_of(key);
+      top_logprobs[r * s.top + place] = value(logit_of(key));
+    } else {
+      top_ids[r * s.top + tid] = -1.0f;
+      top_logprobs[r * s.top + tid] = none || fine ? -INFINITY : NAN;
     }
   }
 }
 
+// With y as above, p = 2^y / s and ln p = y ln 2 - ln s, a value's gradient is 2^y (a + b y)
+// with a and b of the row; the given tokens' own terms are added after.  One block per row
+// and chunk of columns.
+template <bool VEC>
 __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(
-    LogprobShape s, const float* __restrict__ logits, const float* __restrict__ ids, const float* __restrict__ stats,
-    const float* __restrict__ entropy, const float* __restrict__ dout, const float* __restrict__ dentropy,
-    float* __restrict__ grad, int accumulate, int* err) {
+    LogprobShape s, int chunk, const float* __restrict__ logits, const float* __restrict__ ids,
+    const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ dout,
+    const float* __restrict__ dentropy, float* __restrict__ grad, int accumulate, int* err) {
   __shared__ int token[kMaxGivenTokens];
   __shared__ float up[kMaxGivenTokens];
   const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, c0 = blockIdx.y * chunk, c1 = min(s.width, c0 + chunk);
   const float* row = logits + r * s.width;
   float* g = grad + r * s.width;
   const float2 st = *(const float2*)(stats + 2 * r);
-  for (int e = threadIdx.x; e < s.given; e += kThreads) {
+  const float dh = dentropy != nullptr ? dentropy[r] : 0.0f, h = dentropy != nullptr ? entropy[r] : 0.0f;
+  for (int e = tid; e < s.given; e += kThreads) {
     token[e] = dout != nullptr ? token_of(ids[r * s.given + e], s.width, err) : -1;
     up[e] = token[e] < 0 ? 0.0f : dout[r * s.given + e];
   }
   __syncthreads();
+  if (st.x == -INFINITY) {  // nothing but -inf
+    if (!accumulate)
+      for (int i = c0 + tid; i < c1; i += kThreads) g[i] = 0.0f;
+    return;
+  }
   float sum = 0.0f;
   for (int e = 0; e < s.given; ++e) sum += up[e];
-  const float dh = dentropy != nullptr ? dentropy[r] : 0.0f, h = dentropy != nullptr ? entropy[r] : 0.0f;
-  const bool none = st.x == -INFINITY;
-  const float log_sum = logf(st.y), inv = 1.0f / s.temperature;
-  for (int i = threadIdx.x; i < s.width; i += kThreads) {
-    float d = 0.0f;
-    if (!none) {
-      const float lp = (row[i] - st.x) / s.temperature - log_sum, p = expf(lp);
-      d = p == 0.0f ? 0.0f : -p * (sum + dh * (lp + h)) * inv;
+  const float inv_t = 1.0f / s.temperature, c = kLog2e / s.temperature;
+  const float over = -inv_t / st.y;
+  const float a = over * (sum + dh * (h - logf(st.y))), b = over * dh * 0.6931471805599453f;
+  auto of = [&](float z) {
+    const float y = exponent(z, st.x, c);
+    return exp2_fast(y) * fmaf(b, y, a);
+  };
+  const int head = VEC ? min(c1 - c0, (int)((4 - (((uintptr_t)(row + c0) >> 2) & 3)) & 3)) : 0;
+  const int quads = VEC ? (c1 - c0 - head) / 4 : 0;
+  const float4* src = (const float4*)(row + c0 + head);
+  float4* dst = (float4*)(g + c0 + head);
+  for (int i = tid; i < quads; i += kLoads * kThreads) {
+    float4 f[kLoads], old[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u)
+      if (i + u * kThreads < quads) f[u] = src[i + u * kThreads];
+    if (accumulate)
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u)
+        if (i + u * kThreads < quads) old[u] = dst[i + u * kThreads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      if (i + u * kThreads >= quads) break;
+      float4 d = make_float4(of(f[u].x), of(f[u].y), of(f[u].z), of(f[u].w));
+      if (accumulate) d.x += old[u].x, d.y += old[u].y, d.z += old[u].z, d.w += old[u].w;
+      dst[i + u * kThreads] = d;
     }
-    g[i] = accumulate ? g[i] + d : d;
   }
+  auto one = [&](int at) {
+    const float d = of(row[at]);
+    g[at] = accumulate ? g[at] + d : d;
+  };
+  if (VEC && tid < head) one(c0 + tid);
+  for (int at = c0 + head + 4 * quads + tid; at < c1; at += kThreads) one(at);
   __syncthreads();
-  if (none) return;
-  for (int e = threadIdx.x; e < s.given; e += kThreads) {
-    bool first = token[e] >= 0;
-    for (int f = 0; f < e; ++f) first = first && token[f] != token[e];
+  // A token given twice takes its terms in order.
+  for (int e = tid; e < s.given; e += kThreads) {
+    const int id = token[e];
+    if (id < c0 || id >= c1) continue;
+    bool first = true;
+    for (int f = 0; f < e; ++f) first = first && token[f] != id;
     if (!first) continue;
-    float d = 0.0f;
-    for (int f = e; f < s.given; ++f)
-      if (token[f] == token[e]) d += up[f];
-    g[token[e]] += d * inv;
+    float d = up[e];
+    for (int f = e + 1; f < s.given; ++f)
+      if (token[f] == id) d += up[f];
+    g[id] += d * inv_t;
   }
 }
 
@@ -137,8 +451,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(
 void launch_token_logprobs(const LogprobShape& s, const float* logits, const float* ids, float* out, float* entropy,
                            float* top_ids, float* top_logprobs, float* stats, int* err, cudaStream_t st) {
   if (s.rows <= 0) return;
-  logprobs_kernel<<<(unsigned)s.rows, kThreads, 0, st>>>(s, logits, ids, out, entropy, top_ids, top_logprobs, stats,
-                                                         err);
+  // Rows that would leave SMs without a block are shared by a cluster's.
+  int parts = 1;
+  while (parts < kMostParts && s.rows * parts * 2 <= 148 * 4 && s.width / parts > kSlab) parts *= 2;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)s.rows, (unsigned)parts);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = s.top > 0 ? sizeof(TopList) : 0;
+  config.stream = st;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim = {1, (unsigned)parts, 1};
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  auto kernel = s.top > 0 ? logprobs_kernel<true> : logprobs_kernel<false>;
+  TYSOR_CUDA(cudaLaunchKernelEx(&config, kernel, s, logits, ids, out, entropy, top_ids, top_logprobs, stats, err));
   check_launch();
 }
 
@@ -146,8 +473,12 @@ void launch_token_logprobs_backward(const LogprobShape& s, const float* logits, 
                                     const float* entropy, const float* dout, const float* dentropy, float* grad,
                                     int accumulate, int* err, cudaStream_t st) {
   if (s.rows <= 0) return;
-  logprobs_backward_kernel<<<(unsigned)s.rows, kThreads, 0, st>>>(s, logits, ids, stats, entropy, dout, dentropy, grad,
-                                                                  accumulate, err);
+  // Chunks of a row that fill the SMs where rows are few, of at least a slab.
+  int64_t chunks = std::max<int64_t>(1, std::min<int64_t>(ceil_div(148 * 8, s.rows), ceil_div(s.width, kSlab)));
+  const int chunk = (int)(ceil_div(ceil_div(s.width, chunks), 4) * 4);
+  const dim3 grid((unsigned)s.rows, (unsigned)ceil_div(s.width, chunk));
+  auto kernel = (((uintptr_t)logits ^ (uintptr_t)grad) & 15) == 0 ? logprobs_backward_kernel<true> : logprobs_backward_kernel<false>;
+  kernel<<<grid, kThreads, 0, st>>>(s, chunk, logits, ids, stats, entropy, dout, dentropy, grad, accumulate, err);
   check_launch();
 }
 
