@@ -3,6 +3,7 @@
 // writes as much): HBM bounds them, or for a few rows a launch.
 #include <limits.h>
 #include <math.h>
+#include <stddef.h>
 
 #include <algorithm>
 
@@ -81,30 +82,53 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
 
-// The candidates for a row's best tokens: those above `floor` so far.  When more
-// than `limit` have come, the best `top` stay and the floor rises to the last of
-// them.  (Later slabs hold greater ids, so a logit equal to the floor is behind.)
-constexpr int kListSize = kSlab + 4 * kMaxTopTokens + 8;
+// The candidates for a row's best tokens: keys above `low` so far.  When more than
+// `limit` have come, the best `top` stay and `low` rises to the last of them.
+constexpr int kListSize = 1024, kCounted = 256;
 struct TopList {
   uint64_t key[kListSize];
   uint64_t best[kMaxTopTokens];
-  uint64_t incoming[kMostParts * kMaxTopTokens];  // the cluster's, in the first block
+  uint64_t low;
   int count, found, digit, need, same;
-  uint32_t lowest;
   int hist[256];
   float warp_floor[kThreads / 32];
+  uint64_t incoming[kMostParts * kMaxTopTokens];  // a cluster's, in its first block; not there without one
 };
 
-// Leaves the greatest `top` of the list's keys at its start, by their digits of 8
-// bits from the highest on.  All of the block's threads.
+// Leaves the greatest `top` of the list's keys at its start and the last of them as
+// `low`: of a few by counting the greater ones, of more by their digits of 8 bits from the
+// highest on.  All of the block's threads.
 __device__ void keep_best(TopList& l, int top) {
-  const int tid = threadIdx.x, n = l.count;
+  const int tid = threadIdx.x, n = min(l.count, kListSize);
   __syncthreads();
   if (n <= top) return;
+  constexpr int kPer = (kCounted + kThreads - 1) / kThreads;
+  if (n <= kCounted) {
+    uint64_t mine[kPer];
+    int place[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      mine[k] = tid + k * kThreads < n ? l.key[tid + k * kThreads] : 0;
+      place[k] = 0;
+      if ((tid & ~31) + k * kThreads < n)
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) place[k] += l.key[i] > mine[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (tid + k * kThreads < n && place[k] < top) {
+        l.key[place[k]] = mine[k];
+        if (place[k] == top - 1) l.low = mine[k];
+      }
+    if (tid == 0) l.count = top;
+    __syncthreads();
+    return;
+  }
   uint64_t prefix = 0, mask = 0;
   int need = top;
   for (int shift = 56;; shift -= 8) {
-    l.hist[tid] = 0;
+    for (int i = tid; i < 256; i += kThreads) l.hist[i] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += kThreads)
       if ((l.key[i] & mask) == prefix) atomicAdd(&l.hist[(int)(l.key[i] >> shift) & 255], 1);
@@ -141,14 +165,18 @@ __device__ void keep_best(TopList& l, int top) {
     if ((l.key[i] & mask) >= prefix) l.best[atomicAdd(&l.found, 1)] = l.key[i];
   __syncthreads();
   if (tid < top) l.key[tid] = l.best[tid];
-  if (tid == 0) l.count = top;
+  if (tid < 32) {
+    uint64_t least = ~0ull;
+    for (int k = tid; k < top; k += 32) least = min(least, l.best[k]);
+#pragma unroll
+    for (int k = 16; k > 0; k >>= 1) least = min(least, (uint64_t)__shfl_xor_sync(0xffffffffu, least, k));
+    if (tid == 0) l.low = least, l.count = top;
+  }
   __syncthreads();
 }
 
-__device__ __forceinline__ float below(float z) { return nextafterf(z, -INFINITY); }
-
 // A first floor from a slab's greatest values, one a thread: of each warp's 32 the
-// one that enough are not below, so that all warps together hold `top` of them.
+// one that enough are not below, so that all warps together hold `top` of at least that.
 __device__ __forceinline__ float first_floor(TopList& l, float most, int top) {
   const int lane = threadIdx.x & 31, each = (top + kThreads / 32 - 1) / (kThreads / 32);
 #pragma unroll
@@ -165,24 +193,71 @@ __device__ __forceinline__ float first_floor(TopList& l, float most, int top) {
   float floor = l.warp_floor[0];
 #pragma unroll
   for (int w = 1; w < kThreads / 32; ++w) floor = fminf(floor, l.warp_floor[w]);
-  return floor == -INFINITY ? floor : below(floor);
+  return floor;
 }
 
-__device__ __forceinline__ void add_candidate(TopList& l, float z, int id, bool wanted) {
-  const uint32_t mask = __ballot_sync(0xffffffffu, wanted);
-  if (mask == 0) return;
-  const int lane = threadIdx.x & 31;
-  int at = 0;
-  if (lane == 0) at = atomicAdd(&l.count, __popc(mask));
-  at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
-  if (wanted) l.key[at] = key_of(z, id);
+// Adds a key; whether it found no room.
+__device__ __forceinline__ bool add_candidate(TopList& l, uint64_t key) {
+  const int at = atomicAdd(&l.count, 1);
+  if (at < kListSize) l.key[at] = key;
+  return at >= kListSize;
+}
+
+// Candidates among a slab's values; the bits of those that found no room.
+__device__ __forceinline__ uint32_t add_candidates(TopList& l, const float4 (&f)[kLoads], int id, float floor,
+                                                   uint64_t low, uint32_t among) {
+  uint32_t left = 0;
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const float z[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+    if (!(max3(fmaxf(z[0], z[1]), z[2], z[3]) >= floor)) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (z[e] >= floor && (among >> (4 * u + e) & 1)) {
+        const uint64_t key = key_of(z[e], id + 4 * u * kThreads + e);
+        if (key > low && add_candidate(l, key)) left |= 1u << (4 * u + e);
+      }
+  }
+  return left;
+}
+
+__device__ __forceinline__ void load_slab(float4 (&f)[kLoads], const float4* body, int base, int end) {
+#pragma unroll
+  for (int u = 0; u < kLoads; ++u) {
+    const int i = base + threadIdx.x + u * kThreads;
+    f[u] = i < end ? body[i] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  }
+}
+
+// The candidates of [begin, end) once more, where they were more than the list holds
+// (rows that rise, or repeat one value): after each slab the best stay, until all have
+// found room or are behind.
+__device__ __noinline__ void add_slowly(TopList& l, const float4* body, int begin, int end, int head, int top) {
+  for (int base = begin; base < end; base += kLoads * kThreads) {
+    float4 f[kLoads];
+    load_slab(f, body, base, end);
+    uint32_t left = 0xffffu;
+    for (;;) {
+      const uint64_t low = l.low;
+      left = add_candidates(l, f, head + 4 * (base + (int)threadIdx.x), logit_of(low), low, left);
+      __syncthreads();
+      const bool more = l.count > kListSize;
+      keep_best(l, top);
+      __syncthreads();
+      if (!more) break;
+    }
+  }
 }
 
 // One pass over a row, which a cluster of gridDim.y blocks shares where rows are few
 // (its first block joins their sums, and their best tokens through distributed shared
-// memory).
+// memory).  Without best tokens HBM bounds it: 8192 rows of 32000, 1.05 GB, 164 us = 6.4
+// TB/s.  With them the block's waits and choices add up: 2048 rows of 32000 52 us without,
+// 65 with the best, 76 with 20, 125 with 128; they want many blocks on an SM (four instead
+// of seven, 104 us with 20) more than registers.  32 rows of 32000 take 8 us, with the 20
+// best 15: a launch, two exchanges of a cluster, and the choice among its blocks' best.
 template <bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, const float* __restrict__ logits,
+__global__ void __launch_bounds__(kThreads, TOP ? 7 : 6) logprobs_kernel(LogprobShape s, const float* __restrict__ logits,
                                                             const float* __restrict__ ids, float* __restrict__ out,
                                                             float* __restrict__ entropy, float* __restrict__ top_ids,
                                                             float* __restrict__ top_logprobs,
@@ -192,6 +267,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
   __shared__ int part_count[kMostParts];
   extern __shared__ __align__(16) uint8_t dynamic[];
   TopList& list = *(TopList*)dynamic;  // with TOP alone
+  static_assert(kMostParts * kMaxTopTokens <= kListSize, "the cluster's tokens fit the list");
   const int64_t r = blockIdx.x;
   const int parts = gridDim.y, rank = blockIdx.y, tid = threadIdx.x;
   // Arrives for "this block runs": the first block's shared memory is written
@@ -206,7 +282,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
   const int q0 = min(quads, rank * per), q1 = min(quads, q0 + per);
   const int tail = head + 4 * quads;
   const float4* body = (const float4*)(row + head);
-  const int limit = max(4 * s.top, 256);
+  // Candidates that stay without a choice: choosing early raises the floor, and of more
+  // than kCounted takes longer (2048 rows of 32000, 20 best: 76 us, with 84 staying 82; 128
+  // best: 125 us, with 160 staying 164).
+  const int limit = s.top <= 64 ? s.top + max(8, s.top / 4) : 2 * s.top + 8;
   Sums o{-INFINITY, 0.0f, 0.0f};
   bool bad = false;
   float floor = -INFINITY;
@@ -224,21 +303,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
     o.t = fmaf(e, y, o.t);
   };
   if (TOP) {
-    if (tid == 0) list.count = 0;
+    if (tid == 0) list.count = 0, list.low = key_of(-INFINITY, 0);  // tokens of -inf are not above
     __syncthreads();
   }
   if (rank == 0) {
     const bool here = tid < head;
     const float z = here ? row[tid] : -INFINITY;
     if (here) one(z);
-    if (TOP) add_candidate(list, z, tid, here && z > -INFINITY);
+    if (TOP && here && z > -INFINITY) add_candidate(list, key_of(z, tid));
+  }
+  // The list is looked after when twice as much of the row has been seen, not once a slab:
+  // the block's warps then seldom wait for one another.
+  int settled = q0, next = q0 + kLoads * kThreads, held = 0;
+  if (TOP) {
+    __syncthreads();
+    held = list.count;
   }
   for (int base = q0; base < q1; base += kLoads * kThreads) {
     float4 f[kLoads];
-    const int i = base + tid;
-#pragma unroll
-    for (int u = 0; u < kLoads; ++u)
-      f[u] = i + u * kThreads < q1 ? body[i + u * kThreads] : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    load_slab(f, body, base, q1);
     float most = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kLoads; ++u) most = max3(max3(most, f[u].x, f[u].y), f[u].z, f[u].w);
@@ -263,39 +346,32 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
     }
     if (TOP) {
       if (base == q0) floor = first_floor(list, most == most ? most : -INFINITY, s.top);
-      if (__any_sync(0xffffffffu, most > floor)) {
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          const int id = head + 4 * (i + u * kThreads);
-          if (!__any_sync(0xffffffffu, max3(max3(f[u].x, f[u].y, f[u].z), f[u].w, -INFINITY) > floor)) continue;
-          add_candidate(list, f[u].x, id, f[u].x > floor);
-          add_candidate(list, f[u].y, id + 1, f[u].y > floor);
-          add_candidate(list, f[u].z, id + 2, f[u].z > floor);
-          add_candidate(list, f[u].w, id + 3, f[u].w > floor);
-        }
-      }
-      __syncthreads();
-      if (list.count > limit) {
-        keep_best(list, s.top);
-        // The last of those that stay: what comes later has to be above it.
-        if (tid < 32) {
-          uint32_t low = 0xffffffffu;
-          for (int k = tid; k < s.top; k += 32) low = min(low, (uint32_t)(list.key[k] >> 32));
-          low = __reduce_min_sync(0xffffffffu, low);
-          if (tid == 0) list.lowest = low;
-        }
+      if (most >= floor) add_candidates(list, f, head + 4 * (base + tid), floor, list.low, 0xffffu);
+      const int end = base + kLoads * kThreads;
+      if (end >= next || end >= q1) {
+        next = q0 + 2 * (end - q0);
         __syncthreads();
-        floor = logit_of((uint64_t)list.lowest << 32);
+        const int count = list.count;
+        __syncthreads();
+        if (count > kListSize) {
+          if (tid == 0) list.count = held;
+          __syncthreads();
+          add_slowly(list, body, settled, min(end, q1), head, s.top);
+        } else if (count > limit) {
+          keep_best(list, s.top);
+        }
+        held = list.count;
+        if (list.low > key_of(-INFINITY, 0)) floor = logit_of(list.low);
+        settled = end;
+        __syncthreads();
       }
-      // (The next slab's first addition comes after all have read the count.)
-      __syncthreads();
     }
   }
   if (rank == 0) {
     const bool here = tid < s.width - tail;
     const float z = here ? row[tail + tid] : -INFINITY;
     if (here) one(z);
-    if (TOP) add_candidate(list, z, tail + tid, here && z > floor);
+    if (TOP && here && key_of(z, tail + tid) > list.low) add_candidate(list, key_of(z, tail + tid));
   }
   if (bad) o = {NAN, 0.0f, 0.0f};
 #pragma unroll
@@ -318,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
     }
   }
   if (parts > 1) {
-    if (TOP && tid < list.count) {
+    if (TOP && tid < list.count) {  // at most `top`
       uint32_t dst;
       const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&list.incoming[rank * kMaxTopTokens + tid]);
       asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(dst) : "r"(mine));
@@ -371,7 +447,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(LogprobShape s, cons
 
 // With y as above, p = 2^y / s and ln p = y ln 2 - ln s, a value's gradient is 2^y (a + b y)
 // with a and b of the row; the given tokens' own terms are added after.  One block per row
-// and chunk of columns.
+// and chunk of columns.  HBM bounds it: 8192 rows of 32000, 2.1 GB, 333 us = 6.3 TB/s.
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(
     LogprobShape s, int chunk, const float* __restrict__ logits, const float* __restrict__ ids,
@@ -457,7 +533,7 @@ void launch_token_logprobs(const LogprobShape& s, const float* logits, const flo
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)s.rows, (unsigned)parts);
   config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = s.top > 0 ? sizeof(TopList) : 0;
+  config.dynamicSmemBytes = s.top == 0 ? 0 : parts > 1 ? sizeof(TopList) : offsetof(TopList, incoming);
   config.stream = st;
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
