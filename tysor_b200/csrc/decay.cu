@@ -77,16 +77,39 @@ __device__ __forceinline__ float2 decay_over(float decay, int steps) {
   return make_float2(hi, (float)(a - (double)hi));
 }
 
+// Two fp32 values for the paired instructions.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 floats_of(Pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // ---- token by token --------------------------------------------------------------
 
-// A block holds `kSlice` columns of one head's state, four columns and every 32nd
+// A block holds `kSlice` columns of one head's state, four columns and every 16th
 // row a thread, and takes the tokens one after the other.  For few tokens what
 // counts is reading and writing the state.
-constexpr int kStepThreads = 256, kSlice = 32, kStage = 16;
 constexpr int kMostDim = 128;
+constexpr int kStepThreads = 128, kSlice = 32, kStage = 8;
+constexpr int kStepRows = kStepThreads / 8, kStepMine = kMostDim / kStepRows;  // rows at a time, and of a thread
 
 template <bool VEC>
-__global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ Scan s, int* err) {
+__global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_constant__ Scan s, int* err) {
   __shared__ float qs[kStage][kMostDim], ks[kStage][kMostDim];
   __shared__ __align__(16) float vs[kStage][kSlice];
   __shared__ __align__(16) float red[2][kStepThreads / 32][kSlice];
@@ -95,35 +118,29 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
   const int c0 = blockIdx.y * kSlice, width = min(kSlice, s.cols - c0);
   const int c = 4 * (lane & 7), r0 = warp * 4 + (lane >> 3);
   const int64_t state = (int64_t)unit * s.rows * s.cols;
-  float x[4][4];
+  Pair x[kStepMine][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 32 * i;
+  for (int i = 0; i < kStepMine; ++i) {
+    const int r = r0 + kStepRows * i;
+    float f[4] = {};
     if (VEC) {
-      float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (s.from.p != nullptr && r < s.rows && c < width)
-        f = *(const float4*)(s.from.p + state + (int64_t)r * s.cols + c0 + c);
-      x[i][0] = f.x, x[i][1] = f.y, x[i][2] = f.z, x[i][3] = f.w;
-    } else {
+      if (s.from.p != nullptr && r < s.rows && c < width) {
+        const float4 w = *(const float4*)(s.from.p + state + (int64_t)r * s.cols + c0 + c);
+        f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+      }
+    } else if (s.from.p != nullptr && r < s.rows) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        x[i][j] = s.from.p != nullptr && r < s.rows && c + j < width
-                      ? s.from.p[state + r * s.from.si + (c0 + c + j) * s.from.sj]
-                      : 0.0f;
+        if (c + j < width) f[j] = s.from.p[state + r * s.from.si + (c0 + c + j) * s.from.sj];
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[i][j] *= s.from_factor;
+    x[i][0] = pair_of(f[0] * s.from_factor, f[1] * s.from_factor);
+    x[i][1] = pair_of(f[2] * s.from_factor, f[3] * s.from_factor);
   }
   const int n = tokens_of(s, b, err);
   const float2 a = decay_over(decay_of(s, h, err), 1);
   const float *q = s.q.at(b, h), *k = s.k.at(b, h), *v = s.v.at(b, h) + c0;
   float* out = const_cast<float*>(s.out.at(b, h)) + c0;
-  auto fade = [&] {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[i][j] = fmaf(x[i][j], a.x, x[i][j] * a.y);
-  };
+  const Pair fade_hi = pair_of(a.x, a.x), fade_lo = pair_of(a.y, a.y);
   for (int t0 = 0; t0 < n; t0 += kStage) {
     const int m = min(kStage, n - t0);
     auto token = [&](int t) { return (int64_t)(s.back ? n - 1 - t0 - t : t0 + t); };
@@ -140,17 +157,23 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
     __syncthreads();
     for (int t = 0; t < m; ++t) {
       const float4 w = *(const float4*)&vs[t][c];
-      float o[4] = {};
-      if (!s.back) fade();
+      const Pair w2[2] = {pair_of(w.x, w.y), pair_of(w.z, w.w)};
+      Pair sum[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float key = ks[t][r0 + 32 * i], query = qs[t][r0 + 32 * i];
-        x[i][0] = fmaf(key, w.x, x[i][0]), x[i][1] = fmaf(key, w.y, x[i][1]);
-        x[i][2] = fmaf(key, w.z, x[i][2]), x[i][3] = fmaf(key, w.w, x[i][3]);
+      for (int i = 0; i < kStepMine; ++i) {
+        const float key = ks[t][r0 + kStepRows * i], query = qs[t][r0 + kStepRows * i];
+        const Pair key2 = pair_of(key, key), query2 = pair_of(query, query);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = fmaf(query, x[i][j], o[j]);
+        for (int j = 0; j < 2; ++j) {
+          Pair& y = x[i][j];
+          const Pair add = mul2(key2, w2[j]);
+          // Forward in time the state fades first, back in time afterwards.
+          y = s.back ? fma2(key2, w2[j], y) : fma2(y, fade_hi, fma2(y, fade_lo, add));
+          sum[j] = fma2(query2, y, sum[j]);
+          if (s.back) y = fma2(y, fade_hi, mul2(y, fade_lo));
+        }
       }
-      if (s.back) fade();
+      float o[4] = {floats_of(sum[0]).x, floats_of(sum[0]).y, floats_of(sum[1]).x, floats_of(sum[1]).y};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         o[j] += __shfl_xor_sync(0xffffffffu, o[j], 8);
@@ -172,14 +195,13 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
       if (i % kSlice < width) out[(int64_t)(n + i / kSlice) * s.out.token + i % kSlice] = 0.0f;
   if (s.to.p == nullptr) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 32 * i;
+  for (int i = 0; i < kStepMine; ++i) {
+    const int r = r0 + kStepRows * i;
     if (r >= s.rows || c >= width) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[i][j] *= s.to_factor;
+    const float2 y0 = floats_of(x[i][0]), y1 = floats_of(x[i][1]);
+    float4 f = make_float4(y0.x * s.to_factor, y0.y * s.to_factor, y1.x * s.to_factor, y1.y * s.to_factor);
     if (VEC) {
       float4* to = (float4*)(s.to.p + state + (int64_t)r * s.cols + c0 + c);
-      float4 f = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
       if (s.accumulate_state) {
         const float4 g = *to;
         f.x += g.x, f.y += g.y, f.z += g.z, f.w += g.w;
@@ -190,7 +212,8 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
       for (int j = 0; j < 4; ++j)
         if (c + j < width) {
           float* to = s.to.p + state + r * s.to.si + (c0 + c + j) * s.to.sj;
-          *to = s.accumulate_state ? *to + x[i][j] : x[i][j];
+          const float y = j == 0 ? f.x : j == 1 ? f.y : j == 2 ? f.z : f.w;
+          *to = s.accumulate_state ? *to + y : y;
         }
     }
   }
@@ -245,33 +268,14 @@ struct ScanSmem {
 
 struct ScanParts {
   int segments;  // blocks that share a head's tokens
-  float* states; // [unit][segments - 1][rows * cols]: each segment's own, then the next one's first
+  // [unit][segments][rows * cols], with more than one: in each segment's place the one before
+  // its own state, then the state that it starts from.  (The call's new state may replace the
+  // old one, so no segment but a head's only one reads that.)
+  float* states;
 };
 
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
 
-// Two fp32 values for the paired instructions.
-typedef unsigned long long Pair;
-__device__ __forceinline__ Pair pair_of(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 floats_of(Pair v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // The greatest magnitude; NaN if one is.
 __device__ __forceinline__ float most_of(float a, float b, float c) {
   float r;
@@ -503,8 +507,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < kMine; ++i) first[i] = 0.0f;
       if (!STATE_ONLY && col < s.cols) {
-        if (part > 0) {
-          const float* from = parts.states + ((int64_t)unit * (parts.segments - 1) + part - 1) * s.rows * s.cols;
+        if (parts.segments > 1) {
+          const float* from = parts.states + ((int64_t)unit * parts.segments + part) * s.rows * s.cols;
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
             const int r = group * kMine + i;
@@ -855,7 +859,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         const float y = i & 1 ? floats_of(x[i / 2]).y : floats_of(x[i / 2]).x;
         if (r >= s.rows || col >= s.cols) continue;
         if (STATE_ONLY) {
-          parts.states[((int64_t)unit * (parts.segments - 1) + part) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
+          parts.states[((int64_t)unit * parts.segments + part + 1) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
         } else {
           float* to = s.to.p + state + r * s.to.si + col * s.to.sj;
           *to = s.accumulate_state ? *to + y * s.to_factor : y * s.to_factor;
@@ -879,13 +883,15 @@ __global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant_
   const float decay = decay_of(s, h, err);
   const int r = i / s.cols, c = i - r * s.cols;
   float x = s.from.p != nullptr ? s.from.p[(int64_t)unit * elems + r * s.from.si + c * s.from.sj] * s.from_factor : 0.0f;
-  float* at = parts.states + (int64_t)unit * (parts.segments - 1) * elems + i;
+  float* at = parts.states + (int64_t)unit * parts.segments * elems + i;
+  at[0] = x;
   for (int j = 0; j + 1 < parts.segments; ++j) {
     int t0, t1;
     segment_of(n, parts.segments, j, &t0, &t1);
     const float2 a = decay_over(decay, t1 - t0);
-    x = fmaf(x, a.x, fmaf(x, a.y, at[(int64_t)j * elems]));
-    at[(int64_t)j * elems] = x;
+    at += elems;
+    x = fmaf(x, a.x, fmaf(x, a.y, *at));
+    *at = x;
   }
 }
 
@@ -924,7 +930,9 @@ int segments_of(int64_t units, int seq) {
 
 int64_t states_elems(const DecayShape& s) {
   if (s.seq < kChunkedFrom) return 0;
-  return (int64_t)s.batch * s.heads * (segments_of((int64_t)s.batch * s.heads, s.seq) - 1) * s.key_dim * s.value_dim;
+  const int64_t units = (int64_t)s.batch * s.heads;
+  const int segments = segments_of(units, s.seq);
+  return segments > 1 ? units * segments * s.key_dim * s.value_dim : 0;
 }
 
 template <int DK, bool STATE_ONLY, bool VEC>
