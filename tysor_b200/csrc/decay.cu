@@ -77,6 +77,33 @@ __device__ __forceinline__ float2 decay_over(float decay, int steps) {
   return make_float2(hi, (float)(a - (double)hi));
 }
 
+// A bounded wait of a warp whose lanes sleep meanwhile (try_wait with a hint of 2 ms): the
+// pipeline's roles wait for most of a step, and asking again and again takes issue slots
+// from those that work.
+__device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity, int* err) {
+  auto done = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(2000000u)
+        : "memory");
+    return ok != 0;
+  };
+  bool ok = done();
+  if (!ok) {
+    const long long start = clock64();
+    while (!(ok = done()))
+      if (clock64() - start > kWaitCycles) {
+        atomicCAS(err, 0, (int)kErrBarrierTimeout);
+        break;
+      }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // Two fp32 values for the paired instructions.
 typedef unsigned long long Pair;
 __device__ __forceinline__ Pair pair_of(float a, float b) {
@@ -266,6 +293,18 @@ struct ScanSmem {
   static constexpr int kBytes = kMisc + 9216 + 1024;
 };
 
+// Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces.
+struct ScanMaps {
+  CUtensorMap q, k, v;
+};
+__device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, int row, int head, int batch, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          to),
+      "l"((uint64_t)map), "r"(0), "r"(row), "r"(head), "r"(batch), "r"(bar)
+      : "memory");
+}
+
 struct ScanParts {
   int segments;  // blocks that share a head's tokens
   // [unit][segments][rows * cols], with more than one: in each segment's place the one before
@@ -311,9 +350,6 @@ __device__ __forceinline__ void split_pair(Pair v, uint32_t& hi, uint32_t& lo) {
 __device__ __forceinline__ void copy_async4(uint32_t to, const float* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void copy_async16(uint32_t to, const float* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
 
 // The tokens of a sequence that segment `part` takes: [first, last) of the order of the scan.
 __device__ __forceinline__ void segment_of(int n, int segments, int part, int* first, int* last) {
@@ -325,7 +361,8 @@ __device__ __forceinline__ void segment_of(int n, int segments, int part, int* f
 // STATE_ONLY: the segment's own state (from 0), for the segments behind it.  VEC: rows of
 // whole 16-byte pieces.
 template <int DK, bool STATE_ONLY, bool VEC>
-__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s, ScanParts parts,
+__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s,
+                                                               const __grid_constant__ ScanMaps maps, ScanParts parts,
                                                                int* err) {
   using Tm = ScanTmem<DK>;
   using Sm = ScanSmem<DK>;
@@ -357,7 +394,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   auto power = [&](int steps) { return steps == 0 ? 1.0f : expf(-decay * steps); };
 
   if (tid == 0) {
-    mbar_init(raw_full, 32 * kLoaders);
+    mbar_init(raw_full, VEC ? 1 : 32 * kLoaders);
     mbar_init(raw_empty, 1);
     mbar_init(ready, 1);
     mbar_init(values_ready, kWorkers / 32);
@@ -380,7 +417,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // Columns that no copy writes are 0.
-  if (s.rows != DK || s.cols != kMostDim)
+  if (!VEC && (s.rows != DK || s.cols != kMostDim))
     for (int i = tid; i < (Sm::kMisc - Sm::kRawQ) / 16; i += kScanThreads)
       ((uint4*)(smem + Sm::kRawQ))[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
@@ -389,6 +426,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const float *q = s.q.at(b, h), *k = s.k.at(b, h), *v = s.v.at(b, h);
   auto token = [&](int t) { return (int64_t)(s.back ? n - 1 - t : t); };
+  // Rows of a step as they lie in shared memory: boxes hold them as the tensor does.
+  const int key_pitch = VEC ? s.rows : DK, value_pitch = VEC ? s.cols : kMostDim;
+  const bool turned = VEC && s.back;
+  auto place = [&](int i) { return turned ? kStep - 1 - i : i; };
 
   if (warp >= kWorkers / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -399,7 +440,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       uint32_t steps = 0;  // those of the matrix unit
       bool ok = true;
       for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
-        ok = warp_wait(ready, c & 1, err);
+        ok = sleep_wait(ready, c & 1, err);
         if (!ok) break;
         tc_fence_after();
         if (*(volatile int*)&far_step[c & 1]) {
@@ -428,7 +469,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             }
         }
         __syncwarp();
-        ok = warp_wait(values_ready, steps & 1, err);
+        ok = sleep_wait(values_ready, steps & 1, err);
         if (!ok) break;
         tc_fence_after();
         if (leader) {
@@ -445,7 +486,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         }
         if (!STATE_ONLY) {
           __syncwarp();
-          ok = warp_wait(p_ready, steps & 1, err);
+          ok = sleep_wait(p_ready, steps & 1, err);
           if (!ok) break;
           tc_fence_after();
           if (leader) {
@@ -465,22 +506,40 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         ++steps;
         __syncwarp();
       }
+    } else if (VEC) {
+      // The loading warp: a box of each operand a step.
+      if (warp == kWorkers / 32 + 1) {
+        const bool leader = elect_one();
+        bool ok = true;
+        int c = 0;
+        for (int t = t0; t < t1; t += kStep, ++c) {
+          if (c > 0) ok = sleep_wait(raw_empty, (c - 1) & 1, err);
+          if (!ok) break;
+          if (leader) {
+            // What lies outside the tensor comes as 0, what lies behind the sequence's end as it is.
+            const int row = s.back ? n - kStep - t : t;
+            mbar_expect_tx(raw_full, kStep * 4 * ((STATE_ONLY ? 1 : 2) * s.rows + s.cols));
+            load_rows(base + Sm::kRawK, &maps.k, row, h / s.k.share, b, raw_full);
+            if (!STATE_ONLY) load_rows(base + Sm::kRawQ, &maps.q, row, h / s.q.share, b, raw_full);
+            load_rows(base + Sm::kRawV, &maps.v, row, h / s.v.share, b, raw_full);
+          }
+          __syncwarp();
+        }
+        // The last copies end before the block does.
+        if (c > 0) sleep_wait(raw_full, (c - 1) & 1, err);
+      }
     } else {
       // The loading warps, a row at a time.
       const int loader = warp - kWorkers / 32 - 1;
       bool ok = true;
       for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
-        if (c > 0) ok = warp_wait(raw_empty, (c - 1) & 1, err);
+        if (c > 0) ok = sleep_wait(raw_empty, (c - 1) & 1, err);
         if (!ok) break;
         const int m = min(kStep, t1 - t);
         auto row = [&](const float* from, int dim, uint32_t to) {
-          if (VEC) {
-            if (4 * lane < dim) copy_async16(to + 16 * lane, from + 4 * lane);
-          } else {
 #pragma unroll
-            for (int i = 0; i < kMostDim / 32; ++i)
-              if (lane + 32 * i < dim) copy_async4(to + 4 * (lane + 32 * i), from + lane + 32 * i);
-          }
+          for (int i = 0; i < kMostDim / 32; ++i)
+            if (lane + 32 * i < dim) copy_async4(to + 4 * (lane + 32 * i), from + lane + 32 * i);
         };
 #pragma unroll 4
         for (int r = loader; r < m; r += kLoaders) {
@@ -578,13 +637,15 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       const int m = min(kStep, t1 - t);
       const int turn = c & 1;
       float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn, *v_most = v_mosts + 512 * turn;
-      if (ok) ok = warp_wait(raw_full, turn, err);
+      if (ok) ok = sleep_wait(raw_full, turn, err);
       if (m < kStep) {  // zeros behind the sequence's end
-        for (int i = tid; i < (kStep - m) * DK; i += kWorkers) {
-          ((float*)(smem + Sm::kRawQ))[m * DK + i] = 0.0f;
-          ((float*)(smem + Sm::kRawK))[m * DK + i] = 0.0f;
+        const int first = turned ? 0 : m;
+        for (int i = tid; i < (kStep - m) * key_pitch; i += kWorkers) {
+          ((float*)(smem + Sm::kRawQ))[first * key_pitch + i] = 0.0f;
+          ((float*)(smem + Sm::kRawK))[first * key_pitch + i] = 0.0f;
         }
-        for (int i = tid; i < (kStep - m) * kMostDim; i += kWorkers) ((float*)(smem + Sm::kRawV))[m * kMostDim + i] = 0.0f;
+        for (int i = tid; i < (kStep - m) * value_pitch; i += kWorkers)
+          ((float*)(smem + Sm::kRawV))[first * value_pitch + i] = 0.0f;
         worker_sync();
       }
       // q and k rows, a warp eight of one of them.
@@ -593,18 +654,24 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         constexpr int kRowsPer = STATE_ONLY ? 4 : 8;
         const bool is_k = STATE_ONLY || warp >= 8;
         const int row0 = STATE_ONLY ? warp * 4 : (warp & 7) * 8;
-        const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + row0 * DK + lane * (DK / 32);
+        // (Where rows hold fewer than DK values, the lanes behind them hold 0.)
+        const bool held = !VEC || lane * (DK / 32) < s.rows;
+        const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + place(row0) * key_pitch +
+                           (held ? lane * (DK / 32) : 0);
+        const int next_row = turned ? -key_pitch : key_pitch;
         Pair f[kRowsPer][kBoxes];
         float mine = 0.0f;  // of row `lane`
 #pragma unroll
         for (int r = 0; r < kRowsPer; ++r) {
           float most;
           if constexpr (DK == 128) {
-            const float4 w = *(const float4*)(raw + r * DK);
+            float4 w = *(const float4*)(raw + r * next_row);
+            if (VEC && !held) w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             f[r][0] = pair_of(w.x, w.y), f[r][kBoxes - 1] = pair_of(w.z, w.w);
             most = most_of(most_of(w.x, w.y, w.z), w.w, 0.0f);
           } else {
-            const float2 w = *(const float2*)(raw + r * DK);
+            float2 w = *(const float2*)(raw + r * next_row);
+            if (VEC && !held) w = make_float2(0.0f, 0.0f);
             f[r][0] = pair_of(w.x, w.y);
             most = most_of(w.x, w.y, 0.0f);
           }
@@ -643,11 +710,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       // This column's values of 16 tokens.
       Pair val[8];
       {
-        const float* raw = (const float*)(smem + Sm::kRawV) + group * 16 * kMostDim + col;
+        const bool held = !VEC || col < s.cols;
+        const float* raw = (const float*)(smem + Sm::kRawV) + place(group * 16) * value_pitch + (held ? col : 0);
+        const int next_row = turned ? -value_pitch : value_pitch;
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float a = raw[2 * i * kMostDim], d = raw[(2 * i + 1) * kMostDim];
+          const float a = held ? raw[2 * i * next_row] : 0.0f, d = held ? raw[(2 * i + 1) * next_row] : 0.0f;
           val[i] = pair_of(a, d);
           most = most_of(most, a, d);
         }
@@ -667,22 +736,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         // Token by token.
         const float2 one = decay_over(decay, 1);
         const Pair hi = pair_of(one.x, one.x), lo = pair_of(one.y, one.y);
-        const float2* kr = (const float2*)(smem + Sm::kRawK) + group * (kMine / 2);
-        const float2* qr = (const float2*)(smem + Sm::kRawQ) + group * (kMine / 2);
-        const float* vr = (const float*)(smem + Sm::kRawV) + col;
         for (int i = 0; i < m; ++i) {
-          const float w = vr[i * kMostDim];
+          const float* kr = (const float*)(smem + Sm::kRawK) + place(i) * key_pitch;
+          const float* qr = (const float*)(smem + Sm::kRawQ) + place(i) * key_pitch;
+          const float w = col < s.cols ? ((const float*)(smem + Sm::kRawV))[place(i) * value_pitch + col] : 0.0f;
+          auto two = [&](const float* row, int r) {
+            return pair_of(r < s.rows ? row[r] : 0.0f, r + 1 < s.rows ? row[r + 1] : 0.0f);
+          };
           const Pair w2 = pair_of(w, w);
           Pair sum = 0;
 #pragma unroll
           for (int j = 0; j < kMine / 2; ++j) {
-            const float2 key = kr[i * (DK / 2) + j];
+            const int r = group * kMine + 2 * j;
             if (lead) x[j] = fma2(x[j], hi, mul2(x[j], lo));
-            x[j] = fma2(pair_of(key.x, key.y), w2, x[j]);
-            if (!STATE_ONLY) {
-              const float2 query = qr[i * (DK / 2) + j];
-              sum = fma2(pair_of(query.x, query.y), x[j], sum);
-            }
+            x[j] = fma2(two(kr, r), w2, x[j]);
+            if (!STATE_ONLY) sum = fma2(two(qr, r), x[j], sum);
             if (!lead) x[j] = fma2(x[j], hi, mul2(x[j], lo));
           }
           if (!STATE_ONLY) {
@@ -704,7 +772,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           if (t + kStep < t1) put_state(bound);
         }
         // The issuing warp keeps step.
-        if (ok) ok = warp_wait(far_seen, far_steps & 1, err);
+        if (ok) ok = sleep_wait(far_seen, far_steps & 1, err);
         ++far_steps;
         continue;
       }
@@ -760,7 +828,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         const Pair inv2 = pair_of(p_inv, p_inv);
 #pragma unroll
         for (int j = 0; j < 8; ++j) keys[j] = mul2(mul2(keys[j], inv2), near[j]);
-        if (ok) ok = warp_wait(score_full, steps & 1, err);
+        if (ok) ok = sleep_wait(score_full, steps & 1, err);
         tc_fence_after();
         // P of 16 keys: rows (tokens) 0..63 in the lanes of quarters 0 and 1, what q's lo adds in 2 and 3.
         float p[16];
@@ -792,7 +860,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       // X, and a bound of it: 64 products of packed values are at most 2^36.
       const float from_down = x_down;
       const float2 a = m == kStep ? fade : decay_over(decay, m);
-      if (ok) ok = warp_wait(sums_full, steps & 1, err);
+      if (ok) ok = sleep_wait(sums_full, steps & 1, err);
       tc_fence_after();
       {
         const Pair a_hi = pair_of(a.x, a.x), a_lo = pair_of(a.y, a.y), w2 = pair_of(w_down, w_down);
@@ -811,7 +879,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         bound = fmaf(bound, a.x, 0x1p36f * w_down) * 1.000001f;
         far_state = biased_of(bound) >= 254;
         if (t + kStep < t1) put_state(bound);
-        if (ok) ok = warp_wait(out_full, steps & 1, err);
+        if (ok) ok = sleep_wait(out_full, steps & 1, err);
         tc_fence_after();
         float from[16], own[16];
         tmem_ld16(at_lane + Tm::kFrom + group * 16, from);
@@ -936,7 +1004,7 @@ int64_t states_elems(const DecayShape& s) {
 }
 
 template <int DK, bool STATE_ONLY, bool VEC>
-void launch_chunks(const Scan& s, const ScanParts& parts, int blocks, int* err, cudaStream_t st) {
+void launch_chunks(const Scan& s, const ScanMaps& maps, const ScanParts& parts, int blocks, int* err, cudaStream_t st) {
   auto kernel = scan_kernel<DK, STATE_ONLY, VEC>;
   static std::atomic<uint64_t> set{0};  // devices whose limit is set
   int device;
@@ -951,19 +1019,27 @@ void launch_chunks(const Scan& s, const ScanParts& parts, int blocks, int* err, 
     TYSOR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<DK>::kBytes));
     set.fetch_or(bit, std::memory_order_relaxed);
   }
-  kernel<<<blocks, kScanThreads, ScanSmem<DK>::kBytes, st>>>(s, parts, err);
+  kernel<<<blocks, kScanThreads, ScanSmem<DK>::kBytes, st>>>(s, maps, parts, err);
   check_launch();
 }
 
 template <int DK, bool VEC>
 void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st) {
   const int units = s.batch * s.heads;
+  ScanMaps maps{};
+  if (VEC) {
+    auto map = [&](const Rows& r, int dim) {
+      return rows_map(r.p, {(uint64_t)dim, (uint64_t)s.seq, (uint64_t)(s.heads / r.share), (uint64_t)s.batch},
+                      {(uint64_t)r.token, (uint64_t)r.head, (uint64_t)r.batch}, kStep);
+    };
+    maps = {map(s.q, s.rows), map(s.k, s.rows), map(s.v, s.cols)};
+  }
   if (parts.segments > 1) {
-    launch_chunks<DK, true, VEC>(s, parts, units * (parts.segments - 1), err, st);
+    launch_chunks<DK, true, VEC>(s, maps, parts, units * (parts.segments - 1), err, st);
     scan_states_kernel<<<dim3((unsigned)ceil_div(s.rows * s.cols, 256), (unsigned)units), 256, 0, st>>>(s, parts, err);
     check_launch();
   }
-  launch_chunks<DK, false, VEC>(s, parts, units * parts.segments, err, st);
+  launch_chunks<DK, false, VEC>(s, maps, parts, units * parts.segments, err, st);
 }
 
 // `states`: states_elems floats.
