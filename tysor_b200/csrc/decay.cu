@@ -105,27 +105,11 @@ __device__ __forceinline__ bool sleep_wait(uint32_t bar, uint32_t parity, int* e
 }
 
 // Two fp32 values for the paired instructions.
-typedef unsigned long long Pair;
-__device__ __forceinline__ Pair pair_of(float a, float b) {
-  Pair r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 floats_of(Pair v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
+typedef float2 Pair;
+__device__ __forceinline__ Pair pair_of(float a, float b) { return make_float2(a, b); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { return __ffma2_rn(a, b, c); }
+
 // ---- token by token --------------------------------------------------------------
 
 // A block holds `kSlice` columns of one head's state, four columns and every 16th
@@ -185,7 +169,7 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
     for (int t = 0; t < m; ++t) {
       const float4 w = *(const float4*)&vs[t][c];
       const Pair w2[2] = {pair_of(w.x, w.y), pair_of(w.z, w.w)};
-      Pair sum[2] = {0, 0};
+      Pair sum[2] = {pair_of(0.0f, 0.0f), pair_of(0.0f, 0.0f)};
 #pragma unroll
       for (int i = 0; i < kStepMine; ++i) {
         const float key = ks[t][r0 + kStepRows * i], query = qs[t][r0 + kStepRows * i];
@@ -200,7 +184,7 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
           if (s.back) y = fma2(y, fade_hi, mul2(y, fade_lo));
         }
       }
-      float o[4] = {floats_of(sum[0]).x, floats_of(sum[0]).y, floats_of(sum[1]).x, floats_of(sum[1]).y};
+      float o[4] = {sum[0].x, sum[0].y, sum[1].x, sum[1].y};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         o[j] += __shfl_xor_sync(0xffffffffu, o[j], 8);
@@ -225,7 +209,7 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
   for (int i = 0; i < kStepMine; ++i) {
     const int r = r0 + kStepRows * i;
     if (r >= s.rows || c >= width) continue;
-    const float2 y0 = floats_of(x[i][0]), y1 = floats_of(x[i][1]);
+    const float2 y0 = x[i][0], y1 = x[i][1];
     float4 f = make_float4(y0.x * s.to_factor, y0.y * s.to_factor, y1.x * s.to_factor, y1.y * s.to_factor);
     if (VEC) {
       float4* to = (float4*)(s.to.p + state + (int64_t)r * s.cols + c0 + c);
@@ -289,13 +273,16 @@ struct ScanSmem {
   static constexpr int kRawQ = kP + 3 * kBoxBytes;          // fp32 rows of the next step
   static constexpr int kRawK = kRawQ + kStep * DK * 4;
   static constexpr int kRawV = kRawK + kStep * DK * 4;
-  static constexpr int kMisc = kRawV + kStep * kMostDim * 4;
+  static constexpr int kOut = kRawV + kStep * kMostDim * 4;  // [16 warps][16 tokens][32 columns]
+  static constexpr int kMisc = kOut + kStep * kMostDim * 4;
   static constexpr int kBytes = kMisc + 9216 + 1024;
 };
 
-// Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces.
+// Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces, and of
+// 16 rows of 32 columns of the output, if its rows are (`stores`).
 struct ScanMaps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, out;
+  int stores;
 };
 __device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, int row, int head, int batch, uint32_t bar) {
   asm volatile(
@@ -303,6 +290,23 @@ __device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, i
           to),
       "l"((uint64_t)map), "r"(0), "r"(row), "r"(head), "r"(batch), "r"(bar)
       : "memory");
+}
+
+// A box of shared memory to a head's output, or added to it.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from, int col, int row, int head, int batch,
+                                          int accumulate) {
+  if (accumulate)
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.4d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+            (uint64_t)map),
+        "r"(col), "r"(row), "r"(head), "r"(batch), "r"(from)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"((uint64_t)map),
+        "r"(col), "r"(row), "r"(head), "r"(batch), "r"(from)
+        : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
 struct ScanParts {
@@ -340,10 +344,10 @@ __device__ __forceinline__ uint32_t half_pair(float a, float b) {
 }
 // Pairs of values as pairs of halves: hi, and what is left.
 __device__ __forceinline__ void split_pair(Pair v, uint32_t& hi, uint32_t& lo) {
-  const float2 f = floats_of(v);
+  const float2 f = v;
   hi = half_pair(f.x, f.y);
   const float2 back = __half22float2(*(const __half2*)&hi);
-  const float2 rest = floats_of(fma2(pair_of(back.x, back.y), pair_of(-1.0f, -1.0f), v));
+  const float2 rest = fma2(pair_of(back.x, back.y), pair_of(-1.0f, -1.0f), v);
   lo = half_pair(rest.x, rest.y);
 }
 
@@ -368,7 +372,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   using Sm = ScanSmem<DK>;
   constexpr int kBoxes = DK / 64, kMine = DK / 4;  // state values of a thread
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  // (As an offset: the compiler then knows what is derived from it for shared memory.)
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
   float* lefts = since + 64;                  // [2][64] a^(63 - j + tail), and the same of a last, shorter step
   float* q_downs = lefts + 128;               // [2][64] what undoes the rows' factors, steps in turn
@@ -418,7 +423,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   }
   // Columns that no copy writes are 0.
   if (!VEC && (s.rows != DK || s.cols != kMostDim))
-    for (int i = tid; i < (Sm::kMisc - Sm::kRawQ) / 16; i += kScanThreads)
+    for (int i = tid; i < (Sm::kOut - Sm::kRawQ) / 16; i += kScanThreads)
       ((uint4*)(smem + Sm::kRawQ))[i] = make_uint4(0, 0, 0, 0);
   tc_fence_before();
   __syncthreads();
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       float m = 0.0f;
 #pragma unroll
       for (int i = 0; i < kMine / 2; ++i) {
-        const float2 f = floats_of(x[i]);
+        const float2 f = x[i];
         m = most_of(m, f.x, f.y);
       }
       x_most[group * 128 + col] = m;
@@ -744,7 +749,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             return pair_of(r < s.rows ? row[r] : 0.0f, r + 1 < s.rows ? row[r + 1] : 0.0f);
           };
           const Pair w2 = pair_of(w, w);
-          Pair sum = 0;
+          Pair sum = pair_of(0.0f, 0.0f);
 #pragma unroll
           for (int j = 0; j < kMine / 2; ++j) {
             const int r = group * kMine + 2 * j;
@@ -755,7 +760,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           }
           if (!STATE_ONLY) {
             float* sums = i & 1 ? v_most : x_most;
-            sums[group * 128 + col] = floats_of(sum).x + floats_of(sum).y;
+            sums[group * 128 + col] = sum.x + sum.y;
             worker_sync();
             if (group == 0 && col < s.cols) {
               const float all = ((sums[col] + sums[128 + col]) + (sums[256 + col] + sums[384 + col])) * s.scale;
@@ -846,7 +851,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float2 f = floats_of(mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]));
+            const float2 f = mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]);
             hi[j] = half_pair(f.x, f.y);
           }
           *(uint4*)(row + 2 * kBoxBytes + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -893,28 +898,39 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             const int e = 4 * i + 2 * j;
             const Pair o = fma2(pair_of(from[e], from[e + 1]), mul2(j ? pair_of(w.z, w.w) : pair_of(w.x, w.y), f2),
                                 mul2(pair_of(own[e], own[e + 1]), p2));
-            const float2 y = floats_of(mul2(o, mul2(j ? pair_of(d.z, d.w) : pair_of(d.x, d.y), s2)));
+            const float2 y = (mul2(o, mul2(j ? pair_of(d.z, d.w) : pair_of(d.x, d.y), s2)));
             own[e] = y.x, own[e + 1] = y.y;
           }
         }
-        const int rows = col < s.cols ? min(m - group * 16, 16) : 0;  // of this thread's
-        const int64_t pitch = s.back ? -s.out.token : s.out.token;
-        float* to = out + token(t + group * 16) * s.out.token + col;
-        if (s.accumulate) {
+        if (VEC && maps.stores && m == kStep) {
+          // Through shared memory, a box a warp: a thread's stores of single values would take the
+          // load and store units longer than the step's loads.
+          float* patch = (float*)(smem + Sm::kOut) + warp * 512 + lane;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < rows) own[i] = to[i * pitch] + own[i];
-        }
-        if (rows == 16) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) to[i * pitch] = own[i];
+          for (int i = 0; i < 16; ++i) patch[32 * (s.back ? 15 - i : i)] = own[i];
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && quarter * 32 < s.cols) {
+            const int first = t + group * 16;
+            store_box(&maps.out, base + Sm::kOut + warp * 2048, quarter * 32, s.back ? n - 16 - first : first,
+                      h / s.out.share, b, s.accumulate);
+          }
         } else {
+          const int rows = col < s.cols ? min(m - group * 16, 16) : 0;  // of this thread's
+          const int64_t pitch = s.back ? -s.out.token : s.out.token;
+          float* to = out + token(t + group * 16) * s.out.token + col;
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i < rows) to[i * pitch] = own[i];
+          for (int i = 0; i < 16; ++i, to += pitch)
+            if (i < rows) *to = s.accumulate ? *to + own[i] : own[i];
         }
       }
       ++steps;
+    }
+    if (VEC && !STATE_ONLY) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      __syncwarp();
     }
     // Rows behind the sequence's end, spread over its blocks.
     if (!STATE_ONLY && !s.accumulate)
@@ -924,7 +940,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int r = group * kMine + i;
-        const float y = i & 1 ? floats_of(x[i / 2]).y : floats_of(x[i / 2]).x;
+        const float y = i & 1 ? x[i / 2].y : x[i / 2].x;
         if (r >= s.rows || col >= s.cols) continue;
         if (STATE_ONLY) {
           parts.states[((int64_t)unit * parts.segments + part + 1) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
@@ -1003,6 +1019,11 @@ int64_t states_elems(const DecayShape& s) {
   return segments > 1 ? units * segments * s.key_dim * s.value_dim : 0;
 }
 
+// Whether an operand's rows are whole 16-byte pieces.
+bool whole_pieces(const Rows& r, int dim) {
+  return ((uintptr_t)r.p & 15) == 0 && dim % 4 == 0 && r.token % 4 == 0 && r.head % 4 == 0 && r.batch % 4 == 0;
+}
+
 template <int DK, bool STATE_ONLY, bool VEC>
 void launch_chunks(const Scan& s, const ScanMaps& maps, const ScanParts& parts, int blocks, int* err, cudaStream_t st) {
   auto kernel = scan_kernel<DK, STATE_ONLY, VEC>;
@@ -1028,11 +1049,15 @@ void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st
   const int units = s.batch * s.heads;
   ScanMaps maps{};
   if (VEC) {
-    auto map = [&](const Rows& r, int dim) {
+    auto map = [&](const Rows& r, int dim, int box_cols, int box_rows) {
       return rows_map(r.p, {(uint64_t)dim, (uint64_t)s.seq, (uint64_t)(s.heads / r.share), (uint64_t)s.batch},
-                      {(uint64_t)r.token, (uint64_t)r.head, (uint64_t)r.batch}, kStep);
+                      {(uint64_t)r.token, (uint64_t)r.head, (uint64_t)r.batch}, box_cols, box_rows);
     };
-    maps = {map(s.q, s.rows), map(s.k, s.rows), map(s.v, s.cols)};
+    maps.q = map(s.q, s.rows, s.rows, kStep);
+    maps.k = map(s.k, s.rows, s.rows, kStep);
+    maps.v = map(s.v, s.cols, s.cols, kStep);
+    maps.stores = whole_pieces(s.out, s.cols);
+    if (maps.stores) maps.out = map(s.out, s.cols, 32, 16);
   }
   if (parts.segments > 1) {
     launch_chunks<DK, true, VEC>(s, maps, parts, units * (parts.segments - 1), err, st);
@@ -1047,10 +1072,7 @@ void run_scan(const Scan& s, float* states, int* err, cudaStream_t st) {
   if (s.batch <= 0 || s.heads <= 0) return;
   if (s.seq >= kChunkedFrom) {
     const ScanParts parts{segments_of((int64_t)s.batch * s.heads, s.seq), states};
-    auto wide = [](const Rows& r, int dim) {
-      return ((uintptr_t)r.p & 15) == 0 && dim % 4 == 0 && r.token % 4 == 0 && r.head % 4 == 0 && r.batch % 4 == 0;
-    };
-    const bool vec = wide(s.q, s.rows) && wide(s.k, s.rows) && wide(s.v, s.cols);
+    const bool vec = whole_pieces(s.q, s.rows) && whole_pieces(s.k, s.rows) && whole_pieces(s.v, s.cols);
     if (s.rows > 64) vec ? run_chunks<128, true>(s, parts, err, st) : run_chunks<128, false>(s, parts, err, st);
     else vec ? run_chunks<64, true>(s, parts, err, st) : run_chunks<64, false>(s, parts, err, st);
     return;

@@ -1963,11 +1963,12 @@ int64_t gemm_splitk_ws_elems(int batch, int64_t M, int64_t N, int64_t K, int mod
   return (int64_t)parts * batch * M * ((N + 3) & ~(int64_t)3);
 }
 
-CUtensorMap rows_map(const float* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box_rows) {
+CUtensorMap rows_map(const float* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box_cols,
+                     uint32_t box_rows) {
   CUtensorMap m;
   const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
   const cuuint64_t st[3] = {strides[0] * 4, strides[1] * 4, strides[2] * 4};
-  const cuuint32_t box[4] = {(cuuint32_t)dims[0], box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {box_cols, box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (void*)base, d, st, box, one,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -6,9 +6,10 @@
 
 namespace tysor {
 
-// The tensor map of boxes of `box_rows` whole rows of an fp32 tensor of rank 4 (rows of
-// dims[0] values; strides in values, multiples of 4).  Throws where the driver refuses it.
-CUtensorMap rows_map(const float* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box_rows);
+// The tensor map of boxes of `box_rows` rows of `box_cols` values of an fp32 tensor of
+// rank 4 (strides in values, multiples of 4).  Throws where the driver refuses it.
+CUtensorMap rows_map(const float* base, const uint64_t (&dims)[4], const uint64_t (&strides)[3], uint32_t box_cols,
+                     uint32_t box_rows);
 
 constexpr long long kWaitCycles = 4000000000LL;  // about 2 s at 1.9 GHz
 
