@@ -275,7 +275,7 @@ struct ScanSmem {
   static constexpr int kRawV = kRawK + kStep * DK * 4;
   static constexpr int kOut = kRawV + kStep * kMostDim * 4;  // [16 warps][16 tokens][32 columns]
   static constexpr int kMisc = kOut + kStep * kMostDim * 4;
-  static constexpr int kBytes = kMisc + 9216 + 1024;
+  static constexpr int kBytes = kMisc + 10240;
 };
 
 // Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces, and of
@@ -315,6 +315,7 @@ struct ScanParts {
   // its own state, then the state that it starts from.  (The call's new state may replace the
   // old one, so no segment but a head's only one reads that.)
   float* states;
+  int si, sj;  // between their key rows and value columns, for the segments that start from them
 };
 
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
@@ -376,7 +377,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
   float* lefts = since + 64;                  // [2][64] a^(63 - j + tail), and the same of a last, shorter step
-  float* q_downs = lefts + 128;               // [2][64] what undoes the rows' factors, steps in turn
+  float* nears = lefts + 128;                 // [128] a^(d - 63), 0 below
+  float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors, steps in turn
   float* k_downs = q_downs + 128;             // [2][64]
   float* v_mosts = k_downs + 128;             // [2][4][128]
   float* x_most = v_mosts + 1024;             // [4][128]
@@ -416,6 +418,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     const int j = tid & 63, m = tid < 128 ? kStep : (t1 - t0) % kStep;
     lefts[tid - 64] = j < m ? power(m - 1 - j + tail) : 0.0f;
   }
+  if (tid >= 192 && tid < 320) nears[tid - 192] = tid - 192 < 63 ? 0.0f : power(tid - 192 - 63);
   if (warp == kWorkers / 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemColumns));
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
             const int r = group * kMine + i;
-            if (r < s.rows) first[i] = from[(int64_t)r * s.cols + col];
+            if (r < s.rows) first[i] = from[r * parts.si + col * parts.sj];
           }
         } else if (s.from.p != nullptr) {
 #pragma unroll
@@ -618,14 +621,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         tmem_st8(at_lane + Tm::kStateLo + group * (kMine / 2), lo);
       }
     };
-    // P's decay for this thread's row (or, in quarters 2 and 3, what q's lo adds to it) and 16 keys.
-    const int row_i = col & (kStep - 1);
-    Pair near[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int key = group * 16 + 2 * j;
-      near[j] = pair_of(key <= row_i ? power(row_i - key) : 0.0f, key + 1 <= row_i ? power(row_i - key - 1) : 0.0f);
-    }
+    const int row_i = col & (kStep - 1);  // of P
     const float2 fade = decay_over(decay, kStep);
     bool ok = true;
     uint32_t steps = 0, far_steps = 0;
@@ -783,7 +779,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       }
       if (tid == 0 && t + kStep < t1) mbar_arrive(raw_empty);
       // The keys' factors over the greatest (P), and with a^(63 - j + tail) over the greatest of those (w).
-      Pair keys[8];
       float p_down, p_inv, w_down;
       {
         const float* left = lefts + (m < kStep ? kStep : 0);
@@ -798,11 +793,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             most_of(most_of(v_most[col], v_most[128 + col], v_most[256 + col]), v_most[384 + col], 0.0f));
         const float up = power_of(268u - biased), down = power_of(biased - 14u);
         const float inv_w = e ? power_of(254u - e) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 f = *(const float4*)(k_down + group * 16 + 4 * i);
-          keys[2 * i] = pair_of(f.x, f.y), keys[2 * i + 1] = pair_of(f.z, f.w);
-        }
         uint32_t hi[8], lo[8];
         const Pair up2 = pair_of(up, up), inv2 = pair_of(inv_w, inv_w);
 #pragma unroll
@@ -815,9 +805,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 l = *(const float4*)(left + group * 16 + 4 * i);
-          split_pair(mul2(val[2 * i], mul2(mul2(keys[2 * i], pair_of(l.x, l.y)), inv2)), hi[2 * i], lo[2 * i]);
-          split_pair(mul2(val[2 * i + 1], mul2(mul2(keys[2 * i + 1], pair_of(l.z, l.w)), inv2)), hi[2 * i + 1], lo[2 * i + 1]);
+          const float4 l = *(const float4*)(left + group * 16 + 4 * i), f = *(const float4*)(k_down + group * 16 + 4 * i);
+          const Pair w0 = mul2(mul2(pair_of(f.x, f.y), pair_of(l.x, l.y)), inv2);
+          const Pair w1 = mul2(mul2(pair_of(f.z, f.w), pair_of(l.z, l.w)), inv2);
+          split_pair(mul2(val[2 * i], w0), hi[2 * i], lo[2 * i]);
+          split_pair(mul2(val[2 * i + 1], w1), hi[2 * i + 1], lo[2 * i + 1]);
         }
         tmem_st8(at_lane + Tm::kW + group * 8, hi);
         tmem_st8(at_lane + Tm::kWLo + group * 8, lo);
@@ -830,30 +822,35 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       if (lane == 0) mbar_arrive(values_ready);
 
       if (!STATE_ONLY) {
-        const Pair inv2 = pair_of(p_inv, p_inv);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) keys[j] = mul2(mul2(keys[j], inv2), near[j]);
         if (ok) ok = sleep_wait(score_full, steps & 1, err);
         tc_fence_after();
         // P of 16 keys: rows (tokens) 0..63 in the lanes of quarters 0 and 1, what q's lo adds in 2 and 3.
+        const Pair inv2 = pair_of(p_inv, p_inv);
+        const float* near = nears + 63 + row_i - group * 16;
         float p[16];
         tmem_ld16(at_lane + Tm::kScore + group * 16, p);
+        Pair f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 d = *(const float4*)(k_down + group * 16 + 4 * i);
+          const float* a = near - 4 * i;
+          f[2 * i] = mul2(pair_of(p[4 * i], p[4 * i + 1]), mul2(mul2(pair_of(d.x, d.y), inv2), pair_of(a[0], a[-1])));
+          f[2 * i + 1] =
+              mul2(pair_of(p[4 * i + 2], p[4 * i + 3]), mul2(mul2(pair_of(d.z, d.w), inv2), pair_of(a[-2], a[-3])));
+        }
         uint8_t* row = smem + Sm::kP + row_i * 128;
         const int x0 = ((2 * group) ^ (row_i & 7)) << 4, x1 = ((2 * group + 1) ^ (row_i & 7)) << 4;
         uint32_t hi[8], lo[8];
         if (quarter < 2) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) split_pair(mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]), hi[j], lo[j]);
+          for (int j = 0; j < 8; ++j) split_pair(f[j], hi[j], lo[j]);
           *(uint4*)(row + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4*)(row + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
           *(uint4*)(row + kBoxBytes + x0) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           *(uint4*)(row + kBoxBytes + x1) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float2 f = mul2(pair_of(p[2 * j], p[2 * j + 1]), keys[j]);
-            hi[j] = half_pair(f.x, f.y);
-          }
+          for (int j = 0; j < 8; ++j) hi[j] = half_pair(f[j].x, f[j].y);
           *(uint4*)(row + 2 * kBoxBytes + x0) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
           *(uint4*)(row + 2 * kBoxBytes + x1) = make_uint4(hi[4], hi[5], hi[6], hi[7]);
         }
@@ -1045,7 +1042,7 @@ void launch_chunks(const Scan& s, const ScanMaps& maps, const ScanParts& parts, 
 }
 
 template <int DK, bool VEC>
-void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st) {
+void run_chunks(const Scan& s, const ScanParts& parts, bool states_there, int* err, cudaStream_t st) {
   const int units = s.batch * s.heads;
   ScanMaps maps{};
   if (VEC) {
@@ -1059,7 +1056,7 @@ void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st
     maps.stores = whole_pieces(s.out, s.cols);
     if (maps.stores) maps.out = map(s.out, s.cols, 32, 16);
   }
-  if (parts.segments > 1) {
+  if (parts.segments > 1 && !states_there) {
     launch_chunks<DK, true, VEC>(s, maps, parts, units * (parts.segments - 1), err, st);
     scan_states_kernel<<<dim3((unsigned)ceil_div(s.rows * s.cols, 256), (unsigned)units), 256, 0, st>>>(s, parts, err);
     check_launch();
@@ -1067,14 +1064,16 @@ void run_chunks(const Scan& s, const ScanParts& parts, int* err, cudaStream_t st
   launch_chunks<DK, false, VEC>(s, maps, parts, units * parts.segments, err, st);
 }
 
-// `states`: states_elems floats.
-void run_scan(const Scan& s, float* states, int* err, cudaStream_t st) {
+// `states`: states_elems floats.  `turned_states`: they hold those of a scan whose state is this
+// one's transposed.
+void run_scan(const Scan& s, float* states, int* err, cudaStream_t st, bool turned_states = false) {
   if (s.batch <= 0 || s.heads <= 0) return;
   if (s.seq >= kChunkedFrom) {
-    const ScanParts parts{segments_of((int64_t)s.batch * s.heads, s.seq), states};
+    const ScanParts parts{segments_of((int64_t)s.batch * s.heads, s.seq), states, turned_states ? 1 : s.cols,
+                          turned_states ? s.rows : 1};
     const bool vec = whole_pieces(s.q, s.rows) && whole_pieces(s.k, s.rows) && whole_pieces(s.v, s.cols);
-    if (s.rows > 64) vec ? run_chunks<128, true>(s, parts, err, st) : run_chunks<128, false>(s, parts, err, st);
-    else vec ? run_chunks<64, true>(s, parts, err, st) : run_chunks<64, false>(s, parts, err, st);
+    if (s.rows > 64) vec ? run_chunks<128, true>(s, parts, turned_states, err, st) : run_chunks<128, false>(s, parts, turned_states, err, st);
+    else vec ? run_chunks<64, true>(s, parts, turned_states, err, st) : run_chunks<64, false>(s, parts, turned_states, err, st);
     return;
   }
   auto plain = [&](const StateAt& x) {
@@ -1159,32 +1158,28 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.accumulate = accumulate_q;
   run_scan(c, states, err, st);
 
-  // The states of the scans back are the gradients' over `scale`.
+  // The states of the scans back are the gradients' over `scale`.  The second scan's is the
+  // first's transposed: its segments start from the first's states.
   c.back = 1;
   c.from_factor = 1.0f / s.scale;
   c.to_factor = s.scale;
-  auto keys = [&](float* grad, int dim, int accumulate) {
+  auto keys = [&](float* grad, int dim, int accumulate, bool turned_states) {
     const Rows to = rows_of(s, grad, s.kv_heads, dim, 1);
     if (share == 1) {
       c.out = to;
       c.accumulate = accumulate;
-      run_scan(c, states, err, st);
+      run_scan(c, states, err, st, turned_states);
       return;
     }
     c.out = {by_head, (int64_t)s.heads * s.seq * dim, (int64_t)s.seq * dim, dim, 1};
     c.accumulate = 0;
-    run_scan(c, states, err, st);
+    run_scan(c, states, err, st, turned_states);
     const int64_t n = (int64_t)s.batch * s.kv_heads * s.seq * dim;
     if (n <= 0) return;
     sum_heads_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(by_head, to, s.batch, s.kv_heads, share, s.seq, dim,
                                                                  accumulate);
     check_launch();
   };
-  c.q = v;
-  c.k = g;
-  c.v = q;
-  c.from = {const_cast<float*>(dnew_state), 1, s.value_dim};
-  keys(dk, s.key_dim, accumulate_k);
   c.rows = s.key_dim;
   c.cols = s.value_dim;
   c.q = k;
@@ -1193,7 +1188,15 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.from = {const_cast<float*>(dnew_state), s.value_dim, 1};
   c.to = {dstate, s.value_dim, 1};
   c.accumulate_state = accumulate_state;
-  keys(dv, s.value_dim, accumulate_v);
+  keys(dv, s.value_dim, accumulate_v, false);
+  c.rows = s.value_dim;
+  c.cols = s.key_dim;
+  c.q = v;
+  c.k = g;
+  c.v = q;
+  c.from = {const_cast<float*>(dnew_state), 1, s.value_dim};
+  c.to = {};
+  keys(dk, s.key_dim, accumulate_k, true);
 }
 
 }  // namespace tysor
