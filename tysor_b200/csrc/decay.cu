@@ -260,7 +260,7 @@ constexpr uint32_t kLeastBiased = 127 - 100, kFarRange = 160;  // exponents from
 template <int DK>
 struct ScanTmem {
   static constexpr uint32_t kState = 0, kStateLo = DK / 2, kDelta = DK, kFrom = 2 * DK, kScore = kFrom + 64,
-                            kV = kScore + 64, kVLo = kV + 32, kW = kVLo + 32, kWLo = kW + 32;
+                            kV = kScore + 64, kW = kV + 64;  // hi; lo 32 columns behind
 };
 constexpr uint32_t kTmemColumns = 512;
 
@@ -363,7 +363,9 @@ __device__ __forceinline__ void segment_of(int n, int segments, int part, int* f
   *last = min(n, (part + 1) * per * kStep);
 }
 
-// STATE_ONLY: the segment's own state (from 0), for the segments behind it.  VEC: rows of
+// STATE_ONLY: the segment's own state (from 0), for the segments behind it.  Its steps have
+// but one product, which they take in turns of two sets of operands and sums: a step's sums
+// are added while the matrix unit is at the next.  VEC: rows of
 // whole 16-byte pieces.
 template <int DK, bool STATE_ONLY, bool VEC>
 __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s,
@@ -448,6 +450,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       uint32_t steps = 0;  // those of the matrix unit
       bool ok = true;
       for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
+        const bool second = STATE_ONLY && (c & 1);
         ok = sleep_wait(ready, c & 1, err);
         if (!ok) break;
         tc_fence_after();
@@ -486,9 +489,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
             for (int i = 0; i < kStep / 16; ++i) {
-              const uint32_t w = tmem + (pass == 0 ? Tm::kWLo : Tm::kW) + i * 8;
-              const uint32_t k = row_word(base + Sm::kK + (pass == 1) * kBoxes * kBoxBytes, kBoxBytes) + i * kRowStep;
-              umma_ts(tmem + Tm::kDelta, w, k, kRows, pass + i > 0);
+              const uint32_t w = tmem + (second ? Tm::kV : Tm::kW) + (pass == 0 ? 32 : 0) + i * 8;
+              const uint32_t k =
+                  row_word(base + (second ? Sm::kQ : Sm::kK) + (pass == 1) * kBoxes * kBoxBytes, kBoxBytes) + i * kRowStep;
+              umma_ts(tmem + (second ? Tm::kFrom : Tm::kDelta), w, k, kRows, pass + i > 0);
             }
           umma_commit(sums_full);
         }
@@ -503,7 +507,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             for (int pass = 0; pass < 4; ++pass)
 #pragma unroll
               for (int i = 0; i < kStep / 16; ++i) {
-                const uint32_t v = tmem + (pass == 0 ? Tm::kVLo : Tm::kV) + i * 8;
+                const uint32_t v = tmem + Tm::kV + (pass == 0 ? 32 : 0) + i * 8;
                 const int box = pass == 1 ? 1 : pass == 2 ? 2 : 0;
                 const uint32_t p = column_word(base + Sm::kP + box * kBoxBytes) + i * kColumnStep;
                 umma_ts(tmem + Tm::kScore, v, p, kNarrow, pass + i > 0);
@@ -634,6 +638,32 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         put_state(bound);
       }
     }
+    uint32_t sums = 0;
+    // Adds a step's sums to X once the matrix unit has them.
+    auto add_sums = [&](uint32_t at, int m, float w_down) {
+      const float2 a = m == kStep ? fade : decay_over(decay, m);
+      if (ok) ok = sleep_wait(sums_full, sums & 1, err);
+      ++sums;
+      tc_fence_after();
+      const Pair a_hi = pair_of(a.x, a.x), a_lo = pair_of(a.y, a.y), w2 = pair_of(w_down, w_down);
+#pragma unroll
+      for (int part = 0; part < kMine / 16; ++part) {
+        float d[16];
+        tmem_ld16(at_lane + at + group * kMine + 16 * part, d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          Pair& y = x[8 * part + i];
+          y = fma2(y, a_hi, fma2(y, a_lo, mul2(pair_of(d[2 * i], d[2 * i + 1]), w2)));
+        }
+      }
+    };
+    bool pending = false;  // of STATE_ONLY: the step before has sums to add
+    float pending_w = 0.0f;
+    int pending_turn = 0, pending_m = kStep;
+    auto flush = [&] {
+      if (pending) add_sums(pending_turn ? Tm::kFrom : Tm::kDelta, pending_m, pending_w);
+      pending = false;
+    };
     for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
       const int m = min(kStep, t1 - t);
       const int turn = c & 1;
@@ -684,7 +714,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         // A row of zeros has no part in the greatest factor.
         if (lane < kRowsPer) (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u);
         const float up = power_of(268u - biased);
-        uint8_t* box = smem + (is_k ? Sm::kK : Sm::kQ);
+        uint8_t* box = smem + (is_k && !(STATE_ONLY && turn) ? Sm::kK : Sm::kQ);
         const int other = (is_k ? kBoxes : 1) * kBoxBytes;  // from hi to lo
         if (DK == 128) box += (lane >> 4) * (is_k ? 1 : 2) * kBoxBytes;
 #pragma unroll
@@ -735,6 +765,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       }
       if (*(volatile int*)&far_step[turn]) {
         // Token by token.
+        if (STATE_ONLY) flush();
         const float2 one = decay_over(decay, 1);
         const Pair hi = pair_of(one.x, one.x), lo = pair_of(one.y, one.y);
         for (int i = 0; i < m; ++i) {
@@ -801,7 +832,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < 8; ++i) split_pair(val[i], hi[i], lo[i]);
           tmem_st8(at_lane + Tm::kV + group * 8, hi);
-          tmem_st8(at_lane + Tm::kVLo + group * 8, lo);
+          tmem_st8(at_lane + Tm::kV + 32 + group * 8, lo);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -811,8 +842,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           split_pair(mul2(val[2 * i], w0), hi[2 * i], lo[2 * i]);
           split_pair(mul2(val[2 * i + 1], w1), hi[2 * i + 1], lo[2 * i + 1]);
         }
-        tmem_st8(at_lane + Tm::kW + group * 8, hi);
-        tmem_st8(at_lane + Tm::kWLo + group * 8, lo);
+        const uint32_t at_w = at_lane + (STATE_ONLY && turn ? Tm::kV : Tm::kW) + group * 8;
+        tmem_st8(at_w, hi);
+        tmem_st8(at_w + 32, lo);
         p_down *= down * 0x1p22f;
         w_down *= down;
       }
@@ -859,24 +891,18 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
       }
+      if (STATE_ONLY) {
+        if (pending) add_sums(Tm::kDelta + (turn ? 0 : Tm::kFrom - Tm::kDelta), kStep, pending_w);
+        pending = true;
+        pending_w = w_down;
+        pending_turn = turn;
+        pending_m = m;
+        continue;
+      }
       // X, and a bound of it: 64 products of packed values are at most 2^36.
       const float from_down = x_down;
       const float2 a = m == kStep ? fade : decay_over(decay, m);
-      if (ok) ok = sleep_wait(sums_full, steps & 1, err);
-      tc_fence_after();
-      {
-        const Pair a_hi = pair_of(a.x, a.x), a_lo = pair_of(a.y, a.y), w2 = pair_of(w_down, w_down);
-#pragma unroll
-        for (int part = 0; part < kMine / 16; ++part) {
-          float d[16];
-          tmem_ld16(at_lane + Tm::kDelta + group * kMine + 16 * part, d);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            Pair& y = x[8 * part + i];
-            y = fma2(y, a_hi, fma2(y, a_lo, mul2(pair_of(d[2 * i], d[2 * i + 1]), w2)));
-          }
-        }
-      }
+      add_sums(Tm::kDelta, m, w_down);
       if (!STATE_ONLY) {
         bound = fmaf(bound, a.x, 0x1p36f * w_down) * 1.000001f;
         far_state = biased_of(bound) >= 254;
@@ -925,6 +951,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       }
       ++steps;
     }
+    if (STATE_ONLY) flush();
     if (VEC && !STATE_ONLY) {
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
       __syncwarp();
