@@ -173,7 +173,10 @@ def decay_run(lib, t, scale, seq_major, accumulate=None, need=("out", "new_state
 SHAPES = [(1, 1, 1, 1, 1, 1), (2, 2, 1, 1, 128, 128), (1, 1, 1, 2, 3, 5), (1, 2, 2, 5, 128, 128), (2, 3, 3, 17, 33, 40),
           (1, 2, 2, 63, 64, 64), (1, 2, 2, 64, 64, 128), (1, 2, 1, 65, 128, 64), (2, 4, 2, 130, 80, 48),
           (1, 3, 1, 200, 16, 112), (2, 6, 2, 333, 80, 48), (1, 2, 2, 700, 128, 128), (3, 2, 2, 100, 127, 1),
-          (1, 2, 2, 129, 1, 127), (1, 4, 4, 1000, 64, 64), (1, 1, 1, 3000, 32, 32)]
+          (1, 2, 2, 129, 1, 127), (1, 4, 4, 1000, 64, 64), (1, 1, 1, 3000, 32, 32),
+          # Several steps of 64 tokens a block: more heads than SMs, and long sequences in segments.
+          (5, 32, 8, 200, 128, 128), (10, 16, 16, 300, 64, 48), (3, 50, 50, 150, 33, 90), (1, 16, 16, 2500, 128, 128),
+          (1, 8, 4, 4200, 64, 112)]
 
 
 @pytest.mark.parametrize("batch,heads,kv,seq,dk,dv", SHAPES)
@@ -248,6 +251,23 @@ def test_decay_attention_in_parts_is_the_whole(lib, parts):
         at += n
     close(np.concatenate(outs, 1), want["out"], "out")
     close(state.read(), want["new_state"], "state")
+
+
+@pytest.mark.parametrize("seq", [20, 700, 3000])
+def test_decay_attention_replaces_its_state(lib, seq):
+    # Sequences of any length among them empty ones, whose last segments end before the first begin.
+    rng = np.random.default_rng(seq)
+    t = decay_data(rng, 4, 3, 3, seq, 128, 64, True, True)
+    n = np.array([seq, 0, min(seq, 65), 1])
+    t["lengths"] = n.astype(np.float32)
+    want = R.decay_attention(t["q"], t["k"], t["v"], t["decay"], t["state"], n, 0.1, True)
+    buf = [lib.put(t[x]) for x in NAMES]
+    for _ in range(5):
+        buf[4].write(t["state"])
+        out = lib.zeros(t["dout"].size)
+        lib.ok("decay_attention", *buf, out, buf[4], 4, 3, 3, seq, 128, 64, 0.1, True)
+        close(out.read(), want["out"], "out")
+        close(buf[4].read(), want["new_state"], "state")
 
 
 @pytest.mark.parametrize("seq,dim", [(12, 64), (300, 64), (300, 128)])

@@ -385,12 +385,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* v_mosts = k_downs + 128;             // [2][4][128]
   float* x_most = v_mosts + 1024;             // [4][128]
   uint64_t* bars = (uint64_t*)(x_most + 512);
-  int* far_step = (int*)(bars + 9);  // [2]
+  int* far_step = (int*)(bars + 10);  // [2]
   uint32_t* tmem_slot = (uint32_t*)(far_step + 2);
   const uint32_t base = smem_u32(smem);
   const uint32_t raw_full = smem_u32(bars), raw_empty = raw_full + 8, ready = raw_full + 16, values_ready = raw_full + 24,
                  score_full = raw_full + 32, sums_full = raw_full + 40, p_ready = raw_full + 48,
-                 out_full = raw_full + 56, far_seen = raw_full + 64;
+                 out_full = raw_full + 56, far_seen = raw_full + 64,
+                 // Of every second step: with STATE_ONLY the warps may be a step ahead of the issuing one.
+                 ready_odd = raw_full + 72;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int runs = STATE_ONLY ? parts.segments - 1 : parts.segments;
   const int unit = blockIdx.x / runs, part = blockIdx.x - unit * runs;
@@ -406,6 +408,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     mbar_init(raw_full, VEC ? 1 : 32 * kLoaders);
     mbar_init(raw_empty, 1);
     mbar_init(ready, 1);
+    mbar_init(ready_odd, 1);
     mbar_init(values_ready, kWorkers / 32);
     mbar_init(score_full, 1);
     mbar_init(sums_full, 1);
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       bool ok = true;
       for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
         const bool second = STATE_ONLY && (c & 1);
-        ok = sleep_wait(ready, c & 1, err);
+        ok = sleep_wait(c & 1 ? ready_odd : ready, (c >> 1) & 1, err);
         if (!ok) break;
         tc_fence_after();
         if (*(volatile int*)&far_step[c & 1]) {
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       worker_sync();
       if (tid == 0) {
         far_step[turn ^ 1] = 0;
-        mbar_arrive(ready);
+        mbar_arrive(turn ? ready_odd : ready);
       }
       if (*(volatile int*)&far_step[turn]) {
         // Token by token.
@@ -809,6 +812,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         continue;
       }
       if (tid == 0 && t + kStep < t1) mbar_arrive(raw_empty);
+      // (Before this step's values are ready: its own sums would end another phase of the barrier.)
+      if (STATE_ONLY) flush();
       // The keys' factors over the greatest (P), and with a^(63 - j + tail) over the greatest of those (w).
       float p_down, p_inv, w_down;
       {
@@ -892,7 +897,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         if (lane == 0) mbar_arrive(p_ready);
       }
       if (STATE_ONLY) {
-        if (pending) add_sums(Tm::kDelta + (turn ? 0 : Tm::kFrom - Tm::kDelta), kStep, pending_w);
         pending = true;
         pending_w = w_down;
         pending_turn = turn;
