@@ -361,10 +361,10 @@ bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positi
  * [batch] may be NULL (n = seq_len) and holds whole numbers as floats, checked on the
  * device ("Attention start or length out of range"; the sequence then counts as
  * empty); rows from n on are not read, and their out is 0.  Dims 1 to 128, lengths up
- * to 2^29, scale from 2^-60 to 2^60.  Serving calls it with seq_len 1 and the state
+ * to 2^29, scale from 2^-30 to 2^30.  Serving calls it with seq_len 1 and the state
  * kept.  Products carry fp32's accuracy relative to the greatest value in a token's q
  * or k row, in 64 tokens' values of a v column and in a column of the state; where
- * values of 2^60 and more, below 2^-100 (0 aside), infinities or NaN come, 64 tokens
+ * values of 2^60 and more, below 2^-80 (0 aside), infinities or NaN come, 64 tokens
  * at a time go one by one, many times slower.  What leaves fp32's range is infinite or NaN
  * from there on.  The workspace is the context's, as window_attention's. */
 bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* v, void* decay, void* state,

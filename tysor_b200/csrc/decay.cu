@@ -248,13 +248,13 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // A block takes one head's tokens (or a segment of them) step by step: a loading warp
 // brings the next step's rows into shared memory, sixteen warps split them, form P and
 // keep X, an issuing warp feeds the matrix unit.  Values that fp16's range would spoil
-// (2^60 and more, below 2^-100, not finite) send their step through the registers token
+// (2^60 and more, below 2^-80, not finite) send their step through the registers token
 // by token.
 constexpr int kStep = 64;
 constexpr int kWorkers = 512, kScanThreads = kWorkers + 128, kLoaders = 3;  // loading warps
 constexpr int kWorkerRegs = 104, kOtherRegs = 64;  // 4 x 104 + 64 = 5 x 96, what a quarter of an SM is launched with
 constexpr int kBoxBytes = kStep * 128;             // 64 rows of 64 fp16 values
-constexpr uint32_t kLeastBiased = 127 - 100, kFarRange = 160;  // exponents from 2^-100 to 2^60
+constexpr uint32_t kLeastBiased = 127 - 80, kFarRange = 140;  // exponents from 2^-80 to 2^60
 
 // Columns of tensor memory.
 template <int DK>
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
   float* lefts = since + 64;                  // [2][64] a^(63 - j + tail), and the same of a last, shorter step
   float* nears = lefts + 128;                 // [128] a^(d - 63), 0 below
-  float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors, steps in turn
+  float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors (q's times scale), steps in turn
   float* k_downs = q_downs + 128;             // [2][64]
   float* v_mosts = k_downs + 128;             // [2][4][128]
   float* x_most = v_mosts + 1024;             // [4][128]
@@ -688,7 +688,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         constexpr int kRowsPer = STATE_ONLY ? 4 : 8;
         const bool is_k = STATE_ONLY || warp >= 8;
         const int row0 = STATE_ONLY ? warp * 4 : (warp & 7) * 8;
-        // (Where rows hold fewer than DK values, the lanes behind them hold 0.)
+        // (Where rows hold fewer than DK values, the lanes behind them read the first once more
+        // and take them 0 times.)
         const bool held = !VEC || lane * (DK / 32) < s.rows;
         const float* raw = (const float*)(smem + (is_k ? Sm::kRawK : Sm::kRawQ)) + place(row0) * key_pitch +
                            (held ? lane * (DK / 32) : 0);
@@ -699,13 +700,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         for (int r = 0; r < kRowsPer; ++r) {
           float most;
           if constexpr (DK == 128) {
-            float4 w = *(const float4*)(raw + r * next_row);
-            if (VEC && !held) w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 w = *(const float4*)(raw + r * next_row);
             f[r][0] = pair_of(w.x, w.y), f[r][kBoxes - 1] = pair_of(w.z, w.w);
             most = most_of(most_of(w.x, w.y, w.z), w.w, 0.0f);
           } else {
-            float2 w = *(const float2*)(raw + r * next_row);
-            if (VEC && !held) w = make_float2(0.0f, 0.0f);
+            const float2 w = *(const float2*)(raw + r * next_row);
             f[r][0] = pair_of(w.x, w.y);
             most = most_of(w.x, w.y, 0.0f);
           }
@@ -715,14 +714,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         const uint32_t biased = scale_biased(mine);
         far |= far_biased(biased);
         // A row of zeros has no part in the greatest factor.
-        if (lane < kRowsPer) (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u);
+        if (lane < kRowsPer)
+          (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u) * (is_k ? 1.0f : s.scale);
         const float up = power_of(268u - biased);
         uint8_t* box = smem + (is_k && !(STATE_ONLY && turn) ? Sm::kK : Sm::kQ);
         const int other = (is_k ? kBoxes : 1) * kBoxBytes;  // from hi to lo
         if (DK == 128) box += (lane >> 4) * (is_k ? 1 : 2) * kBoxBytes;
 #pragma unroll
         for (int r = 0; r < kRowsPer; ++r) {
-          const float u = __shfl_sync(0xffffffffu, up, r);
+          float u = __shfl_sync(0xffffffffu, up, r);
+          if (VEC && !held) u = 0.0f;
           const Pair u2 = pair_of(u, u);
           const int row = row0 + r;
           if constexpr (DK == 128) {
@@ -744,13 +745,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       // This column's values of 16 tokens.
       Pair val[8];
       {
-        const bool held = !VEC || col < s.cols;
-        const float* raw = (const float*)(smem + Sm::kRawV) + place(group * 16) * value_pitch + (held ? col : 0);
+        // (Threads behind the last column read the first; nothing takes what they hold.)
+        const float* raw = (const float*)(smem + Sm::kRawV) + place(group * 16) * value_pitch + (VEC && col >= s.cols ? 0 : col);
         const int next_row = turned ? -value_pitch : value_pitch;
         float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float a = held ? raw[2 * i * next_row] : 0.0f, d = held ? raw[(2 * i + 1) * next_row] : 0.0f;
+          const float a = raw[2 * i * next_row], d = raw[(2 * i + 1) * next_row];
           val[i] = pair_of(a, d);
           most = most_of(most, a, d);
         }
@@ -916,7 +917,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         float from[16], own[16];
         tmem_ld16(at_lane + Tm::kFrom + group * 16, from);
         tmem_ld16(at_lane + Tm::kScore + group * 16, own);
-        const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down, from_down), s2 = pair_of(s.scale, s.scale);
+        const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down, from_down);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 w = *(const float4*)(since + group * 16 + 4 * i), d = *(const float4*)(q_down + group * 16 + 4 * i);
@@ -925,7 +926,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             const int e = 4 * i + 2 * j;
             const Pair o = fma2(pair_of(from[e], from[e + 1]), mul2(j ? pair_of(w.z, w.w) : pair_of(w.x, w.y), f2),
                                 mul2(pair_of(own[e], own[e + 1]), p2));
-            const float2 y = (mul2(o, mul2(j ? pair_of(d.z, d.w) : pair_of(d.x, d.y), s2)));
+            const Pair y = mul2(o, j ? pair_of(d.z, d.w) : pair_of(d.x, d.y));
             own[e] = y.x, own[e + 1] = y.y;
           }
         }
@@ -1144,7 +1145,8 @@ const char* decay_attention_problem(uint64_t batch, uint64_t heads, uint64_t kv_
   const uint64_t most = 1u << 29;
   if (seq > most || batch > most || heads > most || batch * heads > INT32_MAX)
     return "decay_attention takes lengths, batches and heads up to 2^29, and 2^31 - 1 heads in all";
-  if (!(scale >= 0x1p-60f && scale <= 0x1p60f)) return "decay_attention requires a scale from 2^-60 to 2^60";
+  // (A row's power of two times that stays a normal number.)
+  if (!(scale >= 0x1p-30f && scale <= 0x1p30f)) return "decay_attention requires a scale from 2^-30 to 2^30";
   return nullptr;
 }
 
