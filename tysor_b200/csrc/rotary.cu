@@ -12,8 +12,12 @@ constexpr int kRotaryThreads = 256;
 
 // A thread takes V pairs of a token (or 2 V values behind the turned part, which
 // it copies), forms their angles once, in 64 bits, and goes over a range of heads.
-// Each value is read and written once: HBM bounds it, or one launch's latency.
-template <int V, bool INTERLEAVED>
+// Each value is read and written once: HBM bounds it (8 x 2048 tokens of 16 heads of 128,
+// half of them turned, 268 MB in 51 us = 5.3 TB/s), or one launch's latency (6 us for one
+// token of 32 sequences).  Widths that are no whole float4 move 4 bytes a thread: 16385 x 5
+// heads of 90, 59 MB in 19 us = 3.1 TB/s.
+// `Index` counts the units: 64-bit divisions would take as long as the rest.
+template <int V, bool INTERLEAVED, typename Index>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __restrict__ x,
                                                                 const float* __restrict__ positions,
                                                                 float* __restrict__ out,
@@ -21,12 +25,11 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __r
                                                                 int back, int accumulate) {
   const int turned = s.half / V;                                            // units that turn
   const int per = turned + (s.head_dim - 2 * s.half + 2 * V - 1) / (2 * V);  // and those that do not
-  const int64_t item = (int64_t)blockIdx.x * kRotaryThreads + threadIdx.x;
-  const int64_t tokens = (int64_t)s.batch * s.seq;
-  if (item >= tokens * per) return;
-  const int64_t token = item / per;
-  const int unit = (int)(item - token * per);
-  const int64_t b = token / s.seq, at = token - b * s.seq;
+  const Index item = (Index)blockIdx.x * kRotaryThreads + threadIdx.x;
+  if (item >= (Index)s.batch * (Index)s.seq * (Index)per) return;
+  const Index token32 = item / (Index)per;
+  const int unit = (int)(item - token32 * (Index)per);
+  const int64_t token = (int64_t)token32, b = (int64_t)(token32 / (Index)s.seq), at = token - b * s.seq;
   const int64_t step = s.seq_major ? s.head_dim : (int64_t)s.head_dim * s.seq;
   const int64_t base = (s.seq_major ? (b * s.seq + at) * s.heads : b * s.heads * s.seq + at) * s.head_dim;
   const int h0 = blockIdx.y * head_chunk, h1 = min(s.heads, h0 + head_chunk);
@@ -144,17 +147,22 @@ void launch_rotary(const float* x, const float* positions, float* out, const Rot
   const bool vec = shape.half % 4 == 0 && shape.head_dim % 8 == 0 && (((uintptr_t)x | (uintptr_t)out) & 15) == 0;
   const int V = vec ? 4 : 1;
   const int64_t items = tokens * (shape.half / V + ceil_div(shape.head_dim - 2 * shape.half, 2 * V));
-  // All heads of a token in one thread share its angles; where that leaves
-  // fewer than two blocks per SM, the heads are spread over more threads.
-  int64_t chunk = shape.heads * items / (148 * 2 * kRotaryThreads);
+  // The heads of a token in one thread share its angles; where that leaves fewer than
+  // eight blocks per SM, they are spread over more threads (8 x 2048 tokens of 16 heads
+  // forward and back 107 us with two, 103 with eight, 117 with 32).
+  int64_t chunk = shape.heads * items / (148 * 8 * kRotaryThreads);
   const int64_t least = ceil_div(shape.heads, 65535);  // blocks of the grid's second axis
   chunk = chunk < least ? least : chunk > shape.heads ? shape.heads : chunk;
   const dim3 grid((unsigned)ceil_div(items, kRotaryThreads), (unsigned)ceil_div(shape.heads, chunk));
   auto go = [&](auto kernel) {
     kernel<<<grid, kRotaryThreads, 0, st>>>(x, positions, out, shape, (int)chunk, back, accumulate);
   };
-  if (vec) shape.interleaved ? go(rotary_kernel<4, true>) : go(rotary_kernel<4, false>);
-  else shape.interleaved ? go(rotary_kernel<1, true>) : go(rotary_kernel<1, false>);
+  auto pick = [&]<typename Index>(Index) {
+    if (vec) shape.interleaved ? go(rotary_kernel<4, true, Index>) : go(rotary_kernel<4, false, Index>);
+    else shape.interleaved ? go(rotary_kernel<1, true, Index>) : go(rotary_kernel<1, false, Index>);
+  };
+  if (items < INT64_C(4000000000)) pick(uint32_t{});
+  else pick(int64_t{});
   g_launches.fetch_add(1, std::memory_order_relaxed);
   TYSOR_CUDA(cudaGetLastError());
 }
