@@ -41,7 +41,8 @@ SCALINGS = [PLAIN, (1, 4.0, 0.0, 0.0, 0.0, 1.0), (2, 8.0, 4096.0, 1.0, 4.0, 0.75
 
 @pytest.mark.parametrize("batch,heads,seq,head_dim,rotary_dim", [
     (1, 1, 1, 2, 2), (1, 3, 5, 7, 4), (2, 4, 33, 64, 64), (2, 4, 33, 128, 64), (1, 5, 17, 90, 90), (3, 2, 9, 80, 24),
-    (1, 16, 300, 128, 128), (1, 2, 3, 512, 512), (1, 2, 3, 1000, 512), (1, 70000, 1, 8, 8), (2, 3, 40, 12, 8)])
+    (1, 16, 300, 128, 128), (1, 2, 3, 512, 512), (1, 2, 3, 1000, 512), (1, 70000, 1, 8, 8), (2, 3, 40, 12, 8),
+    (2, 3, 9, 12, 4), (1, 6, 300, 128, 44), (1, 5, 17, 14, 12)])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("scaling", SCALINGS)
 def test_rotary(lib, batch, heads, seq, head_dim, rotary_dim, interleaved, scaling):

@@ -10,12 +10,34 @@ namespace {
 
 constexpr int kRotaryThreads = 256;
 
+// N neighbouring values, at an address that is a multiple of theirs.
+template <int N>
+__device__ __forceinline__ void load_values(float* f, const float* p) {
+  if constexpr (N == 4) {
+    const float4 w = *(const float4*)p;
+    f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+  } else if constexpr (N == 2) {
+    const float2 w = *(const float2*)p;
+    f[0] = w.x, f[1] = w.y;
+  } else {
+    f[0] = *p;
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_values(float* p, const float* f) {
+  if constexpr (N == 4) *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+  else if constexpr (N == 2) *(float2*)p = make_float2(f[0], f[1]);
+  else *p = f[0];
+}
+
 // A thread takes V pairs of a token (or 2 V values behind the turned part, which
 // it copies), forms their angles once, in 64 bits, and goes over a range of heads.
 // Each value is read and written once: HBM bounds it (8 x 2048 tokens of 16 heads of 128,
 // half of them turned, 268 MB in 51 us = 5.3 TB/s), or one launch's latency (6 us for one
-// token of 32 sequences).  Widths that are no whole float4 move 4 bytes a thread: 16385 x 5
-// heads of 90, 59 MB in 19 us = 3.1 TB/s.
+// token of 32 sequences).  An odd number of pairs
+// moves 4 bytes at a time: 16385 x 5 heads of 90, 59 MB in 19 us = 3.1 TB/s (8 bytes for
+// neighbours that turn together are no faster); pairs by two, 8 x 2048 tokens of 16 heads of
+// 128 with 44 turned, take 63 us, one at a time 86.
 // `Index` counts the units: 64-bit divisions would take as long as the rest.
 template <int V, bool INTERLEAVED, typename Index>
 __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __restrict__ x,
@@ -23,6 +45,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __r
                                                                 float* __restrict__ out,
                                                                 const __grid_constant__ RotaryShape s, int head_chunk,
                                                                 int back, int accumulate) {
+  constexpr int W = INTERLEAVED && V == 2 ? 4 : V;  // the turned values of one load
   const int turned = s.half / V;                                            // units that turn
   const int per = turned + (s.head_dim - 2 * s.half + 2 * V - 1) / (2 * V);  // and those that do not
   const Index item = (Index)blockIdx.x * kRotaryThreads + threadIdx.x;
@@ -68,43 +91,29 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const float* __r
   }
   // The unit's values: V and V of them `half` apart, or 2 V in a row.
   const int first = INTERLEAVED ? 2 * i0 : i0, second = INTERLEAVED ? first + V : first + s.half;
+  auto spot = [&](int e) { return e < V ? first + e : second + e - V; };
 #pragma unroll 4
   for (int h = h0; h < h1; ++h) {
     const int64_t o = base + h * step;
-    float f[2][V];
+    float f[2 * V];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float* src = x + o + (k ? second : first);
-      if (V % 4 == 0) {
-        const float4 w = *(const float4*)src;
-        f[k][0] = w.x, f[k][1 % V] = w.y, f[k][2 % V] = w.z, f[k][3 % V] = w.w;
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[k][v] = src[v];
-      }
-    }
+    for (int e = 0; e < 2 * V; e += W) load_values<W>(f + e, x + o + spot(e));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float& lo = INTERLEAVED ? f[2 * v / V][2 * v % V] : f[0][v];
-      float& hi = INTERLEAVED ? f[(2 * v + 1) / V][(2 * v + 1) % V] : f[1][v];
+      float &lo = f[INTERLEAVED ? 2 * v : v], &hi = f[INTERLEAVED ? 2 * v + 1 : V + v];
       const float t = lo * cs[v] - hi * sn[v];
       hi = lo * sn[v] + hi * cs[v];
       lo = t;
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float* dst = out + o + (k ? second : first);
-      if (V % 4 == 0) {
-        float4 w = make_float4(f[k][0], f[k][1 % V], f[k][2 % V], f[k][3 % V]);
-        if (accumulate) {
-          const float4 g = *(const float4*)dst;
-          w.x += g.x, w.y += g.y, w.z += g.z, w.w += g.w;
-        }
-        *(float4*)dst = w;
-      } else {
+    for (int e = 0; e < 2 * V; e += W) {
+      if (accumulate) {
+        float old[W];
+        load_values<W>(old, out + o + spot(e));
 #pragma unroll
-        for (int v = 0; v < V; ++v) dst[v] = accumulate ? dst[v] + f[k][v] : f[k][v];
+        for (int i = 0; i < W; ++i) f[e + i] += old[i];
       }
+      store_values<W>(out + o + spot(e), f + e);
     }
   }
 }
@@ -144,8 +153,11 @@ void launch_rotary(const float* x, const float* positions, float* out, const Rot
                    int accumulate, cudaStream_t st) {
   const int64_t tokens = (int64_t)shape.batch * shape.seq;
   if (tokens <= 0 || shape.heads <= 0) return;
-  const bool vec = shape.half % 4 == 0 && shape.head_dim % 8 == 0 && (((uintptr_t)x | (uintptr_t)out) & 15) == 0;
-  const int V = vec ? 4 : 1;
+  // As wide as a head's halves and width and the tensors' starts allow.
+  const uintptr_t starts = (uintptr_t)x | (uintptr_t)out;
+  const int V = shape.half % 4 == 0 && shape.head_dim % 8 == 0 && starts % 16 == 0   ? 4
+                : shape.half % 2 == 0 && shape.head_dim % 4 == 0 && starts % 16 == 0 ? 2
+                                                                                     : 1;
   const int64_t items = tokens * (shape.half / V + ceil_div(shape.head_dim - 2 * shape.half, 2 * V));
   // The heads of a token in one thread share its angles; where that leaves fewer than
   // eight blocks per SM, they are spread over more threads (8 x 2048 tokens of 16 heads
@@ -158,7 +170,8 @@ void launch_rotary(const float* x, const float* positions, float* out, const Rot
     kernel<<<grid, kRotaryThreads, 0, st>>>(x, positions, out, shape, (int)chunk, back, accumulate);
   };
   auto pick = [&]<typename Index>(Index) {
-    if (vec) shape.interleaved ? go(rotary_kernel<4, true, Index>) : go(rotary_kernel<4, false, Index>);
+    if (V == 4) shape.interleaved ? go(rotary_kernel<4, true, Index>) : go(rotary_kernel<4, false, Index>);
+    else if (V == 2) shape.interleaved ? go(rotary_kernel<2, true, Index>) : go(rotary_kernel<2, false, Index>);
     else shape.interleaved ? go(rotary_kernel<1, true, Index>) : go(rotary_kernel<1, false, Index>);
   };
   if (items < INT64_C(4000000000)) pick(uint32_t{});
