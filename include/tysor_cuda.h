@@ -377,7 +377,8 @@ bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* 
  *   E_n = dnew_state + scale * q_n dout_n^T,   E_t = a * E_(t+1) + scale * q_t dout_t^T:
  * dq_t (+)= scale * dout_t S_t^T, dk_t (+)= v_t E_t^T, dv_t (+)= k_t E_t (dk and dv
  * summed over the query heads that share a key head, in a fixed order), dstate (+)=
- * a * E_1 (may be NULL).  Rows from n on get 0. */
+ * a * E_1 (may be NULL).  Rows from n on get 0.  E is held as E / scale, which is to stay
+ * in fp32's range as well. */
 bool tysor_cuda_dispatch_decay_attention_backward(void* context, void* q, void* k, void* v, void* decay,
                                                   void* state, void* lengths, void* dout, void* dnew_state,
                                                   void* dq, void* dk, void* dv, void* dstate, uint32_t batch,
@@ -392,8 +393,9 @@ bool tysor_cuda_dispatch_decay_attention_backward(void* context, void* q, void* 
  * with given 0, entropy always, top_ids and top_logprobs with top 0.  Tokens whose logit
  * is -inf have ln p = -inf and are no best tokens: where none is left, id -1 and -inf.  A
  * row of nothing but -inf has entropy 0, one with NaN or +inf holds NaN and no best
- * tokens.  T is from 2^-60 to 2^60.  stats may be NULL or receives [rows][2] =
- * (greatest logit, sum of exp((logit - greatest) / T)); the backward reads it. */
+ * tokens.  T is from 2^-60 to 2^60, rows are at most 2^31 - 1.  stats may be NULL or
+ * receives [rows][2] = (greatest logit, sum of exp((logit - greatest) / T)), which the
+ * backward reads; it starts on an 8-byte boundary. */
 bool tysor_cuda_dispatch_token_logprobs(void* context, void* logits, void* ids, void* out, void* entropy,
                                         void* top_ids, void* top_logprobs, void* stats, uint32_t rows,
                                         uint32_t width, uint32_t given, uint32_t top, float temperature);

@@ -538,6 +538,7 @@ def test_token_logprobs_refusals(lib):
 
     bad("width of 1 to 2^24", 8, 0, 1, 0, 1.0)
     bad("width of 1 to 2^24", 0, (1 << 24) + 1, 1, 0, 1.0)
+    bad("up to 2^31 - 1 rows", 1 << 31, 8, 1, 0, 1.0)
     bad("up to 128 given", 8, 8, 129, 0, 1.0)
     bad("up to 128 best", 8, 8, 1, 129, 1.0)
     for t in (0.0, -1.0, float("nan"), float("inf"), 1e-30):

@@ -375,6 +375,7 @@ DecayInputs decay_inputs(Operands& o, const DecayShape& s, void* q, void* k, voi
 LogprobShape logprob_shape(uint32_t rows, uint32_t width, uint32_t given, uint32_t top, float temperature) {
   if (width == 0 || width > (uint32_t)kMaxLogprobWidth)
     throw CudaError("token_logprobs requires a width of 1 to 2^24");
+  if (rows > (uint32_t)INT32_MAX) throw CudaError("token_logprobs takes up to 2^31 - 1 rows");
   if (given > (uint32_t)kMaxGivenTokens)
     throw CudaError("token_logprobs takes up to " + std::to_string(kMaxGivenTokens) + " given ids a row");
   if (top > (uint32_t)kMaxTopTokens)

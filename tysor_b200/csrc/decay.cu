@@ -1045,7 +1045,8 @@ int64_t states_elems(const DecayShape& s) {
   if (s.seq < kChunkedFrom) return 0;
   const int64_t units = (int64_t)s.batch * s.heads;
   const int segments = segments_of(units, s.seq);
-  return segments > 1 ? units * segments * s.key_dim * s.value_dim : 0;
+  // (What lies behind them starts on a 16-byte boundary.)
+  return segments > 1 ? ceil_div(units * segments * s.key_dim * s.value_dim, 4) * 4 : 0;
 }
 
 // Whether an operand's rows are whole 16-byte pieces.

@@ -1411,6 +1411,7 @@ struct Executor {
       fail(with_ids ? "token_logprobs expects (logits, ids, temperature)" : "token_entropy expects (logits, temperature)");
     const int64_t w = z.shape.back(), rows = numel(z.shape) / w;
     if (w > kMaxLogprobWidth) fail(node.op + " requires a width of 1 to 2^24");
+    if (rows > INT32_MAX) fail(node.op + " takes up to 2^31 - 1 rows");
     int64_t given = 0;
     if (with_ids) {
       const HVal& id = tensor(node.inputs[1], "token_logprobs ids");
