@@ -310,12 +310,26 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from,
 }
 
 struct ScanParts {
-  int segments;  // blocks that share a head's tokens
-  // [unit][segments][rows * cols], with more than one: in each segment's place the one before
-  // its own state, then the state that it starts from.  (The call's new state may replace the
-  // old one, so no segment but a head's only one reads that.)
+  // [unit][slots][rows * cols], with several segments: the state that the first starts from,
+  // then each piece's own state, and in their places the states behind the pieces.  (The call's
+  // new state may replace the old one, so no segment but a head's only one reads that.)
   float* states;
   int si, sj;  // between their key rows and value columns, for the segments that start from them
+};
+
+// How a head's tokens are shared: `segments` blocks take turns of whole steps, and where
+// there is more than one, `pieces` blocks each form the own states of all but the last.
+struct Split {
+  int segments, pieces;
+  int slots;  // a head's states: (segments - 1) * pieces + 1
+};
+// Scans of one launch: all of as many sequences and heads, and of one kind.
+constexpr int kMostScans = 3;
+struct Scans {
+  Split split;
+  ScanMaps maps[kMostScans];
+  Scan scan[kMostScans];
+  ScanParts parts[kMostScans];
 };
 
 __device__ __forceinline__ void worker_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory"); }
@@ -356,11 +370,18 @@ __device__ __forceinline__ void copy_async4(uint32_t to, const float* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-// The tokens of a sequence that segment `part` takes: [first, last) of the order of the scan.
-__device__ __forceinline__ void segment_of(int n, int segments, int part, int* first, int* last) {
-  const int steps = (n + kStep - 1) / kStep, per = (steps + segments - 1) / segments;
-  *first = min(n, part * per * kStep);
-  *last = min(n, (part + 1) * per * kStep);
+// The tokens of a sequence that segment `part` takes, or its piece `piece` (or all of it, -1):
+// [first, last) of the order of the scan.
+__device__ __forceinline__ void segment_of(int n, const Split& split, int part, int piece, int* first, int* last) {
+  const int steps = (n + kStep - 1) / kStep, per = (steps + split.segments - 1) / split.segments;
+  int from = part * per, to = from + per;
+  if (piece >= 0) {
+    const int each = (per + split.pieces - 1) / split.pieces;
+    from += piece * each;
+    to = min(to, from + each);
+  }
+  *first = min(n, from * kStep);
+  *last = max(*first, min(n, to * kStep));
 }
 
 // STATE_ONLY: the segment's own state (from 0), for the segments behind it.  Its steps have
@@ -368,9 +389,11 @@ __device__ __forceinline__ void segment_of(int n, int segments, int part, int* f
 // are added while the matrix unit is at the next.  VEC: rows of
 // whole 16-byte pieces.
 template <int DK, bool STATE_ONLY, bool VEC>
-__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scan s,
-                                                               const __grid_constant__ ScanMaps maps, ScanParts parts,
-                                                               int* err) {
+__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Scans all, int* err) {
+  const Scan& s = all.scan[blockIdx.y];
+  const ScanMaps& maps = all.maps[blockIdx.y];
+  const ScanParts& parts = all.parts[blockIdx.y];
+  const int segments = all.split.segments;
   using Tm = ScanTmem<DK>;
   using Sm = ScanSmem<DK>;
   constexpr int kBoxes = DK / 64, kMine = DK / 4;  // state values of a thread
@@ -394,12 +417,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
                  // Of every second step: with STATE_ONLY the warps may be a step ahead of the issuing one.
                  ready_odd = raw_full + 72;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int runs = STATE_ONLY ? parts.segments - 1 : parts.segments;
-  const int unit = blockIdx.x / runs, part = blockIdx.x - unit * runs;
+  const int runs = STATE_ONLY ? (segments - 1) * all.split.pieces : segments;
+  const int unit = blockIdx.x / runs, run = blockIdx.x - unit * runs;
+  const int part = STATE_ONLY ? run / all.split.pieces : run, piece = STATE_ONLY ? run - part * all.split.pieces : -1;
   const int b = unit / s.heads, h = unit - b * s.heads;
   const int n = tokens_of(s, b, err);
   int t0, t1;
-  segment_of(n, parts.segments, part, &t0, &t1);
+  segment_of(n, all.split, part, piece, &t0, &t1);
   const float decay = decay_of(s, h, err);
   const int lead = s.back ? 0 : 1, tail = 1 - lead;
   auto power = [&](int steps) { return steps == 0 ? 1.0f : expf(-decay * steps); };
@@ -581,8 +605,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
 #pragma unroll
       for (int i = 0; i < kMine; ++i) first[i] = 0.0f;
       if (!STATE_ONLY && col < s.cols) {
-        if (parts.segments > 1) {
-          const float* from = parts.states + ((int64_t)unit * parts.segments + part) * s.rows * s.cols;
+        if (segments > 1) {
+          const float* from = parts.states + ((int64_t)unit * all.split.slots + part * all.split.pieces) * s.rows * s.cols;
 #pragma unroll
           for (int i = 0; i < kMine; ++i) {
             const int r = group * kMine + i;
@@ -963,16 +987,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     }
     // Rows behind the sequence's end, spread over its blocks.
     if (!STATE_ONLY && !s.accumulate)
-      for (int r = n + part * 4 + group; r < s.seq; r += 4 * parts.segments)
+      for (int r = n + part * 4 + group; r < s.seq; r += 4 * segments)
         if (col < s.cols) out[(int64_t)r * s.out.token + col] = 0.0f;
-    if (STATE_ONLY || (s.to.p != nullptr && part == parts.segments - 1)) {
+    if (STATE_ONLY || (s.to.p != nullptr && part == segments - 1)) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         const int r = group * kMine + i;
         const float y = i & 1 ? x[i / 2].y : x[i / 2].x;
         if (r >= s.rows || col >= s.cols) continue;
         if (STATE_ONLY) {
-          parts.states[((int64_t)unit * parts.segments + part + 1) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
+          parts.states[((int64_t)unit * all.split.slots + run + 1) * s.rows * s.cols + (int64_t)r * s.cols + col] = y;
         } else {
           float* to = s.to.p + state + r * s.to.si + col * s.to.sj;
           *to = s.accumulate_state ? *to + y * s.to_factor : y * s.to_factor;
@@ -987,66 +1011,90 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
 }
 
-// From each segment's own state the state that the next one starts from, in place.
-__global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant__ Scan s, ScanParts parts, int* err) {
+// From each piece's own state the state behind it, in place.
+__global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant__ Scans all, int* err) {
+  const Scan& s = all.scan[blockIdx.z];
   const int unit = blockIdx.y, b = unit / s.heads, h = unit - b * s.heads;
   const int i = blockIdx.x * 256 + threadIdx.x, elems = s.rows * s.cols;
   if (i >= elems) return;
-  const int n = tokens_of(s, b, err);
+  const int n = tokens_of(s, b, err), runs = all.split.slots - 1;
   const float decay = decay_of(s, h, err);
   const int r = i / s.cols, c = i - r * s.cols;
   float x = s.from.p != nullptr ? s.from.p[(int64_t)unit * elems + r * s.from.si + c * s.from.sj] * s.from_factor : 0.0f;
-  float* at = parts.states + (int64_t)unit * parts.segments * elems + i;
-  at[0] = x;
-  for (int j = 0; j + 1 < parts.segments; ++j) {
-    int t0, t1;
-    segment_of(n, parts.segments, j, &t0, &t1);
-    const float2 a = decay_over(decay, t1 - t0);
-    at += elems;
-    x = fmaf(x, a.x, fmaf(x, a.y, *at));
-    *at = x;
+  float* at = all.parts[blockIdx.z].states + (int64_t)unit * all.split.slots * elems + i;
+  *at = x;
+  float2 a = make_float2(1.0f, 0.0f);
+  int held = 0;
+  constexpr int kAhead = 8;
+  for (int j0 = 0; j0 < runs; j0 += kAhead) {
+    float own[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) own[k] = j0 + k < runs ? at[(int64_t)(k + 1) * elems] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (j0 + k >= runs) break;
+      const int part = (j0 + k) / all.split.pieces;
+      int t0, t1;
+      segment_of(n, all.split, part, j0 + k - part * all.split.pieces, &t0, &t1);
+      if (t1 - t0 != held) a = decay_over(decay, t1 - t0), held = t1 - t0;
+      x = fmaf(x, a.x, fmaf(x, a.y, own[k]));
+      at += elems;
+      *at = x;
+    }
   }
 }
 
 // dst[b][g] (+)= sum over the heads that share key head g of src[b][h], in order.
-__global__ void __launch_bounds__(256) sum_heads_kernel(const float* __restrict__ src, Rows dst, int batch,
-                                                        int kv_heads, int group, int seq, int dim, int accumulate) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)batch * kv_heads * seq * dim;
+struct HeadSum {
+  const float* src;
+  Rows dst;
+  int dim, accumulate;
+};
+struct HeadSums {
+  HeadSum of[2];
+};
+__global__ void __launch_bounds__(256) sum_heads_kernel(const __grid_constant__ HeadSums sums, int batch, int kv_heads,
+                                                        int group, int seq) {
+  const HeadSum& s = sums.of[blockIdx.y];
+  const Rows& dst = s.dst;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)batch * kv_heads * seq * s.dim;
   if (i >= n) return;
-  const int64_t row = i / dim, c = i - row * dim;
+  const int64_t row = i / s.dim, c = i - row * s.dim;
   const int64_t bg = row / seq, t = row - bg * seq;
-  const float* from = src + (bg * group * seq + t) * dim + c;
+  const float* from = s.src + (bg * group * seq + t) * s.dim + c;
   float sum = 0.0f;
-  for (int k = 0; k < group; ++k) sum += from[(int64_t)k * seq * dim];
+  for (int k = 0; k < group; ++k) sum += from[(int64_t)k * seq * s.dim];
   float* to = const_cast<float*>(dst.p) + bg / kv_heads * dst.batch + bg % kv_heads * dst.head + t * dst.token + c;
-  *to = accumulate ? *to + sum : sum;
+  *to = s.accumulate ? *to + sum : sum;
 }
 
 // From how many tokens on 64 at a time are faster than one by one.
 constexpr int kChunkedFrom = 24;
 
-// How many blocks share a head's tokens: they take turns of 64 tokens each, and
-// where there is more than one, a first pass over the keys and values (about half
-// the time) gives their states.
-int segments_of(int64_t units, int seq) {
+// How the tokens of each of `units` heads are shared, of `scans` in one launch, of `states` of
+// which a first launch forms states (in about half the time a step).
+Split split_of(int64_t units, int seq, int scans, int states) {
   const int64_t steps = ceil_div(seq, kStep);
-  double best = 1e30;
-  int segments = 1;
-  for (int64_t n = 1; n <= (units > 1024 ? 1 : std::min<int64_t>(steps, 64)); ++n) {
-    const double per = (double)ceil_div(steps, n);
-    double cost = (double)ceil_div(units * n, 148) * (per + 2.0);
-    if (n > 1) cost += (double)ceil_div(units * (n - 1), 148) * (0.5 * per + 2.0) + 3.0;
-    if (cost < best) best = cost, segments = (int)n;
+  double best = (double)ceil_div(scans * units, 148) * (steps + 2.0);
+  Split split{1, 1, 1};
+  if (units > 1024) return split;
+  for (int64_t n = 2; n <= std::min<int64_t>(steps, 64); ++n) {
+    const int64_t per = ceil_div(steps, n);
+    for (int64_t p = 1; p <= std::min<int64_t>(per, 64 / n); ++p) {
+      const double cost = (double)ceil_div(scans * units * n, 148) * (per + 2.0) +
+                          (double)ceil_div(states * units * (n - 1) * p, 148) * (0.5 * ceil_div(per, p) + 2.0) + 3.0;
+      if (cost < best) best = cost, split = {(int)n, (int)p, (int)((n - 1) * p + 1)};
+    }
   }
-  return segments;
+  return split;
 }
+Split forward_split(const DecayShape& s) { return split_of((int64_t)s.batch * s.heads, s.seq, 1, 1); }
+Split backward_split(const DecayShape& s) { return split_of((int64_t)s.batch * s.heads, s.seq, 3, 2); }
 
-int64_t states_elems(const DecayShape& s) {
-  if (s.seq < kChunkedFrom) return 0;
-  const int64_t units = (int64_t)s.batch * s.heads;
-  const int segments = segments_of(units, s.seq);
-  // (What lies behind them starts on a 16-byte boundary.)
-  return segments > 1 ? ceil_div(units * segments * s.key_dim * s.value_dim, 4) * 4 : 0;
+// Floats of a scan's states.  (What lies behind them starts on a 16-byte boundary.)
+int64_t states_elems(const DecayShape& s, const Split& split) {
+  if (s.seq < kChunkedFrom || split.segments == 1) return 0;
+  return ceil_div((int64_t)s.batch * s.heads * split.slots * s.key_dim * s.value_dim, 4) * 4;
 }
 
 // Whether an operand's rows are whole 16-byte pieces.
@@ -1055,7 +1103,7 @@ bool whole_pieces(const Rows& r, int dim) {
 }
 
 template <int DK, bool STATE_ONLY, bool VEC>
-void launch_chunks(const Scan& s, const ScanMaps& maps, const ScanParts& parts, int blocks, int* err, cudaStream_t st) {
+void launch_chunks(const Scans& scans, int count, int* err, cudaStream_t st) {
   auto kernel = scan_kernel<DK, STATE_ONLY, VEC>;
   static std::atomic<uint64_t> set{0};  // devices whose limit is set
   int device;
@@ -1070,52 +1118,86 @@ void launch_chunks(const Scan& s, const ScanMaps& maps, const ScanParts& parts, 
     TYSOR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<DK>::kBytes));
     set.fetch_or(bit, std::memory_order_relaxed);
   }
-  kernel<<<blocks, kScanThreads, ScanSmem<DK>::kBytes, st>>>(s, maps, parts, err);
+  const int units = scans.scan[0].batch * scans.scan[0].heads, runs = STATE_ONLY ? scans.split.slots - 1 : scans.split.segments;
+  kernel<<<dim3((unsigned)(units * runs), (unsigned)count), kScanThreads, ScanSmem<DK>::kBytes, st>>>(scans, err);
   check_launch();
 }
 
-template <int DK, bool VEC>
-void run_chunks(const Scan& s, const ScanParts& parts, bool states_there, int* err, cudaStream_t st) {
-  const int units = s.batch * s.heads;
-  ScanMaps maps{};
-  if (VEC) {
-    auto map = [&](const Rows& r, int dim, int box_cols, int box_rows) {
-      return rows_map(r.p, {(uint64_t)dim, (uint64_t)s.seq, (uint64_t)(s.heads / r.share), (uint64_t)s.batch},
-                      {(uint64_t)r.token, (uint64_t)r.head, (uint64_t)r.batch}, box_cols, box_rows);
-    };
-    maps.q = map(s.q, s.rows, s.rows, kStep);
-    maps.k = map(s.k, s.rows, s.rows, kStep);
-    maps.v = map(s.v, s.cols, s.cols, kStep);
-    maps.stores = whole_pieces(s.out, s.cols);
-    if (maps.stores) maps.out = map(s.out, s.cols, 32, 16);
-  }
-  if (parts.segments > 1 && !states_there) {
-    launch_chunks<DK, true, VEC>(s, maps, parts, units * (parts.segments - 1), err, st);
-    scan_states_kernel<<<dim3((unsigned)ceil_div(s.rows * s.cols, 256), (unsigned)units), 256, 0, st>>>(s, parts, err);
-    check_launch();
-  }
-  launch_chunks<DK, false, VEC>(s, maps, parts, units * parts.segments, err, st);
+// A scan and where it has the states of its segments.
+struct ScanCall {
+  Scan s;
+  ScanParts parts;
+  bool own_states;  // or those that an earlier call of the launch forms
+
+  bool vec() const { return whole_pieces(s.q, s.rows) && whole_pieces(s.k, s.rows) && whole_pieces(s.v, s.cols); }
+};
+
+ScanMaps maps_of(const Scan& s) {
+  auto map = [&](const Rows& r, int dim, int box_cols, int box_rows) {
+    return rows_map(r.p, {(uint64_t)dim, (uint64_t)s.seq, (uint64_t)(s.heads / r.share), (uint64_t)s.batch},
+                    {(uint64_t)r.token, (uint64_t)r.head, (uint64_t)r.batch}, box_cols, box_rows);
+  };
+  ScanMaps maps{map(s.q, s.rows, s.rows, kStep), map(s.k, s.rows, s.rows, kStep), map(s.v, s.cols, s.cols, kStep), {},
+                whole_pieces(s.out, s.cols)};
+  if (maps.stores) maps.out = map(s.out, s.cols, 32, 16);
+  return maps;
 }
 
-// `states`: states_elems floats.  `turned_states`: they hold those of a scan whose state is this
-// one's transposed.
-void run_scan(const Scan& s, float* states, int* err, cudaStream_t st, bool turned_states = false) {
-  if (s.batch <= 0 || s.heads <= 0) return;
-  if (s.seq >= kChunkedFrom) {
-    const ScanParts parts{segments_of((int64_t)s.batch * s.heads, s.seq), states, turned_states ? 1 : s.cols,
-                          turned_states ? s.rows : 1};
-    const bool vec = whole_pieces(s.q, s.rows) && whole_pieces(s.k, s.rows) && whole_pieces(s.v, s.cols);
-    if (s.rows > 64) vec ? run_chunks<128, true>(s, parts, turned_states, err, st) : run_chunks<128, false>(s, parts, turned_states, err, st);
-    else vec ? run_chunks<64, true>(s, parts, turned_states, err, st) : run_chunks<64, false>(s, parts, turned_states, err, st);
+// Scans of as many sequences and heads that do not need one another's outputs, each kind of
+// kernel in one launch: heads that leave SMs without a block do so once, not once a scan.
+void run_scans(const ScanCall* calls, int count, const Split& split, int* err, cudaStream_t st) {
+  const Scan& any = calls[0].s;
+  if (any.batch <= 0 || any.heads <= 0) return;
+  if (any.seq < kChunkedFrom) {
+    for (int i = 0; i < count; ++i) {
+      const Scan& s = calls[i].s;
+      auto plain = [&](const StateAt& x) {
+        return x.p == nullptr || (x.si == s.cols && x.sj == 1 && ((uintptr_t)x.p & 15) == 0);
+      };
+      const dim3 grid((unsigned)(s.batch * s.heads), (unsigned)ceil_div(s.cols, kSlice));
+      if (s.cols % 4 == 0 && plain(s.from) && plain(s.to)) step_kernel<true><<<grid, kStepThreads, 0, st>>>(s, err);
+      else step_kernel<false><<<grid, kStepThreads, 0, st>>>(s, err);
+      check_launch();
+    }
     return;
   }
-  auto plain = [&](const StateAt& x) {
-    return x.p == nullptr || (x.si == s.cols && x.sj == 1 && ((uintptr_t)x.p & 15) == 0);
+  // (Keys and values of different widths: the gradients' scans still go together.)
+  bool wide = false;
+  for (int i = 0; i < count; ++i) wide |= calls[i].s.rows > 64;
+  auto pass = [&](bool vec, bool state_only) {
+    Scans scans{};
+    scans.split = split;
+    int n = 0;
+    for (int i = 0; i < count; ++i) {
+      const ScanCall& c = calls[i];
+      if (c.vec() != vec || (state_only && !c.own_states)) continue;
+      if (vec) scans.maps[n] = maps_of(c.s);
+      scans.scan[n] = c.s;
+      scans.parts[n++] = c.parts;
+    }
+    if (n == 0) return;
+    auto go = [&]<int DK, bool VEC>() {
+      state_only ? launch_chunks<DK, true, VEC>(scans, n, err, st) : launch_chunks<DK, false, VEC>(scans, n, err, st);
+    };
+    if (wide) vec ? go.template operator()<128, true>() : go.template operator()<128, false>();
+    else vec ? go.template operator()<64, true>() : go.template operator()<64, false>();
   };
-  const dim3 grid((unsigned)(s.batch * s.heads), (unsigned)ceil_div(s.cols, kSlice));
-  if (s.cols % 4 == 0 && plain(s.from) && plain(s.to)) step_kernel<true><<<grid, kStepThreads, 0, st>>>(s, err);
-  else step_kernel<false><<<grid, kStepThreads, 0, st>>>(s, err);
-  check_launch();
+  auto passes = [&](bool state_only) {
+    pass(false, state_only);
+    pass(true, state_only);
+  };
+  if (split.segments > 1) {
+    passes(true);
+    Scans scans{};
+    scans.split = split;
+    int n = 0;
+    for (int i = 0; i < count; ++i)
+      if (calls[i].own_states) scans.scan[n] = calls[i].s, scans.parts[n++] = calls[i].parts;
+    scan_states_kernel<<<dim3((unsigned)ceil_div(any.rows * any.cols, 256), (unsigned)(any.batch * any.heads), (unsigned)n),
+                         256, 0, st>>>(scans, err);
+    check_launch();
+  }
+  passes(false);
 }
 
 Rows rows_of(const DecayShape& s, const float* p, int heads, int dim, int share) {
@@ -1151,11 +1233,14 @@ const char* decay_attention_problem(uint64_t batch, uint64_t heads, uint64_t kv_
   return nullptr;
 }
 
-int64_t decay_attention_work_elems(const DecayShape& s) { return states_elems(s); }
+int64_t decay_attention_work_elems(const DecayShape& s) { return states_elems(s, forward_split(s)); }
 
+// Floats of a gradient of each query head's own, where they share key heads.
+static int64_t by_head_elems(const DecayShape& s, int dim) {
+  return s.heads == s.kv_heads ? 0 : ceil_div((int64_t)s.batch * s.heads * s.seq * dim, 4) * 4;
+}
 int64_t decay_attention_backward_work_elems(const DecayShape& s) {
-  const int64_t shared = s.heads == s.kv_heads ? 0 : (int64_t)s.batch * s.heads * s.seq * std::max(s.key_dim, s.value_dim);
-  return states_elems(s) + shared;
+  return 2 * states_elems(s, backward_split(s)) + by_head_elems(s, s.key_dim) + by_head_elems(s, s.value_dim);
 }
 
 void launch_decay_attention(const DecayShape& s, const DecayInputs& in, float* out, float* new_state, float* work,
@@ -1170,7 +1255,8 @@ void launch_decay_attention(const DecayShape& s, const DecayInputs& in, float* o
   c.out = rows_of(s, out, s.heads, s.value_dim, 1);
   c.from = {const_cast<float*>(in.state), s.value_dim, 1};
   c.to = {new_state, s.value_dim, 1};
-  run_scan(c, work, err, st);
+  const ScanCall call{c, {work, s.value_dim, 1}, true};
+  run_scans(&call, 1, forward_split(s), err, st);
 }
 
 void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in, const float* dout,
@@ -1180,7 +1266,9 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   const int share = s.heads / s.kv_heads;
   const Rows q = rows_of(s, in.q, s.heads, s.key_dim, 1), k = rows_of(s, in.k, s.kv_heads, s.key_dim, share);
   const Rows v = rows_of(s, in.v, s.kv_heads, s.value_dim, share), g = rows_of(s, dout, s.heads, s.value_dim, 1);
-  float *states = work, *by_head = work + states_elems(s);
+  const Split split = backward_split(s);
+  const int64_t states = states_elems(s, split);
+  float* by_head = work + 2 * states;
   Scan c = scan_of(s, in);
   c.rows = s.value_dim;
   c.cols = s.key_dim;
@@ -1190,29 +1278,26 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.out = rows_of(s, dq, s.heads, s.key_dim, 1);
   c.from = {const_cast<float*>(in.state), 1, s.value_dim};
   c.accumulate = accumulate_q;
-  run_scan(c, states, err, st);
+  ScanCall calls[3];
+  calls[0] = {c, {work, s.key_dim, 1}, true};
 
-  // The states of the scans back are the gradients' over `scale`.  The second scan's is the
+  // The states of the scans back are the gradients' over `scale`.  The second one's is the
   // first's transposed: its segments start from the first's states.
   c.back = 1;
   c.from_factor = 1.0f / s.scale;
   c.to_factor = s.scale;
-  auto keys = [&](float* grad, int dim, int accumulate, bool turned_states) {
+  HeadSums sums;
+  auto keys_out = [&](int i, float* grad, int dim, int accumulate) {
     const Rows to = rows_of(s, grad, s.kv_heads, dim, 1);
     if (share == 1) {
       c.out = to;
       c.accumulate = accumulate;
-      run_scan(c, states, err, st, turned_states);
       return;
     }
-    c.out = {by_head, (int64_t)s.heads * s.seq * dim, (int64_t)s.seq * dim, dim, 1};
+    float* part = by_head + (i ? by_head_elems(s, s.value_dim) : 0);
+    c.out = {part, (int64_t)s.heads * s.seq * dim, (int64_t)s.seq * dim, dim, 1};
     c.accumulate = 0;
-    run_scan(c, states, err, st, turned_states);
-    const int64_t n = (int64_t)s.batch * s.kv_heads * s.seq * dim;
-    if (n <= 0) return;
-    sum_heads_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(by_head, to, s.batch, s.kv_heads, share, s.seq, dim,
-                                                                 accumulate);
-    check_launch();
+    sums.of[i] = {part, to, dim, accumulate};
   };
   c.rows = s.key_dim;
   c.cols = s.value_dim;
@@ -1222,7 +1307,8 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.from = {const_cast<float*>(dnew_state), s.value_dim, 1};
   c.to = {dstate, s.value_dim, 1};
   c.accumulate_state = accumulate_state;
-  keys(dv, s.value_dim, accumulate_v, false);
+  keys_out(0, dv, s.value_dim, accumulate_v);
+  calls[1] = {c, {work + states, s.value_dim, 1}, true};
   c.rows = s.value_dim;
   c.cols = s.key_dim;
   c.q = v;
@@ -1230,7 +1316,14 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   c.v = q;
   c.from = {const_cast<float*>(dnew_state), 1, s.value_dim};
   c.to = {};
-  keys(dk, s.key_dim, accumulate_k, true);
+  keys_out(1, dk, s.key_dim, accumulate_k);
+  calls[2] = {c, {work + states, 1, s.value_dim}, false};
+  run_scans(calls, 3, split, err, st);
+
+  const int64_t n = (int64_t)s.batch * s.kv_heads * s.seq * std::max(s.key_dim, s.value_dim);
+  if (share == 1 || n <= 0) return;
+  sum_heads_kernel<<<dim3((unsigned)ceil_div(n, 256), 2), 256, 0, st>>>(sums, s.batch, s.kv_heads, share, s.seq);
+  check_launch();
 }
 
 }  // namespace tysor
