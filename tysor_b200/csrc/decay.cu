@@ -1053,19 +1053,31 @@ struct HeadSum {
 struct HeadSums {
   HeadSum of[2];
 };
-__global__ void __launch_bounds__(256) sum_heads_kernel(const __grid_constant__ HeadSums sums, int batch, int kv_heads,
+template <int V, typename Index>
+__global__ void __launch_bounds__(256) sum_heads_kernel(const __grid_constant__ HeadSums sums, Index rows, int kv_heads,
                                                         int group, int seq) {
   const HeadSum& s = sums.of[blockIdx.y];
-  const Rows& dst = s.dst;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)batch * kv_heads * seq * s.dim;
-  if (i >= n) return;
-  const int64_t row = i / s.dim, c = i - row * s.dim;
-  const int64_t bg = row / seq, t = row - bg * seq;
-  const float* from = s.src + (bg * group * seq + t) * s.dim + c;
-  float sum = 0.0f;
-  for (int k = 0; k < group; ++k) sum += from[(int64_t)k * seq * s.dim];
-  float* to = const_cast<float*>(dst.p) + bg / kv_heads * dst.batch + bg % kv_heads * dst.head + t * dst.token + c;
-  *to = s.accumulate ? *to + sum : sum;
+  const Index i = (Index)blockIdx.x * 256 + threadIdx.x, per = s.dim / V;
+  if (i >= rows * per) return;
+  const Index row = i / per, bg = row / seq, b = bg / kv_heads;
+  const int c = (int)(i - row * per) * V;
+  const int64_t t = row - bg * seq, pitch = (int64_t)seq * s.dim;
+  const float* from = s.src + (int64_t)bg * group * pitch + t * s.dim + c;
+  float* to = const_cast<float*>(s.dst.p) + b * s.dst.batch + (bg - b * kv_heads) * s.dst.head + t * s.dst.token + c;
+  float sum[V] = {};
+  auto add = [&](const float* p) {
+    if constexpr (V == 4) {
+      const float4 w = *(const float4*)p;
+      sum[0] += w.x, sum[1] += w.y, sum[2] += w.z, sum[3] += w.w;
+    } else {
+      sum[0] += *p;
+    }
+  };
+#pragma unroll 4
+  for (int k = 0; k < group; ++k) add(from + k * pitch);
+  if (s.accumulate) add(to);
+  if constexpr (V == 4) *(float4*)to = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  else *to = sum[0];
 }
 
 // From how many tokens on 64 at a time are faster than one by one.
@@ -1320,9 +1332,16 @@ void launch_decay_attention_backward(const DecayShape& s, const DecayInputs& in,
   calls[2] = {c, {work + states, 1, s.value_dim}, false};
   run_scans(calls, 3, split, err, st);
 
-  const int64_t n = (int64_t)s.batch * s.kv_heads * s.seq * std::max(s.key_dim, s.value_dim);
-  if (share == 1 || n <= 0) return;
-  sum_heads_kernel<<<dim3((unsigned)ceil_div(n, 256), 2), 256, 0, st>>>(sums, s.batch, s.kv_heads, share, s.seq);
+  const int64_t rows = (int64_t)s.batch * s.kv_heads * s.seq;
+  if (share == 1 || rows <= 0) return;
+  const bool vec = whole_pieces(sums.of[0].dst, s.value_dim) && whole_pieces(sums.of[1].dst, s.key_dim) &&
+                   whole_pieces({by_head, 0, 0, 0, 1}, 4);
+  const int64_t n = rows * std::max(s.key_dim, s.value_dim) / (vec ? 4 : 1);
+  auto go = [&](auto kernel, auto count) {
+    kernel<<<dim3((unsigned)ceil_div(n, 256), 2), 256, 0, st>>>(sums, count, s.kv_heads, share, s.seq);
+  };
+  if (n < INT64_C(4000000000)) vec ? go(sum_heads_kernel<4, uint32_t>, (uint32_t)rows) : go(sum_heads_kernel<1, uint32_t>, (uint32_t)rows);
+  else vec ? go(sum_heads_kernel<4, int64_t>, rows) : go(sum_heads_kernel<1, int64_t>, rows);
   check_launch();
 }
 
