@@ -323,6 +323,7 @@ struct Split {
   int segments, pieces;
   int slots;  // a head's states: (segments - 1) * pieces + 1
 };
+constexpr int kMostSlots = 64;
 // Scans of one launch: all of as many sequences and heads, and of one kind.
 constexpr int kMostScans = 3;
 struct Scans {
@@ -1016,15 +1017,21 @@ __global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant_
   const Scan& s = all.scan[blockIdx.z];
   const int unit = blockIdx.y, b = unit / s.heads, h = unit - b * s.heads;
   const int i = blockIdx.x * 256 + threadIdx.x, elems = s.rows * s.cols;
-  if (i >= elems) return;
   const int n = tokens_of(s, b, err), runs = all.split.slots - 1;
-  const float decay = decay_of(s, h, err);
+  // What a piece leaves of the state before it, as a sum of two.
+  __shared__ float2 fade[kMostSlots];
+  if (threadIdx.x < runs) {
+    const int part = threadIdx.x / all.split.pieces;
+    int t0, t1;
+    segment_of(n, all.split, part, threadIdx.x - part * all.split.pieces, &t0, &t1);
+    fade[threadIdx.x] = decay_over(decay_of(s, h, err), t1 - t0);
+  }
+  __syncthreads();
+  if (i >= elems) return;
   const int r = i / s.cols, c = i - r * s.cols;
   float x = s.from.p != nullptr ? s.from.p[(int64_t)unit * elems + r * s.from.si + c * s.from.sj] * s.from_factor : 0.0f;
   float* at = all.parts[blockIdx.z].states + (int64_t)unit * all.split.slots * elems + i;
   *at = x;
-  float2 a = make_float2(1.0f, 0.0f);
-  int held = 0;
   constexpr int kAhead = 8;
   for (int j0 = 0; j0 < runs; j0 += kAhead) {
     float own[kAhead];
@@ -1033,10 +1040,7 @@ __global__ void __launch_bounds__(256) scan_states_kernel(const __grid_constant_
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       if (j0 + k >= runs) break;
-      const int part = (j0 + k) / all.split.pieces;
-      int t0, t1;
-      segment_of(n, all.split, part, j0 + k - part * all.split.pieces, &t0, &t1);
-      if (t1 - t0 != held) a = decay_over(decay, t1 - t0), held = t1 - t0;
+      const float2 a = fade[j0 + k];
       x = fmaf(x, a.x, fmaf(x, a.y, own[k]));
       at += elems;
       *at = x;
@@ -1090,9 +1094,9 @@ Split split_of(int64_t units, int seq, int scans, int states) {
   double best = (double)ceil_div(scans * units, 148) * (steps + 2.0);
   Split split{1, 1, 1};
   if (units > 1024) return split;
-  for (int64_t n = 2; n <= std::min<int64_t>(steps, 64); ++n) {
+  for (int64_t n = 2; n <= std::min<int64_t>(steps, kMostSlots); ++n) {
     const int64_t per = ceil_div(steps, n);
-    for (int64_t p = 1; p <= std::min<int64_t>(per, 64 / n); ++p) {
+    for (int64_t p = 1; p <= std::min<int64_t>(per, kMostSlots / n); ++p) {
       const double cost = (double)ceil_div(scans * units * n, 148) * (per + 2.0) +
                           (double)ceil_div(states * units * (n - 1) * p, 148) * (0.5 * ceil_div(per, p) + 2.0) + 3.0;
       if (cost < best) best = cost, split = {(int)n, (int)p, (int)((n - 1) * p + 1)};
