@@ -197,7 +197,8 @@ def test_decay_attention(lib, batch, heads, kv, seq, dk, dv, state, seq_major):
 
 
 @pytest.mark.parametrize("batch,heads,kv,seq,dk,dv", [(4, 2, 1, 1, 64, 64), (4, 3, 3, 70, 80, 48), (5, 4, 2, 300, 64, 128),
-                                                      (5, 2, 2, 129, 33, 20)])
+                                                      (5, 2, 2, 129, 33, 20), (5, 3, 3, 2300, 48, 64),
+                                                      (4, 6, 2, 1500, 80, 40)])
 @pytest.mark.parametrize("seq_major", [False, True])
 def test_decay_attention_of_padded_batches(lib, batch, heads, kv, seq, dk, dv, seq_major):
     rng = np.random.default_rng(seq)
@@ -252,6 +253,31 @@ def test_decay_attention_in_parts_is_the_whole(lib, parts):
         at += n
     close(np.concatenate(outs, 1), want["out"], "out")
     close(state.read(), want["new_state"], "state")
+
+
+@pytest.mark.parametrize("apart", [("q",), ("dout",), ("v", "dq"), ("dk", "dv"), ("q", "k", "v", "dout", "dq", "dk", "dv")])
+@pytest.mark.parametrize("seq", [9, 70, 1700])
+def test_decay_attention_of_rows_off_16_byte_boundaries(lib, seq, apart):
+    # Of the gradients' three scans some then take whole pieces and some do not.
+    rng = np.random.default_rng(seq)
+    t = decay_data(rng, 1, 4, 2, seq, 64, 72, False, True)
+    want = R.decay_attention(t["q"], t["k"], t["v"], t["decay"], t["state"], None, 0.125, False, t["dout"], t["dnew"])
+
+    def place(name, a):
+        if name not in apart:
+            return lib.put(a)
+        base = lib.put(np.concatenate([np.zeros(1, np.float32), a.reshape(-1)]))
+        place.held.append(base)
+        return lib.Buffer(lib.ctx, lib.lib.tysor_cuda_buffer_view(base.handle, 1, a.size), a.size)
+
+    place.held = []
+    buf = {n: place(n, t[n]) for n in ("q", "k", "v", "decay", "state", "dout")}
+    grads = {n: place(n, np.full(t[n[1:]].shape, 7.0, np.float32)) for n in ("dq", "dk", "dv")}
+    grads["dstate"] = lib.zeros(t["state"].size)
+    lib.ok("decay_attention_backward", buf["q"], buf["k"], buf["v"], buf["decay"], buf["state"], None, buf["dout"],
+           lib.put(t["dnew"]), *grads.values(), 1, 4, 2, seq, 64, 72, 0.125, False, False)
+    for n in grads:
+        close(grads[n].read(), want[n], n)
 
 
 @pytest.mark.parametrize("seq", [20, 700, 3000])

@@ -114,7 +114,12 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) { return __ffma2_rn
 
 // A block holds `kSlice` columns of one head's state, four columns and every 16th
 // row a thread, and takes the tokens one after the other.  For few tokens what
-// counts is reading and writing the state.
+// counts is reading and writing the state: one token of 32 sequences of 16 heads of 128, 67 MB,
+// 18 us out of HBM = 3.8 TB/s, 13 us where the state is still in L2; 16 states take 9 us, a
+// launch and the way to memory and back.  The blocks' number counts: 256 threads with 64
+// bytes of state each, four blocks an SM, took 22 us, and the first token's loads
+// before the state is waited for need registers that the threads do not have (15 us in place
+// of 13).  Every further token is 2.3 us, for its sums over the threads.
 constexpr int kMostDim = 128;
 constexpr int kStepThreads = 128, kSlice = 32, kStage = 8;
 constexpr int kStepRows = kStepThreads / 8, kStepMine = kMostDim / kStepRows;  // rows at a time, and of a thread
@@ -246,10 +251,23 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // memory, written there by the threads that hold them.
 //
 // A block takes one head's tokens (or a segment of them) step by step: a loading warp
-// brings the next step's rows into shared memory, sixteen warps split them, form P and
+// brings the next step's rows into shared memory (by tensor maps; rows that are no whole
+// 16-byte pieces by three warps, 4 bytes at a time), sixteen warps split them, form P and
 // keep X, an issuing warp feeds the matrix unit.  Values that fp16's range would spoil
 // (2^60 and more, below 2^-80, not finite) send their step through the registers token
 // by token.
+//
+// What bounds it: the sixteen warps' instructions and waits.  A step takes 5.3 us, the
+// tensor pipe is busy for a quarter of them and the schedulers issue in 55%
+// of cycles (20 K warp instructions a step: splitting 256 rows' worth of values
+// in two halves, their factors, and X in and out of tensor memory); between them lie one barrier
+// and four waits a step, and tensor memory's 512 columns and 226 KB of shared memory leave
+// room for one block an SM.  8 x 2048 tokens of 16 heads of 128, 128 blocks: 172 us, of
+// which the copies of the rows are worth 33 us when left out, the matrix instructions 24, the outputs 19, X 12.
+// Tried: warps of their own for splitting and for X (182 to 238 us, more instructions and
+// exchanges), the next step's rows split while the matrix unit works (171 to 254, registers),
+// row by row bulk copies (80 cycles each to issue), stores by threads instead of boxes (190).
+// Heads of 64 wide leave half of the unit's 128 rows idle: 130 us.  Rows of 4-byte pieces: 127 wide 300 us.
 constexpr int kStep = 64;
 constexpr int kWorkers = 512, kScanThreads = kWorkers + 128, kLoaders = 3;  // loading warps
 constexpr int kWorkerRegs = 104, kOtherRegs = 64;  // 4 x 104 + 64 = 5 x 96, what a quarter of an SM is launched with
@@ -1084,11 +1102,16 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const __grid_constant__ 
   else *to = sum[0];
 }
 
-// From how many tokens on 64 at a time are faster than one by one.
+// From how many tokens on 64 at a time are faster than one by one (24 tokens: 32 sequences of
+// 16 heads 73 us one by one and 68 by 64, one sequence 19 and 20).
 constexpr int kChunkedFrom = 24;
 
 // How the tokens of each of `units` heads are shared, of `scans` in one launch, of `states` of
-// which a first launch forms states (in about half the time a step).
+// which a first launch forms states.  Times in steps of scan_kernel, 5.3 us: 2 for a block's
+// start and end, half a step for one of the first launch, 1.5 for the join's launch (with 3,
+// 3 ragged sequences of 777 train in 114 us in place of 101).  With one segment a head,
+// training on 8192 tokens of 16 heads takes 1220 us in place of 445; with one piece a segment
+// 500.
 Split split_of(int64_t units, int seq, int scans, int states) {
   const int64_t steps = ceil_div(seq, kStep);
   double best = (double)ceil_div(scans * units, 148) * (steps + 2.0);
@@ -1098,7 +1121,7 @@ Split split_of(int64_t units, int seq, int scans, int states) {
     const int64_t per = ceil_div(steps, n);
     for (int64_t p = 1; p <= std::min<int64_t>(per, kMostSlots / n); ++p) {
       const double cost = (double)ceil_div(scans * units * n, 148) * (per + 2.0) +
-                          (double)ceil_div(states * units * (n - 1) * p, 148) * (0.5 * ceil_div(per, p) + 2.0) + 3.0;
+                          (double)ceil_div(states * units * (n - 1) * p, 148) * (0.5 * ceil_div(per, p) + 2.0) + 1.5;
       if (cost < best) best = cost, split = {(int)n, (int)p, (int)((n - 1) * p + 1)};
     }
   }
