@@ -92,6 +92,22 @@ def test_rotary_turns_back_and_its_gradient_is_a_difference(lib):
     assert abs(step - got) <= 60 * U * np.linalg.norm(dy) * (np.linalg.norm(x) + np.linalg.norm(d)) * 1.25
 
 
+@pytest.mark.parametrize("rotary_dim", [64, 44, 10])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_off_16_byte_boundaries(lib, rotary_dim, interleaved):
+    rng = np.random.default_rng(rotary_dim)
+    x = rng.standard_normal((2, 3, 7, 64)).astype(np.float32)
+    want = R.rotary(x, None, rotary_dim, interleaved, 10000.0, PLAIN, False)
+    for a, b in ((0, 1), (1, 0), (2, 2), (3, 1)):
+        base, out = lib.put(np.concatenate([np.zeros(a, np.float32), x.reshape(-1)])), lib.zeros(b + x.size + 1, 9.0)
+        view = [lib.Buffer(lib.ctx, lib.lib.tysor_cuda_buffer_view(p.handle, o, x.size), x.size)
+                for p, o in ((base, a), (out, b))]
+        lib.ok("rotary", view[0], None, view[1], 2, 3, 7, 64, rotary_dim, interleaved, 10000.0, *PLAIN, False)
+        got = out.read()
+        near(got[b:-1], want, 10 * U, "y", 1.5 * abs(x).max())
+        assert (got[:b] == 9.0).all() and got[-1] == 9.0
+
+
 def test_rotary_refusals(lib):
     x, y = lib.zeros(64), lib.zeros(64)
     pos = lib.zeros(2)
