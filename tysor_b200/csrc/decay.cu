@@ -291,13 +291,13 @@ struct ScanSmem {
   static constexpr int kRawQ = kP + 3 * kBoxBytes;          // fp32 rows of the next step
   static constexpr int kRawK = kRawQ + kStep * DK * 4;
   static constexpr int kRawV = kRawK + kStep * DK * 4;
-  static constexpr int kOut = kRawV + kStep * kMostDim * 4;  // [16 warps][16 tokens][32 columns]
+  static constexpr int kOut = kRawV + kStep * kMostDim * 4;  // a step's outputs, as the tensor holds them
   static constexpr int kMisc = kOut + kStep * kMostDim * 4;
   static constexpr int kBytes = kMisc + 10240;
 };
 
 // Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces, and of
-// 16 rows of 32 columns of the output, if its rows are (`stores`).
+// the output, if its rows are (`stores`).
 struct ScanMaps {
   CUtensorMap q, k, v, out;
   int stores;
@@ -311,18 +311,18 @@ __device__ __forceinline__ void load_rows(uint32_t to, const CUtensorMap* map, i
 }
 
 // A box of shared memory to a head's output, or added to it.
-__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t from, int col, int row, int head, int batch,
-                                          int accumulate) {
+__device__ __forceinline__ void store_rows(const CUtensorMap* map, uint32_t from, int row, int head, int batch,
+                                           int accumulate) {
   if (accumulate)
     asm volatile(
         "cp.reduce.async.bulk.tensor.4d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
             (uint64_t)map),
-        "r"(col), "r"(row), "r"(head), "r"(batch), "r"(from)
+        "r"(0), "r"(row), "r"(head), "r"(batch), "r"(from)
         : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"((uint64_t)map),
-        "r"(col), "r"(row), "r"(head), "r"(batch), "r"(from)
+        "r"(0), "r"(row), "r"(head), "r"(batch), "r"(from)
         : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
@@ -427,14 +427,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* v_mosts = k_downs + 128;             // [2][4][128]
   float* x_most = v_mosts + 1024;             // [4][128]
   uint64_t* bars = (uint64_t*)(x_most + 512);
-  int* far_step = (int*)(bars + 10);  // [2]
+  int* far_step = (int*)(bars + 14);  // [2]
   uint32_t* tmem_slot = (uint32_t*)(far_step + 2);
   const uint32_t base = smem_u32(smem);
   const uint32_t raw_full = smem_u32(bars), raw_empty = raw_full + 8, ready = raw_full + 16, values_ready = raw_full + 24,
                  score_full = raw_full + 32, sums_full = raw_full + 40, p_ready = raw_full + 48,
                  out_full = raw_full + 56, far_seen = raw_full + 64,
                  // Of every second step: with STATE_ONLY the warps may be a step ahead of the issuing one.
-                 ready_odd = raw_full + 72;
+                 ready_odd = raw_full + 72, from_full = raw_full + 80, out_ready = raw_full + 88, out_free = raw_full + 96;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int runs = STATE_ONLY ? (segments - 1) * all.split.pieces : segments;
   const int unit = blockIdx.x / runs, run = blockIdx.x - unit * runs;
@@ -458,6 +458,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     mbar_init(p_ready, kWorkers / 32);
     mbar_init(out_full, 1);
     mbar_init(far_seen, 1);
+    mbar_init(from_full, 1);
+    mbar_init(out_ready, kWorkers / 32);
+    mbar_init(out_free, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     far_step[0] = far_step[1] = 0;
   }
@@ -495,10 +498,29 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       const bool leader = elect_one();
       uint32_t steps = 0;  // those of the matrix unit
       bool ok = true;
+      // The outputs of the step before, which its warps have left in shared memory, go from here:
+      // issuing a copy takes as long as a tenth of what they do in a step.
+      bool storing = false;
+      uint32_t stores = 0;
+      auto store_outputs = [&](int t) {
+        ok = sleep_wait(out_ready, stores++ & 1, err);
+        if (ok && leader)
+          store_rows(&maps.out, base + Sm::kOut, s.back ? n - kStep - t : t, h / s.out.share, b, s.accumulate);
+        __syncwarp();
+      };
       for (int t = t0, c = 0; t < t1 && ok; t += kStep, ++c) {
         const bool second = STATE_ONLY && (c & 1);
-        ok = sleep_wait(c & 1 ? ready_odd : ready, (c >> 1) & 1, err);
+        if (VEC && !STATE_ONLY && storing) store_outputs(t - kStep);
+        if (ok) ok = sleep_wait(c & 1 ? ready_odd : ready, (c >> 1) & 1, err);
         if (!ok) break;
+        if (VEC && !STATE_ONLY && storing) {
+          if (leader) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            mbar_arrive(out_free);
+          }
+          __syncwarp();
+          storing = false;
+        }
         tc_fence_after();
         if (*(volatile int*)&far_step[c & 1]) {
           if (leader) mbar_arrive(far_seen);
@@ -515,16 +537,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
               umma_ss(tmem + Tm::kScore, a, k, kNarrow, pass + i > 0);
             }
           umma_commit(score_full);
-          // X^T q^T: lo.hi, hi.lo, hi.hi.
+        }
+        // X^T q^T: lo.hi, hi.lo, hi.hi; the first half (with narrow keys all) while the values are
+        // split, the second behind the sums, which the warps need earlier.
+        auto from_state = [&](bool first_half) {
 #pragma unroll
           for (int pass = 0; pass < 3; ++pass)
 #pragma unroll
-            for (int i = 0; i < DK / 16; ++i) {
-              const uint32_t x = tmem + (pass == 0 ? Tm::kStateLo : Tm::kState) + i * 8;
-              const uint32_t q = column_word(base + Sm::kQ + ((i / 4) * 2 + (pass == 1)) * kBoxBytes) + (i & 3) * kColumnStep;
-              umma_ts(tmem + Tm::kFrom, x, q, kNarrow, pass + i > 0);
-            }
-        }
+            for (int i = 0; i < DK / 16; ++i)
+              if ((DK == 64 || 2 * (pass * (DK / 16) + i) < 3 * (DK / 16)) == first_half) {
+                const uint32_t x = tmem + (pass == 0 ? Tm::kStateLo : Tm::kState) + i * 8;
+                const uint32_t q = column_word(base + Sm::kQ + ((i / 4) * 2 + (pass == 1)) * kBoxBytes) + (i & 3) * kColumnStep;
+                umma_ts(tmem + Tm::kFrom, x, q, kNarrow, pass + i > 0);
+              }
+        };
+        if (!STATE_ONLY && leader) from_state(true);
         __syncwarp();
         ok = sleep_wait(values_ready, steps & 1, err);
         if (!ok) break;
@@ -541,6 +568,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
               umma_ts(tmem + (second ? Tm::kFrom : Tm::kDelta), w, k, kRows, pass + i > 0);
             }
           umma_commit(sums_full);
+          if (!STATE_ONLY) {
+            from_state(false);
+            umma_commit(from_full);
+          }
         }
         if (!STATE_ONLY) {
           __syncwarp();
@@ -560,8 +591,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
               }
             umma_commit(out_full);
           }
+          storing = VEC && maps.stores && t1 - t >= kStep;
         }
         ++steps;
+        __syncwarp();
+      }
+      if (VEC && !STATE_ONLY) {
+        if (ok && storing) store_outputs(t0 + (t1 - t0 - 1) / kStep * kStep);
+        if (leader) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
       }
     } else if (VEC) {
@@ -674,7 +711,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     const int row_i = col & (kStep - 1);  // of P
     const float2 fade = decay_over(decay, kStep);
     bool ok = true;
-    uint32_t steps = 0, far_steps = 0;
+    uint32_t steps = 0, far_steps = 0, stores = 0;
     float bound = 0.0f;  // at least X^T's greatest magnitude in this column
     bool far_state = false;
     if (t0 < t1) {
@@ -954,6 +991,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       if (!STATE_ONLY) {
         bound = fmaf(bound, a.x, 0x1p36f * w_down) * 1.000001f;
         far_state = biased_of(bound) >= 254;
+        if (ok) ok = sleep_wait(from_full, steps & 1, err);
+        tc_fence_after();
         if (t + kStep < t1) put_state(bound);
         if (ok) ok = sleep_wait(out_full, steps & 1, err);
         tc_fence_after();
@@ -974,20 +1013,18 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           }
         }
         if (VEC && maps.stores && m == kStep) {
-          // Through shared memory, a box a warp: a thread's stores of single values would take the
-          // load and store units longer than the step's loads.
-          float* patch = (float*)(smem + Sm::kOut) + warp * 512 + lane;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
+          // Through shared memory: a thread's stores of single values would take the load and
+          // store units longer than the step's loads.
+          if (ok && stores > 0) ok = sleep_wait(out_free, (stores - 1) & 1, err);
+          ++stores;
+          float* to = (float*)(smem + Sm::kOut) + place(group * 16) * value_pitch + col;
+          const int next_row = turned ? -value_pitch : value_pitch;
+          if (col < s.cols)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) patch[32 * (s.back ? 15 - i : i)] = own[i];
+            for (int i = 0; i < 16; ++i) to[i * next_row] = own[i];
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0 && quarter * 32 < s.cols) {
-            const int first = t + group * 16;
-            store_box(&maps.out, base + Sm::kOut + warp * 2048, quarter * 32, s.back ? n - 16 - first : first,
-                      h / s.out.share, b, s.accumulate);
-          }
+          if (lane == 0) mbar_arrive(out_ready);
         } else {
           const int rows = col < s.cols ? min(m - group * 16, 16) : 0;  // of this thread's
           const int64_t pitch = s.back ? -s.out.token : s.out.token;
@@ -1000,10 +1037,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       ++steps;
     }
     if (STATE_ONLY) flush();
-    if (VEC && !STATE_ONLY) {
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      __syncwarp();
-    }
     // Rows behind the sequence's end, spread over its blocks.
     if (!STATE_ONLY && !s.accumulate)
       for (int r = n + part * 4 + group; r < s.seq; r += 4 * segments)
@@ -1178,7 +1211,7 @@ ScanMaps maps_of(const Scan& s) {
   };
   ScanMaps maps{map(s.q, s.rows, s.rows, kStep), map(s.k, s.rows, s.rows, kStep), map(s.v, s.cols, s.cols, kStep), {},
                 whole_pieces(s.out, s.cols)};
-  if (maps.stores) maps.out = map(s.out, s.cols, 32, 16);
+  if (maps.stores) maps.out = map(s.out, s.cols, s.cols, kStep);
   return maps;
 }
 
