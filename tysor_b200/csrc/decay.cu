@@ -257,17 +257,19 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // (2^60 and more, below 2^-80, not finite) send their step through the registers token
 // by token.
 //
-// What bounds it: the sixteen warps' instructions and waits.  A step takes 5.3 us, the
-// tensor pipe is busy for a quarter of them and the schedulers issue in 55%
-// of cycles (20 K warp instructions a step: splitting 256 rows' worth of values
-// in two halves, their factors, and X in and out of tensor memory); between them lie one barrier
-// and four waits a step, and tensor memory's 512 columns and 226 KB of shared memory leave
-// room for one block an SM.  8 x 2048 tokens of 16 heads of 128, 128 blocks: 172 us, of
-// which the copies of the rows are worth 33 us when left out, the matrix instructions 24, the outputs 19, X 12.
-// Tried: warps of their own for splitting and for X (182 to 238 us, more instructions and
-// exchanges), the next step's rows split while the matrix unit works (171 to 254, registers),
-// row by row bulk copies (80 cycles each to issue), stores by threads instead of boxes (190).
-// Heads of 64 wide leave half of the unit's 128 rows idle: 130 us.  Rows of 4-byte pieces: 127 wide 300 us.
+// What bounds it: the sixteen warps' instructions, one behind the other.  A step takes 4.9 us
+// (some 8900 cycles: 1800 to split the q and k rows, 900 for the values and the barrier, 1400
+// for v and w, 1200 for P, 500 for X, 800 to lay it into tensor memory, the rest for the
+// outputs and waits); the tensor pipe is busy for a quarter of them and the schedulers issue
+// in 55% of cycles (20 K warp instructions a step).  Tensor memory's 512 columns and 226 KB of
+// shared memory leave room for one block an SM.  8 x 2048 tokens of 16 heads of 128, 128
+// blocks: 158 us (outputs stored by the sixteen warps 163, all of X q^T before the sums 170).
+// Tried, each beside what was there then: warps of their own for splitting and for X (182 to
+// 238 us, 166 without: more instructions and exchanges), the next step's rows split while the
+// matrix unit works (171 to 254, registers), row by row bulk copies (80 cycles each to issue),
+// stores of single values (190, 178 with boxes), no work on P's blocks of zeros (171, 169).
+// Heads of 64 wide leave half of the unit's 128 rows idle: 126 us.  Rows of 4-byte pieces:
+// 127 wide 302 us.
 constexpr int kStep = 64;
 constexpr int kWorkers = 512, kScanThreads = kWorkers + 128, kLoaders = 3;  // loading warps
 constexpr int kWorkerRegs = 104, kOtherRegs = 64;  // 4 x 104 + 64 = 5 x 96, what a quarter of an SM is launched with
@@ -1140,7 +1142,7 @@ __global__ void __launch_bounds__(256) sum_heads_kernel(const __grid_constant__ 
 constexpr int kChunkedFrom = 24;
 
 // How the tokens of each of `units` heads are shared, of `scans` in one launch, of `states` of
-// which a first launch forms states.  Times in steps of scan_kernel, 5.3 us: 2 for a block's
+// which a first launch forms states.  Times in steps of scan_kernel, 5 us: 2 for a block's
 // start and end, half a step for one of the first launch, 1.5 for the join's launch (with 3,
 // 3 ragged sequences of 777 train in 114 us in place of 101).  With one segment a head,
 // training on 8192 tokens of 16 heads takes 1220 us in place of 445; with one piece a segment
