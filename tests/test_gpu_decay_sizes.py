@@ -1,0 +1,80 @@
+"""decay_attention where tokens' rows differ in size, value by value against its formulas in 64 bits
+(linear_reference.py): what a token sees, not what else its 64 tokens or its head's other columns hold,
+says how far a result may be off.
+
+Tolerance, fixed from the arithmetic, relative to the same sums over absolute values (u = 2^-24): three
+operands of two halves (4u each), 68 instructions that may each lose a step (2u) of what they have added,
+a fade of e^-x whose exponent is rounded (xu, x below 88, where fp32 ends), two roundings a step of the state
+(8 steps at most); or one by one two roundings a token and sum, of which 64 in a row have one sign once
+in 2^64.  Together below 256u.  Where one by one the tokens are up to 1100 more than 64 follow one another
+at random: 256u still holds eight times their root."""
+import numpy as np
+import pytest
+
+import linear_reference as R
+from test_gpu_linear_ops import decay_data, decay_run
+from test_gpu_lm_ops import Lib, U
+
+pytestmark = pytest.mark.gpu
+
+BAR = 256 * U
+RATES = np.array([0.0, 0.01, 0.3, 2.0], np.float32)
+
+
+@pytest.fixture
+def lib(cuda_ctx):
+    return Lib(cuda_ctx)
+
+
+def wanted(t, scale, seq_major):
+    """The results, and the same sums over absolute values."""
+    def of(t):
+        return R.decay_attention(t["q"], t["k"], t["v"], t["decay"], t["state"], None, scale, seq_major, t["dout"], t["dnew"])
+
+    return of(t), of({n: a if a is None else abs(a) for n, a in t.items()})
+
+
+def within(got, want, size, name):
+    off = abs(got.reshape(want.shape).astype(np.float64) - want)
+    bad = ~(off <= BAR * size + 2.0 ** -120)
+    assert not bad.any(), f"{name}: {(off / (size + 1e-300)).max() / U:.0f}u, {bad.sum()} values, first {np.argwhere(bad)[0]}"
+
+
+# ---- the state -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 80), (33, 20)])
+@pytest.mark.parametrize("power", [10, 20, 30, 40, 50])
+@pytest.mark.parametrize("where", [5, 63, 90])
+def test_a_large_key_beside_small_values_leaves_their_columns_as_they_are(lib, dk, dv, power, where):
+    # The key's size reaches the state only by what it is multiplied with.  `batch` 40 leaves a head's
+    # tokens to one block; 1 shares them out.
+    for batch in (1, 40):
+        rng = np.random.default_rng(power + where)
+        t = decay_data(rng, batch, 4, 4, 200, dk, dv, False, True)
+        t["decay"] = RATES
+        t["k"][:, :, where] *= np.float32(2.0 ** power)
+        t["v"][:, :, where, 1::3] = 0
+        t["v"][:, :, where, 2::3] *= np.float32(2.0 ** -power)
+        got = decay_run(lib, t, 0.125, False, need=())
+        t["dout"], t["dnew"] = None, None
+        want = R.decay_attention(t["q"], t["k"], t["v"], RATES, t["state"], None, 0.125, False)
+        size = R.decay_attention(abs(t["q"]), abs(t["k"]), abs(t["v"]), RATES, abs(t["state"]), None, 0.125, False)
+        within(got["new_state"], want["new_state"], size["new_state"], (batch, "new_state"))
+        later = (where // 64 + 1) * 64
+        within(got["out"].reshape(want["out"].shape)[:, :, later:], want["out"][:, :, later:], size["out"][:, :, later:],
+               (batch, "out"))
+
+
+def test_a_state_that_a_large_token_has_left_again(lib):
+    # 18 steps in one block: the token fades and what is left has its own size again.
+    rng = np.random.default_rng(2)
+    t = decay_data(rng, 8, 20, 20, 1100, 16, 16, True, True)
+    t["decay"] = np.resize(np.array([0.0, 0.02, 0.05, 0.2], np.float32), 20)
+    t["k"][:, 70] *= np.float32(2.0 ** 40)
+    t["v"][:, 70] *= np.float32(2.0 ** -20)
+    got = decay_run(lib, t, 0.25, True, need=())
+    want = R.decay_attention(t["q"], t["k"], t["v"], t["decay"], t["state"], None, 0.25, True)
+    size = R.decay_attention(abs(t["q"]), abs(t["k"]), abs(t["v"]), t["decay"], abs(t["state"]), None, 0.25, True)
+    within(got["new_state"], want["new_state"], size["new_state"], "new_state")
+    within(got["out"].reshape(want["out"].shape)[:, 128:], want["out"][:, 128:], size["out"][:, 128:], "out")

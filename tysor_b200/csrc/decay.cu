@@ -244,8 +244,10 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // fp32 accuracy out of fp16 matrix instructions, as in the attention kernels: an
 // operand is scaled by a power of two and split into hi = fp16(x) and lo =
 // fp16(x - hi), and a product is hi.hi + lo.hi + hi.lo.  Each q and k row (token) has
-// its own power of two, each value column one per 64 tokens, each column of X one per
-// step.  The matrix unit adds with truncation, so a step's sums leave it and X is kept
+// its own power of two, each value column one per 64 tokens, and so has each column of w, from
+// its own greatest value, and of X, from a bound of what w's have added to it (one power for all of
+// w, of the greatest key times the column's greatest value, lost the columns in which a large key
+// meets a small value).  The matrix unit adds with truncation, so a step's sums leave it and X is kept
 // in fp32 registers.  Products are formed transposed (values' columns in the unit's
 // 128 rows), so that X^T, v^T and w^T = (a^(63 - j + tail) v_j)^T are operands in tensor
 // memory, written there by the threads that hold them.
@@ -378,6 +380,10 @@ __device__ __forceinline__ uint32_t biased_of(float magnitude) { return __float_
 __device__ __forceinline__ float power_of(uint32_t biased) { return __uint_as_float(biased << 23); }
 // 2^(14 - e) for a greatest magnitude of 2^e to 2^(e+1), and its inverse; for 0, 1.
 __device__ __forceinline__ uint32_t scale_biased(float most) { return most == 0.0f ? 141u : max(biased_of(most), 16u); }
+// The same, of powers below fp32's normal numbers too.
+__device__ __forceinline__ float small_power_of(int biased) {
+  return biased > 0 ? power_of(biased) : power_of(max(biased + 64, 0)) * 0x1p-64f;
+}
 // Whether a tile of this greatest magnitude (0 apart) goes token by token; NaN does.
 __device__ __forceinline__ bool far_biased(uint32_t biased) { return biased - kLeastBiased >= kFarRange; }
 
@@ -429,11 +435,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   // (As an offset: the compiler then knows what is derived from it for shared memory.)
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
-  float* lefts = since + 64;                  // [2][64] a^(63 - j + tail), and the same of a last, shorter step
+  float* lefts = since + 64;                  // [2][64] 2^20 a^(63 - j + tail), and the same of a last, shorter step
   float* nears = lefts + 128;                 // [128] a^(d - 63), 0 below
   float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors (q's times scale), steps in turn
   float* k_downs = q_downs + 128;             // [2][64]
-  float* v_mosts = k_downs + 128;             // [2][4][128]
+  float* v_mosts = k_downs + 128;             // [4][128] pairs
   float* x_most = v_mosts + 1024;             // [4][128]
   uint64_t* bars = (uint64_t*)(x_most + 512);
   int* far_step = (int*)(bars + 14);  // [2]
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   if (tid < 64) since[tid] = power(tid + lead);
   if (tid >= 64 && tid < 192) {
     const int j = tid & 63, m = tid < 128 ? kStep : (t1 - t0) % kStep;
-    lefts[tid - 64] = j < m ? power(m - 1 - j + tail) : 0.0f;
+    lefts[tid - 64] = j < m ? power(m - 1 - j + tail) * 0x1p20f : 0.0f;
   }
   if (tid >= 192 && tid < 320) nears[tid - 192] = tid - 192 < 63 ? 0.0f : power(tid - 192 - 63);
   if (warp == kWorkers / 32) {
@@ -767,7 +773,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
       const int m = min(kStep, t1 - t);
       const int turn = c & 1;
-      float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn, *v_most = v_mosts + 512 * turn;
+      float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn;
       if (ok) ok = sleep_wait(raw_full, turn, err);
       if (m < kStep) {  // zeros behind the sequence's end
         const int first = turned ? 0 : m;
@@ -841,19 +847,18 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       }
       // This column's values of 16 tokens.
       Pair val[8];
+      float val_most = 0.0f;
       {
         // (Threads behind the last column read the first; nothing takes what they hold.)
         const float* raw = (const float*)(smem + Sm::kRawV) + place(group * 16) * value_pitch + (VEC && col >= s.cols ? 0 : col);
         const int next_row = turned ? -value_pitch : value_pitch;
-        float most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float a = raw[2 * i * next_row], d = raw[(2 * i + 1) * next_row];
           val[i] = pair_of(a, d);
-          most = most_of(most, a, d);
+          val_most = most_of(val_most, a, d);
         }
-        far |= far_biased(scale_biased(most));
-        v_most[group * 128 + col] = most;
+        far |= far_biased(scale_biased(val_most));
       }
       if (far) far_step[turn] = 1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -887,7 +892,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             if (!lead) x[j] = fma2(x[j], hi, mul2(x[j], lo));
           }
           if (!STATE_ONLY) {
-            float* sums = i & 1 ? v_most : x_most;
+            float* sums = i & 1 ? v_mosts : x_most;
             sums[group * 128 + col] = sum.x + sum.y;
             worker_sync();
             if (group == 0 && col < s.cols) {
@@ -910,46 +915,55 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         continue;
       }
       if (tid == 0 && t + kStep < t1) mbar_arrive(raw_empty);
-      // (Before this step's values are ready: its own sums would end another phase of the barrier.)
-      if (STATE_ONLY) flush();
-      // The keys' factors over the greatest (P), and with a^(63 - j + tail) over the greatest of those (w).
+      // v, and w = v_j a^(63 - j + tail) times the key's factor, each column with powers of two of its own: what a
+      // large key is not multiplied with does not feel it.  (2^20 w is at most 2^126, and below 2^-126 only
+      // where the product of key and value is.)
       float p_down, p_inv, w_down;
       {
         const float* left = lefts + (m < kStep ? kStep : 0);
-        const float k0 = k_down[lane], k1 = k_down[lane + 32];
-        p_down = warp_most(fmaxf(k0, k1));
-        const float most_w = warp_most(fmaxf(k0 * left[lane], k1 * left[lane + 32]));
-        p_inv = power_of(254u - biased_of(p_down)) * 0x1p-22f;
-        // Below fp32's normal numbers there is nothing to add.
-        const uint32_t e = most_w >= 0x1p-126f ? min(biased_of(most_w) + 1, 253u) : 0;
-        w_down = power_of(e);
-        const uint32_t biased = scale_biased(
-            most_of(most_of(v_most[col], v_most[128 + col], v_most[256 + col]), v_most[384 + col], 0.0f));
-        const float up = power_of(268u - biased), down = power_of(biased - 14u);
-        const float inv_w = e ? power_of(254u - e) : 0.0f;
+        Pair w[8];
+        float w_most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float4 l = *(const float4*)(left + group * 16 + 2 * i), f = *(const float4*)(k_down + group * 16 + 2 * i);
+          w[i] = mul2(val[i], mul2(pair_of(f.x, f.y), pair_of(l.x, l.y)));
+          w[i + 1] = mul2(val[i + 1], mul2(pair_of(f.z, f.w), pair_of(l.z, l.w)));
+          w_most = most_of(most_of(w_most, w[i].x, w[i].y), w[i + 1].x, w[i + 1].y);
+        }
+        // Over the four threads that hold the column.
+        float2* mosts = (float2*)v_mosts + col;
+        mosts[group * 128] = make_float2(val_most, w_most);
+        // The keys' factors are taken over the greatest in P.
+        const float k_most = STATE_ONLY ? 0.0f : warp_most(fmaxf(k_down[lane], k_down[lane + 32]));
+        p_inv = power_of(254u - biased_of(k_most)) * 0x1p-22f;
+        // (Before this step's values are ready: its own sums would end another phase of the barrier.)
+        if (STATE_ONLY) flush();
+        asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
+        {
+          const float2 m0 = mosts[0], m1 = mosts[128], m2 = mosts[256], m3 = mosts[384];
+          val_most = most_of(most_of(m0.x, m1.x, m2.x), m3.x, 0.0f);
+          w_most = most_of(most_of(m0.y, m1.y, m2.y), m3.y, 0.0f);
+        }
         uint32_t hi[8], lo[8];
-        const Pair up2 = pair_of(up, up), inv2 = pair_of(inv_w, inv_w);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) val[i] = mul2(val[i], up2);
         if (!STATE_ONLY) {
+          const uint32_t biased = scale_biased(val_most);
+          const float up = power_of(268u - biased);
+          const Pair up2 = pair_of(up, up);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) split_pair(val[i], hi[i], lo[i]);
+          for (int i = 0; i < 8; ++i) split_pair(mul2(val[i], up2), hi[i], lo[i]);
           tmem_st8(at_lane + Tm::kV + group * 8, hi);
           tmem_st8(at_lane + Tm::kV + 32 + group * 8, lo);
+          p_down = k_most * power_of(biased - 14u) * 0x1p22f;
         }
+        const uint32_t biased = scale_biased(w_most);
+        const float up = power_of(268u - biased);
+        w_down = w_most > 0.0f ? small_power_of((int)biased - (14 + 20)) : 0.0f;
+        const Pair up2 = pair_of(up, up);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 l = *(const float4*)(left + group * 16 + 4 * i), f = *(const float4*)(k_down + group * 16 + 4 * i);
-          const Pair w0 = mul2(mul2(pair_of(f.x, f.y), pair_of(l.x, l.y)), inv2);
-          const Pair w1 = mul2(mul2(pair_of(f.z, f.w), pair_of(l.z, l.w)), inv2);
-          split_pair(mul2(val[2 * i], w0), hi[2 * i], lo[2 * i]);
-          split_pair(mul2(val[2 * i + 1], w1), hi[2 * i + 1], lo[2 * i + 1]);
-        }
+        for (int i = 0; i < 8; ++i) split_pair(mul2(w[i], up2), hi[i], lo[i]);
         const uint32_t at_w = at_lane + (STATE_ONLY && turn ? Tm::kV : Tm::kW) + group * 8;
         tmem_st8(at_w, hi);
         tmem_st8(at_w + 32, lo);
-        p_down *= down * 0x1p22f;
-        w_down *= down;
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
@@ -1007,6 +1021,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       add_sums(Tm::kDelta, m, w_down);
       if (!STATE_ONLY) {
         bound = fmaf(bound, a.x, 0x1p36f * w_down) * 1.000001f;
+        // (It grows by what the sums may be, not by what they are.)
+        if ((c & 15) == 15) bound = most_of_state();
         far_state = biased_of(bound) >= 254;
         if (ok) ok = sleep_wait(from_full, steps & 1, err);
         tc_fence_after();
