@@ -78,3 +78,67 @@ def test_a_state_that_a_large_token_has_left_again(lib):
     size = R.decay_attention(abs(t["q"]), abs(t["k"]), abs(t["v"]), t["decay"], abs(t["state"]), None, 0.25, True)
     within(got["new_state"], want["new_state"], size["new_state"], "new_state")
     within(got["out"].reshape(want["out"].shape)[:, 128:], want["out"][:, 128:], size["out"][:, 128:], "out")
+
+
+# ---- what the tokens of 64 hold, beside one another -----------------------------------
+
+# Whose row stands in the key's place of the products that give a result, and whose in the value's.
+KEYS = {"out": "k", "dq": "v", "dv": "q", "dk": "dout"}
+
+
+def sized_run(lib, t, names):
+    want, size = wanted(t, 0.125, False)
+    got = decay_run(lib, t, 0.125, False)
+    for n in names:
+        within(got[n], want[n], size[n], n)
+
+
+def sized_data(seed, seq, dk, dv, batch=1):
+    t = decay_data(np.random.default_rng(seed), batch, 4, 2, seq, dk, dv, False, True)
+    t["decay"] = RATES
+    t["dout"] *= 1000
+    t["dnew"] *= 1000
+    return t
+
+
+@pytest.mark.parametrize("result", list(KEYS))
+@pytest.mark.parametrize("seq,where", [(23, 11), (24, 11), (64, 0), (64, 63), (200, 40), (200, 100), (700, 300)])
+@pytest.mark.parametrize("power", [10, 16, 24, 32, 40, 50, -20, -50])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 80)])
+def test_a_large_or_small_key_leaves_other_tokens_as_they_are(lib, result, seq, where, power, dk, dv):
+    t = sized_data(seq + power + 50, seq, dk, dv)
+    t[KEYS[result]][:, :, where] *= np.float32(2.0 ** power)
+    sized_run(lib, t, [result])
+
+
+@pytest.mark.parametrize("seq", [100, 700])
+@pytest.mark.parametrize("spread", [8, 20, 40, 70])
+def test_keys_of_all_sizes(lib, seq, spread):
+    for result, key in KEYS.items():
+        t = sized_data(spread, seq, 80, 64)
+        size = np.random.default_rng(seq).integers(-spread // 2, spread // 2 + 1, t[key].shape[:3] + (1,))
+        t[key] *= (2.0 ** size).astype(np.float32)
+        sized_run(lib, t, [result])
+
+
+@pytest.mark.parametrize("result", list(KEYS))
+def test_keys_that_have_faded(lib, result):
+    # Behind rows of zeros a token sees only what has faded: 40 tokens at e^-1.5 are 2^-86.
+    t = sized_data(4, 200, 64, 64)
+    t["decay"] = np.array([0.01, 0.3, 1.0, 1.5], np.float32)
+    t["state"] = t["dnew"] = None
+    t[KEYS[result]][:, :, 10:50] = 0
+    t[KEYS[result]][:, :, 70:120] = 0
+    sized_run(lib, t, [result])
+
+
+@pytest.mark.parametrize("seq", [64, 200])
+@pytest.mark.parametrize("power", [12, 20, 40, 55])
+def test_a_large_key_beside_small_values_within_its_64_tokens(lib, seq, power):
+    for result, value in (("out", "v"), ("dq", "k"), ("dv", "dout"), ("dk", "q")):
+        t = sized_data(power, seq, 64, 64)
+        for where in (9, 30):
+            t[KEYS[result]][:, :, where] *= np.float32(2.0 ** power)
+            t[value][:, :, where, where % 3::3] = 0
+            t[value][:, :, where, where % 3 + 1::3] *= np.float32(2.0 ** -power)
+        sized_run(lib, t, [result])

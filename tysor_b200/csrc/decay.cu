@@ -244,8 +244,8 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // fp32 accuracy out of fp16 matrix instructions, as in the attention kernels: an
 // operand is scaled by a power of two and split into hi = fp16(x) and lo =
 // fp16(x - hi), and a product is hi.hi + lo.hi + hi.lo.  Each q and k row (token) has
-// its own power of two, each value column one per 64 tokens, and so has each column of w, from
-// its own greatest value, and of X, from a bound of what w's have added to it (one power for all of
+// its own power of two, each row of P one of the keys that it sees, each value column one per 64
+// tokens, and so has each column of w, from its own greatest value, and of X, from a bound of what w's have added to it (one power for all of
 // w, of the greatest key times the column's greatest value, lost the columns in which a large key
 // meets a small value).  The matrix unit adds with truncation, so a step's sums leave it and X is kept
 // in fp32 registers.  Products are formed transposed (values' columns in the unit's
@@ -285,6 +285,9 @@ struct ScanTmem {
                             kV = kScore + 64, kW = kV + 64;  // hi; lo 32 columns behind
 };
 constexpr uint32_t kTmemColumns = 512;
+// How far the keys' factors of a step may lie apart, so that the columns need not be looked at, and so that
+// it does not go token by token.
+constexpr float kApart = 0x1p10f, kFarApart = 0x1p60f;
 
 template <int DK>
 struct ScanSmem {
@@ -384,6 +387,8 @@ __device__ __forceinline__ uint32_t scale_biased(float most) { return most == 0.
 __device__ __forceinline__ float small_power_of(int biased) {
   return biased > 0 ? power_of(biased) : power_of(max(biased + 64, 0)) * 0x1p-64f;
 }
+// 1 / x of a power of two, 0 of 0.
+__device__ __forceinline__ float inverse_of(float x) { return x > 0.0f ? power_of(254u - biased_of(x)) : 0.0f; }
 // Whether a tile of this greatest magnitude (0 apart) goes token by token; NaN does.
 __device__ __forceinline__ bool far_biased(uint32_t biased) { return biased - kLeastBiased >= kFarRange; }
 
@@ -441,9 +446,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* k_downs = q_downs + 128;             // [2][64]
   float* v_mosts = k_downs + 128;             // [4][128] pairs
   float* x_most = v_mosts + 1024;             // [4][128]
-  uint64_t* bars = (uint64_t*)(x_most + 512);
-  int* far_step = (int*)(bars + 14);  // [2]
-  uint32_t* tmem_slot = (uint32_t*)(far_step + 2);
+  float* p_downs = x_most + 512;              // [64] what undoes the factors of P's rows
+  uint64_t* bars = (uint64_t*)(p_downs + 64);
+  int* far_step = (int*)(bars + 14);              // [2]
+  int* uneven = far_step + 2;                     // [2] whether the keys' factors differ from `usual`
+  uint32_t* usual = (uint32_t*)(uneven + 2);      // [2] the exponent of the first key of the step before
+  uint32_t* tmem_slot = usual + 2;
   const uint32_t base = smem_u32(smem);
   const uint32_t raw_full = smem_u32(bars), raw_empty = raw_full + 8, ready = raw_full + 16, values_ready = raw_full + 24,
                  score_full = raw_full + 32, sums_full = raw_full + 40, p_ready = raw_full + 48,
@@ -477,7 +485,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     mbar_init(out_ready, kWorkers / 32);
     mbar_init(out_free, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    far_step[0] = far_step[1] = 0;
+    far_step[0] = far_step[1] = uneven[0] = uneven[1] = 0;
+    usual[0] = 0;
   }
   if (tid < 64) since[tid] = power(tid + lead);
   if (tid >= 64 && tid < 192) {
@@ -774,6 +783,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       const int m = min(kStep, t1 - t);
       const int turn = c & 1;
       float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn;
+      const uint32_t of_usual = STATE_ONLY ? 0 : usual[turn];
       if (ok) ok = sleep_wait(raw_full, turn, err);
       if (m < kStep) {  // zeros behind the sequence's end
         const int first = turned ? 0 : m;
@@ -786,7 +796,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         worker_sync();
       }
       // q and k rows, a warp eight of one of them.
-      bool far = far_state;
+      bool far = far_state, odd = false;
       {
         constexpr int kRowsPer = STATE_ONLY ? 4 : 8;
         const bool is_k = STATE_ONLY || warp >= 8;
@@ -816,6 +826,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         }
         const uint32_t biased = scale_biased(mine);
         far |= far_biased(biased);
+        if (!STATE_ONLY && is_k) {
+          odd = lane < kRowsPer && row0 + lane < m && (mine == 0.0f || biased - of_usual + 2 > 4);
+          if (row0 + lane == 0) usual[turn ^ 1] = biased;
+        }
         // A row of zeros has no part in the greatest factor.
         if (lane < kRowsPer)
           (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u) * (is_k ? 1.0f : s.scale);
@@ -861,15 +875,61 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         far |= far_biased(scale_biased(val_most));
       }
       if (far) far_step[turn] = 1;
+      if (odd) uneven[turn] = 1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       worker_sync();
+      bool far_now = *(volatile int*)&far_step[turn];
+      // A row of P takes the greatest factor of the keys that it sees, as far as they have not faded: what
+      // comes later, or has faded, does not take its digits.  Where all are within 2^4, as they mostly
+      // are, one factor serves all rows.  Of row `row_i`:
+      uint32_t p_biased = 0;
+      const bool even = STATE_ONLY || !*(volatile int*)&uneven[turn];
+      if (!STATE_ONLY) {
+        p_biased = of_usual + 2 - 14;
+        if (!even) {
+          const float k0 = k_down[lane], k1 = k_down[lane + 32];  // tokens `lane` and `lane + 32`
+          float seen0 = k0, seen1 = k1;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const float faded = nears[63 + d];
+            const float u0 = __shfl_up_sync(0xffffffffu, seen0, d) * faded, u1 = __shfl_up_sync(0xffffffffu, seen1, d) * faded;
+            if (lane >= d) seen0 = fmaxf(seen0, u0), seen1 = fmaxf(seen1, u1);
+          }
+          seen1 = fmaxf(seen1, __shfl_sync(0xffffffffu, seen0, 31) * nears[64 + lane]);
+          const float most = warp_most(fmaxf(k0, k1)), least_inv = warp_most(fmaxf(inverse_of(k0), inverse_of(k1)));
+          far_now |= most * least_inv > kFarApart;
+          if (most * least_inv > kApart && !far_now) {
+            // Small keys behind a large one: P holds their scores relative to the large one's, which does
+            // where each value column has that one's value.  Where one does not (below 2^-13 of the
+            // column's greatest), the step goes token by token.
+            const bool leads0 = seen0 == k0 && k0 * least_inv > kApart, leads1 = seen1 == k1 && k1 * least_inv > kApart;
+            const uint32_t all0 = __ballot_sync(0xffffffffu, leads0), all1 = __ballot_sync(0xffffffffu, leads1);
+            const uint32_t leads = (group < 2 ? all0 : all1) >> (16 * (group & 1));
+            v_mosts[group * 128 + col] = val_most;
+            worker_sync();
+            const float least = 0x1p-13f * most_of(most_of(v_mosts[col], v_mosts[128 + col], v_mosts[256 + col]),
+                                                   v_mosts[384 + col], 0.0f);
+            bool lost = false;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lost |= (leads >> i & 1) && fabsf(i & 1 ? val[i / 2].y : val[i / 2].x) < least;
+            if (lost) far_step[turn] = 1;
+            worker_sync();
+            far_now = *(volatile int*)&far_step[turn];
+          }
+          // (Rounded up to a power of two; at least 2^-126 of the greatest, so that no later key's factor
+          // over it is infinite.)
+          p_biased = (__float_as_uint(fmaxf(quarter & 1 ? seen1 : seen0, most * 0x1p-126f)) + 0x7fffffu) >> 23;
+          if (warp < 2) p_downs[warp * 32 + lane] = power_of(p_biased);
+        }
+      }
       if (tid == 0) {
-        far_step[turn ^ 1] = 0;
+        far_step[turn ^ 1] = uneven[turn ^ 1] = 0;
+        if (far_now) far_step[turn] = 1;
         mbar_arrive(turn ? ready_odd : ready);
       }
-      if (*(volatile int*)&far_step[turn]) {
+      if (far_now) {
         // Token by token.
         if (STATE_ONLY) flush();
         const float2 one = decay_over(decay, 1);
@@ -918,7 +978,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
       // v, and w = v_j a^(63 - j + tail) times the key's factor, each column with powers of two of its own: what a
       // large key is not multiplied with does not feel it.  (2^20 w is at most 2^126, and below 2^-126 only
       // where the product of key and value is.)
-      float p_down, p_inv, w_down;
+      float p_down, w_down;
       {
         const float* left = lefts + (m < kStep ? kStep : 0);
         Pair w[8];
@@ -933,9 +993,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         // Over the four threads that hold the column.
         float2* mosts = (float2*)v_mosts + col;
         mosts[group * 128] = make_float2(val_most, w_most);
-        // The keys' factors are taken over the greatest in P.
-        const float k_most = STATE_ONLY ? 0.0f : warp_most(fmaxf(k_down[lane], k_down[lane + 32]));
-        p_inv = power_of(254u - biased_of(k_most)) * 0x1p-22f;
         // (Before this step's values are ready: its own sums would end another phase of the barrier.)
         if (STATE_ONLY) flush();
         asm volatile("bar.sync %0, 128;" ::"r"(2 + quarter) : "memory");
@@ -953,7 +1010,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           for (int i = 0; i < 8; ++i) split_pair(mul2(val[i], up2), hi[i], lo[i]);
           tmem_st8(at_lane + Tm::kV + group * 8, hi);
           tmem_st8(at_lane + Tm::kV + 32 + group * 8, lo);
-          p_down = k_most * power_of(biased - 14u) * 0x1p22f;
+          p_down = power_of(biased - 14u) * 0x1p22f * (even ? power_of(p_biased) : 1.0f);
         }
         const uint32_t biased = scale_biased(w_most);
         const float up = power_of(268u - biased);
@@ -974,7 +1031,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         if (ok) ok = sleep_wait(score_full, steps & 1, err);
         tc_fence_after();
         // P of 16 keys: rows (tokens) 0..63 in the lanes of quarters 0 and 1, what q's lo adds in 2 and 3.
-        const Pair inv2 = pair_of(p_inv, p_inv);
+        const float inv = power_of(254u - p_biased) * 0x1p-22f;
+        const Pair inv2 = pair_of(inv, inv);
         const float* near = nears + 63 + row_i - group * 16;
         float p[16];
         tmem_ld16(at_lane + Tm::kScore + group * 16, p);
@@ -1032,6 +1090,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         float from[16], own[16];
         tmem_ld16(at_lane + Tm::kFrom + group * 16, from);
         tmem_ld16(at_lane + Tm::kScore + group * 16, own);
+        if (!even) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) own[i] *= p_downs[group * 16 + i] * p_down;
+          p_down = 1.0f;
+        }
         const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down, from_down);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
