@@ -362,10 +362,13 @@ bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positi
  * device ("Attention start or length out of range"; the sequence then counts as
  * empty); rows from n on are not read, and their out is 0.  Dims 1 to 128, lengths up
  * to 2^29, scale from 2^-30 to 2^30.  Serving calls it with seq_len 1 and the state
- * kept.  Products carry fp32's accuracy relative to the greatest value in a token's q
- * or k row, in 64 tokens' values of a v column and in a column of the state; where
- * values of 2^60 and more, below 2^-80 (0 aside), infinities or NaN come, 64 tokens
- * at a time go one by one, many times slower.  What leaves fp32's range is infinite or NaN
+ * kept.  A token's out has fp32's accuracy relative to the greatest that it sees of
+ * a^(t - j) max |q_t| max |k_j| max |v_j| (over a row each) among its 64 tokens, whatever
+ * others hold, and to each column of the state relative to the greatest product of a key
+ * and a value that has reached it.  64 tokens at a time go one by one, many times slower, where
+ * a row's greatest value is 2^60 and more, below 2^-80 (0 aside), infinite or NaN; where
+ * max |k_j| max |v_j| is 2^60 times another token's; and where it is 2^10 times another's while
+ * a value of v_j is below 2^-13 of those beside it.  What leaves fp32's range is infinite or NaN
  * from there on.  The workspace is the context's, as window_attention's. */
 bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* v, void* decay, void* state,
                                          void* lengths, void* out, void* new_state, uint32_t batch,

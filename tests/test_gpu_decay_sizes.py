@@ -142,3 +142,88 @@ def test_a_large_key_beside_small_values_within_its_64_tokens(lib, seq, power):
             t[value][:, :, where, where % 3::3] = 0
             t[value][:, :, where, where % 3 + 1::3] *= np.float32(2.0 ** -power)
         sized_run(lib, t, [result])
+
+
+VALUES = {"out": "v", "dq": "k", "dv": "dout", "dk": "q"}
+
+
+@pytest.mark.parametrize("result", list(VALUES))
+@pytest.mark.parametrize("seq,where", [(23, 11), (24, 11), (64, 0), (64, 63), (200, 40), (200, 100), (700, 300)])
+@pytest.mark.parametrize("power", [10, 16, 24, 32, 40, 50, -20, -50])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 80)])
+def test_a_large_or_small_value_leaves_other_tokens_as_they_are(lib, result, seq, where, power, dk, dv):
+    t = sized_data(seq + power + 50, seq, dk, dv)
+    t[VALUES[result]][:, :, where] *= np.float32(2.0 ** power)
+    sized_run(lib, t, [result])
+
+
+@pytest.mark.parametrize("seq", [100, 700])
+@pytest.mark.parametrize("spread", [8, 20, 40, 70])
+@pytest.mark.parametrize("dims", [(80, 64), (33, 70)])
+def test_rows_of_all_sizes(lib, seq, spread, dims):
+    for name in ("q", "k", "v", "dout"):
+        t = sized_data(spread, seq, *dims)
+        size = np.random.default_rng(seq).integers(-spread // 2, spread // 2 + 1, t[name].shape[:3] + (1,))
+        t[name] *= (2.0 ** size).astype(np.float32)
+        sized_run(lib, t, ["out", "new_state", "dq", "dk", "dv", "dstate"])
+
+
+@pytest.mark.parametrize("seq", [24, 200])
+def test_large_keys_with_small_values_and_small_ones_with_large(lib, seq):
+    # The products are alike: nothing needs to go token by token, and nothing may be lost.
+    for keys, values in (("k", "v"), ("q", "dout")):
+        t = sized_data(seq, seq, 64, 80)
+        size = (2.0 ** np.random.default_rng(seq).integers(-25, 26, t[keys].shape[:3] + (1,))).astype(np.float32)
+        t[keys] *= size
+        t[values] /= size
+        sized_run(lib, t, ["out", "new_state", "dq", "dk", "dv", "dstate"])
+
+
+@pytest.mark.parametrize("power", [-20, 20])
+def test_columns_of_all_sizes(lib, power):
+    # A column that is small in all tokens keeps its own digits.
+    t = sized_data(1, 200, 64, 64)
+    size = (2.0 ** np.linspace(0, power, 64)).astype(np.float32)
+    t["v"] *= size
+    sized_run(lib, t, ["out", "new_state"])
+    t = sized_data(2, 200, 64, 64)
+    t["k"] *= size
+    sized_run(lib, t, ["dq"])
+
+
+@pytest.mark.parametrize("size", [2.0 ** -62, 2.0 ** -55, 2.0 ** -40, 2.0 ** 50])
+def test_products_near_the_ends_of_fp32(lib, size):
+    # Down to where the products of key and value leave fp32's normal numbers (2^-126), and up.
+    t = sized_data(3, 200, 64, 64)
+    t["state"] = None
+    t["k"] *= np.float32(size)
+    t["v"] *= np.float32(size)
+    t["q"] *= np.float32(min(1.0 / size, 2.0 ** 55))
+    want = R.decay_attention(t["q"], t["k"], t["v"], RATES, None, None, 0.125, False)
+    much = R.decay_attention(abs(t["q"]), abs(t["k"]), abs(t["v"]), RATES, None, None, 0.125, False)
+    got = decay_run(lib, t, 0.125, False, need=())
+    within(got["out"], want["out"], much["out"], "out")
+
+
+@pytest.mark.parametrize("seq_major", [False, True])
+@pytest.mark.parametrize("dims", [(64, 64), (128, 80), (33, 70)])
+def test_rows_of_all_sizes_in_padded_batches(lib, dims, seq_major):
+    rng = np.random.default_rng(7)
+    t = decay_data(rng, 5, 4, 2, 300, *dims, seq_major, True)
+    t["decay"] = RATES
+    n = np.array([300, 0, 64, 65, 190])
+    t["lengths"] = n.astype(np.float32)
+    for name in ("q", "k", "v", "dout"):
+        t[name] *= (2.0 ** rng.integers(-15, 16, t[name].shape[:3] + (1,))).astype(np.float32)
+
+    def of(a):
+        return R.decay_attention(a["q"], a["k"], a["v"], RATES, a["state"], n, 0.125, seq_major, a["dout"], a["dnew"])
+
+    want, size = of(t), of({m: a if a is None else abs(a) for m, a in t.items()})
+    for name in ("q", "k", "v", "dout"):
+        a = t[name] if seq_major else np.moveaxis(t[name], 1, 2)
+        for b in range(5):
+            a[b, n[b]:] = (np.nan, np.inf, -np.inf, 1e30, 1e-30)[b]
+    got = decay_run(lib, t, 0.125, seq_major)
+    for m in got:
+        within(got[m], want[m], size[m], m)

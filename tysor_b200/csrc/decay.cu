@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "lm_ops.cuh"
 #include "tcgen05.cuh"
@@ -243,21 +244,27 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 //   X <- a^64 X + sum over j of a^(63 - j + tail) k_j v_j^T
 // fp32 accuracy out of fp16 matrix instructions, as in the attention kernels: an
 // operand is scaled by a power of two and split into hi = fp16(x) and lo =
-// fp16(x - hi), and a product is hi.hi + lo.hi + hi.lo.  Each q and k row (token) has
-// its own power of two, each row of P one of the keys that it sees, each value column one per 64
-// tokens, and so has each column of w, from its own greatest value, and of X, from a bound of what w's have added to it (one power for all of
-// w, of the greatest key times the column's greatest value, lost the columns in which a large key
-// meets a small value).  The matrix unit adds with truncation, so a step's sums leave it and X is kept
+// fp16(x - hi), and a product is hi.hi + lo.hi + hi.lo.  hi and lo hold 22 bits of a value down
+// to 2^-16 of the greatest that shares its power, and one fewer for each power of two below:
+//   q and k: a power for each row (token);
+//   v: one for each column, of rows each by its own power where rows differ by more than 2^4;
+//   P: one for each row, of the greatest key (with v's row's power) that the token sees, faded as it is
+//     for the token; what comes later does not count.  One for all rows where none differ by more than 2^4;
+//   w: one for each column, of its greatest product (the greatest key times the column's greatest
+//     value lost the columns in which a large key meets a small value);
+//   X: one for each column, of a bound of what w's have added to it.
+// The matrix unit adds with truncation, so a step's sums leave it and X is kept
 // in fp32 registers.  Products are formed transposed (values' columns in the unit's
 // 128 rows), so that X^T, v^T and w^T = (a^(63 - j + tail) v_j)^T are operands in tensor
 // memory, written there by the threads that hold them.
 //
 // A block takes one head's tokens (or a segment of them) step by step: a loading warp
 // brings the next step's rows into shared memory (by tensor maps; rows that are no whole
-// 16-byte pieces by three warps, 4 bytes at a time), sixteen warps split them, form P and
+// 16-byte pieces by three warps, 4 bytes at a time), two that would be idle look at the sizes of
+// v's rows, sixteen warps split the rows, form P and
 // keep X, an issuing warp feeds the matrix unit.  Values that fp16's range would spoil
-// (2^60 and more, below 2^-80, not finite) send their step through the registers token
-// by token.
+// (2^60 and more, below 2^-80, not finite, rows too far apart) send their step through the registers
+// token by token.
 //
 // What bounds it: the sixteen warps' instructions, one behind the other.  A step takes 4.9 us
 // (some 8900 cycles: 1800 to split the q and k rows, 900 for the values and the barrier, 1400
@@ -285,7 +292,7 @@ struct ScanTmem {
                             kV = kScore + 64, kW = kV + 64;  // hi; lo 32 columns behind
 };
 constexpr uint32_t kTmemColumns = 512;
-// How far the keys' factors of a step may lie apart, so that the columns need not be looked at, and so that
+// How far the factors of a step may lie apart, so that the columns need not be looked at, and so that
 // it does not go token by token.
 constexpr float kApart = 0x1p10f, kFarApart = 0x1p60f;
 
@@ -447,11 +454,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* v_mosts = k_downs + 128;             // [4][128] pairs
   float* x_most = v_mosts + 1024;             // [4][128]
   float* p_downs = x_most + 512;              // [64] what undoes the factors of P's rows
-  uint64_t* bars = (uint64_t*)(p_downs + 64);
+  float* v_ups = p_downs + 64;                // [2][64] the powers of two of v's rows
+  float* kv_downs = v_ups + 128;              // [64] what undoes k's and v's rows' factors together
+  uint64_t* bars = (uint64_t*)(kv_downs + 64);
   int* far_step = (int*)(bars + 14);              // [2]
-  int* uneven = far_step + 2;                     // [2] whether the keys' factors differ from `usual`
-  uint32_t* usual = (uint32_t*)(uneven + 2);      // [2] the exponent of the first key of the step before
-  uint32_t* tmem_slot = usual + 2;
+  int* uneven = far_step + 2;                     // [2] whether k's or v's rows differ in size from `usual`
+  uint32_t* usual = (uint32_t*)(uneven + 2);      // [2][2] the exponents of the first key and value of the step before
+  uint32_t* tmem_slot = usual + 4;
   const uint32_t base = smem_u32(smem);
   const uint32_t raw_full = smem_u32(bars), raw_empty = raw_full + 8, ready = raw_full + 16, values_ready = raw_full + 24,
                  score_full = raw_full + 32, sums_full = raw_full + 40, p_ready = raw_full + 48,
@@ -486,7 +495,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     mbar_init(out_free, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     far_step[0] = far_step[1] = uneven[0] = uneven[1] = 0;
-    usual[0] = 0;
+    usual[0] = usual[1] = 0;
   }
   if (tid < 64) since[tid] = power(tid + lead);
   if (tid >= 64 && tid < 192) {
@@ -513,6 +522,25 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   const int key_pitch = VEC ? s.rows : DK, value_pitch = VEC ? s.cols : kMostDim;
   const bool turned = VEC && s.back;
   auto place = [&](int i) { return turned ? kStep - 1 - i : i; };
+
+  // The sizes of v's rows from `row0` on, `rows` (up to 32) of them, and whether they are as usual, as the
+  // splitting warps do for k.
+  auto look_at_values = [&](int row0, auto rows, int turn, int m) {
+    const float* raw = (const float*)(smem + Sm::kRawV) + (!VEC || 4 * lane < s.cols ? 4 * lane : 0);
+    float mine = 0.0f;  // of row `lane`
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      if (row0 + r >= m) break;
+      const float4 w = *(const float4*)(raw + place(row0 + r) * value_pitch);
+      const float most = warp_most(most_of(most_of(w.x, w.y, w.z), w.w, 0.0f));
+      if (lane == r) mine = most;
+    }
+    const uint32_t biased = scale_biased(mine), was = usual[2 * turn + 1];
+    if (lane < rows) v_ups[64 * turn + row0 + lane] = mine == 0.0f ? 0.0f : power_of(251u - biased);
+    if (row0 + lane == 0) usual[2 * (turn ^ 1) + 1] = biased;
+    if (far_biased(biased)) far_step[turn] = 1;
+    if (lane < rows && row0 + lane < m && (mine == 0.0f || biased - was + 2 > 4)) uneven[turn] = 1;
+  };
 
   if (warp >= kWorkers / 32) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -654,6 +682,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         }
         // The last copies end before the block does.
         if (c > 0) sleep_wait(raw_full, (c - 1) & 1, err);
+      } else if (!STATE_ONLY) {
+        // The other two look at a step's values while the sixteen split q and k.
+        bool ok = true;
+        for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
+          if (ok) ok = sleep_wait(raw_full, c & 1, err);
+          look_at_values((warp & 1) * 32, std::integral_constant<int, 32>{}, c & 1, min(kStep, t1 - t));
+          asm volatile("bar.arrive 6, %0;" ::"n"(kWorkers + 64) : "memory");
+        }
       }
     } else {
       // The loading warps, a row at a time.
@@ -782,8 +818,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
     for (int t = t0, c = 0; t < t1; t += kStep, ++c) {
       const int m = min(kStep, t1 - t);
       const int turn = c & 1;
-      float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn;
-      const uint32_t of_usual = STATE_ONLY ? 0 : usual[turn];
+      float *q_down = q_downs + 64 * turn, *k_down = k_downs + 64 * turn, *v_up = v_ups + 64 * turn;
+      const uint32_t usual_k = STATE_ONLY ? 0 : usual[2 * turn];
       if (ok) ok = sleep_wait(raw_full, turn, err);
       if (m < kStep) {  // zeros behind the sequence's end
         const int first = turned ? 0 : m;
@@ -827,8 +863,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         const uint32_t biased = scale_biased(mine);
         far |= far_biased(biased);
         if (!STATE_ONLY && is_k) {
-          odd = lane < kRowsPer && row0 + lane < m && (mine == 0.0f || biased - of_usual + 2 > 4);
-          if (row0 + lane == 0) usual[turn ^ 1] = biased;
+          odd = lane < kRowsPer && row0 + lane < m && (mine == 0.0f || biased - usual_k + 2 > 4);
+          if (row0 + lane == 0) usual[2 * (turn ^ 1)] = biased;
         }
         // A row of zeros has no part in the greatest factor.
         if (lane < kRowsPer)
@@ -872,24 +908,39 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           val[i] = pair_of(a, d);
           val_most = most_of(val_most, a, d);
         }
-        far |= far_biased(scale_biased(val_most));
+        if (STATE_ONLY) far |= far_biased(scale_biased(val_most));
       }
+      if (!STATE_ONLY && !VEC) look_at_values(warp * 4, std::integral_constant<int, 4>{}, turn, m);
       if (far) far_step[turn] = 1;
       if (odd) uneven[turn] = 1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      worker_sync();
+      if (STATE_ONLY || !VEC) worker_sync();
+      else asm volatile("bar.sync 6, %0;" ::"n"(kWorkers + 64) : "memory");
       bool far_now = *(volatile int*)&far_step[turn];
-      // A row of P takes the greatest factor of the keys that it sees, as far as they have not faded: what
-      // comes later, or has faded, does not take its digits.  Where all are within 2^4, as they mostly
-      // are, one factor serves all rows.  Of row `row_i`:
+      // Where the rows of k or of v differ by more than 2^4, which they mostly do not, each row of v goes by its
+      // own power of two as those of k do, and a row of P takes the greatest factor of the two among the
+      // tokens that it sees, as far as they have not faded: what comes later, or has faded, does not take
+      // its digits.  Of row `row_i`:
       uint32_t p_biased = 0;
       const bool even = STATE_ONLY || !*(volatile int*)&uneven[turn];
       if (!STATE_ONLY) {
-        p_biased = of_usual + 2 - 14;
+        p_biased = usual_k + 2 - 14;
         if (!even) {
-          const float k0 = k_down[lane], k1 = k_down[lane + 32];  // tokens `lane` and `lane + 32`
+          const float k0 = k_down[lane] * inverse_of(v_up[lane]);  // tokens `lane` and `lane + 32`
+          const float k1 = k_down[lane + 32] * inverse_of(v_up[lane + 32]);
+          if (warp == 0) kv_downs[lane] = k0, kv_downs[lane + 32] = k1;
+          far_now |= __any_sync(0xffffffffu, (k0 > 0.0f && k0 < 0x1p-126f) || (k1 > 0.0f && k1 < 0x1p-126f));
+          k_down = kv_downs;
+          val_most = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 u = *(const float4*)(v_up + group * 16 + 4 * i);
+            val[2 * i] = mul2(val[2 * i], pair_of(u.x, u.y));
+            val[2 * i + 1] = mul2(val[2 * i + 1], pair_of(u.z, u.w));
+            val_most = most_of(most_of(val_most, val[2 * i].x, val[2 * i].y), val[2 * i + 1].x, val[2 * i + 1].y);
+          }
           float seen0 = k0, seen1 = k1;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
@@ -900,8 +951,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           seen1 = fmaxf(seen1, __shfl_sync(0xffffffffu, seen0, 31) * nears[64 + lane]);
           const float most = warp_most(fmaxf(k0, k1)), least_inv = warp_most(fmaxf(inverse_of(k0), inverse_of(k1)));
           far_now |= most * least_inv > kFarApart;
+          worker_sync();  // kv_downs
           if (most * least_inv > kApart && !far_now) {
-            // Small keys behind a large one: P holds their scores relative to the large one's, which does
+            // Small tokens behind a large one: P holds their scores relative to the large one's, which does
             // where each value column has that one's value.  Where one does not (below 2^-13 of the
             // column's greatest), the step goes token by token.
             const bool leads0 = seen0 == k0 && k0 * least_inv > kApart, leads1 = seen1 == k1 && k1 * least_inv > kApart;
