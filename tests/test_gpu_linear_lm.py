@@ -192,6 +192,35 @@ def test_graph_refusals(cuda_ctx):
         run({"z": [6, 9]}, lambda gb, v: gb.call("token_entropy", *v, 0.0))
 
 
+def test_a_decay_that_would_need_a_gradient_is_refused(cuda_ctx):
+    # It has none, so that a graph which trains it, or asks for its inputs' gradients, would go on without.
+    b, s, h, d = 2, 8, 4, 16
+    shapes = {"x": [b, s, h, d], "r": [1, h]}
+    data = {"x": np.ones((b, s, h, d), np.float32), "r": np.ones((1, h), np.float32)}
+
+    def graph(decay):
+        gb = GraphBuilder("m")
+        x, r = gb.param("x"), gb.param("r")
+        q = gb.apply(gb.ctor("LayerNorm", d), x)
+        loss = gb.let("loss", gb.call("decay_attention", q, x, x, decay(gb, r), True))
+        gb.ret(loss)
+        gb.train(objective="loss", lr=0.1, iterations=1)
+        return CudaGraphExecutor(cuda_ctx, gb.build(), shapes, data)
+
+    direct, scaled = (lambda gb, r: r), (lambda gb, r: gb.binary("*", r, 0.5))
+    trained = lambda gb, r: gb.apply(gb.ctor("linear", h, h, False), r)
+    for decay, train, backward in ((direct, True, True), (scaled, True, False), (trained, False, False)):
+        for call, works in ((lambda ex: ex.train(1, 0.1), train), (lambda ex: ex.backward(), backward),
+                            (lambda ex: ex.run(), True)):
+            ex = graph(decay)
+            if works:
+                call(ex)
+            else:
+                with pytest.raises(RuntimeError, match="no gradient for decay"):
+                    call(ex)
+            ex.close()
+
+
 def test_serving_token_by_token(cuda_ctx):
     # A prompt, then one token at a time over the state: rotary on q and k, decay attention, an output
     # projection, and the answers' log probabilities.

@@ -988,6 +988,28 @@ struct Executor {
     return nullptr;
   }
 
+  // Whether value `id` is made of what gradients are asked for: of trained parameters, or in --backward of
+  // the graph's inputs (`id` itself apart).
+  bool wants_gradient(int id) const {
+    std::vector<int> open{id};
+    std::set<int> seen;
+    while (!open.empty()) {
+      const int at = open.back();
+      open.pop_back();
+      if (!seen.insert(at).second) continue;
+      const GNode* p = producer_node(at);
+      if (!p) {
+        if (mode == kModeBackward && at != id) return true;
+        continue;
+      }
+      if (mode == kModeTrain && p->kind == kNCtor &&
+          (p->op == "linear" || p->op == "Embedding" || p->op == "RMSNorm" || p->op == "LayerNorm"))
+        return true;
+      open.insert(open.end(), p->inputs.begin(), p->inputs.end());
+    }
+    return false;
+  }
+
   // True if `s` scales tensor `m` by a constant, with the constant in *f.
   bool scales_by_const(const GNode& s, int m, float* f) const {
     int c = -1;
@@ -1384,6 +1406,8 @@ struct Executor {
       fail(problem);
     if (numel(decay.shape) != q.shape[hl])
       fail("decay_attention expects one decay per head, got " + shape_str(decay.shape));
+    if (wants_gradient(node.inputs[3]))
+      fail("decay_attention has no gradient for decay: it takes an input of the graph or constants");
     if (end == 5) {
       const HVal& n = tensor(node.inputs[4], "decay_attention lengths");
       if (numel(n.shape) != q.shape[0]) fail("decay_attention expects one length per sequence");

@@ -31,7 +31,8 @@ PRIMITIVE_OPS = ("matmul", "relu", "scale")
 #   distill_loss(logits, ids, teacher, temperature)
 #   rotary(x, positions, theta, rotary_dim, interleaved [, scaling, factor, original_len, low, high, amplitude]
 #          [, seq_major])
-#   decay_attention(q, k, v, decay [, lengths] [, seq_major])
+#   decay_attention(q, k, v, decay [, lengths] [, seq_major])   (decay has no gradient; one that is computed
+#                                                               from what is trained is refused)
 #   token_logprobs(logits, ids, temperature), token_entropy(logits, temperature)
 # x, q, k and v are [batch, heads, length, head_dim], or with a trailing
 # `True` [batch, length, heads, head_dim].
