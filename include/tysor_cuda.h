@@ -367,8 +367,9 @@ bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positi
  * others hold, and to each column of the state relative to the greatest product of a key
  * and a value that has reached it.  64 tokens at a time go one by one, many times slower, where
  * a row's greatest value is 2^60 and more, below 2^-80 (0 aside), infinite or NaN; where
- * max |k_j| max |v_j| is 2^60 times another token's; and where it is 2^10 times another's while
- * a value of v_j is below 2^-13 of those beside it.  What leaves fp32's range is infinite or NaN
+ * max |k_j| max |v_j| is 2^60 times another token's; and where it is 2^10 times another's and
+ * the greatest product in some value column so far is below 2^-15 of what that column's
+ * greatest value would give.  What leaves fp32's range is infinite or NaN
  * from there on.  The workspace is the context's, as window_attention's. */
 bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* v, void* decay, void* state,
                                          void* lengths, void* out, void* new_state, uint32_t batch,

@@ -951,29 +951,41 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           seen1 = fmaxf(seen1, __shfl_sync(0xffffffffu, seen0, 31) * nears[64 + lane]);
           const float most = warp_most(fmaxf(k0, k1)), least_inv = warp_most(fmaxf(inverse_of(k0), inverse_of(k1)));
           far_now |= most * least_inv > kFarApart;
-          worker_sync();  // kv_downs
-          if (most * least_inv > kApart && !far_now) {
-            // Small tokens behind a large one: P holds their scores relative to the large one's, which does
-            // where each value column has that one's value.  Where one does not (below 2^-13 of the
-            // column's greatest), the step goes token by token.
-            const bool leads0 = seen0 == k0 && k0 * least_inv > kApart, leads1 = seen1 == k1 && k1 * least_inv > kApart;
-            const uint32_t all0 = __ballot_sync(0xffffffffu, leads0), all1 = __ballot_sync(0xffffffffu, leads1);
-            const uint32_t leads = (group < 2 ? all0 : all1) >> (16 * (group & 1));
-            v_mosts[group * 128 + col] = val_most;
-            worker_sync();
-            const float least = 0x1p-13f * most_of(most_of(v_mosts[col], v_mosts[128 + col], v_mosts[256 + col]),
-                                                   v_mosts[384 + col], 0.0f);
-            bool lost = false;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) lost |= (leads >> i & 1) && fabsf(i & 1 ? val[i / 2].y : val[i / 2].x) < least;
-            if (lost) far_step[turn] = 1;
-            worker_sync();
-            far_now = *(volatile int*)&far_step[turn];
-          }
           // (Rounded up to a power of two; at least 2^-126 of the greatest, so that no later key's factor
           // over it is infinite.)
           p_biased = (__float_as_uint(fmaxf(quarter & 1 ? seen1 : seen0, most * 0x1p-126f)) + 0x7fffffu) >> 23;
           if (warp < 2) p_downs[warp * 32 + lane] = power_of(p_biased);
+          worker_sync();  // kv_downs, p_downs
+          if (most * least_inv > kApart && !far_now) {
+            // Small tokens behind a large one: P holds their scores relative to the large one's, which does
+            // where a column's greatest product so far (`seen`, faded) is near what P's row is relative to
+            // times the column's greatest value.  Where it is below 2^-15 of that, the step goes token by token.
+            float v_all[16], seen = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              v_all[i] = fabsf(i & 1 ? val[i / 2].y : val[i / 2].x) * k_down[group * 16 + i];
+              seen = fmaxf(seen * nears[64], v_all[i]);
+            }
+            ((float2*)v_mosts)[group * 128 + col] = make_float2(val_most, seen);
+            worker_sync();
+            float column = 0.0f;
+            seen = 0.0f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float2 of_group = ((const float2*)v_mosts)[g * 128 + col];
+              column = fmaxf(column, of_group.x);
+              if (g < group) seen = fmaxf(seen * nears[63 + 16], of_group.y);
+            }
+            bool lost = false;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              seen = fmaxf(seen * nears[64], v_all[i]);
+              lost |= seen > 0.0f && seen < 0x1p-15f * column * p_downs[group * 16 + i];
+            }
+            if (lost) far_step[turn] = 1;
+            worker_sync();
+            far_now = *(volatile int*)&far_step[turn];
+          }
         }
       }
       if (tid == 0) {
