@@ -360,7 +360,7 @@ bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positi
  * be the buffer `state` itself (no other output may overlap anything).  lengths
  * [batch] may be NULL (n = seq_len) and holds whole numbers as floats, checked on the
  * device ("Attention start or length out of range"; the sequence then counts as
- * empty); rows from n on are not read, and their out is 0.  Dims 1 to 128, lengths up
+ * empty); what rows from n on hold is of no consequence, and their out is 0.  Dims 1 to 128, lengths up
  * to 2^29, scale from 2^-30 to 2^30.  Serving calls it with seq_len 1 and the state
  * kept.  A token's out has fp32's accuracy relative to the greatest that it sees of
  * a^(t - j) max |q_t| max |k_j| max |v_j| (over a row each) among its 64 tokens, whatever

@@ -266,19 +266,23 @@ __global__ void __launch_bounds__(kStepThreads, 8) step_kernel(const __grid_cons
 // (2^60 and more, below 2^-80, not finite, rows too far apart) send their step through the registers
 // token by token.
 //
-// What bounds it: the sixteen warps' instructions, one behind the other.  A step takes 4.9 us
-// (some 8900 cycles: 1800 to split the q and k rows, 900 for the values and the barrier, 1400
+// What bounds it: the sixteen warps' instructions, one behind the other.  A step takes 5.1 us, some
+// 9300 cycles.  Of the 8900 before columns' products and rows' sizes were looked at, 1800 split the
+// q and k rows, 900 were for the values and the barrier, 1400
 // for v and w, 1200 for P, 500 for X, 800 to lay it into tensor memory, the rest for the
-// outputs and waits); the tensor pipe is busy for a quarter of them and the schedulers issue
-// in 55% of cycles (20 K warp instructions a step).  Tensor memory's 512 columns and 226 KB of
+// outputs and waits.  The tensor pipe is busy for a quarter of them and the schedulers issue
+// in 57% of cycles (21 K warp instructions a step).  Tensor memory's 512 columns and 226 KB of
 // shared memory leave room for one block an SM.  8 x 2048 tokens of 16 heads of 128, 128
-// blocks: 158 us (outputs stored by the sixteen warps 163, all of X q^T before the sums 170).
-// Tried, each beside what was there then: warps of their own for splitting and for X (182 to
+// blocks: 162 us with the same inputs again and 171 with others between (154 and 168 with one power
+// of two for all of P and of w, which lost digits where tokens differ in size).  Rows unlike by more
+// than 2^4 cost 182 us in place of 170, sizes spread over 2^20 270 to 330, all tokens one by one 1970.
+// Heads of 64 wide leave half of the unit's 128 rows idle: 133 us.  Rows of 4-byte pieces: 127 wide 303 us.
+// Tried, same inputs, each beside what was there then: outputs stored by the sixteen warps (163 us, 158),
+// all of X q^T before the sums (170, 158), warps of their own for splitting and for X (182 to
 // 238 us, 166 without: more instructions and exchanges), the next step's rows split while the
 // matrix unit works (171 to 254, registers), row by row bulk copies (80 cycles each to issue),
-// stores of single values (190, 178 with boxes), no work on P's blocks of zeros (171, 169).
-// Heads of 64 wide leave half of the unit's 128 rows idle: 126 us.  Rows of 4-byte pieces:
-// 127 wide 302 us.
+// stores of single values (190, 178 with boxes), no work on P's blocks of zeros (171, 169), v's rows looked
+// at by the sixteen warps themselves (181 in place of 173, others between).
 constexpr int kStep = 64;
 constexpr int kWorkers = 512, kScanThreads = kWorkers + 128, kLoaders = 3;  // loading warps
 constexpr int kWorkerRegs = 104, kOtherRegs = 64;  // 4 x 104 + 64 = 5 x 96, what a quarter of an SM is launched with
@@ -669,8 +673,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
             load_rows(base + Sm::kRawK, &maps.k, row, h / s.k.share, b, raw_full);
             if (!STATE_ONLY) load_rows(base + Sm::kRawQ, &maps.q, row, h / s.q.share, b, raw_full);
             load_rows(base + Sm::kRawV, &maps.v, row, h / s.v.share, b, raw_full);
-            // The step after next's on their way to L2 (65536 tokens 260 -> 247 us, training on
-            // 8192 467 -> 446), where it is whole.
+            // The step after next's on their way to L2 (without, 65536 tokens took 260 us for 247 and
+            // training on 8192 467 for 446), where it is whole.
             if (t + 2 * kStep <= t1) {
               const int next = s.back ? row - kStep : row + kStep;
               prefetch_rows(&maps.k, next, h / s.k.share, b);
@@ -1303,8 +1307,8 @@ constexpr int kChunkedFrom = 24;
 // which a first launch forms states.  Times in steps of scan_kernel, 5 us: 2 for a block's
 // start and end, half a step for one of the first launch, 1.5 for the join's launch (with 3,
 // 3 ragged sequences of 777 train in 114 us in place of 101).  With one segment a head,
-// training on 8192 tokens of 16 heads takes 1220 us in place of 445; with one piece a segment
-// 500.
+// training on 8192 tokens of 16 heads took 1220 us where it took 445 with these; with one piece a
+// segment 500.
 Split split_of(int64_t units, int seq, int scans, int states) {
   const int64_t steps = ceil_div(seq, kStep);
   double best = (double)ceil_div(scans * units, 148) * (steps + 2.0);
