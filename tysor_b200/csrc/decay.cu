@@ -311,7 +311,9 @@ struct ScanSmem {
   static constexpr int kRawV = kRawK + kStep * DK * 4;
   static constexpr int kOut = kRawV + kStep * kMostDim * 4;  // a step's outputs, as the tensor holds them
   static constexpr int kMisc = kOut + kStep * kMostDim * 4;
-  static constexpr int kBytes = kMisc + 10240;
+  static constexpr int kMiscBytes = 4 * (64 + 5 * 128 + 1024 + 512 + 2 * 64) + 20 * 8;  // factors, sizes, barriers
+  static constexpr int kBytes = kMisc + kMiscBytes + 1023;                           // and what the alignment takes
+  static_assert(kBytes <= 227 * 1024);
 };
 
 // Boxes of 64 rows of a head's q, k and v, where rows are whole 16-byte pieces, and of
