@@ -382,7 +382,8 @@ bool tysor_cuda_dispatch_decay_attention(void* context, void* q, void* k, void* 
  * dq_t (+)= scale * dout_t S_t^T, dk_t (+)= v_t E_t^T, dv_t (+)= k_t E_t (dk and dv
  * summed over the query heads that share a key head, in a fixed order), dstate (+)=
  * a * E_1 (may be NULL).  Rows from n on get 0.  E is held as E / scale, which is to stay
- * in fp32's range as well. */
+ * in fp32's range as well.  Accuracy as above, with dout, v, k (dq), k, q, dout (dv) and v, dout, q
+ * (dk) in the places of q, k, v; dk's is relative to whole rows alone. */
 bool tysor_cuda_dispatch_decay_attention_backward(void* context, void* q, void* k, void* v, void* decay,
                                                   void* state, void* lengths, void* dout, void* dnew_state,
                                                   void* dq, void* dk, void* dv, void* dstate, uint32_t batch,

@@ -227,3 +227,22 @@ def test_rows_of_all_sizes_in_padded_batches(lib, dims, seq_major):
     got = decay_run(lib, t, 0.125, seq_major)
     for m in got:
         within(got[m], want[m], size[m], m)
+
+
+@pytest.mark.parametrize("seq", [23, 200, 700])
+@pytest.mark.parametrize("size", [2.0 ** 50, 2.0 ** 55, 2.0 ** 57])
+def test_large_products_that_fp32_holds(lib, size, seq):
+    # Outputs up to 2^123 with queries of 1: what stands between must not leave fp32's range either.
+    t = sized_data(5, seq, 64, 64)
+    t["dnew"] = None
+    t["state"] *= np.float32(size * size)
+    t["k"] *= np.float32(size)
+    t["v"] *= np.float32(size)
+    t["dout"] *= np.float32(1e-3 / size)  # dq = dout S: 2^63
+    sized_run(lib, t, ["out", "new_state", "dq"])
+    t = sized_data(6, seq, 64, 64)
+    t["state"] = None
+    t["q"] *= np.float32(size)
+    t["dout"] *= np.float32(1e-3 * size)
+    t["dnew"] *= np.float32(1e-3 * size * size)
+    sized_run(lib, t, ["dk", "dv", "dstate"])

@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   float* since = (float*)(smem + Sm::kMisc);  // [64] a^(i + lead)
   float* lefts = since + 64;                  // [2][64] 2^20 a^(63 - j + tail), and the same of a last, shorter step
   float* nears = lefts + 128;                 // [128] a^(d - 63), 0 below
-  float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors (q's times scale), steps in turn
+  float* q_downs = nears + 128;               // [2][64] what undoes the rows' factors (q's times 2^14 scale), steps in turn
   float* k_downs = q_downs + 128;             // [2][64]
   float* v_mosts = k_downs + 128;             // [4][128] pairs
   float* x_most = v_mosts + 1024;             // [4][128]
@@ -874,7 +874,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
         }
         // A row of zeros has no part in the greatest factor.
         if (lane < kRowsPer)
-          (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : power_of(biased - 14u) * (is_k ? 1.0f : s.scale);
+          (is_k ? k_down : q_down)[row0 + lane] = mine == 0.0f ? 0.0f : is_k ? power_of(biased - 14u) : power_of(biased) * s.scale;
         const float up = power_of(268u - biased);
         uint8_t* box = smem + (is_k && !(STATE_ONLY && turn) ? Sm::kK : Sm::kQ);
         const int other = (is_k ? kBoxes : 1) * kBoxBytes;  // from hi to lo
@@ -1080,7 +1080,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           for (int i = 0; i < 8; ++i) split_pair(mul2(val[i], up2), hi[i], lo[i]);
           tmem_st8(at_lane + Tm::kV + group * 8, hi);
           tmem_st8(at_lane + Tm::kV + 32 + group * 8, lo);
-          p_down = power_of(biased - 14u) * 0x1p22f * (even ? power_of(p_biased) : 1.0f);
+          p_down = power_of(biased - 14u) * 0x1p8f * (even ? power_of(p_biased) : 1.0f);
         }
         const uint32_t biased = scale_biased(w_most);
         const float up = power_of(268u - biased);
@@ -1165,14 +1165,16 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
           for (int i = 0; i < 16; ++i) own[i] *= p_downs[group * 16 + i] * p_down;
           p_down = 1.0f;
         }
-        const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down, from_down);
+        // (2^14 of a query's factor stands in q_down: before it is taken, sums are then as large as the
+        // outputs of a query of 1, and no power of two is needed that fp32 does not have.)
+        const Pair p2 = pair_of(p_down, p_down), f2 = pair_of(from_down * 0x1p-14f, from_down * 0x1p-14f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float4 w = *(const float4*)(since + group * 16 + 4 * i), d = *(const float4*)(q_down + group * 16 + 4 * i);
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int e = 4 * i + 2 * j;
-            const Pair o = fma2(pair_of(from[e], from[e + 1]), mul2(j ? pair_of(w.z, w.w) : pair_of(w.x, w.y), f2),
+            const Pair o = fma2(mul2(pair_of(from[e], from[e + 1]), j ? pair_of(w.z, w.w) : pair_of(w.x, w.y)), f2,
                                 mul2(pair_of(own[e], own[e + 1]), p2));
             const Pair y = mul2(o, j ? pair_of(d.z, d.w) : pair_of(d.x, d.y));
             own[e] = y.x, own[e + 1] = y.y;
