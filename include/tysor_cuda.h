@@ -365,7 +365,8 @@ bool tysor_cuda_dispatch_rotary_backward(void* context, void* grad, void* positi
  * kept.  A token's out has fp32's accuracy relative to the greatest that it sees of
  * a^(t - j) max |q_t| max |k_j| max |v_j| (over a row each) among its 64 tokens, whatever
  * others hold, and to each column of the state relative to the greatest product of a key
- * and a value that has reached it.  64 tokens at a time go one by one, many times slower, where
+ * and a value that has reached it; what has faded below 2^-126 of itself within 64 tokens may
+ * count as 0.  64 tokens at a time go one by one, many times slower, where
  * a row's greatest value is 2^60 and more, below 2^-80 (0 aside), infinite or NaN; where
  * max |k_j| max |v_j| is 2^60 times another token's; and where it is 2^10 times another's and
  * the greatest product in some value column so far is below 2^-15 of what that column's
